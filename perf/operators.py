@@ -195,7 +195,7 @@ def _plain_top(logits, k):
 
 
 def _plain_teacher(values, indices, vocab, t):
-    used = (indices >= 0) & (indices < vocab)
+    used = (indices >= 0) & (indices < vocab) & (values > float('-inf'))
     v = torch.where(used, values.float(), float('-inf')) / t
     m = v.amax(1, keepdim=True)
     e = torch.where(used, torch.exp(v - m), 0.0)
