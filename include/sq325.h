@@ -332,6 +332,67 @@ int sq_model_set_exact_skinny(sq_model* model, int exact);
 int sq_model_time_gemm(sq_model* model, int enable);
 int sq_model_gemm_time(sq_model* model, double* seconds, int64_t* launches);
 
+/* ---------------------------------------------------------------- rows of logits
+ * Operators on logits [rows, vocab] of type SQ_F16 / SQ_BF16 / SQ_F32 (no reference
+ * counterpart: the reference's loops pick greedily).  Row r starts at data + r * row_stride
+ * elements; vocab is at most 262144; data needs its type's alignment only.  All three
+ * operators are asynchronous on `stream`, allocate nothing and keep nothing between calls.
+ * rows == 0 is a valid call that does nothing. */
+enum { SQ_F16 = 0, SQ_BF16 = 1, SQ_F32 = 2 };
+typedef struct sq_logits {
+  const void* data;
+  int64_t row_stride;         /* elements, >= 0 (0: every row the same) */
+  int32_t rows, vocab, type;
+} sq_logits;
+
+/* Draws one token a row from given uniform numbers.  With m the row's largest logit and
+ * c = log2(e) / temperature: y_j = 2^((x_j - m) c), weight w_j = rint(y_j 2^31), tokens ordered
+ * by logit (equal ones by index).  top_k > 0 keeps the first top_k tokens; top_p < 1 those
+ * whose predecessors hold less than top_p of the kept weight (the first always); min_p > 0 those
+ * with y_j >= min(min_p, 1).  The token is the first in index order at which the running weight
+ * passes floor(uniform * total).  Weights and sums are integers: the token depends on the
+ * inputs alone.  temperature <= 0 or NaN: the largest logit, lowest index.  NaN logits count
+ * as -inf; a row with nothing above -inf gives -1.  A null per-row array means the value
+ * beside it for every row. */
+typedef struct sq_sample_args {
+  sq_logits logits;
+  const float* uniform;                                  /* [rows], in [0, 1) */
+  const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p;  /* [rows] or NULL */
+  float temperature_all; int32_t top_k_all; float top_p_all, min_p_all;
+  int64_t* tokens;                                       /* [rows] */
+} sq_sample_args;
+int sq_sample(const sq_sample_args* args, void* stream);
+
+/* The k (1..1024, <= vocab) largest logits of each row, largest first, equal ones by index:
+ * values [rows, k] in the logits' type and indices [rows, k].  NaN and -inf are not taken;
+ * places left over hold -inf and -1. */
+int sq_top_logits(const sq_logits* logits, int k, void* values, int32_t* indices, void* stream);
+
+/* Distillation from a teacher's record of its largest logits: values [rows, k] (value_type)
+ * and indices [rows, k], k in 1..1024; entries with an index outside [0, vocab) or a value of
+ * -inf or NaN are unused, repeated indices add up.  With q the softmax of values / temperature
+ * over the used entries and p that of the student's logits / temperature over the vocabulary:
+ *   loss[r] = temperature^2 sum_k q_k (log q_k - log p_jk)
+ *   grad[r, j] = weight[r] temperature (p_j - sum over k with j_k = j of q_k)
+ * (loss is not weighted).  A row without used entries has loss 0 and gradient 0; a student row
+ * whose softmax is not defined (NaN, +inf, nothing above -inf) gives NaN.
+ * sq_distill_forward writes loss and, if not NULL, stats [rows, 2] fp32, which
+ * sq_distill_backward reads to write grad; sq_distill_loss_grad writes loss and grad in one
+ * call.  weight NULL: 1; weight_stride 0: one factor for every row.  grad has the logits'
+ * type and must not overlap them. */
+typedef struct sq_distill_args {
+  sq_logits logits;
+  const void* values; const int32_t* indices;
+  int32_t k, value_type;
+  float temperature;                                     /* > 0, finite */
+  const float* weight; int64_t weight_stride;
+  float* loss; float* stats;
+  void* grad; int64_t grad_stride;
+} sq_distill_args;
+int sq_distill_forward(const sq_distill_args* args, void* stream);
+int sq_distill_backward(const sq_distill_args* args, void* stream);
+int sq_distill_loss_grad(const sq_distill_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -13,6 +13,7 @@
 #include "decode.cuh"
 #include "fp4.cuh"
 #include "layer.cuh"
+#include "logits.cuh"
 #include "s16.cuh"
 #include "ste.cuh"
 #include "scan.cuh"
@@ -835,6 +836,95 @@ int sq_model_check(sq_model* m, void* stream) {
     return fail(SQ_ETIMEOUT, "device: a bounded wait expired (code " + std::to_string(h) + ")");
   }
   return SQ_OK;
+}
+
+namespace {
+int logits_rows(const sq_logits& l, const char* who, LogitsRows& out) {
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  if (l.type < SQ_F16 || l.type > SQ_F32) return bad("unknown logits type");
+  if (l.rows < 0 || l.vocab <= 0 || l.vocab > kMaxVocab) return bad("rows must be >= 0 and vocab in [1, 262144]");
+  if (l.rows > 0 && !l.data) return bad("null logits");
+  if (l.row_stride < 0) return bad("row stride must not be negative");
+  if (!aligned(l.data, l.type == SQ_F32 ? 4 : 2)) return bad("logits are not aligned to their type");
+  out = LogitsRows{l.data, l.row_stride, l.rows, l.vocab, l.type};
+  return SQ_OK;
+}
+
+int distill_params(const sq_distill_args* a, const char* who, DistillParams& P) {
+  if (!a) return fail(SQ_EINVAL, std::string(who) + ": null argument");
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  P = DistillParams{};
+  if (int s = logits_rows(a->logits, who, P.x)) return s;
+  if (a->k < 1 || a->k > kMaxRecord) return bad("k must be in [1, 1024]");
+  if (a->value_type < SQ_F16 || a->value_type > SQ_F32) return bad("unknown value type");
+  if (!(a->temperature > 0.0f) || a->temperature > 3.0e38f) return bad("temperature must be positive and finite");
+  if (a->weight_stride < 0) return bad("weight stride must not be negative");
+  if (P.x.rows > 0) {
+    if (!a->values || !a->indices) return bad("null record");
+    if (!aligned(a->values, a->value_type == SQ_F32 ? 4 : 2) || !aligned(a->indices, 4)) return bad("misaligned record");
+  }
+  P.values = a->values; P.indices = a->indices; P.k = a->k; P.values_type = a->value_type;
+  P.temperature = a->temperature; P.weight = a->weight; P.weight_stride = a->weight_stride;
+  P.loss = a->loss; P.stats = reinterpret_cast<float2*>(a->stats); P.grad = a->grad; P.grad_stride = a->grad_stride;
+  return SQ_OK;
+}
+int distill_grad_params(const DistillParams& P, const char* who) {
+  if (!P.grad) return fail(SQ_EINVAL, std::string(who) + ": null gradient");
+  if (P.grad_stride < P.x.vocab) return fail(SQ_EINVAL, std::string(who) + ": gradient rows overlap");
+  if (!aligned(P.grad, P.x.type == SQ_F32 ? 4 : 2)) return fail(SQ_EINVAL, std::string(who) + ": misaligned gradient");
+  return SQ_OK;
+}
+}  // namespace
+
+int sq_sample(const sq_sample_args* a, void* stream) {
+  if (!a) return fail(SQ_EINVAL, "sample: null argument");
+  SampleParams P{};
+  if (int s = logits_rows(a->logits, "sample", P.x)) return s;
+  if (P.x.rows == 0) return SQ_OK;
+  if (!a->uniform || !a->tokens) return fail(SQ_EINVAL, "sample: null uniform or tokens");
+  P.uniform = a->uniform; P.temperature = a->temperature; P.top_p = a->top_p; P.min_p = a->min_p; P.top_k = a->top_k;
+  P.temperature_all = a->temperature_all; P.top_p_all = a->top_p_all; P.min_p_all = a->min_p_all;
+  P.top_k_all = a->top_k_all; P.tokens = (long long*)a->tokens;
+  return check(launch_sample(P, (cudaStream_t)stream), "sample");
+}
+
+int sq_top_logits(const sq_logits* l, int k, void* values, int32_t* indices, void* stream) {
+  if (!l) return fail(SQ_EINVAL, "top_logits: null argument");
+  TopParams P{};
+  if (int s = logits_rows(*l, "top_logits", P.x)) return s;
+  if (k < 1 || k > kMaxRecord || k > P.x.vocab) return fail(SQ_EINVAL, "top_logits: k must be in [1, min(1024, vocab)]");
+  if (P.x.rows == 0) return SQ_OK;
+  if (!values || !indices) return fail(SQ_EINVAL, "top_logits: null output");
+  P.k = k; P.values = values; P.indices = indices;
+  return check(launch_top_logits(P, (cudaStream_t)stream), "top_logits");
+}
+
+int sq_distill_forward(const sq_distill_args* a, void* stream) {
+  DistillParams P;
+  if (int s = distill_params(a, "distill_forward", P)) return s;
+  if (P.x.rows == 0) return SQ_OK;
+  if (!P.loss) return fail(SQ_EINVAL, "distill_forward: null loss");
+  if (!aligned(P.stats, 8)) return fail(SQ_EINVAL, "distill_forward: stats must be 8-byte aligned");
+  return check(launch_distill_forward(P, (cudaStream_t)stream), "distill_forward");
+}
+
+int sq_distill_backward(const sq_distill_args* a, void* stream) {
+  DistillParams P;
+  if (int s = distill_params(a, "distill_backward", P)) return s;
+  if (P.x.rows == 0) return SQ_OK;
+  if (!P.stats || !aligned(P.stats, 8)) return fail(SQ_EINVAL, "distill_backward: stats missing or not 8-byte aligned");
+  if (int s = distill_grad_params(P, "distill_backward")) return s;
+  return check(launch_distill_backward(P, (cudaStream_t)stream), "distill_backward");
+}
+
+int sq_distill_loss_grad(const sq_distill_args* a, void* stream) {
+  DistillParams P;
+  if (int s = distill_params(a, "distill_loss_grad", P)) return s;
+  if (P.x.rows == 0) return SQ_OK;
+  if (!P.loss) return fail(SQ_EINVAL, "distill_loss_grad: null loss");
+  if (int s = distill_grad_params(P, "distill_loss_grad")) return s;
+  P.stats = nullptr;
+  return check(launch_distill_loss_grad(P, (cudaStream_t)stream), "distill_loss_grad");
 }
 
 }  // extern "C"

@@ -84,6 +84,25 @@ class LayerDesc(C.Structure):
                 ('permutation', p), ('basis', p), ('latent_scale', p), ('predictor', p)]
 
 
+F16, BF16, F32 = range(3)
+
+
+class Logits(C.Structure):
+    _fields_ = [('data', p), ('row_stride', i64), ('rows', i32), ('vocab', i32), ('type', i32)]
+
+
+class SampleArgs(C.Structure):
+    _fields_ = [('logits', Logits), ('uniform', p), ('temperature', p), ('top_k', p), ('top_p', p), ('min_p', p),
+                ('temperature_all', C.c_float), ('top_k_all', i32), ('top_p_all', C.c_float), ('min_p_all', C.c_float),
+                ('tokens', p)]
+
+
+class DistillArgs(C.Structure):
+    _fields_ = [('logits', Logits), ('values', p), ('indices', p), ('k', i32), ('value_type', i32),
+                ('temperature', C.c_float), ('weight', p), ('weight_stride', i64), ('loss', p), ('stats', p),
+                ('grad', p), ('grad_stride', i64)]
+
+
 # name -> (restype, argtypes)
 _PROTOS = {
     'sq_abi_version': (C.c_int, []),
@@ -126,6 +145,11 @@ _PROTOS = {
     'sq_model_score': (C.c_int, [p, p, C.c_int, p, p, p]),
     'sq_model_greedy': (C.c_int, [p, p, C.c_int, p, p, p]),
     'sq_model_check': (C.c_int, [p, p]),
+    'sq_sample': (C.c_int, [C.POINTER(SampleArgs), p]),
+    'sq_top_logits': (C.c_int, [C.POINTER(Logits), C.c_int, p, p, p]),
+    'sq_distill_forward': (C.c_int, [C.POINTER(DistillArgs), p]),
+    'sq_distill_backward': (C.c_int, [C.POINTER(DistillArgs), p]),
+    'sq_distill_loss_grad': (C.c_int, [C.POINTER(DistillArgs), p]),
 }
 
 _lib = None

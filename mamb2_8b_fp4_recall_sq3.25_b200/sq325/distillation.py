@@ -1,0 +1,140 @@
+"""Distillation from a teacher's largest logits (sq_top_logits, sq_distill_*).
+
+The teacher's record of a token is its k largest logits and their indices (`top_logits`).  With
+q the softmax of the recorded logits / T over the record and p the student's softmax of its
+logits / T over the whole vocabulary,
+
+    loss = T^2 sum_k q_k (log q_k - log p_jk),    d loss / d s_j = T (p_j - q_j)
+
+(q_j = 0 outside the record).  `distillation_loss` is differentiable in the student's logits: its
+backward reads the logits again and recomputes p from the row's maximum and sum.
+`distillation_loss_grad` gives loss and gradient in one call, for steps that know each row's
+weight beforehand.  Sums are fp32, the gradient is rounded once to the logits' type.  Places of
+the record with an index outside the vocabulary or a value of -inf or NaN are unused; a row
+without used places has loss 0 and gradient 0.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+from .sampling import _TYPES, logits_args, logits_rows
+
+__all__ = ['top_logits', 'distillation_loss', 'distillation_loss_grad']
+
+MAX_RECORD = 1024
+
+
+@torch.no_grad()
+def top_logits(logits, k):
+    """The k largest of each row of logits [..., vocab], largest first and equal ones by index:
+    (values [..., k] in the logits' dtype, indices int32 [..., k]).  k in [1, min(1024, vocab)].
+    NaN and -inf are not taken; places left over hold -inf and -1."""
+    x = logits_rows(logits)
+    if isinstance(k, bool) or not isinstance(k, int) or not 1 <= k <= min(MAX_RECORD, x.shape[1]):
+        raise ValueError(f'k must be an integer in [1, min({MAX_RECORD}, vocab)]')
+    shape = (*logits.shape[:-1], k)
+    values = torch.empty(shape, device=x.device, dtype=x.dtype)
+    indices = torch.empty(shape, device=x.device, dtype=torch.int32)
+    with torch.cuda.device(x.device):
+        _lib.call('sq_top_logits', C.byref(logits_args(x)), k, values.data_ptr(), indices.data_ptr(), _lib.stream_ptr())
+    return values, indices
+
+
+def _checked(logits, values, indices, temperature):
+    x = logits_rows(logits)
+    if not isinstance(values, torch.Tensor) or not isinstance(indices, torch.Tensor) or values.shape != indices.shape \
+            or values.shape[:-1] != logits.shape[:-1] or values.ndim != logits.ndim:
+        raise ValueError('The record must be values and indices [..., k] with the leading shape of the logits')
+    if not 1 <= values.shape[-1] <= MAX_RECORD:
+        raise ValueError(f'The record must have 1 to {MAX_RECORD} entries a row')
+    if values.dtype not in _TYPES or indices.dtype != torch.int32 or values.device != x.device \
+            or indices.device != x.device:
+        raise ValueError('The record must be FP16, BF16 or FP32 values and int32 indices on the device of the logits')
+    if values.requires_grad:
+        raise ValueError("The teacher's record receives no gradient: detach it")
+    if isinstance(temperature, bool) or not isinstance(temperature, (int, float)) or not 0 < temperature <= 3e38:
+        raise ValueError('temperature must be a positive finite number')
+    return x, values.contiguous(), indices.contiguous()
+
+
+def _args(x, values, indices, temperature, weight=None, loss=None, stats=None, grad=None):
+    a = _lib.DistillArgs()
+    a.logits = logits_args(x)
+    a.values, a.indices = values.data_ptr(), indices.data_ptr()
+    a.k, a.value_type = values.shape[-1], _TYPES[values.dtype]
+    a.temperature = temperature
+    if weight is not None:
+        a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0)
+    a.loss = loss.data_ptr() if loss is not None else None
+    a.stats = stats.data_ptr() if stats is not None else None
+    if grad is not None:
+        a.grad, a.grad_stride = grad.data_ptr(), x.shape[1]
+    return a
+
+
+def _forward(x, values, indices, temperature, lead, with_stats):
+    loss = torch.empty(lead, device=x.device, dtype=torch.float32)
+    stats = torch.empty((x.shape[0], 2), device=x.device, dtype=torch.float32) if with_stats else None
+    with torch.cuda.device(x.device):
+        _lib.call('sq_distill_forward', C.byref(_args(x, values, indices, temperature, loss=loss, stats=stats)),
+                  _lib.stream_ptr())
+    return loss, stats
+
+
+def _row_weights(weight):
+    """Per-row factors as a vector the kernels step through: a broadcast one keeps its stride of 0."""
+    return weight if weight.ndim == 1 else weight.reshape(-1)
+
+
+class _DistillationLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, indices, temperature):
+        x, values, indices = _checked(logits, values, indices, temperature)
+        loss, stats = _forward(x, values, indices, temperature, logits.shape[:-1], True)
+        ctx.save_for_backward(logits, values, indices, stats)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        logits, values, indices, stats = ctx.saved_tensors
+        x = logits_rows(logits)
+        grad = torch.empty(logits.shape, device=x.device, dtype=x.dtype)
+        a = _args(x, values, indices, ctx.temperature, weight=_row_weights(grad_loss), stats=stats, grad=grad)
+        with torch.cuda.device(x.device):
+            _lib.call('sq_distill_backward', C.byref(a), _lib.stream_ptr())
+        return grad, None, None, None
+
+
+def distillation_loss(logits, values, indices, temperature=1.0):
+    """Per-row distillation loss, fp32 [...], of the student's logits [..., vocab] against the
+    teacher's record (values [..., k], int32 indices [..., k], k <= 1024).  Differentiable in the
+    logits; the record receives no gradient."""
+    if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
+        return _DistillationLoss.apply(logits, values, indices, temperature)
+    x, values, indices = _checked(logits, values, indices, temperature)
+    return _forward(x, values, indices, temperature, logits.shape[:-1], False)[0]
+
+
+@torch.no_grad()
+def distillation_loss_grad(logits, values, indices, temperature=1.0, weight=None):
+    """(loss fp32 [...], gradient [..., vocab] in the logits' dtype) in one call.  weight: fp32
+    [...] factor of each row's gradient (None: 1), as the upstream gradient of the loss would be;
+    the loss itself is not weighted."""
+    x, values, indices = _checked(logits, values, indices, temperature)
+    lead = logits.shape[:-1]
+    if weight is not None:
+        if not isinstance(weight, torch.Tensor) or weight.shape != lead or weight.dtype != torch.float32 \
+                or weight.device != x.device:
+            raise ValueError(f'weight must be a float32 tensor of shape {tuple(lead)} on {x.device}')
+        weight = _row_weights(weight)
+    loss = torch.empty(lead, device=x.device, dtype=torch.float32)
+    grad = torch.empty(logits.shape, device=x.device, dtype=x.dtype)
+    with torch.cuda.device(x.device):
+        _lib.call('sq_distill_loss_grad', C.byref(_args(x, values, indices, temperature, weight=weight, loss=loss, grad=grad)),
+                  _lib.stream_ptr())
+    return loss, grad

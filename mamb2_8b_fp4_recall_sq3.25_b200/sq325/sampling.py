@@ -1,0 +1,79 @@
+"""Drawing tokens from rows of logits (sq_sample): temperature, top-k, top-p and min-p, from
+uniform numbers the caller gives.
+
+With m the row's largest logit, y_j = 2^((x_j - m) log2(e) / temperature) and the whole weight
+w_j = rint(y_j 2^31).  Tokens are ordered by logit, equal ones by index.  The settings apply in
+this order: top-k keeps the first k tokens, top-p those whose predecessors hold less than
+top_p of the kept weight (the first always), min-p those with y_j >= min_p.  The token drawn is
+the first in index order at which the running weight passes floor(uniform * total).  Weights and
+sums are integers, so the same inputs give the same token whatever the launch shape.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib
+
+__all__ = ['sample']
+
+MAX_VOCAB = 1 << 18
+_TYPES = {torch.float16: _lib.F16, torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+def logits_rows(logits):
+    """Checks a tensor of logits [..., vocab] and returns it as rows [n, vocab] whose last
+    dimension is contiguous (a copy only where its layout has no single row stride)."""
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _TYPES or not logits.is_cuda:
+        raise ValueError('Logits must be a CUDA FP16, BF16 or FP32 tensor')
+    if logits.ndim == 0 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
+        raise ValueError(f'Logits must be [..., vocab] with vocab in [1, {MAX_VOCAB}]')
+    x = logits if logits.ndim == 2 else logits.reshape(-1, logits.shape[-1])
+    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+
+
+def logits_args(x):
+    """ctypes view of rows that logits_rows() returned."""
+    return _lib.Logits(x.data_ptr(), x.stride(0), x.shape[0], x.shape[1], _TYPES[x.dtype])
+
+
+def _setting(name, value, x, lead, dtype, check):
+    """(tensor or None, number): a tensor holds one value a row, a number stands for all rows."""
+    if isinstance(value, torch.Tensor):
+        if value.shape != lead or value.dtype != dtype or value.device != x.device:
+            raise ValueError(f'{name} must be a number or a {dtype} tensor of shape {tuple(lead)} on {x.device}')
+        return value.contiguous(), 0
+    if isinstance(value, bool) or not isinstance(value, int if dtype == torch.int32 else (int, float)) \
+            or not check(value):
+        raise ValueError(f'{name} is out of range: {value!r}')
+    return None, value
+
+
+@torch.no_grad()
+def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """Draws one token per row of logits [..., vocab]: int64 [...].
+
+    logits: fp16, bf16 or fp32 on the GPU; NaN counts as masked (-inf).
+    uniform: fp32 [...] numbers in [0, 1), one a row.
+    temperature >= 0 (0: the largest logit, lowest index), top_k >= 0 (0: off), top_p in (0, 1]
+    (1: off), min_p in [0, 1] (0: off): a number for all rows, or a tensor [...] on the device
+    (fp32, top_k int32) with a setting per row, whose values are the caller's to check.
+    A row with nothing above -inf gives -1.
+    """
+    x = logits_rows(logits)
+    lead = logits.shape[:-1]
+    if not isinstance(uniform, torch.Tensor) or uniform.shape != lead or uniform.dtype != torch.float32 \
+            or uniform.device != x.device:
+        raise ValueError(f'uniform must be a float32 tensor of shape {tuple(lead)} on {x.device}')
+    uniform = uniform.contiguous()
+    t, t_all = _setting('temperature', temperature, x, lead, torch.float32, lambda v: 0 <= v < float('inf'))
+    k, k_all = _setting('top_k', top_k, x, lead, torch.int32, lambda v: 0 <= v < 2 ** 31)
+    p, p_all = _setting('top_p', top_p, x, lead, torch.float32, lambda v: 0 < v <= 1)
+    q, q_all = _setting('min_p', min_p, x, lead, torch.float32, lambda v: 0 <= v <= 1)
+    tokens = torch.empty(lead, device=x.device, dtype=torch.long)
+    a = _lib.SampleArgs(logits_args(x), uniform.data_ptr(), *(v.data_ptr() if v is not None else None for v in (t, k, p, q)),
+                        t_all, k_all, p_all, q_all, tokens.data_ptr())
+    with torch.cuda.device(x.device):
+        _lib.call('sq_sample', C.byref(a), _lib.stream_ptr())
+    return tokens

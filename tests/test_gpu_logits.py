@@ -1,0 +1,410 @@
+"""GPU tests of the operators on rows of logits against the 64-bit oracle: sq325.sample,
+top_logits, distillation_loss (with its backward) and distillation_loss_grad.
+
+Tolerances.  A draw's weights carry a relative error of at most (|t| + 4) 2^-24 with t the
+exponent (|t| <= 32 where the weight is not 0) plus half a step of 2^-31 each, so weight sums
+are off by less than 3e-6 + vocab 2^-32 < 7e-5 of the largest sum in the worst case and by
+about 1e-6 in practice: a draw whose margin is over 1e-4 must give the oracle's token, one with a
+smaller margin is not compared.  The loss and gradient bounds are written at their use.
+"""
+import numpy as np
+import pytest
+import torch
+
+from oracle import logits as ol
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+MARGIN = 1e-4
+
+
+def make(rows, vocab, dtype, seed, spread=3.0, pad=0, offset=0, banned=0.0):
+    """Logits with a few that stand out; `offset` shifts the rows' start off 16-byte boundaries."""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    buf = torch.randn(rows * (vocab + pad) + offset, generator=g, device='cuda') * spread
+    x = buf[offset:].view(rows, vocab + pad)
+    few = max(1, min(20, vocab // 4))
+    at = (torch.arange(few, device='cuda') * (vocab // few)).expand(rows, few)
+    x.scatter_(1, at, 3.0 + 9.0 * torch.rand((rows, few), generator=g, device='cuda'))
+    if banned:
+        x[:, :vocab].masked_fill_(torch.rand(vocab, generator=g, device='cuda') < banned, float('-inf'))
+    out = torch.empty(rows * (vocab + pad) + offset, device='cuda', dtype=dtype)
+    out[offset:].copy_(x.reshape(-1).to(dtype))
+    return out[offset:].view(rows, vocab + pad)[:, :vocab], g
+
+
+def wide(x):
+    return x.detach().cpu().double().numpy()
+
+
+def check_draw(x, u, t=1.0, k=0, p=1.0, q=0.0, least=0.5):
+    import sq325
+    got = sq325.sample(x, u, temperature=t, top_k=k, top_p=p, min_p=q).cpu().numpy()
+    pick = lambda v, r: float(v[r]) if isinstance(v, torch.Tensor) else v
+    xs, us = wide(x), u.cpu().numpy()
+    compared = 0
+    for r in range(len(xs)):
+        want, margin = ol.draw(xs[r], us[r], pick(t, r), int(pick(k, r)), pick(p, r), pick(q, r))
+        if margin > MARGIN:
+            compared += 1
+            assert got[r] == want, (r, got[r], want, margin)
+        elif want >= 0:
+            assert 0 <= got[r] < xs.shape[1] and xs[r, got[r]] > -np.inf
+    assert compared >= least * len(xs)
+    return got
+
+
+SETTINGS = [dict(t=0.0), dict(t=0.7), dict(k=1), dict(k=7), dict(k=50, p=0.9, t=0.8), dict(p=0.8), dict(p=0.95, t=0.6),
+            dict(q=0.1), dict(k=20, p=0.9, q=0.05, t=1.3), dict(p=1e-6)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [1, 2, 31, 257, 1000, 5003])
+def test_draw_matches_oracle(vocab, dtype):
+    x, g = make(16, vocab, dtype, seed=vocab, pad=3, offset=1)
+    for s in SETTINGS:
+        check_draw(x, torch.rand(16, generator=g, device='cuda'), **s)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [32003, 256000, 262144])
+@pytest.mark.parametrize('spread', [1.0, 3.0])
+def test_draw_large_vocab(vocab, dtype, spread):
+    x, g = make(4, vocab, dtype, seed=vocab, spread=spread, pad=1, banned=0.05)
+    for s in (dict(k=50, p=0.9, t=0.8), dict(k=2000, p=0.9), dict(p=0.7, t=0.8), dict(p=0.9), dict(q=0.02), dict(t=0.0)):
+        check_draw(x, torch.rand(4, generator=g, device='cuda'), least=0.0, **s)
+
+
+def test_draw_settings_per_row():
+    x, g = make(64, 4099, torch.float16, seed=3)
+    pick = lambda v, d: torch.tensor(v, device='cuda', dtype=d)[torch.randint(0, len(v), (64,), generator=g, device='cuda')]
+    check_draw(x, torch.rand(64, generator=g, device='cuda'), t=pick([0.0, 0.5, 1.0], torch.float32),
+               k=pick([0, 1, 40], torch.int32), p=pick([0.5, 0.9, 1.0], torch.float32), q=pick([0.0, 0.1], torch.float32))
+
+
+@pytest.mark.parametrize('vocab,settings', [(37, dict()), (1500, dict(top_k=9)), (1500, dict(top_p=0.9)),
+                                            (70001, dict(top_p=0.6)), (70001, dict(top_k=3000, top_p=0.5, temperature=1.5))])
+def test_draw_follows_the_distribution(vocab, settings):
+    """The same row drawn at an even grid of uniform numbers: every token as often as its share says."""
+    import sq325
+    x, _ = make(1, vocab, torch.float32, seed=5)
+    n = 4096
+    u = (torch.arange(n, device='cuda') + 0.5) / n
+    got = sq325.sample(x.expand(n, vocab), u, **settings).cpu().numpy()
+    xs = wide(x)[0]
+    T = settings.get('temperature', 1.0)
+    by = ol.order(xs)
+    w = np.exp((xs[by] - xs.max()) / T)
+    if settings.get('top_k'):
+        w[settings['top_k']:] = 0
+    if settings.get('top_p'):
+        w[np.cumsum(w) - w >= settings['top_p'] * w.sum()] = 0
+    share = np.zeros(vocab)
+    share[by] = w / w.sum()
+    assert (np.diff(got) >= 0).all()                     # the draw is monotone in the uniform number
+    # a grid of n points puts n share +- 1 of them into an interval; sums are 1e-4 off at most, and
+    # the cut of top-p may take one token more or less
+    assert np.abs(np.bincount(got, minlength=vocab) - n * share).max() <= 2 + n * MARGIN
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_draw_ties_masks_and_nonfinite(dtype):
+    import sq325
+    inf = float('inf')
+    u = lambda *v: torch.tensor(v, device='cuda')
+    for vocab in (64, 5003, 70001):
+        x = torch.zeros((4, vocab), device='cuda', dtype=dtype)
+        # all equal: ties go by index
+        got = sq325.sample(x, u(0.0, 0.25, 0.5, 0.999), top_k=4).tolist()
+        assert got == [0, 1, 2, 3]
+        got = sq325.sample(x, u(0.0, 0.25, 0.5, 0.999)).tolist()
+        assert got == [0, vocab // 4, vocab // 2, int(np.floor(np.float32(0.999).astype(np.float64) * vocab))]
+        p = 0.5
+        last = int(np.ceil(p * vocab)) - 1
+        assert sq325.sample(x, u(0.0, 0.0, 1.0 - 2 ** -24, 1.0 - 2 ** -24), top_p=p).tolist() == [0, 0, last, last]
+        x[:, ::2] = -0.0                                 # -0 and +0 are equal
+        assert sq325.sample(x, u(0.0, 0.25, 0.5, 0.999), top_k=4).tolist() == [0, 1, 2, 3]
+        x = torch.full((6, vocab), -inf, device='cuda', dtype=dtype)
+        x[1, vocab - 1] = -5.0                           # one token left
+        x[2] = float('nan')
+        x[2, 7] = 1.0
+        x[3] = torch.finfo(dtype).min                    # masked by the lowest value: still tokens
+        x[4, 3] = x[4, 9] = inf
+        x[4, 5] = 2.0
+        x[5] = float('nan')
+        for s in (dict(), dict(top_k=3), dict(top_p=0.9), dict(min_p=0.2), dict(temperature=0.0),
+                  dict(top_k=1100, top_p=0.99, min_p=0.1)):
+            got = sq325.sample(x, u(0.6, 0.6, 0.6, 0.0, 0.6, 0.6), **s).tolist()
+            assert got == [-1, vocab - 1, 7, 0, 3 if s.get('temperature') == 0.0 else 9, -1], s
+    x, g = make(8, 3001, dtype, seed=9)
+    r = torch.rand(8, generator=g, device='cuda')
+    base = sq325.sample(x, r, top_k=100, top_p=0.9)
+    holes = torch.cat([x, torch.full((8, 700), float('nan'), device='cuda', dtype=dtype),
+                       torch.full((8, 5), torch.finfo(dtype).min, device='cuda', dtype=dtype)], 1)
+    assert torch.equal(base, sq325.sample(holes, r, top_k=100, top_p=0.9))
+
+
+def test_draw_extremes_of_temperature():
+    import sq325
+    x, g = make(8, 999, torch.float32, seed=1)
+    u = torch.rand(8, generator=g, device='cuda')
+    assert torch.equal(sq325.sample(x, u, temperature=1e-30), x.argmax(1))
+    assert torch.equal(sq325.sample(x, u, temperature=1e-42), x.argmax(1))
+    got = sq325.sample(x, u, temperature=1e30)           # even over the vocabulary
+    assert (got.double() - torch.floor(u.double() * 999)).abs().max() <= 1
+    t = torch.full((8,), float('nan'), device='cuda')    # a setting that is no temperature: greedy
+    assert torch.equal(sq325.sample(x, u, temperature=t), x.argmax(1))
+
+
+def test_draw_shapes_streams_and_repeats():
+    import sq325
+    x, g = make(12, 20011, torch.bfloat16, seed=2, pad=5)
+    u = torch.rand(12, generator=g, device='cuda')
+    want = sq325.sample(x, u, top_p=0.9)
+    assert torch.equal(want.view(3, 4), sq325.sample(x.reshape(3, 4, -1), u.view(3, 4), top_p=0.9))
+    assert torch.equal(want[5], sq325.sample(x[5], u[5], top_p=0.9))
+    assert torch.equal(want, sq325.sample(x.t().contiguous().t(), u, top_p=0.9))      # not contiguous along the row
+    assert sq325.sample(x[:0], u[:0]).shape == (0,)
+    for _ in range(5):
+        assert torch.equal(want, sq325.sample(x, u, top_p=0.9))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        y = x * 1.0
+        got = sq325.sample(y, u, top_p=0.9)
+    side.synchronize()
+    assert torch.equal(want, got)
+
+
+def test_draw_more_rows_than_fit_at_once():
+    x, g = make(1500, 1013, torch.float16, seed=4)
+    check_draw(x, torch.rand(1500, generator=g, device='cuda'), k=40, p=0.9, least=0.9)
+
+
+# ------------------------------------------------------------------ the largest logits
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,vocab,k,pad,offset', [(1, 1, 1, 0, 0), (3, 2, 2, 1, 1), (5, 33, 33, 0, 3), (7, 1000, 1, 5, 0),
+                                                     (7, 1000, 1000, 0, 0), (4, 5003, 64, 3, 1), (3, 70001, 1024, 1, 0),
+                                                     (2, 256000, 20, 0, 0), (2, 262144, 333, 7, 1), (700, 1021, 17, 0, 0)])
+def test_top_logits(rows, vocab, k, pad, offset, dtype):
+    import sq325
+    x, _ = make(rows, vocab, dtype, seed=vocab + k, pad=pad, offset=offset, banned=0.1 if vocab > 100 else 0.0)
+    values, indices = sq325.top_logits(x, k)
+    assert values.dtype == dtype and indices.dtype == torch.int32 and values.shape == indices.shape == (rows, k)
+    xs = wide(x)
+    for r in range(min(rows, 40)):
+        v, i = ol.top(xs[r], k)
+        assert np.array_equal(indices[r].cpu().numpy(), i)
+        assert np.array_equal(wide(values[r]), v)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_top_logits_ties_and_masks(dtype):
+    import sq325
+    inf = float('inf')
+    for vocab in (50, 4097, 70001):
+        x = torch.zeros((7, vocab), device='cuda', dtype=dtype)
+        x[1] = -inf
+        x[2] = -inf
+        x[2, [3, 41]] = torch.tensor([1.0, 2.0], device='cuda', dtype=dtype)
+        x[3] = float('nan')
+        x[3, 40] = torch.finfo(dtype).min
+        x[4, 10] = inf
+        x[4, 49] = 3.0
+        x[5, ::3] = -0.0
+        x[6] = torch.finfo(dtype).min
+        x[6, 5] = -inf
+        values, indices = sq325.top_logits(x, 6)
+        xs = wide(x)
+        for r in range(7):
+            v, i = ol.top(xs[r], 6)
+            assert np.array_equal(indices[r].cpu().numpy(), i), (vocab, r)
+            assert np.array_equal(wide(values[r]), v)
+
+
+# ------------------------------------------------------------------ distillation
+def record(g, rows, vocab, k, dtype, cut=0.3):
+    at = torch.rand((rows, vocab), generator=g, device='cuda').argsort(1)[:, :k] if vocab <= 6000 else \
+        (torch.randint(0, vocab, (rows, 1), generator=g, device='cuda') + torch.arange(k, device='cuda') * (vocab // k)) % vocab
+    values = (torch.randn((rows, k), generator=g, device='cuda') * 3).to(dtype)
+    gone = torch.rand((rows, k), generator=g, device='cuda') < cut
+    return values, at.int().masked_fill(gone, -1)
+
+
+UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+LEAST = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -126}
+
+
+def check_distill(x, values, indices, T, weight, loss, grad=None):
+    """fp32 chains: the exponent t of a power carries |t| 2^-23 (a difference, a product), the
+    hardware's power 2^-22, a sum of n terms added by 512 threads n / 512 + 20 roundings.  With
+    e = (|t| + n / 512 + 40) 2^-23: p and q are off by e relative, the loss by T^2 e (1 + |log|) per
+    unit of q, the gradient by T w e (p + q) and its own rounding."""
+    vocab, k = x.shape[1], values.shape[1]
+    xs, vs, js, ws = wide(x), wide(values), indices.cpu().numpy(), wide(weight)
+    for r in range(len(xs)):
+        want, g, p, q = ol.distill(xs[r], vs[r], js[r], T, ws[r])
+        if not (js[r] >= 0).any():
+            assert float(loss[r]) == 0.0
+            assert grad is None or not grad[r].any()
+            continue
+        finite = xs[r][np.isfinite(xs[r])]
+        far = (finite.max() - finite.min()) / T * 1.45
+        e = (far + (vocab + k) / 512 + 40) * 2.0 ** -23
+        assert abs(float(loss[r]) - want) <= T * T * e * (1 + 3 * far), r
+        if grad is not None:
+            got = wide(grad[r])
+            bound = T * abs(ws[r]) * e * (p + q) + UNIT[x.dtype] * np.abs(g) * 1.01 + LEAST[x.dtype]
+            assert (np.abs(got - g) <= bound).all(), (r, np.abs(got - g).max())
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('rows,vocab,k,T,pad,offset', [(1, 1, 1, 1.0, 0, 0), (5, 2, 2, 2.0, 1, 1), (3, 33, 5, 0.7, 3, 0),
+                                                       (9, 1000, 64, 1.0, 0, 0), (8, 5003, 17, 2.5, 1, 1),
+                                                       (6, 5003, 1024, 1.0, 0, 3), (3, 70001, 100, 1.0, 2, 0),
+                                                       (3, 256000, 64, 2.0, 0, 0), (2, 262143, 1, 1.0, 1, 0)])
+def test_distillation(rows, vocab, k, T, pad, offset, dtype):
+    import sq325
+    x, g = make(rows, vocab, dtype, seed=vocab + k, pad=pad, offset=offset)
+    values, indices = record(g, rows, vocab, k, dtype)
+    weight = torch.rand(rows, generator=g, device='cuda') * 8 - 2
+    loss, grad = sq325.distillation_loss_grad(x, values, indices, temperature=T, weight=weight)
+    assert loss.dtype == torch.float32 and grad.dtype == dtype and grad.shape == x.shape
+    check_distill(x, values, indices, T, weight, loss, grad)
+    check_distill(x, values, indices, T, weight, sq325.distillation_loss(x, values, indices, temperature=T))
+    y = x.detach().requires_grad_(True)
+    loss = sq325.distillation_loss(y, values, indices, temperature=T)
+    check_distill(x, values, indices, T, weight, loss.detach(), torch.autograd.grad(loss, y, weight)[0])
+
+
+def test_distillation_many_rows():
+    import sq325
+    x, g = make(1300, 777, torch.float16, seed=1)
+    values, indices = record(g, 1300, 777, 9, torch.float16)
+    weight = torch.ones(1300, device='cuda')
+    loss, grad = sq325.distillation_loss_grad(x, values, indices)
+    check_distill(x, values, indices, 1.0, weight, loss, grad)
+    y = x.detach().requires_grad_(True)
+    loss = sq325.distillation_loss(y, values, indices)
+    check_distill(x, values, indices, 1.0, weight, loss.detach(), torch.autograd.grad(loss.sum(), y)[0])
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+def test_distillation_masks_and_repeats(dtype):
+    import sq325
+    vocab = 3001
+    x, g = make(8, vocab, dtype, seed=11)
+    values, indices = record(g, 8, vocab, 40, torch.float32, cut=0.0)
+    indices[0] = -1                                      # no teacher
+    indices[1, 5:] = -1
+    indices[2, ::2] = indices[2, 0].clone()              # one token twenty times
+    indices[3, 3] = vocab                                # outside the vocabulary
+    values[4, 1] = float('-inf')
+    values[4, 2] = float('nan')
+    values[5] = float('-inf')                            # a record without values
+    free = torch.ones(vocab, dtype=torch.bool, device='cuda')
+    free[indices[6].long()] = False
+    x[6].masked_fill_(free & (torch.arange(vocab, device='cuda') % 2 == 0), float('-inf'))
+    x[7].masked_fill_(torch.arange(vocab, device='cuda') % 3 == 0, torch.finfo(dtype).min)
+    x[7].scatter_(0, indices[7].long(), torch.ones(40, device='cuda', dtype=dtype))
+    weight = torch.linspace(-1, 2, 8, device='cuda')
+    seen = indices.clone()
+    seen[5] = -1
+    values_seen = torch.where(torch.isnan(values), float('-inf'), values)
+    loss, grad = sq325.distillation_loss_grad(x, values, indices, weight=weight)
+    check_distill(x, values_seen, seen, 1.0, weight, loss, grad)
+    y = x.detach().requires_grad_(True)
+    loss = sq325.distillation_loss(y, values, indices)
+    check_distill(x, values_seen, seen, 1.0, weight, loss.detach(), torch.autograd.grad(loss, y, weight)[0])
+
+
+def test_distillation_undefined_student():
+    import sq325
+    x = torch.zeros((5, 600), device='cuda')
+    x[0, 3] = float('nan')
+    x[1, 3] = float('inf')
+    x[2] = float('-inf')
+    x[3, 4] = float('-inf')                              # the teacher's token is masked: the loss is infinite
+    values = torch.zeros((5, 2), device='cuda')
+    indices = torch.tensor([[4, 5]], device='cuda', dtype=torch.int32).expand(5, 2).contiguous()
+    indices[4] = -1
+    x[4] = float('nan')                                  # no teacher: nothing is learnt
+    loss, grad = sq325.distillation_loss_grad(x, values, indices)
+    y = x.clone().requires_grad_(True)
+    again = sq325.distillation_loss(y, values, indices)
+    back = torch.autograd.grad(again.sum(), y)[0]
+    for l, g in ((loss, grad), (again, back)):
+        assert l[:3].isnan().all() and g[:3].isnan().all()
+        assert l[3] == float('inf') and g[3].isfinite().all() and g[3, 4] == -0.5
+        assert l[4] == 0 and not g[4].any()
+
+
+def test_distillation_gradient_against_differences():
+    """Central differences of the loss along random directions: with a step h = 2^-5 the fp32 loss
+    (about 5, off by 1e-6) gives slopes good to 1e-6 / h, the third derivative adds h^2."""
+    import sq325
+    x, g = make(6, 403, torch.float32, seed=8, spread=1.0)
+    values, indices = record(g, 6, 403, 30, torch.float32)
+    _, grad = sq325.distillation_loss_grad(x, values, indices, temperature=1.5)
+    h = 2.0 ** -5
+    for _ in range(8):
+        d = torch.randn(x.shape, generator=g, device='cuda')
+        up, down = (sq325.distillation_loss(x + s * h * d, values, indices, temperature=1.5) for s in (1, -1))
+        slope = (up.double() - down.double()) / (2 * h)
+        assert (slope - (grad.double() * d.double()).sum(1)).abs().max() <= 1e-4 + 4 * h * h
+
+
+def test_distillation_shapes_strides_and_reductions():
+    import sq325
+    x, g = make(12, 2003, torch.bfloat16, seed=6, pad=4)
+    values, indices = record(g, 12, 2003, 10, torch.bfloat16)
+    loss, grad = sq325.distillation_loss_grad(x, values, indices)
+    l3, g3 = sq325.distillation_loss_grad(x.reshape(3, 4, -1), values.view(3, 4, 10), indices.view(3, 4, 10))
+    assert torch.equal(l3.view(-1), loss) and torch.equal(g3.view(12, -1), grad)
+    l0, g0 = sq325.distillation_loss_grad(x[2], values[2], indices[2])
+    assert l0.shape == () and torch.equal(l0, loss[2]) and torch.equal(g0, grad[2])
+    y = x.detach().clone().requires_grad_(True)          # a mean's upstream gradient is one broadcast number
+    sq325.distillation_loss(y, values, indices).mean().backward()
+    _, want = sq325.distillation_loss_grad(x, values, indices, weight=torch.full((12,), 1 / 12, device='cuda'))
+    assert torch.allclose(y.grad.float(), want.float(), rtol=2 ** -7, atol=1e-7)
+    _, same = sq325.distillation_loss_grad(x, values, indices, weight=torch.full((1,), 1 / 12, device='cuda').expand(12))
+    assert torch.equal(same, want)
+    z = x.t().contiguous().t().detach().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(sq325.distillation_loss(z, values, indices).sum(), z)[0], grad)
+    e = sq325.distillation_loss_grad(x[:0], values[:0], indices[:0])
+    assert e[0].shape == (0,) and e[1].shape == (0, 2003)
+    shared, _ = sq325.distillation_loss_grad(x[:1].expand(12, 2003), values, indices)     # one row read by all
+    assert shared.isfinite().all() and torch.equal(shared[0], loss[0])
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    import sq325
+    x = torch.zeros((2, 10), device='cuda')
+    u = torch.zeros(2, device='cuda')
+    v, i = torch.zeros((2, 3), device='cuda'), torch.zeros((2, 3), device='cuda', dtype=torch.int32)
+    bad = [lambda: sq325.sample(x.cpu(), u), lambda: sq325.sample(x.double(), u), lambda: sq325.sample(x, u[:1]),
+           lambda: sq325.sample(x, u.double()), lambda: sq325.sample(x, u.cpu()), lambda: sq325.sample(x[:, :0], u),
+           lambda: sq325.sample(torch.zeros((1, (1 << 18) + 1), device='cuda'), u[:1]),
+           lambda: sq325.sample(x, u, temperature=-1.0), lambda: sq325.sample(x, u, temperature=float('inf')),
+           lambda: sq325.sample(x, u, temperature=float('nan')), lambda: sq325.sample(x, u, top_k=-1),
+           lambda: sq325.sample(x, u, top_k=2.0), lambda: sq325.sample(x, u, top_p=0.0), lambda: sq325.sample(x, u, top_p=1.5),
+           lambda: sq325.sample(x, u, min_p=-0.1), lambda: sq325.sample(x, u, min_p=1.1),
+           lambda: sq325.sample(x, u, temperature=u[:1]), lambda: sq325.sample(x, u, top_k=u),
+           lambda: sq325.sample(torch.zeros((), device='cuda'), u),
+           lambda: sq325.top_logits(x, 0), lambda: sq325.top_logits(x, 11), lambda: sq325.top_logits(x, 2.0),
+           lambda: sq325.top_logits(torch.zeros((1, 2000), device='cuda'), 1025), lambda: sq325.top_logits(x.int(), 1),
+           lambda: sq325.distillation_loss(x, v, i.long()), lambda: sq325.distillation_loss(x, v[:1], i[:1]),
+           lambda: sq325.distillation_loss(x, v, i[:, :2]), lambda: sq325.distillation_loss(x, v.double(), i),
+           lambda: sq325.distillation_loss(x, v, i, temperature=0.0),
+           lambda: sq325.distillation_loss(x, v, i, temperature=float('nan')),
+           lambda: sq325.distillation_loss(x, v.clone().requires_grad_(True), i),
+           lambda: sq325.distillation_loss(x, v[:, :0], i[:, :0]), lambda: sq325.distillation_loss(x, v.cpu(), i),
+           lambda: sq325.distillation_loss_grad(x, v, i, weight=u[:1]),
+           lambda: sq325.distillation_loss_grad(x, v, i, weight=u.double())]
+    for f in bad:
+        with pytest.raises(ValueError):
+            f()
+    # the context works on
+    assert sq325.sample(x, u).tolist() == [0, 0]
