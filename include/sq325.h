@@ -335,7 +335,7 @@ int sq_model_gemm_time(sq_model* model, double* seconds, int64_t* launches);
 /* ---------------------------------------------------------------- rows of logits
  * Operators on logits [rows, vocab] of type SQ_F16 / SQ_BF16 / SQ_F32 (no reference
  * counterpart: the reference's loops pick greedily).  Row r starts at data + r * row_stride
- * elements; vocab is at most 262144; data needs its type's alignment only.  All three
+ * elements; rows <= 2^24, vocab <= 262144; data needs its type's alignment only.  All three
  * operators are asynchronous on `stream`, allocate nothing and keep nothing between calls.
  * rows == 0 is a valid call that does nothing. */
 enum { SQ_F16 = 0, SQ_BF16 = 1, SQ_F32 = 2 };
@@ -376,7 +376,7 @@ int sq_top_logits(const sq_logits* logits, int k, void* values, int32_t* indices
  *   grad[r, j] = weight[r] temperature (p_j - sum over k with j_k = j of q_k)
  * (loss is not weighted).  A row without used entries has loss 0 and gradient 0; a student row
  * whose softmax is not defined (NaN, +inf, nothing above -inf) gives NaN.
- * sq_distill_forward writes loss and, if not NULL, stats [rows, 2] fp32, which
+ * sq_distill_forward writes loss and, if not NULL, stats [rows, 4] fp32 (16-byte aligned), which
  * sq_distill_backward reads to write grad; sq_distill_loss_grad writes loss and grad in one
  * call.  weight NULL: 1; weight_stride 0: one factor for every row.  grad has the logits'
  * type and must not overlap them. */

@@ -842,7 +842,8 @@ namespace {
 int logits_rows(const sq_logits& l, const char* who, LogitsRows& out) {
   const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
   if (l.type < SQ_F16 || l.type > SQ_F32) return bad("unknown logits type");
-  if (l.rows < 0 || l.vocab <= 0 || l.vocab > kMaxVocab) return bad("rows must be >= 0 and vocab in [1, 262144]");
+  if (l.rows < 0 || l.rows > kMaxRows || l.vocab <= 0 || l.vocab > kMaxVocab)
+    return bad("rows must be in [0, 2^24] and vocab in [1, 262144]");
   if (l.rows > 0 && !l.data) return bad("null logits");
   if (l.row_stride < 0) return bad("row stride must not be negative");
   if (!aligned(l.data, l.type == SQ_F32 ? 4 : 2)) return bad("logits are not aligned to their type");
@@ -865,7 +866,7 @@ int distill_params(const sq_distill_args* a, const char* who, DistillParams& P) 
   }
   P.values = a->values; P.indices = a->indices; P.k = a->k; P.values_type = a->value_type;
   P.temperature = a->temperature; P.weight = a->weight; P.weight_stride = a->weight_stride;
-  P.loss = a->loss; P.stats = reinterpret_cast<float2*>(a->stats); P.grad = a->grad; P.grad_stride = a->grad_stride;
+  P.loss = a->loss; P.stats = reinterpret_cast<float4*>(a->stats); P.grad = a->grad; P.grad_stride = a->grad_stride;
   return SQ_OK;
 }
 int distill_grad_params(const DistillParams& P, const char* who) {
@@ -904,7 +905,7 @@ int sq_distill_forward(const sq_distill_args* a, void* stream) {
   if (int s = distill_params(a, "distill_forward", P)) return s;
   if (P.x.rows == 0) return SQ_OK;
   if (!P.loss) return fail(SQ_EINVAL, "distill_forward: null loss");
-  if (!aligned(P.stats, 8)) return fail(SQ_EINVAL, "distill_forward: stats must be 8-byte aligned");
+  if (!aligned(P.stats, 16)) return fail(SQ_EINVAL, "distill_forward: stats must be 16-byte aligned");
   return check(launch_distill_forward(P, (cudaStream_t)stream), "distill_forward");
 }
 
@@ -912,7 +913,7 @@ int sq_distill_backward(const sq_distill_args* a, void* stream) {
   DistillParams P;
   if (int s = distill_params(a, "distill_backward", P)) return s;
   if (P.x.rows == 0) return SQ_OK;
-  if (!P.stats || !aligned(P.stats, 8)) return fail(SQ_EINVAL, "distill_backward: stats missing or not 8-byte aligned");
+  if (!P.stats || !aligned(P.stats, 16)) return fail(SQ_EINVAL, "distill_backward: stats missing or not 16-byte aligned");
   if (int s = distill_grad_params(P, "distill_backward")) return s;
   return check(launch_distill_backward(P, (cudaStream_t)stream), "distill_backward");
 }

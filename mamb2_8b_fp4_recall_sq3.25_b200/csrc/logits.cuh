@@ -7,6 +7,7 @@ namespace sq {
 
 enum LogitsType : int { kLogitsF16 = 0, kLogitsBf16 = 1, kLogitsF32 = 2 };
 
+constexpr int kMaxRows = 1 << 24;         // rows times CTAs of a row stay within a grid
 constexpr int kMaxVocab = 1 << 18;        // columns of a row
 constexpr int kMaxRecord = 1024;          // entries of one row's record of largest logits
 
@@ -45,7 +46,7 @@ struct DistillParams {
   const float* weight;                    // factor of each row's gradient; null: 1
   long long weight_stride;                // 0: one factor for every row
   float* loss;                            // [rows]
-  float2* stats;                          // [rows] {largest logit, 1 / sum of 2^((s - largest) c)}
+  float4* stats;                          // [rows] {m, 1 / S, v_max, 1 / Q (0: no record)}
   void* grad; long long grad_stride;      // the logits' type
 };
 int launch_distill_forward(const DistillParams& P, cudaStream_t st);   // loss, stats (optional)

@@ -32,6 +32,42 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-constexpr uint32_t kKeyNegInf = 0x007fffffu;     // order_key(-inf)
+
+// 16 bytes of a row.
+template <typename T> constexpr int kUnit = 16 / (int)sizeof(T);
+template <typename T> union Unit {
+  uint4 q;
+  T v[kUnit<T>];
+};
+__device__ __forceinline__ uint4 load_unit(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+
+// A row as whole 16-byte units between two ragged ends of fewer than a unit each: vectors need
+// 16-byte addresses, rows start where their stride puts them.
+template <typename T>
+struct RowSpan {
+  int head, units, tail;
+  __device__ RowSpan(const T* p, int n) {
+    head = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T));
+    units = (n - head) / kUnit<T>;
+    tail = n - head - units * kUnit<T>;
+  }
+  __device__ int edges() const { return head + tail; }
+  __device__ int edge(int i) const { return i < head ? i : units * kUnit<T> + i; }   // column of edge element i
+};
+
+// Cluster of the CTAs that share a row.
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
+// Address of `p` (shared memory of this CTA) in the CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t remote_smem(const void* p, uint32_t rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void remote_store(uint32_t addr, float a, float b) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" :: "r"(addr), "f"(a), "f"(b) : "memory");
+}
 
 }  // namespace sq

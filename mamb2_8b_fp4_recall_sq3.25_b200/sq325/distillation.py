@@ -77,7 +77,7 @@ def _args(x, values, indices, temperature, weight=None, loss=None, stats=None, g
 
 def _forward(x, values, indices, temperature, lead, with_stats):
     loss = torch.empty(lead, device=x.device, dtype=torch.float32)
-    stats = torch.empty((x.shape[0], 2), device=x.device, dtype=torch.float32) if with_stats else None
+    stats = torch.empty((x.shape[0], 4), device=x.device, dtype=torch.float32) if with_stats else None
     with torch.cuda.device(x.device):
         _lib.call('sq_distill_forward', C.byref(_args(x, values, indices, temperature, loss=loss, stats=stats)),
                   _lib.stream_ptr())
