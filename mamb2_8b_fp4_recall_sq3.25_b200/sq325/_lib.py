@@ -194,5 +194,17 @@ def stream_ptr(stream=None):
     return C.c_void_p(s.cuda_stream)
 
 
+def launch(name, device, *args):
+    """call() with the current stream of `device` appended, for short kernels: the device is
+    switched only when another one is current, and the stream handle is read without building
+    a Stream object."""
+    import torch
+    index = device.index
+    if index == torch.cuda.current_device():
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(device):
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
 def ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)

@@ -27,7 +27,6 @@ __all__ = ['top_logits', 'distillation_loss', 'distillation_loss_grad']
 MAX_RECORD = 1024
 
 
-@torch.no_grad()
 def top_logits(logits, k):
     """The k largest of each row of logits [..., vocab], largest first and equal ones by index:
     (values [..., k] in the logits' dtype, indices int32 [..., k]).  k in [1, min(1024, vocab)].
@@ -38,8 +37,7 @@ def top_logits(logits, k):
     shape = (*logits.shape[:-1], k)
     values = torch.empty(shape, device=x.device, dtype=x.dtype)
     indices = torch.empty(shape, device=x.device, dtype=torch.int32)
-    with torch.cuda.device(x.device):
-        _lib.call('sq_top_logits', C.byref(logits_args(x)), k, values.data_ptr(), indices.data_ptr(), _lib.stream_ptr())
+    _lib.launch('sq_top_logits', x.device, C.byref(logits_args(x)), k, values.data_ptr(), indices.data_ptr())
     return values, indices
 
 
@@ -78,9 +76,7 @@ def _args(x, values, indices, temperature, weight=None, loss=None, stats=None, g
 def _forward(x, values, indices, temperature, lead, with_stats):
     loss = torch.empty(lead, device=x.device, dtype=torch.float32)
     stats = torch.empty((x.shape[0], 4), device=x.device, dtype=torch.float32) if with_stats else None
-    with torch.cuda.device(x.device):
-        _lib.call('sq_distill_forward', C.byref(_args(x, values, indices, temperature, loss=loss, stats=stats)),
-                  _lib.stream_ptr())
+    _lib.launch('sq_distill_forward', x.device, C.byref(_args(x, values, indices, temperature, loss=loss, stats=stats)))
     return loss, stats
 
 
@@ -105,8 +101,7 @@ class _DistillationLoss(torch.autograd.Function):
         x = logits_rows(logits)
         grad = torch.empty(logits.shape, device=x.device, dtype=x.dtype)
         a = _args(x, values, indices, ctx.temperature, weight=_row_weights(grad_loss), stats=stats, grad=grad)
-        with torch.cuda.device(x.device):
-            _lib.call('sq_distill_backward', C.byref(a), _lib.stream_ptr())
+        _lib.launch('sq_distill_backward', x.device, C.byref(a))
         return grad, None, None, None
 
 
@@ -120,7 +115,6 @@ def distillation_loss(logits, values, indices, temperature=1.0):
     return _forward(x, values, indices, temperature, logits.shape[:-1], False)[0]
 
 
-@torch.no_grad()
 def distillation_loss_grad(logits, values, indices, temperature=1.0, weight=None):
     """(loss fp32 [...], gradient [..., vocab] in the logits' dtype) in one call.  weight: fp32
     [...] factor of each row's gradient (None: 1), as the upstream gradient of the loss would be;
@@ -134,7 +128,6 @@ def distillation_loss_grad(logits, values, indices, temperature=1.0, weight=None
         weight = _row_weights(weight)
     loss = torch.empty(lead, device=x.device, dtype=torch.float32)
     grad = torch.empty(logits.shape, device=x.device, dtype=x.dtype)
-    with torch.cuda.device(x.device):
-        _lib.call('sq_distill_loss_grad', C.byref(_args(x, values, indices, temperature, weight=weight, loss=loss, grad=grad)),
-                  _lib.stream_ptr())
+    _lib.launch('sq_distill_loss_grad', x.device,
+                C.byref(_args(x, values, indices, temperature, weight=weight, loss=loss, grad=grad)))
     return loss, grad

@@ -50,7 +50,6 @@ def _setting(name, value, x, lead, dtype, check):
     return None, value
 
 
-@torch.no_grad()
 def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """Draws one token per row of logits [..., vocab]: int64 [...].
 
@@ -74,6 +73,5 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     tokens = torch.empty(lead, device=x.device, dtype=torch.long)
     a = _lib.SampleArgs(logits_args(x), uniform.data_ptr(), *(v.data_ptr() if v is not None else None for v in (t, k, p, q)),
                         t_all, k_all, p_all, q_all, tokens.data_ptr())
-    with torch.cuda.device(x.device):
-        _lib.call('sq_sample', C.byref(a), _lib.stream_ptr())
+    _lib.launch('sq_sample', x.device, C.byref(a))
     return tokens
