@@ -47,21 +47,6 @@ __device__ float block_sum(float v, float* part) {
   return v;
 }
 
-// Largest value of a unit; NaN is passed over (it shows up in the sum).
-__device__ __forceinline__ float unit_max(const Unit<__half>& u) {
-  const __half2* h = reinterpret_cast<const __half2*>(&u.q);
-  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(__low2float(m), __high2float(m));
-}
-__device__ __forceinline__ float unit_max(const Unit<__nv_bfloat16>& u) {
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u.q);
-  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(__low2float(m), __high2float(m));
-}
-__device__ __forceinline__ float unit_max(const Unit<float>& u) {
-  return fmaxf(fmaxf(u.v[0], u.v[1]), fmaxf(u.v[2], u.v[3]));
-}
-
 __device__ __forceinline__ float record_value(const DistillParams& P, long long i) {
   switch (P.values_type) {
     case kLogitsF16: return __half2float(reinterpret_cast<const __half*>(P.values)[i]);

@@ -32,6 +32,10 @@ __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float key_logit(uint32_t key) {       // inverse, for keys of numbers
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+constexpr uint32_t kKeyLowest = 0x00800000u;     // order_key of the lowest finite number, one above -inf
 
 // 16 bytes of a row.
 template <typename T> constexpr int kUnit = 16 / (int)sizeof(T);
@@ -40,6 +44,21 @@ template <typename T> union Unit {
   T v[kUnit<T>];
 };
 __device__ __forceinline__ uint4 load_unit(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+
+// Largest value of a unit; NaN is passed over (it shows up in the sum).
+__device__ __forceinline__ float unit_max(const Unit<__half>& u) {
+  const __half2* h = reinterpret_cast<const __half2*>(&u.q);
+  const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float unit_max(const Unit<__nv_bfloat16>& u) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u.q);
+  const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float unit_max(const Unit<float>& u) {
+  return fmaxf(fmaxf(u.v[0], u.v[1]), fmaxf(u.v[2], u.v[3]));
+}
 
 // A row as whole 16-byte units between two ragged ends of fewer than a unit each: vectors need
 // 16-byte addresses, rows start where their stride puts them.
@@ -68,6 +87,14 @@ __device__ __forceinline__ uint32_t remote_smem(const void* p, uint32_t rank) {
 }
 __device__ __forceinline__ void remote_store(uint32_t addr, float a, float b) {
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" :: "r"(addr), "f"(a), "f"(b) : "memory");
+}
+__device__ __forceinline__ void remote_store(uint32_t addr, unsigned long long v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" :: "r"(addr), "l"(v) : "memory");
+}
+__device__ __forceinline__ unsigned long long remote_load(uint32_t addr) {
+  unsigned long long v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 }  // namespace sq
