@@ -61,10 +61,6 @@ __device__ __forceinline__ bool used_entry(const DistillParams& P, int j, float 
 __device__ __forceinline__ float record_power(float v, float vmax, float c) { return v == vmax ? 0.0f : (v - vmax) * c; }
 
 
-template <typename T> __device__ __forceinline__ uint4 neg_inf_unit() {
-  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-  return make_uint4(w, w, w, w);
-}
 // Sum of 2^((x - ref) c) over a unit.
 template <typename T>
 __device__ __forceinline__ float unit_power_sum(const Unit<T>& u, float ref, float c) {

@@ -9,18 +9,19 @@
 // token is a function of the inputs alone.  A token 2^-32 times less likely than the most
 // likely one has weight 0; rounding moves at most 2^-32 of the largest weight a token.
 //
-// A cluster of 1..8 CTAs shares a row, each with its part of it in shared memory: the row is
-// read from HBM once, every later pass runs on chip.  The CTAs exchange single numbers and
-// histograms through distributed shared memory.
+// A cluster of 1..8 CTAs shares a row; CTAs exchange single numbers, lists and histograms through
+// distributed shared memory.
 //
-// Record (few tokens wanted: top_logits, top-k).  Every thread knows the largest of its logits.
-// Each CTA finds the r-th largest of those, r = ceil(k / CTAs), to 16 bits of the key by
-// counting; at least k logits are not below the least of these bounds, and few more
-// (in rows that are not adversarial 1.1 k to 2 k).  Only threads whose largest passes look at their
-// logits again.  The candidates go to the first CTA, which ranks them by comparing all with all.
+// Few tokens wanted (top_logits, top-k up to 256, greedy): every thread streams its units of 16 bytes and
+// keeps eight maxima, of every eighth unit each.  The r-th largest of a CTA's 2048 maxima, r = k / CTAs, to
+// 16 bits of its key, is reached by r logits at least; the least of the CTAs' bounds by k logits of the
+// row, and by few more.  Only the units under a maximum that reaches it are read again (from L2), and
+// CTA 0 sorts what is not below it.  Rows where that is too much (thousands of equal logits at the
+// bound) are listed in column order instead, with a bound that is raised on the way.
 //
-// Cut (top-p, large k).  A histogram over 256 steps of 1/8 octave of y, with exact weights, finds
-// the step in which the running weight reaches what is wanted; the members of that step are
+// Otherwise (top-p, large k, none) the row stays on chip, each CTA with its part in shared memory: it is read
+// from HBM once.  A histogram over 256 steps of 1/8 octave of y, with exact weights, finds the
+// step in which the running weight reaches what is wanted; the members of that step are
 // narrowed by histograms over their keys until one key is left.  What is kept is then "logit
 // above the cut, or equal and index not above the last one kept".
 #include "logits.cuh"
@@ -30,17 +31,21 @@
 namespace sq {
 namespace {
 
-constexpr int NT = 512, NW = NT / 32;
+constexpr int NT = 256, NW = NT / 32;
 typedef unsigned long long u64;
 
-constexpr int kSteps = 256;                      // histogram over -8 log2 y
-constexpr int kCols = 8;                         // copies of it, by lane: fewer lanes meet in one word
-// A word of the histogram sums the low 19 bits of at most NT / 8 threads x 72 elements: < 2^32.
-// The upper 12 bits are not 0 for y >= 2^-12 only, the first 97 steps.
-constexpr int kLowBits = 19, kHighSteps = 98;
-constexpr int kFine = 256, kFineCols = 4, kFineLowBits = 18;   // narrowing: 128 threads x 72 x 2^18 < 2^32
-constexpr int kListBytes = kSteps * kCols * 4;   // candidates: 1024 of 8 bytes, or 2048 where k > 256
+// Histogram over rint(-7.96875 log2 y): 256 steps hold every weight but 0 (y > 2^-32).  Four copies
+// of it, by lane, so that fewer lanes meet in one word.  A word sums the low 18 bits of at most
+// NT / 4 threads x 136 elements: < 2^32.  The upper 13 bits are not 0 for y >= 2^-13 only, the first 105 steps.
+constexpr int kSteps = 256, kCols = 4, kLowBits = 18, kHighSteps = 106;
+constexpr float kPerOctave = 7.96875f;
+constexpr int kFine = 128;                       // entries of the narrowing histograms, laid out alike
+constexpr int kWorkBytes = (kSteps + kHighSteps) * kCols * 4;
 constexpr int kMembers = kHighSteps * kCols * 4 / 2;           // members of a step held as 16-bit positions
+constexpr int kList = 2048;                      // listed logits of a CTA
+constexpr int kGroups = 8 * NT;                  // maxima of a CTA
+constexpr int kListBytes = kList * 8 + kGroups * 2;
+constexpr int kMaxListed = kList / 8;            // top-k up to this many goes by the list
 
 struct Cut { float x; int last; };               // kept: above x, or equal and column <= last
 
@@ -52,8 +57,9 @@ struct Shared {
   u64 scan[NW];
   u64 found_above, found_mine;
   int found, count, pick;
+  uint2 counts[2][NW];
+  int groups;
   uint32_t key_low, key_high;
-  uint32_t weight[1024];
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -62,84 +68,23 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
   return v;
 }
 
-// One CTA's part of a row in shared memory.
-template <typename T>
-struct Part {
-  Unit<T>* unit;
-  int n, col0;                                   // units; column of the first element (may be < 0)
-  __device__ int col(int i, int v) const { return col0 + i * kUnit<T> + v; }
-};
-
-template <typename T>
-struct Row {
+// The CTAs of a cluster and what they exchange.
+struct Team {
   Shared& s;
-  Part<T> d;
-  unsigned char* work;                           // histogram / candidates / members
   uint32_t rank, size;
   int tid, phase;
-
-  __device__ Row(Shared& s, unsigned char* dyn, const LogitsRows& x, int work_bytes)
-      : s(s), work(dyn), rank(cluster_rank()), size(cluster_size()), tid(threadIdx.x), phase(0) {
-    cluster_arrive();
-    const T* p = reinterpret_cast<const T*>(x.data) + (long long)(blockIdx.x / size) * x.stride;
-    const int off = (int)((uintptr_t)p & 15) / (int)sizeof(T);
-    const int units = (off + x.vocab + kUnit<T> - 1) / kUnit<T>;
-    const int per = (units + (int)size - 1) / (int)size, u0 = (int)rank * per;
-    d.unit = reinterpret_cast<Unit<T>*>(dyn + work_bytes);
-    d.n = max(0, min(units, u0 + per) - u0);
-    d.col0 = u0 * kUnit<T> - off;
-    for (int i = tid; i < d.n; i += NT) {
-      const int c = d.col(i, 0);
-      if (c >= 0 && c + kUnit<T> <= x.vocab) {
-        cp_async16(d.unit + i, p + c);
-      } else {                                   // the row's ragged ends
-        Unit<T> u;
-#pragma unroll
-        for (int v = 0; v < kUnit<T>; ++v)
-          u.v[v] = c + v >= 0 && c + v < x.vocab ? p[c + v] : from_f32<T>(-INFINITY);
-        d.unit[i].q = u.q;
-      }
-    }
-    cp_async_wait_all();                         // each thread's own units
-    cluster_wait();
-  }
-
-  // f(x, column) over this thread's elements.
-  template <typename F>
-  __device__ void each(F f) const {
-    for (int i = tid; i < d.n; i += NT) {
-      Unit<T> u;
-      u.q = d.unit[i].q;
-#pragma unroll
-      for (int v = 0; v < kUnit<T>; ++v) f(to_f32(u.v[v]), i, v);
-    }
-  }
-  __device__ float own_max() const {
-    float m = -INFINITY;
-    for (int i = tid; i < d.n; i += NT) {
-      Unit<T> u;
-      u.q = d.unit[i].q;
-      m = fmaxf(m, unit_max(u));
-    }
-    return m;
-  }
-  __device__ void barrier() { cluster_arrive(); cluster_wait(); }
-  // Hands `v` (the same in every thread that stores) to all CTAs; afterwards got(r) is CTA r's.
+  __device__ explicit Team(Shared& s)
+      : s(s), rank(cluster_rank()), size(cluster_size()), tid(threadIdx.x), phase(0) { cluster_arrive(); }
+  // before the first remote access: every CTA runs
+  __device__ void ready() const { cluster_wait(); }
+  __device__ void barrier() const { cluster_arrive(); cluster_wait(); }
+  // Hands `v` (the same in every thread) to all CTAs; afterwards got(r) is CTA r's.
   __device__ void exchange(u64 v) {
     phase ^= 1;
     if (tid < (int)size) remote_store(remote_smem(&s.slot[phase][rank], tid), v);
     barrier();
   }
   __device__ u64 got(int r) const { return s.slot[phase][r]; }
-  __device__ u64 block_sum(u64 v) {
-    v = warp_sum(v);
-    __syncthreads();
-    if ((tid & 31) == 0) s.part[tid >> 5] = v;
-    __syncthreads();
-    u64 t = 0;
-    for (int i = 0; i < NW; ++i) t += s.part[i];
-    return t;
-  }
   __device__ float row_max(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -151,15 +96,392 @@ struct Row {
     for (int r = 0; r < (int)size; ++r) v = fmaxf(v, __uint_as_float((uint32_t)got(r)));
     return v;
   }
+  // Exclusive running sum of v over the threads; `total` the whole.
+  __device__ u64 block_scan(u64 v, u64& total) {
+    u64 run = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 a = __shfl_up_sync(0xffffffffu, run, o);
+      if ((tid & 31) >= o) run += a;
+    }
+    __syncthreads();
+    if ((tid & 31) == 31) s.part[tid >> 5] = run;
+    __syncthreads();
+    u64 before = 0;
+    total = 0;
+    for (int i = 0; i < NW; ++i) {
+      if (i < (tid >> 5)) before += s.part[i];
+      total += s.part[i];
+    }
+    return before + run - v;
+  }
+  // The largest number t of `bits` bits, an even number, for which count(t) summed over the block is at
+  // least r (0 where there is none); count falls with t and is at most 31 a thread.  Two bits a round.
+  template <typename C>
+  __device__ u64 search(int bits, int r, C count) {
+    u64 t = 0;
+#pragma unroll 1
+    for (int b = bits - 2; b >= 0; b -= 2) {
+      uint32_t c[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) c[i] = count(t | (u64)(i + 1) << b);
+      const uint32_t c01 = __reduce_add_sync(0xffffffffu, c[0] | c[1] << 16), c2 = __reduce_add_sync(0xffffffffu, c[2]);
+      uint2* out = s.counts[b >> 1 & 1];         // the other half is being read by slower warps
+      if ((tid & 31) == 0) out[tid >> 5] = make_uint2(c01, c2);
+      __syncthreads();
+      uint2 sum = out[0];
+      for (int i = 1; i < NW; ++i) { sum.x += out[i].x; sum.y += out[i].y; }
+      const int at = (int)sum.y >= r ? 3 : (int)(sum.x >> 16) >= r ? 2 : (int)(sum.x & 0xffffu) >= r ? 1 : 0;
+      t |= (u64)at << b;
+    }
+    return t;
+  }
+};
 
+// Where a CTA's part of a row lies: units of 16 bytes at 16-byte addresses, the first and last of
+// the row filled up with -inf.
+template <typename T>
+struct Span {
+  const T* p;
+  int vocab, off, u0, n;                         // the part's first unit of the row and its units
+  int lo, hi;                                    // whole units of the part: [lo, hi)
+  __device__ Span(const LogitsRows& x, const Team& t) {
+    p = reinterpret_cast<const T*>(x.data) + (long long)(blockIdx.x / t.size) * x.stride;
+    vocab = x.vocab;
+    off = (int)((uintptr_t)p & 15) / (int)sizeof(T);
+    const int units = (off + vocab + kUnit<T> - 1) / kUnit<T>, per = (units + (int)t.size - 1) / (int)t.size;
+    u0 = (int)t.rank * per;
+    n = max(0, min(units, u0 + per) - u0);
+    lo = n > 0 && col(0, 0) < 0 ? 1 : 0;
+    hi = n > lo && col(n, 0) > vocab ? n - 1 : n;
+  }
+  __device__ int col(int i, int v) const { return (u0 + i) * kUnit<T> - off + v; }
+  __device__ Unit<T> ragged(int i) const {
+    Unit<T> u;
+#pragma unroll
+    for (int v = 0; v < kUnit<T>; ++v) {
+      const int c = col(i, v);
+      u.v[v] = c >= 0 && c < vocab ? p[c] : from_f32<T>(-INFINITY);
+    }
+    return u;
+  }
+};
+
+// The k largest logits of a row.  Items are key << 32 | ~column: distinct, and larger
+// ones come first in the order.
+template <typename T>
+struct Listing {
+  static constexpr int NV = 4, G = kGroups / NT;            // units of a batch in column order; maxima of a thread
+  Team& t;
+  Span<T> span;
+  u64* list;                                     // [kList], with room for [kGroups] 16-bit numbers behind it
+  int k;
+  float bound;
+  u64 least;                                     // items not above it are no longer wanted
+
+  // Raises the bound to the k-th largest of the n >= k items listed, to 16 bits.
+  __device__ void raise(int n) {
+    const uint32_t key = (uint32_t)t.search(16, k, [&](u64 q) {
+      uint32_t c = 0;
+      for (int i = t.tid; i < n; i += NT) c += (uint32_t)(list[i] >> 48) >= (uint32_t)q;
+      return c;
+    });
+    bound = fmaxf(bound, key_logit(max(key << 16, kKeyLowest)));
+  }
+  // Leaves the k largest of n > k items.
+  __device__ void compress(int n) {
+    constexpr int N = kList / NT;
+    u64 item[N];
+#pragma unroll
+    for (int a = 0; a < N; ++a) item[a] = t.tid + a * NT < n ? list[t.tid + a * NT] : 0;
+    least = t.search(64, k, [&](u64 q) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int a = 0; a < N; ++a) c += item[a] >= q;
+      return c;
+    });
+    if (t.tid == 0) t.s.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int a = 0; a < N; ++a)
+      if (item[a] >= least) list[atomicAdd(&t.s.count, 1)] = item[a];
+    bound = fmaxf(bound, key_logit((uint32_t)(least >> 32)));
+    __syncthreads();
+  }
+  // Whole units only, so that the loads of a batch are in flight together; -inf past the end.
+  __device__ void load(Unit<T> (&x)[NV], int from) const {
+    const uint4* body = reinterpret_cast<const uint4*>(span.p + span.col(0, 0));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int u = from + i * NT + t.tid;
+      x[i].q = neg_inf_unit<T>();
+      if (u < span.hi) x[i].q = load_unit(body + u);
+    }
+  }
+  // Lists what is wanted of a batch whose unit i starts at column col(i).
+  template <int N, typename C>
+  __device__ void add(const Unit<T> (&x)[N], C col, int& mark) {
+    uint32_t done = 0;                           // elements of this thread that are listed
+    bool again;
+    do {
+      int top = -1;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (unit_max(x[i]) >= bound) {
+#pragma unroll
+          for (int v = 0; v < kUnit<T>; ++v) {
+            const float f = to_f32(x[i].v[v]);
+            if (f >= bound && !(done >> (i * kUnit<T> + v) & 1)) {
+              const u64 item = (u64)order_key(f + 0.0f) << 32 | (uint32_t)~(col(i) + v);
+              if (item > least) {
+                const int at = atomicAdd(&t.s.count, 1);
+                if (at < kList) {
+                  list[at] = item;
+                  done |= 1u << (i * kUnit<T> + v);
+                }
+                top = at;
+              }
+            }
+          }
+        }
+      again = false;
+      if (__syncthreads_or(top >= min(mark, kList))) {
+        const int n = t.s.count;
+        __syncthreads();
+        if (n > kList) {                         // some found no place: room for them, and again
+          compress(kList);
+          again = true;
+          mark = 2 * k;
+        } else {
+          raise(n);
+          mark = n + k;
+        }
+      }
+    } while (again);
+  }
+  // Column order.  Lists at least the k largest of this CTA's part, or all that are not masked; returns
+  // their number.
+  __device__ int collect() {
+    Unit<T> x[NV];
+    load(x, span.lo);
+    uint32_t high[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) high[i] = order_key(unit_max(x[i]) + 0.0f) >> 16;
+    const uint32_t key = (uint32_t)t.search(16, k, [&](u64 q) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) c += high[i] >= (uint32_t)q;
+      return c;
+    });
+    bound = key_logit(max(key << 16, kKeyLowest));
+    least = 0;
+    int mark = 2 * k;                            // raise the bound when this many are listed
+    if (t.tid == 0) t.s.count = 0;
+    __syncthreads();
+    for (int from = span.lo; from < span.hi; from += NT * NV) {
+      Unit<T> next[NV];
+      load(next, from + NT * NV);
+      add(x, [&](int i) { return span.col(from + i * NT + t.tid, 0); }, mark);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) x[i] = next[i];
+    }
+    if (span.lo > 0 || span.hi < span.n) {       // the row's ragged ends
+      Unit<T> end[1];
+      end[0].q = neg_inf_unit<T>();
+      const int at = t.tid == 0 && span.lo > 0 ? 0 : t.tid == 1 && span.hi < span.n ? span.hi : -1;
+      if (at >= 0) end[0] = span.ragged(at);
+      add(end, [&](int) { return span.col(at, 0); }, mark);
+    }
+    __syncthreads();
+    return t.s.count;
+  }
+  // Lists logits that are not below `bound` from unit i of the part (the list's length is not bounded by
+  // kList, what it holds is).
+  __device__ void pick(const Unit<T>& x, int i) {
+    if (!(unit_max(x) >= bound)) return;
+#pragma unroll
+    for (int v = 0; v < kUnit<T>; ++v) {
+      const float f = to_f32(x.v[v]);
+      if (f >= bound) {
+        const int at = atomicAdd(&t.s.count, 1);
+        if (at < kList) list[at] = (u64)order_key(f + 0.0f) << 32 | (uint32_t)~span.col(i, v);
+      }
+    }
+  }
+  // As collect, for the row's k largest, by the maxima of groups of units; the list may not hold them all.
+  __device__ int pick_groups() {
+    const uint4* body = reinterpret_cast<const uint4*>(span.p + span.col(0, 0));
+    Unit<T> top[G];
+#pragma unroll
+    for (int a = 0; a < G; ++a) top[a].q = neg_inf_unit<T>();
+#pragma unroll 1
+    for (int from = span.lo + t.tid; from < span.hi; from += NT * G) {
+      Unit<T> x[G];
+#pragma unroll
+      for (int a = 0; a < G; ++a) {
+        const int u = from + a * NT;
+        x[a].q = neg_inf_unit<T>();
+        if (u < span.hi) x[a].q = load_unit(body + u);
+      }
+#pragma unroll
+      for (int a = 0; a < G; ++a) fold_max(top[a], x[a]);
+    }
+    t.ready();
+    float high[G];
+    uint32_t key[G];
+#pragma unroll
+    for (int a = 0; a < G; ++a) {
+      high[a] = folded_max(top[a]);
+      key[a] = order_key(high[a] + 0.0f) >> 16;
+    }
+    if (t.tid == 0) { t.s.count = 0; t.s.groups = 0; }
+    const u64 mine = t.search(16, (k + (int)t.size - 1) / (int)t.size, [&](u64 q) {
+      uint32_t c = 0;
+#pragma unroll
+      for (int a = 0; a < G; ++a) c += key[a] >= (uint32_t)q;
+      return c;
+    });
+    uint32_t least_key = (uint32_t)mine;
+    if (t.size > 1) {
+      t.exchange(mine);
+      for (int r = 0; r < (int)t.size; ++r) least_key = min(least_key, (uint32_t)t.got(r));
+    }
+    bound = key_logit(max(least_key << 16, kKeyLowest));
+    // groups to be read again, half a warp each
+    uint16_t* groups = reinterpret_cast<uint16_t*>(list + kList);
+#pragma unroll
+    for (int a = 0; a < G; ++a)
+      if (high[a] >= bound) groups[atomicAdd(&t.s.groups, 1)] = (uint16_t)(t.tid * G + a);
+    __syncthreads();
+    const int n = t.s.groups, lane = t.tid & 15;
+    for (int i = t.tid >> 4; i < n; i += NT / 16) {
+      const int g = groups[i];
+      for (int u = span.lo + g / G + (g % G) * NT + lane * NT * G; u < span.hi; u += 16 * NT * G) {
+        Unit<T> x;
+        x.q = load_unit(body + u);
+        pick(x, u);
+      }
+    }
+    if (t.tid == 0 && span.lo > 0) pick(span.ragged(0), 0);
+    if (t.tid == 32 && span.hi < span.n) pick(span.ragged(span.hi), span.hi);
+    __syncthreads();
+    return t.s.count;
+  }
+  // The row's k largest (or more) in the list of CTA 0, largest first; returns their number, to CTA 0 alone.
+  __device__ int gather() {
+    int n = pick_groups(), total = n, at = 0;
+    const auto count = [&] {
+      if (t.size == 1) { total = n; return; }
+      t.exchange((u64)n);
+      total = at = 0;
+      for (int r = 0; r < (int)t.size; ++r) {
+        if (r < (int)t.rank) at += (int)t.got(r);
+        total += (int)t.got(r);
+      }
+    };
+    count();
+    if (total > kList) {
+      n = collect();
+      const int share = kList / (int)t.size;     // >= k
+      if (n > share) {
+        compress(n);
+        n = t.s.count;
+      }
+      count();
+    }
+    if (t.size > 1) {
+      if (t.rank != 0) {
+        const uint32_t to = remote_smem(list, 0);
+        for (int i = t.tid; i < n; i += NT) remote_store(to + 8u * (at + i), list[i]);
+      }
+      t.barrier();
+      if (t.rank != 0) return 0;
+    }
+    sort(total);
+    return total;
+  }
+  // list[0 .. n) by falling value (what follows up to a power of two is lost).
+  __device__ void sort(int n) {
+    int size = 1;
+    while (size < n) size <<= 1;
+    for (int i = n + t.tid; i < size; i += NT) list[i] = 0;
+    for (int len = 2; len <= size; len <<= 1)
+      for (int d = len >> 1; d; d >>= 1) {
+        __syncthreads();
+        for (int i = t.tid; i < size / 2; i += NT) {
+          const int a = 2 * i - (i & (d - 1)), b = a + d;
+          const u64 x = list[a], y = list[b];
+          if ((x < y) == ((a & len) == 0)) { list[a] = y; list[b] = x; }
+        }
+      }
+    __syncthreads();
+  }
+};
+
+// t = (x - m) c of a token, m the largest logit: its weight is rint(2^t 2^31).
+struct Exponent {
+  float m, c;
+  __device__ float operator()(float x) const { return __fmul_rn(x - m, c); }
+  __device__ float2 operator()(float2 x) const { return __fmul2_rn(__fadd2_rn(x, make_float2(-m, -m)), make_float2(c, c)); }
+};
+__device__ __forceinline__ uint32_t weight_of(float t) {
+  const float y = ex2(t);
+  // below 2^-8 the sum y + 2^-8 rounds y to a multiple of 2^-31, as rint does, and holds it in its low bits
+  if (t < -8.01f) return __float_as_uint(y + 0.00390625f) & 0x7fffffu;
+  return __float2uint_rn(y * 2147483648.0f);
+}
+
+// One CTA's part of a row in shared memory.
+template <typename T>
+struct Row : Team {
+  Span<T> d;
+  unsigned char* work;                           // histogram and members
+  Unit<T>* unit;
+  using Team::s; using Team::tid; using Team::rank; using Team::size;
+
+  __device__ Row(const Team& t, const Span<T>& d, unsigned char* dyn)
+      : Team(t), d(d), work(dyn), unit(reinterpret_cast<Unit<T>*>(dyn + kWorkBytes)) {
+    for (int i = tid; i < d.n; i += NT) {
+      if (i >= d.lo && i < d.hi) cp_async16(unit + i, d.p + d.col(i, 0));
+      else unit[i] = d.ragged(i);
+    }
+    cp_async_wait_all();                         // each thread's own units
+    ready();
+  }
+
+  // f(x, t, unit, element) over this thread's elements, t their exponents.
+  template <typename F>
+  __device__ void each(Exponent e, F f) const {
+    for (int i = tid; i < d.n; i += NT) {
+      Unit<T> u;
+      u.q = unit[i].q;
+#pragma unroll
+      for (int v = 0; v < kUnit<T>; v += 2) {
+        const float2 x = make_float2(to_f32(u.v[v]), to_f32(u.v[v + 1])), t = e(x);
+        f(x.x, t.x, i, v);
+        f(x.y, t.y, i, v + 1);
+      }
+    }
+  }
+  __device__ float own_max() const {
+    float m = -INFINITY;
+    for (int i = tid; i < d.n; i += NT) {
+      Unit<T> u;
+      u.q = unit[i].q;
+      m = fmaxf(m, unit_max(u));
+    }
+    return m;
+  }
   // Sums of w(x, col) over contiguous stretches, one a warp, in s.part; returns this CTA's total.
+  // w is 0 below `least`.
   template <typename W>
-  __device__ u64 stretch_sums(W w) {
+  __device__ u64 stretch_sums(W w, float least) {
     const int len = (d.n + NW - 1) / NW, i0 = (tid >> 5) * len, i1 = min(d.n, i0 + len);
     u64 sum = 0;
     for (int i = i0 + (tid & 31); i < i1; i += 32) {
       Unit<T> u;
-      u.q = d.unit[i].q;
+      u.q = unit[i].q;
+      if (!(unit_max(u) >= least)) continue;
 #pragma unroll
       for (int v = 0; v < kUnit<T>; ++v) sum += w(to_f32(u.v[v]), d.col(i, v));
     }
@@ -184,7 +506,7 @@ struct Row {
         Unit<T> u;
         u64 own = 0;
         if (i + lane < i1) {
-          u.q = d.unit[i + lane].q;
+          u.q = unit[i + lane].q;
 #pragma unroll
           for (int v = 0; v < kUnit<T>; ++v) own += w(to_f32(u.v[v]), d.col(i + lane, v));
         }
@@ -215,51 +537,7 @@ struct Row {
     return s.pick;
   }
 
-  // Lower bound of the k-th largest logit of the row (finite): at least k logits, or all that are
-  // not -inf, are not below it.
-  __device__ float bound(float own, int k) {
-    const uint32_t key = order_key(own + 0.0f) >> 16;
-    const int r = (k + (int)size - 1) / (int)size;
-    uint32_t t = 0;
-#pragma unroll 1
-    for (int bit = 15; bit >= 0; --bit)
-      if (__syncthreads_count(key >= (t | (1u << bit))) >= r) t |= 1u << bit;
-    exchange(t);
-    for (int i = 0; i < (int)size; ++i) t = min(t, (uint32_t)got(i));
-    return key_logit(max(t << 16, kKeyLowest));
-  }
-  // Logits from `least` up, as key << 32 | ~column, in the work area of CTA 0 (nothing is written if
-  // there are more than `most`); returns their number.
-  __device__ int gather(float own, float least, int most) {
-    if (tid == 0) s.count = 0;
-    __syncthreads();
-    int mine = 0, at = 0;
-    if (own >= least) {
-      each([&](float x, int, int) { mine += x >= least; });
-      at = atomicAdd(&s.count, mine);
-    }
-    __syncthreads();
-    exchange((u64)s.count);
-    int n = 0;
-    for (int r = 0; r < (int)size; ++r) {
-      if (r < (int)rank) at += (int)got(r);
-      n += (int)got(r);
-    }
-    if (n > most) return n;
-    if (own >= least) {
-      const uint32_t list = remote_smem(work, 0);
-      each([&](float x, int i, int v) {
-        if (x >= least) {
-          remote_store(list + 8u * at, (u64)order_key(x + 0.0f) << 32 | (uint32_t)~d.col(i, v));
-          ++at;
-        }
-      });
-    }
-    barrier();
-    return n;
-  }
-
-  // Scan of `total` (thread i < 256: weight of histogram entry i over the row, `mine` this CTA's) for the
+  // Scan of `total` (thread i: weight of histogram entry i over the row, `mine` this CTA's) for the
   // first entry at which the running weight reaches need(whole weight), starting from `above`; adds the
   // entries before it to `above` and `mine_above`.  Returns -1 if it is not reached.
   template <typename N>
@@ -272,63 +550,60 @@ struct Row {
       if (lane >= o) { run += a; own += b; }
     }
     __syncthreads();
-    if (lane == 31 && warp < kSteps / 32) { s.scan[warp] = run; s.part[warp] = own; }
+    if (lane == 31) { s.scan[warp] = run; s.part[warp] = own; }
     if (tid == 0) s.found = -1;
     __syncthreads();
     u64 whole = 0;
-    for (int i = 0; i < kSteps / 32; ++i) whole += s.scan[i];
+    for (int i = 0; i < NW; ++i) whole += s.scan[i];
     const u64 need = need_of(whole);
-    if (tid < kSteps) {
-      u64 before = above, mb = mine_above;
-      for (int i = 0; i < warp; ++i) { before += s.scan[i]; mb += s.part[i]; }
-      if (before + run >= need && before + run - total < need) {
-        s.found = tid;
-        s.found_above = before + run - total;
-        s.found_mine = mb + own - mine;
-      }
+    u64 before = above, mb = mine_above;
+    for (int i = 0; i < warp; ++i) { before += s.scan[i]; mb += s.part[i]; }
+    if (before + run >= need && before + run - total < need) {
+      s.found = tid;
+      s.found_above = before + run - total;
+      s.found_mine = mb + own - mine;
     }
     __syncthreads();
     if (s.found >= 0) { above = s.found_above; mine_above = s.found_mine; }
     return s.found;
   }
 
-  // The cut after the first tokens of the order whose weights w(x) reach need(whole weight), among
-  // elements with kept(x, col).  w depends on x alone and is below 2^31 + 1; m is the largest logit, c the
-  // scale of the steps.  False: the whole weight does not reach it.
+  // The cut after the first tokens of the order whose weights w(x, t) reach need(whole weight), among
+  // elements with kept(x, col).  t = (x - m) c is the exponent of y; w depends on it alone, is 0 where the
+  // token's weight is, and below 2^31 + 1.  False: the whole weight does not reach it.
   // kept_here: this CTA's share of the weight that is kept.
   template <typename K, typename W, typename N>
-  __device__ bool select(K kept, W w, float m, float c, N need_of, Cut& cut, u64& kept_here) {
+  __device__ bool select(K kept, W w, Exponent e, N need_of, Cut& cut, u64& kept_here) {
+    static_assert(kSteps == NT, "a thread per step");
     constexpr int SH = std::is_same<T, __half>::value ? 13 : std::is_same<T, __nv_bfloat16>::value ? 16 : 0;
+    constexpr uint32_t kLow = (1u << kLowBits) - 1;
     uint32_t* low = reinterpret_cast<uint32_t*>(work);
     uint32_t* high = low + kSteps * kCols;
     uint16_t* members = reinterpret_cast<uint16_t*>(high);
-    const auto step = [&](float x) {             // rint(-8 t), capped; NaN and -inf fall in the last
-      return min((uint32_t)(__float_as_uint(fmaf(fmaxf(__fmul_rn(x - m, c), -32.0f), -8.0f, 8388608.0f)) & 0x7fffffu),
-                 (uint32_t)(kSteps - 1));
-    };
+    const int lane = tid & (kCols - 1);
+    // 2^23 + the step, as a float: its bits are in order and end in the step
+    const auto step = [&](float t) { return __float_as_uint(fmaf(t, -kPerOctave, 8388608.0f)); };
+    constexpr uint32_t kStep0 = 0x4b000000u;
     __syncthreads();
     for (int i = tid; i < (kSteps + kHighSteps) * kCols; i += NT) low[i] = 0;
     __syncthreads();
-    each([&](float x, int i, int v) {
-      const uint32_t q = w(x);
+    each(e, [&](float x, float t, int i, int v) {
+      const uint32_t q = w(t);
       if (q && kept(x, d.col(i, v))) {
-        const uint32_t b = step(x) * kCols + (tid & (kCols - 1));
-        atomicAdd(low + b, q & ((1u << kLowBits) - 1));
+        const uint32_t b = (step(t) - kStep0) * kCols + lane;
+        atomicAdd(low + b, q & kLow);
         if (q >> kLowBits) atomicAdd(high + b, q >> kLowBits);
       }
     });
     __syncthreads();
     u64 mine = 0, total = 0;
-    if (tid < kSteps) {
-      for (int i = 0; i < kCols; ++i) {
-        mine += low[tid * kCols + i];
-        if (tid < kHighSteps) mine += (u64)high[tid * kCols + i] << kLowBits;
-      }
-      s.sums[tid] = mine;
+    for (int i = 0; i < kCols; ++i) {
+      mine += low[tid * kCols + i];
+      if (tid < kHighSteps) mine += (u64)high[tid * kCols + i] << kLowBits;
     }
+    s.sums[tid] = mine;
     barrier();
-    if (tid < kSteps)
-      for (int r = 0; r < (int)size; ++r) total += remote_load(remote_smem(&s.sums[tid], r));
+    for (int r = 0; r < (int)size; ++r) total += remote_load(remote_smem(&s.sums[tid], r));
     u64 above = 0, mine_above = 0, need = 0;
     const int at = crossing(total, mine, [&](u64 whole) { return need = need_of(whole); }, above, mine_above);
     if (at < 0) { barrier(); return false; }
@@ -336,10 +611,11 @@ struct Row {
     // the range of their keys
     if (tid == 0) { s.count = 0; s.key_low = 0xffffffffu; s.key_high = 0; }
     __syncthreads();
-    const auto member = [&](float x, int i, int v) { return step(x) == (uint32_t)at && w(x) && kept(x, d.col(i, v)); };
+    const uint32_t wanted_step = kStep0 + at;
+    const auto member = [&](float x, float t, int i, int v) { return step(t) == wanted_step && w(t) && kept(x, d.col(i, v)); };
     uint32_t lo = 0xffffffffu, hi = 0;
-    each([&](float x, int i, int v) {
-      if (member(x, i, v)) {
+    each(e, [&](float x, float t, int i, int v) {
+      if (member(x, t, i, v)) {
         const int k = atomicAdd(&s.count, 1);
         if (k < kMembers) members[k] = (uint16_t)(i * kUnit<T> + v);
         const uint32_t key = order_key(x + 0.0f) >> SH;
@@ -359,9 +635,9 @@ struct Row {
     }
     const auto each_member = [&](auto f) {
       if (listed <= kMembers) {
-        for (int k = tid; k < listed; k += NT) f(to_f32(d.unit[members[k] / kUnit<T>].v[members[k] % kUnit<T>]));
+        for (int k = tid; k < listed; k += NT) f(to_f32(unit[members[k] / kUnit<T>].v[members[k] % kUnit<T>]));
       } else {
-        each([&](float x, int i, int v) { if (member(x, i, v)) f(x); });
+        each(e, [&](float x, float t, int i, int v) { if (member(x, t, i, v)) f(x); });
       }
     };
     uint32_t key;
@@ -370,23 +646,22 @@ struct Row {
     for (;;) {
       int shift = 0;
       while (((hi - lo) >> shift) >= (uint32_t)kFine) ++shift;
-      uint32_t* flow = low;
-      uint32_t* fhigh = low + kFine * kFineCols;
+      uint32_t* upper = low + kFine * kCols;
       __syncthreads();
-      for (int i = tid; i < 2 * kFine * kFineCols; i += NT) low[i] = 0;
+      for (int i = tid; i < 2 * kFine * kCols; i += NT) low[i] = 0;
       barrier();                                 // and every CTA has read the sums of the round before
       each_member([&](float x) {
         const uint32_t k = order_key(x + 0.0f) >> SH;
         if (k < lo || k > hi) return;            // decided by an earlier round
-        const uint32_t b = ((hi - k) >> shift) * kFineCols + (tid & (kFineCols - 1)), q = w(x);
-        atomicAdd(flow + b, q & ((1u << kFineLowBits) - 1));
-        if (q >> kFineLowBits) atomicAdd(fhigh + b, q >> kFineLowBits);
+        const uint32_t b = ((hi - k) >> shift) * kCols + lane, q = w(e(x));
+        atomicAdd(low + b, q & kLow);
+        if (q >> kLowBits) atomicAdd(upper + b, q >> kLowBits);
       });
       __syncthreads();
       mine = total = 0;
       if (tid < kFine) {
-        for (int i = 0; i < kFineCols; ++i)
-          mine += flow[tid * kFineCols + i] + ((u64)fhigh[tid * kFineCols + i] << kFineLowBits);
+        for (int i = 0; i < kCols; ++i)
+          mine += low[tid * kCols + i] + ((u64)upper[tid * kCols + i] << kLowBits);
         s.sums[tid] = mine;
       }
       barrier();
@@ -405,7 +680,7 @@ struct Row {
     const u64 here = s.sums[entry];
     // the key of 16-bit types stands for one logit: its low bits are those of an exact value
     const float x = key_logit(SH == 0 ? key : (key << SH) | ((key << SH) & 0x80000000u ? 0u : (1u << SH) - 1u));
-    const u64 each_w = w(x), wanted = (need - above + each_w - 1) / each_w, earlier = key_before / each_w;
+    const u64 each_w = w(e(x)), wanted = (need - above + each_w - 1) / each_w, earlier = key_before / each_w;
     const u64 ties = here / each_w;
     cut.x = x;
     u64 taken = ties;
@@ -417,7 +692,7 @@ struct Row {
     } else {
       taken = wanted - earlier;
       const auto tie = [&](float v, int col) -> u64 { return v == x && kept(v, col) ? 1 : 0; };
-      stretch_sums(tie);
+      stretch_sums(tie, x);
       cut.last = locate(tie, taken - 1);
     }
     kept_here = mine_above + taken * each_w;
@@ -426,250 +701,151 @@ struct Row {
   }
 };
 
+__device__ __forceinline__ u64 draw(double u, u64 total) {
+  const long long t = (long long)(u * (double)total);
+  return t < 0 ? 0 : ((u64)t >= total ? total - 1 : (u64)t);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(NT, 2) sample_kernel(const SampleParams P) {
+__global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared s;
-  constexpr int kWork = (kSteps + kHighSteps) * kCols * 4;
-  Row<T> r(s, dyn, P.x, kWork);
-  const int row = blockIdx.x / r.size, tid = threadIdx.x;
+  Team team(s);
+  const Span<T> span(P.x, team);
+  const int row = blockIdx.x / team.size, tid = threadIdx.x;
   const float temperature = P.temperature ? P.temperature[row] : P.temperature_all;
-  const int top_k = P.top_k ? P.top_k[row] : P.top_k_all;
+  const bool greedy = !(temperature > 0.0f);
+  const int top_k = greedy ? 1 : P.top_k ? P.top_k[row] : P.top_k_all;
   const float top_p = P.top_p ? P.top_p[row] : P.top_p_all;
   const float min_p = fminf(P.min_p ? P.min_p[row] : P.min_p_all, 1.0f);
   const double u = P.uniform[row];
-  float own = r.own_max();
-  float m = r.row_max(own);
-  if (m == -INFINITY) {
+  Exponent e;
+  e.c = fminf(__fdiv_rn(kLog2e, temperature), 3.4028234e38f);  // finite: 0 c stays 0
+  // weight that top-p leaves of the whole: tokens with less than p z before them, the first always
+  const auto wanted = [&](u64 z) {
+    const double limit = (double)top_p * (double)z;
+    const u64 need = limit > 1.0 ? (u64)ceil(limit) : 1;
+    return top_p >= 1.0f || need > z ? z : need;
+  };
+
+  if (top_k > 0 && top_k <= kMaxListed) {
+    u64* list = reinterpret_cast<u64*>(dyn);
+    Listing<T> l{team, span, list, top_k};
+    const int n = min(top_k, l.gather());
+    if (team.rank != 0) return;
+    if (n <= 1 || greedy) {
+      if (tid == 0) P.tokens[row] = n ? (long long)~(uint32_t)list[0] : -1;
+      return;
+    }
+    static_assert(kMaxListed == NT, "a thread per listed token");
+    const u64 item = tid < n ? list[tid] : 0;
+    const float x = key_logit((uint32_t)(item >> 32));
+    e.m = key_logit((uint32_t)(list[0] >> 32));
+    const float t = x == e.m ? 0.0f : e(x);      // equal to m: also where that is infinite
+    const uint32_t w = tid < n ? weight_of(t) : 0;
+    u64 whole;
+    const u64 before = team.block_scan(w, whole);
+    const bool in = w && (tid == 0 || (before < wanted(whole) && ex2(t) >= min_p));
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    if (in) list[atomicAdd(&s.count, 1)] = item << 32 | w;     // by falling ~column: in index order
+    __syncthreads();
+    const int left = s.count;
+    l.sort(left);
+    const u64 mine = tid < left ? list[tid] : 0;
+    const u64 from = team.block_scan((uint32_t)mine, whole), target = draw(u, whole);
+    if (tid < left && target >= from && target < from + (uint32_t)mine) P.tokens[row] = (long long)~(uint32_t)(mine >> 32);
+    return;
+  }
+
+  Row<T> r(team, span, dyn);
+  e.m = r.row_max(r.own_max());
+  if (e.m == -INFINITY) {
     if (r.rank == 0 && tid == 0) P.tokens[row] = -1;
     return;
   }
-  if (m == INFINITY) {                           // infinite logits share all the weight
-    __syncthreads();
-    for (int i = tid; i < r.d.n; i += NT)
+  if (e.m == INFINITY) {                         // infinite logits share all the weight
+    for (int i = tid; i < span.n; i += NT)
 #pragma unroll
       for (int v = 0; v < kUnit<T>; ++v)
-        r.d.unit[i].v[v] = from_f32<T>(to_f32(r.d.unit[i].v[v]) == INFINITY ? 1.0f : -INFINITY);
+        r.unit[i].v[v] = from_f32<T>(to_f32(r.unit[i].v[v]) == INFINITY ? 1.0f : -INFINITY);
     __syncthreads();
-    m = 1.0f;
-    own = own == INFINITY ? 1.0f : -INFINITY;
+    e.m = 1.0f;
   }
-  const auto draw = [&](u64 total) {
-    const long long t = (long long)(u * (double)total);
-    return t < 0 ? 0 : ((u64)t >= total ? total - 1 : (u64)t);
-  };
-  // finds the CTA that holds `target` and the token in it; `mine`: this CTA's weight, in s.part if `summed`
-  const auto finish = [&](auto w, u64 mine, bool summed, bool greedy) {
-    __syncthreads();
-    r.exchange(mine);
-    u64 total = 0, before = 0;
-    for (int i = 0; i < (int)r.size; ++i) {
-      if (i < (int)r.rank) before += r.got(i);
-      total += r.got(i);
-    }
-    const u64 target = greedy ? 0 : draw(total);
-    if (target < before || target >= before + mine) return;
-    if (!summed) r.stretch_sums(w);
-    const int at = r.locate(w, target - before);
-    if (tid == 0) P.tokens[row] = at;
-  };
-  if (!(temperature > 0.0f)) {
-    const auto largest = [&](float x, int) -> u64 { return x == m; };
-    const u64 mine = r.stretch_sums(largest);
-    finish(largest, mine, true, true);
-    return;
-  }
-  const float c = fminf(__fdiv_rn(kLog2e, temperature), 3.4028234e38f);      // finite: 0 c stays 0
-  const auto power = [&](float x) { return x == m ? 1.0f : ex2(__fmul_rn(x - m, c)); };
-  const auto weight = [&](float x) { return __float2uint_rn(power(x) * 2147483648.0f); };
   Cut cut{-INFINITY, 0x7fffffff};
   const auto kept = [&](float x, int col) { return x > cut.x || (x == cut.x && col <= cut.last); };
+  const auto all = [](float, int) { return true; };
   bool known = false;                            // `mine` is this CTA's kept weight
   u64 mine = 0;
-  if (top_k > 0 && top_k < P.x.vocab) {
-    const int most = kListBytes / 8;
-    if (top_k <= most / 2) {
-      const float least = r.bound(own, top_k);
-      const int n = r.gather(own, least, most);
-      if (n <= most) {                           // all that is left is on CTA 0's list
-        if (r.rank != 0) return;
-        const u64* list = reinterpret_cast<const u64*>(r.work);
-        for (int i = tid; i < n; i += NT) s.weight[i] = weight(key_logit((uint32_t)(list[i] >> 32)));
-        __syncthreads();
-        constexpr int N = kListBytes / 8 / NT;
-        u64 item[N] = {}, before[N];
-        uint32_t w[N];
-        int place[N];
-        u64 z = 0;
-#pragma unroll
-        for (int a = 0; a < N; ++a) {
-          const int i = tid + a * NT;
-          before[a] = 0;
-          place[a] = top_k;
-          w[a] = 0;
-          if (i < n) {
-            item[a] = list[i];
-            int rank = 0;
-            u64 sum = 0;
-            for (int j = 0; j < n; ++j)
-              if (list[j] > item[a]) { ++rank; sum += s.weight[j]; }
-            place[a] = rank;
-            before[a] = sum;
-            w[a] = rank < top_k ? s.weight[i] : 0;
-            z += w[a];
-          }
-        }
-        z = r.block_sum(z);
-        const double limit = (double)top_p * (double)z;
-        u64 left = 0;
-#pragma unroll
-        for (int a = 0; a < N; ++a) {
-          const bool in = place[a] == 0 || ((top_p >= 1.0f || (double)before[a] < limit) &&
-                                            power(key_logit((uint32_t)(item[a] >> 32))) >= min_p);
-          if (!in) w[a] = 0;
-          if (tid + a * NT < n) s.weight[tid + a * NT] = w[a];
-          left += w[a];
-        }
-        left = r.block_sum(left);
-        const u64 target = draw(left);
-#pragma unroll
-        for (int a = 0; a < N; ++a)
-          if (w[a]) {
-            const uint32_t col = ~(uint32_t)item[a];
-            u64 sum = 0;
-            for (int j = 0; j < n; ++j)
-              if (~(uint32_t)list[j] < col) sum += s.weight[j];
-            if (target >= sum && target < sum + w[a]) P.tokens[row] = (long long)col;
-          }
-        return;
-      }
-    }
-    u64 ignored;
-    r.select([](float, int) { return true; }, [&](float x) { return weight(x) ? 1u : 0u; }, m, c,
-             [&](u64) { return (u64)top_k; }, cut, ignored);
-  }
+  const bool by_rank = top_k > 0 && top_k < P.x.vocab;
+  if (by_rank)
+    r.select(all, [](float t) { return weight_of(t) ? 1u : 0u; }, e, [&](u64) { return (u64)top_k; }, cut, mine);
   if (!(top_p >= 1.0f)) {
     Cut inner;
-    r.select(kept, weight, m, c, [&](u64 z) {
-      const double limit = (double)top_p * (double)z;          // kept: weight before it below this, the first always
-      const u64 need = limit > 1.0 ? (u64)ceil(limit) : 1;
-      return need > z ? z : need;
-    }, inner, mine);
-    if (inner.x != cut.x || inner.last < cut.last) cut = inner;
-    known = true;
+    if (by_rank) {
+      r.select(kept, weight_of, e, wanted, inner, mine);
+      if (inner.x != cut.x || inner.last < cut.last) cut = inner;
+    } else {
+      r.select(all, weight_of, e, wanted, cut, mine);
+    }
+    known = !(min_p > 0.0f);
   }
-  const auto left = [&](float x, int col) -> u64 { return kept(x, col) && power(x) >= min_p ? weight(x) : 0; };
-  if (!known || min_p > 0.0f) mine = r.stretch_sums(left);
-  finish(left, mine, !known || min_p > 0.0f, false);
+  const auto left = [&](float x, int col) -> u64 {
+    const float t = e(x);
+    return kept(x, col) && ex2(t) >= min_p ? weight_of(t) : 0;
+  };
+  // nothing below this passes min-p: a hundredth of an octave is far more than the rounding of t
+  const float least = fmaxf(cut.x, e.m + (log2f(min_p) - 0.01f) / e.c);
+  if (!known) mine = r.stretch_sums(left, least);
+  __syncthreads();
+  r.exchange(mine);
+  u64 total = 0, before = 0;
+  for (int i = 0; i < (int)r.size; ++i) {
+    if (i < (int)r.rank) before += r.got(i);
+    total += r.got(i);
+  }
+  const u64 target = draw(u, total);
+  if (target < before || target >= before + mine) return;      // the token is another CTA's
+  if (known) r.stretch_sums(left, least);
+  const int at = r.locate(left, target - before);
+  if (tid == 0) P.tokens[row] = at;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT, 2) top_kernel(const TopParams P, int most) {
-  extern __shared__ __align__(16) unsigned char dyn[];
+__global__ void __launch_bounds__(NT, 4) top_kernel(const TopParams P) {
   __shared__ Shared s;
-  Row<T> r(s, dyn, P.x, most * 8);
-  const int row = blockIdx.x / r.size, tid = threadIdx.x;
-  const T* p = reinterpret_cast<const T*>(P.x.data) + (long long)row * P.x.stride;
-  const float own = r.own_max();
-  int n = r.gather(own, r.bound(own, P.k), most);
-  if (n > most) {
-    // many equal logits, or k near the width: the k-th key by halving, counted over the cluster
-    u64 all = 0;
-    r.each([&](float x, int, int) { all += x > -INFINITY; });
-    all = r.block_sum(all);
-    __syncthreads();
-    r.exchange(all);
-    all = 0;
-    for (int i = 0; i < (int)r.size; ++i) all += r.got(i);
-    const int k = (int)min((u64)P.k, all);
-    uint32_t key = 0;
-    u64 above = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t t = key | (1u << bit);
-      u64 c = 0;
-      r.each([&](float x, int, int) { c += x > -INFINITY && order_key(x + 0.0f) >= t; });
-      c = r.block_sum(c);
-      __syncthreads();
-      r.exchange(c);
-      c = 0;
-      for (int i = 0; i < (int)r.size; ++i) c += r.got(i);
-      if (c >= (u64)k) key = t;
-      else above = c;                            // logits above the final key
-    }
-    const float x0 = key_logit(key);
-    const auto tie = [&](float x, int) -> u64 { return x == x0; };
-    const u64 ties = r.stretch_sums(tie);
-    __syncthreads();
-    r.exchange(ties);
-    u64 earlier = 0;
-    for (int i = 0; i < (int)r.rank; ++i) earlier += r.got(i);
-    const u64 wanted = k - above;
-    Cut cut{x0, 0x7fffffff};
-    if (wanted <= earlier) cut.last = -1;
-    else if (wanted < earlier + ties) cut.last = r.locate(tie, wanted - earlier - 1);
-    // as gather(), for what the cut keeps
-    const auto kept = [&](float x, int col) { return x > cut.x || (x == cut.x && col <= cut.last); };
-    if (tid == 0) s.count = 0;
-    __syncthreads();
-    int mine = 0, at;
-    r.each([&](float x, int i, int v) { mine += kept(x, r.d.col(i, v)); });
-    at = atomicAdd(&s.count, mine);
-    __syncthreads();
-    r.exchange((u64)s.count);
-    for (int i = 0; i < (int)r.rank; ++i) at += (int)r.got(i);
-    const uint32_t list = remote_smem(r.work, 0);
-    r.each([&](float x, int i, int v) {
-      if (kept(x, r.d.col(i, v))) {
-        remote_store(list + 8u * at, (u64)order_key(x + 0.0f) << 32 | (uint32_t)~r.d.col(i, v));
-        ++at;
-      }
-    });
-    r.barrier();
-    n = k;
-  }
-  if (r.rank != 0) return;
-  const u64* list = reinterpret_cast<const u64*>(r.work);
+  __shared__ u64 list[kListBytes / 8];
+  Team team(s);
+  const Span<T> span(P.x, team);
+  Listing<T> l{team, span, list, P.k};
+  const int n = l.gather(), row = blockIdx.x / team.size;
+  if (team.rank != 0) return;
   T* values = reinterpret_cast<T*>(P.values) + (long long)row * P.k;
   int* indices = P.indices + (long long)row * P.k;
-  for (int i = tid; i < n; i += NT) {
-    const u64 item = list[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += list[j] > item;
-    if (place < P.k) {
-      const int col = (int)~(uint32_t)item;
-      values[place] = p[col];
-      indices[place] = col;
-    }
-  }
-  for (int i = n + tid; i < P.k; i += NT) {
-    values[i] = from_f32<T>(-INFINITY);
-    indices[i] = -1;
+  for (int i = threadIdx.x; i < P.k; i += NT) {
+    const int col = i < n ? (int)~(uint32_t)list[i] : -1;
+    values[i] = col >= 0 ? span.p[col] : from_f32<T>(-INFINITY);
+    indices[i] = col;
   }
 }
 
-template <typename K, typename... A>
-int launch_clusters(K kernel, const LogitsRows& x, int work_bytes, cudaStream_t st, A... args) {
-  const int bytes = x.type == kLogitsF32 ? 4 : 2;
-  const int units = (x.vocab * bytes + 15) / 16 + 1;             // one more where the row starts inside a unit
-  // As many CTAs a row as keep its part within 64 KB; few rows take more, down to a unit a thread.
-  int size = 1;
-  while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
-  while (size < 8 && x.rows * size < 2 * 148 && units > size * NT) size *= 2;
-  const size_t smem = (size_t)work_bytes + (size_t)((units + size - 1) / size) * 16;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return launch_status();
+template <typename K, typename P>
+int launch_clusters(K kernel, const P& params, int size, size_t smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)x.rows * size);
+  cfg.gridDim = dim3((unsigned)params.x.rows * size);
   cfg.blockDim = dim3(NT);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, args...);
+  cudaLaunchKernelEx(&cfg, kernel, params);
   return launch_status();
 }
+// 16-byte units of a row, one more where it may start inside a unit.
+int row_units(const LogitsRows& x) { return (x.vocab * (x.type == kLogitsF32 ? 4 : 2) + 15) / 16 + 1; }
 
 template <typename F>
 int by_type(int type, F f) {
@@ -684,16 +860,29 @@ int by_type(int type, F f) {
 }  // namespace
 
 int launch_sample(const SampleParams& P, cudaStream_t st) {
+  // As many CTAs a row as keep its part within 64 KB, three on an SM; few rows take more, down to a
+  // unit a thread.
+  const int units = row_units(P.x);
+  int size = 1;
+  while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
+  while (size < 8 && P.x.rows * size < 2 * 148 && units > size * NT) size *= 2;
+  size_t smem = (size_t)kWorkBytes + (size_t)((units + size - 1) / size) * 16;
+  if (smem < kListBytes) smem = kListBytes;
   return by_type(P.x.type, [&](auto t) {
-    return launch_clusters(sample_kernel<decltype(t)>, P.x, (kSteps + kHighSteps) * kCols * 4, st, P);
+    const auto kernel = sample_kernel<decltype(t)>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess)
+      return launch_status();
+    return launch_clusters(kernel, P, size, smem, st);
   });
 }
 
 int launch_top_logits(const TopParams& P, cudaStream_t st) {
-  const int most = P.k <= 256 ? 1024 : 2048;
-  return by_type(P.x.type, [&](auto t) {
-    return launch_clusters(top_kernel<decltype(t)>, P.x, most * 8, st, P, most);
-  });
+  // One CTA lists the fewest logits; more where the rows do not fill the GPU, as long as
+  // their lists fit that of the first.
+  const int units = row_units(P.x);
+  int size = 1;
+  while (size < 8 && P.x.rows * size < 4 * 148 && units > size * 2 * NT && 2 * size * P.k <= kList) size *= 2;
+  return by_type(P.x.type, [&](auto t) { return launch_clusters(top_kernel<decltype(t)>, P, size, 0, st); });
 }
 
 }  // namespace sq

@@ -1,6 +1,7 @@
 // Device helpers shared by the kernels on rows of logits (logits.cu, distill.cu).
 #pragma once
 #include <cuda_bf16.h>
+#include <type_traits>
 #include "common.cuh"
 
 namespace sq {
@@ -45,20 +46,40 @@ template <typename T> union Unit {
 };
 __device__ __forceinline__ uint4 load_unit(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
-// Largest value of a unit; NaN is passed over (it shows up in the sum).
+template <typename T> __device__ __forceinline__ uint4 neg_inf_unit() {
+  const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  return make_uint4(w, w, w, w);
+}
+// Largest value of a unit, NaN passed over: -inf where there is nothing else.
 __device__ __forceinline__ float unit_max(const Unit<__half>& u) {
   const __half2* h = reinterpret_cast<const __half2*>(&u.q);
   const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(__low2float(m), __high2float(m));
+  return fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);
 }
 __device__ __forceinline__ float unit_max(const Unit<__nv_bfloat16>& u) {
   const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u.q);
   const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
-  return fmaxf(__low2float(m), __high2float(m));
+  return fmaxf(fmaxf(__low2float(m), __high2float(m)), -INFINITY);
 }
 __device__ __forceinline__ float unit_max(const Unit<float>& u) {
-  return fmaxf(fmaxf(u.v[0], u.v[1]), fmaxf(u.v[2], u.v[3]));
+  return fmaxf(fmaxf(fmaxf(u.v[0], u.v[1]), fmaxf(u.v[2], u.v[3])), -INFINITY);
 }
+
+// Running maximum of units, element by element or two by two; NaN is passed over.
+__device__ __forceinline__ void fold_max(Unit<__half>& top, const Unit<__half>& u) {
+  __half2* t = reinterpret_cast<__half2*>(&top.q);
+  const __half2* h = reinterpret_cast<const __half2*>(&u.q);
+  t[0] = __hmax2(t[0], __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+}
+__device__ __forceinline__ void fold_max(Unit<__nv_bfloat16>& top, const Unit<__nv_bfloat16>& u) {
+  __nv_bfloat162* t = reinterpret_cast<__nv_bfloat162*>(&top.q);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u.q);
+  t[0] = __hmax2(t[0], __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+}
+__device__ __forceinline__ void fold_max(Unit<float>& top, const Unit<float>& u) {
+  top.v[0] = fmaxf(top.v[0], fmaxf(fmaxf(u.v[0], u.v[1]), fmaxf(u.v[2], u.v[3])));
+}
+template <typename T> __device__ __forceinline__ float folded_max(const Unit<T>& top) { return unit_max(top); }
 
 // A row as whole 16-byte units between two ragged ends of fewer than a unit each: vectors need
 // 16-byte addresses, rows start where their stride puts them.
