@@ -9,12 +9,16 @@
 // a row without used entries has loss 0 and gradient 0.  Sums are fp32; p and the difference
 // p - q are fp32 and rounded once to the logits' type.
 //
-// loss_kernel: the forward.  The CTAs of a cluster stream their parts of the row with a running
-// maximum and sum per thread.
-// row_kernel: loss and gradient in one pass.  The CTAs of a cluster hold the row in registers:
-// every thread loads its units of 16 bytes at once, the record is worked through while they
-// travel, and the gradient is written from the registers.
-// In both each warp sends its (max, sum) to every CTA of the cluster through distributed shared
+// Powers are taken as 2^(s c - R) with one fused multiply-add, R = rint(m c): an integer near the
+// exponent of the largest term, so that changing from one R to another is exact and R itself brings no
+// rounding; p does not depend on it.
+//
+// loss_kernel: the forward.  The CTAs of a cluster stream their parts of the row with a running R and
+// sum per thread.
+// row_kernel: loss and gradient in one pass.  The CTAs of a cluster hold the row in shared memory:
+// asynchronous copies bring it while the record is worked through, and the gradient is computed from
+// there, so the logits are read from HBM once.
+// In both each warp sends its (R, sum) to every CTA of the cluster through distributed shared
 // memory, so a row costs one cluster barrier.
 // grad_kernel: the backward of a forward whose statistics were kept, streaming.
 #include "logits.cuh"
@@ -61,64 +65,98 @@ __device__ __forceinline__ bool used_entry(const DistillParams& P, int j, float 
 __device__ __forceinline__ float record_power(float v, float vmax, float c) { return v == vmax ? 0.0f : (v - vmax) * c; }
 
 
-// Sum of 2^((x - ref) c) over a unit.
-template <typename T>
-__device__ __forceinline__ float unit_power_sum(const Unit<T>& u, float ref, float c) {
-  float s = 0.f;
-#pragma unroll
-  for (int v = 0; v < kUnit<T>; ++v) s += ex2((to_f32(u.v[v]) - ref) * c);
-  return s;
+// x c - r for two.
+__device__ __forceinline__ float2 exponent2(float2 x, float c, float r) {
+  return __ffma2_rn(x, make_float2(c, c), make_float2(-r, -r));
 }
-// scale 2^((x - m) c) for a unit, written at column-unit u of `g`.
 template <typename T>
-__device__ __forceinline__ void store_gradient(T* g, int u, bool vec, const Unit<T>& x, float m, float c, float scale) {
+__device__ __forceinline__ float2 pair_of(const Unit<T>& u, int v) { return make_float2(to_f32(u.v[v]), to_f32(u.v[v + 1])); }
+
+// Adds the powers of a unit to two running sums.
+template <typename T>
+__device__ __forceinline__ void add_powers(float2& sum, const Unit<T>& u, float c, float r) {
+#pragma unroll
+  for (int v = 0; v < kUnit<T>; v += 2) {
+    const float2 t = exponent2(pair_of(u, v), c, r);
+    sum = __fadd2_rn(sum, make_float2(ex2(t.x), ex2(t.y)));
+  }
+}
+__device__ __forceinline__ void store_pair(Unit<__half>& o, int v, float2 p) {
+  reinterpret_cast<__half2*>(&o.q)[v / 2] = __float22half2_rn(p);
+}
+__device__ __forceinline__ void store_pair(Unit<__nv_bfloat16>& o, int v, float2 p) {
+  reinterpret_cast<__nv_bfloat162*>(&o.q)[v / 2] = __float22bfloat162_rn(p);
+}
+__device__ __forceinline__ void store_pair(Unit<float>& o, int v, float2 p) { o.v[v] = p.x; o.v[v + 1] = p.y; }
+// Copies n elements from shared memory to `to` in whole 16-byte units of the destination, its ends element
+// by element.
+template <typename T, int NT>
+__device__ void copy_out(T* to, int n, const T* from) {
+  const int head = min(n, (int)((16 - ((uintptr_t)to & 15)) & 15) / (int)sizeof(T)), units = (n - head) / kUnit<T>;
+  const uint32_t src = (uint32_t)__cvta_generic_to_shared(from + head);
+  for (int i = threadIdx.x; i < units; i += NT) {
+    const uint32_t a = src + 16u * i, word = a & ~3u;
+    uint32_t w[5];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[b]) : "r"(word + 4u * b));
+    if (sizeof(T) == 2 && (a & 2)) {
+      asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[4]) : "r"(word + 16u));
+#pragma unroll
+      for (int b = 0; b < 4; ++b) w[b] = __funnelshift_r(w[b], w[b + 1], 16);
+    }
+    reinterpret_cast<uint4*>(to + head)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  const int tail = head + units * kUnit<T>;
+  for (int i = threadIdx.x; i < head + n - tail; i += NT) {
+    const int j = i < head ? i : tail + (i - head);
+    to[j] = from[j];
+  }
+}
+// R of a maximum: 0 where that is -inf (powers of -inf are 0 and a NaN stays one).
+__device__ __forceinline__ float reference(float m, float c) { return m == -INFINITY ? 0.f : rintf(m * c); }
+// scale 2^(x c - r) for a unit; zeros where `any` is not set.
+template <typename T>
+__device__ __forceinline__ Unit<T> gradient(const Unit<T>& x, float c, float r, float scale, bool any) {
   Unit<T> o;
+  o.q = make_uint4(0, 0, 0, 0);
+  if (any) {
 #pragma unroll
-  for (int v = 0; v < kUnit<T>; ++v) o.v[v] = from_f32<T>(ex2((to_f32(x.v[v]) - m) * c) * scale);
-  if (vec) {
-    reinterpret_cast<uint4*>(g)[u] = o.q;
-  } else {
-#pragma unroll
-    for (int v = 0; v < kUnit<T>; ++v) g[u * kUnit<T> + v] = o.v[v];
+    for (int v = 0; v < kUnit<T>; v += 2) {
+      const float2 t = exponent2(pair_of(x, v), c, r);
+      const float2 p = __fmul2_rn(make_float2(ex2(t.x), ex2(t.y)), make_float2(scale, scale));
+      store_pair(o, v, p);
+    }
   }
-}
-template <typename T>
-__device__ __forceinline__ void zero_gradient(T* g, int u, bool vec) {
-  if (vec) {
-    reinterpret_cast<uint4*>(g)[u] = make_uint4(0, 0, 0, 0);
-  } else {
-#pragma unroll
-    for (int v = 0; v < kUnit<T>; ++v) g[u * kUnit<T> + v] = from_f32<T>(0.f);
-  }
+  return o;
 }
 
-// (max, sum) of every warp of the cluster.
+// (R, sum) of every warp of the cluster; R is -inf where the warp has nothing above -inf.
 template <int NW> struct Pairs { float2 p[8 * NW]; };
 
-// Each warp hands its pair to all CTAs; afterwards every thread has the row's.  `m` is the warp's
-// maximum and `sum` this thread's share relative to it (to 0 where m is -inf: powers of -inf
-// are 0 and a NaN stays one).  The caller has arrived at the cluster barrier once before.
+// Each warp hands its pair to all CTAs; afterwards every thread has the row's R and sum.  `m` is the warp's
+// maximum, `sum` this thread's share relative to its reference.  Every CTA of the cluster runs.
 template <int NW>
-__device__ void cluster_merge(float& m, float& sum, float c, Pairs<NW>& pairs, uint32_t rank, uint32_t size) {
+__device__ void cluster_merge(float m, float c, float& r, float& sum, Pairs<NW>& pairs, uint32_t rank, uint32_t size) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  cluster_wait();                                // every CTA of the cluster runs
-  if (lane < (int)size) remote_store(remote_smem(&pairs.p[rank * NW + warp], lane), m, sum);
+  if (lane < (int)size)
+    remote_store(remote_smem(&pairs.p[rank * NW + warp], lane), m == -INFINITY ? m : reference(m, c), sum);
   cluster_arrive();
   cluster_wait();
   const int n = (int)size * NW;
-  m = -INFINITY;
-  for (int i = lane; i < n; i += 32) m = fmaxf(m, pairs.p[i].x);
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += 32) top = fmaxf(top, pairs.p[i].x);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   sum = 0.f;
   for (int i = lane; i < n; i += 32) {
     const float2 p = pairs.p[i];
-    sum += p.x == m ? p.y : p.y * ex2((p.x - m) * c);
+    sum += p.x == top ? p.y : p.y * ex2(p.x - top);
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  r = top == -INFINITY ? 0.f : top;
 }
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -126,30 +164,38 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
-// One row's record: each thread holds entries tid, tid + NT, ...
-template <typename T, int NT>
+// One row's record of at most N NT entries: each thread holds entries tid, tid + NT, ...
+template <typename T, int NT, int N>
 struct Record {
-  static constexpr int N = kMaxRecord / NT;
   int at[N];                                     // -1: unused
   float e[N];                                    // (v - v_max) c
   float taken[N];                                // student's logit there
   float vmax, Q;
-  // Reads it all and, for entries with `wants(index)`, the student's logit.
-  template <typename W>
-  __device__ void load(const DistillParams& P, const T* s, long long base, float c, float (*part)[NT / 32], W wants) {
-    vmax = -INFINITY;
+  // Begins to read row `row`.
+  __device__ void fetch(const DistillParams& P, int row) {
+    const long long base = (long long)row * P.k;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int k = threadIdx.x + i * NT;
       at[i] = -1;
+      e[i] = -INFINITY;
       if (k < P.k) {
-        const int j = P.indices[base + k];
+        at[i] = P.indices[base + k];
         e[i] = record_value(P, base + k);
-        if (used_entry(P, j, e[i])) {
-          at[i] = j;
-          vmax = fmaxf(vmax, e[i]);
-          if (wants(j)) taken[i] = to_f32(s[j]);
-        }
+      }
+    }
+  }
+  // What fetch() read, and the student's logit at entries with wants(index).
+  template <typename W>
+  __device__ void prepare(const DistillParams& P, const T* s, float c, float (*part)[NT / 32], W wants) {
+    vmax = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!used_entry(P, at[i], e[i])) {
+        at[i] = -1;
+      } else {
+        vmax = fmaxf(vmax, e[i]);
+        if (wants(at[i])) taken[i] = to_f32(s[at[i]]);
       }
     }
     vmax = block_max<NT>(vmax, part[0]);
@@ -162,20 +208,20 @@ struct Record {
     Q = block_sum<NT>(q, part[1]);
   }
   // Loss of the row, known to thread 0 (every thread of the CTA calls, `taken` was wanted everywhere).
-  __device__ float loss(float m, float sum, float c, float temperature, float (*part)[NT / 32]) const {
+  __device__ float loss(float r, float sum, float c, float temperature, float (*part)[NT / 32]) const {
     float l = 0.f;
     const float rest = Q > 0.f ? log2f(sum) - log2f(Q) : 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float w = ex2(e[i]);
-      if (at[i] >= 0 && w > 0.f) l += w * (e[i] - (taken[i] - m) * c + rest);
+      if (at[i] >= 0 && w > 0.f) l += w * (e[i] - fmaf(taken[i], c, -r) + rest);
     }
     l = block_sum<NT>(l, part[0]);
     return Q > 0.f ? temperature * temperature * kLn2 * (l / Q) : 0.f;
   }
 };
 
-constexpr int kLossThreads = 256, kLossUnits = 4;
+constexpr int kLossThreads = 256, kLossUnits = 8;
 
 template <typename T>
 __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const DistillParams P) {
@@ -185,51 +231,62 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const DistillPara
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int row = blockIdx.x / size, tid = threadIdx.x;
   const float c = kLog2e / P.temperature;
-  const T* s = reinterpret_cast<const T*>(P.x.data) + (long long)row * P.x.stride;
-  const RowSpan<T> span(s, P.x.vocab);
-  const int per = (span.units + (int)size - 1) / (int)size;
-  const int u0 = (int)rank * per, u1 = min(span.units, u0 + per);
-  cluster_arrive();
-  const uint4* body = reinterpret_cast<const uint4*>(s + span.head);
-  const auto load = [&](Unit<T> (&x)[NV], int at) {
+  const Span<T> span(P.x, row, rank, size);
+  cluster_arrive_relaxed();
+  const uint4* body = reinterpret_cast<const uint4*>(span.p + span.col(0, 0));
+  const auto load = [&](Unit<T> (&x)[NV], int from) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int u = at + i * NT + tid;
-      x[i].q = u < u1 ? load_unit(body + u) : neg_inf_unit<T>();
+      const int u = from + i * NT + tid;
+      x[i].q = neg_inf_unit<T>();
+      if (u < span.hi) x[i].q = load_unit(body + u);
+    }
+  };
+  float m = -INFINITY, ref = 0.f;
+  float2 sum = make_float2(0.f, 0.f);
+  const auto raise = [&](float top) {
+    if (top > m) {
+      const float next = reference(top, c);
+      if (m != -INFINITY) sum = __fmul2_rn(sum, make_float2(ex2(ref - next), ex2(ref - next)));
+      m = top;
+      ref = next;
     }
   };
   Unit<T> x[NV];
-  load(x, u0);
-  float m = rank == 0 && tid < span.edges() ? to_f32(s[span.edge(tid)]) : -INFINITY;
-  float sum = m == -INFINITY ? 0.f : 1.f;
-  if (m != m) { sum = m; m = -INFINITY; }
-  Record<T, NT> rec;
-  if (rank == 0) rec.load(P, s, (long long)row * P.k, c, part, [](int) { return true; });
-  for (int at = u0; at < u1; at += NT * NV) {
-    Unit<T> next[NV];
-    load(next, at + NT * NV);
+  load(x, span.lo);
+  Record<T, NT, kMaxRecord / NT> rec;
+  if (rank == 0) {
+    rec.fetch(P, row);
+    rec.prepare(P, span.p, c, part, [](int) { return true; });
+  }
+#pragma unroll 1
+  for (int from = span.lo; from < span.hi; from += NT * NV) {
+    if (from != span.lo) load(x, from);
     float top = unit_max(x[0]);
 #pragma unroll
     for (int i = 1; i < NV; ++i) top = fmaxf(top, unit_max(x[i]));
-    if (top > m) {
-      sum *= ex2((m - top) * c);
-      m = top;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;
+    raise(top);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) sum += unit_power_sum(x[i], ref, c);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = next[i];
+    for (int i = 0; i < NV; ++i) add_powers(sum, x[i], c, ref);
   }
-  const float wm = warp_max(m);
-  if (m != wm) sum *= ex2((m - wm) * c);
-  m = wm;
-  cluster_merge<NW>(m, sum, c, pairs, rank, size);
+  if (tid < 2) {                                 // the row's ragged ends
+    const int at = tid == 0 ? (span.lo > 0 ? 0 : -1) : (span.hi < span.n ? span.hi : -1);
+    if (at >= 0) {
+      const Unit<T> end = span.ragged(at);
+      raise(unit_max(end));
+      add_powers(sum, end, c, ref);
+    }
+  }
+  const float wm = warp_max(m), wref = reference(wm, c);
+  float own = sum.x + sum.y, r;
+  if (m != -INFINITY && ref != wref) own *= ex2(ref - wref);
+  cluster_wait();                                // every CTA of the cluster runs
+  cluster_merge<NW>(wm, c, r, own, pairs, rank, size);
   if (rank != 0) return;
-  const float l = rec.loss(m, sum, c, P.temperature, part);
+  const float l = rec.loss(r, own, c, P.temperature, part);
   if (tid == 0) {
     P.loss[row] = l;
-    if (P.stats) P.stats[row] = make_float4(m, 1.0f / sum, rec.vmax, rec.Q > 0.f ? 1.0f / rec.Q : 0.f);
+    if (P.stats) P.stats[row] = make_float4(r, 1.0f / own, rec.vmax, rec.Q > 0.f ? 1.0f / rec.Q : 0.f);
   }
 }
 
@@ -251,111 +308,148 @@ __device__ __forceinline__ float sum_of_index(const int* at, const float* w, int
   return sum;
 }
 
-template <typename T, int NT, int NV>
-__global__ void __launch_bounds__(NT, 1024 / NT) row_kernel(const DistillParams P) {
+template <typename T, int NT, int N>
+__global__ void __launch_bounds__(NT, 768 / NT) row_kernel(const DistillParams P) {
   constexpr int NW = NT / 32;
-  __shared__ Pairs<NW> pairs;
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ Pairs<NW> pairs[2];                 // of this row and, from CTAs ahead, of the next
   __shared__ float part[2][NW];
-  __shared__ __align__(16) int at[kMaxRecord];
-  __shared__ float w[kMaxRecord];
   const uint32_t rank = cluster_rank(), size = cluster_size();
-  const int row = blockIdx.x / size, tid = threadIdx.x;
+  const int tid = threadIdx.x, step = gridDim.x / size;
   const float c = kLog2e / P.temperature;
-  const T* s = reinterpret_cast<const T*>(P.x.data) + (long long)row * P.x.stride;
-  const RowSpan<T> span(s, P.x.vocab);
-  const int per = (span.units + (int)size - 1) / (int)size;
-  const int u0 = (int)rank * per, u1 = min(span.units, u0 + per);
-  cluster_arrive();
+  const int k4 = (P.k + 3) & ~3;
+  int* at = reinterpret_cast<int*>(dyn);         // the record's indices (-1: unused) and 2^e
+  float* w = reinterpret_cast<float*>(at + k4);
+  // whole units, from that of column span.col(span.lo, 0); a thread brings and uses tid, tid + NT, ...
+  Unit<T>* unit = reinterpret_cast<Unit<T>*>(w + k4);
+  cluster_arrive_relaxed();
+  int row = blockIdx.x / size;
+  Span<T> span(P.x, row, rank, size);
+  for (int i = tid; i < span.hi - span.lo; i += NT) cp_async16(unit + i, span.p + span.col(span.lo + i, 0));
+  Record<T, NT, N> rec;
+  rec.fetch(P, row);
+  cluster_wait();                                // every CTA of the cluster runs
 
-  Unit<T> x[NV];
-  const uint4* body = reinterpret_cast<const uint4*>(s + span.head);
+  for (int turn = 0; row < P.x.rows; row += step, turn ^= 1) {
+    // the record: this CTA corrects the tokens in its own columns
+    const T* s = span.p;
+    const int units = span.hi - span.lo, first = span.col(span.lo, 0);
+    const int col0 = max(0, span.col(0, 0)), col1 = min(span.vocab, span.col(span.n, 0));
+    const auto mine = [&](int j) { return j >= col0 && j < col1; };
+    rec.prepare(P, s, c, part, [&](int j) { return rank == 0 || mine(j); });
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int u = u0 + i * NT + tid;
-    x[i].q = u < u1 ? load_unit(body + u) : neg_inf_unit<T>();
-  }
-  const bool has_edge = rank == 0 && tid < span.edges();
-  const int edge = has_edge ? span.edge(tid) : 0;
-  const float xe = has_edge ? to_f32(s[edge]) : -INFINITY;
-
-  // the record: this CTA corrects the tokens in its own columns, rank 0 those of the edges too
-  const auto mine = [&](int j) {
-    const int u = (j - span.head) / kUnit<T>;
-    return j < span.head || u >= span.units ? rank == 0 : u >= u0 && u < u1;
-  };
-  Record<T, NT> rec;
-  rec.load(P, s, (long long)row * P.k, c, part, [&](int j) { return rank == 0 || mine(j); });
-#pragma unroll
-  for (int i = 0; i < rec.N; ++i) {
-    at[tid + i * NT] = rec.at[i];
-    w[tid + i * NT] = ex2(rec.e[i]);
-  }
-  __syncthreads();
-  float token[rec.N];                            // sum of the token's q, or < 0: not for this thread
-#pragma unroll
-  for (int i = 0; i < rec.N; ++i)
-    token[i] = rec.at[i] >= 0 && mine(rec.at[i]) ? sum_of_index(at, w, P.k, tid + i * NT, rec.at[i]) : -1.f;
-
-  float m = xe;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) m = fmaxf(m, unit_max(x[i]));
-  m = warp_max(m);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float sum = has_edge ? ex2((xe - ref) * c) : 0.f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) sum += unit_power_sum(x[i], ref, c);
-  cluster_merge<NW>(m, sum, c, pairs, rank, size);
-
-  T* g = reinterpret_cast<T*>(P.grad) + (long long)row * P.grad_stride;
-  T* gb = g + span.head;
-  const bool vec = ((uintptr_t)gb & 15) == 0;
-  const bool any = rec.Q > 0.f;
-  const float f = P.temperature * (P.weight ? P.weight[row * P.weight_stride] : 1.0f), scale = f / sum;
-  if (has_edge) g[edge] = from_f32<T>(any ? ex2((xe - m) * c) * scale : 0.f);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int u = u0 + i * NT + tid;
-    if (u < u1) {
-      if (any) store_gradient(gb, u, vec, x[i], m, c, scale);
-      else zero_gradient(gb, u, vec);
+    for (int i = 0; i < N; ++i) {
+      const int k = tid + i * NT;
+      if (k < k4) { at[k] = rec.at[i]; w[k] = ex2(rec.e[i]); }
     }
-  }
-  if (rank == 0) {
-    const float l = rec.loss(m, sum, c, P.temperature, part);
-    if (tid == 0) P.loss[row] = l;
-  }
-  if (!any) return;
-  __syncthreads();
+    __syncthreads();
+    float token[N];                              // sum of the token's q, or < 0: not for this thread
 #pragma unroll
-  for (int i = 0; i < rec.N; ++i)
-    if (token[i] >= 0.f) g[rec.at[i]] = from_f32<T>(ex2((rec.taken[i] - m) * c) * scale - f * (token[i] / rec.Q));
+    for (int i = 0; i < N; ++i)
+      token[i] = rec.at[i] >= 0 && mine(rec.at[i]) ? sum_of_index(at, w, P.k, tid + i * NT, rec.at[i]) : -1.f;
+    // a ragged end of the row, held by one of two threads
+    const int end_unit = tid == 0 && span.lo > 0 ? 0 : tid == 1 && span.hi < span.n ? span.hi : -1;
+    Unit<T> end;
+    if (end_unit >= 0) end = span.ragged(end_unit);
+
+    cp_async_wait_all();
+    float m = end_unit >= 0 ? unit_max(end) : -INFINITY;
+#pragma unroll 4
+    for (int i = tid; i < units; i += NT) {
+      Unit<T> x;
+      x.q = unit[i].q;
+      m = fmaxf(m, unit_max(x));
+    }
+    m = warp_max(m);
+    const float ref = reference(m, c);
+    float2 sums = make_float2(0.f, 0.f);
+    if (end_unit >= 0) add_powers(sums, end, c, ref);
+#pragma unroll 4
+    for (int i = tid; i < units; i += NT) {
+      Unit<T> x;
+      x.q = unit[i].q;
+      add_powers(sums, x, c, ref);
+    }
+    float sum = sums.x + sums.y, r;
+    cluster_merge<NW>(m, c, r, sum, pairs[turn], rank, size);
+
+    T* g = reinterpret_cast<T*>(P.grad) + (long long)row * P.grad_stride;
+    const bool any = rec.Q > 0.f;
+    const float f = P.temperature * (P.weight ? P.weight[row * P.weight_stride] : 1.0f), scale = f / sum;
+    // the units of the next row follow into the places of this one's as these are done
+    const Span<T> next(P.x, min(row + step, P.x.rows - 1), rank, size);
+    const int fetched = row + step < P.x.rows ? next.hi - next.lo : 0;
+    const T* from = next.p + next.col(next.lo, 0);
+    T* to = g + first;
+    int i = tid;
+    if (((uintptr_t)to & 15) == 0) {
+#pragma unroll 2
+      for (; i < units; i += NT) {
+        Unit<T> x;
+        x.q = unit[i].q;
+        reinterpret_cast<uint4*>(to)[i] = gradient(x, c, r, scale, any).q;
+        if (i < fetched) cp_async16(unit + i, from + i * kUnit<T>);
+      }
+    } else {
+      // The gradient's rows lie otherwise in their 16 bytes than the logits' rows: it takes the logits'
+      // place in shared memory and is copied out from there in whole units of its own.
+      for (; i < units; i += NT) {
+        Unit<T> x;
+        x.q = unit[i].q;
+        unit[i].q = gradient(x, c, r, scale, any).q;
+      }
+      __syncthreads();
+      copy_out<T, NT>(to, units * kUnit<T>, reinterpret_cast<const T*>(unit));
+      __syncthreads();
+      i = tid;
+    }
+    for (; i < fetched; i += NT) cp_async16(unit + i, from + i * kUnit<T>);
+    if (end_unit >= 0) {
+      const Unit<T> o = gradient(end, c, r, scale, any);
+      for (int v = 0; v < kUnit<T>; ++v)
+        if (mine(span.col(end_unit, v))) g[span.col(end_unit, v)] = o.v[v];
+    }
+    if (rank == 0) {
+      const float l = rec.loss(r, sum, c, P.temperature, part);
+      if (tid == 0) P.loss[row] = l;
+    }
+    __syncthreads();
+    if (any) {
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+        if (token[n] >= 0.f) g[rec.at[n]] = from_f32<T>(ex2(fmaf(rec.taken[n], c, -r)) * scale - f * (token[n] / rec.Q));
+    }
+    if (fetched) rec.fetch(P, row + step);
+    span = next;
+  }
 }
 
-constexpr int kGradThreads = 256, kGradUnits = 4, kGradRounds = 4;   // a CTA of the backward writes 64 KB of a row
+constexpr int kGradThreads = 256, kGradUnits = 8, kGradRounds = 2;   // a CTA of the backward writes 64 KB of a row
 
 template <typename T>
-__global__ void __launch_bounds__(kGradThreads) grad_kernel(const DistillParams P, int parts) {
+__global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillParams P, int parts) {
   constexpr int NT = kGradThreads, NV = kGradUnits;
   __shared__ __align__(16) int at[kMaxRecord];
   __shared__ float w[kMaxRecord];
   const int row = blockIdx.x / parts, part = blockIdx.x - row * parts, tid = threadIdx.x;
   const float c = kLog2e / P.temperature;
-  const T* s = reinterpret_cast<const T*>(P.x.data) + (long long)row * P.x.stride;
+  const Span<T> span(P.x, row, part, parts);
+  const T* s = span.p;
   T* g = reinterpret_cast<T*>(P.grad) + (long long)row * P.grad_stride;
-  const RowSpan<T> span(s, P.x.vocab);
-  const int u0 = part * NT * NV * kGradRounds, u1 = min(span.units, u0 + NT * NV * kGradRounds);
-  const uint4* body = reinterpret_cast<const uint4*>(s + span.head);
+  const uint4* body = reinterpret_cast<const uint4*>(s + span.col(span.lo, 0));
+  T* to = g + span.col(span.lo, 0);
+  const int units = span.hi - span.lo;
   const auto load = [&](Unit<T> (&x)[NV], int from) {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = from + i * NT + tid;
-      if (u < u1) x[i].q = load_unit(body + u);
+      if (u < units) x[i].q = load_unit(body + u);
     }
   };
   Unit<T> x[NV];
-  load(x, u0);
+  load(x, 0);
   const float4 st = P.stats[row];
-  const float m = st.x, f = P.temperature * (P.weight ? P.weight[row * P.weight_stride] : 1.0f), scale = f * st.y;
+  const float r = st.x, f = P.temperature * (P.weight ? P.weight[row * P.weight_stride] : 1.0f), scale = f * st.y;
   const bool any = st.w > 0.f;
   const long long base = (long long)row * P.k;
   for (int k = tid; k < ((P.k + 3) & ~3); k += NT) {
@@ -365,78 +459,97 @@ __global__ void __launch_bounds__(kGradThreads) grad_kernel(const DistillParams 
     at[k] = used ? j : -1;
     w[k] = used ? ex2(record_power(v, st.z, c)) : 0.f;
   }
-  if (part == 0 && tid < span.edges()) {
-    const int e = span.edge(tid);
-    g[e] = from_f32<T>(any ? ex2((to_f32(s[e]) - m) * c) * scale : 0.f);
-  }
-  T* gb = g + span.head;
-  const bool vec = ((uintptr_t)gb & 15) == 0;
-  for (int from = u0; from < u1; from += NT * NV) {
-    Unit<T> next[NV];
-    load(next, from + NT * NV);
+  const bool vec = ((uintptr_t)to & 15) == 0;
+#pragma unroll 1
+  for (int from = 0; from < units; from += NT * NV) {
+    if (from) load(x, from);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int u = from + i * NT + tid;
-      if (u < u1) {
-        if (any) store_gradient(gb, u, vec, x[i], m, c, scale);
-        else zero_gradient(gb, u, vec);
+      if (u < units) {
+        const Unit<T> o = gradient(x[i], c, r, scale, any);
+        if (vec) {
+          reinterpret_cast<uint4*>(to)[u] = o.q;
+        } else {
+#pragma unroll
+          for (int v = 0; v < kUnit<T>; ++v) to[u * kUnit<T> + v] = o.v[v];
+        }
       }
     }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) x[i] = next[i];
+  }
+  const int col0 = max(0, span.col(0, 0)), col1 = min(span.vocab, span.col(span.n, 0));
+  if (tid < 2) {                                 // the row's ragged ends
+    const int u = tid == 0 ? (span.lo > 0 ? 0 : -1) : (span.hi < span.n ? span.hi : -1);
+    if (u >= 0) {
+      const Unit<T> o = gradient(span.ragged(u), c, r, scale, any);
+      for (int v = 0; v < kUnit<T>; ++v) {
+        const int j = span.col(u, v);
+        if (j >= col0 && j < col1) g[j] = o.v[v];
+      }
+    }
   }
   __syncthreads();
   if (!any) return;
   for (int k = tid; k < P.k; k += NT) {
     const int j = at[k];
-    if (j < 0) continue;
-    const int u = (j - span.head) / kUnit<T>;
-    if (j < span.head || u >= span.units ? part != 0 : u < u0 || u >= u1) continue;
+    if (j < col0 || j >= col1) continue;         // unused, or another CTA's
     const float q = sum_of_index(at, w, P.k, k, j);
-    if (q >= 0.f) g[j] = from_f32<T>(ex2((to_f32(s[j]) - m) * c) * scale - f * (q * st.w));
+    if (q >= 0.f) g[j] = from_f32<T>(ex2(fmaf(to_f32(s[j]), c, -r)) * scale - f * (q * st.w));
   }
 }
 
+// A cluster of `size` CTAs a row; as many as run at once for a kernel that steps through the rows.
 template <typename K>
-int launch_clusters(K kernel, const DistillParams& P, int size, int threads, cudaStream_t st) {
+int launch_clusters(K kernel, const DistillParams& P, bool steps, int size, int threads, size_t smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)P.x.rows * size);
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (steps && P.x.rows * size > 148) {
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) return launch_status();
+    if (clusters > 0 && clusters < P.x.rows) cfg.gridDim = dim3((unsigned)clusters * size);
+  }
   cudaLaunchKernelEx(&cfg, kernel, P);
   return launch_status();
 }
 
 template <typename T>
 int launch_loss(const DistillParams& P, cudaStream_t st) {
-  const int units = (P.x.vocab + kUnit<T> - 1) / kUnit<T>;
-  // more CTAs a row while the GPU is not many times full and each keeps some rounds of loads
+  // long parts stream best: more CTAs a row only until there are three for each SM
+  const int units = row_units(P.x);
   int size = 1;
-  while (size < 8 && P.x.rows * size < 16 * 148 && units > size * 2 * kLossThreads * kLossUnits) size *= 2;
-  return launch_clusters(loss_kernel<T>, P, size, kLossThreads, st);
+  while (size < 8 && P.x.rows * size < 3 * 148 && units > size * kLossThreads * kLossUnits) size *= 2;
+  return launch_clusters(loss_kernel<T>, P, false, size, kLossThreads, 0, st);
+}
+
+template <typename T, int NT, int N>
+int launch_rows(const DistillParams& P, int size, cudaStream_t st) {
+  const size_t smem = (size_t)((P.k + 3) & ~3) * 8 + (size_t)((row_units(P.x) + size - 1) / size) * 16;
+  const auto kernel = row_kernel<T, NT, N>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess)
+    return launch_status();
+  return launch_clusters(kernel, P, true, size, NT, smem, st);
 }
 
 template <typename T>
-int launch_rows(const DistillParams& P, cudaStream_t st) {
-  const int units = (P.x.vocab + kUnit<T> - 1) / kUnit<T>;
-  // CTAs of 512 threads hold 8 units a thread (64 KB of the row), as many as the row needs; few
-  // rows take more CTAs each until the GPU is full.  Rows over 512 KB
-  // (fp32 only) need 1024 threads.
+int launch_loss_grad(const DistillParams& P, cudaStream_t st) {
+  // As many CTAs a row as keep its part within 64 KB, three of 256 threads on an SM; few rows take more,
+  // down to a unit a thread.  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 512 threads.
+  const int units = row_units(P.x);
   int size = 1;
-  while (size < 8 && size * 512 * 8 < units) size *= 2;
-  while (size < 8 && P.x.rows * size < 2 * 148 && size * 512 < units) size *= 2;
-  const int per = (units + size * 512 - 1) / (size * 512);
-  if (per <= 1) return launch_clusters(row_kernel<T, 512, 1>, P, size, 512, st);
-  if (per <= 2) return launch_clusters(row_kernel<T, 512, 2>, P, size, 512, st);
-  if (per <= 4) return launch_clusters(row_kernel<T, 512, 4>, P, size, 512, st);
+  while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
+  while (size < 8 && P.x.rows * size < 2 * 148 && units > size * 256) size *= 2;
   if constexpr (sizeof(T) == 4)
-    if (per > 8) return launch_clusters(row_kernel<T, 1024, 8>, P, size, 1024, st);
-  return launch_clusters(row_kernel<T, 512, 8>, P, size, 512, st);
+    if ((units + size - 1) / size > 6144)
+      return P.k <= 512 ? launch_rows<T, 512, 1>(P, size, st) : launch_rows<T, 512, 2>(P, size, st);
+  return P.k <= 256 ? launch_rows<T, 256, 1>(P, size, st) : launch_rows<T, 256, 4>(P, size, st);
 }
 
 template <typename F>
@@ -455,13 +568,12 @@ int launch_distill_forward(const DistillParams& P, cudaStream_t st) {
   return by_type(P.x.type, [&](auto t) { return launch_loss<decltype(t)>(P, st); });
 }
 int launch_distill_loss_grad(const DistillParams& P, cudaStream_t st) {
-  return by_type(P.x.type, [&](auto t) { return launch_rows<decltype(t)>(P, st); });
+  return by_type(P.x.type, [&](auto t) { return launch_loss_grad<decltype(t)>(P, st); });
 }
 int launch_distill_backward(const DistillParams& P, cudaStream_t st) {
   return by_type(P.x.type, [&](auto t) {
     using T = decltype(t);
-    const int units = P.x.vocab / kUnit<T>, per = kGradThreads * kGradUnits * kGradRounds;
-    const int parts = units > per ? (units + per - 1) / per : 1;
+    const int per = kGradThreads * kGradUnits * kGradRounds, parts = (row_units(P.x) + per - 1) / per;
     grad_kernel<T><<<(unsigned)P.x.rows * parts, kGradThreads, 0, st>>>(P, parts);
     return launch_status();
   });

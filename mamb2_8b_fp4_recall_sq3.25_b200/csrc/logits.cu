@@ -74,7 +74,7 @@ struct Team {
   uint32_t rank, size;
   int tid, phase;
   __device__ explicit Team(Shared& s)
-      : s(s), rank(cluster_rank()), size(cluster_size()), tid(threadIdx.x), phase(0) { cluster_arrive(); }
+      : s(s), rank(cluster_rank()), size(cluster_size()), tid(threadIdx.x), phase(0) { cluster_arrive_relaxed(); }
   // before the first remote access: every CTA runs
   __device__ void ready() const { cluster_wait(); }
   __device__ void barrier() const { cluster_arrive(); cluster_wait(); }
@@ -135,35 +135,6 @@ struct Team {
       t |= (u64)at << b;
     }
     return t;
-  }
-};
-
-// Where a CTA's part of a row lies: units of 16 bytes at 16-byte addresses, the first and last of
-// the row filled up with -inf.
-template <typename T>
-struct Span {
-  const T* p;
-  int vocab, off, u0, n;                         // the part's first unit of the row and its units
-  int lo, hi;                                    // whole units of the part: [lo, hi)
-  __device__ Span(const LogitsRows& x, const Team& t) {
-    p = reinterpret_cast<const T*>(x.data) + (long long)(blockIdx.x / t.size) * x.stride;
-    vocab = x.vocab;
-    off = (int)((uintptr_t)p & 15) / (int)sizeof(T);
-    const int units = (off + vocab + kUnit<T> - 1) / kUnit<T>, per = (units + (int)t.size - 1) / (int)t.size;
-    u0 = (int)t.rank * per;
-    n = max(0, min(units, u0 + per) - u0);
-    lo = n > 0 && col(0, 0) < 0 ? 1 : 0;
-    hi = n > lo && col(n, 0) > vocab ? n - 1 : n;
-  }
-  __device__ int col(int i, int v) const { return (u0 + i) * kUnit<T> - off + v; }
-  __device__ Unit<T> ragged(int i) const {
-    Unit<T> u;
-#pragma unroll
-    for (int v = 0; v < kUnit<T>; ++v) {
-      const int c = col(i, v);
-      u.v[v] = c >= 0 && c < vocab ? p[c] : from_f32<T>(-INFINITY);
-    }
-    return u;
   }
 };
 
@@ -711,7 +682,7 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared s;
   Team team(s);
-  const Span<T> span(P.x, team);
+  const Span<T> span(P.x, blockIdx.x / team.size, team.rank, team.size);
   const int row = blockIdx.x / team.size, tid = threadIdx.x;
   const float temperature = P.temperature ? P.temperature[row] : P.temperature_all;
   const bool greedy = !(temperature > 0.0f);
@@ -816,7 +787,7 @@ __global__ void __launch_bounds__(NT, 4) top_kernel(const TopParams P) {
   __shared__ Shared s;
   __shared__ u64 list[kListBytes / 8];
   Team team(s);
-  const Span<T> span(P.x, team);
+  const Span<T> span(P.x, blockIdx.x / team.size, team.rank, team.size);
   Listing<T> l{team, span, list, P.k};
   const int n = l.gather(), row = blockIdx.x / team.size;
   if (team.rank != 0) return;
@@ -844,9 +815,6 @@ int launch_clusters(K kernel, const P& params, int size, size_t smem, cudaStream
   cudaLaunchKernelEx(&cfg, kernel, params);
   return launch_status();
 }
-// 16-byte units of a row, one more where it may start inside a unit.
-int row_units(const LogitsRows& x) { return (x.vocab * (x.type == kLogitsF32 ? 4 : 2) + 15) / 16 + 1; }
-
 template <typename F>
 int by_type(int type, F f) {
   switch (type) {

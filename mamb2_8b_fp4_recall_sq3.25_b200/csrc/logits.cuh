@@ -17,6 +17,9 @@ struct LogitsRows {
   int rows, vocab, type;
 };
 
+// 16-byte units of a row, one more where it may start inside a unit.
+inline int row_units(const LogitsRows& x) { return (x.vocab * (x.type == kLogitsF32 ? 4 : 2) + 15) / 16 + 1; }
+
 // Per-row settings of a draw; a null pointer means the one value for every row.
 struct SampleParams {
   LogitsRows x;
@@ -46,7 +49,7 @@ struct DistillParams {
   const float* weight;                    // factor of each row's gradient; null: 1
   long long weight_stride;                // 0: one factor for every row
   float* loss;                            // [rows]
-  float4* stats;                          // [rows] {m, 1 / S, v_max, 1 / Q (0: no record)}
+  float4* stats;                          // [rows] {R, 1 / S, v_max, 1 / Q (0: no record)}
   void* grad; long long grad_stride;      // the logits' type
 };
 int launch_distill_forward(const DistillParams& P, cudaStream_t st);   // loss, stats (optional)

@@ -3,6 +3,7 @@
 #include <cuda_bf16.h>
 #include <type_traits>
 #include "common.cuh"
+#include "logits.cuh"
 
 namespace sq {
 
@@ -81,24 +82,42 @@ __device__ __forceinline__ void fold_max(Unit<float>& top, const Unit<float>& u)
 }
 template <typename T> __device__ __forceinline__ float folded_max(const Unit<T>& top) { return unit_max(top); }
 
-// A row as whole 16-byte units between two ragged ends of fewer than a unit each: vectors need
-// 16-byte addresses, rows start where their stride puts them.
+// Where the part of a row that CTA `rank` of `size` works on lies: units of 16 bytes at 16-byte
+// addresses.  Rows start where their stride puts them: the first and the last unit of a row may be
+// ragged, and are filled up with -inf.
 template <typename T>
-struct RowSpan {
-  int head, units, tail;
-  __device__ RowSpan(const T* p, int n) {
-    head = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(T));
-    units = (n - head) / kUnit<T>;
-    tail = n - head - units * kUnit<T>;
+struct Span {
+  const T* p;
+  int vocab, off, u0, n;                         // the part's first unit of the row and its units
+  int lo, hi;                                    // whole units of the part: [lo, hi)
+  __device__ Span(const LogitsRows& x, int row, uint32_t rank, uint32_t size) {
+    p = reinterpret_cast<const T*>(x.data) + (long long)row * x.stride;
+    vocab = x.vocab;
+    off = (int)((uintptr_t)p & 15) / (int)sizeof(T);
+    const int units = (off + vocab + kUnit<T> - 1) / kUnit<T>, per = (units + (int)size - 1) / (int)size;
+    u0 = (int)rank * per;
+    n = max(0, min(units, u0 + per) - u0);
+    lo = n > 0 && col(0, 0) < 0 ? 1 : 0;
+    hi = n > lo && col(n, 0) > vocab ? n - 1 : n;
   }
-  __device__ int edges() const { return head + tail; }
-  __device__ int edge(int i) const { return i < head ? i : units * kUnit<T> + i; }   // column of edge element i
+  __device__ int col(int i, int v) const { return (u0 + i) * kUnit<T> - off + v; }
+  __device__ Unit<T> ragged(int i) const {
+    Unit<T> u;
+#pragma unroll
+    for (int v = 0; v < kUnit<T>; ++v) {
+      const int c = col(i, v);
+      u.v[v] = c >= 0 && c < vocab ? p[c] : from_f32<T>(-INFINITY);
+    }
+    return u;
+  }
 };
 
 // Cluster of the CTAs that share a row.
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ uint32_t cluster_size() { uint32_t r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+// Says that this CTA runs, without ordering memory.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 // Address of `p` (shared memory of this CTA) in the CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t remote_smem(const void* p, uint32_t rank) {
