@@ -9,16 +9,12 @@
 // a row without used entries has loss 0 and gradient 0.  Sums are fp32; p and the difference
 // p - q are fp32 and rounded once to the logits' type.
 //
-// Powers are taken as 2^(s c - R) with one fused multiply-add, R = rint(m c): an integer near the
-// exponent of the largest term, so that changing from one R to another is exact and R itself brings no
-// rounding; p does not depend on it.
-//
-// loss_kernel: the forward.  The CTAs of a cluster stream their parts of the row with a running R and
-// sum per thread.
+// loss_kernel: the forward.  The CTAs of a cluster stream their parts of the row with a running
+// maximum and sum per thread.
 // row_kernel: loss and gradient in one pass.  The CTAs of a cluster hold the row in shared memory:
 // asynchronous copies bring it while the record is worked through, and the gradient is computed from
 // there, so the logits are read from HBM once.
-// In both each warp sends its (R, sum) to every CTA of the cluster through distributed shared
+// In both each warp sends its (maximum, sum) to every CTA of the cluster through distributed shared
 // memory, so a row costs one cluster barrier.
 // grad_kernel: the backward of a forward whose statistics were kept, streaming.
 #include "logits.cuh"
@@ -65,9 +61,10 @@ __device__ __forceinline__ bool used_entry(const DistillParams& P, int j, float 
 __device__ __forceinline__ float record_power(float v, float vmax, float c) { return v == vmax ? 0.0f : (v - vmax) * c; }
 
 
-// x c - r for two.
+// (x - r) c for two: r is the largest logit, or 0 where there is none above -inf (powers of -inf are 0
+// then, and a NaN stays one).
 __device__ __forceinline__ float2 exponent2(float2 x, float c, float r) {
-  return __ffma2_rn(x, make_float2(c, c), make_float2(-r, -r));
+  return __fmul2_rn(__fadd2_rn(x, make_float2(-r, -r)), make_float2(c, c));
 }
 template <typename T>
 __device__ __forceinline__ float2 pair_of(const Unit<T>& u, int v) { return make_float2(to_f32(u.v[v]), to_f32(u.v[v + 1])); }
@@ -112,9 +109,8 @@ __device__ void copy_out(T* to, int n, const T* from) {
     to[j] = from[j];
   }
 }
-// R of a maximum: 0 where that is -inf (powers of -inf are 0 and a NaN stays one).
-__device__ __forceinline__ float reference(float m, float c) { return m == -INFINITY ? 0.f : rintf(m * c); }
-// scale 2^(x c - r) for a unit; zeros where `any` is not set.
+__device__ __forceinline__ float reference(float m) { return m == -INFINITY ? 0.f : m; }
+// scale 2^((x - r) c) for a unit; zeros where `any` is not set.
 template <typename T>
 __device__ __forceinline__ Unit<T> gradient(const Unit<T>& x, float c, float r, float scale, bool any) {
   Unit<T> o;
@@ -130,34 +126,39 @@ __device__ __forceinline__ Unit<T> gradient(const Unit<T>& x, float c, float r, 
   return o;
 }
 
-// (R, sum) of every warp of the cluster; R is -inf where the warp has nothing above -inf.
-template <int NW> struct Pairs { float2 p[8 * NW]; };
-
-// Each warp hands its pair to all CTAs; afterwards every thread has the row's R and sum.  `m` is the warp's
-// maximum, `sum` this thread's share relative to its reference.  Every CTA of the cluster runs.
-template <int NW>
-__device__ void cluster_merge(float m, float c, float& r, float& sum, Pairs<NW>& pairs, uint32_t rank, uint32_t size) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+__device__ __forceinline__ float warp_total(float v) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane < (int)size)
-    remote_store(remote_smem(&pairs.p[rank * NW + warp], lane), m == -INFINITY ? m : reference(m, c), sum);
-  cluster_arrive();
-  cluster_wait();
-  const int n = (int)size * NW;
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) top = fmaxf(top, pairs.p[i].x);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  sum = 0.f;
-  for (int i = lane; i < n; i += 32) {
-    const float2 p = pairs.p[i];
-    sum += p.x == top ? p.y : p.y * ex2(p.x - top);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  r = top == -INFINITY ? 0.f : top;
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
 }
+// Barrier of the warps that work on the row.
+template <int NT> __device__ __forceinline__ void data_barrier() { asm volatile("bar.sync 1, %0;" :: "n"(NT) : "memory"); }
+
+// (maximum, sum relative to its reference) of every warp of the cluster.
+template <int NW>
+struct Pairs {
+  float2 p[8 * NW];
+  // Hands a warp's maximum and the threads' shares of its sum to all CTAs of the cluster, which run; a
+  // cluster barrier has to follow.
+  __device__ void send(float m, float sum, uint32_t rank, uint32_t size) {
+    sum = warp_total(sum);
+    const int lane = threadIdx.x & 31;
+    if (lane < (int)size)
+      remote_store(remote_smem(&p[rank * NW + (threadIdx.x >> 5)], lane), m, sum);
+  }
+  // The row's reference and sum.
+  __device__ void merge(uint32_t size, float c, float& r, float& sum) const {
+    const int n = (int)size * NW;
+    float top = -INFINITY;
+    for (int i = threadIdx.x & 31; i < n; i += 32) top = fmaxf(top, p[i].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    sum = 0.f;
+    for (int i = threadIdx.x & 31; i < n; i += 32) sum += p[i].x == top ? p[i].y : p[i].y * ex2((p[i].x - top) * c);
+    sum = warp_total(sum);
+    r = reference(top);
+  }
+};
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -214,7 +215,7 @@ struct Record {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float w = ex2(e[i]);
-      if (at[i] >= 0 && w > 0.f) l += w * (e[i] - fmaf(taken[i], c, -r) + rest);
+      if (at[i] >= 0 && w > 0.f) l += w * (e[i] - (taken[i] - r) * c + rest);
     }
     l = block_sum<NT>(l, part[0]);
     return Q > 0.f ? temperature * temperature * kLn2 * (l / Q) : 0.f;
@@ -246,10 +247,9 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const DistillPara
   float2 sum = make_float2(0.f, 0.f);
   const auto raise = [&](float top) {
     if (top > m) {
-      const float next = reference(top, c);
-      if (m != -INFINITY) sum = __fmul2_rn(sum, make_float2(ex2(ref - next), ex2(ref - next)));
-      m = top;
-      ref = next;
+      const float f = m == -INFINITY ? 1.0f : ex2((m - top) * c);
+      sum = __fmul2_rn(sum, make_float2(f, f));
+      m = ref = top;
     }
   };
   Unit<T> x[NV];
@@ -277,11 +277,14 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const DistillPara
       add_powers(sum, end, c, ref);
     }
   }
-  const float wm = warp_max(m), wref = reference(wm, c);
+  const float wm = warp_max(m);
   float own = sum.x + sum.y, r;
-  if (m != -INFINITY && ref != wref) own *= ex2(ref - wref);
+  if (m != -INFINITY && m != wm) own *= ex2((m - wm) * c);
   cluster_wait();                                // every CTA of the cluster runs
-  cluster_merge<NW>(wm, c, r, own, pairs, rank, size);
+  pairs.send(wm, own, rank, size);
+  cluster_arrive();
+  cluster_wait();
+  pairs.merge(size, c, r, own);
   if (rank != 0) return;
   const float l = rec.loss(r, own, c, P.temperature, part);
   if (tid == 0) {
@@ -291,97 +294,201 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const DistillPara
 }
 
 // The record's tokens in the gradient: each by its first entry, repeated indices added up.
-// at, w: the row's indices (-1: unused, and up to a multiple of four) and 2^e in shared memory.
-// Returns the sum of 2^e over the entries of index j if entry k is the first of them, else -1.
-__device__ __forceinline__ float sum_of_index(const int* at, const float* w, int n, int k, int j) {
+// at: the row's indices (-1: unused, and up to a multiple of four) in shared memory; q(i): entry i's 2^e.
+// Returns the sum of q over the entries of index j if entry k is the first of them, else -1.
+template <typename F>
+__device__ __forceinline__ float sum_of_index(const int* at, int n, int k, int j, F q) {
   float sum = 0.f;
   for (int b = 0; b < n; b += 4) {
     const int4 a = *reinterpret_cast<const int4*>(at + b);
+    if (a.x != j && a.y != j && a.z != j && a.w != j) continue;
     const int same[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
     for (int o = 0; o < 4; ++o)
       if (same[o] == j) {
         if (b + o < k) return -1.f;
-        sum += w[b + o];
+        sum += q(b + o);
       }
   }
   return sum;
 }
 
-template <typename T, int NT, int N>
-__global__ void __launch_bounds__(NT, 768 / NT) row_kernel(const DistillParams P) {
-  constexpr int NW = NT / 32;
+// The record warp's side of row_kernel: one row's record in shared memory, lane l works on entries l, l + 32, ...
+template <typename T>
+struct RowRecord {
+  int* at;                                       // index (-1: unused, and up to a multiple of four)
+  float *e, *taken, *token;                      // (v - v_max) c; student's logit; sum of 2^e over the index, or < 0
+  float Q;
+  static __device__ __host__ size_t bytes(int k4) { return (size_t)k4 * 16; }
+  __device__ RowRecord(unsigned char* p, int k4) {
+    at = reinterpret_cast<int*>(p);
+    e = reinterpret_cast<float*>(at + k4);
+    taken = e + k4;
+    token = taken + k4;
+  }
+  // Columns [col0, col1) are this CTA's to correct; CTA 0 needs the student's logit everywhere.
+  __device__ void prepare(const DistillParams& P, int row, const T* s, float c, bool all, int col0, int col1) {
+    const int lane = threadIdx.x & 31, k4 = (P.k + 3) & ~3;
+    const long long base = (long long)row * P.k;
+    float vmax = -INFINITY, q = 0.f;
+    for (int k = lane; k < k4; k += 32) {
+      int j = -1;
+      float v = -INFINITY;
+      if (k < P.k) {
+        j = P.indices[base + k];
+        v = record_value(P, base + k);
+        if (!used_entry(P, j, v)) j = -1;
+        else vmax = fmaxf(vmax, v);
+      }
+      at[k] = j;
+      e[k] = v;
+      const bool mine = j >= col0 && j < col1;
+      token[k] = mine ? 0.f : -1.f;
+      if (j >= 0 && (all || mine)) taken[k] = to_f32(s[j]);
+    }
+    vmax = warp_max(vmax);
+    for (int k = lane; k < k4; k += 32) {
+      const float p = at[k] < 0 ? -INFINITY : record_power(e[k], vmax, c);
+      e[k] = p;
+      q += ex2(p);
+    }
+    Q = warp_total(q);
+    __syncwarp();
+    for (int k = lane; k < P.k; k += 32)
+      if (token[k] == 0.f) token[k] = sum_of_index(at, P.k, k, at[k], [&](int i) { return ex2(e[i]); });
+    __syncwarp();
+  }
+  __device__ float loss(int n, float r, float sum, float c, float temperature) const {
+    float l = 0.f;
+    if (!(Q > 0.f)) return 0.f;
+    const float rest = log2f(sum) - log2f(Q);
+    for (int k = threadIdx.x & 31; k < n; k += 32) {
+      const float w = ex2(e[k]);
+      if (at[k] >= 0 && w > 0.f) l += w * (e[k] - (taken[k] - r) * c + rest);
+    }
+    return temperature * temperature * kLn2 * (warp_total(l) / Q);
+  }
+  // The gradient at the record's tokens, over what the data warps wrote there.
+  __device__ void correct(int n, T* g, float r, float c, float scale, float f) const {
+    if (!(Q > 0.f)) return;
+    const float fq = f / Q;
+    for (int k = threadIdx.x & 31; k < n; k += 32)
+      if (token[k] >= 0.f) g[at[k]] = from_f32<T>(ex2((taken[k] - r) * c) * scale - fq * token[k]);
+  }
+};
+
+// DW warps work on the row, one more on the record: it prepares the next row's while they compute this
+// one's gradient, and corrects the gradient of a row after the next row's barrier.
+template <typename T, int DW>
+__global__ void __launch_bounds__(DW * 32 + 32, 24 / DW) row_kernel(const DistillParams P) {
+  constexpr int NT = DW * 32;
   extern __shared__ __align__(16) unsigned char dyn[];
-  __shared__ Pairs<NW> pairs[2];                 // of this row and, from CTAs ahead, of the next
-  __shared__ float part[2][NW];
+  __shared__ Pairs<DW> pairs[2];                 // of this row and, from CTAs ahead, of the next
+  __shared__ int has_record[2];
   const uint32_t rank = cluster_rank(), size = cluster_size();
-  const int tid = threadIdx.x, step = gridDim.x / size;
+  const int tid = threadIdx.x, step = gridDim.x / size, k4 = (P.k + 3) & ~3;
   const float c = kLog2e / P.temperature;
-  const int k4 = (P.k + 3) & ~3;
-  int* at = reinterpret_cast<int*>(dyn);         // the record's indices (-1: unused) and 2^e
-  float* w = reinterpret_cast<float*>(at + k4);
-  // whole units, from that of column span.col(span.lo, 0); a thread brings and uses tid, tid + NT, ...
-  Unit<T>* unit = reinterpret_cast<Unit<T>*>(w + k4);
   cluster_arrive_relaxed();
   int row = blockIdx.x / size;
   Span<T> span(P.x, row, rank, size);
+  const auto first_col = [](const Span<T>& s) { return max(0, s.col(0, 0)); };
+  const auto last_col = [](const Span<T>& s) { return min(s.vocab, s.col(s.n, 0)); };
+  const auto weight = [&](int row) { return P.temperature * (P.weight ? P.weight[row * P.weight_stride] : 1.0f); };
+
+  if (tid >= NT) {
+    RowRecord<T> now(dyn, k4), before(dyn + RowRecord<T>::bytes(k4), k4);
+    T* g_before = nullptr;
+    float r_before = 0.f, scale_before = 0.f, f_before = 0.f;
+    now.prepare(P, row, span.p, c, rank == 0, first_col(span), last_col(span));
+    if (tid == NT) has_record[0] = now.Q > 0.f;
+    cluster_wait();                              // every CTA of the cluster runs
+    for (int turn = 0; row < P.x.rows; row += step) {
+      float r, sum;
+      const float f = weight(row);
+      cluster_arrive();
+      cluster_wait();
+      pairs[turn].merge(size, c, r, sum);
+      turn ^= 1;
+      if (g_before) before.correct(P.k, g_before, r_before, c, scale_before, f_before);
+      if (rank == 0) {
+        const float l = now.loss(P.k, r, sum, c, P.temperature);
+        if (tid == NT) P.loss[row] = l;
+      }
+      g_before = reinterpret_cast<T*>(P.grad) + (long long)row * P.grad_stride;
+      r_before = r; scale_before = f / sum; f_before = f;
+      const RowRecord<T> swap = before;
+      before = now;
+      now = swap;
+      if (row + step < P.x.rows) {
+        const Span<T> next(P.x, row + step, rank, size);
+        __syncwarp();
+        now.prepare(P, row + step, next.p, c, rank == 0, first_col(next), last_col(next));
+        if (tid == NT) has_record[turn] = now.Q > 0.f;
+      }
+    }
+    __syncthreads();
+    before.correct(P.k, g_before, r_before, c, scale_before, f_before);
+    return;
+  }
+
+  // whole units, from that of column span.col(span.lo, 0); a thread brings and uses tid, tid + NT, ...
+  Unit<T>* unit = reinterpret_cast<Unit<T>*>(dyn + 2 * RowRecord<T>::bytes(k4));
   for (int i = tid; i < span.hi - span.lo; i += NT) cp_async16(unit + i, span.p + span.col(span.lo + i, 0));
-  Record<T, NT, N> rec;
-  rec.fetch(P, row);
+  // a ragged end of the row, held by one of two threads
+  const auto end_of = [&](const Span<T>& s) { return tid == 0 && s.lo > 0 ? 0 : tid == 1 && s.hi < s.n ? s.hi : -1; };
+  int end_unit = end_of(span);
+  Unit<T> end;
+  end.q = neg_inf_unit<T>();
+  if (end_unit >= 0) end = span.ragged(end_unit);
   cluster_wait();                                // every CTA of the cluster runs
 
   for (int turn = 0; row < P.x.rows; row += step, turn ^= 1) {
-    // the record: this CTA corrects the tokens in its own columns
-    const T* s = span.p;
-    const int units = span.hi - span.lo, first = span.col(span.lo, 0);
-    const int col0 = max(0, span.col(0, 0)), col1 = min(span.vocab, span.col(span.n, 0));
-    const auto mine = [&](int j) { return j >= col0 && j < col1; };
-    rec.prepare(P, s, c, part, [&](int j) { return rank == 0 || mine(j); });
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int k = tid + i * NT;
-      if (k < k4) { at[k] = rec.at[i]; w[k] = ex2(rec.e[i]); }
-    }
-    __syncthreads();
-    float token[N];                              // sum of the token's q, or < 0: not for this thread
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      token[i] = rec.at[i] >= 0 && mine(rec.at[i]) ? sum_of_index(at, w, P.k, tid + i * NT, rec.at[i]) : -1.f;
-    // a ragged end of the row, held by one of two threads
-    const int end_unit = tid == 0 && span.lo > 0 ? 0 : tid == 1 && span.hi < span.n ? span.hi : -1;
-    Unit<T> end;
-    if (end_unit >= 0) end = span.ragged(end_unit);
-
+    const int units = span.hi - span.lo;
+    const float f = weight(row);
     cp_async_wait_all();
-    float m = end_unit >= 0 ? unit_max(end) : -INFINITY;
-#pragma unroll 4
-    for (int i = tid; i < units; i += NT) {
-      Unit<T> x;
-      x.q = unit[i].q;
-      m = fmaxf(m, unit_max(x));
-    }
-    m = warp_max(m);
-    const float ref = reference(m, c);
+    float m = unit_max(end), ref = reference(m);
     float2 sums = make_float2(0.f, 0.f);
-    if (end_unit >= 0) add_powers(sums, end, c, ref);
-#pragma unroll 4
-    for (int i = tid; i < units; i += NT) {
+    add_powers(sums, end, c, ref);
+    const auto raise = [&](float top) {
+      if (top > m) {
+        const float f = m == -INFINITY ? 1.0f : ex2((m - top) * c);
+        sums = __fmul2_rn(sums, make_float2(f, f));
+        m = ref = top;
+      }
+    };
+    int i = tid;
+    for (; i + 3 * NT < units; i += 4 * NT) {
+      Unit<T> x[4];
+#pragma unroll
+      for (int a = 0; a < 4; ++a) x[a].q = unit[i + a * NT].q;
+      raise(fmaxf(fmaxf(unit_max(x[0]), unit_max(x[1])), fmaxf(unit_max(x[2]), unit_max(x[3]))));
+#pragma unroll
+      for (int a = 0; a < 4; ++a) add_powers(sums, x[a], c, ref);
+    }
+    for (; i < units; i += NT) {
       Unit<T> x;
       x.q = unit[i].q;
+      raise(unit_max(x));
       add_powers(sums, x, c, ref);
     }
     float sum = sums.x + sums.y, r;
-    cluster_merge<NW>(m, c, r, sum, pairs[turn], rank, size);
+    const float wm = warp_max(m);
+    if (m != -INFINITY && m != wm) sum *= ex2((m - wm) * c);
+    pairs[turn].send(wm, sum, rank, size);
+    cluster_arrive();
+    cluster_wait();
+    pairs[turn].merge(size, c, r, sum);
 
     T* g = reinterpret_cast<T*>(P.grad) + (long long)row * P.grad_stride;
-    const bool any = rec.Q > 0.f;
-    const float f = P.temperature * (P.weight ? P.weight[row * P.weight_stride] : 1.0f), scale = f / sum;
+    const bool any = has_record[turn];
+    const float scale = f / sum;
     // the units of the next row follow into the places of this one's as these are done
-    const Span<T> next(P.x, min(row + step, P.x.rows - 1), rank, size);
-    const int fetched = row + step < P.x.rows ? next.hi - next.lo : 0;
+    const bool more = row + step < P.x.rows;
+    const Span<T> next(P.x, more ? row + step : row, rank, size);
+    const int fetched = more ? next.hi - next.lo : 0;
     const T* from = next.p + next.col(next.lo, 0);
-    T* to = g + first;
-    int i = tid;
+    T* to = g + span.col(span.lo, 0);
+    i = tid;
     if (((uintptr_t)to & 15) == 0) {
 #pragma unroll 2
       for (; i < units; i += NT) {
@@ -398,30 +505,25 @@ __global__ void __launch_bounds__(NT, 768 / NT) row_kernel(const DistillParams P
         x.q = unit[i].q;
         unit[i].q = gradient(x, c, r, scale, any).q;
       }
-      __syncthreads();
+      data_barrier<NT>();
       copy_out<T, NT>(to, units * kUnit<T>, reinterpret_cast<const T*>(unit));
-      __syncthreads();
+      data_barrier<NT>();
       i = tid;
     }
     for (; i < fetched; i += NT) cp_async16(unit + i, from + i * kUnit<T>);
     if (end_unit >= 0) {
       const Unit<T> o = gradient(end, c, r, scale, any);
-      for (int v = 0; v < kUnit<T>; ++v)
-        if (mine(span.col(end_unit, v))) g[span.col(end_unit, v)] = o.v[v];
+      for (int v = 0; v < kUnit<T>; ++v) {
+        const int j = span.col(end_unit, v);
+        if (j >= 0 && j < span.vocab) g[j] = o.v[v];
+      }
     }
-    if (rank == 0) {
-      const float l = rec.loss(r, sum, c, P.temperature, part);
-      if (tid == 0) P.loss[row] = l;
-    }
-    __syncthreads();
-    if (any) {
-#pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (token[n] >= 0.f) g[rec.at[n]] = from_f32<T>(ex2(fmaf(rec.taken[n], c, -r)) * scale - f * (token[n] / rec.Q));
-    }
-    if (fetched) rec.fetch(P, row + step);
     span = next;
+    end_unit = end_of(span);
+    end.q = neg_inf_unit<T>();
+    if (more && end_unit >= 0) end = span.ragged(end_unit);
   }
+  __syncthreads();
 }
 
 constexpr int kGradThreads = 256, kGradUnits = 8, kGradRounds = 2;   // a CTA of the backward writes 64 KB of a row
@@ -493,8 +595,8 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillPara
   for (int k = tid; k < P.k; k += NT) {
     const int j = at[k];
     if (j < col0 || j >= col1) continue;         // unused, or another CTA's
-    const float q = sum_of_index(at, w, P.k, k, j);
-    if (q >= 0.f) g[j] = from_f32<T>(ex2(fmaf(to_f32(s[j]), c, -r)) * scale - f * (q * st.w));
+    const float q = sum_of_index(at, P.k, k, j, [&](int i) { return w[i]; });
+    if (q >= 0.f) g[j] = from_f32<T>(ex2((to_f32(s[j]) - r) * c) * scale - f * (q * st.w));
   }
 }
 
@@ -529,27 +631,26 @@ int launch_loss(const DistillParams& P, cudaStream_t st) {
   return launch_clusters(loss_kernel<T>, P, false, size, kLossThreads, 0, st);
 }
 
-template <typename T, int NT, int N>
+template <typename T, int DW>
 int launch_rows(const DistillParams& P, int size, cudaStream_t st) {
-  const size_t smem = (size_t)((P.k + 3) & ~3) * 8 + (size_t)((row_units(P.x) + size - 1) / size) * 16;
-  const auto kernel = row_kernel<T, NT, N>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess)
+  const size_t smem = 2 * RowRecord<T>::bytes((P.k + 3) & ~3) + (size_t)((row_units(P.x) + size - 1) / size) * 16;
+  const auto kernel = row_kernel<T, DW>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess)
     return launch_status();
-  return launch_clusters(kernel, P, true, size, NT, smem, st);
+  return launch_clusters(kernel, P, true, size, DW * 32 + 32, smem, st);
 }
 
 template <typename T>
 int launch_loss_grad(const DistillParams& P, cudaStream_t st) {
-  // As many CTAs a row as keep its part within 64 KB, three of 256 threads on an SM; few rows take more,
-  // down to a unit a thread.  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 512 threads.
+  // As many CTAs a row as keep its part within 64 KB, three of eight data warps on an SM; few rows take
+  // more, down to a unit a thread.  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 16 warps.
   const int units = row_units(P.x);
   int size = 1;
   while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
   while (size < 8 && P.x.rows * size < 2 * 148 && units > size * 256) size *= 2;
   if constexpr (sizeof(T) == 4)
-    if ((units + size - 1) / size > 6144)
-      return P.k <= 512 ? launch_rows<T, 512, 1>(P, size, st) : launch_rows<T, 512, 2>(P, size, st);
-  return P.k <= 256 ? launch_rows<T, 256, 1>(P, size, st) : launch_rows<T, 256, 4>(P, size, st);
+    if ((units + size - 1) / size > 6144) return launch_rows<T, 16>(P, size, st);
+  return launch_rows<T, 8>(P, size, st);
 }
 
 template <typename F>

@@ -49,7 +49,7 @@ struct DistillParams {
   const float* weight;                    // factor of each row's gradient; null: 1
   long long weight_stride;                // 0: one factor for every row
   float* loss;                            // [rows]
-  float4* stats;                          // [rows] {R, 1 / S, v_max, 1 / Q (0: no record)}
+  float4* stats;                          // [rows] {largest logit, 1 / S, v_max, 1 / Q (0: no record)}
   void* grad; long long grad_stride;      // the logits' type
 };
 int launch_distill_forward(const DistillParams& P, cudaStream_t st);   // loss, stats (optional)

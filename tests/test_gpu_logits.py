@@ -319,6 +319,30 @@ def test_distillation_masks_and_repeats(dtype):
     check_distill(x, values_seen, seen, 1.0, weight, loss.detach(), torch.autograd.grad(loss, y, weight)[0])
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_distillation_rows_of_the_lowest_value(dtype):
+    """A student row masked by the type's lowest value everywhere is even; one logit above takes it all."""
+    import sq325
+    vocab = 2003
+    x = torch.full((3, vocab), torch.finfo(dtype).min, device='cuda', dtype=dtype)
+    x[1, 7] = 0.0
+    x[2, ::2] = float('-inf')
+    values = torch.zeros((3, 2), device='cuda')
+    indices = torch.tensor([[7, 9]] * 3, device='cuda', dtype=torch.int32)
+    left = [vocab, 1, vocab // 2]
+    want = torch.zeros((3, vocab), dtype=torch.float64)
+    want[0] = 1 / left[0]
+    want[1, 7] = 1.0
+    want[2, 1::2] = 1 / left[2]
+    want[:, [7, 9]] -= 0.5
+    y = x.detach().requires_grad_(True)
+    again = sq325.distillation_loss(y, values, indices)
+    for loss, grad in (sq325.distillation_loss_grad(x, values, indices), (again, torch.autograd.grad(again.sum(), y)[0])):
+        assert abs(float(loss[0]) - np.log(left[0] / 2)) < 1e-5 and abs(float(loss[2]) - np.log(left[2] / 2)) < 1e-5
+        assert float(loss[1]) > 1e4                      # half of the teacher's weight lies where the student has none
+        assert ((grad.double().cpu() - want).abs() <= 2 ** -8 * want.abs() + 1e-6).all()
+
+
 def test_distillation_undefined_student():
     import sq325
     x = torch.zeros((5, 600), device='cuda')
