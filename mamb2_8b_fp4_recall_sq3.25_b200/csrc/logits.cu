@@ -53,9 +53,8 @@ struct Shared {
   u64 slot[2][8];
   u64 part[NW];
   float fpart[NW];
-  u64 sums[kSteps];                              // this CTA's histogram
-  u64 scan[NW];
-  u64 found_above, found_mine;
+  u64 sums[kSteps], total[kSteps];               // this CTA's histogram and the row's
+  u64 found_above, found_mine, found_need;
   int found, count, pick;
   uint2 counts[2][NW];
   int groups;
@@ -420,22 +419,31 @@ struct Row : Team {
     ready();
   }
 
-  // f(x, t, unit, element) over this thread's elements, t their exponents.
+  // f(unit, exponents) over this thread's units.
   template <typename F>
-  __device__ void each(Exponent e, F f) const {
+  __device__ void each_unit(Exponent e, F f) const {
     for (int i = tid; i < d.n; i += NT) {
       Unit<T> u;
       u.q = unit[i].q;
+      float2 t[kUnit<T> / 2];
 #pragma unroll
-      for (int v = 0; v < kUnit<T>; v += 2) {
-        const float2 x = make_float2(to_f32(u.v[v]), to_f32(u.v[v + 1])), t = e(x);
-        f(x.x, t.x, i, v);
-        f(x.y, t.y, i, v + 1);
-      }
+      for (int v = 0; v < kUnit<T>; v += 2) t[v / 2] = e(make_float2(to_f32(u.v[v]), to_f32(u.v[v + 1])));
+      f(i, t);
+    }
+  }
+  // f(x, t, position) for the elements of unit i whose bits are set in `which`.
+  template <typename F>
+  __device__ void each_bit(uint32_t which, int i, Exponent e, F f) const {
+    while (which) {
+      const int v = __ffs(which) - 1;
+      which &= which - 1;
+      const float x = to_f32(unit[i].v[v]);
+      f(x, e(x), i * kUnit<T> + v);
     }
   }
   __device__ float own_max() const {
     float m = -INFINITY;
+#pragma unroll 4
     for (int i = tid; i < d.n; i += NT) {
       Unit<T> u;
       u.q = unit[i].q;
@@ -508,42 +516,46 @@ struct Row : Team {
     return s.pick;
   }
 
-  // Scan of `total` (thread i: weight of histogram entry i over the row, `mine` this CTA's) for the
-  // first entry at which the running weight reaches need(whole weight), starting from `above`; adds the
-  // entries before it to `above` and `mine_above`.  Returns -1 if it is not reached.
+  // The first entry of the row's histogram s.total at which the running weight, from `above` on, reaches
+  // need(whole weight); adds the entries before it to `above`, and of this CTA's histogram to
+  // `mine_above`.  Returns -1 if it is not reached.  The first warp does it, eight entries a lane.
   template <typename N>
-  __device__ int crossing(u64 total, u64 mine, N need_of, u64& above, u64& mine_above) {
-    const int warp = tid >> 5, lane = tid & 31;
-    u64 run = total, own = mine;
+  __device__ int crossing(N need_of, u64& above, u64& mine_above) {
+    constexpr int E = kSteps / 32;
+    __syncthreads();
+    if (tid < 32) {
+      u64 sum = 0, own = 0;
+      for (int i = 0; i < E; ++i) { sum += s.total[tid * E + i]; own += s.sums[tid * E + i]; }
+      u64 run = sum, own_run = own;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 a = __shfl_up_sync(0xffffffffu, run, o), b = __shfl_up_sync(0xffffffffu, own, o);
-      if (lane >= o) { run += a; own += b; }
+      for (int o = 1; o < 32; o <<= 1) {
+        const u64 a = __shfl_up_sync(0xffffffffu, run, o), b = __shfl_up_sync(0xffffffffu, own_run, o);
+        if (tid >= o) { run += a; own_run += b; }
+      }
+      const u64 need = need_of(__shfl_sync(0xffffffffu, run, 31));
+      u64 before = above + run - sum, own_before = mine_above + own_run - own;
+      const bool here = before < need && before + sum >= need;
+      if (here) {
+        int i = tid * E;
+        for (; before + s.total[i] < need; ++i) { before += s.total[i]; own_before += s.sums[i]; }
+        s.found = i;
+        s.found_above = before;
+        s.found_mine = own_before;
+        s.found_need = need;
+      }
+      if (!__any_sync(0xffffffffu, here) && tid == 0) s.found = -1;
     }
     __syncthreads();
-    if (lane == 31) { s.scan[warp] = run; s.part[warp] = own; }
-    if (tid == 0) s.found = -1;
-    __syncthreads();
-    u64 whole = 0;
-    for (int i = 0; i < NW; ++i) whole += s.scan[i];
-    const u64 need = need_of(whole);
-    u64 before = above, mb = mine_above;
-    for (int i = 0; i < warp; ++i) { before += s.scan[i]; mb += s.part[i]; }
-    if (before + run >= need && before + run - total < need) {
-      s.found = tid;
-      s.found_above = before + run - total;
-      s.found_mine = mb + own - mine;
-    }
-    __syncthreads();
-    if (s.found >= 0) { above = s.found_above; mine_above = s.found_mine; }
-    return s.found;
+    const int at = s.found;
+    if (at >= 0) { above = s.found_above; mine_above = s.found_mine; }
+    return at;
   }
 
-  // The cut after the first tokens of the order whose weights w(x, t) reach need(whole weight), among
+  // The cut after the first tokens of the order whose weights w(t) reach need(whole weight), among
   // elements with kept(x, col).  t = (x - m) c is the exponent of y; w depends on it alone, is 0 where the
   // token's weight is, and below 2^31 + 1.  False: the whole weight does not reach it.
-  // kept_here: this CTA's share of the weight that is kept.
-  template <typename K, typename W, typename N>
+  // kept_here: this CTA's share of the weight that is kept.  PLAIN: every element is kept and w is weight_of.
+  template <bool PLAIN, typename K, typename W, typename N>
   __device__ bool select(K kept, W w, Exponent e, N need_of, Cut& cut, u64& kept_here) {
     static_assert(kSteps == NT, "a thread per step");
     constexpr int SH = std::is_same<T, __half>::value ? 13 : std::is_same<T, __nv_bfloat16>::value ? 16 : 0;
@@ -553,18 +565,37 @@ struct Row : Team {
     uint16_t* members = reinterpret_cast<uint16_t*>(high);
     const int lane = tid & (kCols - 1);
     // 2^23 + the step, as a float: its bits are in order and end in the step
-    const auto step = [&](float t) { return __float_as_uint(fmaf(t, -kPerOctave, 8388608.0f)); };
+    const auto step = [&](float2 t) { return __ffma2_rn(t, make_float2(-kPerOctave, -kPerOctave), make_float2(8388608.0f, 8388608.0f)); };
     constexpr uint32_t kStep0 = 0x4b000000u;
+    const auto count = [&](float t, uint32_t q) {
+      const uint32_t b = (__float_as_uint(fmaf(t, -kPerOctave, 8388608.0f)) - kStep0) * kCols + lane;
+      atomicAdd(low + b, q & kLow);
+      if (q >> kLowBits) atomicAdd(high + b, q >> kLowBits);
+    };
     __syncthreads();
     for (int i = tid; i < (kSteps + kHighSteps) * kCols; i += NT) low[i] = 0;
     __syncthreads();
-    each(e, [&](float x, float t, int i, int v) {
-      const uint32_t q = w(t);
-      if (q && kept(x, d.col(i, v))) {
-        const uint32_t b = (step(t) - kStep0) * kCols + lane;
-        atomicAdd(low + b, q & kLow);
-        if (q >> kLowBits) atomicAdd(high + b, q >> kLowBits);
+    each_unit(e, [&](int i, const float2 (&t)[kUnit<T> / 2]) {
+      uint32_t rest = 0;                         // elements that are not simply added
+#pragma unroll
+      for (int a = 0; a < kUnit<T> / 2; ++a) {
+        if (PLAIN) {
+          // weight_of for y < 2^-13, which fits the low word
+          const float2 y = __fadd2_rn(make_float2(ex2(t[a].x), ex2(t[a].y)), make_float2(0.00390625f, 0.00390625f)), b = step(t[a]);
+          const bool light0 = t[a].x < -13.02f, light1 = t[a].y < -13.02f;
+          if (light0 && t[a].x > -32.01f) atomicAdd(low + (__float_as_uint(b.x) - kStep0) * kCols + lane, __float_as_uint(y.x) & 0x7fffffu);
+          if (light1 && t[a].y > -32.01f) atomicAdd(low + (__float_as_uint(b.y) - kStep0) * kCols + lane, __float_as_uint(y.y) & 0x7fffffu);
+          if (!light0) rest |= 1u << (2 * a);
+          if (!light1) rest |= 2u << (2 * a);
+        } else {
+          if (t[a].x > -32.01f) rest |= 1u << (2 * a);
+          if (t[a].y > -32.01f) rest |= 2u << (2 * a);
+        }
       }
+      each_bit(rest, i, e, [&](float x, float t, int at) {
+        const uint32_t q = w(t);
+        if (q && (PLAIN || kept(x, d.col(0, at)))) count(t, q);
+      });
     });
     __syncthreads();
     u64 mine = 0, total = 0;
@@ -575,24 +606,35 @@ struct Row : Team {
     s.sums[tid] = mine;
     barrier();
     for (int r = 0; r < (int)size; ++r) total += remote_load(remote_smem(&s.sums[tid], r));
-    u64 above = 0, mine_above = 0, need = 0;
-    const int at = crossing(total, mine, [&](u64 whole) { return need = need_of(whole); }, above, mine_above);
+    s.total[tid] = total;
+    u64 above = 0, mine_above = 0;
+    const int at = crossing(need_of, above, mine_above);
     if (at < 0) { barrier(); return false; }
+    const u64 need = s.found_need;
     // the step's members, a list of positions (the whole part again where they are too many), and
     // the range of their keys
     if (tid == 0) { s.count = 0; s.key_low = 0xffffffffu; s.key_high = 0; }
     __syncthreads();
     const uint32_t wanted_step = kStep0 + at;
-    const auto member = [&](float x, float t, int i, int v) { return step(t) == wanted_step && w(t) && kept(x, d.col(i, v)); };
+    const auto each_in_step = [&](auto f) {
+      each_unit(e, [&](int i, const float2 (&t)[kUnit<T> / 2]) {
+        uint32_t which = 0;
+#pragma unroll
+        for (int a = 0; a < kUnit<T> / 2; ++a) {
+          const float2 b = step(t[a]);
+          if (__float_as_uint(b.x) == wanted_step) which |= 1u << (2 * a);
+          if (__float_as_uint(b.y) == wanted_step) which |= 2u << (2 * a);
+        }
+        each_bit(which, i, e, [&](float x, float t, int at) { if (w(t) && (PLAIN || kept(x, d.col(0, at)))) f(x, at); });
+      });
+    };
     uint32_t lo = 0xffffffffu, hi = 0;
-    each(e, [&](float x, float t, int i, int v) {
-      if (member(x, t, i, v)) {
-        const int k = atomicAdd(&s.count, 1);
-        if (k < kMembers) members[k] = (uint16_t)(i * kUnit<T> + v);
-        const uint32_t key = order_key(x + 0.0f) >> SH;
-        lo = min(lo, key);
-        hi = max(hi, key);
-      }
+    each_in_step([&](float x, int at) {
+      const int k = atomicAdd(&s.count, 1);
+      if (k < kMembers) members[k] = (uint16_t)at;
+      const uint32_t key = order_key(x + 0.0f) >> SH;
+      lo = min(lo, key);
+      hi = max(hi, key);
     });
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
@@ -608,7 +650,7 @@ struct Row : Team {
       if (listed <= kMembers) {
         for (int k = tid; k < listed; k += NT) f(to_f32(unit[members[k] / kUnit<T>].v[members[k] % kUnit<T>]));
       } else {
-        each(e, [&](float x, float t, int i, int v) { if (member(x, t, i, v)) f(x); });
+        each_in_step([&](float x, int) { f(x); });
       }
     };
     uint32_t key;
@@ -630,15 +672,15 @@ struct Row : Team {
       });
       __syncthreads();
       mine = total = 0;
-      if (tid < kFine) {
+      if (tid < kFine)
         for (int i = 0; i < kCols; ++i)
           mine += low[tid * kCols + i] + ((u64)upper[tid * kCols + i] << kLowBits);
-        s.sums[tid] = mine;
-      }
+      s.sums[tid] = mine;
       barrier();
       if (tid < kFine)
         for (int r = 0; r < (int)size; ++r) total += remote_load(remote_smem(&s.sums[tid], r));
-      entry = crossing(total, mine, [&](u64) { return need; }, above, mine_above);
+      s.total[tid] = total;
+      entry = crossing([&](u64) { return need; }, above, mine_above);
       if (shift == 0) {
         key = hi - entry;
         for (int r = 0; r < (int)rank; ++r) key_before += remote_load(remote_smem(&s.sums[entry], r));
@@ -651,8 +693,11 @@ struct Row : Team {
     const u64 here = s.sums[entry];
     // the key of 16-bit types stands for one logit: its low bits are those of an exact value
     const float x = key_logit(SH == 0 ? key : (key << SH) | ((key << SH) & 0x80000000u ? 0u : (1u << SH) - 1u));
-    const u64 each_w = w(e(x)), wanted = (need - above + each_w - 1) / each_w, earlier = key_before / each_w;
-    const u64 ties = here / each_w;
+    // quotients of numbers below 2^50 by one below 2^32: a double holds them closely enough for floor()
+    const u64 each_w = w(e(x));
+    const double by = (double)each_w;
+    const u64 wanted = (u64)floor((double)(need - above + each_w - 1) / by), earlier = (u64)floor((double)key_before / by);
+    const u64 ties = (u64)floor((double)here / by);
     cut.x = x;
     u64 taken = ties;
     if (wanted >= earlier + ties) {
@@ -750,14 +795,14 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
   u64 mine = 0;
   const bool by_rank = top_k > 0 && top_k < P.x.vocab;
   if (by_rank)
-    r.select(all, [](float t) { return weight_of(t) ? 1u : 0u; }, e, [&](u64) { return (u64)top_k; }, cut, mine);
+    r.select<false>(all, [](float t) { return weight_of(t) ? 1u : 0u; }, e, [&](u64) { return (u64)top_k; }, cut, mine);
   if (!(top_p >= 1.0f)) {
     Cut inner;
     if (by_rank) {
-      r.select(kept, weight_of, e, wanted, inner, mine);
+      r.select<false>(kept, weight_of, e, wanted, inner, mine);
       if (inner.x != cut.x || inner.last < cut.last) cut = inner;
     } else {
-      r.select(all, weight_of, e, wanted, cut, mine);
+      r.select<true>(all, weight_of, e, wanted, cut, mine);
     }
     known = !(min_p > 0.0f);
   }

@@ -337,7 +337,7 @@ def test_distillation_rows_of_the_lowest_value(dtype):
     want[:, [7, 9]] -= 0.5
     y = x.detach().requires_grad_(True)
     again = sq325.distillation_loss(y, values, indices)
-    for loss, grad in (sq325.distillation_loss_grad(x, values, indices), (again, torch.autograd.grad(again.sum(), y)[0])):
+    for loss, grad in (sq325.distillation_loss_grad(x, values, indices), (again.detach(), torch.autograd.grad(again.sum(), y)[0])):
         assert abs(float(loss[0]) - np.log(left[0] / 2)) < 1e-5 and abs(float(loss[2]) - np.log(left[2] / 2)) < 1e-5
         assert float(loss[1]) > 1e4                      # half of the teacher's weight lies where the student has none
         assert ((grad.double().cpu() - want).abs() <= 2 ** -8 * want.abs() + 1e-6).all()
