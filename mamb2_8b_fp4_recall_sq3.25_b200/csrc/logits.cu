@@ -53,12 +53,11 @@ struct Shared {
   u64 slot[2][8];
   u64 part[NW];
   float fpart[NW];
-  u64 sums[kSteps], total[kSteps];               // this CTA's histogram and the row's
+  u64 sums[2][kSteps];                           // this CTA's histogram, and the one before
   u64 found_above, found_mine, found_need;
   int found, count, pick;
   uint2 counts[2][NW];
   int groups;
-  uint32_t key_low, key_high;
 };
 
 __device__ __forceinline__ u64 warp_sum(u64 v) {
@@ -407,6 +406,7 @@ struct Row : Team {
   Span<T> d;
   unsigned char* work;                           // histogram and members
   Unit<T>* unit;
+  int turn = 0;                                  // of s.sums
   using Team::s; using Team::tid; using Team::rank; using Team::size;
 
   __device__ Row(const Team& t, const Span<T>& d, unsigned char* dyn)
@@ -472,6 +472,35 @@ struct Row : Team {
     for (int i = 0; i < NW; ++i) t += s.part[i];
     return t;
   }
+  // stretch_sums of the weights of what `cut` and min-p leave; nothing is left below `least`.
+  __device__ u64 left_sums(Exponent e, Cut cut, float min_p, float least) {
+    const int len = (d.n + NW - 1) / NW, i0 = (tid >> 5) * len, i1 = min(d.n, i0 + len);
+    min_p = fmaxf(min_p, 1e-10f);                // below 2^-33 the weight is 0: masked logits are no ties
+    u64 sum = 0;
+    for (int i = i0 + (tid & 31); i < i1; i += 32) {
+      Unit<T> u;
+      u.q = unit[i].q;
+      if (!(unit_max(u) >= least)) continue;
+      uint32_t ties = 0;
+#pragma unroll
+      for (int v = 0; v < kUnit<T>; v += 2) {
+        const float2 x = make_float2(to_f32(u.v[v]), to_f32(u.v[v + 1])), t = e(x);
+        const float2 y = make_float2(ex2(t.x), ex2(t.y));
+        if (x.x > cut.x && y.x >= min_p) sum += __float2uint_rn(y.x * 2147483648.0f);
+        if (x.y > cut.x && y.y >= min_p) sum += __float2uint_rn(y.y * 2147483648.0f);
+        if (x.x == cut.x && y.x >= min_p) ties |= 1u << v;
+        if (x.y == cut.x && y.y >= min_p) ties |= 2u << v;
+      }
+      each_bit(ties, i, e, [&](float, float t, int at) { if (d.col(0, at) <= cut.last) sum += weight_of(t); });
+    }
+    sum = warp_sum(sum);
+    __syncthreads();
+    if ((tid & 31) == 0) s.part[tid >> 5] = sum;
+    __syncthreads();
+    u64 t = 0;
+    for (int i = 0; i < NW; ++i) t += s.part[i];
+    return t;
+  }
   // After stretch_sums: the first column of this CTA, in order, at which the running sum passes
   // `target` (below the total).
   template <typename W>
@@ -516,16 +545,25 @@ struct Row : Team {
     return s.pick;
   }
 
-  // The first entry of the row's histogram s.total at which the running weight, from `above` on, reaches
-  // need(whole weight); adds the entries before it to `above`, and of this CTA's histogram to
-  // `mine_above`.  Returns -1 if it is not reached.  The first warp does it, eight entries a lane.
+  // `mine`: entry tid of this CTA's histogram.  The first entry of the row's histogram, the sum over the CTAs,
+  // at which the running weight, from `above` on, reaches need(whole weight); adds the entries before
+  // it to `above`, and of this CTA's histogram to `mine_above`.  Returns -1 if it is not reached.  s.sums
+  // alternates, so that CTAs ahead do not overwrite what others still read.
   template <typename N>
-  __device__ int crossing(N need_of, u64& above, u64& mine_above) {
+  __device__ int crossing(u64 mine, N need_of, u64& above, u64& mine_above) {
     constexpr int E = kSteps / 32;
+    turn ^= 1;
+    const u64* sums = s.sums[turn];
+    u64* total = reinterpret_cast<u64*>(work);   // the histogram's words have been read
+    s.sums[turn][tid] = mine;
+    barrier();
+    u64 all = 0;
+    for (int r = 0; r < (int)size; ++r) all += remote_load(remote_smem(&sums[tid], r));
+    total[tid] = all;
     __syncthreads();
-    if (tid < 32) {
+    if (tid < 32) {                              // eight entries a lane
       u64 sum = 0, own = 0;
-      for (int i = 0; i < E; ++i) { sum += s.total[tid * E + i]; own += s.sums[tid * E + i]; }
+      for (int i = 0; i < E; ++i) { sum += total[tid * E + i]; own += sums[tid * E + i]; }
       u64 run = sum, own_run = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -537,7 +575,7 @@ struct Row : Team {
       const bool here = before < need && before + sum >= need;
       if (here) {
         int i = tid * E;
-        for (; before + s.total[i] < need; ++i) { before += s.total[i]; own_before += s.sums[i]; }
+        for (; before + total[i] < need; ++i) { before += total[i]; own_before += sums[i]; }
         s.found = i;
         s.found_above = before;
         s.found_mine = own_before;
@@ -551,6 +589,7 @@ struct Row : Team {
     return at;
   }
 
+  // A cluster barrier has to follow before the CTA ends (others read its sums).
   // The cut after the first tokens of the order whose weights w(t) reach need(whole weight), among
   // elements with kept(x, col).  t = (x - m) c is the exponent of y; w depends on it alone, is 0 where the
   // token's weight is, and below 2^31 + 1.  False: the whole weight does not reach it.
@@ -598,23 +637,36 @@ struct Row : Team {
       });
     });
     __syncthreads();
-    u64 mine = 0, total = 0;
+    u64 mine = 0;
     for (int i = 0; i < kCols; ++i) {
       mine += low[tid * kCols + i];
       if (tid < kHighSteps) mine += (u64)high[tid * kCols + i] << kLowBits;
     }
-    s.sums[tid] = mine;
-    barrier();
-    for (int r = 0; r < (int)size; ++r) total += remote_load(remote_smem(&s.sums[tid], r));
-    s.total[tid] = total;
     u64 above = 0, mine_above = 0;
-    const int at = crossing(need_of, above, mine_above);
-    if (at < 0) { barrier(); return false; }
+    const int at = crossing(mine, need_of, above, mine_above);
+    if (at < 0) return false;
     const u64 need = s.found_need;
-    // the step's members, a list of positions (the whole part again where they are too many), and
-    // the range of their keys
-    if (tid == 0) { s.count = 0; s.key_low = 0xffffffffu; s.key_high = 0; }
-    __syncthreads();
+    // keys in which the step can lie: its edges in x, widened by far more than the rounding of t and of this
+    // (NaN, from infinities, widens to everything)
+    const float first = e.m - (at - 0.5f) / kPerOctave / e.c, last = e.m - (at + 0.5f) / kPerOctave / e.c;
+    uint32_t hi = order_key(fminf(e.m, first + 4e-6f * (fabsf(e.m) + fabsf(first - e.m))) + 0.0f) >> SH;
+    uint32_t lo = order_key(fmaxf(-3.4028235e38f, last - 4e-6f * (fabsf(e.m) + fabsf(last - e.m)))) >> SH;
+    // narrowing: histograms of the step's members over their keys.  The first is made on the way through the
+    // part, which also lists the members' positions (if they are too many, every round goes through the part).
+    uint32_t* upper = low + kFine * kCols;
+    int shift;
+    const auto begin = [&] {
+      for (shift = 0; ((hi - lo) >> shift) >= (uint32_t)kFine; ++shift) {}
+      for (int i = tid; i < 2 * kFine * kCols; i += NT) low[i] = 0;
+      __syncthreads();
+    };
+    const auto add = [&](float x, float t) {
+      const uint32_t k = order_key(x + 0.0f) >> SH;
+      if (k < lo || k > hi) return;              // decided by an earlier round
+      const uint32_t b = ((hi - k) >> shift) * kCols + lane, q = w(t);
+      atomicAdd(low + b, q & kLow);
+      if (q >> kLowBits) atomicAdd(upper + b, q >> kLowBits);
+    };
     const uint32_t wanted_step = kStep0 + at;
     const auto each_in_step = [&](auto f) {
       each_unit(e, [&](int i, const float2 (&t)[kUnit<T> / 2]) {
@@ -625,72 +677,43 @@ struct Row : Team {
           if (__float_as_uint(b.x) == wanted_step) which |= 1u << (2 * a);
           if (__float_as_uint(b.y) == wanted_step) which |= 2u << (2 * a);
         }
-        each_bit(which, i, e, [&](float x, float t, int at) { if (w(t) && (PLAIN || kept(x, d.col(0, at)))) f(x, at); });
+        each_bit(which, i, e, [&](float x, float t, int at) { if (PLAIN || (w(t) && kept(x, d.col(0, at)))) f(x, t, at); });
       });
     };
-    uint32_t lo = 0xffffffffu, hi = 0;
-    each_in_step([&](float x, int at) {
+    if (tid == 0) s.count = 0;
+    begin();
+    each_in_step([&](float x, float t, int at) {
       const int k = atomicAdd(&s.count, 1);
       if (k < kMembers) members[k] = (uint16_t)at;
-      const uint32_t key = order_key(x + 0.0f) >> SH;
-      lo = min(lo, key);
-      hi = max(hi, key);
+      add(x, t);
     });
-    lo = __reduce_min_sync(0xffffffffu, lo);
-    hi = __reduce_max_sync(0xffffffffu, hi);
-    if ((tid & 31) == 0 && lo <= hi) { atomicMin(&s.key_low, lo); atomicMax(&s.key_high, hi); }
-    __syncthreads();
-    const int listed = s.count;
-    exchange((u64)s.key_high << 32 | s.key_low);
-    for (int r = 0; r < (int)size; ++r) {
-      lo = min(r ? lo : 0xffffffffu, (uint32_t)got(r));
-      hi = max(r ? hi : 0u, (uint32_t)(got(r) >> 32));
-    }
-    const auto each_member = [&](auto f) {
-      if (listed <= kMembers) {
-        for (int k = tid; k < listed; k += NT) f(to_f32(unit[members[k] / kUnit<T>].v[members[k] % kUnit<T>]));
-      } else {
-        each_in_step([&](float x, int) { f(x); });
-      }
-    };
-    uint32_t key;
     int entry;
-    u64 key_before = 0;                          // weight of that key in the CTAs before this one
     for (;;) {
-      int shift = 0;
-      while (((hi - lo) >> shift) >= (uint32_t)kFine) ++shift;
-      uint32_t* upper = low + kFine * kCols;
       __syncthreads();
-      for (int i = tid; i < 2 * kFine * kCols; i += NT) low[i] = 0;
-      barrier();                                 // and every CTA has read the sums of the round before
-      each_member([&](float x) {
-        const uint32_t k = order_key(x + 0.0f) >> SH;
-        if (k < lo || k > hi) return;            // decided by an earlier round
-        const uint32_t b = ((hi - k) >> shift) * kCols + lane, q = w(e(x));
-        atomicAdd(low + b, q & kLow);
-        if (q >> kLowBits) atomicAdd(upper + b, q >> kLowBits);
-      });
-      __syncthreads();
-      mine = total = 0;
+      mine = 0;
       if (tid < kFine)
         for (int i = 0; i < kCols; ++i)
           mine += low[tid * kCols + i] + ((u64)upper[tid * kCols + i] << kLowBits);
-      s.sums[tid] = mine;
-      barrier();
-      if (tid < kFine)
-        for (int r = 0; r < (int)size; ++r) total += remote_load(remote_smem(&s.sums[tid], r));
-      s.total[tid] = total;
-      entry = crossing([&](u64) { return need; }, above, mine_above);
-      if (shift == 0) {
-        key = hi - entry;
-        for (int r = 0; r < (int)rank; ++r) key_before += remote_load(remote_smem(&s.sums[entry], r));
-        break;
-      }
+      entry = crossing(mine, [&](u64) { return need; }, above, mine_above);
+      if (shift == 0) break;
       hi = hi - ((uint32_t)entry << shift);
       const uint32_t width = (1u << shift) - 1;
       if (hi - lo > width) lo = hi - width;
+      begin();
+      const int listed = s.count;
+      if (listed <= kMembers) {
+        for (int k = tid; k < listed; k += NT) {
+          const float x = to_f32(unit[members[k] / kUnit<T>].v[members[k] % kUnit<T>]);
+          add(x, e(x));
+        }
+      } else {
+        each_in_step([&](float x, float t, int) { add(x, t); });
+      }
     }
-    const u64 here = s.sums[entry];
+    const uint32_t key = hi - entry;
+    u64 key_before = 0;                          // weight of that key in the CTAs before this one
+    for (int r = 0; r < (int)rank; ++r) key_before += remote_load(remote_smem(&s.sums[turn][entry], r));
+    const u64 here = s.sums[turn][entry];
     // the key of 16-bit types stands for one logit: its low bits are those of an exact value
     const float x = key_logit(SH == 0 ? key : (key << SH) | ((key << SH) & 0x80000000u ? 0u : (1u << SH) - 1u));
     // quotients of numbers below 2^50 by one below 2^32: a double holds them closely enough for floor()
@@ -712,7 +735,6 @@ struct Row : Team {
       cut.last = locate(tie, taken - 1);
     }
     kept_here = mine_above + taken * each_w;
-    barrier();                                   // sums are read before anybody goes on
     return true;
   }
 };
@@ -812,7 +834,7 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
   };
   // nothing below this passes min-p: a hundredth of an octave is far more than the rounding of t
   const float least = fmaxf(cut.x, e.m + (log2f(min_p) - 0.01f) / e.c);
-  if (!known) mine = r.stretch_sums(left, least);
+  if (!known) mine = r.left_sums(e, cut, min_p, least);
   __syncthreads();
   r.exchange(mine);
   u64 total = 0, before = 0;
@@ -822,7 +844,7 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
   }
   const u64 target = draw(u, total);
   if (target < before || target >= before + mine) return;      // the token is another CTA's
-  if (known) r.stretch_sums(left, least);
+  if (known) r.left_sums(e, cut, min_p, least);
   const int at = r.locate(left, target - before);
   if (tid == 0) P.tokens[row] = at;
 }
