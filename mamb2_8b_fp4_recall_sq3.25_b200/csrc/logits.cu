@@ -400,6 +400,13 @@ __device__ __forceinline__ uint32_t weight_of(float t) {
   return __float2uint_rn(y * 2147483648.0f);
 }
 
+// Adds `w` to the histogram word at `address` if the weight is light, -32.01 < t < kLight (without a branch: most are).
+constexpr float kLight = -13.02f;
+__device__ __forceinline__ void add_light(uint32_t address, uint32_t w, float t) {
+  asm volatile("{\n.reg .pred p;\nsetp.lt.f32 p, %2, %3;\nsetp.gt.and.f32 p, %2, %4, p;\n@p red.shared.add.u32 [%0], %1;\n}\n"
+               :: "r"(address), "r"(w), "f"(t), "f"(kLight), "f"(-32.01f) : "memory");
+}
+
 // One CTA's part of a row in shared memory.
 template <typename T>
 struct Row : Team {
@@ -431,15 +438,20 @@ struct Row : Team {
       f(i, t);
     }
   }
-  // f(x, t, position) for the elements of unit i whose bits are set in `which`.
+  // f(position) for the elements of unit i whose bits are set in `which`.
   template <typename F>
-  __device__ void each_bit(uint32_t which, int i, Exponent e, F f) const {
+  __device__ void each_bit(uint32_t which, int i, F f) const {
     while (which) {
-      const int v = __ffs(which) - 1;
+      f(i * kUnit<T> + __ffs(which) - 1);
       which &= which - 1;
-      const float x = to_f32(unit[i].v[v]);
-      f(x, e(x), i * kUnit<T> + v);
     }
+  }
+  __device__ float at(int position) const { return to_f32(reinterpret_cast<const T*>(unit)[position]); }
+  // Positions are noted in list[0 .. most) for a second pass with all lanes busy; returns whether there was room.
+  __device__ bool note(uint16_t* list, int most, int position) {
+    const int k = atomicAdd(&s.count, 1);
+    if (k < most) list[k] = (uint16_t)position;
+    return k < most;
   }
   __device__ float own_max() const {
     float m = -INFINITY;
@@ -491,7 +503,7 @@ struct Row : Team {
         if (x.x == cut.x && y.x >= min_p) ties |= 1u << v;
         if (x.y == cut.x && y.y >= min_p) ties |= 2u << v;
       }
-      each_bit(ties, i, e, [&](float, float t, int at) { if (d.col(0, at) <= cut.last) sum += weight_of(t); });
+      each_bit(ties, i, [&](int p) { if (d.col(0, p) <= cut.last) sum += weight_of(e(at(p))); });
     }
     sum = warp_sum(sum);
     __syncthreads();
@@ -606,14 +618,21 @@ struct Row : Team {
     // 2^23 + the step, as a float: its bits are in order and end in the step
     const auto step = [&](float2 t) { return __ffma2_rn(t, make_float2(-kPerOctave, -kPerOctave), make_float2(8388608.0f, 8388608.0f)); };
     constexpr uint32_t kStep0 = 0x4b000000u;
-    const auto count = [&](float t, uint32_t q) {
-      const uint32_t b = (__float_as_uint(fmaf(t, -kPerOctave, 8388608.0f)) - kStep0) * kCols + lane;
+    const auto count = [&](int p) {
+      const float x = at(p), t = e(x);
+      const uint32_t q = w(t), b = (__float_as_uint(fmaf(t, -kPerOctave, 8388608.0f)) - kStep0) * kCols + lane;
+      if (!q || !(PLAIN || kept(x, d.col(0, p)))) return;
       atomicAdd(low + b, q & kLow);
       if (q >> kLowBits) atomicAdd(high + b, q >> kLowBits);
     };
     __syncthreads();
     for (int i = tid; i < (kSteps + kHighSteps) * kCols; i += NT) low[i] = 0;
+    if (tid == 0) s.count = 0;
     __syncthreads();
+    // no CTA reads sums of the other turn any more, and this one writes them after the next barrier of its own
+    uint16_t* noted = reinterpret_cast<uint16_t*>(s.sums[turn ^ 1]);
+    constexpr int kNoted = sizeof(s.sums[0]) / sizeof(uint16_t);
+    const uint32_t words = (uint32_t)__cvta_generic_to_shared(low + lane) - kStep0 * kCols * 4;
     each_unit(e, [&](int i, const float2 (&t)[kUnit<T> / 2]) {
       uint32_t rest = 0;                         // elements that are not simply added
 #pragma unroll
@@ -621,21 +640,19 @@ struct Row : Team {
         if (PLAIN) {
           // weight_of for y < 2^-13, which fits the low word
           const float2 y = __fadd2_rn(make_float2(ex2(t[a].x), ex2(t[a].y)), make_float2(0.00390625f, 0.00390625f)), b = step(t[a]);
-          const bool light0 = t[a].x < -13.02f, light1 = t[a].y < -13.02f;
-          if (light0 && t[a].x > -32.01f) atomicAdd(low + (__float_as_uint(b.x) - kStep0) * kCols + lane, __float_as_uint(y.x) & 0x7fffffu);
-          if (light1 && t[a].y > -32.01f) atomicAdd(low + (__float_as_uint(b.y) - kStep0) * kCols + lane, __float_as_uint(y.y) & 0x7fffffu);
-          if (!light0) rest |= 1u << (2 * a);
-          if (!light1) rest |= 2u << (2 * a);
+          add_light(words + __float_as_uint(b.x) * (kCols * 4), __float_as_uint(y.x) & 0x7fffffu, t[a].x);
+          add_light(words + __float_as_uint(b.y) * (kCols * 4), __float_as_uint(y.y) & 0x7fffffu, t[a].y);
+          if (!(t[a].x < kLight)) rest |= 1u << (2 * a);
+          if (!(t[a].y < kLight)) rest |= 2u << (2 * a);
         } else {
           if (t[a].x > -32.01f) rest |= 1u << (2 * a);
           if (t[a].y > -32.01f) rest |= 2u << (2 * a);
         }
       }
-      each_bit(rest, i, e, [&](float x, float t, int at) {
-        const uint32_t q = w(t);
-        if (q && (PLAIN || kept(x, d.col(0, at)))) count(t, q);
-      });
+      each_bit(rest, i, [&](int p) { if (!note(noted, kNoted, p)) count(p); });
     });
+    __syncthreads();
+    for (int k = tid; k < min(s.count, kNoted); k += NT) count(noted[k]);
     __syncthreads();
     u64 mine = 0;
     for (int i = 0; i < kCols; ++i) {
@@ -643,31 +660,33 @@ struct Row : Team {
       if (tid < kHighSteps) mine += (u64)high[tid * kCols + i] << kLowBits;
     }
     u64 above = 0, mine_above = 0;
-    const int at = crossing(mine, need_of, above, mine_above);
-    if (at < 0) return false;
+    const int found = crossing(mine, need_of, above, mine_above);
+    if (found < 0) return false;
     const u64 need = s.found_need;
     // keys in which the step can lie: its edges in x, widened by far more than the rounding of t and of this
     // (NaN, from infinities, widens to everything)
-    const float first = e.m - (at - 0.5f) / kPerOctave / e.c, last = e.m - (at + 0.5f) / kPerOctave / e.c;
+    const float first = e.m - (found - 0.5f) / kPerOctave / e.c, last = e.m - (found + 0.5f) / kPerOctave / e.c;
     uint32_t hi = order_key(fminf(e.m, first + 4e-6f * (fabsf(e.m) + fabsf(first - e.m))) + 0.0f) >> SH;
     uint32_t lo = order_key(fmaxf(-3.4028235e38f, last - 4e-6f * (fabsf(e.m) + fabsf(last - e.m)))) >> SH;
-    // narrowing: histograms of the step's members over their keys.  The first is made on the way through the
-    // part, which also lists the members' positions (if they are too many, every round goes through the part).
+    // narrowing: histograms of the step's members over their keys; the members' positions are listed first
+    // (if they are too many, every round goes through the part)
     uint32_t* upper = low + kFine * kCols;
     int shift;
     const auto begin = [&] {
       for (shift = 0; ((hi - lo) >> shift) >= (uint32_t)kFine; ++shift) {}
       for (int i = tid; i < 2 * kFine * kCols; i += NT) low[i] = 0;
-      __syncthreads();
+      __syncthreads();                           // and the members are listed
     };
-    const auto add = [&](float x, float t) {
+    const auto add = [&](int p) {
+      const float x = at(p);
       const uint32_t k = order_key(x + 0.0f) >> SH;
       if (k < lo || k > hi) return;              // decided by an earlier round
-      const uint32_t b = ((hi - k) >> shift) * kCols + lane, q = w(t);
+      const uint32_t b = ((hi - k) >> shift) * kCols + lane, q = w(e(x));
+      if (!PLAIN && !kept(x, d.col(0, p))) return;
       atomicAdd(low + b, q & kLow);
       if (q >> kLowBits) atomicAdd(upper + b, q >> kLowBits);
     };
-    const uint32_t wanted_step = kStep0 + at;
+    const uint32_t wanted_step = kStep0 + found;
     const auto each_in_step = [&](auto f) {
       each_unit(e, [&](int i, const float2 (&t)[kUnit<T> / 2]) {
         uint32_t which = 0;
@@ -677,18 +696,20 @@ struct Row : Team {
           if (__float_as_uint(b.x) == wanted_step) which |= 1u << (2 * a);
           if (__float_as_uint(b.y) == wanted_step) which |= 2u << (2 * a);
         }
-        each_bit(which, i, e, [&](float x, float t, int at) { if (PLAIN || (w(t) && kept(x, d.col(0, at)))) f(x, t, at); });
+        each_bit(which, i, f);
       });
     };
     if (tid == 0) s.count = 0;
-    begin();
-    each_in_step([&](float x, float t, int at) {
-      const int k = atomicAdd(&s.count, 1);
-      if (k < kMembers) members[k] = (uint16_t)at;
-      add(x, t);
-    });
+    __syncthreads();
+    each_in_step([&](int p) { note(members, kMembers, p); });
     int entry;
     for (;;) {
+      begin();
+      if (s.count <= kMembers) {
+        for (int k = tid; k < s.count; k += NT) add(members[k]);
+      } else {
+        each_in_step(add);
+      }
       __syncthreads();
       mine = 0;
       if (tid < kFine)
@@ -699,16 +720,6 @@ struct Row : Team {
       hi = hi - ((uint32_t)entry << shift);
       const uint32_t width = (1u << shift) - 1;
       if (hi - lo > width) lo = hi - width;
-      begin();
-      const int listed = s.count;
-      if (listed <= kMembers) {
-        for (int k = tid; k < listed; k += NT) {
-          const float x = to_f32(unit[members[k] / kUnit<T>].v[members[k] % kUnit<T>]);
-          add(x, e(x));
-        }
-      } else {
-        each_in_step([&](float x, float t, int) { add(x, t); });
-      }
     }
     const uint32_t key = hi - entry;
     u64 key_before = 0;                          // weight of that key in the CTAs before this one
