@@ -369,8 +369,29 @@ struct Listing {
     sort(total);
     return total;
   }
-  // list[0 .. n) by falling value (what follows up to a power of two is lost).
+  // list[0 .. n) by falling value.  Few items are placed by counting the larger ones, which takes two
+  // barriers; more by a bitonic network.
   __device__ void sort(int n) {
+    if (n <= 2 * NT) {
+      __syncthreads();
+      u64 item[2];
+      int place[2] = {0, 0};
+#pragma unroll
+      for (int a = 0; a < 2; ++a) item[a] = t.tid + a * NT < n ? list[t.tid + a * NT] : 0;
+      const int both = n > NT;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const u64 other = list[j];
+        place[0] += other > item[0];
+        if (both) place[1] += other > item[1];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+        if (t.tid + a * NT < n) list[place[a]] = item[a];
+      __syncthreads();
+      return;
+    }
     int size = 1;
     while (size < n) size <<= 1;
     for (int i = n + t.tid; i < size; i += NT) list[i] = 0;
@@ -649,7 +670,13 @@ struct Row : Team {
           if (t[a].y > -32.01f) rest |= 2u << (2 * a);
         }
       }
-      each_bit(rest, i, [&](int p) { if (!note(noted, kNoted, p)) count(p); });
+      if (__popc(rest) <= 2) {
+        each_bit(rest, i, [&](int p) { if (!note(noted, kNoted, p)) count(p); });
+      } else {                                   // a flat stretch: element by element, without the detour
+#pragma unroll
+        for (int v = 0; v < kUnit<T>; ++v)
+          if (rest >> v & 1) count(i * kUnit<T> + v);
+      }
     });
     __syncthreads();
     for (int k = tid; k < min(s.count, kNoted); k += NT) count(noted[k]);
@@ -795,15 +822,21 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
     u64 whole;
     const u64 before = team.block_scan(w, whole);
     const bool in = w && (tid == 0 || (before < wanted(whole) && ex2(t) >= min_p));
-    if (tid == 0) s.count = 0;
+    // the first in index order whose running weight passes the target: each sums what stands before it
+    u64* left = list + NT;
+    left[tid] = in ? item << 32 | w : 0;         // ~column above the weight
     __syncthreads();
-    if (in) list[atomicAdd(&s.count, 1)] = item << 32 | w;     // by falling ~column: in index order
-    __syncthreads();
-    const int left = s.count;
-    l.sort(left);
-    const u64 mine = tid < left ? list[tid] : 0;
-    const u64 from = team.block_scan((uint32_t)mine, whole), target = draw(u, whole);
-    if (tid < left && target >= from && target < from + (uint32_t)mine) P.tokens[row] = (long long)~(uint32_t)(mine >> 32);
+    if (!in) return;
+    u64 from = 0;
+    whole = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) {
+      const u64 other = left[j];
+      if (other >> 32 > (item & 0xffffffffu)) from += (uint32_t)other;
+      whole += (uint32_t)other;
+    }
+    const u64 target = draw(u, whole);
+    if (target >= from && target < from + w) P.tokens[row] = (long long)~(uint32_t)item;
     return;
   }
 

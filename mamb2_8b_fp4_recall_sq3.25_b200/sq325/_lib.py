@@ -196,14 +196,14 @@ def stream_ptr(stream=None):
 
 def launch(name, device, *args):
     """call() with the current stream of `device` appended, for short kernels: the device is
-    switched only when another one is current, and the stream handle is read without building
+    switched only where another one is current, and the stream handle is read without building
     a Stream object."""
     import torch
     index = device.index
-    if index == torch.cuda.current_device():
-        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(device):
-        return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(device):
+            return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def ptr(t):

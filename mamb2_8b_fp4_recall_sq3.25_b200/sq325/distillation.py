@@ -34,19 +34,20 @@ def top_logits(logits, k):
     x = logits_rows(logits)
     if isinstance(k, bool) or not isinstance(k, int) or not 1 <= k <= min(MAX_RECORD, x.shape[1]):
         raise ValueError(f'k must be an integer in [1, min({MAX_RECORD}, vocab)]')
-    shape = (*logits.shape[:-1], k)
-    values = torch.empty(shape, device=x.device, dtype=x.dtype)
-    indices = torch.empty(shape, device=x.device, dtype=torch.int32)
+    values = x.new_empty((*logits.shape[:-1], k))
+    indices = torch.empty_like(values, dtype=torch.int32)
     _lib.launch('sq_top_logits', x.device, C.byref(logits_args(x)), k, values.data_ptr(), indices.data_ptr())
     return values, indices
 
 
 def _checked(logits, values, indices, temperature):
     x = logits_rows(logits)
-    if not isinstance(values, torch.Tensor) or not isinstance(indices, torch.Tensor) or values.shape != indices.shape \
-            or values.shape[:-1] != logits.shape[:-1] or values.ndim != logits.ndim:
+    if not isinstance(values, torch.Tensor) or not isinstance(indices, torch.Tensor):
+        raise ValueError('The record must be two tensors, values and indices')
+    shape = values.shape
+    if shape != indices.shape or len(shape) != logits.ndim or shape[:-1] != logits.shape[:-1]:
         raise ValueError('The record must be values and indices [..., k] with the leading shape of the logits')
-    if not 1 <= values.shape[-1] <= MAX_RECORD:
+    if not 1 <= shape[-1] <= MAX_RECORD:
         raise ValueError(f'The record must have 1 to {MAX_RECORD} entries a row')
     if values.dtype not in _TYPES or indices.dtype != torch.int32 or values.device != x.device \
             or indices.device != x.device:
@@ -59,23 +60,16 @@ def _checked(logits, values, indices, temperature):
 
 
 def _args(x, values, indices, temperature, weight=None, loss=None, stats=None, grad=None):
-    a = _lib.DistillArgs()
-    a.logits = logits_args(x)
-    a.values, a.indices = values.data_ptr(), indices.data_ptr()
-    a.k, a.value_type = values.shape[-1], _TYPES[values.dtype]
-    a.temperature = temperature
-    if weight is not None:
-        a.weight, a.weight_stride = weight.data_ptr(), weight.stride(0)
-    a.loss = loss.data_ptr() if loss is not None else None
-    a.stats = stats.data_ptr() if stats is not None else None
-    if grad is not None:
-        a.grad, a.grad_stride = grad.data_ptr(), x.shape[1]
-    return a
+    return _lib.DistillArgs(logits_args(x), values.data_ptr(), indices.data_ptr(), values.shape[-1], _TYPES[values.dtype],
+                            temperature, None if weight is None else weight.data_ptr(),
+                            0 if weight is None else weight.stride(0), None if loss is None else loss.data_ptr(),
+                            None if stats is None else stats.data_ptr(), None if grad is None else grad.data_ptr(),
+                            x.shape[1])
 
 
 def _forward(x, values, indices, temperature, lead, with_stats):
-    loss = torch.empty(lead, device=x.device, dtype=torch.float32)
-    stats = torch.empty((x.shape[0], 4), device=x.device, dtype=torch.float32) if with_stats else None
+    loss = x.new_empty(lead, dtype=torch.float32)
+    stats = x.new_empty((x.shape[0], 4), dtype=torch.float32) if with_stats else None
     _lib.launch('sq_distill_forward', x.device, C.byref(_args(x, values, indices, temperature, loss=loss, stats=stats)))
     return loss, stats
 
@@ -99,7 +93,7 @@ class _DistillationLoss(torch.autograd.Function):
     def backward(ctx, grad_loss):
         logits, values, indices, stats = ctx.saved_tensors
         x = logits_rows(logits)
-        grad = torch.empty(logits.shape, device=x.device, dtype=x.dtype)
+        grad = x.new_empty(logits.shape)
         a = _args(x, values, indices, ctx.temperature, weight=_row_weights(grad_loss), stats=stats, grad=grad)
         _lib.launch('sq_distill_backward', x.device, C.byref(a))
         return grad, None, None, None
@@ -126,8 +120,8 @@ def distillation_loss_grad(logits, values, indices, temperature=1.0, weight=None
                 or weight.device != x.device:
             raise ValueError(f'weight must be a float32 tensor of shape {tuple(lead)} on {x.device}')
         weight = _row_weights(weight)
-    loss = torch.empty(lead, device=x.device, dtype=torch.float32)
-    grad = torch.empty(logits.shape, device=x.device, dtype=x.dtype)
+    loss = x.new_empty(lead, dtype=torch.float32)
+    grad = x.new_empty(logits.shape)
     _lib.launch('sq_distill_loss_grad', x.device,
                 C.byref(_args(x, values, indices, temperature, weight=weight, loss=loss, grad=grad)))
     return loss, grad

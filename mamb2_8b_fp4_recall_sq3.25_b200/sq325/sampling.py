@@ -27,27 +27,30 @@ def logits_rows(logits):
     dimension is contiguous (a copy only where its layout has no single row stride)."""
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _TYPES or not logits.is_cuda:
         raise ValueError('Logits must be a CUDA FP16, BF16 or FP32 tensor')
-    if logits.ndim == 0 or not 1 <= logits.shape[-1] <= MAX_VOCAB:
+    shape = logits.shape
+    if not shape or not 1 <= shape[-1] <= MAX_VOCAB:
         raise ValueError(f'Logits must be [..., vocab] with vocab in [1, {MAX_VOCAB}]')
-    x = logits if logits.ndim == 2 else logits.reshape(-1, logits.shape[-1])
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+    x = logits if len(shape) == 2 else logits.reshape(-1, shape[-1])
+    return x if x.stride(1) == 1 or shape[-1] == 1 else x.contiguous()
 
 
 def logits_args(x):
     """ctypes view of rows that logits_rows() returned."""
-    return _lib.Logits(x.data_ptr(), x.stride(0), x.shape[0], x.shape[1], _TYPES[x.dtype])
+    rows, vocab = x.shape
+    return _lib.Logits(x.data_ptr(), x.stride(0), rows, vocab, _TYPES[x.dtype])
 
 
-def _setting(name, value, x, lead, dtype, check):
-    """(tensor or None, number): a tensor holds one value a row, a number stands for all rows."""
-    if isinstance(value, torch.Tensor):
-        if value.shape != lead or value.dtype != dtype or value.device != x.device:
-            raise ValueError(f'{name} must be a number or a {dtype} tensor of shape {tuple(lead)} on {x.device}')
-        return value.contiguous(), 0
-    if isinstance(value, bool) or not isinstance(value, int if dtype == torch.int32 else (int, float)) \
-            or not check(value):
+def _per_row(name, value, x, lead, dtype):
+    """A tensor with one setting a row."""
+    if value.shape != lead or value.dtype != dtype or value.device != x.device:
+        raise ValueError(f'{name} must be a number or a {dtype} tensor of shape {tuple(lead)} on {x.device}')
+    return value.contiguous()
+
+
+def _number(name, value, kinds, low, high):
+    if isinstance(value, bool) or not isinstance(value, kinds) or not low <= value <= high:
         raise ValueError(f'{name} is out of range: {value!r}')
-    return None, value
+    return value
 
 
 def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -66,12 +69,25 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             or uniform.device != x.device:
         raise ValueError(f'uniform must be a float32 tensor of shape {tuple(lead)} on {x.device}')
     uniform = uniform.contiguous()
-    t, t_all = _setting('temperature', temperature, x, lead, torch.float32, lambda v: 0 <= v < float('inf'))
-    k, k_all = _setting('top_k', top_k, x, lead, torch.int32, lambda v: 0 <= v < 2 ** 31)
-    p, p_all = _setting('top_p', top_p, x, lead, torch.float32, lambda v: 0 < v <= 1)
-    q, q_all = _setting('min_p', min_p, x, lead, torch.float32, lambda v: 0 <= v <= 1)
-    tokens = torch.empty(lead, device=x.device, dtype=torch.long)
-    a = _lib.SampleArgs(logits_args(x), uniform.data_ptr(), *(v.data_ptr() if v is not None else None for v in (t, k, p, q)),
-                        t_all, k_all, p_all, q_all, tokens.data_ptr())
+    t = k = p = q = None
+    if isinstance(temperature, torch.Tensor):
+        t, temperature = _per_row('temperature', temperature, x, lead, torch.float32), 0.0
+    else:
+        _number('temperature', temperature, (int, float), 0, 3.4e38)
+    if isinstance(top_k, torch.Tensor):
+        k, top_k = _per_row('top_k', top_k, x, lead, torch.int32), 0
+    else:
+        _number('top_k', top_k, int, 0, 2 ** 31 - 1)
+    if isinstance(top_p, torch.Tensor):
+        p, top_p = _per_row('top_p', top_p, x, lead, torch.float32), 0.0
+    elif _number('top_p', top_p, (int, float), 0, 1) == 0:
+        raise ValueError('top_p is out of range: 0')
+    if isinstance(min_p, torch.Tensor):
+        q, min_p = _per_row('min_p', min_p, x, lead, torch.float32), 0.0
+    else:
+        _number('min_p', min_p, (int, float), 0, 1)
+    tokens = torch.empty_like(uniform, dtype=torch.long)
+    a = _lib.SampleArgs(logits_args(x), uniform.data_ptr(), *(None if v is None else v.data_ptr() for v in (t, k, p, q)),
+                        temperature, top_k, top_p, min_p, tokens.data_ptr())
     _lib.launch('sq_sample', x.device, C.byref(a))
     return tokens
