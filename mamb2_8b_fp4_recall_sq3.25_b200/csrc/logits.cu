@@ -13,7 +13,7 @@
 // distributed shared memory.
 //
 // Few tokens wanted (top_logits, top-k up to 256, greedy): every thread streams its units of 16 bytes and
-// keeps eight maxima, of every eighth unit each.  The r-th largest of a CTA's 2048 maxima, r = k / CTAs, to
+// keeps eight maxima, of every eighth unit each.  The r-th largest of a CTA's maxima, r = k / CTAs, to
 // 16 bits of its key, is reached by r logits at least; the least of the CTAs' bounds by k logits of the
 // row, and by few more.  Only the units under a maximum that reaches it are read again (from L2), and
 // CTA 0 sorts what is not below it.  Rows where that is too much (thousands of equal logits at the
@@ -31,32 +31,33 @@
 namespace sq {
 namespace {
 
-constexpr int NT = 256, NW = NT / 32;
+constexpr int kTopThreads = 256;
 typedef unsigned long long u64;
 
 // Histogram over rint(-7.96875 log2 y): 256 steps hold every weight but 0 (y > 2^-32).  Four copies
-// of it, by lane, so that fewer lanes meet in one word.  A word sums the low 18 bits of at most
-// NT / 4 threads x 136 elements: < 2^32.  The upper 13 bits are not 0 for y >= 2^-13 only, the first 105 steps.
+// of it, by lane, so that fewer lanes meet in one word: a word sums the low 18 bits of at most a quarter of
+// the threads times the elements of one, < 2^14 (a part has at most 32776 elements).
+// The upper 13 bits are not 0 for y >= 2^-13 only, the first 105 steps.
 constexpr int kSteps = 256, kCols = 4, kLowBits = 18, kHighSteps = 106;
 constexpr float kPerOctave = 7.96875f;
 constexpr int kFine = 128;                       // entries of the narrowing histograms, laid out alike
 constexpr int kWorkBytes = (kSteps + kHighSteps) * kCols * 4;
 constexpr int kMembers = kHighSteps * kCols * 4 / 2;           // members of a step held as 16-bit positions
 constexpr int kList = 2048;                      // listed logits of a CTA
-constexpr int kGroups = 8 * NT;                  // maxima of a CTA
-constexpr int kListBytes = kList * 8 + kGroups * 2;
+constexpr int kMaxima = 8;                       // of a thread
+template <int NT> constexpr int kListBytes = kList * 8 + kMaxima * NT * 2;
 constexpr int kMaxListed = kList / 8;            // top-k up to this many goes by the list
 
 struct Cut { float x; int last; };               // kept: above x, or equal and column <= last
 
 struct Shared {
   u64 slot[2][8];
-  u64 part[NW];
-  float fpart[NW];
+  u64 part[16];                                  // a warp's each
+  float fpart[16];
   u64 sums[2][kSteps];                           // this CTA's histogram, and the one before
   u64 found_above, found_mine, found_need;
   int found, count, pick;
-  uint2 counts[2][NW];
+  uint2 counts[2][16];
   int groups;
 };
 
@@ -66,8 +67,11 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
   return v;
 }
 
-// The CTAs of a cluster and what they exchange.
+// The CTAs of a cluster, NT threads each, and what they exchange.
+template <int NT>
 struct Team {
+  static constexpr int NW = NT / 32;
+  static_assert(NW <= 16, "Shared has room for 16 warps");
   Shared& s;
   uint32_t rank, size;
   int tid, phase;
@@ -138,12 +142,12 @@ struct Team {
 
 // The k largest logits of a row.  Items are key << 32 | ~column: distinct, and larger
 // ones come first in the order.
-template <typename T>
+template <typename T, int NT>
 struct Listing {
-  static constexpr int NV = 4, G = kGroups / NT;            // units of a batch in column order; maxima of a thread
-  Team& t;
+  static constexpr int NV = 4, G = kMaxima;                 // units of a batch in column order; maxima of a thread
+  Team<NT>& t;
   Span<T> span;
-  u64* list;                                     // [kList], with room for [kGroups] 16-bit numbers behind it
+  u64* list;                                     // [kList], with room for [kMaxima NT] 16-bit numbers behind it
   int k;
   float bound;
   u64 least;                                     // items not above it are no longer wanted
@@ -372,13 +376,13 @@ struct Listing {
   // list[0 .. n) by falling value.  Few items are placed by counting the larger ones, which takes two
   // barriers; more by a bitonic network.
   __device__ void sort(int n) {
-    if (n <= 2 * NT) {
+    if (n <= 512) {
       __syncthreads();
       u64 item[2];
       int place[2] = {0, 0};
 #pragma unroll
       for (int a = 0; a < 2; ++a) item[a] = t.tid + a * NT < n ? list[t.tid + a * NT] : 0;
-      const int both = n > NT;
+      const bool both = n > NT;
 #pragma unroll 4
       for (int j = 0; j < n; ++j) {
         const u64 other = list[j];
@@ -429,22 +433,24 @@ __device__ __forceinline__ void add_light(uint32_t address, uint32_t w, float t)
 }
 
 // One CTA's part of a row in shared memory.
-template <typename T>
-struct Row : Team {
+template <typename T, int NT>
+struct Row : Team<NT> {
+  using Base = Team<NT>;
   Span<T> d;
   unsigned char* work;                           // histogram and members
   Unit<T>* unit;
   int turn = 0;                                  // of s.sums
-  using Team::s; using Team::tid; using Team::rank; using Team::size;
+  using Base::s; using Base::tid; using Base::rank; using Base::size; using Base::barrier; using Base::exchange; using Base::got;
+  static constexpr int NW = NT / 32;
 
-  __device__ Row(const Team& t, const Span<T>& d, unsigned char* dyn)
-      : Team(t), d(d), work(dyn), unit(reinterpret_cast<Unit<T>*>(dyn + kWorkBytes)) {
+  __device__ Row(const Base& t, const Span<T>& d, unsigned char* dyn)
+      : Base(t), d(d), work(dyn), unit(reinterpret_cast<Unit<T>*>(dyn + kWorkBytes)) {
     for (int i = tid; i < d.n; i += NT) {
       if (i >= d.lo && i < d.hi) cp_async16(unit + i, d.p + d.col(i, 0));
       else unit[i] = d.ragged(i);
     }
     cp_async_wait_all();                         // each thread's own units
-    ready();
+    this->ready();
   }
 
   // f(unit, exponents) over this thread's units.
@@ -588,11 +594,13 @@ struct Row : Team {
     turn ^= 1;
     const u64* sums = s.sums[turn];
     u64* total = reinterpret_cast<u64*>(work);   // the histogram's words have been read
-    s.sums[turn][tid] = mine;
+    if (tid < kSteps) s.sums[turn][tid] = mine;
     barrier();
-    u64 all = 0;
-    for (int r = 0; r < (int)size; ++r) all += remote_load(remote_smem(&sums[tid], r));
-    total[tid] = all;
+    if (tid < kSteps) {
+      u64 all = 0;
+      for (int r = 0; r < (int)size; ++r) all += remote_load(remote_smem(&sums[tid], r));
+      total[tid] = all;
+    }
     __syncthreads();
     if (tid < 32) {                              // eight entries a lane
       u64 sum = 0, own = 0;
@@ -629,7 +637,7 @@ struct Row : Team {
   // kept_here: this CTA's share of the weight that is kept.  PLAIN: every element is kept and w is weight_of.
   template <bool PLAIN, typename K, typename W, typename N>
   __device__ bool select(K kept, W w, Exponent e, N need_of, Cut& cut, u64& kept_here) {
-    static_assert(kSteps == NT, "a thread per step");
+    static_assert(kSteps <= NT, "a thread per step");
     constexpr int SH = std::is_same<T, __half>::value ? 13 : std::is_same<T, __nv_bfloat16>::value ? 16 : 0;
     constexpr uint32_t kLow = (1u << kLowBits) - 1;
     uint32_t* low = reinterpret_cast<uint32_t*>(work);
@@ -683,7 +691,7 @@ struct Row : Team {
     __syncthreads();
     u64 mine = 0;
     for (int i = 0; i < kCols; ++i) {
-      mine += low[tid * kCols + i];
+      if (tid < kSteps) mine += low[tid * kCols + i];
       if (tid < kHighSteps) mine += (u64)high[tid * kCols + i] << kLowBits;
     }
     u64 above = 0, mine_above = 0;
@@ -782,11 +790,11 @@ __device__ __forceinline__ u64 draw(double u, u64 total) {
   return t < 0 ? 0 : ((u64)t >= total ? total - 1 : (u64)t);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 768 / NT + (NT > 256)) sample_kernel(const SampleParams P) {
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ Shared s;
-  Team team(s);
+  Team<NT> team(s);
   const Span<T> span(P.x, blockIdx.x / team.size, team.rank, team.size);
   const int row = blockIdx.x / team.size, tid = threadIdx.x;
   const float temperature = P.temperature ? P.temperature[row] : P.temperature_all;
@@ -806,14 +814,14 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
 
   if (top_k > 0 && top_k <= kMaxListed) {
     u64* list = reinterpret_cast<u64*>(dyn);
-    Listing<T> l{team, span, list, top_k};
+    Listing<T, NT> l{team, span, list, top_k};
     const int n = min(top_k, l.gather());
     if (team.rank != 0) return;
     if (n <= 1 || greedy) {
       if (tid == 0) P.tokens[row] = n ? (long long)~(uint32_t)list[0] : -1;
       return;
     }
-    static_assert(kMaxListed == NT, "a thread per listed token");
+    static_assert(kMaxListed <= NT, "a thread per listed token");
     const u64 item = tid < n ? list[tid] : 0;
     const float x = key_logit((uint32_t)(item >> 32));
     e.m = key_logit((uint32_t)(list[0] >> 32));
@@ -840,7 +848,7 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
     return;
   }
 
-  Row<T> r(team, span, dyn);
+  Row<T, NT> r(team, span, dyn);
   e.m = r.row_max(r.own_max());
   if (e.m == -INFINITY) {
     if (r.rank == 0 && tid == 0) P.tokens[row] = -1;
@@ -894,12 +902,13 @@ __global__ void __launch_bounds__(NT, 3) sample_kernel(const SampleParams P) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(NT, 4) top_kernel(const TopParams P) {
+__global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const TopParams P) {
+  constexpr int NT = kTopThreads;
   __shared__ Shared s;
-  __shared__ u64 list[kListBytes / 8];
-  Team team(s);
+  __shared__ u64 list[kListBytes<NT> / 8];
+  Team<NT> team(s);
   const Span<T> span(P.x, blockIdx.x / team.size, team.rank, team.size);
-  Listing<T> l{team, span, list, P.k};
+  Listing<T, NT> l{team, span, list, P.k};
   const int n = l.gather(), row = blockIdx.x / team.size;
   if (team.rank != 0) return;
   T* values = reinterpret_cast<T*>(P.values) + (long long)row * P.k;
@@ -912,13 +921,13 @@ __global__ void __launch_bounds__(NT, 4) top_kernel(const TopParams P) {
 }
 
 template <typename K, typename P>
-int launch_clusters(K kernel, const P& params, int size, size_t smem, cudaStream_t st) {
+int launch_clusters(K kernel, const P& params, int size, int threads, size_t smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
   cfg.gridDim = dim3((unsigned)params.x.rows * size);
-  cfg.blockDim = dim3(NT);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -938,20 +947,30 @@ int by_type(int type, F f) {
 
 }  // namespace
 
+template <typename T, int NT>
+int launch_sample_threads(const SampleParams& P, int size, cudaStream_t st) {
+  size_t smem = (size_t)kWorkBytes + (size_t)((row_units(P.x) + size - 1) / size) * 16;
+  if (smem < kListBytes<NT>) smem = kListBytes<NT>;
+  const auto kernel = sample_kernel<T, NT>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess)
+    return launch_status();
+  return launch_clusters(kernel, P, size, NT, smem, st);
+}
+
 int launch_sample(const SampleParams& P, cudaStream_t st) {
-  // As many CTAs a row as keep its part within 64 KB, three on an SM; few rows take more, down to a
-  // unit a thread.
+  // As many CTAs a row as keep its part within 64 KB; few rows take more, down to a unit a thread.
   const int units = row_units(P.x);
   int size = 1;
   while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
-  while (size < 8 && P.x.rows * size < 2 * 148 && units > size * NT) size *= 2;
-  size_t smem = (size_t)kWorkBytes + (size_t)((units + size - 1) / size) * 16;
-  if (smem < kListBytes) smem = kListBytes;
+  while (size < 8 && P.x.rows * size < 2 * 148 && units > size * 256) size *= 2;
+  // Rows that are all on the GPU at once and are not just listed want threads: 512 (one row of 256,000 flat fp16
+  // logits, top-p: 49 us, with 256 threads 74).  Many rows want three CTAs on an SM: 256 (512 rows of bf16, top-p:
+  // 417 us, with 512 threads 464); so do lists (top-k 50 of one row: 9.5 us, with 512 threads 11.5).
+  const bool listed = !P.top_k && P.top_k_all > 0 && P.top_k_all <= kMaxListed;
   return by_type(P.x.type, [&](auto t) {
-    const auto kernel = sample_kernel<decltype(t)>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess)
-      return launch_status();
-    return launch_clusters(kernel, P, size, smem, st);
+    using T = decltype(t);
+    if (P.x.rows * size <= 2 * 148 && !listed && units > size * 256) return launch_sample_threads<T, 512>(P, size, st);
+    return launch_sample_threads<T, 256>(P, size, st);
   });
 }
 
@@ -960,8 +979,8 @@ int launch_top_logits(const TopParams& P, cudaStream_t st) {
   // their lists fit that of the first.
   const int units = row_units(P.x);
   int size = 1;
-  while (size < 8 && P.x.rows * size < 4 * 148 && units > size * 2 * NT && 2 * size * P.k <= kList) size *= 2;
-  return by_type(P.x.type, [&](auto t) { return launch_clusters(top_kernel<decltype(t)>, P, size, 0, st); });
+  while (size < 8 && P.x.rows * size < 4 * 148 && units > size * 2 * kTopThreads && 2 * size * P.k <= kList) size *= 2;
+  return by_type(P.x.type, [&](auto t) { return launch_clusters(top_kernel<decltype(t)>, P, size, kTopThreads, 0, st); });
 }
 
 }  // namespace sq
