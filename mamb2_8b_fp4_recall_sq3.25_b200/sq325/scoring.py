@@ -171,10 +171,15 @@ def evaluate_ppl(execution, windows, batch_windows=16, rank=0, world=1, group=No
 
 
 @torch.no_grad()
-def generate(execution, prompt_ids, max_new_tokens, eos_token_id=None, graphs=False, persistent=True):
-    """Greedy decode: returns int64 [batch, n_generated] (n <= max_new_tokens).
+def generate(execution, prompt_ids, max_new_tokens, eos_token_id=None, graphs=False, persistent=True, sampling=None,
+             uniform=None, generator=None):
+    """Decode loop: returns int64 [batch, n_generated] (n <= max_new_tokens).
 
-    graphs=True runs the token loop without host synchronisation (an EOS stop is then
+    Greedy by default.  sampling = dict(temperature=, top_k=, top_p=, min_p=) draws every token
+    (sampling.sample; numbers, or tensors [batch] with a setting per request) from `uniform`, fp32
+    [max_new_tokens, batch] on the device, or from numbers that `generator` gives.
+
+    graphs=True runs the greedy token loop without host synchronisation (an EOS stop is then
     applied after the fact by truncation): at batch 1 with the factored-scale projections
     one persistent kernel launch per token (persistent=True), otherwise a captured CUDA
     graph per token."""
@@ -182,6 +187,18 @@ def generate(execution, prompt_ids, max_new_tokens, eos_token_id=None, graphs=Fa
     prompt = torch.as_tensor(prompt_ids, dtype=torch.long).to(dev)
     if prompt.ndim == 1:
         prompt = prompt[None]
+    if sampling is None:
+        if uniform is not None or generator is not None:
+            raise ValueError('uniform and generator belong to sampling')
+        pick = lambda step, hidden: execution.greedy(hidden)
+    else:
+        if graphs:
+            raise ValueError('The graph and persistent decode loops are greedy: use graphs=False with sampling')
+        if uniform is None:
+            uniform = torch.rand((max_new_tokens, prompt.shape[0]), device=dev, generator=generator)
+        elif generator is not None or tuple(uniform.shape) != (max_new_tokens, prompt.shape[0]):
+            raise ValueError('uniform must be [max_new_tokens, batch], without a generator')
+        pick = lambda step, hidden: execution.sample(hidden, uniform[step], **sampling)
     hidden = execution.backbone(prompt.contiguous(), reset=True)[:, -1]
     if graphs:
         tok = execution.greedy(hidden).clone()
@@ -202,7 +219,7 @@ def generate(execution, prompt_ids, max_new_tokens, eos_token_id=None, graphs=Fa
         return seq
     out = []
     for step in range(max_new_tokens):
-        tok = execution.greedy(hidden)
+        tok = pick(step, hidden)
         out.append(tok)
         if step + 1 == max_new_tokens:
             break

@@ -15,9 +15,10 @@ import weakref
 
 import torch
 
-from . import _lib
+from . import _lib, fp4
 from .codec import allocate_state, layout_descriptor, layout_index, validate_state
 from .model import D_MODEL, D_XBC
+from .sampling import sample
 
 _OWNERS = weakref.WeakKeyDictionary()
 
@@ -275,6 +276,25 @@ class PredictorState:
         _lib.call('sq_model_greedy', self._handle, _lib.ptr(h2), rows, _lib.ptr(logits), _lib.ptr(tok),
                   _lib.stream_ptr())
         return tok
+
+    @torch.no_grad()
+    def logits(self, hidden):
+        """fp16 logits [..., vocab] of hidden [..., 4096] with the exactly decoded lm_head (the
+        projection that score() runs), for a teacher's record (distillation.top_logits)."""
+        return fp4.linear(self.model.lm_head, hidden)
+
+    @torch.no_grad()
+    def sample(self, hidden, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """One drawn token per hidden row: lm_head (at most 64 rows as greedy(), more as logits()) and
+        sampling.sample with its settings.  uniform: fp32 [rows]; returns int64 [rows]."""
+        h2 = hidden.reshape(-1, D_MODEL).contiguous()
+        rows = h2.shape[0]
+        if rows > 64:
+            logits = self.logits(h2)
+        else:
+            logits = torch.empty((rows, self.model.vocab), device=self.device, dtype=torch.float16)
+            self.greedy(h2, logits=logits)
+        return sample(logits, uniform, temperature, top_k, top_p, min_p)
 
     # ------------------------------------------------------------------ graphed decode
     @torch.no_grad()
