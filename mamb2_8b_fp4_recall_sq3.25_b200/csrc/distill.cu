@@ -600,44 +600,23 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillPara
   }
 }
 
-// A cluster of `size` CTAs a row; as many as run at once for a kernel that steps through the rows.
-template <typename K>
-int launch_clusters(K kernel, const DistillParams& P, bool steps, int size, int threads, size_t smem, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)P.x.rows * size);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (steps && P.x.rows * size > 148) {
-    int clusters = 0;
-    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) return launch_status();
-    if (clusters > 0 && clusters < P.x.rows) cfg.gridDim = dim3((unsigned)clusters * size);
-  }
-  cudaLaunchKernelEx(&cfg, kernel, P);
-  return launch_status();
-}
-
 template <typename T>
 int launch_loss(const DistillParams& P, cudaStream_t st) {
   // long parts stream best: more CTAs a row only until there are three for each SM
   const int units = row_units(P.x);
   int size = 1;
-  while (size < 8 && P.x.rows * size < 3 * 148 && units > size * kLossThreads * kLossUnits) size *= 2;
-  return launch_clusters(loss_kernel<T>, P, false, size, kLossThreads, 0, st);
+  while (size < 8 && P.x.rows * size < 3 * kSms && units > size * kLossThreads * kLossUnits) size *= 2;
+  return launch_clusters(loss_kernel<T>, P, size, kLossThreads, 0, st);
 }
 
 template <typename T, int DW>
 int launch_rows(const DistillParams& P, int size, cudaStream_t st) {
   const size_t smem = 2 * RowRecord<T>::bytes((P.k + 3) & ~3) + (size_t)((row_units(P.x) + size - 1) / size) * 16;
   const auto kernel = row_kernel<T, DW>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess)
-    return launch_status();
-  return launch_clusters(kernel, P, true, size, DW * 32 + 32, smem, st);
+  static std::atomic<uint64_t> done{0};
+  if (allow_shared(kernel, 200 * 1024, done) != cudaSuccess) return launch_status();
+  // up to two CTAs an SM one row is a cluster's work; beyond, clusters step through the rows
+  return launch_clusters(kernel, P, size, DW * 32 + 32, smem, st, true, 2 * kSms);
 }
 
 template <typename T>
@@ -647,7 +626,7 @@ int launch_loss_grad(const DistillParams& P, cudaStream_t st) {
   const int units = row_units(P.x);
   int size = 1;
   while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
-  while (size < 8 && P.x.rows * size < 2 * 148 && units > size * 256) size *= 2;
+  while (size < 8 && P.x.rows * size < 2 * kSms && units > size * 256) size *= 2;
   if constexpr (sizeof(T) == 4)
     if ((units + size - 1) / size > 6144) return launch_rows<T, 16>(P, size, st);
   return launch_rows<T, 8>(P, size, st);

@@ -920,21 +920,6 @@ __global__ void __launch_bounds__(kTopThreads, 4) top_kernel(const TopParams P) 
   }
 }
 
-template <typename K, typename P>
-int launch_clusters(K kernel, const P& params, int size, int threads, size_t smem, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = size; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3((unsigned)params.x.rows * size);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kernel, params);
-  return launch_status();
-}
 template <typename F>
 int by_type(int type, F f) {
   switch (type) {
@@ -952,8 +937,8 @@ int launch_sample_threads(const SampleParams& P, int size, cudaStream_t st) {
   size_t smem = (size_t)kWorkBytes + (size_t)((row_units(P.x) + size - 1) / size) * 16;
   if (smem < kListBytes<NT>) smem = kListBytes<NT>;
   const auto kernel = sample_kernel<T, NT>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024) != cudaSuccess)
-    return launch_status();
+  static std::atomic<uint64_t> done{0};
+  if (allow_shared(kernel, 160 * 1024, done) != cudaSuccess) return launch_status();
   return launch_clusters(kernel, P, size, NT, smem, st);
 }
 
@@ -962,14 +947,14 @@ int launch_sample(const SampleParams& P, cudaStream_t st) {
   const int units = row_units(P.x);
   int size = 1;
   while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
-  while (size < 8 && P.x.rows * size < 2 * 148 && units > size * 256) size *= 2;
+  while (size < 8 && P.x.rows * size < 2 * kSms && units > size * 256) size *= 2;
   // Rows that are all on the GPU at once and are not just listed want threads: 512 (one row of 256,000 flat fp16
   // logits, top-p: 49 us, with 256 threads 74).  Many rows want three CTAs on an SM: 256 (512 rows of bf16, top-p:
   // 417 us, with 512 threads 464); so do lists (top-k 50 of one row: 9.5 us, with 512 threads 11.5).
   const bool listed = !P.top_k && P.top_k_all > 0 && P.top_k_all <= kMaxListed;
   return by_type(P.x.type, [&](auto t) {
     using T = decltype(t);
-    if (P.x.rows * size <= 2 * 148 && !listed && units > size * 256) return launch_sample_threads<T, 512>(P, size, st);
+    if (P.x.rows * size <= 2 * kSms && !listed && units > size * 256) return launch_sample_threads<T, 512>(P, size, st);
     return launch_sample_threads<T, 256>(P, size, st);
   });
 }
@@ -979,7 +964,7 @@ int launch_top_logits(const TopParams& P, cudaStream_t st) {
   // their lists fit that of the first.
   const int units = row_units(P.x);
   int size = 1;
-  while (size < 8 && P.x.rows * size < 4 * 148 && units > size * 2 * kTopThreads && 2 * size * P.k <= kList) size *= 2;
+  while (size < 8 && P.x.rows * size < 4 * kSms && units > size * 2 * kTopThreads && 2 * size * P.k <= kList) size *= 2;
   return by_type(P.x.type, [&](auto t) { return launch_clusters(top_kernel<decltype(t)>, P, size, kTopThreads, 0, st); });
 }
 

@@ -67,13 +67,6 @@ def _args(x, values, indices, temperature, weight=None, loss=None, stats=None, g
                             x.shape[1])
 
 
-def _forward(x, values, indices, temperature, lead, with_stats):
-    loss = x.new_empty(lead, dtype=torch.float32)
-    stats = x.new_empty((x.shape[0], 4), dtype=torch.float32) if with_stats else None
-    _lib.launch('sq_distill_forward', x.device, C.byref(_args(x, values, indices, temperature, loss=loss, stats=stats)))
-    return loss, stats
-
-
 def _row_weights(weight):
     """Per-row factors as a vector the kernels step through: a broadcast one keeps its stride of 0."""
     return weight if weight.ndim == 1 else weight.reshape(-1)
@@ -83,18 +76,22 @@ class _DistillationLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, values, indices, temperature):
         x, values, indices = _checked(logits, values, indices, temperature)
-        loss, stats = _forward(x, values, indices, temperature, logits.shape[:-1], True)
-        ctx.save_for_backward(logits, values, indices, stats)
-        ctx.temperature = temperature
+        loss = x.new_empty(logits.shape[:-1], dtype=torch.float32)
+        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
+        ctx.save_for_backward(x, values, indices, stats)
+        ctx.shape = logits.shape
+        ctx.args = _args(x, values, indices, temperature, loss=loss, stats=stats)     # backward's too
+        _lib.launch('sq_distill_forward', x.device, C.byref(ctx.args))
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        logits, values, indices, stats = ctx.saved_tensors
-        x = logits_rows(logits)
-        grad = x.new_empty(logits.shape)
-        a = _args(x, values, indices, ctx.temperature, weight=_row_weights(grad_loss), stats=stats, grad=grad)
+        x = ctx.saved_tensors[0]                 # raises if one of them was changed in place
+        weight = _row_weights(grad_loss)
+        grad = x.new_empty(ctx.shape)
+        a = ctx.args
+        a.weight, a.weight_stride, a.grad = weight.data_ptr(), weight.stride(0), grad.data_ptr()
         _lib.launch('sq_distill_backward', x.device, C.byref(a))
         return grad, None, None, None
 
@@ -106,7 +103,9 @@ def distillation_loss(logits, values, indices, temperature=1.0):
     if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return _DistillationLoss.apply(logits, values, indices, temperature)
     x, values, indices = _checked(logits, values, indices, temperature)
-    return _forward(x, values, indices, temperature, logits.shape[:-1], False)[0]
+    loss = x.new_empty(logits.shape[:-1], dtype=torch.float32)
+    _lib.launch('sq_distill_forward', x.device, C.byref(_args(x, values, indices, temperature, loss=loss)))
+    return loss
 
 
 def distillation_loss_grad(logits, values, indices, temperature=1.0, weight=None):
