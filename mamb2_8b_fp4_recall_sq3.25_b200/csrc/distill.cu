@@ -85,6 +85,36 @@ __device__ __forceinline__ void store_pair(Unit<__nv_bfloat16>& o, int v, float2
   reinterpret_cast<__nv_bfloat162*>(&o.q)[v / 2] = __float22bfloat162_rn(p);
 }
 __device__ __forceinline__ void store_pair(Unit<float>& o, int v, float2 p) { o.v[v] = p.x; o.v[v + 1] = p.y; }
+// Stores the units of a warp's first n lanes one behind the other from `to` on.  The gradient's rows may lie
+// otherwise in their 16 bytes than the logits' rows: then (`vec` false) the units pass through `buf` (512
+// bytes of shared memory a warp) and leave it in whole units of the destination, whose ends go element by element.
+template <typename T>
+__device__ __forceinline__ void store_units(T* to, const Unit<T>& o, int n, bool vec, uint4* buf) {
+  const int lane = threadIdx.x & 31;
+  if (vec) {
+    if (lane < n) reinterpret_cast<uint4*>(to)[lane] = o.q;
+    return;
+  }
+  __syncwarp();
+  buf[lane] = o.q;
+  __syncwarp();
+  const int head = (16 - (int)((uintptr_t)to & 15)) / (int)sizeof(T);        // elements up to the first whole unit
+  if (lane < n - 1) {
+    const uint32_t a = (uint32_t)__cvta_generic_to_shared(buf) + 16u * lane + head * (uint32_t)sizeof(T), word = a & ~3u;
+    uint32_t w[5];
+#pragma unroll
+    for (int b = 0; b < 5; ++b) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[b]) : "r"(word + 4u * b));
+    if (sizeof(T) == 2 && (a & 2)) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) w[b] = __funnelshift_r(w[b], w[b + 1], 16);
+    }
+    *reinterpret_cast<uint4*>(to + head + lane * kUnit<T>) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (lane < kUnit<T> && n > 0) {
+    const int e = lane < head ? lane : (n - 1) * kUnit<T> + lane;
+    to[e] = reinterpret_cast<const T*>(buf)[e];
+  }
+}
 // Copies n elements from shared memory to `to` in whole 16-byte units of the destination, its ends element
 // by element.
 template <typename T, int NT>
@@ -222,11 +252,11 @@ struct Record {
   }
 };
 
-constexpr int kLossThreads = 256, kLossUnits = 8;
+constexpr int kLossUnits = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const DistillParams P) {
-  constexpr int NT = kLossThreads, NV = kLossUnits, NW = NT / 32;
+template <typename T, int NT, int N>
+__global__ void __launch_bounds__(NT, 1024 / NT) loss_kernel(const DistillParams P) {
+  constexpr int NV = kLossUnits, NW = NT / 32;
   __shared__ Pairs<NW> pairs;
   __shared__ float part[2][NW];
   const uint32_t rank = cluster_rank(), size = cluster_size();
@@ -254,7 +284,7 @@ __global__ void __launch_bounds__(kLossThreads, 4) loss_kernel(const DistillPara
   };
   Unit<T> x[NV];
   load(x, span.lo);
-  Record<T, NT, kMaxRecord / NT> rec;
+  Record<T, NT, N> rec;
   if (rank == 0) {
     rec.fetch(P, row);
     rec.prepare(P, span.p, c, part, [](int) { return true; });
@@ -533,6 +563,7 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillPara
   constexpr int NT = kGradThreads, NV = kGradUnits;
   __shared__ __align__(16) int at[kMaxRecord];
   __shared__ float w[kMaxRecord];
+  __shared__ uint4 bounce[NT / 32][32];
   const int row = blockIdx.x / parts, part = blockIdx.x - row * parts, tid = threadIdx.x;
   const float c = kLog2e / P.temperature;
   const Span<T> span(P.x, row, part, parts);
@@ -567,16 +598,8 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillPara
     if (from) load(x, from);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int u = from + i * NT + tid;
-      if (u < units) {
-        const Unit<T> o = gradient(x[i], c, r, scale, any);
-        if (vec) {
-          reinterpret_cast<uint4*>(to)[u] = o.q;
-        } else {
-#pragma unroll
-          for (int v = 0; v < kUnit<T>; ++v) to[u * kUnit<T> + v] = o.v[v];
-        }
-      }
+      const int first = from + i * NT + tid - (tid & 31);
+      store_units(to + first * kUnit<T>, gradient(x[i], c, r, scale, any), max(0, min(32, units - first)), vec, bounce[tid >> 5]);
     }
   }
   const int col0 = max(0, span.col(0, 0)), col1 = min(span.vocab, span.col(span.n, 0));
@@ -602,11 +625,13 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillPara
 
 template <typename T>
 int launch_loss(const DistillParams& P, cudaStream_t st) {
-  // long parts stream best: more CTAs a row only until there are three for each SM
+  // long parts stream best: more CTAs a row only until there are three for each SM; short rows, many at
+  // once, take CTAs of two warps (LOSSNOTE)
   const int units = row_units(P.x);
+  if (units <= 1280 && P.x.rows > 4 * kSms && P.k <= 128) return launch_clusters(loss_kernel<T, 64, 2>, P, 1, 64, 0, st);
   int size = 1;
-  while (size < 8 && P.x.rows * size < 3 * kSms && units > size * kLossThreads * kLossUnits) size *= 2;
-  return launch_clusters(loss_kernel<T>, P, size, kLossThreads, 0, st);
+  while (size < 8 && P.x.rows * size < 3 * kSms && units > size * 256 * kLossUnits) size *= 2;
+  return launch_clusters(loss_kernel<T, 256, 4>, P, size, 256, 0, st);
 }
 
 template <typename T, int DW>
@@ -622,13 +647,15 @@ int launch_rows(const DistillParams& P, int size, cudaStream_t st) {
 template <typename T>
 int launch_loss_grad(const DistillParams& P, cudaStream_t st) {
   // As many CTAs a row as keep its part within 64 KB, three of eight data warps on an SM; few rows take
-  // more, down to a unit a thread.  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 16 warps.
+  // more, down to a unit a thread.  Short rows, many at once, are better served by more and smaller CTAs
+  // (GRADNOTE).  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 16 warps.
   const int units = row_units(P.x);
   int size = 1;
   while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
   while (size < 8 && P.x.rows * size < 2 * kSms && units > size * 256) size *= 2;
   if constexpr (sizeof(T) == 4)
     if ((units + size - 1) / size > 6144) return launch_rows<T, 16>(P, size, st);
+  if (size == 1 && units <= 1280 && P.x.rows > 4 * kSms) return launch_rows<T, 2>(P, size, st);
   return launch_rows<T, 8>(P, size, st);
 }
 

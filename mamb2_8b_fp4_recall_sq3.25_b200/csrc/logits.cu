@@ -933,38 +933,47 @@ int by_type(int type, F f) {
 }  // namespace
 
 template <typename T, int NT>
-int launch_sample_threads(const SampleParams& P, int size, cudaStream_t st) {
-  size_t smem = (size_t)kWorkBytes + (size_t)((row_units(P.x) + size - 1) / size) * 16;
+int launch_sample_threads(const SampleParams& P, int size, bool listed, cudaStream_t st) {
+  size_t smem = listed ? 0 : (size_t)kWorkBytes + (size_t)((row_units(P.x) + size - 1) / size) * 16;
   if (smem < kListBytes<NT>) smem = kListBytes<NT>;
   const auto kernel = sample_kernel<T, NT>;
   static std::atomic<uint64_t> done{0};
   if (allow_shared(kernel, 160 * 1024, done) != cudaSuccess) return launch_status();
   return launch_clusters(kernel, P, size, NT, smem, st);
 }
+// CTAs a row for listing k: one lists the fewest logits; more where the rows do not fill the GPU, as long as
+// their lists fit that of the first.
+int listing_size(const LogitsRows& x, int k) {
+  const int units = row_units(x);
+  int size = 1;
+  while (size < 8 && x.rows * size < 4 * kSms && units > size * 2 * kTopThreads && 2 * size * k <= kList) size *= 2;
+  return size;
+}
 
 int launch_sample(const SampleParams& P, cudaStream_t st) {
-  // As many CTAs a row as keep its part within 64 KB; few rows take more, down to a unit a thread.
+  // Where every row is known to be listed (one top-k for all), nothing but the lists is on chip.  Otherwise as many
+  // CTAs a row as keep its part within 64 KB; few rows take more, down to a unit a thread.
+  const bool listed = !P.top_k && P.top_k_all > 0 && P.top_k_all <= kMaxListed;
   const int units = row_units(P.x);
   int size = 1;
-  while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
-  while (size < 8 && P.x.rows * size < 2 * kSms && units > size * 256) size *= 2;
+  if (listed) {
+    size = listing_size(P.x, P.top_k_all);
+  } else {
+    while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
+    while (size < 8 && P.x.rows * size < 2 * kSms && units > size * 256) size *= 2;
+  }
   // Rows that are all on the GPU at once and are not just listed want threads: 512 (one row of 256,000 flat fp16
   // logits, top-p: 49 us, with 256 threads 74).  Many rows want three CTAs on an SM: 256 (512 rows of bf16, top-p:
   // 417 us, with 512 threads 464); so do lists (top-k 50 of one row: 9.5 us, with 512 threads 11.5).
-  const bool listed = !P.top_k && P.top_k_all > 0 && P.top_k_all <= kMaxListed;
+  const bool wide = !listed && P.x.rows * size <= 2 * kSms && units > size * 256;
   return by_type(P.x.type, [&](auto t) {
     using T = decltype(t);
-    if (P.x.rows * size <= 2 * kSms && !listed && units > size * 256) return launch_sample_threads<T, 512>(P, size, st);
-    return launch_sample_threads<T, 256>(P, size, st);
+    return wide ? launch_sample_threads<T, 512>(P, size, listed, st) : launch_sample_threads<T, 256>(P, size, listed, st);
   });
 }
 
 int launch_top_logits(const TopParams& P, cudaStream_t st) {
-  // One CTA lists the fewest logits; more where the rows do not fill the GPU, as long as
-  // their lists fit that of the first.
-  const int units = row_units(P.x);
-  int size = 1;
-  while (size < 8 && P.x.rows * size < 4 * kSms && units > size * 2 * kTopThreads && 2 * size * P.k <= kList) size *= 2;
+  const int size = listing_size(P.x, P.k);
   return by_type(P.x.type, [&](auto t) { return launch_clusters(top_kernel<decltype(t)>, P, size, kTopThreads, 0, st); });
 }
 
