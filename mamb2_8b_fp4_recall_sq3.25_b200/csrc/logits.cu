@@ -965,7 +965,8 @@ int launch_sample(const SampleParams& P, cudaStream_t st) {
   // Rows that are all on the GPU at once and are not just listed want threads: 512 (one row of 256,000 flat fp16
   // logits, top-p: 49 us, with 256 threads 74).  Many rows want three CTAs on an SM: 256 (512 rows of bf16, top-p:
   // 417 us, with 512 threads 464); so do lists (top-k 50 of one row: 9.5 us, with 512 threads 11.5).
-  const bool wide = !listed && P.x.rows * size <= 2 * kSms && units > size * 256;
+  // Parts of which one fits an SM (fp32 rows over 768 KB) want 512 as well.
+  const bool wide = !listed && ((P.x.rows * size <= 2 * kSms && units > size * 256) || units > size * 6144);
   return by_type(P.x.type, [&](auto t) {
     using T = decltype(t);
     return wide ? launch_sample_threads<T, 512>(P, size, listed, st) : launch_sample_threads<T, 256>(P, size, listed, st);
