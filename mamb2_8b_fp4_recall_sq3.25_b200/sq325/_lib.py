@@ -91,14 +91,16 @@ class Logits(C.Structure):
     _fields_ = [('data', p), ('row_stride', i64), ('rows', i32), ('vocab', i32), ('type', i32)]
 
 
+# sq_sample_args and sq_distill_args begin with an sq_logits; its fields stand for themselves here (the same
+# layout, one structure less to build per call)
 class SampleArgs(C.Structure):
-    _fields_ = [('logits', Logits), ('uniform', p), ('temperature', p), ('top_k', p), ('top_p', p), ('min_p', p),
+    _fields_ = [*Logits._fields_, ('uniform', p), ('temperature', p), ('top_k', p), ('top_p', p), ('min_p', p),
                 ('temperature_all', C.c_float), ('top_k_all', i32), ('top_p_all', C.c_float), ('min_p_all', C.c_float),
                 ('tokens', p)]
 
 
 class DistillArgs(C.Structure):
-    _fields_ = [('logits', Logits), ('values', p), ('indices', p), ('k', i32), ('value_type', i32),
+    _fields_ = [*Logits._fields_, ('values', p), ('indices', p), ('k', i32), ('value_type', i32),
                 ('temperature', C.c_float), ('weight', p), ('weight_stride', i64), ('loss', p), ('stats', p),
                 ('grad', p), ('grad_stride', i64)]
 

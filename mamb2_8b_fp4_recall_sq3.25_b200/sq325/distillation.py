@@ -20,7 +20,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .sampling import _TYPES, logits_args, logits_rows
+from .sampling import _TYPES, logits_fields, logits_rows
 
 __all__ = ['top_logits', 'distillation_loss', 'distillation_loss_grad']
 
@@ -36,7 +36,7 @@ def top_logits(logits, k):
         raise ValueError(f'k must be an integer in [1, min({MAX_RECORD}, vocab)]')
     values = x.new_empty((*logits.shape[:-1], k))
     indices = torch.empty_like(values, dtype=torch.int32)
-    _lib.launch('sq_top_logits', x.device, C.byref(logits_args(x)), k, values.data_ptr(), indices.data_ptr())
+    _lib.launch('sq_top_logits', x.device, C.byref(_lib.Logits(*logits_fields(x))), k, values.data_ptr(), indices.data_ptr())
     return values, indices
 
 
@@ -59,10 +59,10 @@ def _checked(logits, values, indices, temperature):
     return x, values.contiguous(), indices.contiguous()
 
 
-def _args(x, values, indices, temperature, weight=None, loss=None, stats=None, grad=None):
-    return _lib.DistillArgs(logits_args(x), values.data_ptr(), indices.data_ptr(), values.shape[-1], _TYPES[values.dtype],
+def _args(x, values, indices, temperature, loss, weight=None, stats=None, grad=None):
+    return _lib.DistillArgs(*logits_fields(x), values.data_ptr(), indices.data_ptr(), values.shape[-1], _TYPES[values.dtype],
                             temperature, None if weight is None else weight.data_ptr(),
-                            0 if weight is None else weight.stride(0), None if loss is None else loss.data_ptr(),
+                            0 if weight is None else weight.stride(0), loss.data_ptr(),
                             None if stats is None else stats.data_ptr(), None if grad is None else grad.data_ptr(),
                             x.shape[1])
 

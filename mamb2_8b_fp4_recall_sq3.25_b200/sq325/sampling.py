@@ -34,10 +34,10 @@ def logits_rows(logits):
     return x if x.stride(1) == 1 or shape[-1] == 1 else x.contiguous()
 
 
-def logits_args(x):
-    """ctypes view of rows that logits_rows() returned."""
+def logits_fields(x):
+    """The fields of an sq_logits for rows that logits_rows() returned."""
     rows, vocab = x.shape
-    return _lib.Logits(x.data_ptr(), x.stride(0), rows, vocab, _TYPES[x.dtype])
+    return x.data_ptr(), x.stride(0), rows, vocab, _TYPES[x.dtype]
 
 
 def _per_row(name, value, x, lead, dtype):
@@ -50,7 +50,6 @@ def _per_row(name, value, x, lead, dtype):
 def _number(name, value, kinds, low, high):
     if isinstance(value, bool) or not isinstance(value, kinds) or not low <= value <= high:
         raise ValueError(f'{name} is out of range: {value!r}')
-    return value
 
 
 def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -69,25 +68,29 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
             or uniform.device != x.device:
         raise ValueError(f'uniform must be a float32 tensor of shape {tuple(lead)} on {x.device}')
     uniform = uniform.contiguous()
-    t = k = p = q = None
+    t = k = p = q = None                         # addresses of per-row settings
+    kept = []                                    # alive until the launch
     if isinstance(temperature, torch.Tensor):
-        t, temperature = _per_row('temperature', temperature, x, lead, torch.float32), 0.0
-    else:
+        kept.append(_per_row('temperature', temperature, x, lead, torch.float32))
+        t, temperature = kept[-1].data_ptr(), 0.0
+    elif type(temperature) is not float or not 0 <= temperature <= 3.4e38:
         _number('temperature', temperature, (int, float), 0, 3.4e38)
     if isinstance(top_k, torch.Tensor):
-        k, top_k = _per_row('top_k', top_k, x, lead, torch.int32), 0
-    else:
+        kept.append(_per_row('top_k', top_k, x, lead, torch.int32))
+        k, top_k = kept[-1].data_ptr(), 0
+    elif type(top_k) is not int or not 0 <= top_k < 2 ** 31:
         _number('top_k', top_k, int, 0, 2 ** 31 - 1)
     if isinstance(top_p, torch.Tensor):
-        p, top_p = _per_row('top_p', top_p, x, lead, torch.float32), 0.0
-    elif _number('top_p', top_p, (int, float), 0, 1) == 0:
-        raise ValueError('top_p is out of range: 0')
+        kept.append(_per_row('top_p', top_p, x, lead, torch.float32))
+        p, top_p = kept[-1].data_ptr(), 0.0
+    elif type(top_p) is not float or not 0 < top_p <= 1:
+        _number('top_p', top_p, (int, float), 5e-324, 1)
     if isinstance(min_p, torch.Tensor):
-        q, min_p = _per_row('min_p', min_p, x, lead, torch.float32), 0.0
-    else:
+        kept.append(_per_row('min_p', min_p, x, lead, torch.float32))
+        q, min_p = kept[-1].data_ptr(), 0.0
+    elif type(min_p) is not float or not 0 <= min_p <= 1:
         _number('min_p', min_p, (int, float), 0, 1)
     tokens = torch.empty_like(uniform, dtype=torch.long)
-    a = _lib.SampleArgs(logits_args(x), uniform.data_ptr(), *(None if v is None else v.data_ptr() for v in (t, k, p, q)),
-                        temperature, top_k, top_p, min_p, tokens.data_ptr())
+    a = _lib.SampleArgs(*logits_fields(x), uniform.data_ptr(), t, k, p, q, temperature, top_k, top_p, min_p, tokens.data_ptr())
     _lib.launch('sq_sample', x.device, C.byref(a))
     return tokens

@@ -15,11 +15,24 @@ def lib():
     return _lib.load()
 
 
-def _logits(**kw):
+def _fields(**kw):
     from sq325 import _lib
     a = dict(data=4096, row_stride=10, rows=2, vocab=10, type=_lib.F32)
     a.update(kw)
-    return _lib.Logits(*(a[k] for k in ('data', 'row_stride', 'rows', 'vocab', 'type')))
+    return [a[k] for k in ('data', 'row_stride', 'rows', 'vocab', 'type')]
+
+
+def _logits(**kw):
+    from sq325 import _lib
+    return _lib.Logits(*_fields(**kw))
+
+
+def test_bindings_lay_the_fields_out_as_the_header_does():
+    """sq_logits is 32 bytes, and what follows it in the two argument blocks begins there."""
+    from sq325 import _lib
+    assert C.sizeof(_lib.Logits) == 32
+    assert _lib.SampleArgs.uniform.offset == 32 and C.sizeof(_lib.SampleArgs) == 96
+    assert _lib.DistillArgs.values.offset == 32 and _lib.DistillArgs.weight.offset == 64 and C.sizeof(_lib.DistillArgs) == 112
 
 
 BAD_LOGITS = [dict(data=None), dict(type=3), dict(type=-1), dict(rows=-1), dict(rows=(1 << 24) + 1), dict(vocab=0),
@@ -30,10 +43,10 @@ BAD_LOGITS = [dict(data=None), dict(type=3), dict(type=-1), dict(rows=-1), dict(
 def test_entry_points_refuse_logits(lib, bad):
     """Nothing is read or launched: the pointers are not valid ones."""
     from sq325 import _lib
-    a = _lib.SampleArgs(_logits(**bad), 4096, None, None, None, None, 1.0, 0, 1.0, 0.0, 4096)
+    a = _lib.SampleArgs(*_fields(**bad), 4096, None, None, None, None, 1.0, 0, 1.0, 0.0, 4096)
     assert lib.sq_sample(C.byref(a), None) == _lib.SQ_EINVAL
     assert lib.sq_top_logits(C.byref(_logits(**bad)), 2, 4096, 4096, None) == _lib.SQ_EINVAL
-    d = _lib.DistillArgs(_logits(**bad), 4096, 4096, 2, _lib.F32, 1.0, None, 0, 4096, 4096, 4096, 10)
+    d = _lib.DistillArgs(*_fields(**bad), 4096, 4096, 2, _lib.F32, 1.0, None, 0, 4096, 4096, 4096, 10)
     for name in ('sq_distill_forward', 'sq_distill_backward', 'sq_distill_loss_grad'):
         assert getattr(lib, name)(C.byref(d), None) == _lib.SQ_EINVAL
         assert name[3:].encode() in lib.sq_last_error()
@@ -49,7 +62,7 @@ def test_entry_points_refuse_the_rest(lib):
     assert lib.sq_top_logits(C.byref(_logits()), 2, None, 4096, None) == _lib.SQ_EINVAL
     assert lib.sq_top_logits(C.byref(_logits()), 2, 4096, None, None) == _lib.SQ_EINVAL
     for uniform, tokens in ((None, 4096), (4096, None)):
-        a = _lib.SampleArgs(_logits(), uniform, None, None, None, None, 1.0, 0, 1.0, 0.0, tokens)
+        a = _lib.SampleArgs(*_fields(), uniform, None, None, None, None, 1.0, 0, 1.0, 0.0, tokens)
         assert lib.sq_sample(C.byref(a), None) == _lib.SQ_EINVAL
     good = dict(values=4096, indices=4096, k=2, value_type=_lib.F32, temperature=1.0, weight=None, weight_stride=0,
                 loss=4096, stats=4096, grad=4096, grad_stride=10)
@@ -64,7 +77,7 @@ def test_entry_points_refuse_the_rest(lib):
                        (dict(grad=None), (backward, fused)), (dict(grad=4098), (backward, fused)),
                        (dict(grad_stride=9), (backward, fused))):
         a = dict(good, **bad)
-        d = _lib.DistillArgs(_logits(), *(a[k] for k in good))
+        d = _lib.DistillArgs(*_fields(), *(a[k] for k in good))
         for name in names:
             assert getattr(lib, name)(C.byref(d), None) == _lib.SQ_EINVAL, (name, bad)
 
@@ -72,10 +85,11 @@ def test_entry_points_refuse_the_rest(lib):
 def test_entry_points_accept_no_rows(lib):
     from sq325 import _lib
     none = _logits(rows=0, data=None)
-    a = _lib.SampleArgs(none, None, None, None, None, None, 1.0, 0, 1.0, 0.0, None)
+    fields = _fields(rows=0, data=None)
+    a = _lib.SampleArgs(*fields, None, None, None, None, None, 1.0, 0, 1.0, 0.0, None)
     assert lib.sq_sample(C.byref(a), None) == _lib.SQ_OK
     assert lib.sq_top_logits(C.byref(none), 2, None, None, None) == _lib.SQ_OK
-    d = _lib.DistillArgs(none, None, None, 2, _lib.F32, 1.0, None, 0, None, None, None, 0)
+    d = _lib.DistillArgs(*fields, None, None, 2, _lib.F32, 1.0, None, 0, None, None, None, 0)
     for name in ('sq_distill_forward', 'sq_distill_backward', 'sq_distill_loss_grad'):
         assert getattr(lib, name)(C.byref(d), None) == _lib.SQ_OK
 
