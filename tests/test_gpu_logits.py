@@ -432,3 +432,111 @@ def test_refusals():
             f()
     # the context works on
     assert sq325.sample(x, u).tolist() == [0, 0]
+
+
+# ------------------------------------------------------------------ rows that are hard in other ways
+def hard_rows(vocab, dtype):
+    """Rows of few values, in order, almost flat, and with all that counts in one place."""
+    g = torch.Generator(device='cuda').manual_seed(vocab)
+    r = lambda: torch.rand(vocab, generator=g, device='cuda')
+    line = torch.arange(vocab, device='cuda') / vocab
+    rows = [torch.floor(r() * 3), torch.floor(r() * 40) / 4, line * 20, (1 - line) * 20, 1e-3 * r(), 1e-30 * r(),
+            torch.where(line < 0.98, -30.0, 10 * r()), torch.where(r() < 0.999, 5.0, 6.0), -50 * r().square(),
+            torch.where(line > 0.999, r(), -1e4), 300 * (r() - 0.5)]
+    return torch.stack(rows).to(dtype)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [1500, 20001, 256000])
+def test_hard_rows_top_logits(vocab, dtype):
+    import sq325
+    x = hard_rows(vocab, dtype)
+    xs = wide(x)
+    for k in (1, 64, 1000):
+        values, indices = sq325.top_logits(x, k)
+        for r in range(len(xs)):
+            v, i = ol.top(xs[r], k)
+            assert np.array_equal(indices[r].cpu().numpy(), i), (k, r)
+            assert np.array_equal(wide(values[r]), v), (k, r)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [1500, 20001, 256000])
+def test_hard_rows_draws(vocab, dtype):
+    x = hard_rows(vocab, dtype)
+    g = torch.Generator(device='cuda').manual_seed(1)
+    for s in (dict(), dict(k=200), dict(k=3000), dict(p=0.6), dict(p=0.99, t=0.5), dict(q=0.5), dict(k=1000, p=0.7, q=0.01, t=2.0),
+              dict(t=50.0, p=0.5), dict(t=0.01, p=0.9)):
+        check_draw(x, torch.rand(len(x), generator=g, device='cuda'), least=0.0, **s)
+
+
+def test_hard_rows_draws_agree_with_whole_weights():
+    """Ties decide most of these rows, so the cut's place among equal logits is exact: against the definition
+    in whole weights, computed in torch."""
+    import sq325
+    x = hard_rows(20001, torch.float16)
+    g = torch.Generator(device='cuda').manual_seed(2)
+    for k, p, q in ((0, 0.3, 0.0), (0, 0.8, 0.0), (700, 1.0, 0.0), (700, 0.5, 0.0), (100, 0.9, 0.2), (0, 1.0, 0.0), (5000, 0.9, 0.0)):
+        u = torch.rand(len(x), generator=g, device='cuda')
+        f = x.float()
+        m = f.amax(1, keepdim=True)
+        c = torch.tensor(1.4426950408889634, device='cuda') / torch.tensor(1.0, device='cuda')
+        y = torch.where(f == m, 1.0, torch.exp2((f - m) * c))
+        w = torch.round(y * 2.0 ** 31).long()
+        order = torch.sort(f, dim=1, descending=True, stable=True)[1]
+        ws, ys = w.gather(1, order), y.gather(1, order)
+        rank = torch.arange(x.shape[1], device='cuda')
+        ws = torch.where((rank < k) | (k == 0), ws, 0)
+        before = ws.cumsum(1) - ws
+        keep = (before.double() < float(np.float32(p)) * ws.sum(1, keepdim=True).double()) & (ys >= np.float32(q)) | (rank == 0)
+        run = torch.zeros_like(w).scatter_(1, order, torch.where(keep, ws, 0)).cumsum(1)
+        target = (u.double()[:, None] * run[:, -1:].double()).long()
+        want = (run <= target).sum(1)
+        assert torch.equal(sq325.sample(x, u, top_k=k, top_p=p, min_p=q), want), (k, p, q)
+
+
+def test_rows_past_32_bit_offsets():
+    """Rows that begin more than 2^32 bytes and 2^31 elements into their buffer."""
+    import sq325
+    rows, vocab = 9000, 262144
+    x = torch.zeros((rows, vocab), device='cuda', dtype=torch.float16)
+    last, g = make(3, vocab, torch.float16, seed=12)
+    x[-3:] = last
+    u = torch.rand(3, generator=g, device='cuda')
+    wide_u = torch.cat([torch.zeros(rows - 3, device='cuda'), u])
+    for s in (dict(top_p=0.9), dict(top_k=50)):
+        assert torch.equal(sq325.sample(x, wide_u, **s)[-3:], sq325.sample(last, u, **s))
+    values, indices = sq325.top_logits(x, 5)
+    v, i = sq325.top_logits(last, 5)
+    assert torch.equal(values[-3:], v) and torch.equal(indices[-3:], i) and indices[0].tolist() == [0, 1, 2, 3, 4]
+    loss, grad = sq325.distillation_loss_grad(x, values, indices)
+    l, d = sq325.distillation_loss_grad(last, v, i)
+    assert torch.allclose(loss[-3:], l, rtol=1e-5) and torch.allclose(grad[-3:].float(), d.float(), atol=1e-5)
+    del grad
+    y = x.requires_grad_(True)
+    again = sq325.distillation_loss(y, values, indices)
+    back, = torch.autograd.grad(again.sum(), y)
+    assert torch.allclose(again.detach()[-3:], l, rtol=1e-5) and torch.allclose(back[-3:].float(), d.float(), atol=1e-5)
+
+
+@pytest.mark.parametrize('rows', [5, 700])
+def test_operators_in_a_cuda_graph(rows):
+    """Captured once, replayed on new contents."""
+    import sq325
+    x, g = make(rows, 20011, torch.bfloat16, seed=3)
+    values, indices = record(g, rows, 20011, 12, torch.bfloat16)
+    u = torch.rand(rows, generator=g, device='cuda')
+    calls = (lambda: (sq325.sample(x, u, top_p=0.9),), lambda: (sq325.sample(x, u, top_k=40),), lambda: sq325.top_logits(x, 30),
+             lambda: (sq325.distillation_loss(x, values, indices),), lambda: sq325.distillation_loss_grad(x, values, indices))
+    for call in calls:
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        x.copy_(torch.randn(x.shape, generator=g, device='cuda') * 3)
+        u.copy_(torch.rand(rows, generator=g, device='cuda'))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, call()):
+            assert torch.equal(a, b)
