@@ -210,31 +210,21 @@ struct Record {
   float e[N];                                    // (v - v_max) c
   float taken[N];                                // student's logit there
   float vmax, Q;
-  // Begins to read row `row`.
-  __device__ void fetch(const DistillParams& P, int row) {
+  __device__ void read(const DistillParams& P, int row, const T* s, float c, float (*part)[NT / 32]) {
     const long long base = (long long)row * P.k;
+    vmax = -INFINITY;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int k = threadIdx.x + i * NT;
       at[i] = -1;
-      e[i] = -INFINITY;
       if (k < P.k) {
-        at[i] = P.indices[base + k];
+        const int j = P.indices[base + k];
         e[i] = record_value(P, base + k);
-      }
-    }
-  }
-  // What fetch() read, and the student's logit at entries with wants(index).
-  template <typename W>
-  __device__ void prepare(const DistillParams& P, const T* s, float c, float (*part)[NT / 32], W wants) {
-    vmax = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      if (!used_entry(P, at[i], e[i])) {
-        at[i] = -1;
-      } else {
-        vmax = fmaxf(vmax, e[i]);
-        if (wants(at[i])) taken[i] = to_f32(s[at[i]]);
+        if (used_entry(P, j, e[i])) {
+          at[i] = j;
+          vmax = fmaxf(vmax, e[i]);
+          taken[i] = to_f32(s[j]);
+        }
       }
     }
     vmax = block_max<NT>(vmax, part[0]);
@@ -246,7 +236,7 @@ struct Record {
     }
     Q = block_sum<NT>(q, part[1]);
   }
-  // Loss of the row, known to thread 0 (every thread of the CTA calls, `taken` was wanted everywhere).
+  // Loss of the row, to thread 0; every thread of the CTA calls.
   __device__ float loss(float r, float sum, float c, float temperature, float (*part)[NT / 32]) const {
     float l = 0.f;
     const float rest = Q > 0.f ? log2f(sum) - log2f(Q) : 0.f;
@@ -293,10 +283,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) loss_kernel(const DistillParams
   Unit<T> x[NV];
   load(x, span.lo);
   Record<T, NT, N> rec;
-  if (rank == 0) {
-    rec.fetch(P, row);
-    rec.prepare(P, span.p, c, part, [](int) { return true; });
-  }
+  if (rank == 0) rec.read(P, row, span.p, c, part);
 #pragma unroll 1
   for (int from = span.lo; from < span.hi; from += NT * NV) {
     if (from != span.lo) load(x, from);

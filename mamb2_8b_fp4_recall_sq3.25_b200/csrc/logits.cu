@@ -123,7 +123,7 @@ struct Team {
     }
     return before + run - v;
   }
-  // The largest number t of `bits` bits, an even number, for which count(t) summed over the block is at
+  // The largest number t of `bits` bits (`bits` is even) for which count(t) summed over the block is at
   // least r (0 where there is none); count falls with t and is at most 31 a thread.  Two bits a round.
   template <typename C>
   __device__ u64 search(int bits, int r, C count) {
@@ -310,7 +310,7 @@ struct Listing {
     uint32_t key[G];
 #pragma unroll
     for (int a = 0; a < G; ++a) {
-      high[a] = folded_max(top[a]);
+      high[a] = unit_max(top[a]);
       key[a] = order_key(high[a] + 0.0f) >> 16;
     }
     if (t.tid == 0) { t.s.count = 0; t.s.groups = 0; }
@@ -496,6 +496,15 @@ struct Row : Team<NT> {
     }
     return m;
   }
+  __device__ u64 part_sums(u64 sum) {
+    sum = warp_sum(sum);
+    __syncthreads();
+    if ((tid & 31) == 0) s.part[tid >> 5] = sum;
+    __syncthreads();
+    u64 t = 0;
+    for (int i = 0; i < NW; ++i) t += s.part[i];
+    return t;
+  }
   // Sums of w(x, col) over contiguous stretches, one a warp, in s.part; returns this CTA's total.
   // w is 0 below `least`.
   template <typename W>
@@ -509,13 +518,7 @@ struct Row : Team<NT> {
 #pragma unroll
       for (int v = 0; v < kUnit<T>; ++v) sum += w(to_f32(u.v[v]), d.col(i, v));
     }
-    sum = warp_sum(sum);
-    __syncthreads();
-    if ((tid & 31) == 0) s.part[tid >> 5] = sum;
-    __syncthreads();
-    u64 t = 0;
-    for (int i = 0; i < NW; ++i) t += s.part[i];
-    return t;
+    return part_sums(sum);
   }
   // stretch_sums of the weights of what `cut` and min-p leave; nothing is left below `least`.
   __device__ u64 left_sums(Exponent e, Cut cut, float min_p, float least) {
@@ -538,13 +541,7 @@ struct Row : Team<NT> {
       }
       each_bit(ties, i, [&](int p) { if (d.col(0, p) <= cut.last) sum += weight_of(e(at(p))); });
     }
-    sum = warp_sum(sum);
-    __syncthreads();
-    if ((tid & 31) == 0) s.part[tid >> 5] = sum;
-    __syncthreads();
-    u64 t = 0;
-    for (int i = 0; i < NW; ++i) t += s.part[i];
-    return t;
+    return part_sums(sum);
   }
   // After stretch_sums: the first column of this CTA, in order, at which the running sum passes
   // `target` (below the total).
@@ -636,11 +633,11 @@ struct Row : Team<NT> {
     return at;
   }
 
-  // A cluster barrier has to follow before the CTA ends (others read its sums).
   // The cut after the first tokens of the order whose weights w(t) reach need(whole weight), among
   // elements with kept(x, col).  t = (x - m) c is the exponent of y; w depends on it alone, is 0 where the
   // token's weight is, and below 2^31 + 1.  False: the whole weight does not reach it.
   // kept_here: this CTA's share of the weight that is kept.  PLAIN: every element is kept and w is weight_of.
+  // A cluster barrier has to follow before the CTA ends (others read its sums).
   template <bool PLAIN, typename K, typename W, typename N>
   __device__ bool select(K kept, W w, Exponent e, N need_of, Cut& cut, u64& kept_here) {
     static_assert(kSteps <= NT, "a thread per step");
@@ -936,8 +933,6 @@ int by_type(int type, F f) {
   return kEInval;
 }
 
-}  // namespace
-
 template <typename T, int NT>
 int launch_sample_threads(const SampleParams& P, int size, bool listed, cudaStream_t st) {
   size_t smem = listed ? 0 : (size_t)kWorkBytes + (size_t)((row_units(P.x) + size - 1) / size) * 16;
@@ -955,6 +950,8 @@ int listing_size(const LogitsRows& x, int k) {
   while (size < 8 && x.rows * size < 4 * kSms && units > size * 2 * kTopThreads && 2 * size * k <= kList) size *= 2;
   return size;
 }
+
+}  // namespace
 
 int launch_sample(const SampleParams& P, cudaStream_t st) {
   // Where every row is known to be listed (one top-k for all), nothing but the lists is on chip.  Otherwise as many

@@ -26,10 +26,7 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 
-// A logit as the draw and the record see it: NaN counts as masked (-inf), -0 as +0.
-__device__ __forceinline__ float plain_logit(float v) { return v != v ? -INFINITY : v + 0.0f; }
-
-// Order-preserving key of a plain logit.
+// Order-preserving key of a logit that is no NaN; callers add 0 first, so that -0 and +0 share one.
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t b = __float_as_uint(v);
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
@@ -80,7 +77,6 @@ __device__ __forceinline__ void fold_max(Unit<__nv_bfloat16>& top, const Unit<__
 __device__ __forceinline__ void fold_max(Unit<float>& top, const Unit<float>& u) {
   top.v[0] = fmaxf(top.v[0], fmaxf(fmaxf(u.v[0], u.v[1]), fmaxf(u.v[2], u.v[3])));
 }
-template <typename T> __device__ __forceinline__ float folded_max(const Unit<T>& top) { return unit_max(top); }
 
 // Where the part of a row that CTA `rank` of `size` works on lies: units of 16 bytes at 16-byte
 // addresses.  Rows start where their stride puts them: the first and the last unit of a row may be
