@@ -942,12 +942,12 @@ int launch_sample_threads(const SampleParams& P, int size, bool listed, cudaStre
   if (allow_shared(kernel, 160 * 1024, done) != cudaSuccess) return launch_status();
   return launch_clusters(kernel, P, size, NT, smem, st);
 }
-// CTAs a row for listing k: one lists the fewest logits; more where the rows do not fill the GPU, as long as
-// their lists fit that of the first.
+// CTAs a row for listing k: one lists the fewest logits; more as long as they all run at once (a second wave of a
+// few costs more: 333 rows of 50,001 fp32 logits by one CTA each 28 us, by two 39) and their lists fit that of the first.
 int listing_size(const LogitsRows& x, int k) {
   const int units = row_units(x);
   int size = 1;
-  while (size < 8 && x.rows * size < 4 * kSms && units > size * 2 * kTopThreads && 2 * size * k <= kList) size *= 2;
+  while (size < 8 && x.rows * size * 2 <= 4 * kSms && units > size * 2 * kTopThreads && 2 * size * k <= kList) size *= 2;
   return size;
 }
 
