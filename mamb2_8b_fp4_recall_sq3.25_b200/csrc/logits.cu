@@ -431,11 +431,13 @@ __device__ __forceinline__ uint32_t weight_of(float t) {
   return __float2uint_rn(y * 2147483648.0f);
 }
 
-// Adds `w` to the histogram word at `address` if the weight is light, -32.01 < t < kLight (without a branch: most are).
+// Adds `w` to the histogram word at `address` if the weight is light, -32.01 < t < kLight; sets `bit` of `rest` if t is not
+// below kLight (without branches: most are light).
 constexpr float kLight = -13.02f;
-__device__ __forceinline__ void add_light(uint32_t address, uint32_t w, float t) {
-  asm volatile("{\n.reg .pred p;\nsetp.lt.f32 p, %2, %3;\nsetp.gt.and.f32 p, %2, %4, p;\n@p red.shared.add.u32 [%0], %1;\n}\n"
-               :: "r"(address), "r"(w), "f"(t), "f"(kLight), "f"(-32.01f) : "memory");
+__device__ __forceinline__ void add_light(uint32_t address, uint32_t w, float t, uint32_t& rest, uint32_t bit) {
+  asm volatile("{\n.reg .pred p;\nsetp.lt.f32 p, %3, %4;\n@!p or.b32 %0, %0, %6;\nsetp.gt.and.f32 p, %3, %5, p;\n"
+               "@p red.shared.add.u32 [%1], %2;\n}\n"
+               : "+r"(rest) : "r"(address), "r"(w), "f"(t), "f"(kLight), "f"(-32.01f), "r"(bit) : "memory");
 }
 
 // One CTA's part of a row in shared memory.
@@ -672,10 +674,8 @@ struct Row : Team<NT> {
         if (PLAIN) {
           // weight_of for y < 2^-13, which fits the low word
           const float2 y = __fadd2_rn(make_float2(ex2(t[a].x), ex2(t[a].y)), make_float2(0.00390625f, 0.00390625f)), b = step(t[a]);
-          add_light(words + __float_as_uint(b.x) * (kCols * 4), __float_as_uint(y.x) & 0x7fffffu, t[a].x);
-          add_light(words + __float_as_uint(b.y) * (kCols * 4), __float_as_uint(y.y) & 0x7fffffu, t[a].y);
-          if (!(t[a].x < kLight)) rest |= 1u << (2 * a);
-          if (!(t[a].y < kLight)) rest |= 2u << (2 * a);
+          add_light(words + __float_as_uint(b.x) * (kCols * 4), __float_as_uint(y.x) & 0x7fffffu, t[a].x, rest, 1u << (2 * a));
+          add_light(words + __float_as_uint(b.y) * (kCols * 4), __float_as_uint(y.y) & 0x7fffffu, t[a].y, rest, 2u << (2 * a));
         } else {
           if (t[a].x > -32.01f) rest |= 1u << (2 * a);
           if (t[a].y > -32.01f) rest |= 2u << (2 * a);

@@ -20,7 +20,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .sampling import _TYPES, logits_fields, logits_rows
+from .sampling import _TYPES, logits_fields, logits_rows, row_numbers
 
 __all__ = ['top_logits', 'distillation_loss', 'distillation_loss_grad']
 
@@ -34,7 +34,7 @@ def top_logits(logits, k):
     x = logits_rows(logits)
     if isinstance(k, bool) or not isinstance(k, int) or not 1 <= k <= min(MAX_RECORD, x.shape[1]):
         raise ValueError(f'k must be an integer in [1, min({MAX_RECORD}, vocab)]')
-    values = x.new_empty((*logits.shape[:-1], k))
+    values = torch.empty(*logits.shape[:-1], k, dtype=x.dtype, device=x.device)
     indices = torch.empty_like(values, dtype=torch.int32)
     _lib.launch('sq_top_logits', x.device, C.byref(_lib.Logits(*logits_fields(x))), k, values.data_ptr(), indices.data_ptr())
     return values, indices
@@ -44,19 +44,20 @@ def _checked(logits, values, indices, temperature):
     x = logits_rows(logits)
     if not isinstance(values, torch.Tensor) or not isinstance(indices, torch.Tensor):
         raise ValueError('The record must be two tensors, values and indices')
-    shape = values.shape
-    if shape != indices.shape or len(shape) != logits.ndim or shape[:-1] != logits.shape[:-1]:
+    shape, lead = values.shape, logits.shape[:-1]
+    if shape != indices.shape or not shape or shape[:-1] != lead:
         raise ValueError('The record must be values and indices [..., k] with the leading shape of the logits')
     if not 1 <= shape[-1] <= MAX_RECORD:
         raise ValueError(f'The record must have 1 to {MAX_RECORD} entries a row')
-    if values.dtype not in _TYPES or indices.dtype != torch.int32 or values.device != x.device \
-            or indices.device != x.device:
+    device = x.get_device()
+    if values.dtype not in _TYPES or indices.dtype != torch.int32 or values.get_device() != device \
+            or indices.get_device() != device:
         raise ValueError('The record must be FP16, BF16 or FP32 values and int32 indices on the device of the logits')
     if values.requires_grad:
         raise ValueError("The teacher's record receives no gradient: detach it")
     if isinstance(temperature, bool) or not isinstance(temperature, (int, float)) or not 0 < temperature <= 3e38:
         raise ValueError('temperature must be a positive finite number')
-    return x, values.contiguous(), indices.contiguous()
+    return x, values.contiguous(), indices.contiguous(), lead
 
 
 def _args(x, values, indices, temperature, loss, weight=None, stats=None, grad=None):
@@ -75,9 +76,9 @@ def _row_weights(weight):
 class _DistillationLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, values, indices, temperature):
-        x, values, indices = _checked(logits, values, indices, temperature)
-        loss = x.new_empty(logits.shape[:-1], dtype=torch.float32)
-        stats = x.new_empty((x.shape[0], 4), dtype=torch.float32)
+        x, values, indices, lead = _checked(logits, values, indices, temperature)
+        loss = row_numbers(x, lead)
+        stats = torch.empty(x.shape[0], 4, dtype=torch.float32, device=x.device)
         ctx.save_for_backward(x, values, indices, stats)
         ctx.shape = logits.shape
         ctx.args = _args(x, values, indices, temperature, loss=loss, stats=stats)     # backward's too
@@ -89,7 +90,7 @@ class _DistillationLoss(torch.autograd.Function):
     def backward(ctx, grad_loss):
         x = ctx.saved_tensors[0]                 # raises if one of them was changed in place
         weight = _row_weights(grad_loss)
-        grad = x.new_empty(ctx.shape)
+        grad = torch.empty(*ctx.shape, dtype=x.dtype, device=x.device)
         a = ctx.args
         a.weight, a.weight_stride, a.grad = weight.data_ptr(), weight.stride(0), grad.data_ptr()
         _lib.launch('sq_distill_backward', x.device, C.byref(a))
@@ -102,8 +103,8 @@ def distillation_loss(logits, values, indices, temperature=1.0):
     logits; the record receives no gradient."""
     if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return _DistillationLoss.apply(logits, values, indices, temperature)
-    x, values, indices = _checked(logits, values, indices, temperature)
-    loss = x.new_empty(logits.shape[:-1], dtype=torch.float32)
+    x, values, indices, lead = _checked(logits, values, indices, temperature)
+    loss = row_numbers(x, lead)
     _lib.launch('sq_distill_forward', x.device, C.byref(_args(x, values, indices, temperature, loss=loss)))
     return loss
 
@@ -112,15 +113,14 @@ def distillation_loss_grad(logits, values, indices, temperature=1.0, weight=None
     """(loss fp32 [...], gradient [..., vocab] in the logits' dtype) in one call.  weight: fp32
     [...] factor of each row's gradient (None: 1), as the upstream gradient of the loss would be;
     the loss itself is not weighted."""
-    x, values, indices = _checked(logits, values, indices, temperature)
-    lead = logits.shape[:-1]
+    x, values, indices, lead = _checked(logits, values, indices, temperature)
     if weight is not None:
         if not isinstance(weight, torch.Tensor) or weight.shape != lead or weight.dtype != torch.float32 \
-                or weight.device != x.device:
+                or weight.get_device() != x.get_device():
             raise ValueError(f'weight must be a float32 tensor of shape {tuple(lead)} on {x.device}')
         weight = _row_weights(weight)
-    loss = x.new_empty(lead, dtype=torch.float32)
-    grad = x.new_empty(logits.shape)
+    loss = row_numbers(x, lead)
+    grad = torch.empty(*logits.shape, dtype=x.dtype, device=x.device)
     _lib.launch('sq_distill_loss_grad', x.device,
                 C.byref(_args(x, values, indices, temperature, weight=weight, loss=loss, grad=grad)))
     return loss, grad

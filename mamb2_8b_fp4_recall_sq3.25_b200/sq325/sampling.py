@@ -34,6 +34,12 @@ def logits_rows(logits):
     return x if x.stride(1) == 1 or shape[-1] == 1 else x.contiguous()
 
 
+def row_numbers(x, lead):
+    """An empty fp32 tensor with a number a row of x, of shape `lead`."""
+    out = torch.empty(x.shape[0], dtype=torch.float32, device=x.device)
+    return out if len(lead) == 1 else out.view(lead)
+
+
 def logits_fields(x):
     """The fields of an sq_logits for rows that logits_rows() returned."""
     rows, vocab = x.shape
@@ -42,7 +48,7 @@ def logits_fields(x):
 
 def _per_row(name, value, x, lead, dtype):
     """A tensor with one setting a row."""
-    if value.shape != lead or value.dtype != dtype or value.device != x.device:
+    if value.shape != lead or value.dtype != dtype or value.get_device() != x.get_device():
         raise ValueError(f'{name} must be a number or a {dtype} tensor of shape {tuple(lead)} on {x.device}')
     return value.contiguous()
 
@@ -65,7 +71,7 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     x = logits_rows(logits)
     lead = logits.shape[:-1]
     if not isinstance(uniform, torch.Tensor) or uniform.shape != lead or uniform.dtype != torch.float32 \
-            or uniform.device != x.device:
+            or uniform.get_device() != x.get_device():
         raise ValueError(f'uniform must be a float32 tensor of shape {tuple(lead)} on {x.device}')
     uniform = uniform.contiguous()
     t = k = p = q = None                         # addresses of per-row settings

@@ -540,3 +540,25 @@ def test_operators_in_a_cuda_graph(rows):
         torch.cuda.synchronize()
         for a, b in zip(out, call()):
             assert torch.equal(a, b)
+
+
+def test_backward_again_and_after_a_change():
+    """A retained graph gives the same gradient twice; logits changed in place are refused."""
+    import sq325
+    x, g = make(6, 1500, torch.float32, seed=2)
+    values, indices = record(g, 6, 1500, 8, torch.float32)
+    y = x.clone().requires_grad_(True)
+    loss = sq325.distillation_loss(y, values, indices, temperature=1.5)
+    first, = torch.autograd.grad(loss.sum(), y, retain_graph=True)
+    second, = torch.autograd.grad(loss, y, torch.full((6,), 2.0, device='cuda'))
+    assert torch.allclose(second, 2 * first, rtol=1e-6)
+    z = x.clone().requires_grad_(True)
+    w = z * 1.0
+    loss = sq325.distillation_loss(w, values, indices)
+    w.add_(1.0)
+    with pytest.raises(RuntimeError, match='modified'):
+        loss.sum().backward()
+    with pytest.raises(RuntimeError):                    # the gradient itself is not differentiable
+        loss = sq325.distillation_loss(y, values, indices)
+        grad, = torch.autograd.grad(loss.sum(), y, create_graph=True)
+        grad.sum().backward()
