@@ -60,10 +60,10 @@ def _checked(logits, values, indices, temperature):
     return x, values.contiguous(), indices.contiguous(), lead
 
 
-def _args(x, values, indices, temperature, loss, weight=None, stats=None, grad=None):
+def _args(x, values, indices, temperature, loss=None, weight=None, stats=None, grad=None):
     return _lib.DistillArgs(*logits_fields(x), values.data_ptr(), indices.data_ptr(), values.shape[-1], _TYPES[values.dtype],
                             temperature, None if weight is None else weight.data_ptr(),
-                            0 if weight is None else weight.stride(0), loss.data_ptr(),
+                            0 if weight is None else weight.stride(0), None if loss is None else loss.data_ptr(),
                             None if stats is None else stats.data_ptr(), None if grad is None else grad.data_ptr(),
                             x.shape[1])
 
@@ -80,20 +80,20 @@ class _DistillationLoss(torch.autograd.Function):
         loss = row_numbers(x, lead)
         stats = torch.empty(x.shape[0], 4, dtype=torch.float32, device=x.device)
         ctx.save_for_backward(x, values, indices, stats)
-        ctx.shape = logits.shape
-        ctx.args = _args(x, values, indices, temperature, loss=loss, stats=stats)     # backward's too
-        _lib.launch('sq_distill_forward', x.device, C.byref(ctx.args))
+        ctx.shape, ctx.temperature = logits.shape, temperature
+        _lib.launch('sq_distill_forward', x.device, C.byref(_args(x, values, indices, temperature, loss=loss, stats=stats)))
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
-        x = ctx.saved_tensors[0]                 # raises if one of them was changed in place
+        x, values, indices, stats = ctx.saved_tensors       # raises if one of them was changed in place
+        # Hooks on saved tensors (offloading, recomputation) may have put them elsewhere, with other strides.
+        x, values, indices, stats = logits_rows(x), values.contiguous(), indices.contiguous(), stats.contiguous()
         weight = _row_weights(grad_loss)
         grad = torch.empty(*ctx.shape, dtype=x.dtype, device=x.device)
-        a = ctx.args
-        a.weight, a.weight_stride, a.grad = weight.data_ptr(), weight.stride(0), grad.data_ptr()
-        _lib.launch('sq_distill_backward', x.device, C.byref(a))
+        _lib.launch('sq_distill_backward', x.device,
+                    C.byref(_args(x, values, indices, ctx.temperature, weight=weight, stats=stats, grad=grad)))
         return grad, None, None, None
 
 

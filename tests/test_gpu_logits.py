@@ -562,3 +562,27 @@ def test_backward_again_and_after_a_change():
         loss = sq325.distillation_loss(y, values, indices)
         grad, = torch.autograd.grad(loss.sum(), y, create_graph=True)
         grad.sum().backward()
+
+
+def test_backward_from_saved_tensors_elsewhere():
+    """Hooks that offload what forward saved, or compute it again, give the same gradient: backward reads what the
+    graph hands it, not forward's memory."""
+    import sq325
+    from torch.utils.checkpoint import checkpoint
+    x, g = make(7, 1501, torch.float32, seed=3)
+    values, indices = record(g, 7, 1501, 9, torch.float32)
+    y = x.clone().requires_grad_(True)
+
+    def head(t):
+        return sq325.distillation_loss((t * 1.25)[:, 1:], values, indices, temperature=2.0).sum()
+
+    indices.clamp_(max=1499)
+    want, = torch.autograd.grad(head(y), y)
+    with torch.autograd.graph.save_on_cpu():
+        loss = head(y)
+    full = torch.full((1 << 20,), 3.0, device='cuda')    # takes up what forward released
+    offloaded, = torch.autograd.grad(loss, y)
+    loss = checkpoint(head, y, use_reentrant=False)
+    full = torch.full((1 << 20,), 3.0, device='cuda')
+    again, = torch.autograd.grad(loss, y)
+    assert torch.equal(offloaded, want) and torch.equal(again, want)
