@@ -24,12 +24,13 @@
 // Otherwise (top-p, large k, none) the row stays on chip, each CTA with its part in shared memory: it is read
 // from HBM once.  A histogram over 256 steps of 1/8 octave of y, with exact weights, finds the
 // step in which the running weight reaches what is wanted; the members of that step are
-// narrowed by histograms over their keys until one key is left.  What is kept is then "logit
-// above the cut, or equal and index not above the last one kept".  Elements that need more than an addition to one
-// word (weights of 2^18 and more, members of the step) are noted by position and worked on with all lanes busy.
-// Bound by instructions (47 a logit) and by the waits of eight CTAs for one another: top-p of 512 rows of
-// 256,000 bf16 logits takes 0.42 ms, ten times the time to read them; of that, in a run of 296 rows, the read and the
-// maximum are 14%, the histogram 28%, its members 21%, narrowing and drawing the rest.
+// narrowed by histograms over their keys until one key is left (16-bit types mostly by counting their values, in one
+// pass).  What is kept is then "logit above the cut, or equal and index not above the last one kept".  Elements that need
+// more than an addition to one word (weights of 2^18 and more, members of the step) are noted by position and worked on
+// with all lanes busy.
+// Bound by instructions (43 a logit) and by the waits of eight CTAs for one another: top-p of 512 rows of
+// 256,000 bf16 logits takes 0.34 ms, eight times the time to read them; of that the read and the maximum are 17%, the
+// histogram 35%, the step it crosses in 23%, the cut and the draw 25%.
 #include "logits.cuh"
 #include "logits_util.cuh"
 #include <type_traits>
@@ -54,7 +55,9 @@ constexpr int kMaxima = 8;                       // of a thread
 template <int NT> constexpr int kListBytes = kList * 8 + kMaxima * NT * 2;
 constexpr int kMaxListed = kList / 8;            // top-k up to this many goes by the list
 
-struct Cut { float x; int last; };               // kept: above x, or equal and column <= last
+// Kept: above x, or equal and column <= last.  ties: if not 0, `last` is the column of the CTA's equal token of that number,
+// which is not located yet.
+struct Cut { float x; int last, ties; };
 
 struct Shared {
   u64 slot[2][8];
@@ -440,6 +443,12 @@ __device__ __forceinline__ void add_light(uint32_t address, uint32_t w, float t,
                : "+r"(rest) : "r"(address), "r"(w), "f"(t), "f"(kLight), "f"(-32.01f), "r"(bit) : "memory");
 }
 
+// Counts one at the shared word at `address` if d < width (without a branch).
+__device__ __forceinline__ void count_if(uint32_t address, uint32_t d, uint32_t width) {
+  asm volatile("{\n.reg .pred p;\nsetp.lt.u32 p, %1, %2;\n@p red.shared.add.u32 [%0], 1;\n}\n"
+               :: "r"(address), "r"(d), "r"(width) : "memory");
+}
+
 // One CTA's part of a row in shared memory.
 template <typename T, int NT>
 struct Row : Team<NT> {
@@ -701,11 +710,47 @@ struct Row : Team<NT> {
     const int found = crossing(mine, need_of, above, mine_above);
     if (found < 0) return false;
     const u64 need = s.found_need;
-    // keys in which the step can lie: its edges in x, widened by far more than the rounding of t and of this
-    // (NaN, from infinities, widens to everything)
+    const uint32_t wanted_step = kStep0 + found;
+    // the step's edges in x, widened by far more than the rounding of t and of this (NaN, from infinities, widens
+    // to everything)
     const float first = e.m - (found - 0.5f) / kPerOctave / e.c, last = e.m - (found + 0.5f) / kPerOctave / e.c;
-    uint32_t hi = order_key(fminf(e.m, first + 4e-6f * (fabsf(e.m) + fabsf(first - e.m))) + 0.0f) >> SH;
-    uint32_t lo = order_key(fmaxf(-3.4028235e38f, last - 4e-6f * (fabsf(e.m) + fabsf(last - e.m)))) >> SH;
+    const float most = fminf(e.m, first + 4e-6f * (fabsf(e.m) + fabsf(first - e.m)));
+    const float least = fmaxf(-3.4028235e38f, last - 4e-6f * (fabsf(e.m) + fabsf(last - e.m)));
+    int entry;
+    if constexpr (PLAIN && SH != 0) {
+      // 16-bit logits of one sign take few values in a step: each value's tokens are counted, and a thread a value weighs
+      // them (top-p of 512 rows of 256,000 bf16 logits 388 us; by listing the step's members, as below, 420).
+      const uint32_t a = bits_below<T>(most), b = bits_below<T>(least), base = min(a, b), width = max(a, b) - base + 1;
+      if ((least > 0.0f || most < 0.0f) && width <= kSteps) {
+        for (int i = tid; i < kSteps * kCols; i += NT) low[i] = 0;
+        __syncthreads();
+        const uint32_t counts = (uint32_t)__cvta_generic_to_shared(low + lane);
+        for (int i = tid; i < d.n; i += NT) {
+          const uint4 q = unit[i].q;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const uint32_t two = v == 0 ? q.x : v == 1 ? q.y : v == 2 ? q.z : q.w;
+            const uint32_t d0 = (two & 0xffffu) - base, d1 = (two >> 16) - base;
+            count_if(counts + d0 * (kCols * 4), d0, width);
+            count_if(counts + d1 * (kCols * 4), d1, width);
+          }
+        }
+        __syncthreads();
+        const auto value = [&](int i) { return to_f32(from_bits<T>(base + (least > 0.0f ? width - 1 - i : i))); };
+        mine = 0;
+        if (tid < (int)width) {
+          const float t = e(value(tid));
+          const int i = least > 0.0f ? width - 1 - tid : tid;
+          uint32_t n = 0;
+          for (int c = 0; c < kCols; ++c) n += low[i * kCols + c];
+          // the values beside the step are in the widened window only
+          if (__float_as_uint(fmaf(t, -kPerOctave, 8388608.0f)) == wanted_step) mine = (u64)n * w(t);
+        }
+        entry = crossing(mine, [&](u64) { return need; }, above, mine_above);
+        return finish(value(entry), entry, w, e, need - above, cut, kept_here, mine_above);
+      }
+    }
+    uint32_t hi = order_key(most + 0.0f) >> SH, lo = order_key(least) >> SH;
     // narrowing: histograms of the step's members over their keys; the members' positions are listed first
     // (if they are too many, every round goes through the part)
     uint32_t* upper = low + kFine * kCols;
@@ -724,7 +769,6 @@ struct Row : Team<NT> {
       atomicAdd(low + b, q & kLow);
       if (q >> kLowBits) atomicAdd(upper + b, q >> kLowBits);
     };
-    const uint32_t wanted_step = kStep0 + found;
     const auto each_in_step = [&](auto f) {
       each_unit(e, [&](int i, const float2 (&t)[kUnit<T> / 2]) {
         uint32_t which = 0;
@@ -740,7 +784,6 @@ struct Row : Team<NT> {
     if (tid == 0) s.count = 0;
     __syncthreads();
     each_in_step([&](int p) { note(members, kMembers, p); });
-    int entry;
     for (;;) {
       begin();
       if (s.count <= kMembers) {
@@ -760,17 +803,24 @@ struct Row : Team<NT> {
       if (hi - lo > width) lo = hi - width;
     }
     const uint32_t key = hi - entry;
-    u64 key_before = 0;                          // weight of that key in the CTAs before this one
-    for (int r = 0; r < (int)rank; ++r) key_before += remote_load(remote_smem(&s.sums[turn][entry], r));
-    const u64 here = s.sums[turn][entry];
     // the key of 16-bit types stands for one logit: its low bits are those of an exact value
     const float x = key_logit(SH == 0 ? key : (key << SH) | ((key << SH) & 0x80000000u ? 0u : (1u << SH) - 1u));
+    return finish(x, entry, w, e, need - above, cut, kept_here, mine_above);
+  }
+
+  // The cut at logit x, entry `entry` of the histogram last crossed: of its tokens the first that reach `need` are kept.
+  template <typename W>
+  __device__ bool finish(float x, int entry, W w, Exponent e, u64 need, Cut& cut, u64& kept_here, u64 mine_above) {
+    u64 key_before = 0;                          // weight of that logit in the CTAs before this one
+    for (int r = 0; r < (int)rank; ++r) key_before += remote_load(remote_smem(&s.sums[turn][entry], r));
+    const u64 here = s.sums[turn][entry];
     // quotients of numbers below 2^50 by one below 2^32: a double holds them closely enough for floor()
     const u64 each_w = w(e(x));
     const double by = (double)each_w;
-    const u64 wanted = (u64)floor((double)(need - above + each_w - 1) / by), earlier = (u64)floor((double)key_before / by);
+    const u64 wanted = (u64)floor((double)(need + each_w - 1) / by), earlier = (u64)floor((double)key_before / by);
     const u64 ties = (u64)floor((double)here / by);
     cut.x = x;
+    cut.ties = 0;
     u64 taken = ties;
     if (wanted >= earlier + ties) {
       cut.last = 0x7fffffff;
@@ -779,12 +829,21 @@ struct Row : Team<NT> {
       taken = 0;
     } else {
       taken = wanted - earlier;
-      const auto tie = [&](float v, int col) -> u64 { return v == x && kept(v, col) ? 1 : 0; };
-      stretch_sums(tie, x);
-      cut.last = locate(tie, taken - 1);
+      cut.ties = (int)taken;
     }
     kept_here = mine_above + taken * each_w;
     return true;
+  }
+  // Locates the last equal token that a selection among `kept` took.  Left to the CTA that draws where only that one needs
+  // it: a pass over the part in one CTA holds up the seven others (512 rows of 256,000: 340 us, before the exchange 388).
+  template <typename K>
+  __device__ void settle(K kept, Cut& cut) {
+    if (!cut.ties) return;
+    const float x = cut.x;
+    const auto tie = [&](float v, int col) -> u64 { return v == x && kept(v, col) ? 1 : 0; };
+    stretch_sums(tie, x);
+    cut.last = locate(tie, cut.ties - 1);
+    cut.ties = 0;
   }
 };
 
@@ -865,18 +924,21 @@ __global__ void __launch_bounds__(NT, 768 / NT + (NT > 256)) sample_kernel(const
     __syncthreads();
     e.m = 1.0f;
   }
-  Cut cut{-INFINITY, 0x7fffffff};
+  Cut cut{-INFINITY, 0x7fffffff, 0};
   const auto kept = [&](float x, int col) { return x > cut.x || (x == cut.x && col <= cut.last); };
   const auto all = [](float, int) { return true; };
   bool known = false;                            // `mine` is this CTA's kept weight
   u64 mine = 0;
   const bool by_rank = top_k > 0 && top_k < P.x.vocab;
-  if (by_rank)
+  if (by_rank) {
     r.select<false>(all, [](float t) { return weight_of(t) ? 1u : 0u; }, e, [&](u64) { return (u64)top_k; }, cut, mine);
+    r.settle(all, cut);
+  }
   if (!(top_p >= 1.0f)) {
-    Cut inner;
+    Cut inner = cut;
     if (by_rank) {
       r.select<false>(kept, weight_of, e, wanted, inner, mine);
+      r.settle(kept, inner);
       if (inner.x != cut.x || inner.last < cut.last) cut = inner;
     } else {
       r.select<true>(all, weight_of, e, wanted, cut, mine);
@@ -889,7 +951,10 @@ __global__ void __launch_bounds__(NT, 768 / NT + (NT > 256)) sample_kernel(const
   };
   // nothing below this passes min-p: a hundredth of an octave is far more than the rounding of t
   const float least = fmaxf(cut.x, e.m + (log2f(min_p) - 0.01f) / e.c);
-  if (!known) mine = r.left_sums(e, cut, min_p, least);
+  if (!known) {
+    r.settle(all, cut);
+    mine = r.left_sums(e, cut, min_p, least);
+  }
   __syncthreads();
   r.exchange(mine);
   u64 total = 0, before = 0;
@@ -899,7 +964,10 @@ __global__ void __launch_bounds__(NT, 768 / NT + (NT > 256)) sample_kernel(const
   }
   const u64 target = draw(u, total);
   if (target < before || target >= before + mine) return;      // the token is another CTA's
-  if (known) r.left_sums(e, cut, min_p, least);
+  if (known) {
+    r.settle(all, cut);
+    r.left_sums(e, cut, min_p, least);
+  }
   const int at = r.locate(left, target - before);
   if (tid == 0) P.tokens[row] = at;
 }
@@ -965,9 +1033,9 @@ int launch_sample(const SampleParams& P, cudaStream_t st) {
     while (size < 8 && (units + size - 1) / size > 4096) size *= 2;
     while (size < 8 && P.x.rows * size < 2 * kSms && units > size * 256) size *= 2;
   }
-  // Rows that are all on the GPU at once and are not just listed want threads: 512 (one row of 256,000 flat fp16
-  // logits, top-p: 49 us, with 256 threads 74).  Many rows want three CTAs on an SM: 256 (512 rows of bf16, top-p:
-  // 417 us, with 512 threads 464); so do lists (top-k 50 of one row: 9.5 us, with 512 threads 11.5).
+  // Rows that are all on the GPU at once and are not just listed want threads: 512 (one row of 256,000 fp16
+  // logits, top-p: 26 us, with 256 threads 38).  Many rows want three CTAs on an SM: 256 (512 rows of bf16, top-p:
+  // 340 us, with 512 threads 390); so do lists (top-k 50 of one row: 9.5 us, with 512 threads 11.5).
   // Parts of which one fits an SM (fp32 rows over 768 KB) want 512 as well.
   const bool wide = !listed && ((P.x.rows * size <= 2 * kSms && units > size * 256) || units > size * 6144);
   return by_type(P.x.type, [&](auto t) {

@@ -25,6 +25,15 @@ template <typename T> __device__ __forceinline__ T from_f32(float v);
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+// The bits of a 16-bit number, of the largest one not above v.
+template <typename T> __device__ __forceinline__ uint32_t bits_below(float v) {
+  if constexpr (std::is_same<T, __half>::value) return __half_as_ushort(__float2half_rd(v));
+  else return __bfloat16_as_ushort(__float2bfloat16_rd(v));
+}
+template <typename T> __device__ __forceinline__ T from_bits(uint32_t bits) {
+  if constexpr (std::is_same<T, __half>::value) return __ushort_as_half((unsigned short)bits);
+  else return __ushort_as_bfloat16((unsigned short)bits);
+}
 
 // Order-preserving key of a logit that is no NaN; callers add 0 first, so that -0 and +0 share one.
 __device__ __forceinline__ uint32_t order_key(float v) {

@@ -586,3 +586,38 @@ def test_backward_from_saved_tensors_elsewhere():
     full = torch.full((1 << 20,), 3.0, device='cuda')
     again, = torch.autograd.grad(loss, y)
     assert torch.equal(offloaded, want) and torch.equal(again, want)
+
+
+def whole_weight_draw(x, u, t, p):
+    """The draw by top-p by the definition in whole weights (no rounding is left open: tokens are equal)."""
+    f = x.float()
+    m = f.amax(1, keepdim=True)
+    c = torch.tensor(1.4426950408889634, device='cuda') / torch.tensor(t, device='cuda')
+    w = torch.round(torch.exp2((f - m) * c) * 2.0 ** 31).long()
+    order = torch.sort(f + 0.0, dim=1, descending=True, stable=True)[1]
+    ws = w.gather(1, order)
+    before = ws.cumsum(1) - ws
+    keep = before.double() < float(np.float32(p)) * ws.sum(1, keepdim=True).double()
+    run = torch.zeros_like(w).scatter_(1, order, torch.where(keep, ws, 0)).cumsum(1)
+    target = (u.double()[:, None] * run[:, -1:].double()).long()
+    return (run <= target).sum(1)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('vocab', [701, 60001])
+def test_draw_cut_in_any_range(vocab, dtype):
+    """Top-p whose cut falls on positive, negative and tiny logits, on both sides of 0 at once, among few values that
+    many tokens share, on signed zeros, and among tokens that are all alike."""
+    import sq325
+    g = torch.Generator(device='cuda').manual_seed(vocab)
+    flat = torch.randn((6, vocab), generator=g, device='cuda')
+    u = torch.rand(6, generator=g, device='cuda')
+    zeros = torch.where(flat > 0.4, 0.0, torch.where(flat > -0.4, -0.0, -0.5))
+    rows = [(flat * 3 + 40, 1.0), (flat * 3 - 40, 1.0), (flat * 0.25 - 0.125, 0.05), (flat * 1e-6, 1e-6),
+            (flat.abs() * -1e-6, 3e-7), (flat * 0.01, 0.002), (torch.round(flat * 2) - 1, 1.0), (torch.round(flat) * 2 + 9, 2.0),
+            (zeros, 1.0), (flat.abs() * 100, 50.0)]
+    rows += [(torch.full_like(flat, v), 1.0) for v in (3.0, -3.0, 0.0, -0.0)]
+    for number, (x, t) in enumerate(rows):
+        x = x.to(dtype)
+        for p in (0.05, 0.25, 0.5, 0.9):
+            assert torch.equal(sq325.sample(x, u, temperature=t, top_p=p), whole_weight_draw(x, u, t, p)), (number, p)
