@@ -93,12 +93,11 @@ def decode_packet(w):
     return out
 
 
-_workspace = {}
-
-
 @torch.no_grad()
 def linear(w, x):
-    """y = x @ decode(w).T with fp32 accumulation and fp16 output (the nn.Linear the reference runs)."""
+    """y = x @ decode(w).T with fp32 accumulation and fp16 output (the nn.Linear the reference runs).
+    More than 256 rows decode the weights into a buffer first: it is the call's own, so that calls on other
+    streams or threads do not share it, and goes back to the allocator, which reuses it in stream order."""
     if x.dtype != torch.float16 or x.shape[-1] != w.cols or not x.is_cuda:
         raise ValueError('Input must be CUDA FP16 [..., cols]')
     lead = x.shape[:-1]
@@ -106,13 +105,7 @@ def linear(w, x):
     m = x2.shape[0]
     y = torch.empty((m, w.rows), device=x.device, dtype=torch.float16)
     need = _lib.load().sq_fp4_linear_workspace(m, w.rows, w.cols)
-    ws = None
-    if need:
-        key = x.device
-        ws = _workspace.get(key)
-        if ws is None or ws.numel() < need:
-            ws = torch.empty(need, device=x.device, dtype=torch.uint8)
-            _workspace[key] = ws
+    ws = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
     with torch.cuda.device(x.device):
         _lib.call('sq_fp4_linear', _lib.ptr(w.codes), _lib.ptr(w.block_scale_bytes), _lib.ptr(w.global_scale),
                   w.rows, w.cols, _lib.ptr(x2), w.cols, m, _lib.ptr(y), w.rows,
