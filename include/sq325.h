@@ -294,6 +294,12 @@ int sq_model_mixer_forward(sq_model* model, int layer, const uint16_t* u, int ba
  * fp16 logits lm_head(hidden).float(), computed without materialising the logits. */
 int sq_model_score(sq_model* model, const uint16_t* hidden, int rows, const int64_t* targets,
                    float* nll, void* stream);
+/* fp16 logits [rows,vocab] of hidden [rows,4096] (16-byte aligned) with the exactly decoded lm_head:
+ * the kernels and results of sq_fp4_linear on it, with `workspace` of
+ * sq_fp4_linear_workspace(rows, vocab, 4096) bytes (0 up to 256 rows).  Asynchronous; a failure is
+ * reported by sq_model_check(). */
+int sq_model_logits(sq_model* model, const uint16_t* hidden, int rows, uint16_t* logits_out,
+                    void* workspace, int64_t workspace_bytes, void* stream);
 /* Greedy head (infer_fp4_ridge_resurface_v1.py:103-105): fp16 logits [rows,vocab] (optional,
  * may be NULL) and first-occurrence argmax tokens [rows]. */
 int sq_model_greedy(sq_model* model, const uint16_t* hidden, int rows, uint16_t* logits_out,

@@ -385,6 +385,25 @@ int sq_fp4_validate(const uint8_t* codes, const uint8_t* block_scales, const flo
   return SQ_OK;
 }
 
+namespace {
+// y = x W^T with the exactly decoded W, on checked arguments; expired waits go to `err`.
+int fp4_linear(const Fp4Weight& w, const uint16_t* x, int64_t ldx, int m, uint16_t* y, int64_t ldy, void* workspace,
+               int64_t workspace_bytes, int* err, cudaStream_t st, const char* who) {
+  const bool tma_ok = w.cols % 256 == 0 && aligned(w.scales, 16) && aligned(x, 16) && ldx % 8 == 0;
+  if (m <= kSkinnyMax || (m <= 64 && !tma_ok)) {
+    if (tma_ok) return check(launch_fp4_gemv_stream(w, nullptr, x, ldx, m, y, ldy, err, st), "fp4 gemv");
+    return check(launch_fp4_gemv(w, x, ldx, m, y, ldy, st), "fp4 gemv");
+  }
+  if (m <= kFusedMax && tma_ok)
+    return check(launch_fp4_mma_linear(w, x, ldx, m, y, ldy, err, st), "fp4 tensor-core linear");
+  if (!workspace || workspace_bytes < sq_fp4_linear_workspace(m, w.rows, w.cols) || !aligned(workspace, 16))
+    return fail(SQ_EINVAL, std::string(who) + ": workspace too small");
+  uint16_t* stg = (uint16_t*)workspace;
+  SQ_TRY(launch_fp4_decode(w, stg, w.cols, st), "fp4 decode");
+  return check(launch_gemm_f16(x, ldx, stg, w.cols, y, ldy, m, w.rows, w.cols, 0, nullptr, err, st), "tcgen05 gemm");
+}
+}  // namespace
+
 int64_t sq_fp4_linear_workspace(int m, int n, int k) {
   // rows up to 256 run a kernel that needs no staging (k % 256 == 0 there)
   return (m <= 64 || (m <= kFusedMax && k % 256 == 0)) ? 0 : (int64_t)n * k * 2;
@@ -401,18 +420,7 @@ int sq_fp4_linear(const uint8_t* codes, const uint8_t* block_scales, const float
   cudaStream_t st = (cudaStream_t)stream;
   int* d_err = nullptr;
   if (int s = device_error_word(&d_err)) return s;
-  const bool tma_ok = k % 256 == 0 && aligned(block_scales, 16) && aligned(x, 16) && ldx % 8 == 0;
-  if (m <= kSkinnyMax || (m <= 64 && !tma_ok)) {
-    if (tma_ok) return check(launch_fp4_gemv_stream(w, nullptr, x, ldx, m, y, ldy, d_err, st), "fp4 gemv");
-    return check(launch_fp4_gemv(w, x, ldx, m, y, ldy, st), "fp4 gemv");
-  }
-  if (m <= kFusedMax && tma_ok)
-    return check(launch_fp4_mma_linear(w, x, ldx, m, y, ldy, d_err, st), "fp4 tensor-core linear");
-  if (!workspace || workspace_bytes < sq_fp4_linear_workspace(m, n, k) || !aligned(workspace, 16))
-    return fail(SQ_EINVAL, "fp4_linear: workspace too small");
-  uint16_t* stg = (uint16_t*)workspace;
-  SQ_TRY(launch_fp4_decode(w, stg, k, st), "fp4 decode");
-  return check(launch_gemm_f16(x, ldx, stg, k, y, ldy, m, n, k, 0, nullptr, d_err, st), "tcgen05 gemm");
+  return fp4_linear(w, x, ldx, m, y, ldy, workspace, workspace_bytes, d_err, st, "fp4_linear");
 }
 
 int sq_gemm_f16(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb, uint16_t* c, int64_t ldc, int m,
@@ -674,6 +682,15 @@ int sq_model_score(sq_model* m, const uint16_t* hidden, int rows, const int64_t*
            "lm_head gemm + ce");
   }
   return check(launch_ce_finalize(m->partials, nt, m->tlogit, rows, nll, st), "ce finalize");
+}
+
+int sq_model_logits(sq_model* m, const uint16_t* hidden, int rows, uint16_t* logits_out, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
+  if (!m || !hidden || !logits_out || rows <= 0) return fail(SQ_EINVAL, "logits: bad args");
+  if (!aligned(hidden, 16)) return fail(SQ_EINVAL, "logits: hidden must be 16-byte aligned");
+  if (!m->head.codes) return fail(SQ_ESTATE, "logits: set_globals() first");
+  return fp4_linear(fw(m->head), hidden, kDModel, rows, logits_out, m->cfg.vocab, workspace, workspace_bytes, m->d_err,
+                    (cudaStream_t)stream, "logits");
 }
 
 int sq_model_greedy(sq_model* m, const uint16_t* hidden, int rows, uint16_t* logits_out, int64_t* tokens_out,

@@ -145,6 +145,7 @@ _PROTOS = {
     'sq_model_forward': (C.c_int, [p, p, C.c_int, C.c_int, C.c_int, p, p]),
     'sq_model_mixer_forward': (C.c_int, [p, C.c_int, p, C.c_int, C.c_int, C.c_int, p, p]),
     'sq_model_score': (C.c_int, [p, p, C.c_int, p, p, p]),
+    'sq_model_logits': (C.c_int, [p, p, C.c_int, p, p, i64, p]),
     'sq_model_greedy': (C.c_int, [p, p, C.c_int, p, p, p]),
     'sq_model_check': (C.c_int, [p, p]),
     'sq_sample': (C.c_int, [C.POINTER(SampleArgs), p]),

@@ -15,7 +15,7 @@ import weakref
 
 import torch
 
-from . import _lib, fp4
+from . import _lib
 from .codec import allocate_state, layout_descriptor, layout_index, validate_state
 from .model import D_MODEL, D_XBC
 from .sampling import sample
@@ -279,9 +279,25 @@ class PredictorState:
 
     @torch.no_grad()
     def logits(self, hidden):
-        """fp16 logits [..., vocab] of hidden [..., 4096] with the exactly decoded lm_head (the
-        projection that score() runs), for a teacher's record (distillation.top_logits)."""
-        return fp4.linear(self.model.lm_head, hidden)
+        """fp16 logits [..., vocab] of hidden [..., 4096] with the exactly decoded lm_head, for a
+        teacher's record (distillation.top_logits).  The results of fp4.linear: one row runs the packed
+        skinny GEMM, 2 to 256 the tensor-core linear that decodes on its way, more decode the whole head
+        into a buffer of the call's own and run the GEMM that score() runs chunk by chunk.  check()
+        reports a failure in any of them."""
+        if self._handle is None:
+            raise RuntimeError('Controller is not installed')
+        if not isinstance(hidden, torch.Tensor) or hidden.dtype != torch.float16 or hidden.device != self.device \
+                or hidden.shape[-1:] != (D_MODEL,) or hidden.numel() == 0:
+            raise ValueError('hidden must be nonempty CUDA FP16 [..., 4096] on the model device')
+        h2 = hidden.reshape(-1, D_MODEL).contiguous()
+        rows, vocab = h2.shape[0], self.model.vocab
+        out = torch.empty((rows, vocab), device=self.device, dtype=torch.float16)
+        need = _lib.load().sq_fp4_linear_workspace(rows, vocab, D_MODEL)
+        ws = torch.empty(need, device=self.device, dtype=torch.uint8) if need else None
+        with torch.cuda.device(self.device):
+            _lib.call('sq_model_logits', self._handle, _lib.ptr(h2), rows, _lib.ptr(out), _lib.ptr(ws), need,
+                      _lib.stream_ptr())
+        return out.reshape(*hidden.shape[:-1], vocab)
 
     @torch.no_grad()
     def sample(self, hidden, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
