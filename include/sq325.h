@@ -385,7 +385,8 @@ int sq_top_logits(const sq_logits* logits, int k, void* values, int32_t* indices
  * sq_distill_forward writes loss and, if not NULL, stats [rows, 4] fp32 (16-byte aligned), which
  * sq_distill_backward reads to write grad; sq_distill_loss_grad writes loss and grad in one
  * call.  weight NULL: 1; weight_stride 0: one factor for every row.  grad has the logits'
- * type and must not overlap them. */
+ * type and must not overlap them.  Any positive finite temperature is computed; weight temperature
+ * must be an fp32 number, and a loss past fp32's range (from a temperature of about 1e19) is infinite. */
 typedef struct sq_distill_args {
   sq_logits logits;
   const void* values; const int32_t* indices;

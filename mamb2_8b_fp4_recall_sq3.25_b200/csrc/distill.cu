@@ -3,7 +3,7 @@
 // Student logits s over the whole vocabulary, teacher entries (v_k, j_k), temperature T,
 // c = log2(e) / T, everything in powers of two:
 //   q_k = 2^((v_k - v_max) c) / Q,  Q their sum      p_j = 2^((s_j - m) c) / S,  S the sum
-//   loss = T^2 ln 2 sum_k q_k [ ((v_k - v_max) c - log2 Q) - ((s_jk - m) c - log2 S) ]
+//   loss = T sum_k q_k [ T ln 2 ((v_k - v_max) c + log2 S - log2 Q) - (s_jk - m) ]
 //   d loss / d s_j = T (p_j - sum over k with j_k = j of q_k)
 // An entry whose index lies outside the vocabulary, or whose logit is -inf or NaN, is unused;
 // a row without used entries has loss 0 and gradient 0.  Sums are fp32; p and the difference
@@ -65,9 +65,19 @@ __device__ __forceinline__ float record_value(const DistillParams& P, long long 
 __device__ __forceinline__ bool used_entry(const DistillParams& P, int j, float v) {
   return j >= 0 && j < P.x.vocab && v > -INFINITY;
 }
+// c: finite for every T, so that 0 c stays 0 (infinite below T = 4e-39 otherwise).
+__device__ __forceinline__ float slope(float temperature) { return fminf(kLog2e / temperature, 3.4028234e38f); }
 // (v - v_max) c; the largest entry is 0 even where it is infinite.
 __device__ __forceinline__ float record_power(float v, float vmax, float c) { return v == vmax ? 0.0f : (v - vmax) * c; }
-
+// The loss over T of a row whose record's powers sum to Q, entry by entry: the student's gap is taken as it is and T enters
+// once, since c and T^2 leave fp32's range long before T does.
+struct LossTerm {
+  float scale, rest;                             // T ln 2, T ln 2 (log2 S - log2 Q)
+  __device__ LossTerm(float temperature, float sum, float Q)
+      : scale(temperature * kLn2), rest(scale * (log2f(sum) - log2f(Q))) {}
+  // e: the entry's exponent; gap: the student's logit less its reference
+  __device__ float operator()(float e, float gap) const { return fmaf(e, scale, rest) - gap; }
+};
 
 // (x - r) c for two: r is the largest logit, or 0 where there is none above -inf (powers of -inf are 0
 // then, and a NaN stays one).
@@ -237,16 +247,16 @@ struct Record {
     Q = block_sum<NT>(q, part[1]);
   }
   // Loss of the row, to thread 0; every thread of the CTA calls.
-  __device__ float loss(float r, float sum, float c, float temperature, float (*part)[NT / 32]) const {
+  __device__ float loss(float r, float sum, float temperature, float (*part)[NT / 32]) const {
     float l = 0.f;
-    const float rest = Q > 0.f ? log2f(sum) - log2f(Q) : 0.f;
+    const LossTerm term(temperature, sum, Q);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float w = ex2(e[i]);
-      if (at[i] >= 0 && w > 0.f) l += w * (e[i] - (taken[i] - r) * c + rest);
+      if (at[i] >= 0 && w > 0.f) l += w * term(e[i], taken[i] - r);
     }
     l = block_sum<NT>(l, part[0]);
-    return Q > 0.f ? temperature * temperature * kLn2 * (l / Q) : 0.f;
+    return Q > 0.f ? temperature * (l / Q) : 0.f;
   }
 };
 
@@ -259,7 +269,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) loss_kernel(const DistillParams
   __shared__ float part[2][NW];
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int row = blockIdx.x / size, tid = threadIdx.x;
-  const float c = kLog2e / P.temperature;
+  const float c = slope(P.temperature);
   const Span<T> span(P.x, row, rank, size);
   cluster_arrive_relaxed();
   const uint4* body = reinterpret_cast<const uint4*>(span.p + span.col(0, 0));
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) loss_kernel(const DistillParams
   cluster_wait();
   pairs.merge(size, c, r, own);
   if (rank != 0) return;
-  const float l = rec.loss(r, own, c, P.temperature, part);
+  const float l = rec.loss(r, own, P.temperature, part);
   if (tid == 0) {
     P.loss[row] = l;
     if (P.stats) P.stats[row] = make_float4(r, 1.0f / own, rec.vmax, rec.Q > 0.f ? 1.0f / rec.Q : 0.f);
@@ -383,15 +393,15 @@ struct RowRecord {
       if (token[k] == 0.f) token[k] = sum_of_index(at, P.k, k, at[k], [&](int i) { return ex2(e[i]); });
     __syncwarp();
   }
-  __device__ float loss(int n, float r, float sum, float c, float temperature) const {
+  __device__ float loss(int n, float r, float sum, float temperature) const {
     float l = 0.f;
     if (!(Q > 0.f)) return 0.f;
-    const float rest = log2f(sum) - log2f(Q);
+    const LossTerm term(temperature, sum, Q);
     for (int k = threadIdx.x & 31; k < n; k += 32) {
       const float w = ex2(e[k]);
-      if (at[k] >= 0 && w > 0.f) l += w * (e[k] - (taken[k] - r) * c + rest);
+      if (at[k] >= 0 && w > 0.f) l += w * term(e[k], taken[k] - r);
     }
-    return temperature * temperature * kLn2 * (warp_total(l) / Q);
+    return temperature * (warp_total(l) / Q);
   }
   // The gradient at the record's tokens, over what the data warps wrote there.
   __device__ void correct(int n, T* g, float r, float c, float scale, float f) const {
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(DW * 32 + 32, 24 / DW) row_kernel(const Distil
   __shared__ int has_record[2];
   const uint32_t rank = cluster_rank(), size = cluster_size();
   const int tid = threadIdx.x, step = gridDim.x / size, k4 = (P.k + 3) & ~3;
-  const float c = kLog2e / P.temperature;
+  const float c = slope(P.temperature);
   cluster_arrive_relaxed();
   int row = blockIdx.x / size;
   Span<T> span(P.x, row, rank, size);
@@ -436,7 +446,7 @@ __global__ void __launch_bounds__(DW * 32 + 32, 24 / DW) row_kernel(const Distil
       turn ^= 1;
       if (g_before) before.correct(P.k, g_before, r_before, c, scale_before, f_before);
       if (rank == 0) {
-        const float l = now.loss(P.k, r, sum, c, P.temperature);
+        const float l = now.loss(P.k, r, sum, P.temperature);
         if (tid == NT) P.loss[row] = l;
       }
       g_before = reinterpret_cast<T*>(P.grad) + (long long)row * P.grad_stride;
@@ -561,7 +571,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT) grad_kernel(const DistillParams
   int* at = reinterpret_cast<int*>(dyn);         // the record's indices (-1: unused) and 2^e
   float* w = reinterpret_cast<float*>(at + ((P.k + 3) & ~3));
   const int row = blockIdx.x / parts, part = blockIdx.x - row * parts, tid = threadIdx.x;
-  const float c = kLog2e / P.temperature;
+  const float c = slope(P.temperature);
   const Span<T> span(P.x, row, part, parts);
   const T* s = span.p;
   T* g = reinterpret_cast<T*>(P.grad) + (long long)row * P.grad_stride;
