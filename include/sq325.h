@@ -341,9 +341,9 @@ int sq_model_gemm_time(sq_model* model, double* seconds, int64_t* launches);
 /* ---------------------------------------------------------------- rows of logits
  * Operators on logits [rows, vocab] of type SQ_F16 / SQ_BF16 / SQ_F32 (no reference
  * counterpart: the reference's loops pick greedily).  Row r starts at data + r * row_stride
- * elements; rows <= 2^24, vocab <= 262144; data needs its type's alignment only.  All three
- * operators are asynchronous on `stream`, allocate nothing and keep nothing between calls.
- * rows == 0 is a valid call that does nothing. */
+ * elements; rows <= 2^24, vocab <= 262144; every array needs its type's alignment only, unless
+ * said otherwise.  All three operators are asynchronous on `stream`, allocate nothing and keep
+ * nothing between calls.  rows == 0 is a valid call that does nothing. */
 enum { SQ_F16 = 0, SQ_BF16 = 1, SQ_F32 = 2 };
 typedef struct sq_logits {
   const void* data;

@@ -877,6 +877,7 @@ int distill_params(const sq_distill_args* a, const char* who, DistillParams& P) 
   if (a->value_type < SQ_F16 || a->value_type > SQ_F32) return bad("unknown value type");
   if (!(a->temperature > 0.0f) || a->temperature > 3.0e38f) return bad("temperature must be positive and finite");
   if (a->weight_stride < 0) return bad("weight stride must not be negative");
+  if (!aligned(a->weight, 4) || !aligned(a->loss, 4)) return bad("misaligned weight or loss");
   if (P.x.rows > 0) {
     if (!a->values || !a->indices) return bad("null record");
     if (!aligned(a->values, a->value_type == SQ_F32 ? 4 : 2) || !aligned(a->indices, 4)) return bad("misaligned record");
@@ -900,6 +901,9 @@ int sq_sample(const sq_sample_args* a, void* stream) {
   if (int s = logits_rows(a->logits, "sample", P.x)) return s;
   if (P.x.rows == 0) return SQ_OK;
   if (!a->uniform || !a->tokens) return fail(SQ_EINVAL, "sample: null uniform or tokens");
+  if (!aligned(a->uniform, 4) || !aligned(a->temperature, 4) || !aligned(a->top_k, 4) || !aligned(a->top_p, 4) ||
+      !aligned(a->min_p, 4) || !aligned(a->tokens, 8))
+    return fail(SQ_EINVAL, "sample: misaligned arrays");
   P.uniform = a->uniform; P.temperature = a->temperature; P.top_p = a->top_p; P.min_p = a->min_p; P.top_k = a->top_k;
   P.temperature_all = a->temperature_all; P.top_p_all = a->top_p_all; P.min_p_all = a->min_p_all;
   P.top_k_all = a->top_k_all; P.tokens = (long long*)a->tokens;
@@ -913,6 +917,8 @@ int sq_top_logits(const sq_logits* l, int k, void* values, int32_t* indices, voi
   if (k < 1 || k > kMaxRecord || k > P.x.vocab) return fail(SQ_EINVAL, "top_logits: k must be in [1, min(1024, vocab)]");
   if (P.x.rows == 0) return SQ_OK;
   if (!values || !indices) return fail(SQ_EINVAL, "top_logits: null output");
+  if (!aligned(values, P.x.type == SQ_F32 ? 4 : 2) || !aligned(indices, 4))
+    return fail(SQ_EINVAL, "top_logits: misaligned output");
   P.k = k; P.values = values; P.indices = indices;
   return check(launch_top_logits(P, (cudaStream_t)stream), "top_logits");
 }
