@@ -687,7 +687,7 @@ int sq_model_score(sq_model* m, const uint16_t* hidden, int rows, const int64_t*
 int sq_model_logits(sq_model* m, const uint16_t* hidden, int rows, uint16_t* logits_out, void* workspace,
                     int64_t workspace_bytes, void* stream) {
   if (!m || !hidden || !logits_out || rows <= 0) return fail(SQ_EINVAL, "logits: bad args");
-  if (!aligned(hidden, 16)) return fail(SQ_EINVAL, "logits: hidden must be 16-byte aligned");
+  if (!aligned(hidden, 16) || !aligned(logits_out, 2)) return fail(SQ_EINVAL, "logits: misaligned hidden (16 bytes) or logits");
   if (!m->head.codes) return fail(SQ_ESTATE, "logits: set_globals() first");
   return fp4_linear(fw(m->head), hidden, kDModel, rows, logits_out, m->cfg.vocab, workspace, workspace_bytes, m->d_err,
                     (cudaStream_t)stream, "logits");

@@ -44,3 +44,19 @@ def test_logits_are_those_of_the_decoded_head(rows):
         strided = torch.cat([hidden, hidden], 1)[:, :4096].view(1, rows, 4096)
         assert torch.equal(ex.logits(strided)[0], got)
         ex.check()
+
+
+def test_entry_point_refuses_bad_buffers():
+    """Nothing is launched: a null or misaligned buffer, no rows, a workspace that is too small."""
+    import sq325
+    from sq325 import _lib
+    from sq325.model import benchmark_layouts, synthetic_statics
+    model = sq325.synthetic_model(seed=2, n_layer=1, vocab=512)
+    with sq325.PredictorState(model, *synthetic_statics(benchmark_layouts(1), seed=2)) as ex:
+        hidden = torch.zeros((300, 4096), device='cuda', dtype=torch.float16)
+        out = torch.empty((300, 512), device='cuda', dtype=torch.float16)
+        h, o, call = hidden.data_ptr(), out.data_ptr(), _lib.load().sq_model_logits
+        for args in ((None, 1, o, None, 0), (h + 2, 1, o, None, 0), (h, 0, o, None, 0), (h, 1, None, None, 0), (h, 1, o + 1, None, 0),
+                     (h, 300, o, None, 0), (h, 300, o, h, 300 * 4096)):
+            assert call(ex._handle, *args, None) == _lib.SQ_EINVAL, args
+        ex.check()
