@@ -356,10 +356,11 @@ typedef struct sq_logits {
  * by logit (equal ones by index).  top_k > 0 keeps the first top_k tokens; top_p < 1 those
  * whose predecessors hold less than top_p of the kept weight (the first always); min_p > 0 those
  * with y_j >= min(min_p, 1).  The token is the first in index order at which the running weight
- * passes floor(uniform * total).  Weights and sums are integers: the token depends on the
- * inputs alone.  temperature <= 0 or NaN: the largest logit, lowest index.  NaN logits count
- * as -inf; a row with nothing above -inf gives -1.  A null per-row array means the value
- * beside it for every row. */
+ * passes floor(uniform * total), the product in double.  Weights and sums are integers: the
+ * token depends on the inputs alone.  uniform is fp32: on a grid of 2^-24 a token of a smaller
+ * share is drawn only where a grid point falls on it.  temperature <= 0 or NaN: the largest logit,
+ * lowest index.  NaN logits count as -inf; a row with nothing above -inf gives -1.  A null per-row
+ * array means the value beside it for every row. */
 typedef struct sq_sample_args {
   sq_logits logits;
   const float* uniform;                                  /* [rows], in [0, 1) */

@@ -11,15 +11,17 @@
 //
 // loss_kernel: the forward.  The CTAs of a cluster stream their parts of the row with a running
 // maximum and sum per thread, eight loads of 16 bytes in flight each.  Bound by HBM: 512 rows of 256,000 fp16
-// logits (262 MB) take 60 us, 4.4 TB/s; 2,048 rows of bf16 187 us, 5.6 TB/s; fp32 6.1 TB/s.  With fewer rows the
-// start and the end of the one wave of CTAs weigh more, and in 16 bits the power unit is half busy.
+// logits (262 MB) take 56 us, 4.7 TB/s; 2,048 rows of bf16 182 us, 5.8 TB/s; 1,024 rows of fp32 164 us, 6.4 TB/s.  At 512
+// rows 1,024 CTAs meet 592 places (64 registers, four CTAs an SM): the second wave is three quarters full.  In 16 bits the
+// power unit is half busy.
 // row_kernel: loss and gradient in one pass.  The CTAs of a cluster hold the row in shared memory:
 // asynchronous copies bring it while the record is worked through, and the gradient is computed from
 // there, so the logits are read from HBM once.  Eight data warps and a record warp a CTA, three CTAs on an
 // SM, stepping through the rows: a thread refills the place of a unit as soon as it has written its gradient, and
 // nothing but one cluster barrier a row stands between a row's two passes.  2,048 rows of 256,000 bf16 logits
-// (1.05 GB in, 1.05 GB out) take 0.50 ms, 4.2 TB/s; what is left is the wait at that barrier and the issue of
-// 17 instructions a logit (two powers among them).  Reading the logits a second time from L2 instead of keeping them
+// (1.05 GB in, 1.05 GB out) take 0.49 ms, 4.3 TB/s; what is left is the wait at that barrier and the issue of
+// 17 instructions a logit (two powers among them).  That is with records of 64: equal indices are looked for by a scan of
+// the record for each entry, and records of 256 take 0.97 ms, of 1,024 7.0 ms.  Reading the logits a second time from L2 instead of keeping them
 // (no shared memory, four CTAs on an SM) took 0.62 ms.
 // In both each warp sends its (maximum, sum) to every CTA of the cluster through distributed shared
 // memory.  The sums are formed in a fixed order: the same call gives the same bits.
@@ -631,8 +633,8 @@ __global__ void __launch_bounds__(NT, 1024 / NT) grad_kernel(const DistillParams
 
 template <typename T>
 int launch_loss(const DistillParams& P, cudaStream_t st) {
-  // long parts stream best: more CTAs a row only until there are six for each SM (512 rows of 256,000 fp16: 60 us;
-  // until three or twelve: 64); short rows, many at once, take CTAs of two warps
+  // long parts stream best: more CTAs a row only until there are six for each SM (512 rows of 256,000 fp16: 56 us;
+  // until three 60, until twelve 61); short rows, many at once, take CTAs of two warps
   // (16,384 rows of 8,191 bf16 logits: 98 us, with eight 181)
   const int units = row_units(P.x);
   if (units <= 1280 && P.x.rows > 4 * kSms && P.k <= 128) return launch_clusters(loss_kernel<T, 64, 2>, P, 1, 64, 0, st);
@@ -655,7 +657,8 @@ template <typename T>
 int launch_loss_grad(const DistillParams& P, cudaStream_t st) {
   // As many CTAs a row as keep its part within 64 KB, three of eight data warps on an SM; few rows take
   // more, down to a unit a thread.  Short rows, many at once, are better served by CTAs of two data warps
-  // (16,384 rows of 8,191 bf16 logits: 225 us, with eight 428).  Rows over 512 KB (fp32 only) leave parts of which one fits an SM, with 16 warps.
+  // (16,384 rows of 8,191 bf16 logits: 225 us, with eight 428).  fp32 rows of 512 to 768 KB leave parts of 64 to 96 KB,
+  // two or three of them on an SM; longer ones parts of which one fits an SM, with 16 warps.
   const int units = row_units(P.x);
   int size = 1;
   while (size < 8 && (units + size - 1) / size > 4096) size *= 2;

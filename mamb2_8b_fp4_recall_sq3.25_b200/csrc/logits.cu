@@ -7,7 +7,9 @@
 // at which the running weight passes floor(u W), W the weight that is left.  Weights are
 // integers and their sums 64-bit, so no sum depends on the order it is formed in, and the
 // token is a function of the inputs alone.  A token 2^-32 times less likely than the most
-// likely one has weight 0; rounding moves at most 2^-32 of the largest weight a token.
+// likely one has weight 0; rounding moves at most 2^-32 of the largest weight a token.  Products with u and with p are
+// 64-bit floating point.  u is an fp32 number: on a grid of 2^-24 a token with a smaller share of the weight than that is
+// drawn only where a grid point falls on it.
 //
 // A cluster of 1..8 CTAs shares a row; CTAs exchange single numbers, lists and histograms through
 // distributed shared memory.

@@ -9,7 +9,8 @@ logits / T over the whole vocabulary,
 (q_j = 0 outside the record).  `distillation_loss` is differentiable in the student's logits: its
 backward reads the logits again and recomputes p from the row's maximum and sum.
 `distillation_loss_grad` gives loss and gradient in one call, for steps that know each row's
-weight beforehand.  Sums are fp32, the gradient is rounded once to the logits' type.  Places of
+weight beforehand.  Sums are fp32, the gradient is rounded once to the logits' type.  Any
+positive finite temperature is computed; a loss past fp32's range (temperatures of about 1e19) is infinite.  Places of
 the record with an index outside the vocabulary or a value of -inf or NaN are unused; a row
 without used places has loss 0 and gradient 0.
 """

@@ -5,8 +5,10 @@ With m the row's largest logit, y_j = 2^((x_j - m) log2(e) / temperature) and th
 w_j = rint(y_j 2^31).  Tokens are ordered by logit, equal ones by index.  The settings apply in
 this order: top-k keeps the first k tokens, top-p those whose predecessors hold less than
 top_p of the kept weight (the first always), min-p those with y_j >= min_p.  The token drawn is
-the first in index order at which the running weight passes floor(uniform * total).  Weights and
-sums are integers, so the same inputs give the same token whatever the launch shape.
+the first in index order at which the running weight passes floor(uniform * total), the product
+in 64-bit floating point.  Weights and sums are integers, so the same inputs give the same token
+whatever the launch shape.  Uniform numbers are fp32: on a grid of 2^-24, a token whose share of the
+weight is smaller than that is drawn only where a grid point falls on it.
 """
 from __future__ import annotations
 

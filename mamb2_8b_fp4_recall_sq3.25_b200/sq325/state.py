@@ -302,7 +302,9 @@ class PredictorState:
     @torch.no_grad()
     def sample(self, hidden, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """One drawn token per hidden row: lm_head (at most 64 rows as greedy(), more as logits()) and
-        sampling.sample with its settings.  uniform: fp32 [rows]; returns int64 [rows]."""
+        sampling.sample with its settings.  uniform: fp32 [rows]; returns int64 [rows].  The two heads
+        round differently unless set_exact_projections(True), so a row may draw another token in a
+        batch on the other side of 64 rows."""
         h2 = hidden.reshape(-1, D_MODEL).contiguous()
         rows = h2.shape[0]
         if rows > 64:
