@@ -1,6 +1,6 @@
 """Cases of the operators that a Mamba-2 mixer learns and answers with in unquantised states: the short
 causal convolution (`sq325.causal_conv`), the selective scan over prompts and its gradients
-(`sq325.selective_scan`), both for one token (`sq325.causal_conv_step`, `sq325.selective_step`),
+(`sq325.selective_scan`), both for one token (`sq325.conv_scan_step`),
 activations kept in 8 bits (`sq325.pack_activations`, `sq325.unpack_activations`), and convolution and
 scan in one step of training that keeps its input in 8 bits (`sq325.conv_scan`).
 
@@ -319,11 +319,8 @@ def _own(s):
         packed = sq325.pack_activations(s['x'])
         return sq325.unpack_activations(packed), packed.scales
     if op == 'token':
-        heads, groups, dim = case['heads'], case['groups'], case['dim']
-        z = sq325.causal_conv_step(s['x'], s['carried'], s['weight'], s['bias'])
-        x, B, C = z.split([heads * dim, groups * N, groups * N], -1)
-        y = sq325.selective_step(x.unflatten(1, (heads, dim)), s['dt'], s['A'], B.unflatten(1, (groups, N)),
-                                 C.unflatten(1, (groups, N)), s['state'], s['D'], s['dt_bias'])
+        y = sq325.conv_scan_step(s['x'], s['dt'], s['A'], s['weight'], s['bias'], s['D'], s['dt_bias'], heads=case['heads'],
+                                 groups=case['groups'], conv_state=s['carried'], state=s['state'])
         return y, s['carried'], s['state']
     if op == 'scan':
         return sq325.selective_scan(s['x'], s['dt'], s['A'], s['B'], s['C'], s['D'], s['dt_bias'],
