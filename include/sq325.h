@@ -401,6 +401,120 @@ int sq_distill_forward(const sq_distill_args* args, void* stream);
 int sq_distill_backward(const sq_distill_args* args, void* stream);
 int sq_distill_loss_grad(const sq_distill_args* args, void* stream);
 
+/* ---------------------------------------------------------------- unquantised mixer states
+ * The mixer's recurrence and short convolution in unquantised states, with their gradients, and activations in 8 bits
+ * (no reference counterpart: the reference's scans carry quantised states, its training scan freezes A, D and dt_bias,
+ * its convolution is mamba_ssm's).  All are asynchronous on `stream`, allocate nothing and keep nothing between calls
+ * but the device's error word (sq_device_check).  Element (b,t,...) of a tensor lies at data + b * batch_stride +
+ * t * token_stride, its last axes contiguous; tensors need their type's alignment only, workspaces 256 bytes.
+ * lengths (int32 [batch], NULL: every sequence has `length` tokens) are held within [0, length]; tokens behind a
+ * sequence's end are not read, and are zero in outputs and gradients.
+ *
+ * sq_selective_forward: per head, with s_t = softplus(dt_t + dt_bias),
+ *   H_t = exp(A s_t) H_{t-1} + s_t x_t B_t^T,   y_t = H_t C_t + D x_t
+ * x, y [batch,length,heads,dim], dt [batch,length,heads], B, C [batch,length,groups,128] of `type` SQ_F16 or SQ_BF16;
+ * A fp32 [heads], <= 0; D, dt_bias [heads] of d_type / bias_type, or NULL (no term); state fp32 [batch,heads,dim,128]:
+ * state_in (NULL: zero) before the first token, state_out (may be NULL) after the last.  dim <= 1024, heads a multiple
+ * of groups; batch, and heads times dim / 64 rounded up, at most 65535; length <= 2^24.  The state and its sums are fp32; y, a 16-bit tensor, is made
+ * from pairs' weights and states that are rounded to 16 bits (fp16: scaled) in the products.  A NaN or infinity in a
+ * token reaches every token of its chunk of 128, and later ones.
+ * sq_selective_backward: gradients for the gradient dy of y and dstate_out of state_out (NULL: zero), with the forward's
+ * inputs: dx, ddt (contiguous), dB, dC in `type`, and where not NULL dA fp32, dD, ddt_bias in their types and
+ * dstate_in.  Sums have a fixed order.  workspace: sq_selective_workspace(..., backward) bytes. */
+typedef struct sq_selective_args {
+  int32_t batch, length, heads, dim, groups, type;
+  const void* x;  int64_t x_batch_stride, x_token_stride;
+  const void* dt; int64_t dt_batch_stride, dt_token_stride;
+  const float* A;
+  const void* B;  int64_t b_batch_stride, b_token_stride;
+  const void* C;  int64_t c_batch_stride, c_token_stride;
+  const void* D;       int32_t d_type;
+  const void* dt_bias; int32_t bias_type;
+  const float* state_in;
+  const int32_t* lengths;
+  void* y; int64_t y_batch_stride, y_token_stride;         /* forward */
+  float* state_out;
+  const void* dy; int64_t dy_batch_stride, dy_token_stride; /* backward */
+  const float* dstate_out;
+  void* dx; int64_t dx_batch_stride, dx_token_stride;
+  void* ddt;
+  void* dB; void* dC; int64_t dg_batch_stride, dg_token_stride;
+  float* dA; void* dD; void* ddt_bias; float* dstate_in;
+  void* workspace; int64_t workspace_bytes;
+} sq_selective_args;
+int64_t sq_selective_workspace(int batch, int length, int heads, int dim, int groups, int backward);
+int sq_selective_forward(const sq_selective_args* args, void* stream);
+int sq_selective_backward(const sq_selective_args* args, void* stream);
+
+/* One token of the same recurrence: x, y [batch,heads,dim], dt [batch,heads], B, C [batch,groups,128], the state (16-byte
+ * aligned) updated in place; y contiguous. */
+typedef struct sq_selective_step_args {
+  int32_t batch, heads, dim, groups, type;
+  const void* x;  int64_t x_batch_stride;
+  const void* dt; int64_t dt_batch_stride;
+  const float* A;
+  const void* B;  int64_t b_batch_stride;
+  const void* C;  int64_t c_batch_stride;
+  const void* D;       int32_t d_type;
+  const void* dt_bias; int32_t bias_type;
+  float* state;
+  void* y;
+} sq_selective_step_args;
+int sq_selective_step(const sq_selective_step_args* args, void* stream);
+
+/* Causal depthwise convolution over the tokens of x [batch,length,channels] (SQ_F16, SQ_BF16 or SQ_F32):
+ *   z[t,c] = bias[c] + sum_k weight[c,k] x[t - (taps-1) + k, c],   y = z sigmoid(z) where silu, else z
+ * weight [channels,taps], taps 2..4, bias [channels] or NULL, both of weight_type, which is `type` or SQ_F32.  state_in /
+ * state_out [batch,taps-1,channels] in `type` hold the inputs before the first token (NULL: zero) and the last ones.
+ * sq_causal_conv_forward with x and codes keeps the input in 8 bits (see below); with x NULL and codes it reads the kept
+ * values in x's place.  sq_causal_conv_backward computes z again from x, or from the codes where x is NULL, and writes
+ * dx (contiguous, in `type`) and, where not NULL, dweight, dbias in weight_type and dstate_in; dstate_out may be NULL.
+ * workspace: sq_causal_conv_workspace(...) bytes (backward). */
+typedef struct sq_causal_conv_args {
+  int32_t batch, length, channels, taps, silu, type, weight_type;
+  const void* x; int64_t x_batch_stride, x_token_stride;
+  int8_t* codes; float* scales;
+  const void* weight; const void* bias;
+  const void* state_in;
+  const int32_t* lengths;
+  void* y; int64_t y_batch_stride, y_token_stride;         /* forward */
+  void* state_out;
+  const void* dy; int64_t dy_batch_stride, dy_token_stride; /* backward */
+  const void* dstate_out;
+  void* dx; void* dstate_in; void* dweight; void* dbias;
+  void* workspace; int64_t workspace_bytes;
+} sq_causal_conv_args;
+int64_t sq_causal_conv_workspace(int batch, int length, int channels, int type);
+int sq_causal_conv_forward(const sq_causal_conv_args* args, void* stream);
+int sq_causal_conv_backward(const sq_causal_conv_args* args, void* stream);
+/* One token of each row of x [batch,channels]; the state is updated in place, y is contiguous. */
+int sq_causal_conv_step(const void* x, int64_t x_batch_stride, void* state, const void* weight, const void* bias, void* y,
+                        int batch, int channels, int taps, int silu, int type, int weight_type, void* stream);
+
+/* One token of convolution (silu) and recurrence, as sq_causal_conv_step and sq_selective_step one behind the other but
+ * with the convolution's output in fp32 between them: xbc [batch, heads*dim + 2*groups*128] holds x, B and C side by side.
+ * conv_state [batch,taps-1,channels] in `type` (SQ_F16, SQ_BF16) and state are updated in place.  workspace: batch *
+ * channels fp32, 256-byte aligned. */
+typedef struct sq_conv_scan_step_args {
+  int32_t batch, heads, dim, groups, taps, type, weight_type;
+  const void* xbc; int64_t xbc_batch_stride;
+  const void* dt;  int64_t dt_batch_stride;
+  const float* A;
+  const void* weight; const void* bias;
+  const void* D;       int32_t d_type;
+  const void* dt_bias; int32_t bias_type;
+  void* conv_state; float* state;
+  void* y;
+  void* workspace; int64_t workspace_bytes;
+} sq_conv_scan_step_args;
+int sq_conv_scan_step(const sq_conv_scan_step_args* args, void* stream);
+
+/* Activations in 8 bits: in a row of x [rows,width] each 128 neighbouring values (the last block may have fewer) share
+ * scale = max|x| / 127 (fp32) and are kept as codes rint(x / scale) in [-127, 127]; scales [rows, ceil(width/128)].  A block
+ * with a NaN or an infinity comes back as NaN.  sq_unpack_activations writes code * scale, rounded to `type`. */
+int sq_pack_activations(const void* x, int64_t row_stride, int64_t rows, int width, int type, int8_t* codes, float* scales, void* stream);
+int sq_unpack_activations(const int8_t* codes, const float* scales, int64_t rows, int width, int type, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

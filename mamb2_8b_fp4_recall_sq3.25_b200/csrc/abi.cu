@@ -14,6 +14,8 @@
 #include "fp4.cuh"
 #include "layer.cuh"
 #include "logits.cuh"
+#include "conv.cuh"
+#include "selective.cuh"
 #include "s16.cuh"
 #include "ste.cuh"
 #include "scan.cuh"
@@ -79,6 +81,12 @@ int device_error_word(int** out) {
   std::lock_guard<std::mutex> lock(g_err_mutex);
   if (!g_dev_err[dev]) {
     int* p = nullptr;
+    // the first call may come while a stream is captured, which this set-up is no part of
+    struct Relaxed {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+      ~Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    } relaxed;
     // [0]: the sticky error word; [1]: per-call flags of sq_fp4_validate
     if (cudaMalloc(&p, 2 * sizeof(int)) != cudaSuccess) return cuda_fail("cudaMalloc (error word)");
     if (cudaMemset(p, 0, 2 * sizeof(int)) != cudaSuccess) { cudaFree(p); return cuda_fail("cudaMemset (error word)"); }
@@ -949,6 +957,238 @@ int sq_distill_loss_grad(const sq_distill_args* a, void* stream) {
   if (int s = distill_grad_params(P, "distill_loss_grad")) return s;
   P.stats = nullptr;
   return check(launch_distill_loss_grad(P, (cudaStream_t)stream), "distill_loss_grad");
+}
+
+namespace {
+constexpr int kMaxGrid = 65535;      // of a grid's second and third dimension
+
+int selective_params(const sq_selective_args* a, const char* who, bool backward, SelectiveParams& P) {
+  if (!a) return fail(SQ_EINVAL, std::string(who) + ": null argument");
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  if (a->type != SQ_F16 && a->type != SQ_BF16) return bad("type must be SQ_F16 or SQ_BF16");
+  if (a->batch < 1 || a->length < 1 || a->heads < 1 || a->dim < 1 || a->groups < 1) return bad("positive geometry required");
+  if (a->heads % a->groups) return bad("heads must be divisible by B/C groups");
+  if (a->dim > kScanMaxDim || a->length > 1 << 24 || a->batch > kMaxGrid) return bad("batch, length or dim is too large");
+  if ((int64_t)a->heads * ((a->dim + kScanTile - 1) / kScanTile) > kMaxGrid) return bad("heads is too large");
+  if (!a->x || !a->dt || !a->A || !a->B || !a->C || !a->workspace) return bad("null pointer argument");
+  if (!aligned(a->x, 2) || !aligned(a->dt, 2) || !aligned(a->B, 2) || !aligned(a->C, 2) || !aligned(a->A, 4) ||
+      !aligned(a->state_in, 4) || !aligned(a->lengths, 4) || !aligned(a->workspace, 256))
+    return bad("misaligned argument");
+  const auto number_type = [](int t) { return t >= SQ_F16 && t <= SQ_F32; };
+  if ((a->D && (!number_type(a->d_type) || !aligned(a->D, a->d_type == SQ_F32 ? 4 : 2))) ||
+      (a->dt_bias && (!number_type(a->bias_type) || !aligned(a->dt_bias, a->bias_type == SQ_F32 ? 4 : 2))))
+    return bad("unknown type or misaligned D or dt_bias");
+  if (a->workspace_bytes < selective_workspace(a->batch, a->length, a->heads, a->dim, a->groups, backward)) return bad("workspace too small");
+  P = SelectiveParams{};
+  P.batch = a->batch; P.length = a->length; P.heads = a->heads; P.dim = a->dim; P.groups = a->groups; P.type = a->type;
+  P.x = a->x; P.x_sb = a->x_batch_stride; P.x_st = a->x_token_stride;
+  P.dt = a->dt; P.dt_sb = a->dt_batch_stride; P.dt_st = a->dt_token_stride;
+  P.A = a->A;
+  P.B = a->B; P.b_sb = a->b_batch_stride; P.b_st = a->b_token_stride;
+  P.C = a->C; P.c_sb = a->c_batch_stride; P.c_st = a->c_token_stride;
+  P.D = a->D; P.d_type = a->d_type; P.dt_bias = a->dt_bias; P.bias_type = a->bias_type;
+  P.state_in = a->state_in; P.lengths = a->lengths; P.workspace = a->workspace;
+  return device_error_word(&P.err);
+}
+}  // namespace
+
+int64_t sq_selective_workspace(int batch, int length, int heads, int dim, int groups, int backward) {
+  if (batch < 1 || length < 1 || heads < 1 || dim < 1 || groups < 1 || heads % groups) return -1;
+  return selective_workspace(batch, length, heads, dim, groups, backward != 0);
+}
+
+int sq_selective_forward(const sq_selective_args* a, void* stream) {
+  SelectiveParams P;
+  if (int s = selective_params(a, "selective_forward", false, P)) return s;
+  if (!a->y) return fail(SQ_EINVAL, "selective_forward: null y");
+  if (!aligned(a->y, 2) || !aligned(a->state_out, 4)) return fail(SQ_EINVAL, "selective_forward: misaligned output");
+  P.y = a->y; P.y_sb = a->y_batch_stride; P.y_st = a->y_token_stride; P.state_out = a->state_out;
+  return check(launch_selective_forward(P, (cudaStream_t)stream), "selective_forward");
+}
+
+int sq_selective_backward(const sq_selective_args* a, void* stream) {
+  SelectiveParams P;
+  if (int s = selective_params(a, "selective_backward", true, P)) return s;
+  if (!a->dy || !a->dx || !a->ddt || !a->dB || !a->dC) return fail(SQ_EINVAL, "selective_backward: null gradient");
+  if (!aligned(a->dy, 2) || !aligned(a->dstate_out, 4) || !aligned(a->dx, 2) || !aligned(a->ddt, 2) || !aligned(a->dB, 2) ||
+      !aligned(a->dC, 2) || !aligned(a->dA, 4) || !aligned(a->dD, a->d_type == SQ_F32 ? 4 : 2) ||
+      !aligned(a->ddt_bias, a->bias_type == SQ_F32 ? 4 : 2) || !aligned(a->dstate_in, 4))
+    return fail(SQ_EINVAL, "selective_backward: misaligned gradient");
+  P.dy = a->dy; P.dy_sb = a->dy_batch_stride; P.dy_st = a->dy_token_stride; P.dstate_out = a->dstate_out;
+  P.dx = a->dx; P.dx_sb = a->dx_batch_stride; P.dx_st = a->dx_token_stride; P.ddt = a->ddt;
+  P.dB = a->dB; P.dC = a->dC; P.dg_sb = a->dg_batch_stride; P.dg_st = a->dg_token_stride;
+  P.dA = a->dA; P.dD = a->D ? a->dD : nullptr; P.dbias = a->dt_bias ? a->ddt_bias : nullptr; P.dstate_in = a->dstate_in;
+  return check(launch_selective_backward(P, (cudaStream_t)stream), "selective_backward");
+}
+
+namespace {
+// Checks of a token's step; x, B and C are not looked at.
+int step_params(const char* who, int batch, int heads, int dim, int groups, int type, const void* dt, const float* A, const void* D,
+                int d_type, const void* dt_bias, int bias_type, const float* state, const void* y) {
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  if (type != SQ_F16 && type != SQ_BF16) return bad("type must be SQ_F16 or SQ_BF16");
+  if (batch < 1 || heads < 1 || dim < 1 || groups < 1) return bad("positive geometry required");
+  if (heads % groups) return bad("heads must be divisible by B/C groups");
+  if (batch > kMaxGrid || heads > kMaxGrid || dim > 1 << 20) return bad("batch, heads or dim is too large");
+  if (!dt || !A || !state || !y) return bad("null pointer argument");
+  if (!aligned(dt, 2) || !aligned(y, 2) || !aligned(A, 4)) return bad("misaligned argument");
+  if (!aligned(state, 16)) return bad("state must be 16-byte aligned");
+  const auto number_type = [](int t) { return t >= SQ_F16 && t <= SQ_F32; };
+  if ((D && (!number_type(d_type) || !aligned(D, d_type == SQ_F32 ? 4 : 2))) ||
+      (dt_bias && (!number_type(bias_type) || !aligned(dt_bias, bias_type == SQ_F32 ? 4 : 2))))
+    return bad("unknown type or misaligned D or dt_bias");
+  return SQ_OK;
+}
+}  // namespace
+
+int sq_selective_step(const sq_selective_step_args* a, void* stream) {
+  if (!a) return fail(SQ_EINVAL, "selective_step: null argument");
+  if (int s = step_params("selective_step", a->batch, a->heads, a->dim, a->groups, a->type, a->dt, a->A, a->D, a->d_type, a->dt_bias,
+                          a->bias_type, a->state, a->y))
+    return s;
+  if (!a->x || !a->B || !a->C) return fail(SQ_EINVAL, "selective_step: null pointer argument");
+  if (!aligned(a->x, 2) || !aligned(a->B, 2) || !aligned(a->C, 2)) return fail(SQ_EINVAL, "selective_step: misaligned argument");
+  SelectiveStepParams P{};
+  P.batch = a->batch; P.heads = a->heads; P.dim = a->dim; P.groups = a->groups; P.type = a->type;
+  P.x = a->x; P.x_sb = a->x_batch_stride; P.dt = a->dt; P.dt_sb = a->dt_batch_stride; P.A = a->A;
+  P.B = a->B; P.b_sb = a->b_batch_stride; P.C = a->C; P.c_sb = a->c_batch_stride;
+  P.D = a->D; P.d_type = a->d_type; P.dt_bias = a->dt_bias; P.bias_type = a->bias_type;
+  P.state = a->state; P.y = a->y;
+  return check(launch_selective_step(P, (cudaStream_t)stream), "selective_step");
+}
+
+namespace {
+// Checks that the convolution's entry points share.
+int conv_shape(const char* who, int batch, int channels, int taps, int type, int weight_type, const void* weight, const void* bias) {
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  if (type < SQ_F16 || type > SQ_F32) return bad("unknown type");
+  if (weight_type != type && weight_type != SQ_F32) return bad("weight_type must be the input's type or SQ_F32");
+  if (batch < 1 || channels < 1) return bad("positive geometry required");
+  if (taps < 2 || taps > 4) return bad("taps must be in [2, 4]");
+  if (batch > kMaxGrid || channels > 1 << 24) return bad("batch or channels is too large");
+  if (!weight) return bad("null weight");
+  const size_t w = weight_type == SQ_F32 ? 4 : 2;
+  if (!aligned(weight, w) || !aligned(bias, w)) return bad("misaligned weight or bias");
+  return SQ_OK;
+}
+int conv_params(const sq_causal_conv_args* a, const char* who, ConvParams& P) {
+  if (!a) return fail(SQ_EINVAL, std::string(who) + ": null argument");
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  if (int s = conv_shape(who, a->batch, a->channels, a->taps, a->type, a->weight_type, a->weight, a->bias)) return s;
+  if (a->length < 1 || a->length > 1 << 24) return bad("length must be in [1, 2^24]");
+  if (!a->x && !a->codes) return bad("null input");
+  if (!a->codes != !a->scales) return bad("codes and scales go together");
+  const size_t n = a->type == SQ_F32 ? 4 : 2;
+  if (!aligned(a->x, n) || !aligned(a->scales, 4) || !aligned(a->state_in, n) || !aligned(a->lengths, 4)) return bad("misaligned argument");
+  P = ConvParams{};
+  P.batch = a->batch; P.length = a->length; P.channels = a->channels; P.taps = a->taps; P.silu = a->silu; P.type = a->type;
+  P.weight_type = a->weight_type;
+  P.x = a->x; P.x_sb = a->x_batch_stride; P.x_st = a->x_token_stride; P.codes = a->codes; P.scales = a->scales;
+  P.weight = a->weight; P.bias = a->bias; P.state_in = a->state_in; P.lengths = a->lengths;
+  return SQ_OK;
+}
+}  // namespace
+
+int64_t sq_causal_conv_workspace(int batch, int length, int channels, int type) {
+  if (batch < 1 || length < 1 || channels < 1 || type < SQ_F16 || type > SQ_F32) return -1;
+  return conv_workspace(batch, length, channels, type);
+}
+
+int sq_causal_conv_forward(const sq_causal_conv_args* a, void* stream) {
+  ConvParams P;
+  if (int s = conv_params(a, "causal_conv_forward", P)) return s;
+  const size_t n = a->type == SQ_F32 ? 4 : 2;
+  if (!a->y) return fail(SQ_EINVAL, "causal_conv_forward: null y");
+  if (!aligned(a->y, n) || !aligned(a->state_out, n)) return fail(SQ_EINVAL, "causal_conv_forward: misaligned output");
+  if (a->state_out && a->state_out == a->state_in) return fail(SQ_EINVAL, "causal_conv_forward: state_out must not be state_in");
+  P.y = a->y; P.y_sb = a->y_batch_stride; P.y_st = a->y_token_stride; P.state_out = a->state_out;
+  return check(launch_conv_forward(P, (cudaStream_t)stream), "causal_conv_forward");
+}
+
+int sq_causal_conv_backward(const sq_causal_conv_args* a, void* stream) {
+  ConvParams P;
+  if (int s = conv_params(a, "causal_conv_backward", P)) return s;
+  const auto bad = [](const char* what) { return fail(SQ_EINVAL, std::string("causal_conv_backward: ") + what); };
+  if (!a->dy || !a->dx) return bad("null gradient");
+  const size_t n = a->type == SQ_F32 ? 4 : 2, w = a->weight_type == SQ_F32 ? 4 : 2;
+  if (!aligned(a->dy, n) || !aligned(a->dstate_out, n) || !aligned(a->dx, n) || !aligned(a->dstate_in, n) || !aligned(a->dweight, w) || !aligned(a->dbias, w))
+    return bad("misaligned gradient");
+  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < conv_workspace(a->batch, a->length, a->channels, a->type))
+    return bad("workspace missing, misaligned or too small");
+  if (a->x) P.codes = nullptr;
+  P.dy = a->dy; P.dy_sb = a->dy_batch_stride; P.dy_st = a->dy_token_stride; P.dstate_out = a->dstate_out;
+  P.dx = a->dx; P.dstate_in = a->dstate_in; P.dweight = a->dweight; P.dbias = a->dbias;
+  P.workspace = reinterpret_cast<float*>(a->workspace);
+  return check(launch_conv_backward(P, (cudaStream_t)stream), "causal_conv_backward");
+}
+
+int sq_causal_conv_step(const void* x, int64_t x_batch_stride, void* state, const void* weight, const void* bias, void* y,
+                        int batch, int channels, int taps, int silu, int type, int weight_type, void* stream) {
+  if (int s = conv_shape("causal_conv_step", batch, channels, taps, type, weight_type, weight, bias)) return s;
+  const size_t n = type == SQ_F32 ? 4 : 2;
+  if (!x || !state || !y) return fail(SQ_EINVAL, "causal_conv_step: null pointer argument");
+  if (!aligned(x, n) || !aligned(state, n) || !aligned(y, n)) return fail(SQ_EINVAL, "causal_conv_step: misaligned argument");
+  ConvStepParams P{};
+  P.batch = batch; P.channels = channels; P.taps = taps; P.silu = silu; P.type = type; P.weight_type = weight_type;
+  P.x = x; P.x_sb = x_batch_stride; P.weight = weight; P.bias = bias; P.state = state; P.y = y;
+  return check(launch_conv_step(P, (cudaStream_t)stream), "causal_conv_step");
+}
+
+int sq_conv_scan_step(const sq_conv_scan_step_args* a, void* stream) {
+  if (!a) return fail(SQ_EINVAL, "conv_scan_step: null argument");
+  const auto bad = [](const char* what) { return fail(SQ_EINVAL, std::string("conv_scan_step: ") + what); };
+  if (int s = step_params("conv_scan_step", a->batch, a->heads, a->dim, a->groups, a->type, a->dt, a->A, a->D, a->d_type, a->dt_bias,
+                          a->bias_type, a->state, a->y))
+    return s;
+  const int64_t inner = (int64_t)a->heads * a->dim, width = inner + 256ll * a->groups;
+  if (width > 1 << 24) return bad("channels is too large");
+  if (int s = conv_shape("conv_scan_step", a->batch, (int)width, a->taps, a->type, a->weight_type, a->weight, a->bias)) return s;
+  if (!a->xbc || !a->conv_state) return bad("null pointer argument");
+  if (!aligned(a->xbc, 2) || !aligned(a->conv_state, 2)) return bad("misaligned argument");
+  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < a->batch * width * 4) return bad("workspace missing, misaligned or too small");
+  ConvStepParams C{};
+  C.batch = a->batch; C.channels = (int)width; C.taps = a->taps; C.silu = 1; C.type = a->type; C.weight_type = a->weight_type;
+  C.x = a->xbc; C.x_sb = a->xbc_batch_stride; C.weight = a->weight; C.bias = a->bias; C.state = a->conv_state;
+  C.y = a->workspace; C.y_f32 = 1;
+  if (int s = check(launch_conv_step(C, (cudaStream_t)stream), "conv_scan_step")) return s;
+  const float* z = reinterpret_cast<const float*>(a->workspace);
+  SelectiveStepParams P{};
+  P.batch = a->batch; P.heads = a->heads; P.dim = a->dim; P.groups = a->groups; P.type = a->type;
+  P.x = z; P.B = z + inner; P.C = z + inner + 128ll * a->groups; P.x_sb = P.b_sb = P.c_sb = width;
+  P.dt = a->dt; P.dt_sb = a->dt_batch_stride; P.A = a->A;
+  P.D = a->D; P.d_type = a->d_type; P.dt_bias = a->dt_bias; P.bias_type = a->bias_type;
+  P.state = a->state; P.y = a->y; P.x_f32 = 1; P.behind = 1;
+  return check(launch_selective_step(P, (cudaStream_t)stream), "conv_scan_step");
+}
+
+namespace {
+int pack_params(const char* who, const void* x, int64_t rows, int width, int type, const int8_t* codes, const float* scales, PackParams& P) {
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  if (type < SQ_F16 || type > SQ_F32) return bad("unknown type");
+  if (rows < 0 || width < 1 || width > 1 << 30) return bad("rows or width out of range");
+  if (rows && (!x || !codes || !scales)) return bad("null pointer argument");
+  if (!aligned(x, type == SQ_F32 ? 4 : 2) || !aligned(scales, 4)) return bad("misaligned argument");
+  P = PackParams{};
+  P.rows = rows; P.width = width; P.type = type;
+  P.codes = const_cast<int8_t*>(codes); P.scales = const_cast<float*>(scales);
+  return SQ_OK;
+}
+}  // namespace
+
+int sq_pack_activations(const void* x, int64_t row_stride, int64_t rows, int width, int type, int8_t* codes, float* scales, void* stream) {
+  PackParams P;
+  if (int s = pack_params("pack_activations", x, rows, width, type, codes, scales, P)) return s;
+  if (rows == 0) return SQ_OK;
+  P.x = x; P.x_stride = row_stride;
+  return check(launch_pack(P, (cudaStream_t)stream), "pack_activations");
+}
+
+int sq_unpack_activations(const int8_t* codes, const float* scales, int64_t rows, int width, int type, void* out, void* stream) {
+  PackParams P;
+  if (int s = pack_params("unpack_activations", out, rows, width, type, codes, scales, P)) return s;
+  if (rows == 0) return SQ_OK;
+  P.y = out;
+  return check(launch_unpack(P, (cudaStream_t)stream), "unpack_activations");
 }
 
 }  // extern "C"

@@ -56,6 +56,11 @@ __device__ __forceinline__ void stage16(void* smem_dst, const void* gsrc, int by
     cp_async16(reinterpret_cast<char*>(smem_dst) + 16 * i, reinterpret_cast<const char*>(gsrc) + 16 * i);
 }
 
+// Programmatic launches: lets the kernel launched behind this one begin, and waits for the one before.  Without the
+// launch attribute both do nothing.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_launch() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Bounded mbarrier / flag waits: every spin has an iteration limit.
 constexpr uint32_t kSpinLimit = 1u << 26;
 

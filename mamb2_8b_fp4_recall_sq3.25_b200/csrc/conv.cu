@@ -1,0 +1,511 @@
+// Short causal convolution of a mixer's channels, its gradients and its one-token form, and activations kept in 8 bits
+// (sm_100a).
+//
+//   z[t,c] = bias[c] + sum_k w[c,k] x[t - (taps-1) + k, c],   y = z sigmoid(z) or z
+//
+// Tokens before the first are the carried state's, or zero.  Everything is fp32 inside and rounded once.  All of it is
+// bound by memory: a thread owns 16 bytes of channels and a strip of tokens, with the last taps' inputs in registers, so
+// that each input is read once but for the strips' edges.  The backward pass computes z again from the input (or from
+// its 8-bit codes); sums for weights and bias are kept a strip and added in order by a second kernel.
+//
+// 8 bits: 128 neighbouring channels of a token share the scale max|x| / 127; a code is x / scale rounded to even.
+#include "conv.cuh"
+#include "device_util.cuh"
+#include "logits_util.cuh"
+
+namespace sq {
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kTaps = 4;                            // most taps; fewer use the last ones
+
+// kUnit<T> values, as fp32; `n` of them are there.
+template <typename T> __device__ __forceinline__ void load_values(const T* p, bool vec, int n, float (&f)[kUnit<T>]) {
+  Unit<T> u;
+  if (vec) {
+    u.q = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+    for (int i = 0; i < kUnit<T>; ++i) f[i] = to_f32(u.v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kUnit<T>; ++i) f[i] = i < n ? to_f32(p[i]) : 0.f;
+  }
+}
+template <typename T> __device__ __forceinline__ void store_values(T* p, bool vec, int n, const float (&f)[kUnit<T>]) {
+  if (vec) {
+    Unit<T> u;
+#pragma unroll
+    for (int i = 0; i < kUnit<T>; ++i) u.v[i] = from_f32<T>(f[i]);
+    *reinterpret_cast<uint4*>(p) = u.q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kUnit<T>; ++i)
+      if (i < n) p[i] = from_f32<T>(f[i]);
+  }
+}
+template <int V> __device__ __forceinline__ void store_codes(int8_t* p, bool vec, int n, const int (&q)[V]) {
+  if (vec) {
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      w[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 | (uint32_t)q[4 * i + 3] << 24;
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) p[i] = (int8_t)q[i];
+  }
+}
+template <int V> __device__ __forceinline__ void load_codes(const int8_t* p, bool vec, int n, float scale, float (&f)[V]) {
+  if (vec) {
+    uint32_t w[V / 4];
+    if constexpr (V == 8) { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
+    else w[0] = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * scale;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i < n ? (float)p[i] * scale : 0.f;
+  }
+}
+// Scale and codes of the 128 values of which this thread has V; the others are its neighbours'.  A NaN or an infinity
+// makes the block's scale one, and its values NaN.
+template <int V> __device__ __forceinline__ float encode(const float (&f)[V], int (&q)[V]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+#pragma unroll
+  for (int o = kPackBlock / V / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const float scale = __fdiv_rn(__uint_as_float(m), 127.0f);
+  const bool fine = scale > 0.f && scale <= 3.0e38f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) q[i] = fine ? max(-127, min(127, __float2int_rn(__fdiv_rn(f[i], scale)))) : 0;
+  return scale;
+}
+
+template <typename T> __device__ __forceinline__ float sigmoid(float z) {
+  if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
+  else return __fdividef(1.0f, 1.0f + __expf(-z));  // a few ulp of fp32, far below a 16-bit result's half step
+}
+
+template <typename T, typename WT>
+struct Taps {
+  float w[kTaps][kUnit<T>], b[kUnit<T>];
+  __device__ Taps(const ConvParams& P, int c, int n) {
+    const WT* weight = reinterpret_cast<const WT*>(P.weight) + (long long)c * P.taps;
+    const WT* bias = reinterpret_cast<const WT*>(P.bias) + c;
+#pragma unroll
+    for (int i = 0; i < kUnit<T>; ++i) {
+#pragma unroll
+      for (int k = 0; k < kTaps; ++k) {
+        const int j = k - (kTaps - P.taps);
+        w[k][i] = i < n && j >= 0 ? to_f32(weight[i * P.taps + j]) : 0.f;
+      }
+      b[i] = i < n && P.bias ? to_f32(bias[i]) : 0.f;
+    }
+  }
+};
+
+__device__ __forceinline__ int tokens_of(const ConvParams& P, int b) {
+  return P.lengths ? max(0, min(P.length, P.lengths[b])) : P.length;
+}
+
+// The input at token t of a sequence, the state's before the first.
+template <typename T, bool CODES>
+__device__ __forceinline__ void input_at(const ConvParams& P, int b, int t, int c, int n, bool vec, float (&f)[kUnit<T>]) {
+  constexpr int V = kUnit<T>;
+  if (t >= 0) {
+    if constexpr (CODES) {
+      const long long row = (long long)b * P.length + t;
+      const float scale = P.scales[row * ((P.channels + kPackBlock - 1) / kPackBlock) + c / kPackBlock];
+      load_codes<V>(P.codes + row * P.channels + c, vec, n, scale, f);
+    } else {
+      load_values<T>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + t * P.x_st + c, vec, n, f);
+    }
+  } else if (P.state_in && t >= 1 - P.taps) {
+    const long long at = ((long long)b * (P.taps - 1) + t + P.taps - 1) * P.channels + c;
+    load_values<T>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = 0.f;
+  }
+}
+
+// z of a token whose last four inputs are x[0..3], oldest first.  Taps that are not there are passed over, not
+// multiplied by zero: their inputs may be infinite.
+template <typename T, typename WT>
+__device__ __forceinline__ float conv_at(const Taps<T, WT>& W, int taps, int i, float x0, float x1, float x2, float x3) {
+  float z = W.b[i];
+  if (taps > 3) z += W.w[0][i] * x0;
+  if (taps > 2) z += W.w[1][i] * x1;
+  return (z + W.w[2][i] * x2) + W.w[3][i] * x3;
+}
+
+struct ConvFlags { int vec_in, vec_out, vec_codes; };
+
+// MODE: 0 reads the input, 1 keeps it in 8 bits besides, 2 reads what was kept.
+template <typename T, typename WT, int MODE>
+__global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams P, const ConvFlags F, int strip) {
+  constexpr int V = kUnit<T>;
+  constexpr bool KEEP = MODE == 1, CODES = MODE == 2;
+  const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
+  const int n = min(V, P.channels - c);                                // may be negative: shuffles need every lane
+  if (!KEEP && n <= 0) return;
+  const bool vec_in = (CODES ? F.vec_codes : F.vec_in) && n == V, vec_out = F.vec_out && n == V, vec_codes = F.vec_codes && n == V;
+  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip);
+  T* y = reinterpret_cast<T*>(P.y) + b * P.y_sb + c;
+  const int blocks = (P.channels + kPackBlock - 1) / kPackBlock;
+  float x[kTaps][V];
+  if (n > 0 && blockIdx.x == 0 && P.state_out) {                       // the last inputs
+    for (int j = 0; j < P.taps - 1; ++j) {
+      input_at<T, CODES>(P, b, len - (P.taps - 1) + j, c, n, vec_in, x[0]);
+      store_values<T>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (P.taps - 1) + j) * P.channels + c, false, n, x[0]);
+    }
+  }
+  if (t0 < len) {
+    const Taps<T, WT> W(P, c, n);
+#pragma unroll
+    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES>(P, b, n > 0 ? t0 - (kTaps - 1) + k : -kTaps, c, n, vec_in, x[k]);
+    constexpr int U = 4;                                               // tokens whose loads are in flight together
+    for (int t = t0; t < min(t1, len); t += U) {
+      float next[U][V];
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        input_at<T, CODES>(P, b, n > 0 && t + j < min(t1, len) ? t + j : -kTaps, c, n, vec_in, next[j]);
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const bool in = t + j < min(t1, len);
+        float out[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float z = conv_at<T, WT>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
+          out[i] = P.silu ? z * sigmoid<T>(z) : z;
+          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = next[j][i];
+        }
+        if (in && n > 0) store_values<T>(y + (t + j) * P.y_st, vec_out, n, out);
+        if constexpr (KEEP) {
+          int q[V];
+          const float scale = encode<V>(next[j], q);
+          const long long row = (long long)b * P.length + t + j;
+          if (in && n > 0) {
+            store_codes<V>(P.codes + row * P.channels + c, vec_codes, n, q);
+            if ((c & (kPackBlock - 1)) == 0) P.scales[row * blocks + c / kPackBlock] = scale;
+          }
+        }
+      }
+    }
+  }
+  if (n <= 0) return;
+  const float zero[V] = {};
+  for (int t = max(t0, len); t < t1; ++t) {
+    store_values<T>(y + t * P.y_st, vec_out, n, zero);
+    if constexpr (KEEP) {
+      const long long row = (long long)b * P.length + t;
+      const int none[V] = {};
+      store_codes<V>(P.codes + row * P.channels + c, vec_codes, n, none);
+      if ((c & (kPackBlock - 1)) == 0) P.scales[row * blocks + c / kPackBlock] = 0.f;
+    }
+  }
+}
+
+// A strip's gradients: dz_t = dy_t y'(z_t), dx_t = sum_k w_k dz_{t + taps-1 - k}, and the strip's sums of dz_t x_{t - (taps-1) + k}
+// and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.
+template <typename T, typename WT, bool CODES>
+__global__ void __launch_bounds__(kThreads) conv_grad_kernel(const ConvParams P, const ConvFlags F, int strip) {
+  constexpr int V = kUnit<T>;
+  const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
+  const int n = min(V, P.channels - c);
+  if (n <= 0) return;
+  const bool vec_in = (CODES ? F.vec_codes : F.vec_in) && n == V, vec_out = F.vec_out && n == V;
+  const bool vec_dx = n == V && P.channels % V == 0 && ((uintptr_t)P.dx & 15) == 0;
+  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip);
+  const T* dy = reinterpret_cast<const T*>(P.dy) + b * P.dy_sb + c;
+  T* dx = reinterpret_cast<T*>(P.dx) + (long long)b * P.length * P.channels + c;
+  const int back = P.taps - 1;
+  float dw[kTaps][V] = {}, db[V] = {};
+  if (t0 < len || t0 == 0) {
+    const Taps<T, WT> W(P, c, n);
+    float x[kTaps - 1][V], dz[kTaps][V] = {};
+#pragma unroll
+    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES>(P, b, t0 - (kTaps - 1) + k, c, n, vec_in, x[k]);
+    constexpr int U = 4;
+    for (int t = t0; t < t1 + kTaps - 1; t += U) {
+      float next[U][V], up[U][V];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const bool in = t + j < min(t1 + kTaps - 1, len);
+        input_at<T, CODES>(P, b, in ? t + j : -kTaps, c, n, vec_in, next[j]);
+        if (in) {
+          load_values<T>(dy + (t + j) * P.dy_st, vec_out, n, up[j]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) up[j][i] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int at = t + j, to = at - (kTaps - 1);                   // the token whose input's gradient is whole now
+        const bool in = at < len, mine = in && at < t1;
+        float out[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float d = up[j][i];
+          if (in && P.silu) {
+            const float z = conv_at<T, WT>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
+            const float s = sigmoid<T>(z);
+            d *= s * (1.0f + z * (1.0f - s));
+          }
+          dz[0][i] = dz[1][i]; dz[1][i] = dz[2][i]; dz[2][i] = dz[3][i]; dz[3][i] = d;
+          if (mine) {
+            db[i] += d;
+            if (P.taps > 3) dw[0][i] += d * x[0][i];
+            if (P.taps > 2) dw[1][i] += d * x[1][i];
+            dw[2][i] += d * x[2][i];
+            dw[3][i] += d * next[j][i];
+          }
+          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = next[j][i];
+          // dz[0..3] are those of `to` .. `to` + 3
+          float g = W.w[3][i] * dz[0][i] + W.w[2][i] * dz[1][i];
+          if (P.taps > 2) g += W.w[1][i] * dz[2][i];
+          if (P.taps > 3) g += W.w[0][i] * dz[3][i];
+          out[i] = g;
+        }
+        if (to >= t1 || to < (t0 == 0 ? -back : t0)) continue;
+        if (P.dstate_out && to >= len - back && to < len) {
+          float late[V];
+          const long long at = ((long long)b * back + to - (len - back)) * P.channels + c;
+          load_values<T>(reinterpret_cast<const T*>(P.dstate_out) + at, false, n, late);
+#pragma unroll
+          for (int i = 0; i < V; ++i) out[i] += late[i];
+        }
+        if (to >= 0) {
+          if (to < len) store_values<T>(dx + (long long)to * P.channels, vec_dx, n, out);
+        } else if (P.dstate_in) {
+          store_values<T>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
+        }
+      }
+    }
+  }
+  const float zero[V] = {};
+  for (int t = max(t0, len); t < t1; ++t) store_values<T>(dx + (long long)t * P.channels, vec_dx, n, zero);
+  if (P.dweight || P.dbias) {
+    float* part = P.workspace + ((long long)b * gridDim.x + blockIdx.x) * (kTaps + 1) * P.channels + c;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) {
+#pragma unroll
+        for (int k = 0; k < kTaps; ++k) part[(long long)k * P.channels + i] = dw[k][i];
+        part[(long long)kTaps * P.channels + i] = db[i];
+      }
+  }
+}
+
+// The strips' sums for a channel's tap or bias, in order: eight threads share a channel's strips.
+template <typename WT>
+__global__ void __launch_bounds__(256) conv_weights_kernel(const ConvParams P, int strips) {
+  __shared__ float sums[8][33];
+  const int lane = threadIdx.x & 31, sub = threadIdx.x >> 5, k = blockIdx.y;
+  const int c = blockIdx.x * 32 + lane;
+  if (k < kTaps - P.taps) return;
+  float v = 0.f;
+  if (c < P.channels)
+    for (int s = sub; s < strips; s += 8) v += P.workspace[((long long)s * (kTaps + 1) + k) * P.channels + c];
+  sums[sub][lane] = v;
+  __syncthreads();
+  if (sub || c >= P.channels) return;
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v += sums[i][lane];
+  if (k == kTaps) {
+    if (P.dbias) reinterpret_cast<WT*>(P.dbias)[c] = from_f32<WT>(v);
+  } else if (P.dweight) {
+    reinterpret_cast<WT*>(P.dweight)[(long long)c * P.taps + k - (kTaps - P.taps)] = from_f32<WT>(v);
+  }
+}
+
+// One token: a thread owns 16 bytes of channels, shifts their state and puts the token at its end.
+template <typename T, typename WT, typename YT>
+__global__ void __launch_bounds__(kThreads) conv_step_kernel(const ConvStepParams P, int vec) {
+  constexpr int V = kUnit<T>;
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * V, b = blockIdx.y;
+  const int n = min(V, P.channels - c);
+  launch_dependents();
+  if (n <= 0) return;
+  const bool v = vec && n == V;
+  ConvParams C{};
+  C.taps = P.taps; C.weight = P.weight; C.bias = P.bias;
+  T* state = reinterpret_cast<T*>(P.state) + (long long)b * (P.taps - 1) * P.channels + c;
+  float x[kTaps][V] = {};
+  load_values<T>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + c, v, n, x[3]);
+#pragma unroll
+  for (int k = 0; k < kTaps - 1; ++k) {
+    const int j = k - (kTaps - P.taps);
+    if (j >= 0) load_values<T>(state + (long long)j * P.channels, v, n, x[k]);
+  }
+  const Taps<T, WT> W(C, c, n);
+  float out[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const float z = conv_at<T, WT>(W, P.taps, i, x[0][i], x[1][i], x[2][i], x[3][i]);
+    out[i] = P.silu ? z * sigmoid<T>(z) : z;
+  }
+  YT* y = reinterpret_cast<YT*>(P.y) + (long long)b * P.channels + c;
+  if constexpr (sizeof(YT) == sizeof(T)) {
+    store_values<T>(y, v, n, out);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) y[i] = out[i];
+  }
+#pragma unroll
+  for (int k = 0; k < kTaps - 1; ++k) {
+    const int j = k - (kTaps - P.taps);
+    if (j >= 0) store_values<T>(state + (long long)j * P.channels, v, n, x[k + 1]);
+  }
+}
+
+// Rows in 8 bits: a thread has 16 bytes of the input, kRows rows at a time.
+constexpr int kRows = 4;
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams P, int vec, int vec_codes) {
+  constexpr int V = kUnit<T>;
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * V;
+  const int n = min(V, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
+  for (long long r0 = (long long)blockIdx.y * kRows; r0 < P.rows; r0 += (long long)gridDim.y * kRows) {
+    float f[kRows][V];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      if (n > 0 && r0 + j < P.rows) {
+        load_values<T>(reinterpret_cast<const T*>(P.x) + (r0 + j) * P.x_stride + c, vec && n == V, n, f[j]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[j][i] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      int q[V];
+      const float scale = encode<V>(f[j], q);
+      if (n > 0 && r0 + j < P.rows) {
+        store_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, q);
+        if ((c & (kPackBlock - 1)) == 0) P.scales[(r0 + j) * blocks + c / kPackBlock] = scale;
+      }
+    }
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(kThreads) unpack_kernel(const PackParams P, int vec, int vec_codes) {
+  constexpr int V = kUnit<T>;
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * V;
+  const int n = min(V, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
+  if (n <= 0) return;
+  for (long long r0 = (long long)blockIdx.y * kRows; r0 < P.rows; r0 += (long long)gridDim.y * kRows) {
+    float f[kRows][V];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+      if (r0 + j < P.rows)
+        load_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, P.scales[(r0 + j) * blocks + c / kPackBlock], f[j]);
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+      if (r0 + j < P.rows) store_values<T>(reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c, vec && n == V, n, f[j]);
+  }
+}
+
+int unit_of(int type) { return type == 2 ? 4 : 8; }
+bool whole(const void* p, int type, long long a, long long b = 0) {
+  return ((uintptr_t)p & 15) == 0 && (a | b) % unit_of(type) == 0;
+}
+
+// Tokens of a strip: long ones read fewer edges twice, short ones make more CTAs.
+int strip_of(int batch, int length, int channels, int type, int least, int most) {
+  const long long wide = (long long)batch * ((channels + unit_of(type) - 1) / unit_of(type));
+  int s = most;
+  while (s > least && wide * ((length + s - 1) / s) < 148 * 1024) s /= 2;
+  return s;
+}
+constexpr int kLeast = 16, kMost = 128;
+
+template <typename F> int by_type(int type, int weight_type, F f) {
+  if (type == 2) return f(float{}, float{});
+  if (type == 1) return weight_type == 2 ? f(__nv_bfloat16{}, float{}) : f(__nv_bfloat16{}, __nv_bfloat16{});
+  return weight_type == 2 ? f(__half{}, float{}) : f(__half{}, __half{});
+}
+
+}  // namespace
+
+long long conv_workspace(int batch, int length, int channels, int type) {
+  const int strip = strip_of(batch, length, channels, type, kLeast, kMost);
+  return (long long)batch * ((length + strip - 1) / strip) * (kTaps + 1) * channels * 4;
+}
+
+int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
+  const int strip = strip_of(P.batch, P.length, P.channels, P.type, 8, 64), per = kThreads * unit_of(P.type);
+  const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
+  const ConvFlags F{P.x && whole(P.x, P.type, P.x_sb, P.x_st), whole(P.y, P.type, P.y_sb, P.y_st),
+                    P.channels % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0};
+  return by_type(P.type, P.weight_type, [&](auto t, auto w) {
+    using T = decltype(t);
+    using WT = decltype(w);
+    if (!P.codes) conv_kernel<T, WT, 0><<<grid, kThreads, 0, st>>>(P, F, strip);
+    else if (P.x) conv_kernel<T, WT, 1><<<grid, kThreads, 0, st>>>(P, F, strip);
+    else conv_kernel<T, WT, 2><<<grid, kThreads, 0, st>>>(P, F, strip);
+    return launch_status();
+  });
+}
+
+int launch_conv_backward(const ConvParams& P, cudaStream_t st) {
+  const int strip = strip_of(P.batch, P.length, P.channels, P.type, kLeast, kMost), per = kThreads * unit_of(P.type);
+  const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
+  const ConvFlags F{P.x && whole(P.x, P.type, P.x_sb, P.x_st), whole(P.dy, P.type, P.dy_sb, P.dy_st),
+                    P.channels % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0};
+  return by_type(P.type, P.weight_type, [&](auto t, auto w) {
+    using T = decltype(t);
+    using WT = decltype(w);
+    if (P.codes) conv_grad_kernel<T, WT, true><<<grid, kThreads, 0, st>>>(P, F, strip);
+    else conv_grad_kernel<T, WT, false><<<grid, kThreads, 0, st>>>(P, F, strip);
+    if (int s = launch_status()) return s;
+    if (P.dweight || P.dbias) {
+      conv_weights_kernel<WT><<<dim3((P.channels + 31) / 32, kTaps + 1), 256, 0, st>>>(P, (int)grid.x * P.batch);
+      return launch_status();
+    }
+    return (int)kOk;
+  });
+}
+
+int launch_conv_step(const ConvStepParams& P, cudaStream_t st) {
+  const int per = kThreads * unit_of(P.type);
+  const dim3 grid((P.channels + per - 1) / per, P.batch);
+  const int vec = whole(P.x, P.type, P.x_sb, P.channels) && ((uintptr_t)P.state & 15) == 0 && ((uintptr_t)P.y & 15) == 0;
+  return by_type(P.type, P.weight_type, [&](auto t, auto w) {
+    using T = decltype(t);
+    using WT = decltype(w);
+    if (P.y_f32) conv_step_kernel<T, WT, float><<<grid, kThreads, 0, st>>>(P, vec);
+    else conv_step_kernel<T, WT, T><<<grid, kThreads, 0, st>>>(P, vec);
+    return launch_status();
+  });
+}
+
+namespace {
+dim3 pack_grid(const PackParams& P) {
+  const int per = kThreads * unit_of(P.type);
+  const long long rows = (P.rows + kRows - 1) / kRows;
+  return dim3((P.width + per - 1) / per, (unsigned)(rows < 65535 ? rows : 65535));
+}
+}  // namespace
+
+int launch_pack(const PackParams& P, cudaStream_t st) {
+  const int vec = whole(P.x, P.type, P.x_stride), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
+  if (P.type == 0) pack_kernel<__half><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  else if (P.type == 1) pack_kernel<__nv_bfloat16><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  else pack_kernel<float><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  return launch_status();
+}
+int launch_unpack(const PackParams& P, cudaStream_t st) {
+  const int vec = whole(P.y, P.type, P.width), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
+  if (P.type == 0) unpack_kernel<__half><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  else if (P.type == 1) unpack_kernel<__nv_bfloat16><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  else unpack_kernel<float><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  return launch_status();
+}
+
+}  // namespace sq

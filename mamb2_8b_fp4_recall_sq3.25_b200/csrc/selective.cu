@@ -1,0 +1,1339 @@
+// Selective scan in unquantised states (sm_100a): prompts, gradients, single tokens.
+//
+//   s_t = softplus(dt_t + bias),  H_t = exp(A s_t) H_{t-1} + s_t x_t B_t^T,  y_t = H_t C_t + D x_t
+//
+// per head, H fp32 [dim, 128], B and C shared by the heads of a group.  Work goes by chunks of 128 tokens.  With
+// l_t the sum of A s over the chunk up to t,
+//
+//   y_t   = sum_{s<=t} exp(l_t - l_s) s_s (C_t . B_s) x_s + exp(l_t) H_in C_t + D x_t
+//   H_out = exp(l_end) H_in + sum_s exp(l_end - l_s) s_s x_s B_s^T
+//
+// so that all but the chunks' order is matrix products: state_pass_kernel walks a head's chunks and leaves the state
+// that enters each one, out_kernel then does every (chunk, group) on its own, and grad_kernel does the same for the
+// gradients, with the states' own gradients from state_pass_kernel walking backwards (G_in = exp(l_end) G_out +
+// sum_t exp(l_t) dy_t C_t^T).  All products run on tcgen05 with fp32 accumulators in TMEM.
+//
+// Operands are 16 bits.  Inputs enter as they are; what is computed is rounded, in these places:
+//   * the weighted tokens of state_pass_kernel and the states themselves as two numbers (value and remainder, 16 bits
+//     of bf16, 22 of fp16) wherever an fp32 result hangs on them;
+//   * the pairs' weights exp(l_t - l_s) s_s (C_t . B_s), the states in y, and the operands of dB and dC as one number:
+//     their results are 16-bit tensors, whose own rounding is as large.
+// fp16 operands are scaled by powers of two per row, chunk or CTA (bf16 has fp32's range and needs none).
+// Sums of A s are doubles, kept as two floats: neighbours' differences keep 24 bits wherever in the chunk they lie.
+#include "selective.cuh"
+#include <type_traits>
+#include "device_util.cuh"
+#include "logits_util.cuh"
+#include "tc_util.cuh"
+
+namespace sq {
+namespace {
+
+using namespace tc;
+
+constexpr int Q = kScanChunk;
+constexpr int TP = kScanTile;
+constexpr int kN = 128;
+constexpr int kThreads = 256;
+constexpr uint32_t kTile128 = 32768, kTile64 = 16384;      // bytes of a [128][128] and a [128][64] 16-bit tile
+
+// ---------------------------------------------------------------- operands in shared memory
+// Tiles are rows of 128 bytes (64 numbers) with the 128-byte swizzle: 16-byte piece j of row r lies at
+// r * 128 + ((j ^ (r & 7)) << 4).  A [128][128] tile is two such tiles, columns 0..63 and 64..127.
+__device__ __forceinline__ uint32_t piece(int row, int j) { return (uint32_t)(row * 128 + ((j ^ (row & 7)) << 4)); }
+__device__ __forceinline__ uint32_t piece2(int row, int j) { return (uint32_t)((j >> 3) * kTile64) + piece(row, j & 7); }
+
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" :: "r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int K> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(K) : "memory"); }
+// What the threads wrote to shared memory becomes visible to the tensor cores (after the next CTA barrier).
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Matrix descriptors of operands in such tiles.  K-major: a row is an index of M or N, its columns are K
+// (16 of K: 32 bytes on).  MN-major: a row is an index of K, its columns are M or N (16 of K: 2,048 bytes on; the
+// second 64 columns of M or N 16,384 bytes on).
+__device__ __forceinline__ uint64_t desc_k(uint32_t a) { return sw128_desc(a); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t a) {
+  return (uint64_t)((a & 0x3FFFFu) >> 4) | (uint64_t)(kTile64 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+template <typename T> __device__ __forceinline__ constexpr uint32_t idesc(int n, bool a_mn, bool b_mn) {
+  const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+// D[128][n] (+)= A . B over K = 16 * steps; a / b: addresses of the tiles.  K-major tiles of 128 columns go on in
+// their second half after four steps.
+template <bool A_MN, bool B_MN>
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t id, int steps, bool accumulate) {
+  for (int k = 0; k < steps; ++k) {
+    const uint32_t kk = (uint32_t)((k >> 2) * kTile64 + (k & 3) * 32), km = (uint32_t)k * 2048;
+    umma_f16(d, A_MN ? desc_mn(a + km) : desc_k(a + kk), B_MN ? desc_mn(b + km) : desc_k(b + kk), id, accumulate || k);
+  }
+}
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+
+// Keeps uses of a tcgen05.ld's registers behind the wait that precedes this call.
+__device__ __forceinline__ void settle(uint32_t (&r)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ void unpack8(uint4 u, float (&f)[8]) {
+  const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y), c = unpack2<T>(u.z), d = unpack2<T>(u.w);
+  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+}
+template <typename T> __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+}
+// Value and remainder of eight numbers.
+template <typename T> __device__ __forceinline__ void split8(const float (&f)[8], uint4& hi, uint4& lo) {
+  hi = pack8<T>(f);
+  float r[8];
+  unpack8<T>(hi, r);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = f[i] - r[i];
+  lo = pack8<T>(r);
+}
+
+// The power of two that brings `bits` (a maximum's, sign cleared) to [2^13, 2^14) and its inverse: {there, back}.
+__device__ __forceinline__ float2 scale_of(uint32_t bits) {
+  int e = (int)(bits >> 23) - 140;
+  e = bits ? max(-60, min(60, e)) : 0;                  // products of two scales stay numbers
+  return make_float2(__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23));
+}
+
+__device__ __forceinline__ float number(const void* p, int type, int i) {
+  if (!p) return 0.f;
+  return type == SQ_TYPE_F32 ? reinterpret_cast<const float*>(p)[i]
+         : type == SQ_TYPE_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i])
+                                : __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void put_number(void* p, int type, int i, float v) {
+  if (type == SQ_TYPE_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (type == SQ_TYPE_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+__device__ __forceinline__ int tokens_of(const SelectiveParams& P, int b) {
+  return P.lengths ? max(0, min(P.length, P.lengths[b])) : P.length;
+}
+
+// ---------------------------------------------------------------- workspace
+struct Space {
+  int nc, ptiles, units;              // chunks of the longest sequence, tiles of a head's rows, heads * ptiles
+  long long lp;
+  float4* prm;                        // [B][H][lp]: s, l (value and remainder, base 2), sigmoid(dt + bias)
+  float* smax;                        // [B][H][nc]: the largest s of a chunk
+  uint16_t *h, *g;                    // [B][nc][units][2][8][128][8]: states entering a chunk, gradients of those leaving it
+  float2 *hs, *gs;                    // [B][nc][units]: scale of the state, scale of the chunk's weighted tokens
+  float2* parts;                      // [B][units][lp]: gradient of A s, gradient of s through the tokens
+  float2* unit_sums;                  // [B][nc][units]: gradients of D and of A by chunk
+  float* bias_sums;                   // [B][nc][H]: gradient of the bias by chunk
+  float *pb, *pc;                     // [splits][B][nc * Q][G][128]: dB and dC by split
+  int splits;
+  long long bytes;
+};
+
+constexpr int kSms = 148;
+
+// CTAs that share a group's heads: enough for every SM (two CTAs an SM in the forward, one in the backward), and no
+// more than there are units.
+int splits_of(long long tiles, int units, int want) {
+  long long s = (want + tiles - 1) / tiles;
+  if (s > units) s = units;
+  if (s < 1) s = 1;
+  const int per = (units + (int)s - 1) / (int)s;
+  return (units + per - 1) / per;
+}
+
+Space space_of(const SelectiveParams& P, bool backward) {
+  Space w{};
+  w.nc = (P.length + Q - 1) / Q;
+  w.lp = (long long)w.nc * Q;
+  w.ptiles = (P.dim + TP - 1) / TP;
+  w.units = P.heads * w.ptiles;
+  const long long bc = (long long)P.batch * w.nc, bcu = bc * w.units, bh = (long long)P.batch * P.heads;
+  char* base = reinterpret_cast<char*>(P.workspace);
+  long long at = 0;
+  auto take = [&](long long bytes) { char* p = base + at; at += (bytes + 255) / 256 * 256; return p; };
+  w.prm = reinterpret_cast<float4*>(take(bh * w.lp * 16));
+  w.smax = reinterpret_cast<float*>(take(bh * w.nc * 4));
+  const long long plane = (long long)kN * TP * 2 * 2;
+  w.h = reinterpret_cast<uint16_t*>(take(bcu * plane));
+  w.hs = reinterpret_cast<float2*>(take(bcu * 8));
+  w.splits = splits_of(bc * P.groups, w.units / P.groups, backward ? kSms : 2 * kSms);
+  if (backward) {
+    w.g = reinterpret_cast<uint16_t*>(take(bcu * plane));
+    w.gs = reinterpret_cast<float2*>(take(bcu * 8));
+    w.parts = reinterpret_cast<float2*>(take((long long)P.batch * w.units * w.lp * 8));
+    w.unit_sums = reinterpret_cast<float2*>(take(bcu * 8));
+    w.bias_sums = reinterpret_cast<float*>(take(bc * P.heads * 4));
+    if (w.splits > 1) {
+      const long long part = bc * Q * P.groups * kN * 4 * w.splits;
+      w.pb = reinterpret_cast<float*>(take(part));
+      w.pc = reinterpret_cast<float*>(take(part));
+    }
+  }
+  w.bytes = at;
+  return w;
+}
+
+// ---------------------------------------------------------------- tiles from global memory
+// 16-byte pieces of 128 rows of `pieces` pieces: row t at src + t * stride, rows from `rows` on and columns from
+// `cols` on are zero.  vec: pieces are whole and aligned.
+template <typename T, int PIECES>
+__device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long stride, int rows, int cols, bool vec) {
+  for (int i = threadIdx.x; i < Q * PIECES; i += kThreads) {
+    const int r = i / PIECES, j = i % PIECES;
+    const uint32_t a = dst + (PIECES == 16 ? piece2(r, j) : piece(r, j));
+    const T* p = src + (long long)r * stride + j * 8;
+    if (vec) {
+      const bool in = r < rows && j * 8 < cols;
+      cp16(a, in ? p : src, in);
+    } else {
+      uint32_t u[4] = {0, 0, 0, 0};
+      if (r < rows)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (j * 8 + e < cols) u[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+      sts16(a, make_uint4(u[0], u[1], u[2], u[3]));
+    }
+  }
+}
+// A state's plane [8 pieces][128 rows] of 16 bytes.
+__device__ __forceinline__ void load_plane(uint32_t dst, const uint16_t* src) {
+  for (int i = threadIdx.x; i < 8 * kN; i += kThreads) cp16(dst + piece(i & 127, i >> 7), src + (long long)i * 8, true);
+}
+// The first `rows` rows and `cols` columns of a tile [128][64] to global memory.
+template <typename T>
+__device__ __forceinline__ void store_tile(T* dst, long long stride, uint32_t src, int rows, int cols, bool vec) {
+  for (int i = threadIdx.x; i < Q * 8; i += kThreads) {
+    const int r = i >> 3, j = i & 7;
+    if (r >= rows || j * 8 >= cols) continue;
+    const uint4 v = lds16(src + piece(r, j));
+    T* p = dst + (long long)r * stride + j * 8;
+    if (vec) {
+      *reinterpret_cast<uint4*>(p) = v;
+    } else {
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (j * 8 + e < cols) reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(u[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+__device__ __forceinline__ bool vector_ok(const void* p, long long s0, long long s1, int cols) {
+  return ((uintptr_t)p & 15) == 0 && ((s0 | s1 | cols) & 7) == 0;
+}
+
+// A CTA's own barrier on the tensor cores' work; a wait that expires is recorded once and no further one is begun.
+struct Mma {
+  uint32_t bar, parity;
+  bool ok;
+  int* err;
+  __device__ void commit() { umma_commit(bar); }
+  __device__ void wait() {
+    if (ok && !mbar_wait(bar, parity)) {
+      ok = false;
+      if (threadIdx.x == 0) atomicOr(err, (int)kDevTimeoutMma);
+    }
+    parity ^= 1;
+    tc_fence_after();
+  }
+};
+template <int COLS>
+__device__ __forceinline__ Mma mma_begin(uint64_t* bar, uint32_t* slot, int* err, uint32_t& tmem) {
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(bar), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x < 32) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(slot)), "n"(COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  tmem = *slot;
+  return Mma{smem_u32(bar), 0, true, err};
+}
+template <int COLS> __device__ __forceinline__ void mma_end(uint32_t tmem) {
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (threadIdx.x < 32) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(tmem), "n"(COLS));
+}
+
+// ---------------------------------------------------------------- steps and decays
+// A in base 2.  An A of zero becomes one that decays nothing either, so that time can be told from l.
+__device__ __forceinline__ double decay_rate(float A) {
+  return fabsf(A) < 1e-20f ? -1e-20 : (double)A * 1.4426950408889634;
+}
+// One CTA: a chunk of 32 heads.  A warp takes a head at a time, four tokens a lane.
+template <typename T>
+__global__ void __launch_bounds__(128) prepare_kernel(const SelectiveParams P, const Space W) {
+  __shared__ float step[Q][33], slope[Q][33];
+  const int c = blockIdx.x, h0 = blockIdx.y * 32, b = blockIdx.z;
+  const int len = tokens_of(P, b);
+  const T* dt = reinterpret_cast<const T*>(P.dt) + (long long)b * P.dt_sb;
+  const int hl = threadIdx.x & 31, h = h0 + hl;
+  const float bias = h < P.heads ? number(P.dt_bias, P.bias_type, h) : 0.f;
+#pragma unroll 4
+  for (int t = threadIdx.x >> 5; t < Q; t += 4) {
+    const int token = c * Q + t;
+    float s = 0.f, d = 0.f;
+    if (token < len && h < P.heads) {
+      const float v = to_f32(dt[(long long)token * P.dt_st + h]) + bias;
+      s = v <= 20.0f ? log1pf(expf(v)) : v;
+      d = 1.0f / (1.0f + expf(-v));
+    }
+    step[t][hl] = s;
+    slope[t][hl] = d;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  for (int k = threadIdx.x >> 5; k < 32 && h0 + k < P.heads; k += 4) {
+    const double rate = decay_rate(P.A[h0 + k]);
+    float s[4], top = 0.f;
+    double l[4], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[i] = step[4 * lane + i][k];
+      sum += rate * (double)s[i];
+      l[i] = sum;
+      top = fmaxf(top, s[i]);
+    }
+    double before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double v = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += v;
+    }
+    before -= sum;
+    const long long row = (long long)b * P.heads + h0 + k;
+    float4* out = W.prm + row * W.lp + (long long)c * Q + 4 * lane;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double v = before + l[i];
+      const float hi = (float)v;
+      out[i] = make_float4(s[i], hi, (float)(v - (double)hi), slope[4 * lane + i][k]);
+    }
+    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (lane == 0) W.smax[row * W.nc + c] = __uint_as_float(m);
+  }
+}
+
+// ---------------------------------------------------------------- states by chunk
+// One CTA walks the chunks of one unit (64 rows of a head's state), forwards or backwards.  The state is fp32 in
+// registers: thread (n, half) holds state[n][32 half .. +32].  A chunk's addition is B^T (w x), with w x as value and
+// remainder.  Written before each chunk: the state that enters it, value and (LO) remainder.
+constexpr uint32_t kPassX = 2 * kTile128, kPassW = kPassX + kTile64, kPassBytes = kPassW + 2 * kTile64;
+constexpr uint32_t kPassSmem = kPassBytes + 64;
+
+template <typename T, bool REV, bool LO>
+__global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const SelectiveParams P, const Space W) {
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t base = smem_u32(smem);
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kPassBytes);
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kPassBytes + 8);
+  uint32_t* tops = reinterpret_cast<uint32_t*>(smem + kPassBytes + 16);      // [2][2]: of the tokens, of the state
+  const int u = blockIdx.x, b = blockIdx.y;
+  const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, g = h / (P.heads / P.groups);
+  const int cols = min(TP, P.dim - p0);
+  const int len = tokens_of(P, b), nc = (len + Q - 1) / Q;
+  const int n = threadIdx.x & 127, half = threadIdx.x >> 7, lane_base = (threadIdx.x >> 5 & 3) * 32;
+  const float* first = REV ? P.dstate_out : P.state_in;
+  float* last = REV ? P.dstate_in : P.state_out;
+  uint16_t* planes = REV ? W.g : W.h;
+  float2* scales = REV ? W.gs : W.hs;
+  const T* tok = reinterpret_cast<const T*>(REV ? P.dy : P.x) + (long long)b * (REV ? P.dy_sb : P.x_sb) + (long long)h * P.dim + p0;
+  const long long tok_st = REV ? P.dy_st : P.x_st;
+  const bool tok_vec = vector_ok(tok, tok_st, 0, cols);
+  const T* vec = reinterpret_cast<const T*>(REV ? P.C : P.B) + (long long)b * (REV ? P.c_sb : P.b_sb) + g * kN;
+  const long long vec_st = REV ? P.c_st : P.b_st;
+  const bool vec_vec = vector_ok(vec, vec_st, 0, kN);
+  const float4* prm = W.prm + ((long long)b * P.heads + h) * W.lp;
+  const long long state_at = (((long long)b * P.heads + h) * P.dim + p0) * kN + n;
+
+  float S[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    S[i] = first && half * 32 + i < cols ? first[state_at + (long long)(half * 32 + i) * kN] : 0.f;
+
+  if (threadIdx.x < 4) tops[threadIdx.x] = 0;
+  uint32_t tmem;
+  Mma mm = mma_begin<64>(bar, slot, P.err, tmem);
+  const uint32_t mine = tmem + ((uint32_t)lane_base << 16) + (uint32_t)half * 32;
+
+  auto load = [&](int i) {
+    const int c = REV ? nc - 1 - i : i;
+    load_tile<T, 8>(base + kPassX, tok + (long long)c * Q * tok_st, tok_st, len - c * Q, cols, tok_vec);
+    load_tile<T, 16>(base + (i & 1) * kTile128, vec + (long long)c * Q * vec_st, vec_st, len - c * Q, kN, vec_vec);
+    cp_commit();
+  };
+  if (nc > 0) load(0);
+  for (int i = 0; i < nc; ++i) {
+    const int c = REV ? nc - 1 - i : i;
+    const long long at = ((long long)b * W.nc + c) * W.units + u;
+    const bool update = i + 1 < nc || last;
+    const float4 mine_prm = prm[(long long)c * Q + n], end_prm = prm[(long long)c * Q + Q - 1];
+    const bool write = i > 0 || first;
+    if (kScaled && write) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < 32; ++k) m = max(m, __float_as_uint(S[k]) & 0x7fffffffu);
+      m = __reduce_max_sync(0xffffffffu, m);
+      if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1) + 1], m);
+    }
+    cp_wait<0>();
+    __syncthreads();
+    float wscale = 1.f, sscale = 1.f;
+    if (update || REV || kScaled) {
+      float w;
+      if (REV) w = exp2f(mine_prm.y + mine_prm.z);
+      else w = mine_prm.x * exp2f((end_prm.y - mine_prm.y) + (end_prm.z - mine_prm.z));
+      float v[4][8];
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        unpack8<T>(lds16(base + kPassX + piece(n, half * 4 + j)), v[j]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          v[j][e] *= w;
+          if (kScaled) m = max(m, __float_as_uint(v[j][e]) & 0x7fffffffu);
+        }
+      }
+      float there = 1.f;
+      if (kScaled) {
+        m = __reduce_max_sync(0xffffffffu, m);
+        if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1)], m);
+        __syncthreads();
+        const float2 sc = scale_of(tops[2 * (i & 1)]);
+        there = sc.x;
+        wscale = sc.y;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (kScaled)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[j][e] *= there;
+        uint4 hi, lo;
+        split8<T>(v[j], hi, lo);
+        sts16(base + kPassW + piece(n, half * 4 + j), hi);
+        sts16(base + kPassW + kTile64 + piece(n, half * 4 + j), lo);
+      }
+    }
+    float sthere = 1.f;
+    if (kScaled && write) {
+      const float2 sc = scale_of(tops[2 * (i & 1) + 1]);
+      sthere = sc.x;
+      sscale = sc.y;
+    }
+    fence_async();
+    __syncthreads();
+    if (kScaled && threadIdx.x < 2) tops[2 * (i & 1) + threadIdx.x] = 0;      // read by all, used again in two chunks
+    if (update && threadIdx.x == 0 && mm.ok) {
+      tc_fence_after();
+      mma<true, true>(tmem, base + (i & 1) * kTile128, base + kPassW, idesc<T>(TP, true, true), 8, false);
+      mma<true, true>(tmem, base + (i & 1) * kTile128, base + kPassW + kTile64, idesc<T>(TP, true, true), 8, true);
+      mm.commit();
+    }
+    if (i + 1 < nc) load(i + 1);
+    if (write) {
+      uint16_t* out = planes + at * (2 * kN * TP);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = kScaled ? S[8 * j + e] * sthere : S[8 * j + e];
+        uint4 hi, lo;
+        split8<T>(f, hi, lo);
+        *reinterpret_cast<uint4*>(out + ((half * 4 + j) * kN + n) * 8) = hi;
+        if (LO) *reinterpret_cast<uint4*>(out + kN * TP + ((half * 4 + j) * kN + n) * 8) = lo;
+      }
+    }
+    if (threadIdx.x == 0) scales[at] = make_float2(sscale, wscale);
+    if (update) {
+      mm.wait();
+      uint32_t r[32];
+      tmem_ld32(mine, r);
+      tc_fence_before();
+      const float decay = exp2f(end_prm.y + end_prm.z);
+#pragma unroll
+      for (int k = 0; k < 32; ++k) S[k] = S[k] * decay + __uint_as_float(r[k]) * wscale;
+    }
+  }
+  if (last)
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (half * 32 + i < cols) last[state_at + (long long)(half * 32 + i) * kN] = S[i];
+  mma_end<64>(tmem);
+}
+
+// ---------------------------------------------------------------- outputs by chunk and group
+// One CTA: a chunk and some units of a group.  C B^T once (128 columns of TMEM), then a unit at a time: the pairs'
+// weights go to shared memory as the operand M, C H_in and M x to 64 columns each.
+constexpr uint32_t kOutM = kTile128, kOutX = 2 * kTile128, kOutH = kOutX + kTile64, kOutBytes = kOutH + kTile64;
+constexpr uint32_t kOutPrm = kOutBytes, kOutTop = kOutPrm + Q * 16, kOutBar = kOutTop + 2 * Q * 4, kOutSmem = kOutBar + 16;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams P, const Space W, int per) {
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t base = smem_u32(smem);
+  float4* prm = reinterpret_cast<float4*>(smem + kOutPrm);
+  float* tops = reinterpret_cast<float*>(smem + kOutTop);
+  const int c = blockIdx.x, b = blockIdx.z;
+  const int gunits = W.units / P.groups, g = blockIdx.y / W.splits;
+  const int u0 = g * gunits + (blockIdx.y % W.splits) * per, u1 = min(u0 + per, (g + 1) * gunits);
+  const int len = tokens_of(P, b), rows = min(Q, len - c * Q), out_rows = min(Q, P.length - c * Q);
+  const int row = threadIdx.x & 127, half = threadIdx.x >> 7, quad = threadIdx.x >> 5 & 3;
+  T* y = reinterpret_cast<T*>(P.y) + (long long)b * P.y_sb + (long long)c * Q * P.y_st;
+  if (rows <= 0) {                                       // behind the sequence's end
+    for (int u = u0; u < u1; ++u) {
+      const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+      for (int i = threadIdx.x; i < out_rows * cols; i += kThreads)
+        y[(long long)(i / cols) * P.y_st + (long long)h * P.dim + p0 + i % cols] = from_f32<T>(0.f);
+    }
+    return;
+  }
+  const bool has_state = c > 0 || P.state_in;
+  const T* Cc = reinterpret_cast<const T*>(P.C) + (long long)b * P.c_sb + (long long)c * Q * P.c_st + g * kN;
+  const T* Bc = reinterpret_cast<const T*>(P.B) + (long long)b * P.b_sb + (long long)c * Q * P.b_st + g * kN;
+  const T* xc = reinterpret_cast<const T*>(P.x) + (long long)b * P.x_sb + (long long)c * Q * P.x_st;
+  auto load_state = [&](int u) {
+    if (has_state) load_plane(base + kOutH, W.h + (((long long)b * W.nc + c) * W.units + u) * (2 * kN * TP));
+  };
+  auto load_x = [&](int u) {
+    const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+    const T* p = xc + (long long)h * P.dim + p0;
+    load_tile<T, 8>(base + kOutX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
+    const float4* s = W.prm + ((long long)b * P.heads + h) * W.lp + (long long)c * Q;
+    if (threadIdx.x < Q) cp16(base + kOutPrm + threadIdx.x * 16, s + threadIdx.x, true);
+  };
+  load_tile<T, 16>(base, Cc, P.c_st, rows, kN, vector_ok(Cc, P.c_st, 0, kN));
+  load_tile<T, 16>(base + kOutM, Bc, P.b_st, rows, kN, vector_ok(Bc, P.b_st, 0, kN));
+  cp_commit();
+  load_state(u0);
+  load_x(u0);
+  cp_commit();
+  uint32_t tmem;
+  Mma mm = mma_begin<256>(reinterpret_cast<uint64_t*>(smem + kOutBar), reinterpret_cast<uint32_t*>(smem + kOutBar + 8), P.err, tmem);
+  const uint32_t lanes = tmem + ((uint32_t)quad << 21);
+  cp_wait<1>();
+  fence_async();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    tc_fence_after();
+    mma<false, false>(tmem, base, base + kOutM, idesc<T>(Q, false, false), 8, false);
+    mm.commit();
+  }
+  mm.wait();
+  if (kScaled) {                                         // the largest |C_t . B_s| of my row's pairs
+    uint32_t m = 0;
+    for (int cb = half; cb <= quad; cb += 2) {
+      uint32_t r[32];
+      tmem_ld32(lanes + cb * 32, r);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (cb * 32 + i <= row) m = max(m, r[i] & 0x7fffffffu);
+    }
+    tops[half * Q + row] = __uint_as_float(m);
+  }
+  for (int cb = half; cb < 4; cb += 2)                   // pairs above the diagonal weigh nothing, for every unit
+    if (cb > quad)
+      for (int k = 0; k < 4; ++k) sts16(base + kOutM + piece2(row, cb * 4 + k), make_uint4(0, 0, 0, 0));
+  cp_wait<0>();
+  fence_async();
+  __syncthreads();
+  const float top = kScaled ? fmaxf(tops[row], tops[Q + row]) : 0.f;
+
+  for (int u = u0; u < u1; ++u) {
+    const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+    if (threadIdx.x == 0 && has_state && mm.ok) {
+      tc_fence_after();
+      mma<false, true>(tmem + 128, base, base + kOutH, idesc<T>(TP, false, true), 8, false);
+    }
+    const float4 me = prm[row];
+    float2 sc = make_float2(1.f, 1.f);
+    if (kScaled) sc = scale_of(__float_as_uint(top * W.smax[((long long)b * P.heads + h) * W.nc + c]) & 0x7fffffffu);
+    for (int cb = half; cb <= quad; cb += 2) {
+      uint32_t r[32];
+      tmem_ld32(lanes + cb * 32, r);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int s = cb * 32 + k * 8 + e;
+          const float4 to = prm[s];
+          const float w = ex2((me.y - to.y) + (me.z - to.z)) * to.x;
+          f[e] = __uint_as_float(r[k * 8 + e]) * (kScaled ? w * sc.x : w);
+          if (s > row) f[e] = 0.f;
+        }
+        sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<T>(f));
+      }
+    }
+    tc_fence_before();
+    fence_async();
+    __syncthreads();
+    if (threadIdx.x == 0 && mm.ok) {
+      tc_fence_after();
+      mma<false, true>(tmem + 192, base + kOutM, base + kOutX, idesc<T>(TP, false, true), 8, false);
+      mm.commit();
+    }
+    const float d = number(P.D, P.d_type, h);
+    float carry = 0.f;
+    if (has_state) {
+      carry = ex2(me.y + me.z);
+      if (kScaled) carry *= W.hs[((long long)b * W.nc + c) * W.units + u].x;
+    }
+    mm.wait();
+    if (u + 1 < u1) load_state(u + 1);
+    uint32_t y0[32], y1[32];
+    if (has_state) tmem_ld32_nowait(lanes + 128 + half * 32, y0);
+    tmem_ld32(lanes + 192 + half * 32, y1);
+    if (has_state) settle(y0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = base + kOutX + piece(row, half * 4 + j);
+      float f[8];
+      unpack8<T>(lds16(at), f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float v = __uint_as_float(y1[j * 8 + e]);
+        v = (kScaled ? v * sc.y : v) + d * f[e];
+        if (has_state) v += carry * __uint_as_float(y0[j * 8 + e]);
+        f[e] = row < rows ? v : 0.f;
+      }
+      sts16(at, pack8<T>(f));
+    }
+    tc_fence_before();
+    __syncthreads();
+    T* out = y + (long long)h * P.dim + p0;
+    store_tile<T>(out, P.y_st, base + kOutX, out_rows, cols, vector_ok(out, P.y_st, 0, cols));
+    if (u + 1 < u1) {
+      __syncthreads();
+      load_x(u + 1);
+      cp_commit();
+      cp_wait<0>();
+      fence_async();
+      __syncthreads();
+    }
+  }
+  mma_end<256>(tmem);
+}
+
+// ---------------------------------------------------------------- gradients by chunk and group
+// One CTA: a chunk and some units of a group, tokens s as rows.  TMEM: B C^T (128 columns), a work area (128), and the
+// sums over the units of what reaches C and B through the states (128 each).  A unit takes three steps:
+//   1. G B_s and H C_t (64 columns each): the states' part of x's gradient, and q_t = exp(l_t) dy_t . H C_t and
+//      r_s = exp(l_end - l_s) x_s . G B_s, from states with their remainders: the gradients of A, dt and the bias, which
+//      are 32-bit sums, hang on them.
+//   2. x_s . dy_t (128 columns), and the units' sums for C and B on the tensor cores.  The pairs' weights give the
+//      operand of step 3, the group's sum of s_s exp(l_t - l_s) (dy_t . x_s), and its products with C_t . B_s summed
+//      by row and by column.
+//   3. the pairs' part of x's gradient; prefix and suffix sums over the tokens give the gradient of A s.
+// After the last unit the group's sum gives the pairs' part of dB and dC in two products.
+constexpr uint32_t kGB = 0, kGC = kTile128, kGX = 2 * kTile128, kGY = kGX + kTile64, kGH = kGY + kTile64, kGG = kGH + 2 * kTile64,
+                   kGM = kGG + 2 * kTile64, kGPrm = kGM + kTile128, kGRow = kGPrm + Q * 16, kGCol = kGRow + 7 * Q * 4,
+                   kGRed = kGCol + 4 * Q * 4, kGBar = kGRed + 32 * 4, kGradSmem = kGBar + 16;
+
+// Sums over a warp's lanes of e[column], for column = lane.
+__device__ __forceinline__ float column_sums(float (&e)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float send = up ? e[i] : e[i + o], keep = up ? e[i + o] : e[i];
+      e[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  }
+  return e[0];
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams P, const Space W, int per) {
+  constexpr bool kScaled = std::is_same<T, __half>::value;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const uint32_t base = smem_u32(smem);
+  const float4* prm = reinterpret_cast<const float4*>(smem + kGPrm);
+  float* rpairs = reinterpret_cast<float*>(smem + kGRow);        // [2][Q] each: r by pairs, r by states, q by states; [Q]: r by the token itself
+  float *rstate = rpairs + 2 * Q, *qstate = rpairs + 4 * Q, *rself = rpairs + 6 * Q;
+  float* qpairs = reinterpret_cast<float*>(smem + kGCol);        // [4][Q]
+  float* red = reinterpret_cast<float*>(smem + kGRed);           // [0..8) <G, H>, [8..16) x . dy, [16..24) pairs' time, [24..32) maxima
+  const int c = blockIdx.x, b = blockIdx.z;
+  const int gunits = W.units / P.groups, g = blockIdx.y / W.splits, split = blockIdx.y % W.splits;
+  const int u0 = g * gunits + split * per, u1 = min(u0 + per, (g + 1) * gunits);
+  const int len = tokens_of(P, b), rows = min(Q, len - c * Q), out_rows = min(Q, P.length - c * Q);
+  const int row = threadIdx.x & 127, half = threadIdx.x >> 7, warp = threadIdx.x >> 5, quad = warp & 3, lane = threadIdx.x & 31;
+  const long long bc = (long long)b * W.nc + c, dx_st = P.dx_st, grp_st = P.dg_st;
+  T* dx = reinterpret_cast<T*>(P.dx) + b * P.dx_sb + (long long)c * Q * dx_st;
+  const long long grp_at = b * P.dg_sb + (long long)c * Q * grp_st + g * kN;
+  T *dB = reinterpret_cast<T*>(P.dB) + grp_at, *dC = reinterpret_cast<T*>(P.dC) + grp_at;
+  if (rows <= 0) {                                       // behind the sequence's end
+    for (int u = u0; u < u1; ++u) {
+      const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+      for (int i = threadIdx.x; i < out_rows * cols; i += kThreads)
+        dx[(long long)(i / cols) * dx_st + (long long)h * P.dim + p0 + i % cols] = from_f32<T>(0.f);
+      if (threadIdx.x == 0) W.unit_sums[bc * W.units + u] = make_float2(0.f, 0.f);
+    }
+    if (W.splits == 1)
+      for (int i = threadIdx.x; i < out_rows * kN; i += kThreads)
+        dB[(long long)(i / kN) * grp_st + i % kN] = dC[(long long)(i / kN) * grp_st + i % kN] = from_f32<T>(0.f);
+    return;
+  }
+  const bool has_h = c > 0 || P.state_in, has_g = (c + 1) * Q < len || P.dstate_out;
+  const T* Bc = reinterpret_cast<const T*>(P.B) + (long long)b * P.b_sb + (long long)c * Q * P.b_st + g * kN;
+  const T* Cc = reinterpret_cast<const T*>(P.C) + (long long)b * P.c_sb + (long long)c * Q * P.c_st + g * kN;
+  const T* xc = reinterpret_cast<const T*>(P.x) + (long long)b * P.x_sb + (long long)c * Q * P.x_st;
+  const T* yc = reinterpret_cast<const T*>(P.dy) + (long long)b * P.dy_sb + (long long)c * Q * P.dy_st;
+  auto load_states = [&](int u) {
+    const long long at = (bc * W.units + u) * (2 * kN * TP);
+    if (has_h) { load_plane(base + kGH, W.h + at); load_plane(base + kGH + kTile64, W.h + at + kN * TP); }
+    if (has_g) { load_plane(base + kGG, W.g + at); load_plane(base + kGG + kTile64, W.g + at + kN * TP); }
+  };
+  auto load_tokens = [&](int u) {
+    const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+    const T *px = xc + (long long)h * P.dim + p0, *py = yc + (long long)h * P.dim + p0;
+    load_tile<T, 8>(base + kGX, px, P.x_st, rows, cols, vector_ok(px, P.x_st, 0, cols));
+    load_tile<T, 8>(base + kGY, py, P.dy_st, rows, cols, vector_ok(py, P.dy_st, 0, cols));
+    const float4* s = W.prm + ((long long)b * P.heads + h) * W.lp + (long long)c * Q;
+    if (threadIdx.x < Q) cp16(base + kGPrm + threadIdx.x * 16, s + threadIdx.x, true);
+  };
+  load_tile<T, 16>(base + kGB, Bc, P.b_st, rows, kN, vector_ok(Bc, P.b_st, 0, kN));
+  load_tile<T, 16>(base + kGC, Cc, P.c_st, rows, kN, vector_ok(Cc, P.c_st, 0, kN));
+  cp_commit();
+  load_states(u0);
+  load_tokens(u0);
+  cp_commit();
+  // units' sums for C and B share a scale: that of the largest product of a state's and its tokens' scales
+  float cscale = 1.f, bscale = 1.f;
+  if (kScaled && (has_h || has_g)) {
+    cscale = bscale = 0.f;
+    for (int u = u0; u < u1; ++u) {
+      const float2 hs = W.hs[bc * W.units + u], gs = W.gs[bc * W.units + u];
+      cscale = fmaxf(cscale, hs.x * gs.y);
+      bscale = fmaxf(bscale, gs.x * hs.y);
+    }
+  }
+  uint32_t tmem;
+  Mma mm = mma_begin<512>(reinterpret_cast<uint64_t*>(smem + kGBar), reinterpret_cast<uint32_t*>(smem + kGBar + 8), P.err, tmem);
+  const uint32_t lanes = tmem + ((uint32_t)quad << 21), work = tmem + 128, sum_c = tmem + 256, sum_b = tmem + 384;
+  cp_wait<1>();
+  fence_async();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    tc_fence_after();
+    mma<false, false>(tmem, base + kGB, base + kGC, idesc<T>(Q, false, false), 8, false);
+    mm.commit();
+  }
+  mm.wait();
+  float top = 0.f;
+  if (kScaled) {                                         // the largest |B_s . C_t| of my row's pairs
+    uint32_t m = 0;
+    for (int cb = half; cb < 4; cb += 2) {
+      if (cb < quad) continue;
+      uint32_t r[32];
+      tmem_ld32(lanes + cb * 32, r);
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (cb * 32 + i >= row) m = max(m, r[i] & 0x7fffffffu);
+    }
+    rpairs[half * Q + row] = __uint_as_float(m);
+    __syncthreads();
+    top = fmaxf(rpairs[row], rpairs[Q + row]);
+  }
+  const float2 sc = kScaled ? scale_of(__float_as_uint(top)) : make_float2(1.f, 1.f);
+  float ds[2][32];
+#pragma unroll
+  for (int i = 0; i < 64; ++i) ds[i >> 5][i & 31] = 0.f;
+  cp_wait<0>();
+  fence_async();
+  __syncthreads();
+
+  for (int u = u0; u < u1; ++u) {
+    const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+    // step 1
+    if (threadIdx.x == 0 && (has_h || has_g) && mm.ok) {
+      tc_fence_after();
+      if (has_g) {
+        mma<false, true>(work, base + kGB, base + kGG, idesc<T>(TP, false, true), 8, false);
+        mma<false, true>(work, base + kGB, base + kGG + kTile64, idesc<T>(TP, false, true), 8, true);
+      }
+      if (has_h) {
+        mma<false, true>(work + 64, base + kGC, base + kGH, idesc<T>(TP, false, true), 8, false);
+        mma<false, true>(work + 64, base + kGC, base + kGH + kTile64, idesc<T>(TP, false, true), 8, true);
+      }
+      mm.commit();
+    }
+    const float4 me = prm[row], end = prm[Q - 1];
+    float2 hs = make_float2(1.f, 1.f), gs = make_float2(1.f, 1.f);
+    if (kScaled && (has_h || has_g)) { hs = W.hs[bc * W.units + u]; gs = W.gs[bc * W.units + u]; }
+    const float from_in = ex2(me.y + me.z), to_end = ex2((end.y - me.y) + (end.z - me.z));
+    const float wy = kScaled ? from_in * (hs.x / cscale) : from_in, wx = me.x * (kScaled ? to_end * (gs.x / bscale) : to_end);
+    float gh = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = piece(row, half * 4 + j);
+      float f[8], o[8];
+      if (has_h) {
+        unpack8<T>(lds16(base + kGY + at), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= wy;
+        sts16(base + kGM + at, pack8<T>(f));
+      }
+      if (has_g) {
+        unpack8<T>(lds16(base + kGX + at), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] *= wx;
+        sts16(base + kGM + kTile64 + at, pack8<T>(f));
+      }
+      if (has_h && has_g) {                              // my row of the states: <G, H>
+        float hl[8], gl[8];
+        unpack8<T>(lds16(base + kGH + at), f);
+        unpack8<T>(lds16(base + kGH + kTile64 + at), hl);
+        unpack8<T>(lds16(base + kGG + at), o);
+        unpack8<T>(lds16(base + kGG + kTile64 + at), gl);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) gh += (f[e] + hl[e]) * (o[e] + gl[e]);
+      }
+    }
+    gh = warp_sum(gh);
+    if (lane == 0) red[warp] = gh;
+    fence_async();
+    float dxi[32];
+    if (has_h || has_g) {
+      mm.wait();
+      uint32_t r[32];
+      float r_part = 0.f, q_part = 0.f;
+      if (has_g) {
+        tmem_ld32(lanes + 128 + half * 32, r);
+        const float f = to_end * gs.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float x[8];
+          unpack8<T>(lds16(base + kGX + piece(row, half * 4 + j)), x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            dxi[j * 8 + e] = f * __uint_as_float(r[j * 8 + e]);
+            r_part += dxi[j * 8 + e] * x[e];
+          }
+        }
+      }
+      if (has_h) {
+        tmem_ld32(lanes + 192 + half * 32, r);
+        const float f = from_in * hs.x;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float y[8];
+          unpack8<T>(lds16(base + kGY + piece(row, half * 4 + j)), y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) q_part += __uint_as_float(r[j * 8 + e]) * y[e];
+        }
+        q_part *= f;
+      }
+      rstate[half * Q + row] = r_part;
+      qstate[half * Q + row] = q_part;
+      tc_fence_before();
+    } else {
+      rstate[half * Q + row] = qstate[half * Q + row] = 0.f;
+    }
+    if (!has_g)
+#pragma unroll
+      for (int i = 0; i < 32; ++i) dxi[i] = 0.f;
+    __syncthreads();
+    // step 2
+    if (threadIdx.x == 0 && mm.ok) {
+      tc_fence_after();
+      mma<false, false>(work, base + kGX, base + kGY, idesc<T>(Q, false, false), 4, false);
+      if (has_h) mma<false, false>(sum_c, base + kGM, base + kGH, idesc<T>(kN, false, false), 4, u > u0);
+      if (has_g) mma<false, false>(sum_b, base + kGM + kTile64, base + kGG, idesc<T>(kN, false, false), 4, u > u0);
+      mm.commit();
+    }
+    mm.wait();
+    float r_sum = 0.f, diag = 0.f, pair_time = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int cb = half + 2 * k;
+      if (cb >= quad) {
+        uint32_t r[32], d[32];
+        float e[32];
+        tmem_ld32_nowait(lanes + cb * 32, r);
+        tmem_ld32(lanes + 128 + cb * 32, d);
+        settle(r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int t = cb * 32 + j * 8 + i;
+            const float4 to = prm[t];
+            const float gap = (to.y - me.y) + (to.z - me.z);
+            float w = ex2(gap);
+            if (t < row) w = 0.f;
+            const float m = __uint_as_float(r[j * 8 + i]) * w, dm = __uint_as_float(d[j * 8 + i]);
+            f[i] = kScaled ? m * sc.x : m;
+            ds[k][j * 8 + i] += me.x * (dm * w);
+            float both = m * dm;
+            if (t == row) {                              // no decay between a token and itself: kept out of the sums
+              diag = dm;
+              rself[row] = both;
+              both = 0.f;
+            }
+            r_sum += both;
+            both *= me.x;
+            e[j * 8 + i] = both;
+            if (t > row) pair_time += both * gap;
+          }
+          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<T>(f));
+        }
+        qpairs[quad * Q + cb * 32 + lane] = column_sums(e, lane);
+      } else {
+        for (int j = 0; j < 4; ++j) sts16(base + kGM + piece2(row, cb * 4 + j), make_uint4(0, 0, 0, 0));
+        qpairs[quad * Q + cb * 32 + lane] = 0.f;
+      }
+    }
+    rpairs[half * Q + row] = r_sum;
+    diag = warp_sum(diag);
+    pair_time = warp_sum(pair_time);
+    if (lane == 0) { red[8 + warp] = diag; red[16 + warp] = pair_time; }
+    tc_fence_before();
+    fence_async();
+    __syncthreads();
+    // step 3
+    if (threadIdx.x == 0 && mm.ok) {
+      tc_fence_after();
+      mma<false, true>(work, base + kGM, base + kGY, idesc<T>(TP, false, true), 8, false);
+      mm.commit();
+    }
+    if (u + 1 < u1) load_states(u + 1);
+    if (warp == 7) {                                     // four tokens a lane
+      float a[4], r[4], sa = 0.f, sb = 0.f, bs[4], time = 0.f;
+      float through = 0.f, dd = 0.f, da = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { through += red[i]; dd += red[8 + i]; da += red[16 + i]; }
+      through *= ex2(end.y + end.z) * (hs.x * gs.x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = 4 * lane + i;
+        const float s = prm[t].x, rp = rpairs[t] + rpairs[Q + t], rs = rstate[t] + rstate[Q + t];
+        const float qs = qstate[t] + qstate[Q + t];
+        r[i] = rp + rs + rself[t];
+        a[i] = ((qpairs[t] + qpairs[Q + t]) + (qpairs[2 * Q + t] + qpairs[3 * Q + t])) + qs - s * rp;
+        bs[i] = s * rs;
+        time += qs * (prm[t].y + prm[t].z) + bs[i] * ((end.y - prm[t].y) + (end.z - prm[t].z));
+        sa += a[i];
+        sb += bs[i];
+      }
+      float after = sa, before = sb;                     // sums over the lanes from mine on, and up to mine
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float va = __shfl_down_sync(0xffffffffu, after, o), vb = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane + o < 32) after += va;
+        if (lane >= o) before += vb;
+      }
+      before -= sb;
+      after -= sa;
+      float from[4];                                     // sum of a over t' >= t
+#pragma unroll
+      for (int i = 3; i >= 0; --i) { after += a[i]; from[i] = after; }
+      float2* out = W.parts + ((long long)b * W.units + u) * W.lp + (long long)c * Q + 4 * lane;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        out[i] = make_float2(from[i] + before + through, r[i]);
+        before += bs[i];
+      }
+      time = warp_sum(time);
+      // A's gradient: each contribution by the time that A works on it, which l tells; no differences of large sums
+      if (lane == 0) {
+        da = (da + time) + through * (end.y + end.z);
+        W.unit_sums[bc * W.units + u] = make_float2(dd, (float)((double)da / decay_rate(P.A[h])));
+      }
+    }
+    const float dskip = number(P.D, P.d_type, h);
+    mm.wait();
+    {
+      uint32_t r[32];
+      tmem_ld32(lanes + 128 + half * 32, r);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t at = piece(row, half * 4 + j);
+        float f[8];
+        unpack8<T>(lds16(base + kGY + at), f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float v = __uint_as_float(r[j * 8 + e]);
+          f[e] = row < rows ? me.x * ((kScaled ? v * sc.y : v) + dxi[j * 8 + e]) + dskip * f[e] : 0.f;
+        }
+        sts16(base + kGX + at, pack8<T>(f));
+      }
+    }
+    tc_fence_before();
+    __syncthreads();
+    T* out = dx + (long long)h * P.dim + p0;
+    store_tile<T>(out, dx_st, base + kGX, out_rows, cols, vector_ok(out, dx_st, 0, cols));
+    __syncthreads();
+    if (u + 1 < u1) {
+      load_tokens(u + 1);
+      cp_commit();
+      cp_wait<0>();
+      fence_async();
+      __syncthreads();
+    }
+  }
+
+  // the pairs' part of dB and dC
+  float2 all = make_float2(1.f, 1.f);
+  if (kScaled) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 64; ++i) m = max(m, __float_as_uint(ds[i >> 5][i & 31]) & 0x7fffffffu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) red[24 + warp] = __uint_as_float(m);
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(red[24 + i]));
+    all = scale_of(m);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = kScaled ? ds[k][j * 8 + i] * all.x : ds[k][j * 8 + i];
+      sts16(base + kGM + piece2(row, (half + 2 * k) * 4 + j), pack8<T>(f));
+    }
+  fence_async();
+  __syncthreads();
+  if (threadIdx.x == 0 && mm.ok) {
+    tc_fence_after();
+    mma<false, true>(work, base + kGM, base + kGC, idesc<T>(kN, false, true), 8, false);
+    mma<true, true>(tmem, base + kGM, base + kGB, idesc<T>(kN, true, true), 8, false);
+    mm.commit();
+  }
+  mm.wait();
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {              // dB, dC
+    const uint32_t pairs = lanes + (which ? 0 : 128), states = lanes + (which ? 256 : 384);
+    const bool has = which ? has_h : has_g;
+    const float back = kScaled ? (which ? cscale : bscale) : 1.f;
+    float* part = which ? W.pc : W.pb;
+    for (int k = 0; k < 2; ++k) {
+      uint32_t r[32], d[32];
+      if (has) tmem_ld32_nowait(states + half * 64 + k * 32, d);
+      tmem_ld32(pairs + half * 64 + k * 32, r);
+      if (has) settle(d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          f[e] = __uint_as_float(r[j * 8 + e]) * all.y;
+          if (has) f[e] += __uint_as_float(d[j * 8 + e]) * back;
+          if (row >= rows) f[e] = 0.f;
+        }
+        if (W.splits > 1) {
+          float* p = part + ((((long long)split * P.batch + b) * W.lp + (long long)c * Q + row) * P.groups + g) * kN + half * 64 + k * 32 + j * 8;
+          *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+          *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+          sts16(base + (which ? kGX : kGM) + piece2(row, half * 8 + k * 4 + j), pack8<T>(f));
+        }
+      }
+    }
+  }
+  if (W.splits == 1) {
+    __syncthreads();
+    for (int hf = 0; hf < 2; ++hf) {
+      store_tile<T>(dB + hf * 64, grp_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB + hf * 64, grp_st, 0, 64));
+      store_tile<T>(dC + hf * 64, grp_st, base + kGX + hf * kTile64, out_rows, 64, vector_ok(dC + hf * 64, grp_st, 0, 64));
+    }
+  }
+  mma_end<512>(tmem);
+}
+
+// ---------------------------------------------------------------- sums behind the gradients
+// One CTA: a chunk of 32 heads.  The gradient of dt, and the chunk's sum for the bias.
+template <typename T>
+__global__ void __launch_bounds__(128) finish_dt_kernel(const SelectiveParams P, const Space W) {
+  __shared__ float grad[Q][33];
+  const int c = blockIdx.x, h0 = blockIdx.y * 32, b = blockIdx.z, lane = threadIdx.x & 31;
+  const int len = tokens_of(P, b);
+  for (int k = threadIdx.x >> 5; k < 32 && h0 + k < P.heads; k += 4) {
+    const int h = h0 + k;
+    const float rate = P.A[h];
+    float db = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      const int t = i * 32 + lane, token = c * Q + t;
+      float out = 0.f;
+      if (token < len) {
+        const float4 m = W.prm[((long long)b * P.heads + h) * W.lp + token];
+        float ga = 0.f, gs = 0.f;
+        for (int p = 0; p < W.ptiles; ++p) {
+          const float2 v = W.parts[((long long)b * W.units + h * W.ptiles + p) * W.lp + token];
+          ga += v.x;
+          gs += v.y;
+        }
+        out = (rate * ga + gs) * m.w;
+        db += out;
+      }
+      grad[t][k] = out;
+    }
+    db = warp_sum(db);
+    if (lane == 0) W.bias_sums[((long long)b * W.nc + c) * P.heads + h] = db;
+  }
+  __syncthreads();
+  T* ddt = reinterpret_cast<T*>(P.ddt) + (long long)b * P.length * P.heads;
+  for (int t = threadIdx.x >> 5; t < Q && c * Q + t < P.length; t += 4)
+    if (h0 + lane < P.heads) ddt[(long long)(c * Q + t) * P.heads + h0 + lane] = from_f32<T>(grad[t][lane]);
+}
+
+// One warp a head: gradients of A, the bias and D.
+__global__ void __launch_bounds__(128) finish_heads_kernel(const SelectiveParams P, const Space W) {
+  const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (h >= P.heads) return;
+  float da = 0.f, db = 0.f, dd = 0.f;
+  for (int i = lane; i < P.batch * W.nc; i += 32) {
+    db += W.bias_sums[(long long)i * P.heads + h];
+    for (int p = 0; p < W.ptiles; ++p) {
+      const float2 v = W.unit_sums[(long long)i * W.units + h * W.ptiles + p];
+      dd += v.x;
+      da += v.y;
+    }
+  }
+  da = warp_sum(da);
+  db = warp_sum(db);
+  dd = warp_sum(dd);
+  if (lane == 0) {
+    if (P.dA) P.dA[h] = da;
+    if (P.dbias) put_number(P.dbias, P.bias_type, h, db);
+    if (P.dD) put_number(P.dD, P.d_type, h, dd);
+  }
+}
+
+// dB and dC from the splits' sums, four columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) finish_groups_kernel(const SelectiveParams P, const Space W) {
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, width = (long long)P.groups * kN;
+  const long long all = (long long)P.batch * P.length * width;
+  if (i * 4 >= all) return;
+  const long long token = i * 4 / width, b = token / P.length, t = token % P.length;
+  const bool in = t < tokens_of(P, (int)b);
+  const long long at = (b * W.lp + t) * width + i * 4 % width, step = (long long)P.batch * W.lp * width;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const float* p = which ? W.pc : W.pb;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (in)
+      for (int s = 0; s < W.splits; ++s) {
+        const float4 a = *reinterpret_cast<const float4*>(p + s * step + at);
+        v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
+      }
+    T* out = reinterpret_cast<T*>(which ? P.dC : P.dB) + b * P.dg_sb + t * P.dg_st + i * 4 % width;
+    const uint32_t lo = pack2<T>(v.x, v.y), hi = pack2<T>(v.z, v.w);
+    if (((uintptr_t)out & 7) == 0) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
+    } else {
+      uint16_t* o = reinterpret_cast<uint16_t*>(out);
+      o[0] = (uint16_t)lo; o[1] = (uint16_t)(lo >> 16); o[2] = (uint16_t)hi; o[3] = (uint16_t)(hi >> 16);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- one token
+// Four neighbouring numbers.
+template <typename T> __device__ __forceinline__ float4 four(const T* p, bool vec) {
+  if constexpr (std::is_same<T, float>::value) {
+    if (vec) return *reinterpret_cast<const float4*>(p);
+  } else if (vec) {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y);
+    return make_float4(a.x, a.y, b.x, b.y);
+  }
+  return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
+}
+
+// A warp takes eight rows of a head's state, four at a time: eight lanes a row, four 16-byte loads a lane.  The state
+// does not wait for the kernel before, which may still be writing x, B and C.
+template <typename T, typename X>
+__global__ void __launch_bounds__(128) step_kernel(const SelectiveStepParams P) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y, b = blockIdx.z, g = h / (P.heads / P.groups);
+  const int l8 = lane & 7, sub = lane >> 3;
+  float4* state = reinterpret_cast<float4*>(P.state) + ((long long)b * P.heads + h) * P.dim * 32 + l8;
+  float4 now[2][4];
+  int row[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    row[k] = blockIdx.x * 32 + warp * 8 + k * 4 + sub;
+    if (row[k] < P.dim)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) now[k][j] = state[(long long)row[k] * 32 + j * 8];
+  }
+  const float v = to_f32((reinterpret_cast<const T*>(P.dt) + b * P.dt_sb)[h]) + number(P.dt_bias, P.bias_type, h);
+  const float s = v <= 20.0f ? log1pf(expf(v)) : v, decay = expf(s * P.A[h]), skip = number(P.D, P.d_type, h);
+  const X* Bp = reinterpret_cast<const X*>(P.B) + b * P.b_sb + g * kN + l8 * 4;
+  const X* Cp = reinterpret_cast<const X*>(P.C) + b * P.c_sb + g * kN + l8 * 4;
+  const X* xp = reinterpret_cast<const X*>(P.x) + b * P.x_sb + (long long)h * P.dim;
+  const bool bvec = ((uintptr_t)Bp & (4 * sizeof(X) - 1)) == 0, cvec = ((uintptr_t)Cp & (4 * sizeof(X) - 1)) == 0;
+  T* yp = reinterpret_cast<T*>(P.y) + ((long long)b * P.heads + h) * P.dim;
+  wait_for_launch();
+  float x[2];
+  float4 Bv[4], Cv[4];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) x[k] = row[k] < P.dim ? to_f32(xp[row[k]]) : 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    Bv[j] = four(Bp + j * 32, bvec);
+    Cv[j] = four(Cp + j * 32, cvec);
+  }
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float y = 0.f;
+    if (row[k] < P.dim) {
+      const float u = s * x[k];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float4 n = now[k][j];
+        n.x = n.x * decay + u * Bv[j].x; n.y = n.y * decay + u * Bv[j].y;
+        n.z = n.z * decay + u * Bv[j].z; n.w = n.w * decay + u * Bv[j].w;
+        y += (n.x * Cv[j].x + n.y * Cv[j].y) + (n.z * Cv[j].z + n.w * Cv[j].w);
+        state[(long long)row[k] * 32 + j * 8] = n;
+      }
+    }
+    y += __shfl_xor_sync(0xffffffffu, y, 4);
+    y += __shfl_xor_sync(0xffffffffu, y, 2);
+    y += __shfl_xor_sync(0xffffffffu, y, 1);
+    if (l8 == 0 && row[k] < P.dim) yp[row[k]] = from_f32<T>(y + skip * x[k]);
+  }
+}
+
+// ---------------------------------------------------------------- launches
+// Dynamic shared memory of a kernel beyond 48 KB, asked for once a thread and device.
+template <auto K> int allow(uint32_t bytes) {
+  static thread_local bool done[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return kECuda;
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(K, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) { last_launch_error() = e; return kECuda; }
+    done[dev] = true;
+  }
+  return kOk;
+}
+
+template <typename T, bool REV, bool LO> int pass(const SelectiveParams& P, const Space& W, cudaStream_t st) {
+  if (int s = allow<state_pass_kernel<T, REV, LO>>(kPassSmem)) return s;
+  state_pass_kernel<T, REV, LO><<<dim3(W.units, P.batch), kThreads, kPassSmem, st>>>(P, W);
+  return launch_status();
+}
+
+template <typename T> int prepare(const SelectiveParams& P, const Space& W, cudaStream_t st) {
+  prepare_kernel<T><<<dim3(W.nc, (P.heads + 31) / 32, P.batch), 128, 0, st>>>(P, W);
+  return launch_status();
+}
+
+template <typename T> int forward(const SelectiveParams& P, cudaStream_t st) {
+  const Space W = space_of(P, false);
+  if (int s = prepare<T>(P, W, st)) return s;
+  if (W.nc > 1 || P.state_in || P.state_out)
+    if (int s = pass<T, false, false>(P, W, st)) return s;
+  if (int s = allow<out_kernel<T>>(kOutSmem)) return s;
+  const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
+  out_kernel<T><<<dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kOutSmem, st>>>(P, W, per);
+  return launch_status();
+}
+
+template <typename T> int backward(const SelectiveParams& P, cudaStream_t st) {
+  const Space W = space_of(P, true);
+  if (int s = prepare<T>(P, W, st)) return s;
+  if (W.nc > 1 || P.state_in || P.dstate_out || P.dstate_in) {
+    SelectiveParams F = P;
+    F.state_out = nullptr;
+    if (int s = pass<T, false, true>(F, W, st)) return s;
+    if (int s = pass<T, true, true>(P, W, st)) return s;
+  }
+  if (int s = allow<grad_kernel<T>>(kGradSmem)) return s;
+  const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
+  grad_kernel<T><<<dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kGradSmem, st>>>(P, W, per);
+  if (int s = launch_status()) return s;
+  finish_dt_kernel<T><<<dim3(W.nc, (P.heads + 31) / 32, P.batch), 128, 0, st>>>(P, W);
+  if (int s = launch_status()) return s;
+  finish_heads_kernel<<<(P.heads + 3) / 4, 128, 0, st>>>(P, W);
+  if (int s = launch_status()) return s;
+  if (W.splits > 1) {
+    const long long all = (long long)P.batch * P.length * P.groups * (kN / 4);
+    finish_groups_kernel<T><<<(unsigned)((all + 255) / 256), 256, 0, st>>>(P, W);
+    return launch_status();
+  }
+  return kOk;
+}
+
+}  // namespace
+
+long long selective_workspace(int batch, int length, int heads, int dim, int groups, bool backward) {
+  SelectiveParams P{};
+  P.batch = batch; P.length = length; P.heads = heads; P.dim = dim; P.groups = groups;
+  return space_of(P, backward).bytes;
+}
+int launch_selective_forward(const SelectiveParams& P, cudaStream_t st) {
+  return P.type == SQ_TYPE_F16 ? forward<__half>(P, st) : forward<__nv_bfloat16>(P, st);
+}
+int launch_selective_backward(const SelectiveParams& P, cudaStream_t st) {
+  return P.type == SQ_TYPE_F16 ? backward<__half>(P, st) : backward<__nv_bfloat16>(P, st);
+}
+int launch_selective_step(const SelectiveStepParams& P, cudaStream_t st) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t at{};
+  at.gridDim = dim3((P.dim + 31) / 32, P.heads, P.batch);
+  at.blockDim = dim3(128);
+  at.stream = st;
+  at.attrs = &early;
+  at.numAttrs = P.behind ? 1 : 0;
+  const cudaError_t e = P.type == SQ_TYPE_F16 ? (P.x_f32 ? cudaLaunchKernelEx(&at, step_kernel<__half, float>, P)
+                                                         : cudaLaunchKernelEx(&at, step_kernel<__half, __half>, P))
+                                              : (P.x_f32 ? cudaLaunchKernelEx(&at, step_kernel<__nv_bfloat16, float>, P)
+                                                         : cudaLaunchKernelEx(&at, step_kernel<__nv_bfloat16, __nv_bfloat16>, P));
+  if (e != cudaSuccess) { cudaGetLastError(); last_launch_error() = e; return kECuda; }
+  return launch_status();
+}
+
+}  // namespace sq

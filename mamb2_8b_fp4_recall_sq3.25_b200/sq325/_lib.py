@@ -105,6 +105,47 @@ class DistillArgs(C.Structure):
                 ('grad', p), ('grad_stride', i64)]
 
 
+class SelectiveArgs(C.Structure):
+    _fields_ = [('batch', i32), ('length', i32), ('heads', i32), ('dim', i32), ('groups', i32), ('type', i32),
+                ('x', p), ('x_batch_stride', i64), ('x_token_stride', i64),
+                ('dt', p), ('dt_batch_stride', i64), ('dt_token_stride', i64),
+                ('A', p),
+                ('B', p), ('b_batch_stride', i64), ('b_token_stride', i64),
+                ('C', p), ('c_batch_stride', i64), ('c_token_stride', i64),
+                ('D', p), ('d_type', i32), ('dt_bias', p), ('bias_type', i32), ('state_in', p), ('lengths', p),
+                ('y', p), ('y_batch_stride', i64), ('y_token_stride', i64), ('state_out', p),
+                ('dy', p), ('dy_batch_stride', i64), ('dy_token_stride', i64), ('dstate_out', p),
+                ('dx', p), ('dx_batch_stride', i64), ('dx_token_stride', i64), ('ddt', p),
+                ('dB', p), ('dC', p), ('dg_batch_stride', i64), ('dg_token_stride', i64),
+                ('dA', p), ('dD', p), ('ddt_bias', p), ('dstate_in', p),
+                ('workspace', p), ('workspace_bytes', i64)]
+
+
+class SelectiveStepArgs(C.Structure):
+    _fields_ = [('batch', i32), ('heads', i32), ('dim', i32), ('groups', i32), ('type', i32),
+                ('x', p), ('x_batch_stride', i64), ('dt', p), ('dt_batch_stride', i64), ('A', p),
+                ('B', p), ('b_batch_stride', i64), ('C', p), ('c_batch_stride', i64),
+                ('D', p), ('d_type', i32), ('dt_bias', p), ('bias_type', i32), ('state', p), ('y', p)]
+
+
+class ConvScanStepArgs(C.Structure):
+    _fields_ = [('batch', i32), ('heads', i32), ('dim', i32), ('groups', i32), ('taps', i32), ('type', i32), ('weight_type', i32),
+                ('xbc', p), ('xbc_batch_stride', i64), ('dt', p), ('dt_batch_stride', i64), ('A', p), ('weight', p), ('bias', p),
+                ('D', p), ('d_type', i32), ('dt_bias', p), ('bias_type', i32), ('conv_state', p), ('state', p), ('y', p),
+                ('workspace', p), ('workspace_bytes', i64)]
+
+
+class CausalConvArgs(C.Structure):
+    _fields_ = [('batch', i32), ('length', i32), ('channels', i32), ('taps', i32), ('silu', i32), ('type', i32),
+                ('weight_type', i32),
+                ('x', p), ('x_batch_stride', i64), ('x_token_stride', i64), ('codes', p), ('scales', p),
+                ('weight', p), ('bias', p), ('state_in', p), ('lengths', p),
+                ('y', p), ('y_batch_stride', i64), ('y_token_stride', i64), ('state_out', p),
+                ('dy', p), ('dy_batch_stride', i64), ('dy_token_stride', i64), ('dstate_out', p),
+                ('dx', p), ('dstate_in', p), ('dweight', p), ('dbias', p),
+                ('workspace', p), ('workspace_bytes', i64)]
+
+
 # name -> (restype, argtypes)
 _PROTOS = {
     'sq_abi_version': (C.c_int, []),
@@ -153,6 +194,17 @@ _PROTOS = {
     'sq_distill_forward': (C.c_int, [C.POINTER(DistillArgs), p]),
     'sq_distill_backward': (C.c_int, [C.POINTER(DistillArgs), p]),
     'sq_distill_loss_grad': (C.c_int, [C.POINTER(DistillArgs), p]),
+    'sq_selective_workspace': (i64, [C.c_int] * 6),
+    'sq_selective_forward': (C.c_int, [C.POINTER(SelectiveArgs), p]),
+    'sq_selective_backward': (C.c_int, [C.POINTER(SelectiveArgs), p]),
+    'sq_selective_step': (C.c_int, [C.POINTER(SelectiveStepArgs), p]),
+    'sq_conv_scan_step': (C.c_int, [C.POINTER(ConvScanStepArgs), p]),
+    'sq_causal_conv_workspace': (i64, [C.c_int] * 4),
+    'sq_causal_conv_forward': (C.c_int, [C.POINTER(CausalConvArgs), p]),
+    'sq_causal_conv_backward': (C.c_int, [C.POINTER(CausalConvArgs), p]),
+    'sq_causal_conv_step': (C.c_int, [p, i64, p, p, p, p] + [C.c_int] * 6 + [p]),
+    'sq_pack_activations': (C.c_int, [p, i64, i64, C.c_int, C.c_int, p, p, p]),
+    'sq_unpack_activations': (C.c_int, [p, p, i64, C.c_int, C.c_int, p, p]),
 }
 
 _lib = None
