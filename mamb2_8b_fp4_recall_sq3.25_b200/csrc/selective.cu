@@ -13,12 +13,12 @@
 // gradients, with the states' own gradients from state_pass_kernel walking backwards (G_in = exp(l_end) G_out +
 // sum_t exp(l_t) dy_t C_t^T).  All products run on tcgen05 with fp32 accumulators in TMEM.
 //
-// Operands are 16 bits.  Inputs enter as they are; what is computed is rounded, in these places:
-//   * the weighted tokens of state_pass_kernel and the states themselves as two numbers (value and remainder, 16 bits
-//     of bf16, 22 of fp16) wherever an fp32 result hangs on them;
-//   * the pairs' weights exp(l_t - l_s) s_s (C_t . B_s), the states in y, and the operands of dB and dC as one number:
-//     their results are 16-bit tensors, whose own rounding is as large.
-// fp16 operands are scaled by powers of two per row, chunk or CTA (bf16 has fp32's range and needs none).
+// Operands are 16 bits.  B and C are brought to scaled fp16 once (prepare_kernel), so that states and weighted tokens can
+// be fp16 beside them, value and remainder (22 bits) wherever a 32-bit result hangs on them.  Rounded to one number are:
+//   * the pairs' weights exp(l_t - l_s) s_s (C_t . B_s) beside x and dy, in their type;
+//   * the states in y, and the operands of dB and dC beside the states and of the pairs' part, in fp16.
+// Their results are 16-bit tensors, whose own rounding is as large.  fp16 operands are scaled by powers of two per row,
+// tile, chunk or CTA.  A bf16 number of B or C below 2^-28 of its tile's largest loses bits that no sum can hold.
 // Sums of A s are doubles, kept as two floats: neighbours' differences keep 24 bits wherever in the chunk they lie.
 #include "selective.cuh"
 #include <type_traits>
@@ -70,14 +70,29 @@ template <typename T> __device__ __forceinline__ constexpr uint32_t idesc(int n,
   const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (f << 7) | (f << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
+// A state's plane: 16-byte pieces (eight rows p) [8][128 columns n], without swizzle.  As N = p, K = n: 16 of K are
+// 256 bytes on; as N = n, K = p: 4,096 bytes on.
+__device__ __forceinline__ uint64_t desc_plain(uint32_t a, uint32_t lbo, uint32_t sbo) {
+  return (uint64_t)((a & 0x3FFFFu) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(sbo >> 4) << 32 | (uint64_t)1 << 46;
+}
+enum Form { kK, kMn, kPlaneP, kPlaneN };            // K-major tile, MN-major tile, plane with N = p, plane with N = n
+template <Form F> __device__ __forceinline__ uint64_t desc_at(uint32_t a, int k) {
+  if constexpr (F == kK) return desc_k(a + (uint32_t)((k >> 2) * kTile64 + (k & 3) * 32));
+  else if constexpr (F == kMn) return desc_mn(a + (uint32_t)k * 2048);
+  else if constexpr (F == kPlaneP) return desc_plain(a + (uint32_t)k * 256, 128, 2048);
+  else return desc_plain(a + (uint32_t)k * 4096, 2048, 128);
+}
 // D[128][n] (+)= A . B over K = 16 * steps; a / b: addresses of the tiles.  K-major tiles of 128 columns go on in
 // their second half after four steps.
-template <bool A_MN, bool B_MN>
+template <Form FA, Form FB>
 __device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t id, int steps, bool accumulate) {
-  for (int k = 0; k < steps; ++k) {
-    const uint32_t kk = (uint32_t)((k >> 2) * kTile64 + (k & 3) * 32), km = (uint32_t)k * 2048;
-    umma_f16(d, A_MN ? desc_mn(a + km) : desc_k(a + kk), B_MN ? desc_mn(b + km) : desc_k(b + kk), id, accumulate || k);
-  }
+#pragma unroll
+  for (int k = 0; k < steps; ++k) umma_f16(d, desc_at<FA>(a, k), desc_at<FB>(b, k), id, accumulate || k);
+}
+// `bytes` (a multiple of 16) from global to shared memory, counted by the barrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -128,9 +143,9 @@ template <typename T> __device__ __forceinline__ void split8(const float (&f)[8]
 }
 
 // The power of two that brings `bits` (a maximum's, sign cleared) to [2^13, 2^14) and its inverse: {there, back}.
-__device__ __forceinline__ float2 scale_of(uint32_t bits) {
+__device__ __forceinline__ float2 scale_of(uint32_t bits, int most = 60) {
   int e = (int)(bits >> 23) - 140;
-  e = bits ? max(-60, min(60, e)) : 0;                  // products of two scales stay numbers
+  e = bits ? max(-most, min(most, e)) : 0;              // products of two scales stay numbers
   return make_float2(__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23));
 }
 
@@ -154,8 +169,10 @@ __device__ __forceinline__ int tokens_of(const SelectiveParams& P, int b) {
 struct Space {
   int nc, ptiles, units;              // chunks of the longest sequence, tiles of a head's rows, heads * ptiles
   long long lp;
-  float4* prm;                        // [B][H][lp]: s, l (value and remainder, base 2), sigmoid(dt + bias)
+  float* rec;                         // [B][H][nc][4][Q]: s, l (value, remainder; base 2), sigmoid(dt + bias)
   float* smax;                        // [B][H][nc]: the largest s of a chunk
+  uint16_t *bt, *ct;                  // [B][nc][G][128][128]: B and C as shared memory holds them
+  float *bback, *cback;               // [B][nc][G]: what brings them back
   uint16_t *h, *g;                    // [B][nc][units][2][8][128][8]: states entering a chunk, gradients of those leaving it
   float2 *hs, *gs;                    // [B][nc][units]: scale of the state, scale of the chunk's weighted tokens
   float2* parts;                      // [B][units][lp]: gradient of A s, gradient of s through the tokens
@@ -188,7 +205,11 @@ Space space_of(const SelectiveParams& P, bool backward) {
   char* base = reinterpret_cast<char*>(P.workspace);
   long long at = 0;
   auto take = [&](long long bytes) { char* p = base + at; at += (bytes + 255) / 256 * 256; return p; };
-  w.prm = reinterpret_cast<float4*>(take(bh * w.lp * 16));
+  w.rec = reinterpret_cast<float*>(take(bh * w.lp * 16));
+  w.bt = reinterpret_cast<uint16_t*>(take(bc * P.groups * kTile128));
+  w.ct = reinterpret_cast<uint16_t*>(take(bc * P.groups * kTile128));
+  w.bback = reinterpret_cast<float*>(take(bc * P.groups * 4));
+  w.cback = reinterpret_cast<float*>(take(bc * P.groups * 4));
   w.smax = reinterpret_cast<float*>(take(bh * w.nc * 4));
   const long long plane = (long long)kN * TP * 2 * 2;
   w.h = reinterpret_cast<uint16_t*>(take(bcu * plane));
@@ -211,30 +232,28 @@ Space space_of(const SelectiveParams& P, bool backward) {
 }
 
 // ---------------------------------------------------------------- tiles from global memory
-// 16-byte pieces of 128 rows of `pieces` pieces: row t at src + t * stride, rows from `rows` on and columns from
-// `cols` on are zero.  vec: pieces are whole and aligned.
-template <typename T, int PIECES>
-__device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long stride, int rows, int cols, bool vec) {
-  for (int i = threadIdx.x; i < Q * PIECES; i += kThreads) {
-    const int r = i / PIECES, j = i % PIECES;
-    const uint32_t a = dst + (PIECES == 16 ? piece2(r, j) : piece(r, j));
-    const T* p = src + (long long)r * stride + j * 8;
-    if (vec) {
-      const bool in = r < rows && j * 8 < cols;
-      cp16(a, in ? p : src, in);
-    } else {
-      uint32_t u[4] = {0, 0, 0, 0};
-      if (r < rows)
+// A tile [128][64]: row t at src + t * stride, rows from `rows` on and columns from `cols` on are zero.  vec: 16-byte
+// pieces are whole and aligned.
+template <typename T>
+__device__ __forceinline__ uint4 ragged_piece(const T* p, int n) {
+  uint32_t u[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (j * 8 + e < cols) u[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
-      sts16(a, make_uint4(u[0], u[1], u[2], u[3]));
-    }
-  }
+  for (int e = 0; e < 8; ++e)
+    if (e < n) u[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+  return make_uint4(u[0], u[1], u[2], u[3]);
 }
-// A state's plane [8 pieces][128 rows] of 16 bytes.
-__device__ __forceinline__ void load_plane(uint32_t dst, const uint16_t* src) {
-  for (int i = threadIdx.x; i < 8 * kN; i += kThreads) cp16(dst + piece(i & 127, i >> 7), src + (long long)i * 8, true);
+template <typename T>
+__device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long stride, int rows, int cols, bool vec) {
+  const int j = threadIdx.x & 7;
+  const T* p = src + (long long)(threadIdx.x >> 3) * stride + j * 8;
+#pragma unroll
+  for (int i = 0; i < Q * 8 / kThreads; ++i, p += (kThreads / 8) * stride) {
+    const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
+    const uint32_t a = dst + piece(r, j);
+    const bool in = r < rows && j * 8 < cols;
+    if (vec) cp16(a, in ? p : src, in);
+    else sts16(a, in ? ragged_piece(p, cols - j * 8) : make_uint4(0, 0, 0, 0));
+  }
 }
 // The first `rows` rows and `cols` columns of a tile [128][64] to global memory.
 template <typename T>
@@ -258,26 +277,25 @@ __device__ __forceinline__ bool vector_ok(const void* p, long long s0, long long
   return ((uintptr_t)p & 15) == 0 && ((s0 | s1 | cols) & 7) == 0;
 }
 
-// A CTA's own barrier on the tensor cores' work; a wait that expires is recorded once and no further one is begun.
-struct Mma {
+// A barrier that a CTA's threads wait on: for the tensor cores' work, or for bulk copies.  A wait that expires is
+// recorded, and no further one is begun (`ok` is the thread's own).
+struct Gate {
   uint32_t bar, parity;
-  bool ok;
-  int* err;
-  __device__ void commit() { umma_commit(bar); }
-  __device__ void wait() {
+  __device__ void wait(bool& ok, int* err) {
     if (ok && !mbar_wait(bar, parity)) {
       ok = false;
-      if (threadIdx.x == 0) atomicOr(err, (int)kDevTimeoutMma);
+      atomicOr(err, (int)kDevTimeoutMma);
     }
     parity ^= 1;
-    tc_fence_after();
   }
 };
+// Barriers [count] at `bars` and COLS columns of TMEM; `slot` holds their address.
 template <int COLS>
-__device__ __forceinline__ Mma mma_begin(uint64_t* bar, uint32_t* slot, int* err, uint32_t& tmem) {
+__device__ __forceinline__ uint32_t tensor_begin(uint64_t* bars, int count, uint32_t* slot) {
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(bar), 1);
+    for (int i = 0; i < count; ++i) mbar_init(smem_u32(bars + i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_async();
   }
   if (threadIdx.x < 32) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(slot)), "n"(COLS));
@@ -286,10 +304,9 @@ __device__ __forceinline__ Mma mma_begin(uint64_t* bar, uint32_t* slot, int* err
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  tmem = *slot;
-  return Mma{smem_u32(bar), 0, true, err};
+  return *slot;
 }
-template <int COLS> __device__ __forceinline__ void mma_end(uint32_t tmem) {
+template <int COLS> __device__ __forceinline__ void tensor_end(uint32_t tmem) {
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -301,80 +318,120 @@ template <int COLS> __device__ __forceinline__ void mma_end(uint32_t tmem) {
 __device__ __forceinline__ double decay_rate(float A) {
   return fabsf(A) < 1e-20f ? -1e-20 : (double)A * 1.4426950408889634;
 }
-// One CTA: a chunk of 32 heads.  A warp takes a head at a time, four tokens a lane.
+// One CTA: a chunk of eight heads (a warp a head, four tokens a lane), or a chunk's tile of B or C.
+constexpr int kPrepHeads = 8;
 template <typename T>
-__global__ void __launch_bounds__(128) prepare_kernel(const SelectiveParams P, const Space W) {
-  __shared__ float step[Q][33], slope[Q][33];
-  const int c = blockIdx.x, h0 = blockIdx.y * 32, b = blockIdx.z;
-  const int len = tokens_of(P, b);
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams P, const Space W, int head_blocks) {
+  __shared__ float step[kPrepHeads][Q + 4], slope[kPrepHeads][Q + 4];
+  __shared__ uint32_t tops[kThreads / 32];
+  const int c = blockIdx.x, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int len = tokens_of(P, b), rows = min(Q, len - c * Q);
+  if ((int)blockIdx.y >= head_blocks) {
+    const int i = blockIdx.y - head_blocks, g = i >> 1;
+    if (rows <= 0) return;                               // not read
+    const long long st = i & 1 ? P.c_st : P.b_st;
+    const T* src = reinterpret_cast<const T*>(i & 1 ? P.C : P.B) + (long long)b * (i & 1 ? P.c_sb : P.b_sb) + (long long)c * Q * st + g * kN;
+    const bool vec = vector_ok(src, st, 0, kN);
+    const int j = threadIdx.x & 15;
+    uint4 u[8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int r = (threadIdx.x >> 4) + k * 16;
+      const T* p = src + (long long)r * st + j * 8;
+      u[k] = r >= rows ? make_uint4(0, 0, 0, 0) : vec ? *reinterpret_cast<const uint4*>(p) : ragged_piece(p, 8);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
+    }
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffff, m >> 16));
+    if (lane == 0) tops[warp] = m;
+    __syncthreads();
+    m = 0;
+#pragma unroll
+    for (int k = 0; k < kThreads / 32; ++k) m = max(m, tops[k]);
+    const float2 sc = scale_of(__float_as_uint(to_f32(from_bits<T>(m))), 110);
+    const long long at = ((long long)b * W.nc + c) * P.groups + g;
+    char* out = reinterpret_cast<char*>((i & 1 ? W.ct : W.bt) + at * (Q * kN));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      float f[8];
+      unpack8<T>(u[k], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] *= sc.x;
+      *reinterpret_cast<uint4*>(out + piece2((threadIdx.x >> 4) + k * 16, j)) = pack8<__half>(f);
+    }
+    if (threadIdx.x == 0) (i & 1 ? W.cback : W.bback)[at] = sc.y;
+    return;
+  }
+  const int h0 = blockIdx.y * kPrepHeads, hl = threadIdx.x & 7;
   const T* dt = reinterpret_cast<const T*>(P.dt) + (long long)b * P.dt_sb;
-  const int hl = threadIdx.x & 31, h = h0 + hl;
-  const float bias = h < P.heads ? number(P.dt_bias, P.bias_type, h) : 0.f;
-#pragma unroll 4
-  for (int t = threadIdx.x >> 5; t < Q; t += 4) {
-    const int token = c * Q + t;
+  const float bias = h0 + hl < P.heads ? number(P.dt_bias, P.bias_type, h0 + hl) : 0.f;
+#pragma unroll
+  for (int k = 0; k < Q / 32; ++k) {
+    const int t = (threadIdx.x >> 3) + k * 32;
     float s = 0.f, d = 0.f;
-    if (token < len && h < P.heads) {
-      const float v = to_f32(dt[(long long)token * P.dt_st + h]) + bias;
+    if (t < rows && h0 + hl < P.heads) {
+      const float v = to_f32(dt[(long long)(c * Q + t) * P.dt_st + h0 + hl]) + bias;
       s = v <= 20.0f ? log1pf(expf(v)) : v;
       d = 1.0f / (1.0f + expf(-v));
     }
-    step[t][hl] = s;
-    slope[t][hl] = d;
+    step[hl][t] = s;
+    slope[hl][t] = d;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  for (int k = threadIdx.x >> 5; k < 32 && h0 + k < P.heads; k += 4) {
-    const double rate = decay_rate(P.A[h0 + k]);
-    float s[4], top = 0.f;
-    double l[4], sum = 0.0;
+  const int h = h0 + warp;
+  if (h >= P.heads) return;
+  const double rate = decay_rate(P.A[h]);
+  const float4 s4 = *reinterpret_cast<const float4*>(&step[warp][4 * lane]);
+  const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+  double l[4], sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s[i] = step[4 * lane + i][k];
-      sum += rate * (double)s[i];
-      l[i] = sum;
-      top = fmaxf(top, s[i]);
-    }
-    double before = sum;
+  for (int i = 0; i < 4; ++i) l[i] = sum += rate * (double)s[i];
+  double before = sum;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double v = __shfl_up_sync(0xffffffffu, before, o);
-      if (lane >= o) before += v;
-    }
-    before -= sum;
-    const long long row = (long long)b * P.heads + h0 + k;
-    float4* out = W.prm + row * W.lp + (long long)c * Q + 4 * lane;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double v = before + l[i];
-      const float hi = (float)v;
-      out[i] = make_float4(s[i], hi, (float)(v - (double)hi), slope[4 * lane + i][k]);
-    }
-    const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-    if (lane == 0) W.smax[row * W.nc + c] = __uint_as_float(m);
+  for (int o = 1; o < 32; o <<= 1) {
+    const double v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
   }
+  before -= sum;
+  float hi[4], lo[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    hi[i] = (float)(before + l[i]);
+    lo[i] = (float)(before + l[i] - (double)hi[i]);
+  }
+  const long long row = ((long long)b * P.heads + h) * W.nc + c;
+  float4* out = reinterpret_cast<float4*>(W.rec + row * (4 * Q)) + lane;
+  out[0] = s4;
+  out[Q / 4] = make_float4(hi[0], hi[1], hi[2], hi[3]);
+  out[2 * Q / 4] = make_float4(lo[0], lo[1], lo[2], lo[3]);
+  out[3 * Q / 4] = *reinterpret_cast<const float4*>(&slope[warp][4 * lane]);
+  const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
+  if (lane == 0) W.smax[row] = __uint_as_float(m);
 }
 
 // ---------------------------------------------------------------- states by chunk
 // One CTA walks the chunks of one unit (64 rows of a head's state), forwards or backwards.  The state is fp32 in
 // registers: thread (n, half) holds state[n][32 half .. +32].  A chunk's addition is B^T (w x), with w x as value and
 // remainder.  Written before each chunk: the state that enters it, value and (LO) remainder.
-constexpr uint32_t kPassX = 2 * kTile128, kPassW = kPassX + kTile64, kPassBytes = kPassW + 2 * kTile64;
-constexpr uint32_t kPassSmem = kPassBytes + 64;
+constexpr uint32_t kPassX = 2 * kTile128, kPassW = kPassX + kTile64, kPassBytes = kPassW + 2 * kTile64, kPassSmem = kPassBytes + 64;
 
 template <typename T, bool REV, bool LO>
 __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const SelectiveParams P, const Space W) {
-  constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kPassBytes);
-  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kPassBytes + 8);
-  uint32_t* tops = reinterpret_cast<uint32_t*>(smem + kPassBytes + 16);      // [2][2]: of the tokens, of the state
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPassBytes);           // tensor cores, tile 0, tile 1
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kPassBytes + 24);
+  uint32_t* tops = reinterpret_cast<uint32_t*>(smem + kPassBytes + 32);      // [2][2]: of the tokens, of the state
   const int u = blockIdx.x, b = blockIdx.y;
   const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, g = h / (P.heads / P.groups);
   const int cols = min(TP, P.dim - p0);
   const int len = tokens_of(P, b), nc = (len + Q - 1) / Q;
-  const int n = threadIdx.x & 127, half = threadIdx.x >> 7, lane_base = (threadIdx.x >> 5 & 3) * 32;
+  const int n = threadIdx.x & 127, half = threadIdx.x >> 7, quad = threadIdx.x >> 5 & 3;
   const float* first = REV ? P.dstate_out : P.state_in;
   float* last = REV ? P.dstate_in : P.state_out;
   uint16_t* planes = REV ? W.g : W.h;
@@ -382,140 +439,142 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
   const T* tok = reinterpret_cast<const T*>(REV ? P.dy : P.x) + (long long)b * (REV ? P.dy_sb : P.x_sb) + (long long)h * P.dim + p0;
   const long long tok_st = REV ? P.dy_st : P.x_st;
   const bool tok_vec = vector_ok(tok, tok_st, 0, cols);
-  const T* vec = reinterpret_cast<const T*>(REV ? P.C : P.B) + (long long)b * (REV ? P.c_sb : P.b_sb) + g * kN;
-  const long long vec_st = REV ? P.c_st : P.b_st;
-  const bool vec_vec = vector_ok(vec, vec_st, 0, kN);
-  const float4* prm = W.prm + ((long long)b * P.heads + h) * W.lp;
+  const uint16_t* tiles = (REV ? W.ct : W.bt) + ((long long)b * W.nc * P.groups + g) * (Q * kN);
+  const float* tile_back = (REV ? W.cback : W.bback) + (long long)b * W.nc * P.groups + g;
+  const float* recs = W.rec + ((long long)b * P.heads + h) * W.lp * 4;
   const long long state_at = (((long long)b * P.heads + h) * P.dim + p0) * kN + n;
+  if (threadIdx.x < 4) tops[threadIdx.x] = 0;
+  const uint32_t tmem = tensor_begin<64>(bars, 3, slot);
+  Gate done{smem_u32(bars), 0}, tile[2] = {{smem_u32(bars + 1), 0}, {smem_u32(bars + 2), 0}};
+  bool ok = true;
+  const uint32_t mine = tmem + ((uint32_t)quad << 21) + (uint32_t)half * 32;
 
+  auto load = [&](int i) {
+    const int c = REV ? nc - 1 - i : i;
+    if (threadIdx.x == 0 && (i + 1 < nc || last)) {
+      mbar_expect_tx(tile[i & 1].bar, kTile128);
+      bulk_load(base + (i & 1) * kTile128, tiles + (long long)c * P.groups * (Q * kN), kTile128, tile[i & 1].bar);
+    }
+    load_tile<T>(base + kPassX, tok + (long long)c * Q * tok_st, tok_st, len - c * Q, cols, tok_vec);
+    cp_commit();
+  };
+  float s, lh, ll, eh, el, back;                         // of the next chunk: my token's, the chunk's end's, the tile's
+  auto load_record = [&](int i) {
+    const int c = REV ? nc - 1 - i : i;
+    const float* r = recs + (long long)c * (4 * Q);
+    s = r[n]; lh = r[Q + n]; ll = r[2 * Q + n]; eh = r[2 * Q - 1]; el = r[3 * Q - 1];
+    back = tile_back[(long long)c * P.groups];
+  };
+  if (nc > 0) { load(0); load_record(0); }
   float S[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i)
     S[i] = first && half * 32 + i < cols ? first[state_at + (long long)(half * 32 + i) * kN] : 0.f;
 
-  if (threadIdx.x < 4) tops[threadIdx.x] = 0;
-  uint32_t tmem;
-  Mma mm = mma_begin<64>(bar, slot, P.err, tmem);
-  const uint32_t mine = tmem + ((uint32_t)lane_base << 16) + (uint32_t)half * 32;
-
-  auto load = [&](int i) {
-    const int c = REV ? nc - 1 - i : i;
-    load_tile<T, 8>(base + kPassX, tok + (long long)c * Q * tok_st, tok_st, len - c * Q, cols, tok_vec);
-    load_tile<T, 16>(base + (i & 1) * kTile128, vec + (long long)c * Q * vec_st, vec_st, len - c * Q, kN, vec_vec);
-    cp_commit();
-  };
-  if (nc > 0) load(0);
   for (int i = 0; i < nc; ++i) {
     const int c = REV ? nc - 1 - i : i;
     const long long at = ((long long)b * W.nc + c) * W.units + u;
-    const bool update = i + 1 < nc || last;
-    const float4 mine_prm = prm[(long long)c * Q + n], end_prm = prm[(long long)c * Q + Q - 1];
-    const bool write = i > 0 || first;
-    if (kScaled && write) {
+    const bool update = i + 1 < nc || last, write = i > 0 || first;
+    if (write) {
       uint32_t m = 0;
 #pragma unroll
       for (int k = 0; k < 32; ++k) m = max(m, __float_as_uint(S[k]) & 0x7fffffffu);
       m = __reduce_max_sync(0xffffffffu, m);
       if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1) + 1], m);
     }
+    const float w = REV ? exp2f(lh + ll) : s * exp2f((eh - lh) + (el - ll)), decay = exp2f(eh + el), tback = back;
     cp_wait<0>();
     __syncthreads();
-    float wscale = 1.f, sscale = 1.f;
-    if (update || REV || kScaled) {
-      float w;
-      if (REV) w = exp2f(mine_prm.y + mine_prm.z);
-      else w = mine_prm.x * exp2f((end_prm.y - mine_prm.y) + (end_prm.z - mine_prm.z));
-      float v[4][8];
-      uint32_t m = 0;
+    float v[4][8];
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      unpack8<T>(lds16(base + kPassX + piece(n, half * 4 + j)), v[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        v[j][e] *= w;
+        m = max(m, __float_as_uint(v[j][e]) & 0x7fffffffu);
+      }
+    }
+    m = __reduce_max_sync(0xffffffffu, m);
+    if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1)], m);
+    __syncthreads();
+    if (i + 1 < nc) load(i + 1);                         // all have their tokens, and the other tile was used two chunks ago
+    const float2 wsc = scale_of(tops[2 * (i & 1)]), ssc = scale_of(tops[2 * (i & 1) + 1]);
+    if (update) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        unpack8<T>(lds16(base + kPassX + piece(n, half * 4 + j)), v[j]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[j][e] *= w;
-          if (kScaled) m = max(m, __float_as_uint(v[j][e]) & 0x7fffffffu);
-        }
-      }
-      float there = 1.f;
-      if (kScaled) {
-        m = __reduce_max_sync(0xffffffffu, m);
-        if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1)], m);
-        __syncthreads();
-        const float2 sc = scale_of(tops[2 * (i & 1)]);
-        there = sc.x;
-        wscale = sc.y;
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (kScaled)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[j][e] *= there;
+        for (int e = 0; e < 8; ++e) v[j][e] *= wsc.x;
         uint4 hi, lo;
-        split8<T>(v[j], hi, lo);
+        split8<__half>(v[j], hi, lo);
         sts16(base + kPassW + piece(n, half * 4 + j), hi);
         sts16(base + kPassW + kTile64 + piece(n, half * 4 + j), lo);
       }
+      fence_async();
     }
-    float sthere = 1.f;
-    if (kScaled && write) {
-      const float2 sc = scale_of(tops[2 * (i & 1) + 1]);
-      sthere = sc.x;
-      sscale = sc.y;
-    }
-    fence_async();
     __syncthreads();
-    if (kScaled && threadIdx.x < 2) tops[2 * (i & 1) + threadIdx.x] = 0;      // read by all, used again in two chunks
-    if (update && threadIdx.x == 0 && mm.ok) {
-      tc_fence_after();
-      mma<true, true>(tmem, base + (i & 1) * kTile128, base + kPassW, idesc<T>(TP, true, true), 8, false);
-      mma<true, true>(tmem, base + (i & 1) * kTile128, base + kPassW + kTile64, idesc<T>(TP, true, true), 8, true);
-      mm.commit();
+    if (threadIdx.x < 2) tops[2 * (i & 1) + threadIdx.x] = 0;                // read by all, used again in two chunks
+    if (update && threadIdx.x == 0) {
+      tile[i & 1].wait(ok, P.err);
+      if (ok) {
+        tc_fence_after();
+        mma<kMn, kMn>(tmem, base + (i & 1) * kTile128, base + kPassW, idesc<__half>(TP, true, true), 8, false);
+        mma<kMn, kMn>(tmem, base + (i & 1) * kTile128, base + kPassW + kTile64, idesc<__half>(TP, true, true), 8, true);
+        umma_commit(done.bar);
+      }
     }
-    if (i + 1 < nc) load(i + 1);
+    if (i + 1 < nc) load_record(i + 1);
     if (write) {
       uint16_t* out = planes + at * (2 * kN * TP);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = kScaled ? S[8 * j + e] * sthere : S[8 * j + e];
+        for (int e = 0; e < 8; ++e) f[e] = S[8 * j + e] * ssc.x;
         uint4 hi, lo;
-        split8<T>(f, hi, lo);
+        if (LO) split8<__half>(f, hi, lo);
+        else hi = pack8<__half>(f);
         *reinterpret_cast<uint4*>(out + ((half * 4 + j) * kN + n) * 8) = hi;
         if (LO) *reinterpret_cast<uint4*>(out + kN * TP + ((half * 4 + j) * kN + n) * 8) = lo;
       }
     }
-    if (threadIdx.x == 0) scales[at] = make_float2(sscale, wscale);
+    if (threadIdx.x == 0) scales[at] = make_float2(ssc.y, wsc.y);
     if (update) {
-      mm.wait();
+      done.wait(ok, P.err);
+      tc_fence_after();
       uint32_t r[32];
       tmem_ld32(mine, r);
       tc_fence_before();
-      const float decay = exp2f(end_prm.y + end_prm.z);
+      const float f = wsc.y * tback;
 #pragma unroll
-      for (int k = 0; k < 32; ++k) S[k] = S[k] * decay + __uint_as_float(r[k]) * wscale;
+      for (int k = 0; k < 32; ++k) S[k] = S[k] * decay + __uint_as_float(r[k]) * f;
     }
   }
   if (last)
 #pragma unroll
     for (int i = 0; i < 32; ++i)
       if (half * 32 + i < cols) last[state_at + (long long)(half * 32 + i) * kN] = S[i];
-  mma_end<64>(tmem);
+  tensor_end<64>(tmem);
 }
 
 // ---------------------------------------------------------------- outputs by chunk and group
 // One CTA: a chunk and some units of a group.  C B^T once (128 columns of TMEM), then a unit at a time: the pairs'
-// weights go to shared memory as the operand M, C H_in and M x to 64 columns each.
-constexpr uint32_t kOutM = kTile128, kOutX = 2 * kTile128, kOutH = kOutX + kTile64, kOutBytes = kOutH + kTile64;
-constexpr uint32_t kOutPrm = kOutBytes, kOutTop = kOutPrm + Q * 16, kOutBar = kOutTop + 2 * Q * 4, kOutSmem = kOutBar + 16;
+// weights go to shared memory as the operand M, C H_in and M x to 64 columns each.  What a unit needs of the next is
+// on its way as soon as its products are done.
+constexpr uint32_t kOutM = kTile128, kOutX = 2 * kTile128, kOutH = kOutX + kTile64, kOutRec = kOutH + kTile64, kRecBytes = 4 * Q * 4,
+                   kOutTop = kOutRec + 2 * kRecBytes, kOutBar = kOutTop + 2 * Q * 4, kOutSmem = kOutBar + 32;
+
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 words2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams P, const Space W, int per) {
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  float4* prm = reinterpret_cast<float4*>(smem + kOutPrm);
   float* tops = reinterpret_cast<float*>(smem + kOutTop);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kOutBar);              // tensor cores, tiles, units
   const int c = blockIdx.x, b = blockIdx.z;
   const int gunits = W.units / P.groups, g = blockIdx.y / W.splits;
   const int u0 = g * gunits + (blockIdx.y % W.splits) * per, u1 = min(u0 + per, (g + 1) * gunits);
@@ -531,37 +590,41 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     return;
   }
   const bool has_state = c > 0 || P.state_in;
-  const T* Cc = reinterpret_cast<const T*>(P.C) + (long long)b * P.c_sb + (long long)c * Q * P.c_st + g * kN;
-  const T* Bc = reinterpret_cast<const T*>(P.B) + (long long)b * P.b_sb + (long long)c * Q * P.b_st + g * kN;
+  const long long bc = (long long)b * W.nc + c, tile_at = bc * P.groups + g;
   const T* xc = reinterpret_cast<const T*>(P.x) + (long long)b * P.x_sb + (long long)c * Q * P.x_st;
-  auto load_state = [&](int u) {
-    if (has_state) load_plane(base + kOutH, W.h + (((long long)b * W.nc + c) * W.units + u) * (2 * kN * TP));
-  };
-  auto load_x = [&](int u) {
+  const uint32_t tmem = tensor_begin<256>(bars, 3, reinterpret_cast<uint32_t*>(smem + kOutBar + 24));
+  Gate done{smem_u32(bars), 0}, tiles{smem_u32(bars + 1), 0}, unit{smem_u32(bars + 2), 0};
+  bool ok = true;
+  auto load_unit = [&](int u) {                          // state and record (one thread), tokens (all)
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+    if (threadIdx.x == 0) {
+      mbar_expect_tx(unit.bar, kRecBytes + (has_state ? kTile64 : 0));
+      bulk_load(base + kOutRec + ((u - u0) & 1) * kRecBytes, W.rec + (((long long)b * P.heads + h) * W.nc + c) * (4 * Q), kRecBytes, unit.bar);
+      if (has_state) bulk_load(base + kOutH, W.h + (bc * W.units + u) * (2 * kN * TP), kTile64, unit.bar);
+    }
     const T* p = xc + (long long)h * P.dim + p0;
-    load_tile<T, 8>(base + kOutX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
-    const float4* s = W.prm + ((long long)b * P.heads + h) * W.lp + (long long)c * Q;
-    if (threadIdx.x < Q) cp16(base + kOutPrm + threadIdx.x * 16, s + threadIdx.x, true);
+    load_tile<T>(base + kOutX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
+    cp_commit();
   };
-  load_tile<T, 16>(base, Cc, P.c_st, rows, kN, vector_ok(Cc, P.c_st, 0, kN));
-  load_tile<T, 16>(base + kOutM, Bc, P.b_st, rows, kN, vector_ok(Bc, P.b_st, 0, kN));
-  cp_commit();
-  load_state(u0);
-  load_x(u0);
-  cp_commit();
-  uint32_t tmem;
-  Mma mm = mma_begin<256>(reinterpret_cast<uint64_t*>(smem + kOutBar), reinterpret_cast<uint32_t*>(smem + kOutBar + 8), P.err, tmem);
-  const uint32_t lanes = tmem + ((uint32_t)quad << 21);
-  cp_wait<1>();
-  fence_async();
-  __syncthreads();
   if (threadIdx.x == 0) {
-    tc_fence_after();
-    mma<false, false>(tmem, base, base + kOutM, idesc<T>(Q, false, false), 8, false);
-    mm.commit();
+    mbar_expect_tx(tiles.bar, 2 * kTile128);
+    bulk_load(base, W.ct + tile_at * (Q * kN), kTile128, tiles.bar);
+    bulk_load(base + kOutM, W.bt + tile_at * (Q * kN), kTile128, tiles.bar);
   }
-  mm.wait();
+  load_unit(u0);
+  const float cback = W.cback[tile_at], both_back = cback * W.bback[tile_at];
+  const uint32_t lanes = tmem + ((uint32_t)quad << 21);
+  if (threadIdx.x == 0) {
+    tiles.wait(ok, P.err);
+    tc_fence_after();
+    if (ok) {
+      mma<kK, kK>(tmem, base, base + kOutM, idesc<__half>(Q, false, false), 8, false);
+      umma_commit(done.bar);
+    }
+  }
+  done.wait(ok, P.err);
+  tc_fence_after();
+  float top = 0.f;
   if (kScaled) {                                         // the largest |C_t . B_s| of my row's pairs
     uint32_t m = 0;
     for (int cb = half; cb <= quad; cb += 2) {
@@ -572,22 +635,28 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
         if (cb * 32 + i <= row) m = max(m, r[i] & 0x7fffffffu);
     }
     tops[half * Q + row] = __uint_as_float(m);
+    __syncthreads();
+    top = fmaxf(tops[row], tops[Q + row]);
   }
   for (int cb = half; cb < 4; cb += 2)                   // pairs above the diagonal weigh nothing, for every unit
     if (cb > quad)
       for (int k = 0; k < 4; ++k) sts16(base + kOutM + piece2(row, cb * 4 + k), make_uint4(0, 0, 0, 0));
-  cp_wait<0>();
-  fence_async();
-  __syncthreads();
-  const float top = kScaled ? fmaxf(tops[row], tops[Q + row]) : 0.f;
 
   for (int u = u0; u < u1; ++u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
-    if (threadIdx.x == 0 && has_state && mm.ok) {
+    const float* rec = reinterpret_cast<const float*>(smem + kOutRec + ((u - u0) & 1) * kRecBytes);
+    cp_wait<0>();
+    fence_async();
+    unit.wait(ok, P.err);
+    __syncthreads();
+    if (threadIdx.x == 0 && has_state && ok) {
       tc_fence_after();
-      mma<false, true>(tmem + 128, base, base + kOutH, idesc<T>(TP, false, true), 8, false);
+      mma<kK, kPlaneP>(tmem + 128, base, base + kOutH, idesc<__half>(TP, false, true), 8, false);
     }
-    const float4 me = prm[row];
+    const float lh = rec[Q + row], ll = rec[2 * Q + row];
+    uint4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = lds16(base + kOutX + piece(row, half * 4 + j));
     float2 sc = make_float2(1.f, 1.f);
     if (kScaled) sc = scale_of(__float_as_uint(top * W.smax[((long long)b * P.heads + h) * W.nc + c]) & 0x7fffffffu);
     for (int cb = half; cb <= quad; cb += 2) {
@@ -597,64 +666,65 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
       for (int k = 0; k < 4; ++k) {
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int s = cb * 32 + k * 8 + e;
-          const float4 to = prm[s];
-          const float w = ex2((me.y - to.y) + (me.z - to.z)) * to.x;
-          f[e] = __uint_as_float(r[k * 8 + e]) * (kScaled ? w * sc.x : w);
-          if (s > row) f[e] = 0.f;
+        for (int e = 0; e < 8; e += 4) {
+          const int at = cb * 8 + k * 2 + (e >> 2);
+          const float4 s4 = reinterpret_cast<const float4*>(rec)[at], h4 = reinterpret_cast<const float4*>(rec + Q)[at],
+                       l4 = reinterpret_cast<const float4*>(rec + 2 * Q)[at];
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float2 sv = i ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y), hv = i ? make_float2(h4.z, h4.w) : make_float2(h4.x, h4.y),
+                         lv = i ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+            const float2 gap = __fadd2_rn(__ffma2_rn(hv, pair(-1.f), pair(lh)), __ffma2_rn(lv, pair(-1.f), pair(ll)));
+            float2 v = __fmul2_rn(__fmul2_rn(make_float2(ex2(gap.x), ex2(gap.y)), sv), words2(r[k * 8 + e + i], r[k * 8 + e + i + 1]));
+            if (kScaled) v = __fmul2_rn(v, pair(sc.x));
+            f[e + i] = v.x;
+            f[e + i + 1] = v.y;
+          }
         }
+        if (cb == quad)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (cb * 32 + k * 8 + e > row) f[e] = 0.f;
         sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<T>(f));
       }
     }
+    if (quad == 0 && half == 1)                          // where the output of the unit before was laid out
+      for (int k = 0; k < 4; ++k) sts16(base + kOutM + piece2(row, 4 + k), make_uint4(0, 0, 0, 0));
     tc_fence_before();
     fence_async();
     __syncthreads();
-    if (threadIdx.x == 0 && mm.ok) {
+    if (threadIdx.x == 0 && ok) {
       tc_fence_after();
-      mma<false, true>(tmem + 192, base + kOutM, base + kOutX, idesc<T>(TP, false, true), 8, false);
-      mm.commit();
+      mma<kK, kMn>(tmem + 192, base + kOutM, base + kOutX, idesc<T>(TP, false, true), 8, false);
+      umma_commit(done.bar);
     }
     const float d = number(P.D, P.d_type, h);
-    float carry = 0.f;
-    if (has_state) {
-      carry = ex2(me.y + me.z);
-      if (kScaled) carry *= W.hs[((long long)b * W.nc + c) * W.units + u].x;
-    }
-    mm.wait();
-    if (u + 1 < u1) load_state(u + 1);
+    const float carry = has_state ? ex2(lh + ll) * W.hs[bc * W.units + u].x * cback : 0.f, mixed = sc.y * both_back;
+    done.wait(ok, P.err);
+    tc_fence_after();
+    if (u + 1 < u1) load_unit(u + 1);
     uint32_t y0[32], y1[32];
     if (has_state) tmem_ld32_nowait(lanes + 128 + half * 32, y0);
     tmem_ld32(lanes + 192 + half * 32, y1);
     if (has_state) settle(y0);
+    tc_fence_before();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t at = base + kOutX + piece(row, half * 4 + j);
       float f[8];
-      unpack8<T>(lds16(at), f);
+      unpack8<T>(x[j], f);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float v = __uint_as_float(y1[j * 8 + e]);
-        v = (kScaled ? v * sc.y : v) + d * f[e];
+        float v = __uint_as_float(y1[j * 8 + e]) * mixed + d * f[e];
         if (has_state) v += carry * __uint_as_float(y0[j * 8 + e]);
         f[e] = row < rows ? v : 0.f;
       }
-      sts16(at, pack8<T>(f));
+      sts16(base + kOutM + piece(row, half * 4 + j), pack8<T>(f));
     }
-    tc_fence_before();
     __syncthreads();
     T* out = y + (long long)h * P.dim + p0;
-    store_tile<T>(out, P.y_st, base + kOutX, out_rows, cols, vector_ok(out, P.y_st, 0, cols));
-    if (u + 1 < u1) {
-      __syncthreads();
-      load_x(u + 1);
-      cp_commit();
-      cp_wait<0>();
-      fence_async();
-      __syncthreads();
-    }
+    store_tile<T>(out, P.y_st, base + kOutM, out_rows, cols, vector_ok(out, P.y_st, 0, cols));
   }
-  mma_end<256>(tmem);
+  tensor_end<256>(tmem);
 }
 
 // ---------------------------------------------------------------- gradients by chunk and group
@@ -668,9 +738,9 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
 //      by row and by column.
 //   3. the pairs' part of x's gradient; prefix and suffix sums over the tokens give the gradient of A s.
 // After the last unit the group's sum gives the pairs' part of dB and dC in two products.
-constexpr uint32_t kGB = 0, kGC = kTile128, kGX = 2 * kTile128, kGY = kGX + kTile64, kGH = kGY + kTile64, kGG = kGH + 2 * kTile64,
-                   kGM = kGG + 2 * kTile64, kGPrm = kGM + kTile128, kGRow = kGPrm + Q * 16, kGCol = kGRow + 7 * Q * 4,
-                   kGRed = kGCol + 4 * Q * 4, kGBar = kGRed + 32 * 4, kGradSmem = kGBar + 16;
+constexpr uint32_t kGB = 0, kGC = kTile128, kGX = 2 * kTile128, kGY = kGX + kTile64, kGHigh = kGY + 2 * kTile64,
+                   kGLow = kGHigh + 2 * kTile64, kGM = kGLow + 2 * kTile64, kGRec = kGM + kTile128, kGRow = kGRec + 2 * kRecBytes,
+                   kGCol = kGRow + 7 * Q * 4, kGRed = kGCol + 4 * Q * 4, kGBar = kGRed + 32 * 4, kGradSmem = kGBar + 48;
 
 // Sums over a warp's lanes of e[column], for column = lane.
 __device__ __forceinline__ float column_sums(float (&e)[32], int lane) {
@@ -691,17 +761,17 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  const float4* prm = reinterpret_cast<const float4*>(smem + kGPrm);
   float* rpairs = reinterpret_cast<float*>(smem + kGRow);        // [2][Q] each: r by pairs, r by states, q by states; [Q]: r by the token itself
   float *rstate = rpairs + 2 * Q, *qstate = rpairs + 4 * Q, *rself = rpairs + 6 * Q;
   float* qpairs = reinterpret_cast<float*>(smem + kGCol);        // [4][Q]
   float* red = reinterpret_cast<float*>(smem + kGRed);           // [0..8) <G, H>, [8..16) x . dy, [16..24) pairs' time, [24..32) maxima
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kGBar);    // tensor cores, tiles, values, remainders
   const int c = blockIdx.x, b = blockIdx.z;
   const int gunits = W.units / P.groups, g = blockIdx.y / W.splits, split = blockIdx.y % W.splits;
   const int u0 = g * gunits + split * per, u1 = min(u0 + per, (g + 1) * gunits);
   const int len = tokens_of(P, b), rows = min(Q, len - c * Q), out_rows = min(Q, P.length - c * Q);
   const int row = threadIdx.x & 127, half = threadIdx.x >> 7, warp = threadIdx.x >> 5, quad = warp & 3, lane = threadIdx.x & 31;
-  const long long bc = (long long)b * W.nc + c, dx_st = P.dx_st, grp_st = P.dg_st;
+  const long long bc = (long long)b * W.nc + c, dx_st = P.dx_st, grp_st = P.dg_st, tile_at = bc * P.groups + g;
   T* dx = reinterpret_cast<T*>(P.dx) + b * P.dx_sb + (long long)c * Q * dx_st;
   const long long grp_at = b * P.dg_sb + (long long)c * Q * grp_st + g * kN;
   T *dB = reinterpret_cast<T*>(P.dB) + grp_at, *dC = reinterpret_cast<T*>(P.dC) + grp_at;
@@ -718,53 +788,68 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     return;
   }
   const bool has_h = c > 0 || P.state_in, has_g = (c + 1) * Q < len || P.dstate_out;
-  const T* Bc = reinterpret_cast<const T*>(P.B) + (long long)b * P.b_sb + (long long)c * Q * P.b_st + g * kN;
-  const T* Cc = reinterpret_cast<const T*>(P.C) + (long long)b * P.c_sb + (long long)c * Q * P.c_st + g * kN;
   const T* xc = reinterpret_cast<const T*>(P.x) + (long long)b * P.x_sb + (long long)c * Q * P.x_st;
   const T* yc = reinterpret_cast<const T*>(P.dy) + (long long)b * P.dy_sb + (long long)c * Q * P.dy_st;
-  auto load_states = [&](int u) {
+  const uint32_t tmem = tensor_begin<512>(bars, 4, reinterpret_cast<uint32_t*>(smem + kGBar + 32));
+  const uint32_t lanes = tmem + ((uint32_t)quad << 21), work = tmem + 128, sum_c = tmem + 256, sum_b = tmem + 384;
+  Gate done{smem_u32(bars), 0}, tiles{smem_u32(bars + 1), 0}, high{smem_u32(bars + 2), 0}, low{smem_u32(bars + 3), 0};
+  bool ok = true;
+  // One thread: the record and the states' values of a unit, and their remainders.  H lies at 0, G 16,384 bytes on.
+  auto load_high = [&](int u) {
     const long long at = (bc * W.units + u) * (2 * kN * TP);
-    if (has_h) { load_plane(base + kGH, W.h + at); load_plane(base + kGH + kTile64, W.h + at + kN * TP); }
-    if (has_g) { load_plane(base + kGG, W.g + at); load_plane(base + kGG + kTile64, W.g + at + kN * TP); }
+    mbar_expect_tx(high.bar, kRecBytes + ((int)has_h + (int)has_g) * kTile64);
+    bulk_load(base + kGRec + ((u - u0) & 1) * kRecBytes, W.rec + (((long long)b * P.heads + u / W.ptiles) * W.nc + c) * (4 * Q), kRecBytes, high.bar);
+    if (has_h) bulk_load(base + kGHigh, W.h + at, kTile64, high.bar);
+    if (has_g) bulk_load(base + kGHigh + kTile64, W.g + at, kTile64, high.bar);
   };
-  auto load_tokens = [&](int u) {
+  auto load_low = [&](int u) {
+    if (!has_h && !has_g) return;
+    const long long at = (bc * W.units + u) * (2 * kN * TP) + kN * TP;
+    mbar_expect_tx(low.bar, ((int)has_h + (int)has_g) * kTile64);
+    if (has_h) bulk_load(base + kGLow, W.h + at, kTile64, low.bar);
+    if (has_g) bulk_load(base + kGLow + kTile64, W.g + at, kTile64, low.bar);
+  };
+  auto load_x = [&](int u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
-    const T *px = xc + (long long)h * P.dim + p0, *py = yc + (long long)h * P.dim + p0;
-    load_tile<T, 8>(base + kGX, px, P.x_st, rows, cols, vector_ok(px, P.x_st, 0, cols));
-    load_tile<T, 8>(base + kGY, py, P.dy_st, rows, cols, vector_ok(py, P.dy_st, 0, cols));
-    const float4* s = W.prm + ((long long)b * P.heads + h) * W.lp + (long long)c * Q;
-    if (threadIdx.x < Q) cp16(base + kGPrm + threadIdx.x * 16, s + threadIdx.x, true);
+    const T* p = xc + (long long)h * P.dim + p0;
+    load_tile<T>(base + kGX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
   };
-  load_tile<T, 16>(base + kGB, Bc, P.b_st, rows, kN, vector_ok(Bc, P.b_st, 0, kN));
-  load_tile<T, 16>(base + kGC, Cc, P.c_st, rows, kN, vector_ok(Cc, P.c_st, 0, kN));
-  cp_commit();
-  load_states(u0);
-  load_tokens(u0);
+  auto load_y = [&](int u) {
+    const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+    const T* p = yc + (long long)h * P.dim + p0;
+    load_tile<T>(base + kGY + ((u - u0) & 1) * kTile64, p, P.dy_st, rows, cols, vector_ok(p, P.dy_st, 0, cols));
+  };
+  if (threadIdx.x == 0) {
+    mbar_expect_tx(tiles.bar, 2 * kTile128);
+    bulk_load(base + kGB, W.bt + tile_at * (Q * kN), kTile128, tiles.bar);
+    bulk_load(base + kGC, W.ct + tile_at * (Q * kN), kTile128, tiles.bar);
+    load_high(u0);
+    load_low(u0);
+  }
+  load_x(u0);
+  load_y(u0);
   cp_commit();
   // units' sums for C and B share a scale: that of the largest product of a state's and its tokens' scales
-  float cscale = 1.f, bscale = 1.f;
-  if (kScaled && (has_h || has_g)) {
-    cscale = bscale = 0.f;
+  float cscale = 0.f, bscale = 0.f;
+  if (has_h || has_g)
     for (int u = u0; u < u1; ++u) {
       const float2 hs = W.hs[bc * W.units + u], gs = W.gs[bc * W.units + u];
       cscale = fmaxf(cscale, hs.x * gs.y);
       bscale = fmaxf(bscale, gs.x * hs.y);
     }
-  }
-  uint32_t tmem;
-  Mma mm = mma_begin<512>(reinterpret_cast<uint64_t*>(smem + kGBar), reinterpret_cast<uint32_t*>(smem + kGBar + 8), P.err, tmem);
-  const uint32_t lanes = tmem + ((uint32_t)quad << 21), work = tmem + 128, sum_c = tmem + 256, sum_b = tmem + 384;
-  cp_wait<1>();
-  fence_async();
-  __syncthreads();
+  const float bback = W.bback[tile_at], cback = W.cback[tile_at], both_back = bback * cback;
   if (threadIdx.x == 0) {
+    tiles.wait(ok, P.err);
     tc_fence_after();
-    mma<false, false>(tmem, base + kGB, base + kGC, idesc<T>(Q, false, false), 8, false);
-    mm.commit();
+    if (ok) {
+      mma<kK, kK>(tmem, base + kGB, base + kGC, idesc<__half>(Q, false, false), 8, false);
+      umma_commit(done.bar);
+    }
   }
-  mm.wait();
-  float top = 0.f;
-  if (kScaled) {                                         // the largest |B_s . C_t| of my row's pairs
+  done.wait(ok, P.err);
+  tc_fence_after();
+  float2 sc = make_float2(1.f, 1.f);
+  if (kScaled) {                                         // by the largest |B_s . C_t| of my row's pairs
     uint32_t m = 0;
     for (int cb = half; cb < 4; cb += 2) {
       if (cb < quad) continue;
@@ -776,59 +861,62 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     }
     rpairs[half * Q + row] = __uint_as_float(m);
     __syncthreads();
-    top = fmaxf(rpairs[row], rpairs[Q + row]);
+    sc = scale_of(__float_as_uint(fmaxf(rpairs[row], rpairs[Q + row])));
   }
-  const float2 sc = kScaled ? scale_of(__float_as_uint(top)) : make_float2(1.f, 1.f);
-  float ds[2][32];
+  float2 ds[2][16];
 #pragma unroll
-  for (int i = 0; i < 64; ++i) ds[i >> 5][i & 31] = 0.f;
-  cp_wait<0>();
-  fence_async();
-  __syncthreads();
+  for (int i = 0; i < 32; ++i) ds[i >> 4][i & 15] = make_float2(0.f, 0.f);
 
   for (int u = u0; u < u1; ++u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
+    const float* rec = reinterpret_cast<const float*>(smem + kGRec + ((u - u0) & 1) * kRecBytes);
+    const uint32_t ytile = base + kGY + ((u - u0) & 1) * kTile64;
+    cp_wait<0>();
+    fence_async();
+    high.wait(ok, P.err);
+    if (has_h || has_g) low.wait(ok, P.err);
+    __syncthreads();
     // step 1
-    if (threadIdx.x == 0 && (has_h || has_g) && mm.ok) {
+    if (threadIdx.x == 0 && (has_h || has_g) && ok) {
       tc_fence_after();
       if (has_g) {
-        mma<false, true>(work, base + kGB, base + kGG, idesc<T>(TP, false, true), 8, false);
-        mma<false, true>(work, base + kGB, base + kGG + kTile64, idesc<T>(TP, false, true), 8, true);
+        mma<kK, kPlaneP>(work, base + kGB, base + kGHigh + kTile64, idesc<__half>(TP, false, true), 8, false);
+        mma<kK, kPlaneP>(work, base + kGB, base + kGLow + kTile64, idesc<__half>(TP, false, true), 8, true);
       }
       if (has_h) {
-        mma<false, true>(work + 64, base + kGC, base + kGH, idesc<T>(TP, false, true), 8, false);
-        mma<false, true>(work + 64, base + kGC, base + kGH + kTile64, idesc<T>(TP, false, true), 8, true);
+        mma<kK, kPlaneP>(work + 64, base + kGC, base + kGHigh, idesc<__half>(TP, false, true), 8, false);
+        mma<kK, kPlaneP>(work + 64, base + kGC, base + kGLow, idesc<__half>(TP, false, true), 8, true);
       }
-      mm.commit();
+      umma_commit(done.bar);
     }
-    const float4 me = prm[row], end = prm[Q - 1];
+    const float s = rec[row], lh = rec[Q + row], ll = rec[2 * Q + row], eh = rec[2 * Q - 1], el = rec[3 * Q - 1];
     float2 hs = make_float2(1.f, 1.f), gs = make_float2(1.f, 1.f);
-    if (kScaled && (has_h || has_g)) { hs = W.hs[bc * W.units + u]; gs = W.gs[bc * W.units + u]; }
-    const float from_in = ex2(me.y + me.z), to_end = ex2((end.y - me.y) + (end.z - me.z));
-    const float wy = kScaled ? from_in * (hs.x / cscale) : from_in, wx = me.x * (kScaled ? to_end * (gs.x / bscale) : to_end);
+    if (has_h || has_g) { hs = W.hs[bc * W.units + u]; gs = W.gs[bc * W.units + u]; }
+    const float from_in = ex2(lh + ll), to_end = ex2((eh - lh) + (el - ll));
+    const float wy = has_h ? from_in * (hs.x / cscale) : 0.f, wx = has_g ? s * to_end * (gs.x / bscale) : 0.f;
     float gh = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t at = piece(row, half * 4 + j);
+      const uint32_t at = piece(row, half * 4 + j), plane = (uint32_t)((half * 4 + j) * kN + row) * 16;
       float f[8], o[8];
       if (has_h) {
-        unpack8<T>(lds16(base + kGY + at), f);
+        unpack8<T>(lds16(ytile + at), f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] *= wy;
-        sts16(base + kGM + at, pack8<T>(f));
+        sts16(base + kGM + at, pack8<__half>(f));
       }
       if (has_g) {
         unpack8<T>(lds16(base + kGX + at), f);
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] *= wx;
-        sts16(base + kGM + kTile64 + at, pack8<T>(f));
+        sts16(base + kGM + kTile64 + at, pack8<__half>(f));
       }
       if (has_h && has_g) {                              // my row of the states: <G, H>
         float hl[8], gl[8];
-        unpack8<T>(lds16(base + kGH + at), f);
-        unpack8<T>(lds16(base + kGH + kTile64 + at), hl);
-        unpack8<T>(lds16(base + kGG + at), o);
-        unpack8<T>(lds16(base + kGG + kTile64 + at), gl);
+        unpack8<__half>(lds16(base + kGHigh + plane), f);
+        unpack8<__half>(lds16(base + kGLow + plane), hl);
+        unpack8<__half>(lds16(base + kGHigh + kTile64 + plane), o);
+        unpack8<__half>(lds16(base + kGLow + kTile64 + plane), gl);
 #pragma unroll
         for (int e = 0; e < 8; ++e) gh += (f[e] + hl[e]) * (o[e] + gl[e]);
       }
@@ -837,13 +925,14 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     if (lane == 0) red[warp] = gh;
     fence_async();
     float dxi[32];
+    float r_part = 0.f, q_part = 0.f;
     if (has_h || has_g) {
-      mm.wait();
+      done.wait(ok, P.err);
+      tc_fence_after();
       uint32_t r[32];
-      float r_part = 0.f, q_part = 0.f;
       if (has_g) {
         tmem_ld32(lanes + 128 + half * 32, r);
-        const float f = to_end * gs.x;
+        const float f = to_end * gs.x * bback;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float x[8];
@@ -857,78 +946,100 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
       }
       if (has_h) {
         tmem_ld32(lanes + 192 + half * 32, r);
-        const float f = from_in * hs.x;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float y[8];
-          unpack8<T>(lds16(base + kGY + piece(row, half * 4 + j)), y);
+          unpack8<T>(lds16(ytile + piece(row, half * 4 + j)), y);
 #pragma unroll
           for (int e = 0; e < 8; ++e) q_part += __uint_as_float(r[j * 8 + e]) * y[e];
         }
-        q_part *= f;
+        q_part *= from_in * hs.x * cback;
       }
-      rstate[half * Q + row] = r_part;
-      qstate[half * Q + row] = q_part;
       tc_fence_before();
-    } else {
-      rstate[half * Q + row] = qstate[half * Q + row] = 0.f;
     }
+    rstate[half * Q + row] = r_part;
+    qstate[half * Q + row] = q_part;
     if (!has_g)
 #pragma unroll
       for (int i = 0; i < 32; ++i) dxi[i] = 0.f;
     __syncthreads();
     // step 2
-    if (threadIdx.x == 0 && mm.ok) {
-      tc_fence_after();
-      mma<false, false>(work, base + kGX, base + kGY, idesc<T>(Q, false, false), 4, false);
-      if (has_h) mma<false, false>(sum_c, base + kGM, base + kGH, idesc<T>(kN, false, false), 4, u > u0);
-      if (has_g) mma<false, false>(sum_b, base + kGM + kTile64, base + kGG, idesc<T>(kN, false, false), 4, u > u0);
-      mm.commit();
+    if (threadIdx.x == 0) {
+      if (u + 1 < u1) load_low(u + 1);
+      if (ok) {
+        tc_fence_after();
+        mma<kK, kK>(work, base + kGX, ytile, idesc<T>(Q, false, false), 4, false);
+        if (has_h) mma<kK, kPlaneN>(sum_c, base + kGM, base + kGHigh, idesc<__half>(kN, false, false), 4, u > u0);
+        if (has_g) mma<kK, kPlaneN>(sum_b, base + kGM + kTile64, base + kGHigh + kTile64, idesc<__half>(kN, false, false), 4, u > u0);
+        umma_commit(done.bar);
+      }
     }
-    mm.wait();
+    if (u + 1 < u1) { load_y(u + 1); cp_commit(); }
+    done.wait(ok, P.err);
+    tc_fence_after();
+    if (u + 1 < u1) {
+      if (threadIdx.x == 0) load_high(u + 1);
+      load_x(u + 1);
+      cp_commit();
+    }
     float r_sum = 0.f, diag = 0.f, pair_time = 0.f;
+    const float sb = s * both_back;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int cb = half + 2 * k;
       if (cb >= quad) {
         uint32_t r[32], d[32];
-        float e[32];
         tmem_ld32_nowait(lanes + cb * 32, r);
         tmem_ld32(lanes + 128 + cb * 32, d);
         settle(r);
+        float e[32];
+        float2 rs2 = make_float2(0.f, 0.f), time2 = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           float f[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int t = cb * 32 + j * 8 + i;
-            const float4 to = prm[t];
-            const float gap = (to.y - me.y) + (to.z - me.z);
-            float w = ex2(gap);
-            if (t < row) w = 0.f;
-            const float m = __uint_as_float(r[j * 8 + i]) * w, dm = __uint_as_float(d[j * 8 + i]);
-            f[i] = kScaled ? m * sc.x : m;
-            ds[k][j * 8 + i] += me.x * (dm * w);
-            float both = m * dm;
-            if (t == row) {                              // no decay between a token and itself: kept out of the sums
-              diag = dm;
-              rself[row] = both;
-              both = 0.f;
+          for (int i = 0; i < 8; i += 4) {
+            const int at = cb * 8 + j * 2 + (i >> 2);
+            const float4 h4 = reinterpret_cast<const float4*>(rec + Q)[at], l4 = reinterpret_cast<const float4*>(rec + 2 * Q)[at];
+#pragma unroll
+            for (int o = 0; o < 4; o += 2) {
+              const int q = j * 8 + i + o;
+              const float2 hv = o ? make_float2(h4.z, h4.w) : make_float2(h4.x, h4.y), lv = o ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+              float2 gap = __fadd2_rn(__ffma2_rn(pair(lh), pair(-1.f), hv), __ffma2_rn(pair(ll), pair(-1.f), lv));
+              float2 w = make_float2(ex2(gap.x), ex2(gap.y));
+              if (cb == quad) {                          // pairs under the diagonal weigh nothing
+                const int t = cb * 32 + q;
+                if (t < row) { w.x = 0.f; gap.x = 0.f; }
+                if (t + 1 < row) { w.y = 0.f; gap.y = 0.f; }
+              }
+              const float2 dm = words2(d[q], d[q + 1]), m = __fmul2_rn(words2(r[q], r[q + 1]), w);
+              ds[k][q >> 1] = __ffma2_rn(pair(s), __fmul2_rn(dm, w), ds[k][q >> 1]);
+              float2 both = __fmul2_rn(m, dm);
+              if (cb == quad) {                          // no decay between a token and itself: kept out of the sums
+                const int t = cb * 32 + q;
+                if (t == row) { diag = dm.x; rself[row] = both.x * both_back; both.x = 0.f; }
+                if (t + 1 == row) { diag = dm.y; rself[row] = both.y * both_back; both.y = 0.f; }
+              }
+              rs2 = __fadd2_rn(rs2, both);
+              both = __fmul2_rn(both, pair(sb));
+              time2 = __ffma2_rn(both, gap, time2);
+              e[q] = both.x;
+              e[q + 1] = both.y;
+              f[i + o] = kScaled ? m.x * sc.x : m.x;
+              f[i + o + 1] = kScaled ? m.y * sc.x : m.y;
             }
-            r_sum += both;
-            both *= me.x;
-            e[j * 8 + i] = both;
-            if (t > row) pair_time += both * gap;
           }
           sts16(base + kGM + piece2(row, cb * 4 + j), pack8<T>(f));
         }
+        r_sum += rs2.x + rs2.y;
+        pair_time += time2.x + time2.y;
         qpairs[quad * Q + cb * 32 + lane] = column_sums(e, lane);
       } else {
         for (int j = 0; j < 4; ++j) sts16(base + kGM + piece2(row, cb * 4 + j), make_uint4(0, 0, 0, 0));
         qpairs[quad * Q + cb * 32 + lane] = 0.f;
       }
     }
-    rpairs[half * Q + row] = r_sum;
+    rpairs[half * Q + row] = r_sum * both_back;
     diag = warp_sum(diag);
     pair_time = warp_sum(pair_time);
     if (lane == 0) { red[8 + warp] = diag; red[16 + warp] = pair_time; }
@@ -936,38 +1047,36 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     fence_async();
     __syncthreads();
     // step 3
-    if (threadIdx.x == 0 && mm.ok) {
+    if (threadIdx.x == 0 && ok) {
       tc_fence_after();
-      mma<false, true>(work, base + kGM, base + kGY, idesc<T>(TP, false, true), 8, false);
-      mm.commit();
+      mma<kK, kMn>(work, base + kGM, ytile, idesc<T>(TP, false, true), 8, false);
+      umma_commit(done.bar);
     }
-    if (u + 1 < u1) load_states(u + 1);
     if (warp == 7) {                                     // four tokens a lane
-      float a[4], r[4], sa = 0.f, sb = 0.f, bs[4], time = 0.f;
+      float a[4], r[4], sa = 0.f, sum = 0.f, bs[4], time = 0.f;
       float through = 0.f, dd = 0.f, da = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) { through += red[i]; dd += red[8 + i]; da += red[16 + i]; }
-      through *= ex2(end.y + end.z) * (hs.x * gs.x);
+      through *= ex2(eh + el) * (hs.x * gs.x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int t = 4 * lane + i;
-        const float s = prm[t].x, rp = rpairs[t] + rpairs[Q + t], rs = rstate[t] + rstate[Q + t];
-        const float qs = qstate[t] + qstate[Q + t];
+        const float st = rec[t], rp = rpairs[t] + rpairs[Q + t], rs = rstate[t] + rstate[Q + t], qs = qstate[t] + qstate[Q + t];
         r[i] = rp + rs + rself[t];
-        a[i] = ((qpairs[t] + qpairs[Q + t]) + (qpairs[2 * Q + t] + qpairs[3 * Q + t])) + qs - s * rp;
-        bs[i] = s * rs;
-        time += qs * (prm[t].y + prm[t].z) + bs[i] * ((end.y - prm[t].y) + (end.z - prm[t].z));
+        a[i] = ((qpairs[t] + qpairs[Q + t]) + (qpairs[2 * Q + t] + qpairs[3 * Q + t])) + qs - st * rp;
+        bs[i] = st * rs;
+        time += qs * (rec[Q + t] + rec[2 * Q + t]) + bs[i] * ((eh - rec[Q + t]) + (el - rec[2 * Q + t]));
         sa += a[i];
-        sb += bs[i];
+        sum += bs[i];
       }
-      float after = sa, before = sb;                     // sums over the lanes from mine on, and up to mine
+      float after = sa, before = sum;                    // sums over the lanes from mine on, and up to mine
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const float va = __shfl_down_sync(0xffffffffu, after, o), vb = __shfl_up_sync(0xffffffffu, before, o);
         if (lane + o < 32) after += va;
         if (lane >= o) before += vb;
       }
-      before -= sb;
+      before -= sum;
       after -= sa;
       float from[4];                                     // sum of a over t' >= t
 #pragma unroll
@@ -981,79 +1090,74 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
       time = warp_sum(time);
       // A's gradient: each contribution by the time that A works on it, which l tells; no differences of large sums
       if (lane == 0) {
-        da = (da + time) + through * (end.y + end.z);
+        da = (da + time) + through * (eh + el);
         W.unit_sums[bc * W.units + u] = make_float2(dd, (float)((double)da / decay_rate(P.A[h])));
       }
     }
-    const float dskip = number(P.D, P.d_type, h);
-    mm.wait();
+    const float dskip = number(P.D, P.d_type, h), mixed = sc.y * both_back;
+    done.wait(ok, P.err);
+    tc_fence_after();
     {
       uint32_t r[32];
       tmem_ld32(lanes + 128 + half * 32, r);
+      tc_fence_before();
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint32_t at = piece(row, half * 4 + j);
         float f[8];
-        unpack8<T>(lds16(base + kGY + at), f);
+        unpack8<T>(lds16(ytile + at), f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float v = __uint_as_float(r[j * 8 + e]);
-          f[e] = row < rows ? me.x * ((kScaled ? v * sc.y : v) + dxi[j * 8 + e]) + dskip * f[e] : 0.f;
-        }
-        sts16(base + kGX + at, pack8<T>(f));
+        for (int e = 0; e < 8; ++e)
+          f[e] = row < rows ? s * (__uint_as_float(r[j * 8 + e]) * mixed + dxi[j * 8 + e]) + dskip * f[e] : 0.f;
+        sts16(base + kGM + at, pack8<T>(f));
       }
     }
-    tc_fence_before();
     __syncthreads();
     T* out = dx + (long long)h * P.dim + p0;
-    store_tile<T>(out, dx_st, base + kGX, out_rows, cols, vector_ok(out, dx_st, 0, cols));
-    __syncthreads();
-    if (u + 1 < u1) {
-      load_tokens(u + 1);
-      cp_commit();
-      cp_wait<0>();
-      fence_async();
-      __syncthreads();
-    }
+    store_tile<T>(out, dx_st, base + kGM, out_rows, cols, vector_ok(out, dx_st, 0, cols));
   }
+  __syncthreads();
 
   // the pairs' part of dB and dC
-  float2 all = make_float2(1.f, 1.f);
-  if (kScaled) {
-    uint32_t m = 0;
+  uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 64; ++i) m = max(m, __float_as_uint(ds[i >> 5][i & 31]) & 0x7fffffffu);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) red[24 + warp] = __uint_as_float(m);
-    __syncthreads();
-    m = 0;
+  for (int i = 0; i < 32; ++i)
+    top = max(top, max(__float_as_uint(ds[i >> 4][i & 15].x) & 0x7fffffffu, __float_as_uint(ds[i >> 4][i & 15].y) & 0x7fffffffu));
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) red[24 + warp] = __uint_as_float(top);
+  __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(red[24 + i]));
-    all = scale_of(m);
-  }
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(red[24 + i]));
+  const float2 all = scale_of(top);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       float f[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = kScaled ? ds[k][j * 8 + i] * all.x : ds[k][j * 8 + i];
-      sts16(base + kGM + piece2(row, (half + 2 * k) * 4 + j), pack8<T>(f));
+      for (int i = 0; i < 8; i += 2) {
+        const float2 v = __fmul2_rn(ds[k][j * 4 + (i >> 1)], pair(all.x));
+        f[i] = v.x;
+        f[i + 1] = v.y;
+      }
+      sts16(base + kGM + piece2(row, (half + 2 * k) * 4 + j), pack8<__half>(f));
     }
+  tc_fence_before();
   fence_async();
   __syncthreads();
-  if (threadIdx.x == 0 && mm.ok) {
+  if (threadIdx.x == 0 && ok) {
     tc_fence_after();
-    mma<false, true>(work, base + kGM, base + kGC, idesc<T>(kN, false, true), 8, false);
-    mma<true, true>(tmem, base + kGM, base + kGB, idesc<T>(kN, true, true), 8, false);
-    mm.commit();
+    mma<kK, kMn>(work, base + kGM, base + kGC, idesc<__half>(kN, false, true), 8, false);
+    mma<kMn, kMn>(tmem, base + kGM, base + kGB, idesc<__half>(kN, true, true), 8, false);
+    umma_commit(done.bar);
   }
-  mm.wait();
+  done.wait(ok, P.err);
+  tc_fence_after();
 #pragma unroll
   for (int which = 0; which < 2; ++which) {              // dB, dC
     const uint32_t pairs = lanes + (which ? 0 : 128), states = lanes + (which ? 256 : 384);
     const bool has = which ? has_h : has_g;
-    const float back = kScaled ? (which ? cscale : bscale) : 1.f;
+    const float back = which ? cscale : bscale, pairs_back = all.y * (which ? bback : cback);
     float* part = which ? W.pc : W.pb;
     for (int k = 0; k < 2; ++k) {
       uint32_t r[32], d[32];
@@ -1065,7 +1169,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
         float f[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          f[e] = __uint_as_float(r[j * 8 + e]) * all.y;
+          f[e] = __uint_as_float(r[j * 8 + e]) * pairs_back;
           if (has) f[e] += __uint_as_float(d[j * 8 + e]) * back;
           if (row >= rows) f[e] = 0.f;
         }
@@ -1074,7 +1178,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
           *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
           *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
         } else {
-          sts16(base + (which ? kGX : kGM) + piece2(row, half * 8 + k * 4 + j), pack8<T>(f));
+          sts16(base + (which ? kGHigh : kGM) + piece2(row, half * 8 + k * 4 + j), pack8<T>(f));
         }
       }
     }
@@ -1083,10 +1187,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     __syncthreads();
     for (int hf = 0; hf < 2; ++hf) {
       store_tile<T>(dB + hf * 64, grp_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB + hf * 64, grp_st, 0, 64));
-      store_tile<T>(dC + hf * 64, grp_st, base + kGX + hf * kTile64, out_rows, 64, vector_ok(dC + hf * 64, grp_st, 0, 64));
+      store_tile<T>(dC + hf * 64, grp_st, base + kGHigh + hf * kTile64, out_rows, 64, vector_ok(dC + hf * 64, grp_st, 0, 64));
     }
   }
-  mma_end<512>(tmem);
+  tensor_end<512>(tmem);
 }
 
 // ---------------------------------------------------------------- sums behind the gradients
@@ -1104,14 +1208,14 @@ __global__ void __launch_bounds__(128) finish_dt_kernel(const SelectiveParams P,
       const int t = i * 32 + lane, token = c * Q + t;
       float out = 0.f;
       if (token < len) {
-        const float4 m = W.prm[((long long)b * P.heads + h) * W.lp + token];
+        const float slope = W.rec[(((long long)b * P.heads + h) * W.nc + c) * (4 * Q) + 3 * Q + t];
         float ga = 0.f, gs = 0.f;
         for (int p = 0; p < W.ptiles; ++p) {
           const float2 v = W.parts[((long long)b * W.units + h * W.ptiles + p) * W.lp + token];
           ga += v.x;
           gs += v.y;
         }
-        out = (rate * ga + gs) * m.w;
+        out = (rate * ga + gs) * slope;
         db += out;
       }
       grad[t][k] = out;
@@ -1265,7 +1369,8 @@ template <typename T, bool REV, bool LO> int pass(const SelectiveParams& P, cons
 }
 
 template <typename T> int prepare(const SelectiveParams& P, const Space& W, cudaStream_t st) {
-  prepare_kernel<T><<<dim3(W.nc, (P.heads + 31) / 32, P.batch), 128, 0, st>>>(P, W);
+  const int head_blocks = (P.heads + kPrepHeads - 1) / kPrepHeads;
+  prepare_kernel<T><<<dim3(W.nc, head_blocks + 2 * P.groups, P.batch), kThreads, 0, st>>>(P, W, head_blocks);
   return launch_status();
 }
 
