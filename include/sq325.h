@@ -484,7 +484,7 @@ typedef struct sq_causal_conv_args {
   void* dx; void* dstate_in; void* dweight; void* dbias;
   void* workspace; int64_t workspace_bytes;
 } sq_causal_conv_args;
-int64_t sq_causal_conv_workspace(int batch, int length, int channels, int type);
+int64_t sq_causal_conv_workspace(int batch, int length, int channels);
 int sq_causal_conv_forward(const sq_causal_conv_args* args, void* stream);
 int sq_causal_conv_backward(const sq_causal_conv_args* args, void* stream);
 /* One token of each row of x [batch,channels]; the state is updated in place, y is contiguous. */

@@ -1089,9 +1089,9 @@ int conv_params(const sq_causal_conv_args* a, const char* who, ConvParams& P) {
 }
 }  // namespace
 
-int64_t sq_causal_conv_workspace(int batch, int length, int channels, int type) {
-  if (batch < 1 || length < 1 || channels < 1 || type < SQ_F16 || type > SQ_F32) return -1;
-  return conv_workspace(batch, length, channels, type);
+int64_t sq_causal_conv_workspace(int batch, int length, int channels) {
+  if (batch < 1 || length < 1 || channels < 1) return -1;
+  return conv_workspace(batch, length, channels);
 }
 
 int sq_causal_conv_forward(const sq_causal_conv_args* a, void* stream) {
@@ -1113,7 +1113,7 @@ int sq_causal_conv_backward(const sq_causal_conv_args* a, void* stream) {
   const size_t n = a->type == SQ_F32 ? 4 : 2, w = a->weight_type == SQ_F32 ? 4 : 2;
   if (!aligned(a->dy, n) || !aligned(a->dstate_out, n) || !aligned(a->dx, n) || !aligned(a->dstate_in, n) || !aligned(a->dweight, w) || !aligned(a->dbias, w))
     return bad("misaligned gradient");
-  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < conv_workspace(a->batch, a->length, a->channels, a->type))
+  if (!a->workspace || !aligned(a->workspace, 256) || a->workspace_bytes < conv_workspace(a->batch, a->length, a->channels))
     return bad("workspace missing, misaligned or too small");
   if (a->x) P.codes = nullptr;
   P.dy = a->dy; P.dy_sb = a->dy_batch_stride; P.dy_st = a->dy_token_stride; P.dstate_out = a->dstate_out;

@@ -18,28 +18,38 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kTaps = 4;                            // most taps; fewer use the last ones
+// Channels of a thread of the convolutions.  Four: eight of 16 bits would take 235 registers in the gradients, with too few
+// warps on an SM to have the loads in flight that memory needs.
+constexpr int kWide = 4;
 
-// kUnit<T> values, as fp32; `n` of them are there.
-template <typename T> __device__ __forceinline__ void load_values(const T* p, bool vec, int n, float (&f)[kUnit<T>]) {
-  Unit<T> u;
+// V neighbouring values, as fp32; `n` of them are there.  vec: all are, and lie at a multiple of their size.
+template <int BYTES> struct Word;
+template <> struct Word<16> { using type = uint4; };
+template <> struct Word<8> { using type = uint2; };
+template <typename T, int V> union Values {
+  typename Word<V * (int)sizeof(T)>::type q;
+  T v[V];
+};
+template <typename T, int V> __device__ __forceinline__ void load_values(const T* p, bool vec, int n, float (&f)[V]) {
   if (vec) {
-    u.q = *reinterpret_cast<const uint4*>(p);
+    Values<T, V> u;
+    u.q = *reinterpret_cast<const decltype(u.q)*>(p);
 #pragma unroll
-    for (int i = 0; i < kUnit<T>; ++i) f[i] = to_f32(u.v[i]);
+    for (int i = 0; i < V; ++i) f[i] = to_f32(u.v[i]);
   } else {
 #pragma unroll
-    for (int i = 0; i < kUnit<T>; ++i) f[i] = i < n ? to_f32(p[i]) : 0.f;
+    for (int i = 0; i < V; ++i) f[i] = i < n ? to_f32(p[i]) : 0.f;
   }
 }
-template <typename T> __device__ __forceinline__ void store_values(T* p, bool vec, int n, const float (&f)[kUnit<T>]) {
+template <typename T, int V> __device__ __forceinline__ void store_values(T* p, bool vec, int n, const float (&f)[V]) {
   if (vec) {
-    Unit<T> u;
+    Values<T, V> u;
 #pragma unroll
-    for (int i = 0; i < kUnit<T>; ++i) u.v[i] = from_f32<T>(f[i]);
-    *reinterpret_cast<uint4*>(p) = u.q;
+    for (int i = 0; i < V; ++i) u.v[i] = from_f32<T>(f[i]);
+    *reinterpret_cast<decltype(u.q)*>(p) = u.q;
   } else {
 #pragma unroll
-    for (int i = 0; i < kUnit<T>; ++i)
+    for (int i = 0; i < V; ++i)
       if (i < n) p[i] = from_f32<T>(f[i]);
   }
 }
@@ -79,8 +89,14 @@ template <int V> __device__ __forceinline__ float encode(const float (&f)[V], in
   for (int o = kPackBlock / V / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float scale = __fdiv_rn(__uint_as_float(m), 127.0f);
   const bool fine = scale > 0.f && scale <= 3.0e38f;
+  // x times 1 / scale tells the code but where it lies next to a half (or 1 / scale is infinite): there the quotient does
+  const float inverse = __frcp_rn(scale);
 #pragma unroll
-  for (int i = 0; i < V; ++i) q[i] = fine ? max(-127, min(127, __float2int_rn(__fdiv_rn(f[i], scale)))) : 0;
+  for (int i = 0; i < V; ++i) {
+    float t = f[i] * inverse, r = rintf(t);
+    if (!(fabsf(fabsf(t - r) - 0.5f) >= 1e-4f)) r = rintf(__fdiv_rn(f[i], scale));
+    q[i] = fine ? max(-127, min(127, (int)r)) : 0;
+  }
   return scale;
 }
 
@@ -89,20 +105,35 @@ template <typename T> __device__ __forceinline__ float sigmoid(float z) {
   else return __fdividef(1.0f, 1.0f + __expf(-z));  // a few ulp of fp32, far below a 16-bit result's half step
 }
 
-template <typename T, typename WT>
+// A thread's V channels: weights and bias.
+template <typename WT, int V>
 struct Taps {
-  float w[kTaps][kUnit<T>], b[kUnit<T>];
-  __device__ Taps(const ConvParams& P, int c, int n) {
-    const WT* weight = reinterpret_cast<const WT*>(P.weight) + (long long)c * P.taps;
-    const WT* bias = reinterpret_cast<const WT*>(P.bias) + c;
+  float w[kTaps][V], b[V];
+  __device__ Taps(const void* weights, const void* biases, int taps, int c, int n) {
+    const WT* weight = reinterpret_cast<const WT*>(weights) + (long long)c * taps;
+    if (taps == kTaps && n == V && ((uintptr_t)weight & (4 * sizeof(WT) - 1)) == 0) {
 #pragma unroll
-    for (int i = 0; i < kUnit<T>; ++i) {
+      for (int i = 0; i < V; ++i) {
+        float f[kTaps];
+        load_values<WT, kTaps>(weight + i * kTaps, true, kTaps, f);
 #pragma unroll
-      for (int k = 0; k < kTaps; ++k) {
-        const int j = k - (kTaps - P.taps);
-        w[k][i] = i < n && j >= 0 ? to_f32(weight[i * P.taps + j]) : 0.f;
+        for (int k = 0; k < kTaps; ++k) w[k][i] = f[k];
       }
-      b[i] = i < n && P.bias ? to_f32(bias[i]) : 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int k = 0; k < kTaps; ++k) {
+          const int j = k - (kTaps - taps);
+          w[k][i] = i < n && j >= 0 ? to_f32(weight[i * taps + j]) : 0.f;
+        }
+    }
+    const WT* bias = reinterpret_cast<const WT*>(biases) + c;
+    if (biases) {
+      load_values<WT, V>(bias, n == V && ((uintptr_t)bias & (V * sizeof(WT) - 1)) == 0, n, b);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) b[i] = 0.f;
     }
   }
 };
@@ -112,20 +143,19 @@ __device__ __forceinline__ int tokens_of(const ConvParams& P, int b) {
 }
 
 // The input at token t of a sequence, the state's before the first.
-template <typename T, bool CODES>
-__device__ __forceinline__ void input_at(const ConvParams& P, int b, int t, int c, int n, bool vec, float (&f)[kUnit<T>]) {
-  constexpr int V = kUnit<T>;
+template <typename T, bool CODES, int V>
+__device__ __forceinline__ void input_at(const ConvParams& P, int b, int t, int c, int n, bool vec, float (&f)[V]) {
   if (t >= 0) {
     if constexpr (CODES) {
       const long long row = (long long)b * P.length + t;
       const float scale = P.scales[row * ((P.channels + kPackBlock - 1) / kPackBlock) + c / kPackBlock];
       load_codes<V>(P.codes + row * P.channels + c, vec, n, scale, f);
     } else {
-      load_values<T>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + t * P.x_st + c, vec, n, f);
+      load_values<T, V>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + t * P.x_st + c, vec, n, f);
     }
   } else if (P.state_in && t >= 1 - P.taps) {
     const long long at = ((long long)b * (P.taps - 1) + t + P.taps - 1) * P.channels + c;
-    load_values<T>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
+    load_values<T, V>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = 0.f;
@@ -134,8 +164,8 @@ __device__ __forceinline__ void input_at(const ConvParams& P, int b, int t, int 
 
 // z of a token whose last four inputs are x[0..3], oldest first.  Taps that are not there are passed over, not
 // multiplied by zero: their inputs may be infinite.
-template <typename T, typename WT>
-__device__ __forceinline__ float conv_at(const Taps<T, WT>& W, int taps, int i, float x0, float x1, float x2, float x3) {
+template <typename WT, int V>
+__device__ __forceinline__ float conv_at(const Taps<WT, V>& W, int taps, int i, float x0, float x1, float x2, float x3) {
   float z = W.b[i];
   if (taps > 3) z += W.w[0][i] * x0;
   if (taps > 2) z += W.w[1][i] * x1;
@@ -147,7 +177,7 @@ struct ConvFlags { int vec_in, vec_out, vec_codes; };
 // MODE: 0 reads the input, 1 keeps it in 8 bits besides, 2 reads what was kept.
 template <typename T, typename WT, int MODE>
 __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams P, const ConvFlags F, int strip) {
-  constexpr int V = kUnit<T>;
+  constexpr int V = kWide;
   constexpr bool KEEP = MODE == 1, CODES = MODE == 2;
   const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
   const int n = min(V, P.channels - c);                                // may be negative: shuffles need every lane
@@ -159,31 +189,31 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams P, cons
   float x[kTaps][V];
   if (n > 0 && blockIdx.x == 0 && P.state_out) {                       // the last inputs
     for (int j = 0; j < P.taps - 1; ++j) {
-      input_at<T, CODES>(P, b, len - (P.taps - 1) + j, c, n, vec_in, x[0]);
-      store_values<T>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (P.taps - 1) + j) * P.channels + c, false, n, x[0]);
+      input_at<T, CODES, V>(P, b, len - (P.taps - 1) + j, c, n, vec_in, x[0]);
+      store_values<T, V>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (P.taps - 1) + j) * P.channels + c, false, n, x[0]);
     }
   }
   if (t0 < len) {
-    const Taps<T, WT> W(P, c, n);
+    const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
 #pragma unroll
-    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES>(P, b, n > 0 ? t0 - (kTaps - 1) + k : -kTaps, c, n, vec_in, x[k]);
+    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES, V>(P, b, n > 0 ? t0 - (kTaps - 1) + k : -kTaps, c, n, vec_in, x[k]);
     constexpr int U = 4;                                               // tokens whose loads are in flight together
     for (int t = t0; t < min(t1, len); t += U) {
       float next[U][V];
 #pragma unroll
       for (int j = 0; j < U; ++j)
-        input_at<T, CODES>(P, b, n > 0 && t + j < min(t1, len) ? t + j : -kTaps, c, n, vec_in, next[j]);
+        input_at<T, CODES, V>(P, b, n > 0 && t + j < min(t1, len) ? t + j : -kTaps, c, n, vec_in, next[j]);
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const bool in = t + j < min(t1, len);
         float out[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float z = conv_at<T, WT>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
+          const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
           out[i] = P.silu ? z * sigmoid<T>(z) : z;
           x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = next[j][i];
         }
-        if (in && n > 0) store_values<T>(y + (t + j) * P.y_st, vec_out, n, out);
+        if (in && n > 0) store_values<T, V>(y + (t + j) * P.y_st, vec_out, n, out);
         if constexpr (KEEP) {
           int q[V];
           const float scale = encode<V>(next[j], q);
@@ -199,7 +229,7 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams P, cons
   if (n <= 0) return;
   const float zero[V] = {};
   for (int t = max(t0, len); t < t1; ++t) {
-    store_values<T>(y + t * P.y_st, vec_out, n, zero);
+    store_values<T, V>(y + t * P.y_st, vec_out, n, zero);
     if constexpr (KEEP) {
       const long long row = (long long)b * P.length + t;
       const int none[V] = {};
@@ -213,31 +243,31 @@ __global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams P, cons
 // and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.
 template <typename T, typename WT, bool CODES>
 __global__ void __launch_bounds__(kThreads) conv_grad_kernel(const ConvParams P, const ConvFlags F, int strip) {
-  constexpr int V = kUnit<T>;
+  constexpr int V = kWide;
   const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
   const int n = min(V, P.channels - c);
   if (n <= 0) return;
   const bool vec_in = (CODES ? F.vec_codes : F.vec_in) && n == V, vec_out = F.vec_out && n == V;
-  const bool vec_dx = n == V && P.channels % V == 0 && ((uintptr_t)P.dx & 15) == 0;
+  const bool vec_dx = n == V && P.channels % V == 0 && ((uintptr_t)P.dx & (V * sizeof(T) - 1)) == 0;
   const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip);
   const T* dy = reinterpret_cast<const T*>(P.dy) + b * P.dy_sb + c;
   T* dx = reinterpret_cast<T*>(P.dx) + (long long)b * P.length * P.channels + c;
   const int back = P.taps - 1;
   float dw[kTaps][V] = {}, db[V] = {};
   if (t0 < len || t0 == 0) {
-    const Taps<T, WT> W(P, c, n);
+    const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
     float x[kTaps - 1][V], dz[kTaps][V] = {};
 #pragma unroll
-    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES>(P, b, t0 - (kTaps - 1) + k, c, n, vec_in, x[k]);
+    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES, V>(P, b, t0 - (kTaps - 1) + k, c, n, vec_in, x[k]);
     constexpr int U = 4;
     for (int t = t0; t < t1 + kTaps - 1; t += U) {
       float next[U][V], up[U][V];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         const bool in = t + j < min(t1 + kTaps - 1, len);
-        input_at<T, CODES>(P, b, in ? t + j : -kTaps, c, n, vec_in, next[j]);
+        input_at<T, CODES, V>(P, b, in ? t + j : -kTaps, c, n, vec_in, next[j]);
         if (in) {
-          load_values<T>(dy + (t + j) * P.dy_st, vec_out, n, up[j]);
+          load_values<T, V>(dy + (t + j) * P.dy_st, vec_out, n, up[j]);
         } else {
 #pragma unroll
           for (int i = 0; i < V; ++i) up[j][i] = 0.f;
@@ -252,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) conv_grad_kernel(const ConvParams P,
         for (int i = 0; i < V; ++i) {
           float d = up[j][i];
           if (in && P.silu) {
-            const float z = conv_at<T, WT>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
+            const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
             const float s = sigmoid<T>(z);
             d *= s * (1.0f + z * (1.0f - s));
           }
@@ -275,20 +305,20 @@ __global__ void __launch_bounds__(kThreads) conv_grad_kernel(const ConvParams P,
         if (P.dstate_out && to >= len - back && to < len) {
           float late[V];
           const long long at = ((long long)b * back + to - (len - back)) * P.channels + c;
-          load_values<T>(reinterpret_cast<const T*>(P.dstate_out) + at, false, n, late);
+          load_values<T, V>(reinterpret_cast<const T*>(P.dstate_out) + at, false, n, late);
 #pragma unroll
           for (int i = 0; i < V; ++i) out[i] += late[i];
         }
         if (to >= 0) {
-          if (to < len) store_values<T>(dx + (long long)to * P.channels, vec_dx, n, out);
+          if (to < len) store_values<T, V>(dx + (long long)to * P.channels, vec_dx, n, out);
         } else if (P.dstate_in) {
-          store_values<T>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
+          store_values<T, V>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
         }
       }
     }
   }
   const float zero[V] = {};
-  for (int t = max(t0, len); t < t1; ++t) store_values<T>(dx + (long long)t * P.channels, vec_dx, n, zero);
+  for (int t = max(t0, len); t < t1; ++t) store_values<T, V>(dx + (long long)t * P.channels, vec_dx, n, zero);
   if (P.dweight || P.dbias) {
     float* part = P.workspace + ((long long)b * gridDim.x + blockIdx.x) * (kTaps + 1) * P.channels + c;
 #pragma unroll
@@ -326,41 +356,37 @@ __global__ void __launch_bounds__(256) conv_weights_kernel(const ConvParams P, i
 // One token: a thread owns 16 bytes of channels, shifts their state and puts the token at its end.
 template <typename T, typename WT, typename YT>
 __global__ void __launch_bounds__(kThreads) conv_step_kernel(const ConvStepParams P, int vec) {
-  constexpr int V = kUnit<T>;
+  constexpr int V = kWide;
   const int c = (blockIdx.x * kThreads + threadIdx.x) * V, b = blockIdx.y;
   const int n = min(V, P.channels - c);
   launch_dependents();
   if (n <= 0) return;
   const bool v = vec && n == V;
-  ConvParams C{};
-  C.taps = P.taps; C.weight = P.weight; C.bias = P.bias;
   T* state = reinterpret_cast<T*>(P.state) + (long long)b * (P.taps - 1) * P.channels + c;
   float x[kTaps][V] = {};
-  load_values<T>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + c, v, n, x[3]);
+  load_values<T, V>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + c, v, n, x[3]);
 #pragma unroll
   for (int k = 0; k < kTaps - 1; ++k) {
     const int j = k - (kTaps - P.taps);
-    if (j >= 0) load_values<T>(state + (long long)j * P.channels, v, n, x[k]);
+    if (j >= 0) load_values<T, V>(state + (long long)j * P.channels, v, n, x[k]);
   }
-  const Taps<T, WT> W(C, c, n);
+  const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
   float out[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    const float z = conv_at<T, WT>(W, P.taps, i, x[0][i], x[1][i], x[2][i], x[3][i]);
+    const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], x[3][i]);
     out[i] = P.silu ? z * sigmoid<T>(z) : z;
   }
   YT* y = reinterpret_cast<YT*>(P.y) + (long long)b * P.channels + c;
   if constexpr (sizeof(YT) == sizeof(T)) {
-    store_values<T>(y, v, n, out);
+    store_values<T, V>(y, v, n, out);
   } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) y[i] = out[i];
+    store_values<float, V>(y, v, n, out);
   }
 #pragma unroll
   for (int k = 0; k < kTaps - 1; ++k) {
     const int j = k - (kTaps - P.taps);
-    if (j >= 0) store_values<T>(state + (long long)j * P.channels, v, n, x[k + 1]);
+    if (j >= 0) store_values<T, V>(state + (long long)j * P.channels, v, n, x[k + 1]);
   }
 }
 
@@ -376,7 +402,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams P, int 
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       if (n > 0 && r0 + j < P.rows) {
-        load_values<T>(reinterpret_cast<const T*>(P.x) + (r0 + j) * P.x_stride + c, vec && n == V, n, f[j]);
+        load_values<T, V>(reinterpret_cast<const T*>(P.x) + (r0 + j) * P.x_stride + c, vec && n == V, n, f[j]);
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) f[j][i] = 0.f;
@@ -400,25 +426,27 @@ __global__ void __launch_bounds__(kThreads) unpack_kernel(const PackParams P, in
   const int n = min(V, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
   if (n <= 0) return;
   for (long long r0 = (long long)blockIdx.y * kRows; r0 < P.rows; r0 += (long long)gridDim.y * kRows) {
-    float f[kRows][V];
+    float f[kRows][V], scale[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) scale[j] = r0 + j < P.rows ? P.scales[(r0 + j) * blocks + c / kPackBlock] : 0.f;
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      if (r0 + j < P.rows)
-        load_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, P.scales[(r0 + j) * blocks + c / kPackBlock], f[j]);
+      if (r0 + j < P.rows) load_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, scale[j], f[j]);
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      if (r0 + j < P.rows) store_values<T>(reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c, vec && n == V, n, f[j]);
+      if (r0 + j < P.rows) store_values<T, V>(reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c, vec && n == V, n, f[j]);
   }
 }
 
 int unit_of(int type) { return type == 2 ? 4 : 8; }
-bool whole(const void* p, int type, long long a, long long b = 0) {
-  return ((uintptr_t)p & 15) == 0 && (a | b) % unit_of(type) == 0;
+// Whether `wide` neighbours starting at multiples of `wide` can be moved at once.
+bool whole(const void* p, int type, int wide, long long a, long long b = 0) {
+  return ((uintptr_t)p & (wide * (type == 2 ? 4 : 2) - 1)) == 0 && (a | b) % wide == 0;
 }
 
 // Tokens of a strip: long ones read fewer edges twice, short ones make more CTAs.
-int strip_of(int batch, int length, int channels, int type, int least, int most) {
-  const long long wide = (long long)batch * ((channels + unit_of(type) - 1) / unit_of(type));
+int strip_of(int batch, int length, int channels, int least, int most) {
+  const long long wide = (long long)batch * ((channels + kWide - 1) / kWide);
   int s = most;
   while (s > least && wide * ((length + s - 1) / s) < 148 * 1024) s /= 2;
   return s;
@@ -433,16 +461,16 @@ template <typename F> int by_type(int type, int weight_type, F f) {
 
 }  // namespace
 
-long long conv_workspace(int batch, int length, int channels, int type) {
-  const int strip = strip_of(batch, length, channels, type, kLeast, kMost);
+long long conv_workspace(int batch, int length, int channels) {
+  const int strip = strip_of(batch, length, channels, kLeast, kMost);
   return (long long)batch * ((length + strip - 1) / strip) * (kTaps + 1) * channels * 4;
 }
 
 int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
-  const int strip = strip_of(P.batch, P.length, P.channels, P.type, 8, 64), per = kThreads * unit_of(P.type);
+  const int strip = strip_of(P.batch, P.length, P.channels, 16, 64), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
-  const ConvFlags F{P.x && whole(P.x, P.type, P.x_sb, P.x_st), whole(P.y, P.type, P.y_sb, P.y_st),
-                    P.channels % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0};
+  const ConvFlags F{P.x && whole(P.x, P.type, kWide, P.x_sb, P.x_st), whole(P.y, P.type, kWide, P.y_sb, P.y_st),
+                    P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0};
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
@@ -454,10 +482,10 @@ int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
 }
 
 int launch_conv_backward(const ConvParams& P, cudaStream_t st) {
-  const int strip = strip_of(P.batch, P.length, P.channels, P.type, kLeast, kMost), per = kThreads * unit_of(P.type);
+  const int strip = strip_of(P.batch, P.length, P.channels, kLeast, kMost), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
-  const ConvFlags F{P.x && whole(P.x, P.type, P.x_sb, P.x_st), whole(P.dy, P.type, P.dy_sb, P.dy_st),
-                    P.channels % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0};
+  const ConvFlags F{P.x && whole(P.x, P.type, kWide, P.x_sb, P.x_st), whole(P.dy, P.type, kWide, P.dy_sb, P.dy_st),
+                    P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0};
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
@@ -473,9 +501,9 @@ int launch_conv_backward(const ConvParams& P, cudaStream_t st) {
 }
 
 int launch_conv_step(const ConvStepParams& P, cudaStream_t st) {
-  const int per = kThreads * unit_of(P.type);
+  const int per = kThreads * kWide;
   const dim3 grid((P.channels + per - 1) / per, P.batch);
-  const int vec = whole(P.x, P.type, P.x_sb, P.channels) && ((uintptr_t)P.state & 15) == 0 && ((uintptr_t)P.y & 15) == 0;
+  const int vec = whole(P.x, P.type, kWide, P.x_sb, P.channels) && whole(P.state, P.type, kWide, 0) && whole(P.y, P.y_f32 ? 2 : P.type, kWide, 0);
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
@@ -487,21 +515,22 @@ int launch_conv_step(const ConvStepParams& P, cudaStream_t st) {
 
 namespace {
 dim3 pack_grid(const PackParams& P) {
-  const int per = kThreads * unit_of(P.type);
-  const long long rows = (P.rows + kRows - 1) / kRows;
-  return dim3((P.width + per - 1) / per, (unsigned)(rows < 65535 ? rows : 65535));
+  const int per = kThreads * unit_of(P.type), wide = (P.width + per - 1) / per;
+  long long rows = (P.rows + kRows - 1) / kRows, most = 148 * 16 / wide;      // CTAs that an SM's threads hold
+  most = most < 1 ? 1 : most > 65535 ? 65535 : most;
+  return dim3(wide, (unsigned)(rows < most ? rows : most));
 }
 }  // namespace
 
 int launch_pack(const PackParams& P, cudaStream_t st) {
-  const int vec = whole(P.x, P.type, P.x_stride), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
+  const int vec = whole(P.x, P.type, unit_of(P.type), P.x_stride), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
   if (P.type == 0) pack_kernel<__half><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
   else if (P.type == 1) pack_kernel<__nv_bfloat16><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
   else pack_kernel<float><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
   return launch_status();
 }
 int launch_unpack(const PackParams& P, cudaStream_t st) {
-  const int vec = whole(P.y, P.type, P.width), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
+  const int vec = whole(P.y, P.type, unit_of(P.type), P.width), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
   if (P.type == 0) unpack_kernel<__half><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
   else if (P.type == 1) unpack_kernel<__nv_bfloat16><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
   else unpack_kernel<float><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);

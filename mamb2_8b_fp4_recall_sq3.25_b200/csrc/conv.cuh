@@ -41,7 +41,7 @@ struct PackParams {
   void* y;                                          // unpacked, contiguous
 };
 
-long long conv_workspace(int batch, int length, int channels, int type);
+long long conv_workspace(int batch, int length, int channels);
 int launch_conv_forward(const ConvParams& p, cudaStream_t stream);
 int launch_conv_backward(const ConvParams& p, cudaStream_t stream);
 int launch_conv_step(const ConvStepParams& p, cudaStream_t stream);

@@ -105,6 +105,15 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[3
       : "r"(taddr));
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
 // Keeps uses of a tcgen05.ld's registers behind the wait that precedes this call.
 __device__ __forceinline__ void settle(uint32_t (&r)[32]) {
 #pragma unroll
@@ -242,13 +251,13 @@ __device__ __forceinline__ uint4 ragged_piece(const T* p, int n) {
     if (e < n) u[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
   return make_uint4(u[0], u[1], u[2], u[3]);
 }
-template <typename T>
+template <typename T, int THREADS = kThreads>
 __device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long stride, int rows, int cols, bool vec) {
   const int j = threadIdx.x & 7;
   const T* p = src + (long long)(threadIdx.x >> 3) * stride + j * 8;
 #pragma unroll
-  for (int i = 0; i < Q * 8 / kThreads; ++i, p += (kThreads / 8) * stride) {
-    const int r = (threadIdx.x >> 3) + i * (kThreads / 8);
+  for (int i = 0; i < Q * 8 / THREADS; ++i, p += (THREADS / 8) * stride) {
+    const int r = (threadIdx.x >> 3) + i * (THREADS / 8);
     const uint32_t a = dst + piece(r, j);
     const bool in = r < rows && j * 8 < cols;
     if (vec) cp16(a, in ? p : src, in);
@@ -256,9 +265,9 @@ __device__ __forceinline__ void load_tile(uint32_t dst, const T* src, long long 
   }
 }
 // The first `rows` rows and `cols` columns of a tile [128][64] to global memory.
-template <typename T>
+template <typename T, int THREADS = kThreads>
 __device__ __forceinline__ void store_tile(T* dst, long long stride, uint32_t src, int rows, int cols, bool vec) {
-  for (int i = threadIdx.x; i < Q * 8; i += kThreads) {
+  for (int i = threadIdx.x; i < Q * 8; i += THREADS) {
     const int r = i >> 3, j = i & 7;
     if (r >= rows || j * 8 >= cols) continue;
     const uint4 v = lds16(src + piece(r, j));
@@ -740,7 +749,8 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
 // After the last unit the group's sum gives the pairs' part of dB and dC in two products.
 constexpr uint32_t kGB = 0, kGC = kTile128, kGX = 2 * kTile128, kGY = kGX + kTile64, kGHigh = kGY + 2 * kTile64,
                    kGLow = kGHigh + 2 * kTile64, kGM = kGLow + 2 * kTile64, kGRec = kGM + kTile128, kGRow = kGRec + 2 * kRecBytes,
-                   kGCol = kGRow + 7 * Q * 4, kGRed = kGCol + 4 * Q * 4, kGBar = kGRed + 32 * 4, kGradSmem = kGBar + 48;
+                   kGCol = kGRow + 13 * Q * 4, kGRed = kGCol + 4 * Q * 4, kGBar = kGRed + 64 * 4, kGradSmem = kGBar + 48;
+constexpr int kGradThreads = 512;                  // four threads a token: sixteen warps hide each other's waits
 
 // Sums over a warp's lanes of e[column], for column = lane.
 __device__ __forceinline__ float column_sums(float (&e)[32], int lane) {
@@ -757,20 +767,20 @@ __device__ __forceinline__ float column_sums(float (&e)[32], int lane) {
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams P, const Space W, int per) {
+__global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectiveParams P, const Space W, int per) {
   constexpr bool kScaled = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  float* rpairs = reinterpret_cast<float*>(smem + kGRow);        // [2][Q] each: r by pairs, r by states, q by states; [Q]: r by the token itself
-  float *rstate = rpairs + 2 * Q, *qstate = rpairs + 4 * Q, *rself = rpairs + 6 * Q;
+  float* rpairs = reinterpret_cast<float*>(smem + kGRow);        // [4][Q] each: r by pairs, r by states, q by states; [Q]: r by the token itself
+  float *rstate = rpairs + 4 * Q, *qstate = rpairs + 8 * Q, *rself = rpairs + 12 * Q;
   float* qpairs = reinterpret_cast<float*>(smem + kGCol);        // [4][Q]
-  float* red = reinterpret_cast<float*>(smem + kGRed);           // [0..8) <G, H>, [8..16) x . dy, [16..24) pairs' time, [24..32) maxima
+  float* red = reinterpret_cast<float*>(smem + kGRed);           // [16] each: <G, H>, x . dy, pairs' time, maxima
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kGBar);    // tensor cores, tiles, values, remainders
   const int c = blockIdx.x, b = blockIdx.z;
   const int gunits = W.units / P.groups, g = blockIdx.y / W.splits, split = blockIdx.y % W.splits;
   const int u0 = g * gunits + split * per, u1 = min(u0 + per, (g + 1) * gunits);
   const int len = tokens_of(P, b), rows = min(Q, len - c * Q), out_rows = min(Q, P.length - c * Q);
-  const int row = threadIdx.x & 127, half = threadIdx.x >> 7, warp = threadIdx.x >> 5, quad = warp & 3, lane = threadIdx.x & 31;
+  const int row = threadIdx.x & 127, part = threadIdx.x >> 7, warp = threadIdx.x >> 5, quad = warp & 3, lane = threadIdx.x & 31;
   const long long bc = (long long)b * W.nc + c, dx_st = P.dx_st, grp_st = P.dg_st, tile_at = bc * P.groups + g;
   T* dx = reinterpret_cast<T*>(P.dx) + b * P.dx_sb + (long long)c * Q * dx_st;
   const long long grp_at = b * P.dg_sb + (long long)c * Q * grp_st + g * kN;
@@ -778,12 +788,12 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
   if (rows <= 0) {                                       // behind the sequence's end
     for (int u = u0; u < u1; ++u) {
       const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
-      for (int i = threadIdx.x; i < out_rows * cols; i += kThreads)
+      for (int i = threadIdx.x; i < out_rows * cols; i += kGradThreads)
         dx[(long long)(i / cols) * dx_st + (long long)h * P.dim + p0 + i % cols] = from_f32<T>(0.f);
       if (threadIdx.x == 0) W.unit_sums[bc * W.units + u] = make_float2(0.f, 0.f);
     }
     if (W.splits == 1)
-      for (int i = threadIdx.x; i < out_rows * kN; i += kThreads)
+      for (int i = threadIdx.x; i < out_rows * kN; i += kGradThreads)
         dB[(long long)(i / kN) * grp_st + i % kN] = dC[(long long)(i / kN) * grp_st + i % kN] = from_f32<T>(0.f);
     return;
   }
@@ -812,12 +822,12 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
   auto load_x = [&](int u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
     const T* p = xc + (long long)h * P.dim + p0;
-    load_tile<T>(base + kGX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
+    load_tile<T, kGradThreads>(base + kGX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
   };
   auto load_y = [&](int u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
     const T* p = yc + (long long)h * P.dim + p0;
-    load_tile<T>(base + kGY + ((u - u0) & 1) * kTile64, p, P.dy_st, rows, cols, vector_ok(p, P.dy_st, 0, cols));
+    load_tile<T, kGradThreads>(base + kGY + ((u - u0) & 1) * kTile64, p, P.dy_st, rows, cols, vector_ok(p, P.dy_st, 0, cols));
   };
   if (threadIdx.x == 0) {
     mbar_expect_tx(tiles.bar, 2 * kTile128);
@@ -851,21 +861,20 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
   float2 sc = make_float2(1.f, 1.f);
   if (kScaled) {                                         // by the largest |B_s . C_t| of my row's pairs
     uint32_t m = 0;
-    for (int cb = half; cb < 4; cb += 2) {
-      if (cb < quad) continue;
+    if (part >= quad) {
       uint32_t r[32];
-      tmem_ld32(lanes + cb * 32, r);
+      tmem_ld32(lanes + part * 32, r);
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (cb * 32 + i >= row) m = max(m, r[i] & 0x7fffffffu);
+        if (part * 32 + i >= row) m = max(m, r[i] & 0x7fffffffu);
     }
-    rpairs[half * Q + row] = __uint_as_float(m);
+    rpairs[part * Q + row] = __uint_as_float(m);
     __syncthreads();
-    sc = scale_of(__float_as_uint(fmaxf(rpairs[row], rpairs[Q + row])));
+    sc = scale_of(__float_as_uint(fmaxf(fmaxf(rpairs[row], rpairs[Q + row]), fmaxf(rpairs[2 * Q + row], rpairs[3 * Q + row]))));
   }
-  float2 ds[2][16];
+  float2 ds[16];
 #pragma unroll
-  for (int i = 0; i < 32; ++i) ds[i >> 4][i & 15] = make_float2(0.f, 0.f);
+  for (int i = 0; i < 16; ++i) ds[i] = make_float2(0.f, 0.f);
 
   for (int u = u0; u < u1; ++u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
@@ -896,8 +905,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     const float wy = has_h ? from_in * (hs.x / cscale) : 0.f, wx = has_g ? s * to_end * (gs.x / bscale) : 0.f;
     float gh = 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t at = piece(row, half * 4 + j), plane = (uint32_t)((half * 4 + j) * kN + row) * 16;
+    for (int j = 0; j < 2; ++j) {
+      const uint32_t at = piece(row, part * 2 + j), plane = (uint32_t)((part * 2 + j) * kN + row) * 16;
       float f[8], o[8];
       if (has_h) {
         unpack8<T>(lds16(ytile + at), f);
@@ -924,19 +933,19 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     gh = warp_sum(gh);
     if (lane == 0) red[warp] = gh;
     fence_async();
-    float dxi[32];
+    float dxi[16];
     float r_part = 0.f, q_part = 0.f;
     if (has_h || has_g) {
       done.wait(ok, P.err);
       tc_fence_after();
-      uint32_t r[32];
+      uint32_t r[16];
       if (has_g) {
-        tmem_ld32(lanes + 128 + half * 32, r);
+        tmem_ld16(lanes + 128 + part * 16, r);
         const float f = to_end * gs.x * bback;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           float x[8];
-          unpack8<T>(lds16(base + kGX + piece(row, half * 4 + j)), x);
+          unpack8<T>(lds16(base + kGX + piece(row, part * 2 + j)), x);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             dxi[j * 8 + e] = f * __uint_as_float(r[j * 8 + e]);
@@ -945,11 +954,11 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
         }
       }
       if (has_h) {
-        tmem_ld32(lanes + 192 + half * 32, r);
+        tmem_ld16(lanes + 192 + part * 16, r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < 2; ++j) {
           float y[8];
-          unpack8<T>(lds16(ytile + piece(row, half * 4 + j)), y);
+          unpack8<T>(lds16(ytile + piece(row, part * 2 + j)), y);
 #pragma unroll
           for (int e = 0; e < 8; ++e) q_part += __uint_as_float(r[j * 8 + e]) * y[e];
         }
@@ -957,11 +966,11 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
       }
       tc_fence_before();
     }
-    rstate[half * Q + row] = r_part;
-    qstate[half * Q + row] = q_part;
+    rstate[part * Q + row] = r_part;
+    qstate[part * Q + row] = q_part;
     if (!has_g)
 #pragma unroll
-      for (int i = 0; i < 32; ++i) dxi[i] = 0.f;
+      for (int i = 0; i < 16; ++i) dxi[i] = 0.f;
     __syncthreads();
     // step 2
     if (threadIdx.x == 0) {
@@ -984,9 +993,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     }
     float r_sum = 0.f, diag = 0.f, pair_time = 0.f;
     const float sb = s * both_back;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int cb = half + 2 * k;
+    {
+      const int cb = part;
       if (cb >= quad) {
         uint32_t r[32], d[32];
         tmem_ld32_nowait(lanes + cb * 32, r);
@@ -1013,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
                 if (t + 1 < row) { w.y = 0.f; gap.y = 0.f; }
               }
               const float2 dm = words2(d[q], d[q + 1]), m = __fmul2_rn(words2(r[q], r[q + 1]), w);
-              ds[k][q >> 1] = __ffma2_rn(pair(s), __fmul2_rn(dm, w), ds[k][q >> 1]);
+              ds[q >> 1] = __ffma2_rn(pair(s), __fmul2_rn(dm, w), ds[q >> 1]);
               float2 both = __fmul2_rn(m, dm);
               if (cb == quad) {                          // no decay between a token and itself: kept out of the sums
                 const int t = cb * 32 + q;
@@ -1039,10 +1047,10 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
         qpairs[quad * Q + cb * 32 + lane] = 0.f;
       }
     }
-    rpairs[half * Q + row] = r_sum * both_back;
+    rpairs[part * Q + row] = r_sum * both_back;
     diag = warp_sum(diag);
     pair_time = warp_sum(pair_time);
-    if (lane == 0) { red[8 + warp] = diag; red[16 + warp] = pair_time; }
+    if (lane == 0) { red[16 + warp] = diag; red[32 + warp] = pair_time; }
     tc_fence_before();
     fence_async();
     __syncthreads();
@@ -1052,18 +1060,19 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
       mma<kK, kMn>(work, base + kGM, ytile, idesc<T>(TP, false, true), 8, false);
       umma_commit(done.bar);
     }
-    if (warp == 7) {                                     // four tokens a lane
+    if (warp == 15) {                                    // four tokens a lane
       float a[4], r[4], sa = 0.f, sum = 0.f, bs[4], time = 0.f;
       float through = 0.f, dd = 0.f, da = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { through += red[i]; dd += red[8 + i]; da += red[16 + i]; }
+      for (int i = 0; i < 16; ++i) { through += red[i]; dd += red[16 + i]; da += red[32 + i]; }
       through *= ex2(eh + el) * (hs.x * gs.x);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int t = 4 * lane + i;
-        const float st = rec[t], rp = rpairs[t] + rpairs[Q + t], rs = rstate[t] + rstate[Q + t], qs = qstate[t] + qstate[Q + t];
+        const auto four = [&](const float* v) { return (v[t] + v[Q + t]) + (v[2 * Q + t] + v[3 * Q + t]); };
+        const float st = rec[t], rp = four(rpairs), rs = four(rstate), qs = four(qstate);
         r[i] = rp + rs + rself[t];
-        a[i] = ((qpairs[t] + qpairs[Q + t]) + (qpairs[2 * Q + t] + qpairs[3 * Q + t])) + qs - st * rp;
+        a[i] = four(qpairs) + qs - st * rp;
         bs[i] = st * rs;
         time += qs * (rec[Q + t] + rec[2 * Q + t]) + bs[i] * ((eh - rec[Q + t]) + (el - rec[2 * Q + t]));
         sa += a[i];
@@ -1098,12 +1107,12 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     done.wait(ok, P.err);
     tc_fence_after();
     {
-      uint32_t r[32];
-      tmem_ld32(lanes + 128 + half * 32, r);
+      uint32_t r[16];
+      tmem_ld16(lanes + 128 + part * 16, r);
       tc_fence_before();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t at = piece(row, half * 4 + j);
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t at = piece(row, part * 2 + j);
         float f[8];
         unpack8<T>(lds16(ytile + at), f);
 #pragma unroll
@@ -1114,34 +1123,31 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     }
     __syncthreads();
     T* out = dx + (long long)h * P.dim + p0;
-    store_tile<T>(out, dx_st, base + kGM, out_rows, cols, vector_ok(out, dx_st, 0, cols));
+    store_tile<T, kGradThreads>(out, dx_st, base + kGM, out_rows, cols, vector_ok(out, dx_st, 0, cols));
   }
   __syncthreads();
 
   // the pairs' part of dB and dC
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    top = max(top, max(__float_as_uint(ds[i >> 4][i & 15].x) & 0x7fffffffu, __float_as_uint(ds[i >> 4][i & 15].y) & 0x7fffffffu));
+  for (int i = 0; i < 16; ++i) top = max(top, max(__float_as_uint(ds[i].x) & 0x7fffffffu, __float_as_uint(ds[i].y) & 0x7fffffffu));
   top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) red[24 + warp] = __uint_as_float(top);
+  if (lane == 0) red[48 + warp] = __uint_as_float(top);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(red[24 + i]));
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(red[48 + i]));
   const float2 all = scale_of(top);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int j = 0; j < 4; ++j) {
+    float f[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const float2 v = __fmul2_rn(ds[k][j * 4 + (i >> 1)], pair(all.x));
-        f[i] = v.x;
-        f[i + 1] = v.y;
-      }
-      sts16(base + kGM + piece2(row, (half + 2 * k) * 4 + j), pack8<__half>(f));
+    for (int i = 0; i < 8; i += 2) {
+      const float2 v = __fmul2_rn(ds[j * 4 + (i >> 1)], pair(all.x));
+      f[i] = v.x;
+      f[i + 1] = v.y;
     }
+    sts16(base + kGM + piece2(row, part * 4 + j), pack8<__half>(f));
+  }
   tc_fence_before();
   fence_async();
   __syncthreads();
@@ -1158,11 +1164,11 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
     const uint32_t pairs = lanes + (which ? 0 : 128), states = lanes + (which ? 256 : 384);
     const bool has = which ? has_h : has_g;
     const float back = which ? cscale : bscale, pairs_back = all.y * (which ? bback : cback);
-    float* part = which ? W.pc : W.pb;
-    for (int k = 0; k < 2; ++k) {
+    float* sums = which ? W.pc : W.pb;
+    {
       uint32_t r[32], d[32];
-      if (has) tmem_ld32_nowait(states + half * 64 + k * 32, d);
-      tmem_ld32(pairs + half * 64 + k * 32, r);
+      if (has) tmem_ld32_nowait(states + part * 32, d);
+      tmem_ld32(pairs + part * 32, r);
       if (has) settle(d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -1174,11 +1180,11 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
           if (row >= rows) f[e] = 0.f;
         }
         if (W.splits > 1) {
-          float* p = part + ((((long long)split * P.batch + b) * W.lp + (long long)c * Q + row) * P.groups + g) * kN + half * 64 + k * 32 + j * 8;
+          float* p = sums + ((((long long)split * P.batch + b) * W.lp + (long long)c * Q + row) * P.groups + g) * kN + part * 32 + j * 8;
           *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
           *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
         } else {
-          sts16(base + (which ? kGHigh : kGM) + piece2(row, half * 8 + k * 4 + j), pack8<T>(f));
+          sts16(base + (which ? kGHigh : kGM) + piece2(row, part * 4 + j), pack8<T>(f));
         }
       }
     }
@@ -1186,8 +1192,8 @@ __global__ void __launch_bounds__(kThreads, 1) grad_kernel(const SelectiveParams
   if (W.splits == 1) {
     __syncthreads();
     for (int hf = 0; hf < 2; ++hf) {
-      store_tile<T>(dB + hf * 64, grp_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB + hf * 64, grp_st, 0, 64));
-      store_tile<T>(dC + hf * 64, grp_st, base + kGHigh + hf * kTile64, out_rows, 64, vector_ok(dC + hf * 64, grp_st, 0, 64));
+      store_tile<T, kGradThreads>(dB + hf * 64, grp_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB + hf * 64, grp_st, 0, 64));
+      store_tile<T, kGradThreads>(dC + hf * 64, grp_st, base + kGHigh + hf * kTile64, out_rows, 64, vector_ok(dC + hf * 64, grp_st, 0, 64));
     }
   }
   tensor_end<512>(tmem);
@@ -1396,7 +1402,7 @@ template <typename T> int backward(const SelectiveParams& P, cudaStream_t st) {
   }
   if (int s = allow<grad_kernel<T>>(kGradSmem)) return s;
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
-  grad_kernel<T><<<dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kGradSmem, st>>>(P, W, per);
+  grad_kernel<T><<<dim3(W.nc, P.groups * W.splits, P.batch), kGradThreads, kGradSmem, st>>>(P, W, per);
   if (int s = launch_status()) return s;
   finish_dt_kernel<T><<<dim3(W.nc, (P.heads + 31) / 32, P.batch), 128, 0, st>>>(P, W);
   if (int s = launch_status()) return s;

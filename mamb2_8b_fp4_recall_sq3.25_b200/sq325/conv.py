@@ -93,7 +93,7 @@ def conv_backward(shape, dtype, x, packed, weight, bias, state, lengths, silu, d
     dweight = torch.empty_like(weight) if want_weight else None
     dbias = torch.empty_like(bias) if want_bias else None
     dstate = torch.empty_like(state) if want_state else None
-    nbytes = int(_lib.load().sq_causal_conv_workspace(*shape, TYPES[dtype]))
+    nbytes = int(_lib.load().sq_causal_conv_workspace(*shape))
     work = torch.empty(nbytes, dtype=torch.uint8, device=device)
     a = conv_args(shape, dtype, x, packed, weight, bias, state, lengths, silu)
     a.dy, a.dy_batch_stride, a.dy_token_stride, a.dstate_out = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
