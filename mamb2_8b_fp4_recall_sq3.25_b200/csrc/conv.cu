@@ -22,81 +22,102 @@ constexpr int kTaps = 4;                            // most taps; fewer use the 
 // warps on an SM to have the loads in flight that memory needs.
 constexpr int kWide = 4;
 
-// V neighbouring values, as fp32; `n` of them are there.  vec: all are, and lie at a multiple of their size.
+// V neighbouring values as memory has them; `n` of them are there.  vec: all are, and lie at a multiple of their size.
 template <int BYTES> struct Word;
 template <> struct Word<16> { using type = uint4; };
 template <> struct Word<8> { using type = uint2; };
+template <> struct Word<4> { using type = uint32_t; };
 template <typename T, int V> union Values {
   typename Word<V * (int)sizeof(T)>::type q;
   T v[V];
 };
-template <typename T, int V> __device__ __forceinline__ void load_values(const T* p, bool vec, int n, float (&f)[V]) {
-  if (vec) {
-    Values<T, V> u;
-    u.q = *reinterpret_cast<const decltype(u.q)*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = to_f32(u.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = i < n ? to_f32(p[i]) : 0.f;
-  }
+template <typename T, int V> __device__ __forceinline__ Values<T, V> no_values() {
+  Values<T, V> u;
+  u.q = decltype(u.q){};
+  return u;
 }
-template <typename T, int V> __device__ __forceinline__ void store_values(T* p, bool vec, int n, const float (&f)[V]) {
+template <typename T, int V> __device__ __forceinline__ Values<T, V> raw_values(const T* p, bool vec, int n) {
+  Values<T, V> u;
   if (vec) {
-    Values<T, V> u;
+    u.q = *reinterpret_cast<const decltype(u.q)*>(p);
+  } else {
+    u.q = decltype(u.q){};
 #pragma unroll
-    for (int i = 0; i < V; ++i) u.v[i] = from_f32<T>(f[i]);
+    for (int i = 0; i < V; ++i)
+      if (i < n) u.v[i] = p[i];
+  }
+  return u;
+}
+template <typename T, int V> __device__ __forceinline__ void load_values(const T* p, bool vec, int n, float (&f)[V]) {
+  const Values<T, V> u = raw_values<T, V>(p, vec, n);
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = to_f32(u.v[i]);
+}
+// Two neighbours are converted by one instruction.
+__device__ __forceinline__ void to_pair(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
+__device__ __forceinline__ void to_pair(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+__device__ __forceinline__ void to_pair(float* p, float a, float b) { p[0] = a; p[1] = b; }
+template <typename T, int V> __device__ __forceinline__ void store_values(T* p, bool vec, int n, const float (&f)[V]) {
+  Values<T, V> u;
+#pragma unroll
+  for (int i = 0; i < V; i += 2) to_pair(&u.v[i], f[i], f[i + 1]);
+  if (vec) {
     *reinterpret_cast<decltype(u.q)*>(p) = u.q;
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = from_f32<T>(f[i]);
+      if (i < n) p[i] = u.v[i];
   }
 }
-template <int V> __device__ __forceinline__ void store_codes(int8_t* p, bool vec, int n, const int (&q)[V]) {
+
+// ---------------------------------------------------------------- 8 bits
+constexpr float kWhole = 12582912.0f;               // 1.5 * 2^23: added to a small number it leaves the rounded one in the low bits
+
+template <int V> __device__ __forceinline__ void store_codes(int8_t* p, bool vec, int n, const Values<int8_t, V>& u) {
   if (vec) {
-    uint32_t w[V / 4];
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i)
-      w[i] = (q[4 * i] & 255) | (q[4 * i + 1] & 255) << 8 | (q[4 * i + 2] & 255) << 16 | (uint32_t)q[4 * i + 3] << 24;
-    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-    else *reinterpret_cast<uint32_t*>(p) = w[0];
+    *reinterpret_cast<decltype(u.q)*>(p) = u.q;
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = (int8_t)q[i];
+      if (i < n) p[i] = u.v[i];
   }
 }
-template <int V> __device__ __forceinline__ void load_codes(const int8_t* p, bool vec, int n, float scale, float (&f)[V]) {
-  if (vec) {
-    uint32_t w[V / 4];
-    if constexpr (V == 8) { const uint2 u = *reinterpret_cast<const uint2*>(p); w[0] = u.x; w[1] = u.y; }
-    else w[0] = *reinterpret_cast<const uint32_t*>(p);
+// A code as the low byte of 2^23 + 128 + code: no conversion, which has a sixteenth of the adds' rate.
+template <int V> __device__ __forceinline__ void decode(const Values<int8_t, V>& u, float scale, float (&f)[V]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = (float)(int8_t)(w[i >> 2] >> (8 * (i & 3))) * scale;
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = i < n ? (float)p[i] * scale : 0.f;
-  }
+  for (int i = 0; i < V; ++i)
+    f[i] = (__uint_as_float(__byte_perm(w[i >> 2] ^ 0x80808080u, 0x4b000000u, 0x7540 + (i & 3))) - 8388736.0f) * scale;
 }
 // Scale and codes of the 128 values of which this thread has V; the others are its neighbours'.  A NaN or an infinity
 // makes the block's scale one, and its values NaN.
-template <int V> __device__ __forceinline__ float encode(const float (&f)[V], int (&q)[V]) {
+template <int V> __device__ __forceinline__ float encode(const float (&f)[V], Values<int8_t, V>& u) {
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
 #pragma unroll
   for (int o = kPackBlock / V / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float scale = __fdiv_rn(__uint_as_float(m), 127.0f);
-  const bool fine = scale > 0.f && scale <= 3.0e38f;
-  // x times 1 / scale tells the code but where it lies next to a half (or 1 / scale is infinite): there the quotient does
-  const float inverse = __frcp_rn(scale);
+  uint32_t q[V];
+  if (scale >= 1e-30f && scale <= 3.0e38f) {
+    // x times 1 / scale tells the code but where it lies next to a half: there the quotient does
+    const float inverse = __frcp_rn(scale);
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    float t = f[i] * inverse, r = rintf(t);
-    if (!(fabsf(fabsf(t - r) - 0.5f) >= 1e-4f)) r = rintf(__fdiv_rn(f[i], scale));
-    q[i] = fine ? max(-127, min(127, (int)r)) : 0;
+    for (int i = 0; i < V; ++i) {
+      const float t = f[i] * inverse;
+      float whole = t + kWhole;
+      if (fabsf(t - (whole - kWhole)) > 0.4999f) whole = __fdiv_rn(f[i], scale) + kWhole;
+      q[i] = __float_as_uint(whole);
+    }
+  } else {                                          // tiny ones by the quotient; none of zeros, infinities and NaN
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      q[i] = scale > 0.f && scale <= 3.0e38f ? (uint32_t)__float2int_rn(fmaxf(-127.f, fminf(127.f, __fdiv_rn(f[i], scale)))) : 0;
   }
+  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+  for (int i = 0; i < V; i += 4)
+    w[i >> 2] = __byte_perm(__byte_perm(q[i], q[i + 1], 0x0040), __byte_perm(q[i + 2], q[i + 3], 0x0040), 0x5410);
   return scale;
 }
 
@@ -142,25 +163,63 @@ __device__ __forceinline__ int tokens_of(const ConvParams& P, int b) {
   return P.lengths ? max(0, min(P.length, P.lengths[b])) : P.length;
 }
 
-// The input at token t of a sequence, the state's before the first.
-template <typename T, bool CODES, int V>
-__device__ __forceinline__ void input_at(const ConvParams& P, int b, int t, int c, int n, bool vec, float (&f)[V]) {
-  if (t >= 0) {
+// A thread's inputs along the tokens, as memory has them: of x, or of codes and scales.  VEC: its channels are all there
+// and lie at multiples of their size.  Loads come in two steps, so that those of later tokens are under way while
+// earlier ones are worked on.
+template <typename T, bool CODES, bool VEC, int V> struct Inputs {
+  using Raw = Values<typename std::conditional<CODES, int8_t, T>::type, V>;
+  const T* x;
+  const int8_t* codes;
+  const float* scales;
+  long long step, scale_step;
+  int n;
+  __device__ Inputs(const ConvParams& P, int b, int c, int n_) : x(nullptr), codes(nullptr), scales(nullptr), n(n_) {
     if constexpr (CODES) {
-      const long long row = (long long)b * P.length + t;
-      const float scale = P.scales[row * ((P.channels + kPackBlock - 1) / kPackBlock) + c / kPackBlock];
-      load_codes<V>(P.codes + row * P.channels + c, vec, n, scale, f);
+      step = P.channels;
+      scale_step = (P.channels + kPackBlock - 1) / kPackBlock;
+      codes = P.codes + (long long)b * P.length * step + c;
+      scales = P.scales + (long long)b * P.length * scale_step + c / kPackBlock;
     } else {
-      load_values<T, V>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + t * P.x_st + c, vec, n, f);
+      step = P.x_st;
+      scale_step = 0;
+      x = reinterpret_cast<const T*>(P.x) + b * P.x_sb + c;
     }
-  } else if (P.state_in && t >= 1 - P.taps) {
-    const long long at = ((long long)b * (P.taps - 1) + t + P.taps - 1) * P.channels + c;
-    load_values<T, V>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = 0.f;
   }
-}
+  __device__ __forceinline__ Raw load(int t, bool take, float& scale) const {
+    Raw u;
+    if constexpr (CODES) {
+      scale = take ? scales[t * scale_step] : 0.f;
+      if (take) u = raw_values<int8_t, V>(codes + t * step, VEC, n);
+      else u = Raw{};
+    } else {
+      if (take) u = raw_values<T, V>(x + t * step, VEC, n);
+      else u = no_values<T, V>();
+    }
+    return u;
+  }
+  static __device__ __forceinline__ void get(const Raw& u, float scale, float (&f)[V]) {
+    if constexpr (CODES) {
+      decode<V>(u, scale, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = to_f32(u.v[i]);
+    }
+  }
+  // The input at any token, the state's before the first.
+  __device__ void at(const ConvParams& P, int b, int t, int c, float (&f)[V]) const {
+    if (t >= 0) {
+      float scale = 0.f;
+      const Raw u = load(t, true, scale);
+      get(u, scale, f);
+    } else if (P.state_in && t >= 1 - P.taps) {
+      const long long at = ((long long)b * (P.taps - 1) + t + P.taps - 1) * P.channels + c;
+      load_values<T, V>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = 0.f;
+    }
+  }
+};
 
 // z of a token whose last four inputs are x[0..3], oldest first.  Taps that are not there are passed over, not
 // multiplied by zero: their inputs may be infinite.
@@ -172,135 +231,160 @@ __device__ __forceinline__ float conv_at(const Taps<WT, V>& W, int taps, int i, 
   return (z + W.w[2][i] * x2) + W.w[3][i] * x3;
 }
 
-struct ConvFlags { int vec_in, vec_out, vec_codes; };
-
 // MODE: 0 reads the input, 1 keeps it in 8 bits besides, 2 reads what was kept.
-template <typename T, typename WT, int MODE>
-__global__ void __launch_bounds__(kThreads) conv_kernel(const ConvParams P, const ConvFlags F, int strip) {
-  constexpr int V = kWide;
+template <typename T, typename WT, int MODE, bool VEC>
+__global__ void __launch_bounds__(kThreads, 8) conv_kernel(const ConvParams P, int strip) {
+  constexpr int V = kWide, U = 4;                                      // U: tokens whose loads are in flight together
   constexpr bool KEEP = MODE == 1, CODES = MODE == 2;
   const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
   const int n = min(V, P.channels - c);                                // may be negative: shuffles need every lane
   if (!KEEP && n <= 0) return;
-  const bool vec_in = (CODES ? F.vec_codes : F.vec_in) && n == V, vec_out = F.vec_out && n == V, vec_codes = F.vec_codes && n == V;
-  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip);
-  T* y = reinterpret_cast<T*>(P.y) + b * P.y_sb + c;
+  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip), end = min(t1, len);
+  const Inputs<T, CODES, VEC, V> in(P, b, n > 0 ? c : 0, n);
+  T* y = reinterpret_cast<T*>(P.y) + b * P.y_sb + (long long)t0 * P.y_st + c;
   const int blocks = (P.channels + kPackBlock - 1) / kPackBlock;
-  float x[kTaps][V];
+  int8_t* codes = KEEP ? P.codes + ((long long)b * P.length + t0) * P.channels + c : nullptr;
+  float* scales = KEEP ? P.scales + ((long long)b * P.length + t0) * blocks + c / kPackBlock : nullptr;
   if (n > 0 && blockIdx.x == 0 && P.state_out) {                       // the last inputs
     for (int j = 0; j < P.taps - 1; ++j) {
-      input_at<T, CODES, V>(P, b, len - (P.taps - 1) + j, c, n, vec_in, x[0]);
-      store_values<T, V>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (P.taps - 1) + j) * P.channels + c, false, n, x[0]);
+      float f[V];
+      in.at(P, b, len - (P.taps - 1) + j, c, f);
+      store_values<T, V>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (P.taps - 1) + j) * P.channels + c, false, n, f);
     }
   }
-  if (t0 < len) {
-    const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
+  if (t0 < end) {
+    float x[kTaps - 1][V], scale[U];
+    typename Inputs<T, CODES, VEC, V>::Raw now[U];
 #pragma unroll
-    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES, V>(P, b, n > 0 ? t0 - (kTaps - 1) + k : -kTaps, c, n, vec_in, x[k]);
-    constexpr int U = 4;                                               // tokens whose loads are in flight together
-    for (int t = t0; t < min(t1, len); t += U) {
-      float next[U][V];
+    for (int j = 0; j < U; ++j) now[j] = in.load(t0 + j, n > 0 && t0 + j < end, scale[j]);
+    const Taps<WT, V> W(P.weight, P.bias, P.taps, n > 0 ? c : 0, n);
 #pragma unroll
-      for (int j = 0; j < U; ++j)
-        input_at<T, CODES, V>(P, b, n > 0 && t + j < min(t1, len) ? t + j : -kTaps, c, n, vec_in, next[j]);
+    for (int k = 0; k < kTaps - 1; ++k) {
+      if (n > 0) in.at(P, b, t0 - (kTaps - 1) + k, c, x[k]);
+    }
+    for (int t = t0; t < end; t += U) {
+      typename Inputs<T, CODES, VEC, V>::Raw next[U];
+      float later[U];
+#pragma unroll
+      for (int j = 0; j < U; ++j) next[j] = in.load(t + U + j, n > 0 && t + U + j < end, later[j]);
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const bool in = t + j < min(t1, len);
-        float out[V];
+        const bool there = n > 0 && t + j < end;
+        float out[V], f[V];
+        in.get(now[j], scale[j], f);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
+          const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], f[i]);
           out[i] = P.silu ? z * sigmoid<T>(z) : z;
-          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = next[j][i];
+          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
         }
-        if (in && n > 0) store_values<T, V>(y + (t + j) * P.y_st, vec_out, n, out);
+        if (there) store_values<T, V>(y, VEC, n, out);
+        y += P.y_st;
         if constexpr (KEEP) {
-          int q[V];
-          const float scale = encode<V>(next[j], q);
-          const long long row = (long long)b * P.length + t + j;
-          if (in && n > 0) {
-            store_codes<V>(P.codes + row * P.channels + c, vec_codes, n, q);
-            if ((c & (kPackBlock - 1)) == 0) P.scales[row * blocks + c / kPackBlock] = scale;
+          Values<int8_t, V> q;
+          const float s = encode<V>(f, q);
+          if (there) {
+            store_codes<V>(codes, VEC, n, q);
+            if ((threadIdx.x & 31) == 0) *scales = s;
           }
+          codes += P.channels;
+          scales += blocks;
         }
+        now[j] = next[j];
+        scale[j] = later[j];
       }
     }
   }
   if (n <= 0) return;
   const float zero[V] = {};
+  y = reinterpret_cast<T*>(P.y) + b * P.y_sb + c;
   for (int t = max(t0, len); t < t1; ++t) {
-    store_values<T, V>(y + t * P.y_st, vec_out, n, zero);
+    store_values<T, V>(y + t * P.y_st, VEC, n, zero);
     if constexpr (KEEP) {
       const long long row = (long long)b * P.length + t;
-      const int none[V] = {};
-      store_codes<V>(P.codes + row * P.channels + c, vec_codes, n, none);
-      if ((c & (kPackBlock - 1)) == 0) P.scales[row * blocks + c / kPackBlock] = 0.f;
+      store_codes<V>(P.codes + row * P.channels + c, VEC, n, Values<int8_t, V>{});
+      if ((threadIdx.x & 31) == 0) P.scales[row * blocks + c / kPackBlock] = 0.f;
     }
   }
 }
 
 // A strip's gradients: dz_t = dy_t y'(z_t), dx_t = sum_k w_k dz_{t + taps-1 - k}, and the strip's sums of dz_t x_{t - (taps-1) + k}
 // and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.
-template <typename T, typename WT, bool CODES>
-__global__ void __launch_bounds__(kThreads) conv_grad_kernel(const ConvParams P, const ConvFlags F, int strip) {
-  constexpr int V = kWide;
+template <typename T, typename WT, bool CODES, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams P, int strip) {
+  constexpr int V = kWide, U = 4;
   const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
   const int n = min(V, P.channels - c);
   if (n <= 0) return;
-  const bool vec_in = (CODES ? F.vec_codes : F.vec_in) && n == V, vec_out = F.vec_out && n == V;
-  const bool vec_dx = n == V && P.channels % V == 0 && ((uintptr_t)P.dx & (V * sizeof(T) - 1)) == 0;
-  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip);
+  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip), back = P.taps - 1;
+  const Inputs<T, CODES, VEC, V> in(P, b, c, n);
   const T* dy = reinterpret_cast<const T*>(P.dy) + b * P.dy_sb + c;
   T* dx = reinterpret_cast<T*>(P.dx) + (long long)b * P.length * P.channels + c;
-  const int back = P.taps - 1;
   float dw[kTaps][V] = {}, db[V] = {};
   if (t0 < len || t0 == 0) {
-    const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
-    float x[kTaps - 1][V], dz[kTaps][V] = {};
+    const int stop = t1 + kTaps - 1, end = min(stop, len);
+    float x[kTaps - 1][V], dz[kTaps - 1][V] = {}, scale[U];
+    typename Inputs<T, CODES, VEC, V>::Raw now[U];
+    Values<T, V> up[U];
+    auto load_up = [&](int t) {
+      Values<T, V> u;
+      if (t < end) u = raw_values<T, V>(dy + t * P.dy_st, VEC, n);
+      else u = no_values<T, V>();
+      return u;
+    };
 #pragma unroll
-    for (int k = 0; k < kTaps - 1; ++k) input_at<T, CODES, V>(P, b, t0 - (kTaps - 1) + k, c, n, vec_in, x[k]);
-    constexpr int U = 4;
-    for (int t = t0; t < t1 + kTaps - 1; t += U) {
-      float next[U][V], up[U][V];
+    for (int j = 0; j < U; ++j) {
+      now[j] = in.load(t0 + j, t0 + j < end, scale[j]);
+      up[j] = load_up(t0 + j);
+    }
+    const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
+#pragma unroll
+    for (int k = 0; k < kTaps - 1; ++k) in.at(P, b, t0 - (kTaps - 1) + k, c, x[k]);
+    T* put = dx + (long long)(t0 - (kTaps - 1)) * P.channels;          // of the token whose input's gradient is whole next
+    for (int t = t0; t < stop; t += U) {
+      typename Inputs<T, CODES, VEC, V>::Raw next[U];
+      Values<T, V> up_next[U];
+      float later[U];
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const bool in = t + j < min(t1 + kTaps - 1, len);
-        input_at<T, CODES, V>(P, b, in ? t + j : -kTaps, c, n, vec_in, next[j]);
-        if (in) {
-          load_values<T, V>(dy + (t + j) * P.dy_st, vec_out, n, up[j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) up[j][i] = 0.f;
-        }
+        next[j] = in.load(t + U + j, t + U + j < end, later[j]);
+        up_next[j] = load_up(t + U + j);
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int at = t + j, to = at - (kTaps - 1);                   // the token whose input's gradient is whole now
-        const bool in = at < len, mine = in && at < t1;
-        float out[V];
+        const int at = t + j, to = at - (kTaps - 1);
+        const bool mine = at < min(t1, len);
+        float f[V], out[V];
+        in.get(now[j], scale[j], f);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float d = up[j][i];
-          if (in && P.silu) {
-            const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], next[j][i]);
+          float d = to_f32(up[j].v[i]);
+          if (P.silu) {
+            const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], f[i]);
             const float s = sigmoid<T>(z);
             d *= s * (1.0f + z * (1.0f - s));
           }
-          dz[0][i] = dz[1][i]; dz[1][i] = dz[2][i]; dz[2][i] = dz[3][i]; dz[3][i] = d;
+          if (at >= end) d = 0.f;                                      // z of what is not there may be anything
           if (mine) {
             db[i] += d;
             if (P.taps > 3) dw[0][i] += d * x[0][i];
             if (P.taps > 2) dw[1][i] += d * x[1][i];
             dw[2][i] += d * x[2][i];
-            dw[3][i] += d * next[j][i];
+            dw[3][i] += d * f[i];
           }
-          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = next[j][i];
-          // dz[0..3] are those of `to` .. `to` + 3
+          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
+          // dz[0..2] and d are those of `to` .. `to` + 3
           float g = W.w[3][i] * dz[0][i] + W.w[2][i] * dz[1][i];
           if (P.taps > 2) g += W.w[1][i] * dz[2][i];
-          if (P.taps > 3) g += W.w[0][i] * dz[3][i];
+          if (P.taps > 3) g += W.w[0][i] * d;
+          dz[0][i] = dz[1][i]; dz[1][i] = dz[2][i]; dz[2][i] = d;
           out[i] = g;
         }
+        now[j] = next[j];
+        scale[j] = later[j];
+        up[j] = up_next[j];
+        T* here = put;
+        put += P.channels;
         if (to >= t1 || to < (t0 == 0 ? -back : t0)) continue;
         if (P.dstate_out && to >= len - back && to < len) {
           float late[V];
@@ -310,7 +394,7 @@ __global__ void __launch_bounds__(kThreads) conv_grad_kernel(const ConvParams P,
           for (int i = 0; i < V; ++i) out[i] += late[i];
         }
         if (to >= 0) {
-          if (to < len) store_values<T, V>(dx + (long long)to * P.channels, vec_dx, n, out);
+          if (to < len) store_values<T, V>(here, VEC, n, out);
         } else if (P.dstate_in) {
           store_values<T, V>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
         }
@@ -318,16 +402,11 @@ __global__ void __launch_bounds__(kThreads) conv_grad_kernel(const ConvParams P,
     }
   }
   const float zero[V] = {};
-  for (int t = max(t0, len); t < t1; ++t) store_values<T, V>(dx + (long long)t * P.channels, vec_dx, n, zero);
+  for (int t = max(t0, len); t < t1; ++t) store_values<T, V>(dx + (long long)t * P.channels, VEC, n, zero);
   if (P.dweight || P.dbias) {
     float* part = P.workspace + ((long long)b * gridDim.x + blockIdx.x) * (kTaps + 1) * P.channels + c;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) {
-#pragma unroll
-        for (int k = 0; k < kTaps; ++k) part[(long long)k * P.channels + i] = dw[k][i];
-        part[(long long)kTaps * P.channels + i] = db[i];
-      }
+    for (int k = 0; k <= kTaps; ++k) store_values<float, V>(part + (long long)k * P.channels, VEC, n, k < kTaps ? dw[k] : db);
   }
 }
 
@@ -393,25 +472,23 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const ConvStepParam
 // Rows in 8 bits: a thread has 16 bytes of the input, kRows rows at a time.
 constexpr int kRows = 4;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams P, int vec, int vec_codes) {
+__global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P, int vec, int vec_codes) {
   constexpr int V = kUnit<T>;
   const int c = (blockIdx.x * kThreads + threadIdx.x) * V;
   const int n = min(V, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
   for (long long r0 = (long long)blockIdx.y * kRows; r0 < P.rows; r0 += (long long)gridDim.y * kRows) {
-    float f[kRows][V];
+    Values<T, V> x[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j)
+      x[j] = n > 0 && r0 + j < P.rows ? raw_values<T, V>(reinterpret_cast<const T*>(P.x) + (r0 + j) * P.x_stride + c, vec && n == V, n)
+                                      : no_values<T, V>();
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      if (n > 0 && r0 + j < P.rows) {
-        load_values<T, V>(reinterpret_cast<const T*>(P.x) + (r0 + j) * P.x_stride + c, vec && n == V, n, f[j]);
-      } else {
+      float f[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) f[j][i] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < kRows; ++j) {
-      int q[V];
-      const float scale = encode<V>(f[j], q);
+      for (int i = 0; i < V; ++i) f[i] = to_f32(x[j].v[i]);
+      Values<int8_t, V> q;
+      const float scale = encode<V>(f, q);
       if (n > 0 && r0 + j < P.rows) {
         store_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, q);
         if ((c & (kPackBlock - 1)) == 0) P.scales[(r0 + j) * blocks + c / kPackBlock] = scale;
@@ -420,21 +497,27 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(const PackParams P, int 
   }
 }
 template <typename T>
-__global__ void __launch_bounds__(kThreads) unpack_kernel(const PackParams P, int vec, int vec_codes) {
+__global__ void __launch_bounds__(kThreads, 12) unpack_kernel(const PackParams P, int vec, int vec_codes) {
   constexpr int V = kUnit<T>;
   const int c = (blockIdx.x * kThreads + threadIdx.x) * V;
   const int n = min(V, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
   if (n <= 0) return;
   for (long long r0 = (long long)blockIdx.y * kRows; r0 < P.rows; r0 += (long long)gridDim.y * kRows) {
-    float f[kRows][V], scale[kRows];
+    float scale[kRows];
+    Values<int8_t, V> q[kRows];
 #pragma unroll
-    for (int j = 0; j < kRows; ++j) scale[j] = r0 + j < P.rows ? P.scales[(r0 + j) * blocks + c / kPackBlock] : 0.f;
+    for (int j = 0; j < kRows; ++j) {
+      const bool in = r0 + j < P.rows;
+      scale[j] = in ? P.scales[(r0 + j) * blocks + c / kPackBlock] : 0.f;
+      q[j] = in ? raw_values<int8_t, V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n) : Values<int8_t, V>{};
+    }
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      if (r0 + j < P.rows) load_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, scale[j], f[j]);
-#pragma unroll
-    for (int j = 0; j < kRows; ++j)
-      if (r0 + j < P.rows) store_values<T, V>(reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c, vec && n == V, n, f[j]);
+      if (r0 + j < P.rows) {
+        float f[V];
+        decode<V>(q[j], scale[j], f);
+        store_values<T, V>(reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c, vec && n == V, n, f);
+      }
   }
 }
 
@@ -469,14 +552,15 @@ long long conv_workspace(int batch, int length, int channels) {
 int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
   const int strip = strip_of(P.batch, P.length, P.channels, 16, 64), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
-  const ConvFlags F{P.x && whole(P.x, P.type, kWide, P.x_sb, P.x_st), whole(P.y, P.type, kWide, P.y_sb, P.y_st),
-                    P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0};
+  const bool vec = (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) && whole(P.y, P.type, kWide, P.y_sb, P.y_st) &&
+                   P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0;
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
-    if (!P.codes) conv_kernel<T, WT, 0><<<grid, kThreads, 0, st>>>(P, F, strip);
-    else if (P.x) conv_kernel<T, WT, 1><<<grid, kThreads, 0, st>>>(P, F, strip);
-    else conv_kernel<T, WT, 2><<<grid, kThreads, 0, st>>>(P, F, strip);
+    const int mode = !P.codes ? 0 : P.x ? 1 : 2;
+    if (mode == 0) vec ? conv_kernel<T, WT, 0, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 0, false><<<grid, kThreads, 0, st>>>(P, strip);
+    else if (mode == 1) vec ? conv_kernel<T, WT, 1, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 1, false><<<grid, kThreads, 0, st>>>(P, strip);
+    else vec ? conv_kernel<T, WT, 2, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 2, false><<<grid, kThreads, 0, st>>>(P, strip);
     return launch_status();
   });
 }
@@ -484,13 +568,13 @@ int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
 int launch_conv_backward(const ConvParams& P, cudaStream_t st) {
   const int strip = strip_of(P.batch, P.length, P.channels, kLeast, kMost), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
-  const ConvFlags F{P.x && whole(P.x, P.type, kWide, P.x_sb, P.x_st), whole(P.dy, P.type, kWide, P.dy_sb, P.dy_st),
-                    P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0};
+  const bool vec = (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) && whole(P.dy, P.type, kWide, P.dy_sb, P.dy_st) &&
+                   whole(P.dx, P.type, kWide, P.channels) && whole(P.workspace, 2, kWide, 0) && ((uintptr_t)P.codes & (kWide - 1)) == 0;
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
-    if (P.codes) conv_grad_kernel<T, WT, true><<<grid, kThreads, 0, st>>>(P, F, strip);
-    else conv_grad_kernel<T, WT, false><<<grid, kThreads, 0, st>>>(P, F, strip);
+    if (P.codes) vec ? conv_grad_kernel<T, WT, true, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, true, false><<<grid, kThreads, 0, st>>>(P, strip);
+    else vec ? conv_grad_kernel<T, WT, false, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, false, false><<<grid, kThreads, 0, st>>>(P, strip);
     if (int s = launch_status()) return s;
     if (P.dweight || P.dbias) {
       conv_weights_kernel<WT><<<dim3((P.channels + 31) / 32, kTaps + 1), 256, 0, st>>>(P, (int)grid.x * P.batch);

@@ -1200,39 +1200,42 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
 }
 
 // ---------------------------------------------------------------- sums behind the gradients
-// One CTA: a chunk of 32 heads.  The gradient of dt, and the chunk's sum for the bias.
+// One CTA: a chunk of eight heads, a warp a head, four tokens a lane.  The gradient of dt, and the chunk's sum for the bias.
 template <typename T>
-__global__ void __launch_bounds__(128) finish_dt_kernel(const SelectiveParams P, const Space W) {
-  __shared__ float grad[Q][33];
-  const int c = blockIdx.x, h0 = blockIdx.y * 32, b = blockIdx.z, lane = threadIdx.x & 31;
-  const int len = tokens_of(P, b);
-  for (int k = threadIdx.x >> 5; k < 32 && h0 + k < P.heads; k += 4) {
-    const int h = h0 + k;
+__global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectiveParams P, const Space W) {
+  __shared__ float grad[kPrepHeads][Q + 4];
+  const int c = blockIdx.x, h0 = blockIdx.y * kPrepHeads, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int h = h0 + warp, rows = min(Q, tokens_of(P, b) - c * Q);
+  if (h < P.heads) {
+    const long long row = (long long)b * P.heads + h;
     const float rate = P.A[h];
-    float db = 0.f;
-    for (int i = 0; i < 4; ++i) {
-      const int t = i * 32 + lane, token = c * Q + t;
-      float out = 0.f;
-      if (token < len) {
-        const float slope = W.rec[(((long long)b * P.heads + h) * W.nc + c) * (4 * Q) + 3 * Q + t];
-        float ga = 0.f, gs = 0.f;
-        for (int p = 0; p < W.ptiles; ++p) {
-          const float2 v = W.parts[((long long)b * W.units + h * W.ptiles + p) * W.lp + token];
-          ga += v.x;
-          gs += v.y;
-        }
-        out = (rate * ga + gs) * slope;
-        db += out;
+    const float4 slope = *(reinterpret_cast<const float4*>(W.rec + (row * W.nc + c) * (4 * Q) + 3 * Q) + lane);
+    float out[4] = {0.f, 0.f, 0.f, 0.f};
+    if (4 * lane < rows) {
+      float4 ga = make_float4(0.f, 0.f, 0.f, 0.f), gs = ga;
+      for (int p = 0; p < W.ptiles; ++p) {
+        const float4* v = reinterpret_cast<const float4*>(W.parts + ((long long)b * W.units + h * W.ptiles + p) * W.lp + (long long)c * Q + 4 * lane);
+        const float4 u = v[0], w = v[1];
+        ga.x += u.x; gs.x += u.y; ga.y += u.z; gs.y += u.w;
+        ga.z += w.x; gs.z += w.y; ga.w += w.z; gs.w += w.w;
       }
-      grad[t][k] = out;
+      out[0] = (rate * ga.x + gs.x) * slope.x;
+      out[1] = (rate * ga.y + gs.y) * slope.y;
+      out[2] = (rate * ga.z + gs.z) * slope.z;
+      out[3] = (rate * ga.w + gs.w) * slope.w;
+#pragma unroll
+      for (int i = 1; i < 4; ++i)
+        if (4 * lane + i >= rows) out[i] = 0.f;
     }
-    db = warp_sum(db);
+    const float db = warp_sum((out[0] + out[1]) + (out[2] + out[3]));
     if (lane == 0) W.bias_sums[((long long)b * W.nc + c) * P.heads + h] = db;
+    *reinterpret_cast<float4*>(&grad[warp][4 * lane]) = make_float4(out[0], out[1], out[2], out[3]);
   }
   __syncthreads();
-  T* ddt = reinterpret_cast<T*>(P.ddt) + (long long)b * P.length * P.heads;
-  for (int t = threadIdx.x >> 5; t < Q && c * Q + t < P.length; t += 4)
-    if (h0 + lane < P.heads) ddt[(long long)(c * Q + t) * P.heads + h0 + lane] = from_f32<T>(grad[t][lane]);
+  T* ddt = reinterpret_cast<T*>(P.ddt) + ((long long)b * P.length + (long long)c * Q) * P.heads + h0;
+  const int hl = threadIdx.x & 7;
+  for (int t = threadIdx.x >> 3; t < Q && c * Q + t < P.length; t += 32)
+    if (h0 + hl < P.heads) ddt[(long long)t * P.heads + hl] = from_f32<T>(grad[hl][t]);
 }
 
 // One warp a head: gradients of A, the bias and D.
@@ -1404,7 +1407,7 @@ template <typename T> int backward(const SelectiveParams& P, cudaStream_t st) {
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
   grad_kernel<T><<<dim3(W.nc, P.groups * W.splits, P.batch), kGradThreads, kGradSmem, st>>>(P, W, per);
   if (int s = launch_status()) return s;
-  finish_dt_kernel<T><<<dim3(W.nc, (P.heads + 31) / 32, P.batch), 128, 0, st>>>(P, W);
+  finish_dt_kernel<T><<<dim3(W.nc, (P.heads + kPrepHeads - 1) / kPrepHeads, P.batch), kThreads, 0, st>>>(P, W);
   if (int s = launch_status()) return s;
   finish_heads_kernel<<<(P.heads + 3) / 4, 128, 0, st>>>(P, W);
   if (int s = launch_status()) return s;
