@@ -35,6 +35,7 @@ constexpr int Q = kScanChunk;
 constexpr int TP = kScanTile;
 constexpr int kN = 128;
 constexpr int kThreads = 256;
+constexpr int kRecord = 7;                                 // numbers that a token of a head has
 constexpr uint32_t kTile128 = 32768, kTile64 = 16384;      // bytes of a [128][128] and a [128][64] 16-bit tile
 
 // ---------------------------------------------------------------- operands in shared memory
@@ -134,22 +135,35 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v) {
   if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
   else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
-template <typename T> __device__ __forceinline__ void unpack8(uint4 u, float (&f)[8]) {
-  const float2 a = unpack2<T>(u.x), b = unpack2<T>(u.y), c = unpack2<T>(u.z), d = unpack2<T>(u.w);
-  f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
+// Eight numbers are worked on as four pairs: the adders and multipliers take two fp32 numbers an instruction.
+struct Eight { float2 v[4]; };
+template <typename T> __device__ __forceinline__ Eight unpack8(uint4 u) {
+  return {{unpack2<T>(u.x), unpack2<T>(u.y), unpack2<T>(u.z), unpack2<T>(u.w)}};
 }
-template <typename T> __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
+template <typename T> __device__ __forceinline__ uint4 pack8(const Eight& f) {
+  return make_uint4(pack2<T>(f.v[0].x, f.v[0].y), pack2<T>(f.v[1].x, f.v[1].y), pack2<T>(f.v[2].x, f.v[2].y), pack2<T>(f.v[3].x, f.v[3].y));
+}
+__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 words2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return __ffma2_rn(b, pair(-1.f), a); }
+__device__ __forceinline__ Eight mul8(const Eight& a, float f) {
+  return {{mul2(a.v[0], pair(f)), mul2(a.v[1], pair(f)), mul2(a.v[2], pair(f)), mul2(a.v[3], pair(f))}};
 }
 // Value and remainder of eight numbers.
-template <typename T> __device__ __forceinline__ void split8(const float (&f)[8], uint4& hi, uint4& lo) {
+template <typename T> __device__ __forceinline__ void split8(const Eight& f, uint4& hi, uint4& lo) {
   hi = pack8<T>(f);
-  float r[8];
-  unpack8<T>(hi, r);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = f[i] - r[i];
-  lo = pack8<T>(r);
+  const Eight r = unpack8<T>(hi);
+  lo = pack8<T>({{sub2(f.v[0], r.v[0]), sub2(f.v[1], r.v[1]), sub2(f.v[2], r.v[2]), sub2(f.v[3], r.v[3])}});
 }
+// The largest magnitude of two by two 16-bit numbers; NaN is passed over.
+__device__ __forceinline__ __half2 fold(__half2 m, uint32_t v) { return __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&v))); }
+__device__ __forceinline__ __nv_bfloat162 fold(__nv_bfloat162 m, uint32_t v) { return __hmax2(m, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v))); }
+template <typename T> struct Two;
+template <> struct Two<__half> { using type = __half2; };
+template <> struct Two<__nv_bfloat16> { using type = __nv_bfloat162; };
 
 // The power of two that brings `bits` (a maximum's, sign cleared) to [2^13, 2^14) and its inverse: {there, back}.
 __device__ __forceinline__ float2 scale_of(uint32_t bits, int most = 60) {
@@ -178,7 +192,7 @@ __device__ __forceinline__ int tokens_of(const SelectiveParams& P, int b) {
 struct Space {
   int nc, ptiles, units;              // chunks of the longest sequence, tiles of a head's rows, heads * ptiles
   long long lp;
-  float* rec;                         // [B][H][nc][4][Q]: s, l (value, remainder; base 2), sigmoid(dt + bias)
+  float* rec;                         // [B][H][nc][kRecord][Q], see prepare_kernel
   float* smax;                        // [B][H][nc]: the largest s of a chunk
   uint16_t *bt, *ct;                  // [B][nc][G][128][128]: B and C as shared memory holds them
   float *bback, *cback;               // [B][nc][G]: what brings them back
@@ -214,7 +228,7 @@ Space space_of(const SelectiveParams& P, bool backward) {
   char* base = reinterpret_cast<char*>(P.workspace);
   long long at = 0;
   auto take = [&](long long bytes) { char* p = base + at; at += (bytes + 255) / 256 * 256; return p; };
-  w.rec = reinterpret_cast<float*>(take(bh * w.lp * 16));
+  w.rec = reinterpret_cast<float*>(take(bh * w.lp * kRecord * 4));
   w.bt = reinterpret_cast<uint16_t*>(take(bc * P.groups * kTile128));
   w.ct = reinterpret_cast<uint16_t*>(take(bc * P.groups * kTile128));
   w.bback = reinterpret_cast<float*>(take(bc * P.groups * 4));
@@ -367,11 +381,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
     char* out = reinterpret_cast<char*>((i & 1 ? W.ct : W.bt) + at * (Q * kN));
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      float f[8];
-      unpack8<T>(u[k], f);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= sc.x;
-      *reinterpret_cast<uint4*>(out + piece2((threadIdx.x >> 4) + k * 16, j)) = pack8<__half>(f);
+      *reinterpret_cast<uint4*>(out + piece2((threadIdx.x >> 4) + k * 16, j)) = pack8<__half>(mul8(unpack8<T>(u[k]), sc.x));
     }
     if (threadIdx.x == 0) (i & 1 ? W.cback : W.bback)[at] = sc.y;
     return;
@@ -413,12 +423,24 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
     hi[i] = (float)(before + l[i]);
     lo[i] = (float)(before + l[i] - (double)hi[i]);
   }
+  // The chunk in blocks of 32 tokens: l from the block's beginning (the l before its first token) and to its end
+  const double begin = __shfl_sync(0xffffffffu, before, lane & 24), finish = __shfl_sync(0xffffffffu, before + l[3], lane | 7);
+  float in_block[4], since[4], until[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    in_block[i] = (float)(before + l[i] - begin);
+    since[i] = exp2f(in_block[i]);
+    until[i] = s[i] * exp2f((float)(finish - (before + l[i])));
+  }
   const long long row = ((long long)b * P.heads + h) * W.nc + c;
-  float4* out = reinterpret_cast<float4*>(W.rec + row * (4 * Q)) + lane;
-  out[0] = s4;
-  out[Q / 4] = make_float4(hi[0], hi[1], hi[2], hi[3]);
-  out[2 * Q / 4] = make_float4(lo[0], lo[1], lo[2], lo[3]);
-  out[3 * Q / 4] = *reinterpret_cast<const float4*>(&slope[warp][4 * lane]);
+  float4* out = reinterpret_cast<float4*>(W.rec + row * (kRecord * Q)) + lane;
+  out[0] = s4;                                                               // s
+  out[Q / 4] = make_float4(hi[0], hi[1], hi[2], hi[3]);                      // l in base 2, value
+  out[2 * Q / 4] = make_float4(lo[0], lo[1], lo[2], lo[3]);                  // and remainder
+  out[3 * Q / 4] = make_float4(until[0], until[1], until[2], until[3]);      // s 2^(l at the block's end - l)
+  out[4 * Q / 4] = make_float4(since[0], since[1], since[2], since[3]);      // 2^(l - l before the block)
+  out[5 * Q / 4] = make_float4(in_block[0], in_block[1], in_block[2], in_block[3]);
+  out[6 * Q / 4] = *reinterpret_cast<const float4*>(&slope[warp][4 * lane]); // sigmoid(dt + bias)
   const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]))));
   if (lane == 0) W.smax[row] = __uint_as_float(m);
 }
@@ -450,19 +472,19 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
   const bool tok_vec = vector_ok(tok, tok_st, 0, cols);
   const uint16_t* tiles = (REV ? W.ct : W.bt) + ((long long)b * W.nc * P.groups + g) * (Q * kN);
   const float* tile_back = (REV ? W.cback : W.bback) + (long long)b * W.nc * P.groups + g;
-  const float* recs = W.rec + ((long long)b * P.heads + h) * W.lp * 4;
+  const float* recs = W.rec + ((long long)b * P.heads + h) * W.nc * (kRecord * Q);
   const long long state_at = (((long long)b * P.heads + h) * P.dim + p0) * kN + n;
   if (threadIdx.x < 4) tops[threadIdx.x] = 0;
   const uint32_t tmem = tensor_begin<64>(bars, 3, slot);
-  Gate done{smem_u32(bars), 0}, tile[2] = {{smem_u32(bars + 1), 0}, {smem_u32(bars + 2), 0}};
+  Gate done{smem_u32(bars), 0};
   bool ok = true;
   const uint32_t mine = tmem + ((uint32_t)quad << 21) + (uint32_t)half * 32;
 
   auto load = [&](int i) {
     const int c = REV ? nc - 1 - i : i;
     if (threadIdx.x == 0 && (i + 1 < nc || last)) {
-      mbar_expect_tx(tile[i & 1].bar, kTile128);
-      bulk_load(base + (i & 1) * kTile128, tiles + (long long)c * P.groups * (Q * kN), kTile128, tile[i & 1].bar);
+      mbar_expect_tx(smem_u32(bars + 1 + (i & 1)), kTile128);
+      bulk_load(base + (i & 1) * kTile128, tiles + (long long)c * P.groups * (Q * kN), kTile128, smem_u32(bars + 1 + (i & 1)));
     }
     load_tile<T>(base + kPassX, tok + (long long)c * Q * tok_st, tok_st, len - c * Q, cols, tok_vec);
     cp_commit();
@@ -470,53 +492,55 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
   float s, lh, ll, eh, el, back;                         // of the next chunk: my token's, the chunk's end's, the tile's
   auto load_record = [&](int i) {
     const int c = REV ? nc - 1 - i : i;
-    const float* r = recs + (long long)c * (4 * Q);
+    const float* r = recs + (long long)c * (kRecord * Q);
     s = r[n]; lh = r[Q + n]; ll = r[2 * Q + n]; eh = r[2 * Q - 1]; el = r[3 * Q - 1];
     back = tile_back[(long long)c * P.groups];
   };
   if (nc > 0) { load(0); load_record(0); }
-  float S[32];
+  float2 S[16];
 #pragma unroll
-  for (int i = 0; i < 32; ++i)
-    S[i] = first && half * 32 + i < cols ? first[state_at + (long long)(half * 32 + i) * kN] : 0.f;
-
+  for (int i = 0; i < 16; ++i) {
+    const int p = half * 32 + 2 * i;
+    S[i].x = first && p < cols ? first[state_at + (long long)p * kN] : 0.f;
+    S[i].y = first && p + 1 < cols ? first[state_at + (long long)(p + 1) * kN] : 0.f;
+  }
+  using Pair = typename Two<T>::type;
+  uint32_t parity = 0;                                   // of the tiles' barriers, a bit each
   for (int i = 0; i < nc; ++i) {
     const int c = REV ? nc - 1 - i : i;
     const long long at = ((long long)b * W.nc + c) * W.units + u;
     const bool update = i + 1 < nc || last, write = i > 0 || first;
     if (write) {
-      uint32_t m = 0;
+      float m = 0.f;
 #pragma unroll
-      for (int k = 0; k < 32; ++k) m = max(m, __float_as_uint(S[k]) & 0x7fffffffu);
-      m = __reduce_max_sync(0xffffffffu, m);
-      if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1) + 1], m);
+      for (int k = 0; k < 16; ++k) m = fmaxf(m, fmaxf(fabsf(S[k].x), fabsf(S[k].y)));
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
+      if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1) + 1], bits);
     }
     const float w = REV ? exp2f(lh + ll) : s * exp2f((eh - lh) + (el - ll)), decay = exp2f(eh + el), tback = back;
     cp_wait<0>();
     __syncthreads();
-    float v[4][8];
-    uint32_t m = 0;
+    uint4 v[4];
+    const uint32_t none = 0;
+    Pair m2 = *reinterpret_cast<const Pair*>(&none);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      unpack8<T>(lds16(base + kPassX + piece(n, half * 4 + j)), v[j]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[j][e] *= w;
-        m = max(m, __float_as_uint(v[j][e]) & 0x7fffffffu);
-      }
+      v[j] = lds16(base + kPassX + piece(n, half * 4 + j));
+      m2 = fold(fold(fold(fold(m2, v[j].x), v[j].y), v[j].z), v[j].w);
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1)], m);
+    {
+      const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(to_f32(m2.x), to_f32(m2.y)) * w));
+      if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1)], bits);
+    }
     __syncthreads();
     if (i + 1 < nc) load(i + 1);                         // all have their tokens, and the other tile was used two chunks ago
     const float2 wsc = scale_of(tops[2 * (i & 1)]), ssc = scale_of(tops[2 * (i & 1) + 1]);
     if (update) {
+      const float ws = w * wsc.x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[j][e] *= wsc.x;
         uint4 hi, lo;
-        split8<__half>(v[j], hi, lo);
+        split8<__half>(mul8(unpack8<T>(v[j]), ws), hi, lo);
         sts16(base + kPassW + piece(n, half * 4 + j), hi);
         sts16(base + kPassW + kTile64 + piece(n, half * 4 + j), lo);
       }
@@ -525,7 +549,9 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
     __syncthreads();
     if (threadIdx.x < 2) tops[2 * (i & 1) + threadIdx.x] = 0;                // read by all, used again in two chunks
     if (update && threadIdx.x == 0) {
-      tile[i & 1].wait(ok, P.err);
+      Gate tile{smem_u32(bars + 1 + (i & 1)), parity >> (i & 1) & 1};
+      tile.wait(ok, P.err);
+      parity ^= 1u << (i & 1);
       if (ok) {
         tc_fence_after();
         mma<kMn, kMn>(tmem, base + (i & 1) * kTile128, base + kPassW, idesc<__half>(TP, true, true), 8, false);
@@ -535,17 +561,15 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
     }
     if (i + 1 < nc) load_record(i + 1);
     if (write) {
-      uint16_t* out = planes + at * (2 * kN * TP);
+      uint16_t* out = planes + at * (2 * kN * TP) + ((half * 4) * kN + n) * 8;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float f[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = S[8 * j + e] * ssc.x;
+        const Eight f = mul8({{S[4 * j], S[4 * j + 1], S[4 * j + 2], S[4 * j + 3]}}, ssc.x);
         uint4 hi, lo;
         if (LO) split8<__half>(f, hi, lo);
         else hi = pack8<__half>(f);
-        *reinterpret_cast<uint4*>(out + ((half * 4 + j) * kN + n) * 8) = hi;
-        if (LO) *reinterpret_cast<uint4*>(out + kN * TP + ((half * 4 + j) * kN + n) * 8) = lo;
+        *reinterpret_cast<uint4*>(out + j * (kN * 8)) = hi;
+        if (LO) *reinterpret_cast<uint4*>(out + kN * TP + j * (kN * 8)) = lo;
       }
     }
     if (threadIdx.x == 0) scales[at] = make_float2(ssc.y, wsc.y);
@@ -557,13 +581,16 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
       tc_fence_before();
       const float f = wsc.y * tback;
 #pragma unroll
-      for (int k = 0; k < 32; ++k) S[k] = S[k] * decay + __uint_as_float(r[k]) * f;
+      for (int k = 0; k < 16; ++k) S[k] = fma2(S[k], pair(decay), mul2(words2(r[2 * k], r[2 * k + 1]), pair(f)));
     }
   }
   if (last)
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if (half * 32 + i < cols) last[state_at + (long long)(half * 32 + i) * kN] = S[i];
+    for (int i = 0; i < 16; ++i) {
+      const int p = half * 32 + 2 * i;
+      if (p < cols) last[state_at + (long long)p * kN] = S[i].x;
+      if (p + 1 < cols) last[state_at + (long long)(p + 1) * kN] = S[i].y;
+    }
   tensor_end<64>(tmem);
 }
 
@@ -573,9 +600,6 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
 // on its way as soon as its products are done.
 constexpr uint32_t kOutM = kTile128, kOutX = 2 * kTile128, kOutH = kOutX + kTile64, kOutRec = kOutH + kTile64, kRecBytes = 4 * Q * 4,
                    kOutTop = kOutRec + 2 * kRecBytes, kOutBar = kOutTop + 2 * Q * 4, kOutSmem = kOutBar + 32;
-
-__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 words2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams P, const Space W, int per) {
@@ -608,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
     if (threadIdx.x == 0) {
       mbar_expect_tx(unit.bar, kRecBytes + (has_state ? kTile64 : 0));
-      bulk_load(base + kOutRec + ((u - u0) & 1) * kRecBytes, W.rec + (((long long)b * P.heads + h) * W.nc + c) * (4 * Q), kRecBytes, unit.bar);
+      bulk_load(base + kOutRec + ((u - u0) & 1) * kRecBytes, W.rec + (((long long)b * P.heads + h) * W.nc + c) * (kRecord * Q), kRecBytes, unit.bar);
       if (has_state) bulk_load(base + kOutH, W.h + (bc * W.units + u) * (2 * kN * TP), kTile64, unit.bar);
     }
     const T* p = xc + (long long)h * P.dim + p0;
@@ -671,30 +695,37 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     for (int cb = half; cb <= quad; cb += 2) {
       uint32_t r[32];
       tmem_ld32(lanes + cb * 32, r);
+      if (cb < quad) {
+        // a block of earlier tokens: the decay to the block's end and from there on are both at most 1
+        const float from = ex2((lh - rec[Q + cb * 32 + 31]) + (ll - rec[2 * Q + cb * 32 + 31])) * sc.x;
+        const float4* until = reinterpret_cast<const float4*>(rec + 3 * Q) + cb * 8;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float f[8];
+        for (int k = 0; k < 4; ++k) {
+          Eight f;
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-          const int at = cb * 8 + k * 2 + (e >> 2);
-          const float4 s4 = reinterpret_cast<const float4*>(rec)[at], h4 = reinterpret_cast<const float4*>(rec + Q)[at],
-                       l4 = reinterpret_cast<const float4*>(rec + 2 * Q)[at];
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-            const float2 sv = i ? make_float2(s4.z, s4.w) : make_float2(s4.x, s4.y), hv = i ? make_float2(h4.z, h4.w) : make_float2(h4.x, h4.y),
-                         lv = i ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
-            const float2 gap = __fadd2_rn(__ffma2_rn(hv, pair(-1.f), pair(lh)), __ffma2_rn(lv, pair(-1.f), pair(ll)));
-            float2 v = __fmul2_rn(__fmul2_rn(make_float2(ex2(gap.x), ex2(gap.y)), sv), words2(r[k * 8 + e + i], r[k * 8 + e + i + 1]));
-            if (kScaled) v = __fmul2_rn(v, pair(sc.x));
-            f[e + i] = v.x;
-            f[e + i + 1] = v.y;
+          for (int e = 0; e < 2; ++e) {
+            const float4 v = until[k * 2 + e];
+            f.v[2 * e] = mul2(mul2(words2(r[k * 8 + 4 * e], r[k * 8 + 4 * e + 1]), pair(from)), make_float2(v.x, v.y));
+            f.v[2 * e + 1] = mul2(mul2(words2(r[k * 8 + 4 * e + 2], r[k * 8 + 4 * e + 3]), pair(from)), make_float2(v.z, v.w));
           }
+          sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<T>(f));
         }
-        if (cb == quad)
+      } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (cb * 32 + k * 8 + e > row) f[e] = 0.f;
-        sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<T>(f));
+        for (int k = 0; k < 4; ++k) {
+          Eight f;
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const int col = cb * 32 + k * 8 + e;
+            const float2 sv = *reinterpret_cast<const float2*>(rec + col), hv = *reinterpret_cast<const float2*>(rec + Q + col),
+                         lv = *reinterpret_cast<const float2*>(rec + 2 * Q + col);
+            const float2 gap = add2(sub2(pair(lh), hv), sub2(pair(ll), lv));
+            float2 v = mul2(mul2(make_float2(ex2(gap.x), ex2(gap.y)), sv), words2(r[k * 8 + e], r[k * 8 + e + 1]));
+            if (kScaled) v = mul2(v, pair(sc.x));
+            f.v[e >> 1] = make_float2(col <= row ? v.x : 0.f, col + 1 <= row ? v.y : 0.f);
+          }
+          sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<T>(f));
+        }
       }
     }
     if (quad == 0 && half == 1)                          // where the output of the unit before was laid out
@@ -719,15 +750,13 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     tc_fence_before();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float f[8];
-      unpack8<T>(x[j], f);
+      Eight f = mul8(unpack8<T>(x[j]), d);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float v = __uint_as_float(y1[j * 8 + e]) * mixed + d * f[e];
-        if (has_state) v += carry * __uint_as_float(y0[j * 8 + e]);
-        f[e] = row < rows ? v : 0.f;
+      for (int e = 0; e < 4; ++e) {
+        f.v[e] = fma2(words2(y1[j * 8 + 2 * e], y1[j * 8 + 2 * e + 1]), pair(mixed), f.v[e]);
+        if (has_state) f.v[e] = fma2(words2(y0[j * 8 + 2 * e], y0[j * 8 + 2 * e + 1]), pair(carry), f.v[e]);
       }
-      sts16(base + kOutM + piece(row, half * 4 + j), pack8<T>(f));
+      sts16(base + kOutM + piece(row, half * 4 + j), row < rows ? pack8<T>(f) : make_uint4(0, 0, 0, 0));
     }
     __syncthreads();
     T* out = y + (long long)h * P.dim + p0;
@@ -747,8 +776,9 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
 //      by row and by column.
 //   3. the pairs' part of x's gradient; prefix and suffix sums over the tokens give the gradient of A s.
 // After the last unit the group's sum gives the pairs' part of dB and dC in two products.
+constexpr uint32_t kGRecBytes = 6 * Q * 4;               // of a token's record, all but the last number
 constexpr uint32_t kGB = 0, kGC = kTile128, kGX = 2 * kTile128, kGY = kGX + kTile64, kGHigh = kGY + 2 * kTile64,
-                   kGLow = kGHigh + 2 * kTile64, kGM = kGLow + 2 * kTile64, kGRec = kGM + kTile128, kGRow = kGRec + 2 * kRecBytes,
+                   kGLow = kGHigh + 2 * kTile64, kGM = kGLow + 2 * kTile64, kGRec = kGM + kTile128, kGRow = kGRec + 2 * kGRecBytes,
                    kGCol = kGRow + 13 * Q * 4, kGRed = kGCol + 4 * Q * 4, kGBar = kGRed + 64 * 4, kGradSmem = kGBar + 48;
 constexpr int kGradThreads = 512;                  // four threads a token: sixteen warps hide each other's waits
 
@@ -807,8 +837,9 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   // One thread: the record and the states' values of a unit, and their remainders.  H lies at 0, G 16,384 bytes on.
   auto load_high = [&](int u) {
     const long long at = (bc * W.units + u) * (2 * kN * TP);
-    mbar_expect_tx(high.bar, kRecBytes + ((int)has_h + (int)has_g) * kTile64);
-    bulk_load(base + kGRec + ((u - u0) & 1) * kRecBytes, W.rec + (((long long)b * P.heads + u / W.ptiles) * W.nc + c) * (4 * Q), kRecBytes, high.bar);
+    mbar_expect_tx(high.bar, kGRecBytes + ((int)has_h + (int)has_g) * kTile64);
+    bulk_load(base + kGRec + ((u - u0) & 1) * kGRecBytes, W.rec + (((long long)b * P.heads + u / W.ptiles) * W.nc + c) * (kRecord * Q), kGRecBytes,
+              high.bar);
     if (has_h) bulk_load(base + kGHigh, W.h + at, kTile64, high.bar);
     if (has_g) bulk_load(base + kGHigh + kTile64, W.g + at, kTile64, high.bar);
   };
@@ -878,7 +909,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
 
   for (int u = u0; u < u1; ++u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
-    const float* rec = reinterpret_cast<const float*>(smem + kGRec + ((u - u0) & 1) * kRecBytes);
+    const float* rec = reinterpret_cast<const float*>(smem + kGRec + ((u - u0) & 1) * kGRecBytes);
     const uint32_t ytile = base + kGY + ((u - u0) & 1) * kTile64;
     cp_wait<0>();
     fence_async();
@@ -903,37 +934,24 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     if (has_h || has_g) { hs = W.hs[bc * W.units + u]; gs = W.gs[bc * W.units + u]; }
     const float from_in = ex2(lh + ll), to_end = ex2((eh - lh) + (el - ll));
     const float wy = has_h ? from_in * (hs.x / cscale) : 0.f, wx = has_g ? s * to_end * (gs.x / bscale) : 0.f;
-    float gh = 0.f;
+    float2 gh2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint32_t at = piece(row, part * 2 + j), plane = (uint32_t)((part * 2 + j) * kN + row) * 16;
-      float f[8], o[8];
-      if (has_h) {
-        unpack8<T>(lds16(ytile + at), f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= wy;
-        sts16(base + kGM + at, pack8<__half>(f));
-      }
-      if (has_g) {
-        unpack8<T>(lds16(base + kGX + at), f);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= wx;
-        sts16(base + kGM + kTile64 + at, pack8<__half>(f));
-      }
+      if (has_h) sts16(base + kGM + at, pack8<__half>(mul8(unpack8<T>(lds16(ytile + at)), wy)));
+      if (has_g) sts16(base + kGM + kTile64 + at, pack8<__half>(mul8(unpack8<T>(lds16(base + kGX + at)), wx)));
       if (has_h && has_g) {                              // my row of the states: <G, H>
-        float hl[8], gl[8];
-        unpack8<__half>(lds16(base + kGHigh + plane), f);
-        unpack8<__half>(lds16(base + kGLow + plane), hl);
-        unpack8<__half>(lds16(base + kGHigh + kTile64 + plane), o);
-        unpack8<__half>(lds16(base + kGLow + kTile64 + plane), gl);
+        const Eight h1 = unpack8<__half>(lds16(base + kGHigh + plane)), h2 = unpack8<__half>(lds16(base + kGLow + plane));
+        const Eight g1 = unpack8<__half>(lds16(base + kGHigh + kTile64 + plane)), g2 = unpack8<__half>(lds16(base + kGLow + kTile64 + plane));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) gh += (f[e] + hl[e]) * (o[e] + gl[e]);
+        for (int e = 0; e < 4; ++e) gh2 = fma2(add2(h1.v[e], h2.v[e]), add2(g1.v[e], g2.v[e]), gh2);
       }
     }
+    float gh = gh2.x + gh2.y;
     gh = warp_sum(gh);
     if (lane == 0) red[warp] = gh;
     fence_async();
-    float dxi[16];
+    float2 dxi[8];
     float r_part = 0.f, q_part = 0.f;
     if (has_h || has_g) {
       done.wait(ok, P.err);
@@ -942,27 +960,28 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       if (has_g) {
         tmem_ld16(lanes + 128 + part * 16, r);
         const float f = to_end * gs.x * bback;
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float x[8];
-          unpack8<T>(lds16(base + kGX + piece(row, part * 2 + j)), x);
+          const Eight x = unpack8<T>(lds16(base + kGX + piece(row, part * 2 + j)));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            dxi[j * 8 + e] = f * __uint_as_float(r[j * 8 + e]);
-            r_part += dxi[j * 8 + e] * x[e];
+          for (int e = 0; e < 4; ++e) {
+            dxi[j * 4 + e] = mul2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), pair(f));
+            sum = fma2(dxi[j * 4 + e], x.v[e], sum);
           }
         }
+        r_part = sum.x + sum.y;
       }
       if (has_h) {
         tmem_ld16(lanes + 192 + part * 16, r);
+        float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float y[8];
-          unpack8<T>(lds16(ytile + piece(row, part * 2 + j)), y);
+          const Eight y = unpack8<T>(lds16(ytile + piece(row, part * 2 + j)));
 #pragma unroll
-          for (int e = 0; e < 8; ++e) q_part += __uint_as_float(r[j * 8 + e]) * y[e];
+          for (int e = 0; e < 4; ++e) sum = fma2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), y.v[e], sum);
         }
-        q_part *= from_in * hs.x * cback;
+        q_part = (sum.x + sum.y) * (from_in * hs.x * cback);
       }
       tc_fence_before();
     }
@@ -970,7 +989,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     qstate[part * Q + row] = q_part;
     if (!has_g)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dxi[i] = 0.f;
+      for (int i = 0; i < 8; ++i) dxi[i] = make_float2(0.f, 0.f);
     __syncthreads();
     // step 2
     if (threadIdx.x == 0) {
@@ -993,61 +1012,81 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     }
     float r_sum = 0.f, diag = 0.f, pair_time = 0.f;
     const float sb = s * both_back;
-    {
-      const int cb = part;
-      if (cb >= quad) {
-        uint32_t r[32], d[32];
-        tmem_ld32_nowait(lanes + cb * 32, r);
-        tmem_ld32(lanes + 128 + cb * 32, d);
-        settle(r);
-        float e[32];
-        float2 rs2 = make_float2(0.f, 0.f), time2 = make_float2(0.f, 0.f);
+    const int cb = part;
+    if (cb >= quad) {
+      uint32_t r[32], d[32];
+      tmem_ld32_nowait(lanes + cb * 32, r);
+      tmem_ld32(lanes + 128 + cb * 32, d);
+      settle(r);
+      float e[32];
+      float2 rs2 = make_float2(0.f, 0.f), time2 = make_float2(0.f, 0.f);
+      if (cb > quad) {
+        // a block of later tokens: the decay to its beginning and from there on are both at most 1
+        const float th = rec[Q + cb * 32 - 1] - lh, tl = rec[2 * Q + cb * 32 - 1] - ll, to_block = ex2(th + tl), ds_in = s * to_block, pairs_in = sb * to_block;
+        const float mine = kScaled ? to_block * sc.x : to_block;
+        const float4 *since = reinterpret_cast<const float4*>(rec + 4 * Q) + cb * 8, *in_block = reinterpret_cast<const float4*>(rec + 5 * Q) + cb * 8;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float f[8];
+          Eight f;
 #pragma unroll
-          for (int i = 0; i < 8; i += 4) {
-            const int at = cb * 8 + j * 2 + (i >> 2);
-            const float4 h4 = reinterpret_cast<const float4*>(rec + Q)[at], l4 = reinterpret_cast<const float4*>(rec + 2 * Q)[at];
+          for (int i = 0; i < 2; ++i) {
+            const float4 w4 = since[j * 2 + i], l4 = in_block[j * 2 + i];
 #pragma unroll
-            for (int o = 0; o < 4; o += 2) {
-              const int q = j * 8 + i + o;
-              const float2 hv = o ? make_float2(h4.z, h4.w) : make_float2(h4.x, h4.y), lv = o ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
-              float2 gap = __fadd2_rn(__ffma2_rn(pair(lh), pair(-1.f), hv), __ffma2_rn(pair(ll), pair(-1.f), lv));
-              float2 w = make_float2(ex2(gap.x), ex2(gap.y));
-              if (cb == quad) {                          // pairs under the diagonal weigh nothing
-                const int t = cb * 32 + q;
-                if (t < row) { w.x = 0.f; gap.x = 0.f; }
-                if (t + 1 < row) { w.y = 0.f; gap.y = 0.f; }
-              }
-              const float2 dm = words2(d[q], d[q + 1]), m = __fmul2_rn(words2(r[q], r[q + 1]), w);
-              ds[q >> 1] = __ffma2_rn(pair(s), __fmul2_rn(dm, w), ds[q >> 1]);
-              float2 both = __fmul2_rn(m, dm);
-              if (cb == quad) {                          // no decay between a token and itself: kept out of the sums
-                const int t = cb * 32 + q;
-                if (t == row) { diag = dm.x; rself[row] = both.x * both_back; both.x = 0.f; }
-                if (t + 1 == row) { diag = dm.y; rself[row] = both.y * both_back; both.y = 0.f; }
-              }
-              rs2 = __fadd2_rn(rs2, both);
-              both = __fmul2_rn(both, pair(sb));
-              time2 = __ffma2_rn(both, gap, time2);
+            for (int o = 0; o < 2; ++o) {
+              const int q = j * 8 + i * 4 + o * 2;
+              const float2 w = o ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y), l = o ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+              const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
+              ds[q >> 1] = fma2(mul2(dm, w), pair(ds_in), ds[q >> 1]);
+              f.v[i * 2 + o] = mul2(m, pair(mine));
+              const float2 both = mul2(mul2(m, dm), pair(pairs_in));
+              rs2 = add2(rs2, both);
+              time2 = fma2(both, l, time2);
               e[q] = both.x;
               e[q + 1] = both.y;
-              f[i + o] = kScaled ? m.x * sc.x : m.x;
-              f[i + o + 1] = kScaled ? m.y * sc.x : m.y;
             }
           }
           sts16(base + kGM + piece2(row, cb * 4 + j), pack8<T>(f));
         }
-        r_sum += rs2.x + rs2.y;
-        pair_time += time2.x + time2.y;
-        qpairs[quad * Q + cb * 32 + lane] = column_sums(e, lane);
+        r_sum = rs2.x + rs2.y;                           // by s: the row's own factor
+        pair_time = (time2.x + time2.y) + r_sum * (th + tl);
       } else {
-        for (int j = 0; j < 4; ++j) sts16(base + kGM + piece2(row, cb * 4 + j), make_uint4(0, 0, 0, 0));
-        qpairs[quad * Q + cb * 32 + lane] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          Eight f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int q = j * 8 + i * 2, t = cb * 32 + q;
+            const float2 hv = *reinterpret_cast<const float2*>(rec + Q + t), lv = *reinterpret_cast<const float2*>(rec + 2 * Q + t);
+            float2 gap = add2(sub2(hv, pair(lh)), sub2(lv, pair(ll)));
+            if (t < row) gap.x = 0.f;
+            if (t + 1 < row) gap.y = 0.f;
+            float2 w = make_float2(ex2(gap.x), ex2(gap.y));
+            if (t < row) w.x = 0.f;                      // pairs under the diagonal weigh nothing
+            if (t + 1 < row) w.y = 0.f;
+            const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
+            ds[q >> 1] = fma2(pair(s), mul2(dm, w), ds[q >> 1]);
+            f.v[i] = kScaled ? mul2(m, pair(sc.x)) : m;
+            float2 both = mul2(mul2(m, dm), pair(sb));
+            if (t == row) { diag = dm.x; both.x = 0.f; } // no decay between a token and itself: kept out of the sums
+            if (t + 1 == row) { diag = dm.y; both.y = 0.f; }
+            if (t == row) rself[row] = m.x * dm.x * both_back;
+            if (t + 1 == row) rself[row] = m.y * dm.y * both_back;
+            rs2 = add2(rs2, both);
+            time2 = fma2(both, gap, time2);
+            e[q] = both.x;
+            e[q + 1] = both.y;
+          }
+          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<T>(f));
+        }
+        r_sum = rs2.x + rs2.y;
+        pair_time = time2.x + time2.y;
       }
+      qpairs[quad * Q + cb * 32 + lane] = column_sums(e, lane);
+    } else {
+      for (int j = 0; j < 4; ++j) sts16(base + kGM + piece2(row, cb * 4 + j), make_uint4(0, 0, 0, 0));
+      qpairs[quad * Q + cb * 32 + lane] = 0.f;
     }
-    rpairs[part * Q + row] = r_sum * both_back;
+    rpairs[part * Q + row] = r_sum;
     diag = warp_sum(diag);
     pair_time = warp_sum(pair_time);
     if (lane == 0) { red[16 + warp] = diag; red[32 + warp] = pair_time; }
@@ -1071,8 +1110,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
         const int t = 4 * lane + i;
         const auto four = [&](const float* v) { return (v[t] + v[Q + t]) + (v[2 * Q + t] + v[3 * Q + t]); };
         const float st = rec[t], rp = four(rpairs), rs = four(rstate), qs = four(qstate);
-        r[i] = rp + rs + rself[t];
-        a[i] = four(qpairs) + qs - st * rp;
+        r[i] = (st > 0.f ? rp / st : 0.f) + rs + rself[t];   // rp is by s, as the columns' sums are
+        a[i] = four(qpairs) + qs - rp;
         bs[i] = st * rs;
         time += qs * (rec[Q + t] + rec[2 * Q + t]) + bs[i] * ((eh - rec[Q + t]) + (el - rec[2 * Q + t]));
         sa += a[i];
@@ -1113,12 +1152,11 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t at = piece(row, part * 2 + j);
-        float f[8];
-        unpack8<T>(lds16(ytile + at), f);
+        Eight f = mul8(unpack8<T>(lds16(ytile + at)), dskip);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          f[e] = row < rows ? s * (__uint_as_float(r[j * 8 + e]) * mixed + dxi[j * 8 + e]) + dskip * f[e] : 0.f;
-        sts16(base + kGM + at, pack8<T>(f));
+        for (int e = 0; e < 4; ++e)
+          f.v[e] = fma2(fma2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), pair(mixed), dxi[j * 4 + e]), pair(s), f.v[e]);
+        sts16(base + kGM + at, row < rows ? pack8<T>(f) : make_uint4(0, 0, 0, 0));
       }
     }
     __syncthreads();
@@ -1139,14 +1177,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   const float2 all = scale_of(top);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float2 v = __fmul2_rn(ds[j * 4 + (i >> 1)], pair(all.x));
-      f[i] = v.x;
-      f[i + 1] = v.y;
-    }
-    sts16(base + kGM + piece2(row, part * 4 + j), pack8<__half>(f));
+    sts16(base + kGM + piece2(row, part * 4 + j), pack8<__half>(mul8({{ds[4 * j], ds[4 * j + 1], ds[4 * j + 2], ds[4 * j + 3]}}, all.x)));
   }
   tc_fence_before();
   fence_async();
@@ -1172,17 +1203,17 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       if (has) settle(d);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        float f[8];
+        Eight f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[e] = __uint_as_float(r[j * 8 + e]) * pairs_back;
-          if (has) f[e] += __uint_as_float(d[j * 8 + e]) * back;
-          if (row >= rows) f[e] = 0.f;
+        for (int e = 0; e < 4; ++e) {
+          f.v[e] = mul2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), pair(pairs_back));
+          if (has) f.v[e] = fma2(words2(d[j * 8 + 2 * e], d[j * 8 + 2 * e + 1]), pair(back), f.v[e]);
+          if (row >= rows) f.v[e] = make_float2(0.f, 0.f);
         }
         if (W.splits > 1) {
           float* p = sums + ((((long long)split * P.batch + b) * W.lp + (long long)c * Q + row) * P.groups + g) * kN + part * 32 + j * 8;
-          *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-          *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+          *reinterpret_cast<float4*>(p) = make_float4(f.v[0].x, f.v[0].y, f.v[1].x, f.v[1].y);
+          *reinterpret_cast<float4*>(p + 4) = make_float4(f.v[2].x, f.v[2].y, f.v[3].x, f.v[3].y);
         } else {
           sts16(base + (which ? kGHigh : kGM) + piece2(row, part * 4 + j), pack8<T>(f));
         }
@@ -1209,7 +1240,7 @@ __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectivePara
   if (h < P.heads) {
     const long long row = (long long)b * P.heads + h;
     const float rate = P.A[h];
-    const float4 slope = *(reinterpret_cast<const float4*>(W.rec + (row * W.nc + c) * (4 * Q) + 3 * Q) + lane);
+    const float4 slope = *(reinterpret_cast<const float4*>(W.rec + (row * W.nc + c) * (kRecord * Q) + 6 * Q) + lane);
     float out[4] = {0.f, 0.f, 0.f, 0.f};
     if (4 * lane < rows) {
       float4 ga = make_float4(0.f, 0.f, 0.f, 0.f), gs = ga;
