@@ -106,19 +106,22 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[3
       : "r"(taddr));
 }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  tmem_ld16_nowait(taddr, r);
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
 // Keeps uses of a tcgen05.ld's registers behind the wait that precedes this call.
-__device__ __forceinline__ void settle(uint32_t (&r)[32]) {
+template <int N> __device__ __forceinline__ void settle(uint32_t (&r)[N]) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 8)
+  for (int i = 0; i < N; i += 8)
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
@@ -208,14 +211,18 @@ struct Space {
 
 constexpr int kSms = 148;
 
-// CTAs that share a group's heads: enough for every SM (two CTAs an SM in the forward, one in the backward), and no
-// more than there are units.
-int splits_of(long long tiles, int units, int want) {
-  long long s = (want + tiles - 1) / tiles;
-  if (s > units) s = units;
-  if (s < 1) s = 1;
-  const int per = (units + (int)s - 1) / (int)s;
-  return (units + per - 1) / per;
+// CTAs that share a group's units.  A CTA's time is that of its units and of what it does once; all CTAs' time is that of
+// the rounds in which the SMs' places take them.  2 x 2,048 tokens at 128 heads, gradients: 16 units a CTA (2 rounds).
+int splits_of(long long tiles, int units, int places, double once) {
+  int best = 1;
+  double least = 1e30;
+  for (int s = 1; s <= units; ++s) {
+    const int per = (units + s - 1) / s, used = (units + per - 1) / per;
+    if (used != s) continue;
+    const double time = (double)((tiles * s + places - 1) / places) * (per + once * (s > 1 ? 1.5 : 1.0));
+    if (time < 0.999 * least) { least = time; best = s; }
+  }
+  return best;
 }
 
 Space space_of(const SelectiveParams& P, bool backward) {
@@ -237,7 +244,7 @@ Space space_of(const SelectiveParams& P, bool backward) {
   const long long plane = (long long)kN * TP * 2 * 2;
   w.h = reinterpret_cast<uint16_t*>(take(bcu * plane));
   w.hs = reinterpret_cast<float2*>(take(bcu * 8));
-  w.splits = splits_of(bc * P.groups, w.units / P.groups, backward ? kSms : 2 * kSms);
+  w.splits = splits_of(bc * P.groups, w.units / P.groups, backward ? kSms : 2 * kSms, backward ? 1.0 : 0.5);
   if (backward) {
     w.g = reinterpret_cast<uint16_t*>(take(bcu * plane));
     w.gs = reinterpret_cast<float2*>(take(bcu * 8));
@@ -347,6 +354,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams P, const Space W, int head_blocks) {
   __shared__ float step[kPrepHeads][Q + 4], slope[kPrepHeads][Q + 4];
   __shared__ uint32_t tops[kThreads / 32];
+  launch_dependents();
   const int c = blockIdx.x, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int len = tokens_of(P, b), rows = min(Q, len - c * Q);
   if ((int)blockIdx.y >= head_blocks) {
@@ -475,7 +483,9 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
   const float* recs = W.rec + ((long long)b * P.heads + h) * W.nc * (kRecord * Q);
   const long long state_at = (((long long)b * P.heads + h) * P.dim + p0) * kN + n;
   if (threadIdx.x < 4) tops[threadIdx.x] = 0;
-  const uint32_t tmem = tensor_begin<64>(bars, 3, slot);
+  launch_dependents();
+  const uint32_t tmem = tensor_begin<128>(bars, 3, slot);
+  wait_for_launch();
   Gate done{smem_u32(bars), 0};
   bool ok = true;
   const uint32_t mine = tmem + ((uint32_t)quad << 21) + (uint32_t)half * 32;
@@ -554,8 +564,8 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
       parity ^= 1u << (i & 1);
       if (ok) {
         tc_fence_after();
-        mma<kMn, kMn>(tmem, base + (i & 1) * kTile128, base + kPassW, idesc<__half>(TP, true, true), 8, false);
-        mma<kMn, kMn>(tmem, base + (i & 1) * kTile128, base + kPassW + kTile64, idesc<__half>(TP, true, true), 8, true);
+        // values and remainders side by side: a product of 128 columns takes little longer than one of 64
+        mma<kMn, kMn>(tmem, base + (i & 1) * kTile128, base + kPassW, idesc<__half>(2 * TP, true, true), 8, false);
         umma_commit(done.bar);
       }
     }
@@ -576,12 +586,18 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
     if (update) {
       done.wait(ok, P.err);
       tc_fence_after();
-      uint32_t r[32];
-      tmem_ld32(mine, r);
-      tc_fence_before();
       const float f = wsc.y * tback;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) S[k] = fma2(S[k], pair(decay), mul2(words2(r[2 * k], r[2 * k + 1]), pair(f)));
+      for (int j = 0; j < 32; j += 16) {
+        uint32_t r[16], q[16];
+        tmem_ld16_nowait(mine + j, r);
+        tmem_ld16(mine + TP + j, q);
+        settle(r);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          S[j / 2 + k] = fma2(S[j / 2 + k], pair(decay), mul2(add2(words2(r[2 * k], r[2 * k + 1]), words2(q[2 * k], q[2 * k + 1])), pair(f)));
+      }
+      tc_fence_before();
     }
   }
   if (last)
@@ -591,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
       if (p < cols) last[state_at + (long long)p * kN] = S[i].x;
       if (p + 1 < cols) last[state_at + (long long)(p + 1) * kN] = S[i].y;
     }
-  tensor_end<64>(tmem);
+  tensor_end<128>(tmem);
 }
 
 // ---------------------------------------------------------------- outputs by chunk and group
@@ -614,18 +630,21 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
   const int len = tokens_of(P, b), rows = min(Q, len - c * Q), out_rows = min(Q, P.length - c * Q);
   const int row = threadIdx.x & 127, half = threadIdx.x >> 7, quad = threadIdx.x >> 5 & 3;
   T* y = reinterpret_cast<T*>(P.y) + (long long)b * P.y_sb + (long long)c * Q * P.y_st;
+  launch_dependents();
   if (rows <= 0) {                                       // behind the sequence's end
     for (int u = u0; u < u1; ++u) {
       const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
       for (int i = threadIdx.x; i < out_rows * cols; i += kThreads)
         y[(long long)(i / cols) * P.y_st + (long long)h * P.dim + p0 + i % cols] = from_f32<T>(0.f);
     }
+    wait_for_launch();
     return;
   }
   const bool has_state = c > 0 || P.state_in;
   const long long bc = (long long)b * W.nc + c, tile_at = bc * P.groups + g;
   const T* xc = reinterpret_cast<const T*>(P.x) + (long long)b * P.x_sb + (long long)c * Q * P.x_st;
   const uint32_t tmem = tensor_begin<256>(bars, 3, reinterpret_cast<uint32_t*>(smem + kOutBar + 24));
+  wait_for_launch();
   Gate done{smem_u32(bars), 0}, tiles{smem_u32(bars + 1), 0}, unit{smem_u32(bars + 2), 0};
   bool ok = true;
   auto load_unit = [&](int u) {                          // state and record (one thread), tokens (all)
@@ -815,6 +834,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   T* dx = reinterpret_cast<T*>(P.dx) + b * P.dx_sb + (long long)c * Q * dx_st;
   const long long grp_at = b * P.dg_sb + (long long)c * Q * grp_st + g * kN;
   T *dB = reinterpret_cast<T*>(P.dB) + grp_at, *dC = reinterpret_cast<T*>(P.dC) + grp_at;
+  launch_dependents();
   if (rows <= 0) {                                       // behind the sequence's end
     for (int u = u0; u < u1; ++u) {
       const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
@@ -825,6 +845,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     if (W.splits == 1)
       for (int i = threadIdx.x; i < out_rows * kN; i += kGradThreads)
         dB[(long long)(i / kN) * grp_st + i % kN] = dC[(long long)(i / kN) * grp_st + i % kN] = from_f32<T>(0.f);
+    wait_for_launch();
     return;
   }
   const bool has_h = c > 0 || P.state_in, has_g = (c + 1) * Q < len || P.dstate_out;
@@ -832,6 +853,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   const T* yc = reinterpret_cast<const T*>(P.dy) + (long long)b * P.dy_sb + (long long)c * Q * P.dy_st;
   const uint32_t tmem = tensor_begin<512>(bars, 4, reinterpret_cast<uint32_t*>(smem + kGBar + 32));
   const uint32_t lanes = tmem + ((uint32_t)quad << 21), work = tmem + 128, sum_c = tmem + 256, sum_b = tmem + 384;
+  wait_for_launch();
   Gate done{smem_u32(bars), 0}, tiles{smem_u32(bars + 1), 0}, high{smem_u32(bars + 2), 0}, low{smem_u32(bars + 3), 0};
   bool ok = true;
   // One thread: the record and the states' values of a unit, and their remainders.  H lies at 0, G 16,384 bytes on.
@@ -1235,6 +1257,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
 template <typename T>
 __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectiveParams P, const Space W) {
   __shared__ float grad[kPrepHeads][Q + 4];
+  launch_dependents();
+  wait_for_launch();
   const int c = blockIdx.x, h0 = blockIdx.y * kPrepHeads, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int h = h0 + warp, rows = min(Q, tokens_of(P, b) - c * Q);
   if (h < P.heads) {
@@ -1272,6 +1296,8 @@ __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectivePara
 // One warp a head: gradients of A, the bias and D.
 __global__ void __launch_bounds__(128) finish_heads_kernel(const SelectiveParams P, const Space W) {
   const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  launch_dependents();
+  wait_for_launch();
   if (h >= P.heads) return;
   float da = 0.f, db = 0.f, dd = 0.f;
   for (int i = lane; i < P.batch * W.nc; i += 32) {
@@ -1297,6 +1323,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) finish_groups_kernel(const SelectiveParams P, const Space W) {
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x, width = (long long)P.groups * kN;
   const long long all = (long long)P.batch * P.length * width;
+  wait_for_launch();
   if (i * 4 >= all) return;
   const long long token = i * 4 / width, b = token / P.length, t = token % P.length;
   const bool in = t < tokens_of(P, (int)b);
@@ -1402,10 +1429,28 @@ template <auto K> int allow(uint32_t bytes) {
   return kOk;
 }
 
+// Launches a kernel that begins while the one before it ends: every kernel here waits (wait_for_launch) before it reads
+// what earlier ones wrote or ends, so that each of a call's kernels comes after all before it.  The first is launched
+// plainly, behind whatever the stream holds.
+template <typename... A> int behind(void (*kernel)(A...), dim3 grid, int threads, uint32_t bytes, cudaStream_t st, A... args) {
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t at{};
+  at.gridDim = grid;
+  at.blockDim = dim3(threads);
+  at.dynamicSmemBytes = bytes;
+  at.stream = st;
+  at.attrs = &early;
+  at.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&at, kernel, args...);
+  if (e != cudaSuccess) { cudaGetLastError(); last_launch_error() = e; return kECuda; }
+  return launch_status();
+}
+
 template <typename T, bool REV, bool LO> int pass(const SelectiveParams& P, const Space& W, cudaStream_t st) {
   if (int s = allow<state_pass_kernel<T, REV, LO>>(kPassSmem)) return s;
-  state_pass_kernel<T, REV, LO><<<dim3(W.units, P.batch), kThreads, kPassSmem, st>>>(P, W);
-  return launch_status();
+  return behind(state_pass_kernel<T, REV, LO>, dim3(W.units, P.batch), kThreads, kPassSmem, st, P, W);
 }
 
 template <typename T> int prepare(const SelectiveParams& P, const Space& W, cudaStream_t st) {
@@ -1416,17 +1461,17 @@ template <typename T> int prepare(const SelectiveParams& P, const Space& W, cuda
 
 template <typename T> int forward(const SelectiveParams& P, cudaStream_t st) {
   const Space W = space_of(P, false);
+  if (int s = allow<out_kernel<T>>(kOutSmem)) return s;
   if (int s = prepare<T>(P, W, st)) return s;
   if (W.nc > 1 || P.state_in || P.state_out)
     if (int s = pass<T, false, false>(P, W, st)) return s;
-  if (int s = allow<out_kernel<T>>(kOutSmem)) return s;
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
-  out_kernel<T><<<dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kOutSmem, st>>>(P, W, per);
-  return launch_status();
+  return behind(out_kernel<T>, dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kOutSmem, st, P, W, per);
 }
 
 template <typename T> int backward(const SelectiveParams& P, cudaStream_t st) {
   const Space W = space_of(P, true);
+  if (int s = allow<grad_kernel<T>>(kGradSmem)) return s;
   if (int s = prepare<T>(P, W, st)) return s;
   if (W.nc > 1 || P.state_in || P.dstate_out || P.dstate_in) {
     SelectiveParams F = P;
@@ -1434,18 +1479,14 @@ template <typename T> int backward(const SelectiveParams& P, cudaStream_t st) {
     if (int s = pass<T, false, true>(F, W, st)) return s;
     if (int s = pass<T, true, true>(P, W, st)) return s;
   }
-  if (int s = allow<grad_kernel<T>>(kGradSmem)) return s;
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
-  grad_kernel<T><<<dim3(W.nc, P.groups * W.splits, P.batch), kGradThreads, kGradSmem, st>>>(P, W, per);
-  if (int s = launch_status()) return s;
-  finish_dt_kernel<T><<<dim3(W.nc, (P.heads + kPrepHeads - 1) / kPrepHeads, P.batch), kThreads, 0, st>>>(P, W);
-  if (int s = launch_status()) return s;
-  finish_heads_kernel<<<(P.heads + 3) / 4, 128, 0, st>>>(P, W);
-  if (int s = launch_status()) return s;
+  if (int s = behind(grad_kernel<T>, dim3(W.nc, P.groups * W.splits, P.batch), kGradThreads, kGradSmem, st, P, W, per)) return s;
+  if (int s = behind(finish_dt_kernel<T>, dim3(W.nc, (P.heads + kPrepHeads - 1) / kPrepHeads, P.batch), kThreads, 0, st, P, W)) return s;
+  if (P.dA || P.dD || P.dbias)
+    if (int s = behind(finish_heads_kernel, dim3((P.heads + 3) / 4), 128, 0, st, P, W)) return s;
   if (W.splits > 1) {
     const long long all = (long long)P.batch * P.length * P.groups * (kN / 4);
-    finish_groups_kernel<T><<<(unsigned)((all + 255) / 256), 256, 0, st>>>(P, W);
-    return launch_status();
+    return behind(finish_groups_kernel<T>, dim3((unsigned)((all + 255) / 256)), 256, 0, st, P, W);
   }
   return kOk;
 }
