@@ -89,27 +89,49 @@ template <int V> __device__ __forceinline__ void decode(const Values<int8_t, V>&
   for (int i = 0; i < V; ++i)
     f[i] = (__uint_as_float(__byte_perm(w[i >> 2] ^ 0x80808080u, 0x4b000000u, 0x7540 + (i & 3))) - 8388736.0f) * scale;
 }
-// Scale and codes of the 128 values of which this thread has V; the others are its neighbours'.  A NaN or an infinity
-// makes the block's scale one, and its values NaN.
-template <int V> __device__ __forceinline__ float encode(const float (&f)[V], Values<int8_t, V>& u) {
+// The largest magnitude of some values, as its fp32 bits; a NaN is larger than any number.
+template <int V> __device__ __forceinline__ uint32_t top_bits(const Values<float, V>& u) {
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(u.v[i]) & 0x7fffffffu);
+  return m;
+}
+template <typename T, int V> __device__ __forceinline__ uint32_t top_bits(const Values<T, V>& u) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+  return __float_as_uint(to_f32(from_bits<T>(max(m & 0xffffu, m >> 16))));
+}
+// Scale and codes of the 128 values of which this thread has V; the others are its neighbours'.  A NaN or an infinity
+// makes the block's scale one, and its values NaN.
+template <typename T, int V> __device__ __forceinline__ float encode(const Values<T, V>& x, const float (&f)[V], Values<int8_t, V>& u) {
+  uint32_t m = top_bits(x);
 #pragma unroll
   for (int o = kPackBlock / V / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float scale = __fdiv_rn(__uint_as_float(m), 127.0f);
+  const float top = __uint_as_float(m);
+  float scale;
   uint32_t q[V];
-  if (scale >= 1e-30f && scale <= 3.0e38f) {
-    // x times 1 / scale tells the code but where it lies next to a half: there the quotient does
-    const float inverse = __frcp_rn(scale);
+  bool plain = top >= 1e-28f && top <= 3.0e38f;
+  if (plain) {
+    // top / 127, its remainder taken once more: the quotient's rounding.  x times about 1 / scale tells the code but
+    // where it lies next to a half.
+    constexpr float kPart = 1.0f / 127.0f;
+    const float guess = top * kPart;
+    scale = fmaf(fmaf(-127.0f, guess, top), kPart, guess);
+    const float inverse = __fdividef(1.0f, scale);
+    float off = 0.f;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float t = f[i] * inverse;
-      float whole = t + kWhole;
-      if (fabsf(t - (whole - kWhole)) > 0.4999f) whole = __fdiv_rn(f[i], scale) + kWhole;
+      const float t = f[i] * inverse, whole = t + kWhole;
+      off = fmaxf(off, fabsf(t - (whole - kWhole)));
       q[i] = __float_as_uint(whole);
     }
-  } else {                                          // tiny ones by the quotient; none of zeros, infinities and NaN
+    plain = off <= 0.4999f;
+  } else {
+    scale = __fdiv_rn(top, 127.0f);
+  }
+  if (!plain) {                                     // by the quotients; none of zeros, infinities and NaN
 #pragma unroll
     for (int i = 0; i < V; ++i)
       q[i] = scale > 0.f && scale <= 3.0e38f ? (uint32_t)__float2int_rn(fmaxf(-127.f, fminf(127.f, __fdiv_rn(f[i], scale)))) : 0;
@@ -282,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 8) conv_kernel(const ConvParams P, i
         y += P.y_st;
         if constexpr (KEEP) {
           Values<int8_t, V> q;
-          const float s = encode<V>(f, q);
+          const float s = encode<T, V>(now[j], f, q);
           if (there) {
             store_codes<V>(codes, VEC, n, q);
             if ((threadIdx.x & 31) == 0) *scales = s;
@@ -488,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P, 
 #pragma unroll
       for (int i = 0; i < V; ++i) f[i] = to_f32(x[j].v[i]);
       Values<int8_t, V> q;
-      const float scale = encode<V>(f, q);
+      const float scale = encode<T, V>(x[j], f, q);
       if (n > 0 && r0 + j < P.rows) {
         store_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, q);
         if ((c & (kPackBlock - 1)) == 0) P.scales[(r0 + j) * blocks + c / kPackBlock] = scale;
@@ -496,27 +518,36 @@ __global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P, 
     }
   }
 }
+// Back: a thread has sixteen codes.
+constexpr int kCodes = 16;
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 12) unpack_kernel(const PackParams P, int vec, int vec_codes) {
+__global__ void __launch_bounds__(kThreads, 10) unpack_kernel(const PackParams P, int vec, int vec_codes) {
   constexpr int V = kUnit<T>;
-  const int c = (blockIdx.x * kThreads + threadIdx.x) * V;
-  const int n = min(V, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * kCodes;
+  const int n = min(kCodes, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
   if (n <= 0) return;
   for (long long r0 = (long long)blockIdx.y * kRows; r0 < P.rows; r0 += (long long)gridDim.y * kRows) {
     float scale[kRows];
-    Values<int8_t, V> q[kRows];
+    Values<int8_t, kCodes> q[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
       const bool in = r0 + j < P.rows;
       scale[j] = in ? P.scales[(r0 + j) * blocks + c / kPackBlock] : 0.f;
-      q[j] = in ? raw_values<int8_t, V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n) : Values<int8_t, V>{};
+      if (in) q[j] = raw_values<int8_t, kCodes>(P.codes + (r0 + j) * P.width + c, vec_codes && n == kCodes, n);
     }
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
       if (r0 + j < P.rows) {
-        float f[V];
-        decode<V>(q[j], scale[j], f);
-        store_values<T, V>(reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c, vec && n == V, n, f);
+        float f[kCodes];
+        decode<kCodes>(q[j], scale[j], f);
+        T* out = reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c;
+#pragma unroll
+        for (int i = 0; i < kCodes; i += V) {
+          float part[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) part[e] = f[i + e];
+          store_values<T, V>(out + i, vec && n == kCodes, n - i, part);
+        }
       }
   }
 }
@@ -598,8 +629,8 @@ int launch_conv_step(const ConvStepParams& P, cudaStream_t st) {
 }
 
 namespace {
-dim3 pack_grid(const PackParams& P) {
-  const int per = kThreads * unit_of(P.type), wide = (P.width + per - 1) / per;
+dim3 pack_grid(const PackParams& P, int of_a_thread) {
+  const int per = kThreads * of_a_thread, wide = (P.width + per - 1) / per;
   long long rows = (P.rows + kRows - 1) / kRows, most = 148 * 16 / wide;      // CTAs that an SM's threads hold
   most = most < 1 ? 1 : most > 65535 ? 65535 : most;
   return dim3(wide, (unsigned)(rows < most ? rows : most));
@@ -607,17 +638,19 @@ dim3 pack_grid(const PackParams& P) {
 }  // namespace
 
 int launch_pack(const PackParams& P, cudaStream_t st) {
-  const int vec = whole(P.x, P.type, unit_of(P.type), P.x_stride), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
-  if (P.type == 0) pack_kernel<__half><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
-  else if (P.type == 1) pack_kernel<__nv_bfloat16><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
-  else pack_kernel<float><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  const int unit = unit_of(P.type), vec = whole(P.x, P.type, unit, P.x_stride), vec_codes = P.width % unit == 0 && ((uintptr_t)P.codes & 7) == 0;
+  const dim3 grid = pack_grid(P, unit);
+  if (P.type == 0) pack_kernel<__half><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
+  else if (P.type == 1) pack_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
+  else pack_kernel<float><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
   return launch_status();
 }
 int launch_unpack(const PackParams& P, cudaStream_t st) {
-  const int vec = whole(P.y, P.type, unit_of(P.type), P.width), vec_codes = P.width % unit_of(P.type) == 0 && ((uintptr_t)P.codes & 7) == 0;
-  if (P.type == 0) unpack_kernel<__half><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
-  else if (P.type == 1) unpack_kernel<__nv_bfloat16><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
-  else unpack_kernel<float><<<pack_grid(P), kThreads, 0, st>>>(P, vec, vec_codes);
+  const int vec = whole(P.y, P.type, unit_of(P.type), P.width), vec_codes = P.width % kCodes == 0 && ((uintptr_t)P.codes & 15) == 0;
+  const dim3 grid = pack_grid(P, kCodes);
+  if (P.type == 0) unpack_kernel<__half><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
+  else if (P.type == 1) unpack_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
+  else unpack_kernel<float><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
   return launch_status();
 }
 

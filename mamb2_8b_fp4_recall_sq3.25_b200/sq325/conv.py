@@ -20,6 +20,8 @@ __all__ = ['causal_conv', 'causal_conv_step']
 
 def inner_packed(t, axes):
     """t with its last `axes` axes contiguous (a copy only where they are not)."""
+    if t.is_contiguous():
+        return t
     step = 1
     for k in range(t.ndim - 1, t.ndim - 1 - axes, -1):
         if t.shape[k] != 1 and t.stride(k) != step:
@@ -31,7 +33,8 @@ def inner_packed(t, axes):
 def checked_lengths(lengths, batch, device):
     if lengths is None:
         return None
-    if not isinstance(lengths, torch.Tensor) or lengths.shape != (batch,) or lengths.dtype != torch.int32 or lengths.device != device:
+    if not isinstance(lengths, torch.Tensor) or lengths.shape != (batch,) or lengths.dtype != torch.int32 \
+            or lengths.get_device() != device.index:
         raise ValueError(f'lengths must be an int32 tensor of shape ({batch},) on {device}')
     return lengths.contiguous()
 
@@ -39,10 +42,10 @@ def checked_lengths(lengths, batch, device):
 def checked_weight(weight, bias, channels, dtype, device):
     if not isinstance(weight, torch.Tensor) or weight.ndim != 2 or weight.shape[0] != channels or not 2 <= weight.shape[1] <= 4:
         raise ValueError(f'weight must be [{channels}, taps] with 2 to 4 taps')
-    if weight.dtype not in (dtype, torch.float32) or weight.device != device:
+    if weight.dtype != dtype and weight.dtype != torch.float32 or weight.get_device() != device.index:
         raise ValueError("weight must have the input's dtype or FP32, on its device")
     if bias is not None and (not isinstance(bias, torch.Tensor) or bias.shape != (channels,) or bias.dtype != weight.dtype
-                             or bias.device != device):
+                             or bias.get_device() != device.index):
         raise ValueError(f"bias must be [{channels}] in the weight's dtype, on its device")
     return weight.contiguous(), None if bias is None else bias.contiguous()
 
@@ -66,13 +69,10 @@ def _ptr(t):
 def conv_args(shape, dtype, x, packed, weight, bias, state, lengths, silu):
     """The arguments that forward and backward share."""
     batch, length, channels = shape
-    a = _lib.CausalConvArgs(batch, length, channels, weight.shape[1], silu, TYPES[dtype], TYPES[weight.dtype])
-    if x is not None:
-        a.x, a.x_batch_stride, a.x_token_stride = x.data_ptr(), x.stride(0), x.stride(1)
-    if packed is not None:
-        a.codes, a.scales = packed.codes.data_ptr(), packed.scales.data_ptr()
-    a.weight, a.bias, a.state_in, a.lengths = weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(lengths)
-    return a
+    at = (None, 0, 0) if x is None else (x.data_ptr(), x.stride(0), x.stride(1))
+    codes = (None, None) if packed is None else (packed.codes.data_ptr(), packed.scales.data_ptr())
+    return _lib.CausalConvArgs(batch, length, channels, weight.shape[1], silu, TYPES[dtype], TYPES[weight.dtype], *at, *codes,
+                               weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(lengths))
 
 
 def conv_forward(shape, dtype, x, packed, weight, bias, state, lengths, silu, want_state=False):

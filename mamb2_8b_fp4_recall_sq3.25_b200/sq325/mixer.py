@@ -75,7 +75,8 @@ def _checked(xbc, dt, A, conv_weight, conv_bias, D, dt_bias, heads, groups, lead
     inner = width - 2 * groups * N
     if heads % groups or inner < heads or inner % heads:
         raise ValueError('xbc must have heads*dim + 2*groups*128 channels, with heads divisible by groups')
-    if not isinstance(dt, torch.Tensor) or dt.shape != (*lead, heads) or dt.dtype != xbc.dtype or dt.device != device:
+    if not isinstance(dt, torch.Tensor) or dt.shape != (*lead, heads) or dt.dtype != xbc.dtype \
+            or dt.get_device() != device.index:
         raise ValueError(f"dt must be {[*lead, heads]} in xbc's dtype, on its device")
     weight, bias = checked_weight(conv_weight, conv_bias, width, xbc.dtype, device)
     A, D, dt_bias = checked_heads(A, D, dt_bias, heads, device)

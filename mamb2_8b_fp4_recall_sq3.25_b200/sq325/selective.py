@@ -12,6 +12,7 @@ gradients for everything, the states among them.  Nothing but the inputs is kept
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -27,10 +28,11 @@ _HALF = (torch.float16, torch.bfloat16)
 
 def checked_heads(A, D, dt_bias, heads, device):
     """Per-head parameters: A fp32, D and dt_bias fp16, bf16, fp32 or None."""
-    if not isinstance(A, torch.Tensor) or A.shape != (heads,) or A.dtype != torch.float32 or A.device != device:
+    if not isinstance(A, torch.Tensor) or A.shape != (heads,) or A.dtype != torch.float32 or A.get_device() != device.index:
         raise ValueError(f'A must be FP32 [{heads}] on {device}')
     for name, t in (('D', D), ('dt_bias', dt_bias)):
-        if t is not None and (not isinstance(t, torch.Tensor) or t.shape != (heads,) or t.dtype not in TYPES or t.device != device):
+        if t is not None and (not isinstance(t, torch.Tensor) or t.shape != (heads,) or t.dtype not in TYPES
+                              or t.get_device() != device.index):
             raise ValueError(f'{name} must be None or FP16, BF16 or FP32 [{heads}] on {device}')
     return A.contiguous(), None if D is None else D.contiguous(), None if dt_bias is None else dt_bias.contiguous()
 
@@ -38,7 +40,8 @@ def checked_heads(A, D, dt_bias, heads, device):
 def checked_state(state, shape, device, name='initial_state'):
     if state is None:
         return None
-    if not isinstance(state, torch.Tensor) or state.shape != shape or state.dtype != torch.float32 or state.device != device:
+    if not isinstance(state, torch.Tensor) or state.shape != shape or state.dtype != torch.float32 \
+            or state.get_device() != device.index:
         raise ValueError(f'{name} must be FP32 {list(shape)} on {device}')
     return state.contiguous()
 
@@ -46,19 +49,20 @@ def checked_state(state, shape, device, name='initial_state'):
 def scan_args(x, dt, A, B, C_, D, dt_bias, state, lengths):
     """The arguments that forward and backward share, of checked tensors."""
     batch, length, heads, dim = x.shape
-    a = _lib.SelectiveArgs(batch, length, heads, dim, B.shape[2], TYPES[x.dtype],
-                           x.data_ptr(), x.stride(0), x.stride(1), dt.data_ptr(), dt.stride(0), dt.stride(1), A.data_ptr(),
-                           B.data_ptr(), B.stride(0), B.stride(1), C_.data_ptr(), C_.stride(0), C_.stride(1))
-    if D is not None:
-        a.D, a.d_type = D.data_ptr(), TYPES[D.dtype]
-    if dt_bias is not None:
-        a.dt_bias, a.bias_type = dt_bias.data_ptr(), TYPES[dt_bias.dtype]
-    a.state_in, a.lengths = _ptr(state), _ptr(lengths)
-    return a
+    sx, st, sb, sc = x.stride(), dt.stride(), B.stride(), C_.stride()
+    return _lib.SelectiveArgs(batch, length, heads, dim, B.shape[2], TYPES[x.dtype], x.data_ptr(), sx[0], sx[1],
+                              dt.data_ptr(), st[0], st[1], A.data_ptr(), B.data_ptr(), sb[0], sb[1], C_.data_ptr(), sc[0], sc[1],
+                              _ptr(D), 0 if D is None else TYPES[D.dtype], _ptr(dt_bias), 0 if dt_bias is None else TYPES[dt_bias.dtype],
+                              _ptr(state), _ptr(lengths))
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch, length, heads, dim, groups, backward):
+    return int(_lib.load().sq_selective_workspace(batch, length, heads, dim, groups, backward))
 
 
 def _workspace(a, backward, device):
-    nbytes = int(_lib.load().sq_selective_workspace(a.batch, a.length, a.heads, a.dim, a.groups, backward))
+    nbytes = _workspace_bytes(a.batch, a.length, a.heads, a.dim, a.groups, backward)
     work = torch.empty(nbytes, dtype=torch.uint8, device=device)
     a.workspace, a.workspace_bytes = work.data_ptr(), nbytes
     return work                                              # alive until the launch
@@ -67,7 +71,7 @@ def _workspace(a, backward, device):
 def scan_forward(x, dt, A, B, C_, D, dt_bias, state, lengths, want_state):
     """(y, final state or None) of checked tensors."""
     batch, length, heads, dim = x.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     last = torch.empty(batch, heads, dim, N, dtype=torch.float32, device=x.device) if want_state else None
     a = scan_args(x, dt, A, B, C_, D, dt_bias, state, lengths)
     a.y, a.y_batch_stride, a.y_token_stride, a.state_out = y.data_ptr(), length * heads * dim, heads * dim, _ptr(last)
@@ -81,7 +85,7 @@ def scan_backward(x, dt, A, B, C_, D, dt_bias, state, lengths, dy, dlast, dx, dB
     """Writes dx, dB, dC (dB and dC with the same strides) and returns (ddt, dA, dD, ddt_bias, dstate); need: which
     of A, D, dt_bias, state have a gradient."""
     device = x.device
-    ddt = torch.empty(dt.shape, dtype=dt.dtype, device=device)
+    ddt = torch.empty_like(dt, memory_format=torch.contiguous_format)
     dA, dD, dbias, dstate = (torch.empty_like(t) if want else None for t, want in zip((A, D, dt_bias, state), need))
     a = scan_args(x, dt, A, B, C_, D, dt_bias, state, lengths)
     a.dy, a.dy_batch_stride, a.dy_token_stride, a.dstate_out = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
@@ -117,7 +121,7 @@ class _SelectiveScan(torch.autograd.Function):
         dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else inner_packed(dy, 2)
         dlast = None if dlast is None else dlast.contiguous()
         need = ctx.needs_input_grad
-        dx, dB, dC = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, B, C_))
+        dx, dB, dC = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (x, B, C_))
         ddt, dA, dD, dbias, dstate = scan_backward(x, dt, A, B, C_, D, dt_bias, state, lengths, dy, dlast, dx, dB, dC,
                                                    (need[2], need[5], need[6], need[7]))
         return dx, ddt, dA, dB, dC, dD, dbias, dstate, None, None
@@ -139,7 +143,7 @@ def selective_scan(x, dt, A, B, C_, D=None, dt_bias=None, initial_state=None, le
         raise ValueError('heads must be divisible by B/C groups')
     groups = (batch, length, B.shape[2], N)
     for name, t, shape in (('dt', dt, (batch, length, heads)), ('B', B, groups), ('C', C_, groups)):
-        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != x.dtype or t.device != device:
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != x.dtype or t.get_device() != device.index:
             raise ValueError(f"{name} must be {list(shape)} in x's dtype, on its device")
     A, D, dt_bias = checked_heads(A, D, dt_bias, heads, device)
     state = checked_state(initial_state, (batch, heads, dim, N), device)
@@ -163,7 +167,7 @@ def selective_step(x, dt, A, B, C_, state, D=None, dt_bias=None):
         raise ValueError('heads must be divisible by B/C groups')
     groups = (batch, B.shape[1], N)
     for name, t, shape in (('dt', dt, (batch, heads)), ('B', B, groups), ('C', C_, groups)):
-        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != x.dtype or t.device != device:
+        if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != x.dtype or t.get_device() != device.index:
             raise ValueError(f"{name} must be {list(shape)} in x's dtype, on its device")
     A, D, dt_bias = checked_heads(A, D, dt_bias, heads, device)
     if checked_state(state, (batch, heads, dim, N), device, 'state') is not state:
