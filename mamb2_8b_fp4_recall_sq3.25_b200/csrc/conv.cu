@@ -143,9 +143,14 @@ template <typename T, int V> __device__ __forceinline__ float encode(const Value
   return scale;
 }
 
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 template <typename T> __device__ __forceinline__ float sigmoid(float z) {
   if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
-  else return __fdividef(1.0f, 1.0f + __expf(-z));  // a few ulp of fp32, far below a 16-bit result's half step
+  else return reciprocal(1.0f + ex2(z * -kLog2e));  // a few ulp of fp32, far below a 16-bit result's half step
 }
 
 // A thread's V channels: weights and bias.
@@ -219,6 +224,38 @@ template <typename T, bool CODES, bool VEC, int V> struct Inputs {
     }
     return u;
   }
+  // U tokens from t on, those from `end` on as zero.
+  template <int U> __device__ __forceinline__ void load_batch(int t, int end, bool take, Raw (&u)[U], float (&scale)[U]) const {
+    if constexpr (CODES) {
+      const int8_t* p = codes + t * step;
+      const float* s = scales + t * scale_step;
+      if (take && t + U <= end) {
+#pragma unroll
+        for (int j = 0; j < U; ++j, p += step, s += scale_step) { u[j] = raw_values<int8_t, V>(p, VEC, n); scale[j] = *s; }
+      } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j, p += step, s += scale_step) {
+          const bool in = take && t + j < end;
+          if (in) u[j] = raw_values<int8_t, V>(p, VEC, n);
+          else u[j] = Raw{};
+          scale[j] = in ? *s : 0.f;
+        }
+      }
+    } else {
+      const T* p = x + t * step;
+      if (take && t + U <= end) {
+#pragma unroll
+        for (int j = 0; j < U; ++j, p += step) { u[j] = raw_values<T, V>(p, VEC, n); scale[j] = 0.f; }
+      } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j, p += step) {
+          scale[j] = 0.f;
+          if (take && t + j < end) u[j] = raw_values<T, V>(p, VEC, n);
+          else u[j] = no_values<T, V>();
+        }
+      }
+    }
+  }
   static __device__ __forceinline__ void get(const Raw& u, float scale, float (&f)[V]) {
     if constexpr (CODES) {
       decode<V>(u, scale, f);
@@ -246,72 +283,81 @@ template <typename T, bool CODES, bool VEC, int V> struct Inputs {
 // z of a token whose last four inputs are x[0..3], oldest first.  Taps that are not there are passed over, not
 // multiplied by zero: their inputs may be infinite.
 template <typename WT, int V>
-__device__ __forceinline__ float conv_at(const Taps<WT, V>& W, int taps, int i, float x0, float x1, float x2, float x3) {
+__device__ __forceinline__ float conv_at(const Taps<WT, V>& W, const int taps, int i, float x0, float x1, float x2, float x3) {
   float z = W.b[i];
   if (taps > 3) z += W.w[0][i] * x0;
   if (taps > 2) z += W.w[1][i] * x1;
   return (z + W.w[2][i] * x2) + W.w[3][i] * x3;
 }
 
-// MODE: 0 reads the input, 1 keeps it in 8 bits besides, 2 reads what was kept.
-template <typename T, typename WT, int MODE, bool VEC>
-__global__ void __launch_bounds__(kThreads, 8) conv_kernel(const ConvParams P, int strip) {
+// MODE: 0 reads the input, 1 keeps it in 8 bits besides, 2 reads what was kept.  FAST: four taps, silu and whole aligned
+// pieces, as mixers have them; without them a third of the instructions would be the questions.
+template <typename T, typename WT, int MODE, bool FAST>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || MODE == 1 ? 5 : MODE == 2 ? 6 : 8) conv_kernel(const ConvParams P, int strip) {
   constexpr int V = kWide, U = 4;                                      // U: tokens whose loads are in flight together
-  constexpr bool KEEP = MODE == 1, CODES = MODE == 2;
+  constexpr bool KEEP = MODE == 1, CODES = MODE == 2, VEC = FAST;
+  using In = Inputs<T, CODES, VEC, V>;
+  const int taps = FAST ? kTaps : P.taps;
+  const bool silu = FAST || P.silu;
   const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
   const int n = min(V, P.channels - c);                                // may be negative: shuffles need every lane
   if (!KEEP && n <= 0) return;
   const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip), end = min(t1, len);
-  const Inputs<T, CODES, VEC, V> in(P, b, n > 0 ? c : 0, n);
+  const In in(P, b, n > 0 ? c : 0, n);
   T* y = reinterpret_cast<T*>(P.y) + b * P.y_sb + (long long)t0 * P.y_st + c;
   const int blocks = (P.channels + kPackBlock - 1) / kPackBlock;
   int8_t* codes = KEEP ? P.codes + ((long long)b * P.length + t0) * P.channels + c : nullptr;
   float* scales = KEEP ? P.scales + ((long long)b * P.length + t0) * blocks + c / kPackBlock : nullptr;
   if (n > 0 && blockIdx.x == 0 && P.state_out) {                       // the last inputs
-    for (int j = 0; j < P.taps - 1; ++j) {
+    for (int j = 0; j < taps - 1; ++j) {
       float f[V];
-      in.at(P, b, len - (P.taps - 1) + j, c, f);
-      store_values<T, V>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (P.taps - 1) + j) * P.channels + c, false, n, f);
+      in.at(P, b, len - (taps - 1) + j, c, f);
+      store_values<T, V>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (taps - 1) + j) * P.channels + c, false, n, f);
     }
   }
   if (t0 < end) {
     float x[kTaps - 1][V], scale[U];
-    typename Inputs<T, CODES, VEC, V>::Raw now[U];
+    typename In::Raw now[U];
+    in.template load_batch<U>(t0, end, n > 0, now, scale);
+    const Taps<WT, V> W(P.weight, P.bias, taps, n > 0 ? c : 0, n);
 #pragma unroll
-    for (int j = 0; j < U; ++j) now[j] = in.load(t0 + j, n > 0 && t0 + j < end, scale[j]);
-    const Taps<WT, V> W(P.weight, P.bias, P.taps, n > 0 ? c : 0, n);
-#pragma unroll
-    for (int k = 0; k < kTaps - 1; ++k) {
+    for (int k = 0; k < kTaps - 1; ++k)
       if (n > 0) in.at(P, b, t0 - (kTaps - 1) + k, c, x[k]);
-    }
-    for (int t = t0; t < end; t += U) {
-      typename Inputs<T, CODES, VEC, V>::Raw next[U];
-      float later[U];
+    auto token = [&](const typename In::Raw& raw, float s, bool there) {
+      float out[V], f[V];
+      In::get(raw, s, f);
 #pragma unroll
-      for (int j = 0; j < U; ++j) next[j] = in.load(t + U + j, n > 0 && t + U + j < end, later[j]);
+      for (int i = 0; i < V; ++i) {
+        const float z = conv_at<WT, V>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
+        out[i] = silu ? z * sigmoid<T>(z) : z;
+        x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
+      }
+      if (there) store_values<T, V>(y, VEC, n, out);
+      y += P.y_st;
+      if constexpr (KEEP) {
+        Values<int8_t, V> q;
+        const float top = encode<T, V>(raw, f, q);
+        if (there) {
+          store_codes<V>(codes, VEC, n, q);
+          if ((threadIdx.x & 31) == 0) *scales = top;
+        }
+        codes += P.channels;
+        scales += blocks;
+      }
+    };
+    for (int t = t0; t < end; t += U) {
+      typename In::Raw next[U];
+      float later[U];
+      in.template load_batch<U>(t + U, end, n > 0, next, later);
+      if (n > 0 && t + U <= end) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) token(now[j], scale[j], true);
+      } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j) token(now[j], scale[j], n > 0 && t + j < end);
+      }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const bool there = n > 0 && t + j < end;
-        float out[V], f[V];
-        in.get(now[j], scale[j], f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], f[i]);
-          out[i] = P.silu ? z * sigmoid<T>(z) : z;
-          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
-        }
-        if (there) store_values<T, V>(y, VEC, n, out);
-        y += P.y_st;
-        if constexpr (KEEP) {
-          Values<int8_t, V> q;
-          const float s = encode<T, V>(now[j], f, q);
-          if (there) {
-            store_codes<V>(codes, VEC, n, q);
-            if ((threadIdx.x & 31) == 0) *scales = s;
-          }
-          codes += P.channels;
-          scales += blocks;
-        }
         now[j] = next[j];
         scale[j] = later[j];
       }
@@ -332,94 +378,115 @@ __global__ void __launch_bounds__(kThreads, 8) conv_kernel(const ConvParams P, i
 
 // A strip's gradients: dz_t = dy_t y'(z_t), dx_t = sum_k w_k dz_{t + taps-1 - k}, and the strip's sums of dz_t x_{t - (taps-1) + k}
 // and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.
-template <typename T, typename WT, bool CODES, bool VEC>
+template <typename T, typename WT, bool CODES, bool FAST>
 __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams P, int strip) {
   constexpr int V = kWide, U = 4;
+  constexpr bool VEC = FAST;
+  using In = Inputs<T, CODES, VEC, V>;
+  const int taps = FAST ? kTaps : P.taps;
+  const bool silu = FAST || P.silu;
   const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
   const int n = min(V, P.channels - c);
   if (n <= 0) return;
-  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip), back = P.taps - 1;
-  const Inputs<T, CODES, VEC, V> in(P, b, c, n);
+  const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip), back = taps - 1;
+  const In in(P, b, c, n);
   const T* dy = reinterpret_cast<const T*>(P.dy) + b * P.dy_sb + c;
   T* dx = reinterpret_cast<T*>(P.dx) + (long long)b * P.length * P.channels + c;
   float dw[kTaps][V] = {}, db[V] = {};
   if (t0 < len || t0 == 0) {
-    const int stop = t1 + kTaps - 1, end = min(stop, len);
+    const int stop = t1 + kTaps - 1, end = min(stop, len), own = min(t1, len), lowest = t0 == 0 ? -back : t0;
     float x[kTaps - 1][V], dz[kTaps - 1][V] = {}, scale[U];
-    typename Inputs<T, CODES, VEC, V>::Raw now[U];
+    typename In::Raw now[U];
     Values<T, V> up[U];
-    auto load_up = [&](int t) {
-      Values<T, V> u;
-      if (t < end) u = raw_values<T, V>(dy + t * P.dy_st, VEC, n);
-      else u = no_values<T, V>();
-      return u;
-    };
+    auto load_up = [&](int t, Values<T, V>(&u)[U]) {
+      const T* p = dy + t * P.dy_st;
+      if (t + U <= end) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) {
-      now[j] = in.load(t0 + j, t0 + j < end, scale[j]);
-      up[j] = load_up(t0 + j);
-    }
-    const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
+        for (int j = 0; j < U; ++j, p += P.dy_st) u[j] = raw_values<T, V>(p, VEC, n);
+      } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j, p += P.dy_st) {
+          if (t + j < end) u[j] = raw_values<T, V>(p, VEC, n);
+          else u[j] = no_values<T, V>();
+        }
+      }
+    };
+    in.template load_batch<U>(t0, end, true, now, scale);
+    load_up(t0, up);
+    const Taps<WT, V> W(P.weight, P.bias, taps, c, n);
 #pragma unroll
     for (int k = 0; k < kTaps - 1; ++k) in.at(P, b, t0 - (kTaps - 1) + k, c, x[k]);
     T* put = dx + (long long)(t0 - (kTaps - 1)) * P.channels;          // of the token whose input's gradient is whole next
+    // inner: the token and the one whose gradient becomes whole are both this strip's
+    auto token = [&](const typename In::Raw& raw, float s_in, const Values<T, V>& raw_up, int at, auto inner) {
+      constexpr bool INNER = decltype(inner)::value;
+      const int to = at - (kTaps - 1);
+      const bool mine = INNER || at < own;
+      float f[V], out[V];
+      In::get(raw, s_in, f);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        float d = to_f32(raw_up.v[i]);
+        if (silu) {
+          const float z = conv_at<WT, V>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
+          const float s = sigmoid<T>(z);
+          d *= fmaf(s, z * (1.0f - s), s);
+        }
+        if (!INNER && at >= end) d = 0.f;                              // z of what is not there may be anything
+        if (mine) {
+          db[i] += d;
+          if (taps > 3) dw[0][i] += d * x[0][i];
+          if (taps > 2) dw[1][i] += d * x[1][i];
+          dw[2][i] += d * x[2][i];
+          dw[3][i] += d * f[i];
+        }
+        x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
+        // dz[0..2] and d are those of `to` .. `to` + 3
+        float g = W.w[3][i] * dz[0][i] + W.w[2][i] * dz[1][i];
+        if (taps > 2) g += W.w[1][i] * dz[2][i];
+        if (taps > 3) g += W.w[0][i] * d;
+        dz[0][i] = dz[1][i]; dz[1][i] = dz[2][i]; dz[2][i] = d;
+        out[i] = g;
+      }
+      T* here = put;
+      put += P.channels;
+      if (INNER) {
+        store_values<T, V>(here, VEC, n, out);
+        return;
+      }
+      if (to >= t1 || to < lowest) return;
+      if (P.dstate_out && to >= len - back && to < len) {
+        float late[V];
+        const long long at_state = ((long long)b * back + to - (len - back)) * P.channels + c;
+        load_values<T, V>(reinterpret_cast<const T*>(P.dstate_out) + at_state, false, n, late);
+#pragma unroll
+        for (int i = 0; i < V; ++i) out[i] += late[i];
+      }
+      if (to >= 0) {
+        if (to < len) store_values<T, V>(here, VEC, n, out);
+      } else if (P.dstate_in) {
+        store_values<T, V>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
+      }
+    };
+    const int calm = P.dstate_out ? min(own, len - back) : own;        // below it no gradient of the last inputs comes in
     for (int t = t0; t < stop; t += U) {
-      typename Inputs<T, CODES, VEC, V>::Raw next[U];
+      typename In::Raw next[U];
       Values<T, V> up_next[U];
       float later[U];
+      in.template load_batch<U>(t + U, end, true, next, later);
+      load_up(t + U, up_next);
+      if (t >= t0 + U && t + U <= calm) {
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        next[j] = in.load(t + U + j, t + U + j < end, later[j]);
-        up_next[j] = load_up(t + U + j);
+        for (int j = 0; j < U; ++j) token(now[j], scale[j], up[j], t + j, std::true_type{});
+      } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j) token(now[j], scale[j], up[j], t + j, std::false_type{});
       }
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const int at = t + j, to = at - (kTaps - 1);
-        const bool mine = at < min(t1, len);
-        float f[V], out[V];
-        in.get(now[j], scale[j], f);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float d = to_f32(up[j].v[i]);
-          if (P.silu) {
-            const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], f[i]);
-            const float s = sigmoid<T>(z);
-            d *= s * (1.0f + z * (1.0f - s));
-          }
-          if (at >= end) d = 0.f;                                      // z of what is not there may be anything
-          if (mine) {
-            db[i] += d;
-            if (P.taps > 3) dw[0][i] += d * x[0][i];
-            if (P.taps > 2) dw[1][i] += d * x[1][i];
-            dw[2][i] += d * x[2][i];
-            dw[3][i] += d * f[i];
-          }
-          x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
-          // dz[0..2] and d are those of `to` .. `to` + 3
-          float g = W.w[3][i] * dz[0][i] + W.w[2][i] * dz[1][i];
-          if (P.taps > 2) g += W.w[1][i] * dz[2][i];
-          if (P.taps > 3) g += W.w[0][i] * d;
-          dz[0][i] = dz[1][i]; dz[1][i] = dz[2][i]; dz[2][i] = d;
-          out[i] = g;
-        }
         now[j] = next[j];
         scale[j] = later[j];
         up[j] = up_next[j];
-        T* here = put;
-        put += P.channels;
-        if (to >= t1 || to < (t0 == 0 ? -back : t0)) continue;
-        if (P.dstate_out && to >= len - back && to < len) {
-          float late[V];
-          const long long at = ((long long)b * back + to - (len - back)) * P.channels + c;
-          load_values<T, V>(reinterpret_cast<const T*>(P.dstate_out) + at, false, n, late);
-#pragma unroll
-          for (int i = 0; i < V; ++i) out[i] += late[i];
-        }
-        if (to >= 0) {
-          if (to < len) store_values<T, V>(here, VEC, n, out);
-        } else if (P.dstate_in) {
-          store_values<T, V>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
-        }
       }
     }
   }
@@ -493,8 +560,8 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const ConvStepParam
 
 // Rows in 8 bits: a thread has 16 bytes of the input, kRows rows at a time.
 constexpr int kRows = 4;
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P, int vec, int vec_codes) {
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P) {
   constexpr int V = kUnit<T>;
   const int c = (blockIdx.x * kThreads + threadIdx.x) * V;
   const int n = min(V, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
@@ -502,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P, 
     Values<T, V> x[kRows];
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
-      x[j] = n > 0 && r0 + j < P.rows ? raw_values<T, V>(reinterpret_cast<const T*>(P.x) + (r0 + j) * P.x_stride + c, vec && n == V, n)
+      x[j] = n > 0 && r0 + j < P.rows ? raw_values<T, V>(reinterpret_cast<const T*>(P.x) + (r0 + j) * P.x_stride + c, VEC, n)
                                       : no_values<T, V>();
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
@@ -512,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P, 
       Values<int8_t, V> q;
       const float scale = encode<T, V>(x[j], f, q);
       if (n > 0 && r0 + j < P.rows) {
-        store_codes<V>(P.codes + (r0 + j) * P.width + c, vec_codes && n == V, n, q);
+        store_codes<V>(P.codes + (r0 + j) * P.width + c, VEC, n, q);
         if ((c & (kPackBlock - 1)) == 0) P.scales[(r0 + j) * blocks + c / kPackBlock] = scale;
       }
     }
@@ -520,8 +587,8 @@ __global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P, 
 }
 // Back: a thread has sixteen codes.
 constexpr int kCodes = 16;
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 10) unpack_kernel(const PackParams P, int vec, int vec_codes) {
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kThreads, 10) unpack_kernel(const PackParams P) {
   constexpr int V = kUnit<T>;
   const int c = (blockIdx.x * kThreads + threadIdx.x) * kCodes;
   const int n = min(kCodes, P.width - c), blocks = (P.width + kPackBlock - 1) / kPackBlock;
@@ -533,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 10) unpack_kernel(const PackParams P
     for (int j = 0; j < kRows; ++j) {
       const bool in = r0 + j < P.rows;
       scale[j] = in ? P.scales[(r0 + j) * blocks + c / kPackBlock] : 0.f;
-      if (in) q[j] = raw_values<int8_t, kCodes>(P.codes + (r0 + j) * P.width + c, vec_codes && n == kCodes, n);
+      if (in) q[j] = raw_values<int8_t, kCodes>(P.codes + (r0 + j) * P.width + c, VEC, n);
     }
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
@@ -546,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 10) unpack_kernel(const PackParams P
           float part[V];
 #pragma unroll
           for (int e = 0; e < V; ++e) part[e] = f[i + e];
-          store_values<T, V>(out + i, vec && n == kCodes, n - i, part);
+          store_values<T, V>(out + i, VEC, n - i, part);
         }
       }
   }
@@ -583,15 +650,15 @@ long long conv_workspace(int batch, int length, int channels) {
 int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
   const int strip = strip_of(P.batch, P.length, P.channels, 16, 64), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
-  const bool vec = (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) && whole(P.y, P.type, kWide, P.y_sb, P.y_st) &&
-                   P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0;
+  const bool fast = P.taps == kTaps && P.silu && (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) &&
+                   whole(P.y, P.type, kWide, P.y_sb, P.y_st) && P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0;
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
     const int mode = !P.codes ? 0 : P.x ? 1 : 2;
-    if (mode == 0) vec ? conv_kernel<T, WT, 0, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 0, false><<<grid, kThreads, 0, st>>>(P, strip);
-    else if (mode == 1) vec ? conv_kernel<T, WT, 1, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 1, false><<<grid, kThreads, 0, st>>>(P, strip);
-    else vec ? conv_kernel<T, WT, 2, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 2, false><<<grid, kThreads, 0, st>>>(P, strip);
+    if (mode == 0) fast ? conv_kernel<T, WT, 0, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 0, false><<<grid, kThreads, 0, st>>>(P, strip);
+    else if (mode == 1) fast ? conv_kernel<T, WT, 1, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 1, false><<<grid, kThreads, 0, st>>>(P, strip);
+    else fast ? conv_kernel<T, WT, 2, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 2, false><<<grid, kThreads, 0, st>>>(P, strip);
     return launch_status();
   });
 }
@@ -599,13 +666,13 @@ int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
 int launch_conv_backward(const ConvParams& P, cudaStream_t st) {
   const int strip = strip_of(P.batch, P.length, P.channels, kLeast, kMost), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
-  const bool vec = (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) && whole(P.dy, P.type, kWide, P.dy_sb, P.dy_st) &&
-                   whole(P.dx, P.type, kWide, P.channels) && whole(P.workspace, 2, kWide, 0) && ((uintptr_t)P.codes & (kWide - 1)) == 0;
+  const bool fast = P.taps == kTaps && P.silu && (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) &&
+                   whole(P.dy, P.type, kWide, P.dy_sb, P.dy_st) && whole(P.dx, P.type, kWide, P.channels) && whole(P.workspace, 2, kWide, 0) && ((uintptr_t)P.codes & (kWide - 1)) == 0;
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
-    if (P.codes) vec ? conv_grad_kernel<T, WT, true, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, true, false><<<grid, kThreads, 0, st>>>(P, strip);
-    else vec ? conv_grad_kernel<T, WT, false, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, false, false><<<grid, kThreads, 0, st>>>(P, strip);
+    if (P.codes) fast ? conv_grad_kernel<T, WT, true, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, true, false><<<grid, kThreads, 0, st>>>(P, strip);
+    else fast ? conv_grad_kernel<T, WT, false, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, false, false><<<grid, kThreads, 0, st>>>(P, strip);
     if (int s = launch_status()) return s;
     if (P.dweight || P.dbias) {
       conv_weights_kernel<WT><<<dim3((P.channels + 31) / 32, kTaps + 1), 256, 0, st>>>(P, (int)grid.x * P.batch);
@@ -637,21 +704,25 @@ dim3 pack_grid(const PackParams& P, int of_a_thread) {
 }
 }  // namespace
 
+// VEC: whole aligned pieces.
 int launch_pack(const PackParams& P, cudaStream_t st) {
-  const int unit = unit_of(P.type), vec = whole(P.x, P.type, unit, P.x_stride), vec_codes = P.width % unit == 0 && ((uintptr_t)P.codes & 7) == 0;
+  const int unit = unit_of(P.type);
+  const bool vec = whole(P.x, P.type, unit, P.x_stride, P.width) && ((uintptr_t)P.codes & 7) == 0;
   const dim3 grid = pack_grid(P, unit);
-  if (P.type == 0) pack_kernel<__half><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
-  else if (P.type == 1) pack_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
-  else pack_kernel<float><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
-  return launch_status();
+  return by_type(P.type, P.type, [&](auto t, auto) {
+    using T = decltype(t);
+    vec ? pack_kernel<T, true><<<grid, kThreads, 0, st>>>(P) : pack_kernel<T, false><<<grid, kThreads, 0, st>>>(P);
+    return launch_status();
+  });
 }
 int launch_unpack(const PackParams& P, cudaStream_t st) {
-  const int vec = whole(P.y, P.type, unit_of(P.type), P.width), vec_codes = P.width % kCodes == 0 && ((uintptr_t)P.codes & 15) == 0;
+  const bool vec = whole(P.y, P.type, unit_of(P.type), P.width) && P.width % kCodes == 0 && ((uintptr_t)P.codes & 15) == 0;
   const dim3 grid = pack_grid(P, kCodes);
-  if (P.type == 0) unpack_kernel<__half><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
-  else if (P.type == 1) unpack_kernel<__nv_bfloat16><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
-  else unpack_kernel<float><<<grid, kThreads, 0, st>>>(P, vec, vec_codes);
-  return launch_status();
+  return by_type(P.type, P.type, [&](auto t, auto) {
+    using T = decltype(t);
+    vec ? unpack_kernel<T, true><<<grid, kThreads, 0, st>>>(P) : unpack_kernel<T, false><<<grid, kThreads, 0, st>>>(P);
+    return launch_status();
+  });
 }
 
 }  // namespace sq
