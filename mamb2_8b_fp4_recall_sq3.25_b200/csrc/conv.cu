@@ -112,26 +112,20 @@ template <typename T, int V> __device__ __forceinline__ float encode(const Value
   const float top = __uint_as_float(m);
   float scale;
   uint32_t q[V];
-  bool plain = top >= 1e-28f && top <= 3.0e38f;
-  if (plain) {
-    // top / 127, its remainder taken once more: the quotient's rounding.  x times about 1 / scale tells the code but
-    // where it lies next to a half.
+  if (top >= 1e-20f && top <= 3.0e38f) {
+    // Quotients by the reciprocal: product, remainder, and the remainder's share give the quotient's rounding where
+    // nothing underflows (Markstein).
     constexpr float kPart = 1.0f / 127.0f;
     const float guess = top * kPart;
     scale = fmaf(fmaf(-127.0f, guess, top), kPart, guess);
-    const float inverse = __fdividef(1.0f, scale);
-    float off = 0.f;
+    const float inverse = __frcp_rn(scale);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const float t = f[i] * inverse, whole = t + kWhole;
-      off = fmaxf(off, fabsf(t - (whole - kWhole)));
-      q[i] = __float_as_uint(whole);
+      const float t = f[i] * inverse;
+      q[i] = __float_as_uint(fmaf(fmaf(-t, scale, f[i]), inverse, t) + kWhole);
     }
-    plain = off <= 0.4999f;
-  } else {
+  } else {                                          // tiny ones by division; none of zeros, infinities and NaN
     scale = __fdiv_rn(top, 127.0f);
-  }
-  if (!plain) {                                     // by the quotients; none of zeros, infinities and NaN
 #pragma unroll
     for (int i = 0; i < V; ++i)
       q[i] = scale > 0.f && scale <= 3.0e38f ? (uint32_t)__float2int_rn(fmaxf(-127.f, fminf(127.f, __fdiv_rn(f[i], scale)))) : 0;
