@@ -510,7 +510,7 @@ typedef struct sq_conv_scan_step_args {
 int sq_conv_scan_step(const sq_conv_scan_step_args* args, void* stream);
 
 /* Activations in 8 bits: in a row of x [rows,width] each 128 neighbouring values (the last block may have fewer) share
- * scale = max|x| / 127 (fp32) and are kept as codes rint(x / scale) in [-127, 127]; scales [rows, ceil(width/128)].  A block
+ * scale = max|x| (1 / 127), an fp32 product, and are kept as codes rint(x / scale) in [-127, 127]; scales [rows, ceil(width/128)].  A block
  * with a NaN or an infinity comes back as NaN.  sq_unpack_activations writes code * scale, rounded to `type`. */
 int sq_pack_activations(const void* x, int64_t row_stride, int64_t rows, int width, int type, int8_t* codes, float* scales, void* stream);
 int sq_unpack_activations(const int8_t* codes, const float* scales, int64_t rows, int width, int type, void* out, void* stream);

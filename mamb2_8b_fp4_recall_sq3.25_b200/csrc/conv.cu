@@ -8,7 +8,8 @@
 // that each input is read once but for the strips' edges.  The backward pass computes z again from the input (or from
 // its 8-bit codes); sums for weights and bias are kept a strip and added in order by a second kernel.
 //
-// 8 bits: 128 neighbouring channels of a token share the scale max|x| / 127; a code is x / scale rounded to even.
+// 8 bits: 128 neighbouring channels of a token share the scale max|x| (1 / 127), an fp32 product; a code is the fp32 quotient
+// x / scale rounded to even, at most 127.
 #include "conv.cuh"
 #include "device_util.cuh"
 #include "logits_util.cuh"
@@ -110,14 +111,11 @@ template <typename T, int V> __device__ __forceinline__ float encode(const Value
 #pragma unroll
   for (int o = kPackBlock / V / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
   const float top = __uint_as_float(m);
-  float scale;
+  const float scale = top * (1.0f / 127.0f);
   uint32_t q[V];
   if (top >= 1e-20f && top <= 3.0e38f) {
     // Quotients by the reciprocal: product, remainder, and the remainder's share give the quotient's rounding where
     // nothing underflows (Markstein).
-    constexpr float kPart = 1.0f / 127.0f;
-    const float guess = top * kPart;
-    scale = fmaf(fmaf(-127.0f, guess, top), kPart, guess);
     const float inverse = __frcp_rn(scale);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -125,7 +123,6 @@ template <typename T, int V> __device__ __forceinline__ float encode(const Value
       q[i] = __float_as_uint(fmaf(fmaf(-t, scale, f[i]), inverse, t) + kWhole);
     }
   } else {                                          // tiny ones by division; none of zeros, infinities and NaN
-    scale = __fdiv_rn(top, 127.0f);
 #pragma unroll
     for (int i = 0; i < V; ++i)
       q[i] = scale > 0.f && scale <= 3.0e38f ? (uint32_t)__float2int_rn(fmaxf(-127.f, fminf(127.f, __fdiv_rn(f[i], scale)))) : 0;

@@ -1,6 +1,6 @@
 """Activations in 8 bits (sq_pack_activations, sq_unpack_activations), for what a backward pass keeps.
 
-In the last axis each 128 neighbouring values (the last block may have fewer) share scale = max|x| / 127 in fp32 and
+In the last axis each 128 neighbouring values (the last block may have fewer) share scale = max|x| (1 / 127) in fp32 and
 are kept as codes rint(x / scale): 1.03 bytes a value, off by at most half a scale.  A block with a NaN or an infinity
 comes back as NaN.  `causal_conv(..., keep='int8')` and `conv_scan(..., keep='int8')` keep their input in this form.
 """
