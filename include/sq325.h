@@ -491,6 +491,15 @@ int sq_causal_conv_backward(const sq_causal_conv_args* args, void* stream);
 int sq_causal_conv_step(const void* x, int64_t x_batch_stride, void* state, const void* weight, const void* bias, void* y,
                         int batch, int channels, int taps, int silu, int type, int weight_type, void* stream);
 
+/* Convolution (silu) and scan as one: conv's output [batch, length, heads*dim + 2*groups*128] is x, B and C side by side, and
+ * goes to the scan in scaled fp16 (11 bits of a tile's largest value, whatever `type`), not in `type`.  conv's y, and scan's
+ * x, B, C, dx, dB and dC are not used; both have the same lengths.  The forward reads conv's x, or the codes where x is
+ * NULL, and so does the backward, whose results are conv's dx, dweight, dbias, dstate_in and scan's ddt, dA, dD, ddt_bias,
+ * dstate_in.  scan's workspace: sq_conv_scan_workspace(...) bytes. */
+int64_t sq_conv_scan_workspace(int batch, int length, int heads, int dim, int groups, int backward);
+int sq_conv_scan_forward(const sq_causal_conv_args* conv, const sq_selective_args* scan, void* stream);
+int sq_conv_scan_backward(const sq_causal_conv_args* conv, const sq_selective_args* scan, void* stream);
+
 /* One token of convolution (silu) and recurrence, as sq_causal_conv_step and sq_selective_step one behind the other but
  * with the convolution's output in fp32 between them: xbc [batch, heads*dim + 2*groups*128] holds x, B and C side by side.
  * conv_state [batch,taps-1,channels] in `type` (SQ_F16, SQ_BF16) and state are updated in place.  workspace: batch *

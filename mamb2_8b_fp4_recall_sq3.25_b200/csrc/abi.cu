@@ -962,7 +962,8 @@ int sq_distill_loss_grad(const sq_distill_args* a, void* stream) {
 namespace {
 constexpr int kMaxGrid = 65535;      // of a grid's second and third dimension
 
-int selective_params(const sq_selective_args* a, const char* who, bool backward, SelectiveParams& P) {
+// tiled: x, B and C come from a convolution and are not looked at; `extra` bytes of the workspace are another's.
+int selective_params(const sq_selective_args* a, const char* who, bool backward, SelectiveParams& P, bool tiled = false, int64_t extra = 0) {
   if (!a) return fail(SQ_EINVAL, std::string(who) + ": null argument");
   const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
   if (a->type != SQ_F16 && a->type != SQ_BF16) return bad("type must be SQ_F16 or SQ_BF16");
@@ -970,7 +971,7 @@ int selective_params(const sq_selective_args* a, const char* who, bool backward,
   if (a->heads % a->groups) return bad("heads must be divisible by B/C groups");
   if (a->dim > kScanMaxDim || a->length > 1 << 24 || a->batch > kMaxGrid) return bad("batch, length or dim is too large");
   if ((int64_t)a->heads * ((a->dim + kScanTile - 1) / kScanTile) > kMaxGrid) return bad("heads is too large");
-  if (!a->x || !a->dt || !a->A || !a->B || !a->C || !a->workspace) return bad("null pointer argument");
+  if (!a->dt || !a->A || !a->workspace || (!tiled && (!a->x || !a->B || !a->C))) return bad("null pointer argument");
   if (!aligned(a->x, 2) || !aligned(a->dt, 2) || !aligned(a->B, 2) || !aligned(a->C, 2) || !aligned(a->A, 4) ||
       !aligned(a->state_in, 4) || !aligned(a->lengths, 4) || !aligned(a->workspace, 256))
     return bad("misaligned argument");
@@ -978,7 +979,8 @@ int selective_params(const sq_selective_args* a, const char* who, bool backward,
   if ((a->D && (!number_type(a->d_type) || !aligned(a->D, a->d_type == SQ_F32 ? 4 : 2))) ||
       (a->dt_bias && (!number_type(a->bias_type) || !aligned(a->dt_bias, a->bias_type == SQ_F32 ? 4 : 2))))
     return bad("unknown type or misaligned D or dt_bias");
-  if (a->workspace_bytes < selective_workspace(a->batch, a->length, a->heads, a->dim, a->groups, backward)) return bad("workspace too small");
+  if (a->workspace_bytes < selective_workspace(a->batch, a->length, a->heads, a->dim, a->groups, backward, tiled) + extra)
+    return bad("workspace too small");
   P = SelectiveParams{};
   P.batch = a->batch; P.length = a->length; P.heads = a->heads; P.dim = a->dim; P.groups = a->groups; P.type = a->type;
   P.x = a->x; P.x_sb = a->x_batch_stride; P.x_st = a->x_token_stride;
@@ -987,14 +989,14 @@ int selective_params(const sq_selective_args* a, const char* who, bool backward,
   P.B = a->B; P.b_sb = a->b_batch_stride; P.b_st = a->b_token_stride;
   P.C = a->C; P.c_sb = a->c_batch_stride; P.c_st = a->c_token_stride;
   P.D = a->D; P.d_type = a->d_type; P.dt_bias = a->dt_bias; P.bias_type = a->bias_type;
-  P.state_in = a->state_in; P.lengths = a->lengths; P.workspace = a->workspace;
+  P.state_in = a->state_in; P.lengths = a->lengths; P.workspace = a->workspace; P.tiled = tiled;
   return device_error_word(&P.err);
 }
 }  // namespace
 
 int64_t sq_selective_workspace(int batch, int length, int heads, int dim, int groups, int backward) {
   if (batch < 1 || length < 1 || heads < 1 || dim < 1 || groups < 1 || heads % groups) return -1;
-  return selective_workspace(batch, length, heads, dim, groups, backward != 0);
+  return selective_workspace(batch, length, heads, dim, groups, backward != 0, false);
 }
 
 int sq_selective_forward(const sq_selective_args* a, void* stream) {
@@ -1132,6 +1134,75 @@ int sq_causal_conv_step(const void* x, int64_t x_batch_stride, void* state, cons
   P.batch = batch; P.channels = channels; P.taps = taps; P.silu = silu; P.type = type; P.weight_type = weight_type;
   P.x = x; P.x_sb = x_batch_stride; P.weight = weight; P.bias = bias; P.state = state; P.y = y;
   return check(launch_conv_step(P, (cudaStream_t)stream), "causal_conv_step");
+}
+
+namespace {
+int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
+// Bytes of a conv_scan's workspace behind the scan's: the gradient of the convolution's output, and its own workspace.
+int64_t conv_scan_extra(int batch, int length, int heads, int dim, int groups, bool backward) {
+  if (!backward) return 0;
+  const int64_t width = (int64_t)heads * dim + 256ll * groups;
+  return round256((int64_t)batch * length * width * 2) + conv_workspace(batch, length, (int)width);
+}
+int conv_scan_params(const sq_causal_conv_args* c, const sq_selective_args* a, const char* who, bool backward, ConvParams& C, SelectiveParams& P) {
+  if (!a) return fail(SQ_EINVAL, std::string(who) + ": null argument");
+  if (int s = conv_params(c, who, C)) return s;
+  const auto bad = [&](const char* what) { return fail(SQ_EINVAL, std::string(who) + ": " + what); };
+  if (a->heads < 1 || a->dim < 1 || a->groups < 1) return bad("positive geometry required");
+  if (c->batch != a->batch || c->length != a->length || c->type != a->type || c->channels != (int64_t)a->heads * a->dim + 256ll * a->groups)
+    return bad("the convolution's geometry is not the scan's");
+  if (!c->silu) return bad("the convolution before a scan ends in silu");
+  if (c->lengths != a->lengths) return bad("the convolution's lengths are not the scan's");
+  if (c->x) C.codes = nullptr;
+  return selective_params(a, who, backward, P, true, conv_scan_extra(a->batch, a->length, a->heads, a->dim, a->groups, backward));
+}
+}  // namespace
+
+int64_t sq_conv_scan_workspace(int batch, int length, int heads, int dim, int groups, int backward) {
+  if (batch < 1 || length < 1 || heads < 1 || dim < 1 || groups < 1 || heads % groups) return -1;
+  return selective_workspace(batch, length, heads, dim, groups, backward != 0, true) +
+         conv_scan_extra(batch, length, heads, dim, groups, backward != 0);
+}
+
+int sq_conv_scan_forward(const sq_causal_conv_args* c, const sq_selective_args* a, void* stream) {
+  ConvParams C;
+  SelectiveParams P;
+  if (int s = conv_scan_params(c, a, "conv_scan_forward", false, C, P)) return s;
+  if (!a->y) return fail(SQ_EINVAL, "conv_scan_forward: null y");
+  if (!aligned(a->y, 2) || !aligned(a->state_out, 4) || !aligned(c->state_out, 2)) return fail(SQ_EINVAL, "conv_scan_forward: misaligned output");
+  if (c->state_out && c->state_out == c->state_in) return fail(SQ_EINVAL, "conv_scan_forward: state_out must not be state_in");
+  P.y = a->y; P.y_sb = a->y_batch_stride; P.y_st = a->y_token_stride; P.state_out = a->state_out;
+  C.state_out = c->state_out;
+  if (int s = check(launch_conv_tiles(C, selective_tiles(P, false), (cudaStream_t)stream), "conv_scan_forward")) return s;
+  if (C.state_out)
+    if (int s = check(launch_conv_last(C, (cudaStream_t)stream), "conv_scan_forward")) return s;
+  return check(launch_selective_forward(P, (cudaStream_t)stream), "conv_scan_forward");
+}
+
+int sq_conv_scan_backward(const sq_causal_conv_args* c, const sq_selective_args* a, void* stream) {
+  ConvParams C;
+  SelectiveParams P;
+  if (int s = conv_scan_params(c, a, "conv_scan_backward", true, C, P)) return s;
+  const auto bad = [](const char* what) { return fail(SQ_EINVAL, std::string("conv_scan_backward: ") + what); };
+  if (!a->dy || !a->ddt || !c->dx) return bad("null gradient");
+  const size_t w = c->weight_type == SQ_F32 ? 4 : 2;
+  if (!aligned(a->dy, 2) || !aligned(a->dstate_out, 4) || !aligned(a->ddt, 2) || !aligned(a->dA, 4) || !aligned(a->dD, a->d_type == SQ_F32 ? 4 : 2) ||
+      !aligned(a->ddt_bias, a->bias_type == SQ_F32 ? 4 : 2) || !aligned(a->dstate_in, 4) || !aligned(c->dx, 2) || !aligned(c->dstate_out, 2) ||
+      !aligned(c->dstate_in, 2) || !aligned(c->dweight, w) || !aligned(c->dbias, w))
+    return bad("misaligned gradient");
+  const int64_t inner = (int64_t)a->heads * a->dim, width = inner + 256ll * a->groups;
+  uint16_t* dz = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(a->workspace) +
+                                             selective_workspace(a->batch, a->length, a->heads, a->dim, a->groups, true, true));
+  P.dy = a->dy; P.dy_sb = a->dy_batch_stride; P.dy_st = a->dy_token_stride; P.dstate_out = a->dstate_out;
+  P.dx = dz; P.dB = dz + inner; P.dC = dz + inner + 128ll * a->groups;
+  P.dx_sb = P.dg_sb = a->length * width; P.dx_st = P.dg_st = width; P.ddt = a->ddt;
+  P.dA = a->dA; P.dD = a->D ? a->dD : nullptr; P.dbias = a->dt_bias ? a->ddt_bias : nullptr; P.dstate_in = a->dstate_in;
+  if (int s = check(launch_conv_tiles(C, selective_tiles(P, true), (cudaStream_t)stream), "conv_scan_backward")) return s;
+  if (int s = check(launch_selective_backward(P, (cudaStream_t)stream), "conv_scan_backward")) return s;
+  C.dy = dz; C.dy_sb = a->length * width; C.dy_st = width; C.dstate_out = c->dstate_out;
+  C.dx = c->dx; C.dstate_in = c->dstate_in; C.dweight = c->dweight; C.dbias = c->dbias;
+  C.workspace = reinterpret_cast<float*>(reinterpret_cast<char*>(dz) + round256((int64_t)a->batch * a->length * width * 2));
+  return check(launch_conv_backward(C, (cudaStream_t)stream), "conv_scan_backward");
 }
 
 int sq_conv_scan_step(const sq_conv_scan_step_args* a, void* stream) {

@@ -11,6 +11,7 @@
 // 8 bits: 128 neighbouring channels of a token share the scale max|x| (1 / 127), an fp32 product; a code is the fp32 quotient
 // x / scale rounded to even, at most 127.
 #include "conv.cuh"
+#include "selective.cuh"
 #include "device_util.cuh"
 #include "logits_util.cuh"
 
@@ -490,6 +491,110 @@ __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams
   }
 }
 
+// ---------------------------------------------------------------- tiles for a scan
+// Four channels c .. c + 3 of a token, `n` of them there; codes may lie on both sides of a block's border.
+template <typename T, bool CODES>
+__device__ __forceinline__ void four_channels(const ConvParams& P, int b, int t, int c, int n, bool vec, float (&f)[4]) {
+  if (t < 0) {
+    if (P.state_in && t >= 1 - P.taps) {
+      const long long at = ((long long)b * (P.taps - 1) + t + P.taps - 1) * P.channels + c;
+      load_values<T, 4>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = 0.f;
+    }
+  } else if constexpr (CODES) {
+    const long long row = (long long)b * P.length + t;
+    const int8_t* q = P.codes + row * P.channels + c;
+    const float* s = P.scales + row * ((P.channels + kPackBlock - 1) / kPackBlock);
+    if (vec) {
+      decode<4>(raw_values<int8_t, 4>(q, true, 4), s[c / kPackBlock], f);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = i < n ? (float)q[i] * s[(c + i) / kPackBlock] : 0.f;
+    }
+  } else {
+    load_values<T, 4>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + t * P.x_st + c, vec, n, f);
+  }
+}
+
+// One CTA: a chunk's tile of x (64 channels of a head) or of B or C (128 of a group).  A thread has four channels of
+// TOKENS neighbouring tokens in registers; the tile's largest value gives its scale.
+template <typename T, typename WT, bool CODES, int TOKENS>
+__device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk, int c0, int cols, int rows, uint16_t* out, float* back,
+                                          uint32_t* tops) {
+  constexpr int kWideTile = TOKENS == 8 ? 16 : 32;                     // threads side by side: of 64 or 128 channels
+  const int at = threadIdx.x % kWideTile, c = c0 + at * 4, n = max(0, min(4, cols - at * 4)), r0 = threadIdx.x / kWideTile * TOKENS;
+  const bool vec = n == 4 && c % 4 == 0 && P.channels % 4 == 0 &&
+                   (CODES ? ((uintptr_t)P.codes & 3) == 0 : (((uintptr_t)P.x & 7) == 0 && ((P.x_sb | P.x_st) & 3) == 0));
+  float z[TOKENS][4];
+  float x[3][4];
+  const Taps<WT, 4> W(P.weight, P.bias, P.taps, n > 0 ? c : 0, n);
+  const int t0 = chunk * kScanChunk + r0;
+  uint32_t top = 0;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) four_channels<T, CODES>(P, b, n > 0 && r0 < rows ? t0 - 3 + k : -kTaps, n > 0 ? c : 0, n, vec, x[k]);
+#pragma unroll
+  for (int j = 0; j < TOKENS; ++j) {
+    const bool in = n > 0 && r0 + j < rows;
+    float f[4];
+    four_channels<T, CODES>(P, b, in ? t0 + j : -kTaps, n > 0 ? c : 0, n, vec, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float v = conv_at<WT, 4>(W, P.taps, i, x[0][i], x[1][i], x[2][i], f[i]);
+      z[j][i] = in && i < n ? v * sigmoid<T>(v) : 0.f;
+      top = max(top, __float_as_uint(z[j][i]) & 0x7fffffffu);
+      x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) top = max(top, tops[k]);
+  int e = (int)(top >> 23) - 140;                                      // to [2^13, 2^14)
+  e = top ? max(-60, min(60, e)) : 0;
+  const float there = __uint_as_float((uint32_t)(127 - e) << 23);
+  if (threadIdx.x == 0) *back = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+  for (int j = 0; j < TOKENS; ++j) {
+    const int row = r0 + j, piece = at / 2;
+    const __half2 lo = __floats2half2_rn(z[j][0] * there, z[j][1] * there), hi = __floats2half2_rn(z[j][2] * there, z[j][3] * there);
+    char* p = reinterpret_cast<char*>(out) + (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4) + (at & 1) * 8;
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  }
+}
+template <typename T, typename WT, bool CODES>
+__global__ void __launch_bounds__(256) conv_tiles_kernel(const ConvParams P, const ConvTiles A) {
+  __shared__ uint32_t tops[8];
+  const int chunk = blockIdx.x, b = blockIdx.z, u = blockIdx.y;
+  const int rows = min(kScanChunk, tokens_of(P, b) - chunk * kScanChunk);
+  if (rows <= 0) return;                                               // not read
+  const long long bc = (long long)b * A.chunks + chunk;
+  if (u < A.units) {
+    const int ptiles = A.units / A.heads, h = u / ptiles, p0 = (u % ptiles) * kScanTile, cols = min(kScanTile, A.dim - p0);
+    conv_tile<T, WT, CODES, 8>(P, b, chunk, h * A.dim + p0, cols, rows, A.x + (bc * A.units + u) * (kScanChunk * kScanTile),
+                               A.xback + bc * A.units + u, tops);
+  } else {
+    const int i = u - A.units, g = i >> 1;
+    const long long at = bc * A.groups + g;
+    conv_tile<T, WT, CODES, 16>(P, b, chunk, A.heads * A.dim + (i & 1 ? A.groups * 128 : 0) + g * 128, 128, rows,
+                                (i & 1 ? A.c : A.b) + at * (kScanChunk * 128), (i & 1 ? A.cback : A.bback) + at, tops);
+  }
+}
+// The last inputs of a sequence.
+template <typename T, bool CODES>
+__global__ void __launch_bounds__(kThreads) conv_last_kernel(const ConvParams P) {
+  const int c = (blockIdx.x * kThreads + threadIdx.x) * 4, b = blockIdx.y, n = min(4, P.channels - c), back = P.taps - 1;
+  if (n <= 0) return;
+  const int len = tokens_of(P, b);
+  for (int j = 0; j < back; ++j) {
+    float f[4];
+    four_channels<T, CODES>(P, b, len - back + j, c, n, false, f);
+    store_values<T, 4>(reinterpret_cast<T*>(P.state_out) + ((long long)b * back + j) * P.channels + c, false, n, f);
+  }
+}
+
 // The strips' sums for a channel's tap or bias, in order: eight threads share a channel's strips.
 template <typename WT>
 __global__ void __launch_bounds__(256) conv_weights_kernel(const ConvParams P, int strips) {
@@ -632,6 +737,29 @@ template <typename F> int by_type(int type, int weight_type, F f) {
 }
 
 }  // namespace
+
+int launch_conv_tiles(const ConvParams& P, const ConvTiles& A, cudaStream_t st) {
+  const dim3 grid(A.chunks, A.units + 2 * A.groups, P.batch);
+  return by_type(P.type, P.weight_type, [&](auto t, auto w) {
+    using T = decltype(t);
+    using WT = decltype(w);
+    if constexpr (sizeof(T) == 2) {
+      if (P.codes) conv_tiles_kernel<T, WT, true><<<grid, 256, 0, st>>>(P, A);
+      else conv_tiles_kernel<T, WT, false><<<grid, 256, 0, st>>>(P, A);
+      return launch_status();
+    }
+    return (int)kEInval;
+  });
+}
+int launch_conv_last(const ConvParams& P, cudaStream_t st) {
+  const dim3 grid((P.channels + 4 * kThreads - 1) / (4 * kThreads), P.batch);
+  return by_type(P.type, P.weight_type, [&](auto t, auto) {
+    using T = decltype(t);
+    if (P.codes) conv_last_kernel<T, true><<<grid, kThreads, 0, st>>>(P);
+    else conv_last_kernel<T, false><<<grid, kThreads, 0, st>>>(P);
+    return launch_status();
+  });
+}
 
 long long conv_workspace(int batch, int length, int channels) {
   const int strip = strip_of(batch, length, channels, kLeast, kMost);

@@ -41,6 +41,11 @@ struct PackParams {
   void* y;                                          // unpacked, contiguous
 };
 
+struct ConvTiles;
+// The convolution (silu) of P's x or codes as a scan's tiles; P's channels are x, B and C side by side.
+int launch_conv_tiles(const ConvParams& p, const ConvTiles& tiles, cudaStream_t stream);
+// state_out alone, of x or codes.
+int launch_conv_last(const ConvParams& p, cudaStream_t stream);
 long long conv_workspace(int batch, int length, int channels);
 int launch_conv_forward(const ConvParams& p, cudaStream_t stream);
 int launch_conv_backward(const ConvParams& p, cudaStream_t stream);

@@ -199,6 +199,8 @@ struct Space {
   float* smax;                        // [B][H][nc]: the largest s of a chunk
   uint16_t *bt, *ct;                  // [B][nc][G][128][128]: B and C as shared memory holds them
   float *bback, *cback;               // [B][nc][G]: what brings them back
+  uint16_t *xt, *yt;                  // [B][nc][units][128][64]: x and dy in the same form, behind a convolution
+  float *xback, *yback;               // [B][nc][units]
   uint16_t *h, *g;                    // [B][nc][units][2][8][128][8]: states entering a chunk, gradients of those leaving it
   float2 *hs, *gs;                    // [B][nc][units]: scale of the state, scale of the chunk's weighted tokens
   float2* parts;                      // [B][units][lp]: gradient of A s, gradient of s through the tokens
@@ -225,7 +227,7 @@ int splits_of(long long tiles, int units, int places, double once) {
   return best;
 }
 
-Space space_of(const SelectiveParams& P, bool backward) {
+Space space_of(const SelectiveParams& P, bool backward, bool tiled) {
   Space w{};
   w.nc = (P.length + Q - 1) / Q;
   w.lp = (long long)w.nc * Q;
@@ -241,6 +243,14 @@ Space space_of(const SelectiveParams& P, bool backward) {
   w.bback = reinterpret_cast<float*>(take(bc * P.groups * 4));
   w.cback = reinterpret_cast<float*>(take(bc * P.groups * 4));
   w.smax = reinterpret_cast<float*>(take(bh * w.nc * 4));
+  if (tiled) {
+    w.xt = reinterpret_cast<uint16_t*>(take(bcu * kTile64));
+    w.xback = reinterpret_cast<float*>(take(bcu * 4));
+    if (backward) {
+      w.yt = reinterpret_cast<uint16_t*>(take(bcu * kTile64));
+      w.yback = reinterpret_cast<float*>(take(bcu * 4));
+    }
+  }
   const long long plane = (long long)kN * TP * 2 * 2;
   w.h = reinterpret_cast<uint16_t*>(take(bcu * plane));
   w.hs = reinterpret_cast<float2*>(take(bcu * 8));
@@ -358,23 +368,35 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
   const int c = blockIdx.x, b = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int len = tokens_of(P, b), rows = min(Q, len - c * Q);
   if ((int)blockIdx.y >= head_blocks) {
-    const int i = blockIdx.y - head_blocks, g = i >> 1;
+    const int i = blockIdx.y - head_blocks;
     if (rows <= 0) return;                               // not read
-    const long long st = i & 1 ? P.c_st : P.b_st;
-    const T* src = reinterpret_cast<const T*>(i & 1 ? P.C : P.B) + (long long)b * (i & 1 ? P.c_sb : P.b_sb) + (long long)c * Q * st + g * kN;
-    const bool vec = vector_ok(src, st, 0, kN);
-    const int j = threadIdx.x & 15;
-    uint4 u[8];
+    // a tile of B or C [128][128], or behind a convolution one of dy [128][64]
+    const bool narrow = P.tiled;
+    const int g = i >> 1, u = i, pieces = narrow ? 8 : 16, j = threadIdx.x & (pieces - 1), step = kThreads / pieces;
+    const long long st = narrow ? P.dy_st : i & 1 ? P.c_st : P.b_st;
+    const T* src;
+    int cols = kN;
+    if (narrow) {
+      const int p0 = (u % W.ptiles) * TP;
+      cols = min(TP, P.dim - p0);
+      src = reinterpret_cast<const T*>(P.dy) + (long long)b * P.dy_sb + (long long)c * Q * st + (long long)(u / W.ptiles) * P.dim + p0;
+    } else {
+      src = reinterpret_cast<const T*>(i & 1 ? P.C : P.B) + (long long)b * (i & 1 ? P.c_sb : P.b_sb) + (long long)c * Q * st + g * kN;
+    }
+    const bool vec = vector_ok(src, st, 0, cols);
+    const int count = pieces / 2;
+    uint4 u4[8];
     uint32_t m = 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const int r = (threadIdx.x >> 4) + k * 16;
+      u4[k] = make_uint4(0, 0, 0, 0);
+      const int r = threadIdx.x / pieces + k * step;
       const T* p = src + (long long)r * st + j * 8;
-      u[k] = r >= rows ? make_uint4(0, 0, 0, 0) : vec ? *reinterpret_cast<const uint4*>(p) : ragged_piece(p, 8);
+      if (k < count && r < rows && j * 8 < cols) u4[k] = vec ? *reinterpret_cast<const uint4*>(p) : ragged_piece(p, cols - j * 8);
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t w[4] = {u[k].x, u[k].y, u[k].z, u[k].w};
+      const uint32_t w[4] = {u4[k].x, u4[k].y, u4[k].z, u4[k].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) m = __vmaxu2(m, w[e] & 0x7fff7fffu);
     }
@@ -384,14 +406,13 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
     m = 0;
 #pragma unroll
     for (int k = 0; k < kThreads / 32; ++k) m = max(m, tops[k]);
-    const float2 sc = scale_of(__float_as_uint(to_f32(from_bits<T>(m))), 110);
-    const long long at = ((long long)b * W.nc + c) * P.groups + g;
-    char* out = reinterpret_cast<char*>((i & 1 ? W.ct : W.bt) + at * (Q * kN));
+    const float2 sc = scale_of(__float_as_uint(to_f32(from_bits<T>(m))), narrow ? 60 : 110);
+    const long long bc = (long long)b * W.nc + c, at = narrow ? bc * W.units + u : bc * P.groups + g;
+    char* out = reinterpret_cast<char*>(narrow ? W.yt + at * (Q * TP) : (i & 1 ? W.ct : W.bt) + at * (Q * kN));
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      *reinterpret_cast<uint4*>(out + piece2((threadIdx.x >> 4) + k * 16, j)) = pack8<__half>(mul8(unpack8<T>(u[k]), sc.x));
-    }
-    if (threadIdx.x == 0) (i & 1 ? W.cback : W.bback)[at] = sc.y;
+    for (int k = 0; k < 8; ++k)
+      if (k < count) *reinterpret_cast<uint4*>(out + piece2(threadIdx.x / pieces + k * step, j)) = pack8<__half>(mul8(unpack8<T>(u4[k]), sc.x));
+    if (threadIdx.x == 0) (narrow ? W.yback : i & 1 ? W.cback : W.bback)[at] = sc.y;
     return;
   }
   const int h0 = blockIdx.y * kPrepHeads, hl = threadIdx.x & 7;
@@ -459,12 +480,12 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
 // remainder.  Written before each chunk: the state that enters it, value and (LO) remainder.
 constexpr uint32_t kPassX = 2 * kTile128, kPassW = kPassX + kTile64, kPassBytes = kPassW + 2 * kTile64, kPassSmem = kPassBytes + 64;
 
-template <typename T, bool REV, bool LO>
+template <typename T, bool REV, bool LO, bool TILED>
 __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const SelectiveParams P, const Space W) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPassBytes);           // tensor cores, tile 0, tile 1
-  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kPassBytes + 24);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPassBytes);           // tensor cores, tile 0, tile 1, tokens (TILED)
+  uint32_t* slot = reinterpret_cast<uint32_t*>(smem + kPassBytes + 48);
   uint32_t* tops = reinterpret_cast<uint32_t*>(smem + kPassBytes + 32);      // [2][2]: of the tokens, of the state
   const int u = blockIdx.x, b = blockIdx.y;
   const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, g = h / (P.heads / P.groups);
@@ -484,9 +505,12 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
   const long long state_at = (((long long)b * P.heads + h) * P.dim + p0) * kN + n;
   if (threadIdx.x < 4) tops[threadIdx.x] = 0;
   launch_dependents();
-  const uint32_t tmem = tensor_begin<128>(bars, 3, slot);
+  const uint32_t tmem = tensor_begin<128>(bars, 4, slot);
   wait_for_launch();
-  Gate done{smem_u32(bars), 0};
+  Gate done{smem_u32(bars), 0}, tokens{smem_u32(bars + 3), 0};
+  using X = typename std::conditional<TILED, __half, T>::type;
+  const uint16_t* xt = TILED ? (REV ? W.yt : W.xt) + ((long long)b * W.nc * W.units + u) * (Q * TP) : nullptr;
+  const float* xback = TILED ? (REV ? W.yback : W.xback) + (long long)b * W.nc * W.units + u : nullptr;
   bool ok = true;
   const uint32_t mine = tmem + ((uint32_t)quad << 21) + (uint32_t)half * 32;
 
@@ -496,15 +520,23 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
       mbar_expect_tx(smem_u32(bars + 1 + (i & 1)), kTile128);
       bulk_load(base + (i & 1) * kTile128, tiles + (long long)c * P.groups * (Q * kN), kTile128, smem_u32(bars + 1 + (i & 1)));
     }
-    load_tile<T>(base + kPassX, tok + (long long)c * Q * tok_st, tok_st, len - c * Q, cols, tok_vec);
-    cp_commit();
+    if constexpr (TILED) {
+      if (threadIdx.x == 0) {
+        mbar_expect_tx(tokens.bar, kTile64);
+        bulk_load(base + kPassX, xt + (long long)c * W.units * (Q * TP), kTile64, tokens.bar);
+      }
+    } else {
+      load_tile<T>(base + kPassX, tok + (long long)c * Q * tok_st, tok_st, len - c * Q, cols, tok_vec);
+      cp_commit();
+    }
   };
-  float s, lh, ll, eh, el, back;                         // of the next chunk: my token's, the chunk's end's, the tile's
+  float s, lh, ll, eh, el, back, xb = 1.f;                         // of the next chunk: my token's, the chunk's end's, the tile's
   auto load_record = [&](int i) {
     const int c = REV ? nc - 1 - i : i;
     const float* r = recs + (long long)c * (kRecord * Q);
     s = r[n]; lh = r[Q + n]; ll = r[2 * Q + n]; eh = r[2 * Q - 1]; el = r[3 * Q - 1];
     back = tile_back[(long long)c * P.groups];
+    if (TILED) xb = xback[(long long)c * W.units];
   };
   if (nc > 0) { load(0); load_record(0); }
   float2 S[16];
@@ -514,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
     S[i].x = first && p < cols ? first[state_at + (long long)p * kN] : 0.f;
     S[i].y = first && p + 1 < cols ? first[state_at + (long long)(p + 1) * kN] : 0.f;
   }
-  using Pair = typename Two<T>::type;
+  using Pair = typename Two<X>::type;
   uint32_t parity = 0;                                   // of the tiles' barriers, a bit each
   for (int i = 0; i < nc; ++i) {
     const int c = REV ? nc - 1 - i : i;
@@ -527,8 +559,9 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
       const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(m));
       if ((threadIdx.x & 31) == 0) atomicMax(&tops[2 * (i & 1) + 1], bits);
     }
-    const float w = REV ? exp2f(lh + ll) : s * exp2f((eh - lh) + (el - ll)), decay = exp2f(eh + el), tback = back;
-    cp_wait<0>();
+    const float w = (REV ? exp2f(lh + ll) : s * exp2f((eh - lh) + (el - ll))) * xb, decay = exp2f(eh + el), tback = back;
+    if constexpr (TILED) tokens.wait(ok, P.err);
+    else cp_wait<0>();
     __syncthreads();
     uint4 v[4];
     const uint32_t none = 0;
@@ -550,7 +583,7 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         uint4 hi, lo;
-        split8<__half>(mul8(unpack8<T>(v[j]), ws), hi, lo);
+        split8<__half>(mul8(unpack8<X>(v[j]), ws), hi, lo);
         sts16(base + kPassW + piece(n, half * 4 + j), hi);
         sts16(base + kPassW + kTile64 + piece(n, half * 4 + j), lo);
       }
@@ -617,9 +650,10 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
 constexpr uint32_t kOutM = kTile128, kOutX = 2 * kTile128, kOutH = kOutX + kTile64, kOutRec = kOutH + kTile64, kRecBytes = 4 * Q * 4,
                    kOutTop = kOutRec + 2 * kRecBytes, kOutBar = kOutTop + 2 * Q * 4, kOutSmem = kOutBar + 32;
 
-template <typename T>
+template <typename T, bool TILED>
 __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams P, const Space W, int per) {
-  constexpr bool kScaled = std::is_same<T, __half>::value;
+  using X = typename std::conditional<TILED, __half, T>::type;
+  constexpr bool kScaled = std::is_same<X, __half>::value;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
   float* tops = reinterpret_cast<float*>(smem + kOutTop);
@@ -650,13 +684,17 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
   auto load_unit = [&](int u) {                          // state and record (one thread), tokens (all)
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
     if (threadIdx.x == 0) {
-      mbar_expect_tx(unit.bar, kRecBytes + (has_state ? kTile64 : 0));
+      mbar_expect_tx(unit.bar, kRecBytes + (has_state ? kTile64 : 0) + (TILED ? kTile64 : 0));
       bulk_load(base + kOutRec + ((u - u0) & 1) * kRecBytes, W.rec + (((long long)b * P.heads + h) * W.nc + c) * (kRecord * Q), kRecBytes, unit.bar);
       if (has_state) bulk_load(base + kOutH, W.h + (bc * W.units + u) * (2 * kN * TP), kTile64, unit.bar);
     }
-    const T* p = xc + (long long)h * P.dim + p0;
-    load_tile<T>(base + kOutX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
-    cp_commit();
+    if constexpr (TILED) {
+      if (threadIdx.x == 0) bulk_load(base + kOutX, W.xt + (bc * W.units + u) * (Q * TP), kTile64, unit.bar);
+    } else {
+      const T* p = xc + (long long)h * P.dim + p0;
+      load_tile<T>(base + kOutX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
+      cp_commit();
+    }
   };
   if (threadIdx.x == 0) {
     mbar_expect_tx(tiles.bar, 2 * kTile128);
@@ -697,8 +735,10 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
   for (int u = u0; u < u1; ++u) {
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
     const float* rec = reinterpret_cast<const float*>(smem + kOutRec + ((u - u0) & 1) * kRecBytes);
-    cp_wait<0>();
-    fence_async();
+    if constexpr (!TILED) {
+      cp_wait<0>();
+      fence_async();
+    }
     unit.wait(ok, P.err);
     __syncthreads();
     if (threadIdx.x == 0 && has_state && ok) {
@@ -727,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
             f.v[2 * e] = mul2(mul2(words2(r[k * 8 + 4 * e], r[k * 8 + 4 * e + 1]), pair(from)), make_float2(v.x, v.y));
             f.v[2 * e + 1] = mul2(mul2(words2(r[k * 8 + 4 * e + 2], r[k * 8 + 4 * e + 3]), pair(from)), make_float2(v.z, v.w));
           }
-          sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<T>(f));
+          sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<X>(f));
         }
       } else {
 #pragma unroll
@@ -743,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
             if (kScaled) v = mul2(v, pair(sc.x));
             f.v[e >> 1] = make_float2(col <= row ? v.x : 0.f, col + 1 <= row ? v.y : 0.f);
           }
-          sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<T>(f));
+          sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<X>(f));
         }
       }
     }
@@ -754,11 +794,11 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     __syncthreads();
     if (threadIdx.x == 0 && ok) {
       tc_fence_after();
-      mma<kK, kMn>(tmem + 192, base + kOutM, base + kOutX, idesc<T>(TP, false, true), 8, false);
+      mma<kK, kMn>(tmem + 192, base + kOutM, base + kOutX, idesc<X>(TP, false, true), 8, false);
       umma_commit(done.bar);
     }
-    const float d = number(P.D, P.d_type, h);
-    const float carry = has_state ? ex2(lh + ll) * W.hs[bc * W.units + u].x * cback : 0.f, mixed = sc.y * both_back;
+    const float xb = TILED ? W.xback[bc * W.units + u] : 1.f, d = number(P.D, P.d_type, h) * xb;
+    const float carry = has_state ? ex2(lh + ll) * W.hs[bc * W.units + u].x * cback : 0.f, mixed = sc.y * both_back * xb;
     done.wait(ok, P.err);
     tc_fence_after();
     if (u + 1 < u1) load_unit(u + 1);
@@ -769,7 +809,7 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     tc_fence_before();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      Eight f = mul8(unpack8<T>(x[j]), d);
+      Eight f = mul8(unpack8<X>(x[j]), d);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         f.v[e] = fma2(words2(y1[j * 8 + 2 * e], y1[j * 8 + 2 * e + 1]), pair(mixed), f.v[e]);
@@ -815,9 +855,10 @@ __device__ __forceinline__ float column_sums(float (&e)[32], int lane) {
   return e[0];
 }
 
-template <typename T>
+template <typename T, bool TILED>
 __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectiveParams P, const Space W, int per) {
-  constexpr bool kScaled = std::is_same<T, __half>::value;
+  using X = typename std::conditional<TILED, __half, T>::type;
+  constexpr bool kScaled = std::is_same<X, __half>::value;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
   float* rpairs = reinterpret_cast<float*>(smem + kGRow);        // [4][Q] each: r by pairs, r by states, q by states; [Q]: r by the token itself
@@ -859,9 +900,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   // One thread: the record and the states' values of a unit, and their remainders.  H lies at 0, G 16,384 bytes on.
   auto load_high = [&](int u) {
     const long long at = (bc * W.units + u) * (2 * kN * TP);
-    mbar_expect_tx(high.bar, kGRecBytes + ((int)has_h + (int)has_g) * kTile64);
+    mbar_expect_tx(high.bar, kGRecBytes + ((int)has_h + (int)has_g + (TILED ? 2 : 0)) * kTile64);
     bulk_load(base + kGRec + ((u - u0) & 1) * kGRecBytes, W.rec + (((long long)b * P.heads + u / W.ptiles) * W.nc + c) * (kRecord * Q), kGRecBytes,
               high.bar);
+    if (TILED) {
+      bulk_load(base + kGX, W.xt + (bc * W.units + u) * (Q * TP), kTile64, high.bar);
+      bulk_load(base + kGY + ((u - u0) & 1) * kTile64, W.yt + (bc * W.units + u) * (Q * TP), kTile64, high.bar);
+    }
     if (has_h) bulk_load(base + kGHigh, W.h + at, kTile64, high.bar);
     if (has_g) bulk_load(base + kGHigh + kTile64, W.g + at, kTile64, high.bar);
   };
@@ -873,11 +918,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     if (has_g) bulk_load(base + kGLow + kTile64, W.g + at, kTile64, low.bar);
   };
   auto load_x = [&](int u) {
+    if constexpr (TILED) return;
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
     const T* p = xc + (long long)h * P.dim + p0;
     load_tile<T, kGradThreads>(base + kGX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
   };
   auto load_y = [&](int u) {
+    if constexpr (TILED) return;
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
     const T* p = yc + (long long)h * P.dim + p0;
     load_tile<T, kGradThreads>(base + kGY + ((u - u0) & 1) * kTile64, p, P.dy_st, rows, cols, vector_ok(p, P.dy_st, 0, cols));
@@ -951,17 +998,18 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       }
       umma_commit(done.bar);
     }
+    const float xb = TILED ? W.xback[bc * W.units + u] : 1.f, yb = TILED ? W.yback[bc * W.units + u] : 1.f, xy = xb * yb;
     const float s = rec[row], lh = rec[Q + row], ll = rec[2 * Q + row], eh = rec[2 * Q - 1], el = rec[3 * Q - 1];
     float2 hs = make_float2(1.f, 1.f), gs = make_float2(1.f, 1.f);
     if (has_h || has_g) { hs = W.hs[bc * W.units + u]; gs = W.gs[bc * W.units + u]; }
     const float from_in = ex2(lh + ll), to_end = ex2((eh - lh) + (el - ll));
-    const float wy = has_h ? from_in * (hs.x / cscale) : 0.f, wx = has_g ? s * to_end * (gs.x / bscale) : 0.f;
+    const float wy = has_h ? from_in * (hs.x / cscale) * yb : 0.f, wx = has_g ? s * to_end * (gs.x / bscale) * xb : 0.f;
     float2 gh2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const uint32_t at = piece(row, part * 2 + j), plane = (uint32_t)((part * 2 + j) * kN + row) * 16;
-      if (has_h) sts16(base + kGM + at, pack8<__half>(mul8(unpack8<T>(lds16(ytile + at)), wy)));
-      if (has_g) sts16(base + kGM + kTile64 + at, pack8<__half>(mul8(unpack8<T>(lds16(base + kGX + at)), wx)));
+      if (has_h) sts16(base + kGM + at, pack8<__half>(mul8(unpack8<X>(lds16(ytile + at)), wy)));
+      if (has_g) sts16(base + kGM + kTile64 + at, pack8<__half>(mul8(unpack8<X>(lds16(base + kGX + at)), wx)));
       if (has_h && has_g) {                              // my row of the states: <G, H>
         const Eight h1 = unpack8<__half>(lds16(base + kGHigh + plane)), h2 = unpack8<__half>(lds16(base + kGLow + plane));
         const Eight g1 = unpack8<__half>(lds16(base + kGHigh + kTile64 + plane)), g2 = unpack8<__half>(lds16(base + kGLow + kTile64 + plane));
@@ -985,25 +1033,25 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const Eight x = unpack8<T>(lds16(base + kGX + piece(row, part * 2 + j)));
+          const Eight x = unpack8<X>(lds16(base + kGX + piece(row, part * 2 + j)));
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             dxi[j * 4 + e] = mul2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), pair(f));
             sum = fma2(dxi[j * 4 + e], x.v[e], sum);
           }
         }
-        r_part = sum.x + sum.y;
+        r_part = (sum.x + sum.y) * xb;
       }
       if (has_h) {
         tmem_ld16(lanes + 192 + part * 16, r);
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const Eight y = unpack8<T>(lds16(ytile + piece(row, part * 2 + j)));
+          const Eight y = unpack8<X>(lds16(ytile + piece(row, part * 2 + j)));
 #pragma unroll
           for (int e = 0; e < 4; ++e) sum = fma2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), y.v[e], sum);
         }
-        q_part = (sum.x + sum.y) * (from_in * hs.x * cback);
+        q_part = (sum.x + sum.y) * (from_in * hs.x * cback * yb);
       }
       tc_fence_before();
     }
@@ -1018,7 +1066,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       if (u + 1 < u1) load_low(u + 1);
       if (ok) {
         tc_fence_after();
-        mma<kK, kK>(work, base + kGX, ytile, idesc<T>(Q, false, false), 4, false);
+        mma<kK, kK>(work, base + kGX, ytile, idesc<X>(Q, false, false), 4, false);
         if (has_h) mma<kK, kPlaneN>(sum_c, base + kGM, base + kGHigh, idesc<__half>(kN, false, false), 4, u > u0);
         if (has_g) mma<kK, kPlaneN>(sum_b, base + kGM + kTile64, base + kGHigh + kTile64, idesc<__half>(kN, false, false), 4, u > u0);
         umma_commit(done.bar);
@@ -1033,7 +1081,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       cp_commit();
     }
     float r_sum = 0.f, diag = 0.f, pair_time = 0.f;
-    const float sb = s * both_back;
+    const float sb = s * both_back * xy, sxy = s * xy;       // of a pair, and of a pair without C . B
     const int cb = part;
     if (cb >= quad) {
       uint32_t r[32], d[32];
@@ -1044,7 +1092,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       float2 rs2 = make_float2(0.f, 0.f), time2 = make_float2(0.f, 0.f);
       if (cb > quad) {
         // a block of later tokens: the decay to its beginning and from there on are both at most 1
-        const float th = rec[Q + cb * 32 - 1] - lh, tl = rec[2 * Q + cb * 32 - 1] - ll, to_block = ex2(th + tl), ds_in = s * to_block, pairs_in = sb * to_block;
+        const float th = rec[Q + cb * 32 - 1] - lh, tl = rec[2 * Q + cb * 32 - 1] - ll, to_block = ex2(th + tl), ds_in = sxy * to_block, pairs_in = sb * to_block;
         const float mine = kScaled ? to_block * sc.x : to_block;
         const float4 *since = reinterpret_cast<const float4*>(rec + 4 * Q) + cb * 8, *in_block = reinterpret_cast<const float4*>(rec + 5 * Q) + cb * 8;
 #pragma unroll
@@ -1067,7 +1115,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
               e[q + 1] = both.y;
             }
           }
-          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<T>(f));
+          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<X>(f));
         }
         r_sum = rs2.x + rs2.y;                           // by s: the row's own factor
         pair_time = (time2.x + time2.y) + r_sum * (th + tl);
@@ -1086,19 +1134,19 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
             if (t < row) w.x = 0.f;                      // pairs under the diagonal weigh nothing
             if (t + 1 < row) w.y = 0.f;
             const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
-            ds[q >> 1] = fma2(pair(s), mul2(dm, w), ds[q >> 1]);
+            ds[q >> 1] = fma2(pair(sxy), mul2(dm, w), ds[q >> 1]);
             f.v[i] = kScaled ? mul2(m, pair(sc.x)) : m;
             float2 both = mul2(mul2(m, dm), pair(sb));
             if (t == row) { diag = dm.x; both.x = 0.f; } // no decay between a token and itself: kept out of the sums
             if (t + 1 == row) { diag = dm.y; both.y = 0.f; }
-            if (t == row) rself[row] = m.x * dm.x * both_back;
-            if (t + 1 == row) rself[row] = m.y * dm.y * both_back;
+            if (t == row) rself[row] = m.x * dm.x * (both_back * xy);
+            if (t + 1 == row) rself[row] = m.y * dm.y * (both_back * xy);
             rs2 = add2(rs2, both);
             time2 = fma2(both, gap, time2);
             e[q] = both.x;
             e[q + 1] = both.y;
           }
-          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<T>(f));
+          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<X>(f));
         }
         r_sum = rs2.x + rs2.y;
         pair_time = time2.x + time2.y;
@@ -1109,7 +1157,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       qpairs[quad * Q + cb * 32 + lane] = 0.f;
     }
     rpairs[part * Q + row] = r_sum;
-    diag = warp_sum(diag);
+    diag = warp_sum(diag * xy);
     pair_time = warp_sum(pair_time);
     if (lane == 0) { red[16 + warp] = diag; red[32 + warp] = pair_time; }
     tc_fence_before();
@@ -1118,7 +1166,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     // step 3
     if (threadIdx.x == 0 && ok) {
       tc_fence_after();
-      mma<kK, kMn>(work, base + kGM, ytile, idesc<T>(TP, false, true), 8, false);
+      mma<kK, kMn>(work, base + kGM, ytile, idesc<X>(TP, false, true), 8, false);
       umma_commit(done.bar);
     }
     if (warp == 15) {                                    // four tokens a lane
@@ -1164,7 +1212,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
         W.unit_sums[bc * W.units + u] = make_float2(dd, (float)((double)da / decay_rate(P.A[h])));
       }
     }
-    const float dskip = number(P.D, P.d_type, h), mixed = sc.y * both_back;
+    const float dskip = number(P.D, P.d_type, h) * yb, mixed = sc.y * both_back * yb;
     done.wait(ok, P.err);
     tc_fence_after();
     {
@@ -1174,7 +1222,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const uint32_t at = piece(row, part * 2 + j);
-        Eight f = mul8(unpack8<T>(lds16(ytile + at)), dskip);
+        Eight f = mul8(unpack8<X>(lds16(ytile + at)), dskip);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           f.v[e] = fma2(fma2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), pair(mixed), dxi[j * 4 + e]), pair(s), f.v[e]);
@@ -1448,39 +1496,39 @@ template <typename... A> int behind(void (*kernel)(A...), dim3 grid, int threads
   return launch_status();
 }
 
-template <typename T, bool REV, bool LO> int pass(const SelectiveParams& P, const Space& W, cudaStream_t st) {
-  if (int s = allow<state_pass_kernel<T, REV, LO>>(kPassSmem)) return s;
-  return behind(state_pass_kernel<T, REV, LO>, dim3(W.units, P.batch), kThreads, kPassSmem, st, P, W);
+template <typename T, bool REV, bool LO, bool TILED> int pass(const SelectiveParams& P, const Space& W, cudaStream_t st) {
+  if (int s = allow<state_pass_kernel<T, REV, LO, TILED>>(kPassSmem)) return s;
+  return behind(state_pass_kernel<T, REV, LO, TILED>, dim3(W.units, P.batch), kThreads, kPassSmem, st, P, W);
 }
 
-template <typename T> int prepare(const SelectiveParams& P, const Space& W, cudaStream_t st) {
-  const int head_blocks = (P.heads + kPrepHeads - 1) / kPrepHeads;
-  prepare_kernel<T><<<dim3(W.nc, head_blocks + 2 * P.groups, P.batch), kThreads, 0, st>>>(P, W, head_blocks);
+template <typename T> int prepare(const SelectiveParams& P, const Space& W, bool backward, cudaStream_t st) {
+  const int head_blocks = (P.heads + kPrepHeads - 1) / kPrepHeads, tiles = !P.tiled ? 2 * P.groups : backward ? W.units : 0;
+  prepare_kernel<T><<<dim3(W.nc, head_blocks + tiles, P.batch), kThreads, 0, st>>>(P, W, head_blocks);
   return launch_status();
 }
 
-template <typename T> int forward(const SelectiveParams& P, cudaStream_t st) {
-  const Space W = space_of(P, false);
-  if (int s = allow<out_kernel<T>>(kOutSmem)) return s;
-  if (int s = prepare<T>(P, W, st)) return s;
+template <typename T, bool TILED> int forward(const SelectiveParams& P, cudaStream_t st) {
+  const Space W = space_of(P, false, TILED);
+  if (int s = allow<out_kernel<T, TILED>>(kOutSmem)) return s;
+  if (int s = prepare<T>(P, W, false, st)) return s;
   if (W.nc > 1 || P.state_in || P.state_out)
-    if (int s = pass<T, false, false>(P, W, st)) return s;
+    if (int s = pass<T, false, false, TILED>(P, W, st)) return s;
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
-  return behind(out_kernel<T>, dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kOutSmem, st, P, W, per);
+  return behind(out_kernel<T, TILED>, dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kOutSmem, st, P, W, per);
 }
 
-template <typename T> int backward(const SelectiveParams& P, cudaStream_t st) {
-  const Space W = space_of(P, true);
-  if (int s = allow<grad_kernel<T>>(kGradSmem)) return s;
-  if (int s = prepare<T>(P, W, st)) return s;
+template <typename T, bool TILED> int backward(const SelectiveParams& P, cudaStream_t st) {
+  const Space W = space_of(P, true, TILED);
+  if (int s = allow<grad_kernel<T, TILED>>(kGradSmem)) return s;
+  if (int s = prepare<T>(P, W, true, st)) return s;
   if (W.nc > 1 || P.state_in || P.dstate_out || P.dstate_in) {
     SelectiveParams F = P;
     F.state_out = nullptr;
-    if (int s = pass<T, false, true>(F, W, st)) return s;
-    if (int s = pass<T, true, true>(P, W, st)) return s;
+    if (int s = pass<T, false, true, TILED>(F, W, st)) return s;
+    if (int s = pass<T, true, true, TILED>(P, W, st)) return s;
   }
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
-  if (int s = behind(grad_kernel<T>, dim3(W.nc, P.groups * W.splits, P.batch), kGradThreads, kGradSmem, st, P, W, per)) return s;
+  if (int s = behind(grad_kernel<T, TILED>, dim3(W.nc, P.groups * W.splits, P.batch), kGradThreads, kGradSmem, st, P, W, per)) return s;
   if (int s = behind(finish_dt_kernel<T>, dim3(W.nc, (P.heads + kPrepHeads - 1) / kPrepHeads, P.batch), kThreads, 0, st, P, W)) return s;
   if (P.dA || P.dD || P.dbias)
     if (int s = behind(finish_heads_kernel, dim3((P.heads + 3) / 4), 128, 0, st, P, W)) return s;
@@ -1493,16 +1541,22 @@ template <typename T> int backward(const SelectiveParams& P, cudaStream_t st) {
 
 }  // namespace
 
-long long selective_workspace(int batch, int length, int heads, int dim, int groups, bool backward) {
+long long selective_workspace(int batch, int length, int heads, int dim, int groups, bool backward, bool tiled) {
   SelectiveParams P{};
   P.batch = batch; P.length = length; P.heads = heads; P.dim = dim; P.groups = groups;
-  return space_of(P, backward).bytes;
+  return space_of(P, backward, tiled).bytes;
+}
+ConvTiles selective_tiles(const SelectiveParams& P, bool backward) {
+  const Space W = space_of(P, backward, true);
+  return {P.heads, P.dim, P.groups, W.nc, W.units, W.xt, W.bt, W.ct, W.xback, W.bback, W.cback};
 }
 int launch_selective_forward(const SelectiveParams& P, cudaStream_t st) {
-  return P.type == SQ_TYPE_F16 ? forward<__half>(P, st) : forward<__nv_bfloat16>(P, st);
+  if (P.tiled) return P.type == SQ_TYPE_F16 ? forward<__half, true>(P, st) : forward<__nv_bfloat16, true>(P, st);
+  return P.type == SQ_TYPE_F16 ? forward<__half, false>(P, st) : forward<__nv_bfloat16, false>(P, st);
 }
 int launch_selective_backward(const SelectiveParams& P, cudaStream_t st) {
-  return P.type == SQ_TYPE_F16 ? backward<__half>(P, st) : backward<__nv_bfloat16>(P, st);
+  if (P.tiled) return P.type == SQ_TYPE_F16 ? backward<__half, true>(P, st) : backward<__nv_bfloat16, true>(P, st);
+  return P.type == SQ_TYPE_F16 ? backward<__half, false>(P, st) : backward<__nv_bfloat16, false>(P, st);
 }
 int launch_selective_step(const SelectiveStepParams& P, cudaStream_t st) {
   cudaLaunchAttribute early{};

@@ -33,7 +33,17 @@ struct SelectiveParams {
   float* dstate_in;                                         // may be null
   void* workspace;
   int* err;
+  int tiled;                                                // x, B and C are tiles in the workspace (conv_tiles), not read from above
 };
+
+// Where a convolution puts its output for a scan: tiles of 128 tokens by 64 (x) or 128 (B, C) channels, scaled fp16 as
+// shared memory holds them, and what brings each back.
+struct ConvTiles {
+  int heads, dim, groups, chunks, units;
+  uint16_t *x, *b, *c;
+  float *xback, *bback, *cback;
+};
+ConvTiles selective_tiles(const SelectiveParams& p, bool backward);
 
 struct SelectiveStepParams {
   int batch, heads, dim, groups, type;
@@ -50,7 +60,7 @@ struct SelectiveStepParams {
   int behind;                                               // launched behind the kernel that writes x, B and C
 };
 
-long long selective_workspace(int batch, int length, int heads, int dim, int groups, bool backward);
+long long selective_workspace(int batch, int length, int heads, int dim, int groups, bool backward, bool tiled);
 int launch_selective_forward(const SelectiveParams& p, cudaStream_t stream);
 int launch_selective_backward(const SelectiveParams& p, cudaStream_t stream);
 int launch_selective_step(const SelectiveStepParams& p, cudaStream_t stream);

@@ -198,6 +198,9 @@ _PROTOS = {
     'sq_selective_forward': (C.c_int, [C.POINTER(SelectiveArgs), p]),
     'sq_selective_backward': (C.c_int, [C.POINTER(SelectiveArgs), p]),
     'sq_selective_step': (C.c_int, [C.POINTER(SelectiveStepArgs), p]),
+    'sq_conv_scan_workspace': (i64, [C.c_int] * 6),
+    'sq_conv_scan_forward': (C.c_int, [C.POINTER(CausalConvArgs), C.POINTER(SelectiveArgs), p]),
+    'sq_conv_scan_backward': (C.c_int, [C.POINTER(CausalConvArgs), C.POINTER(SelectiveArgs), p]),
     'sq_conv_scan_step': (C.c_int, [C.POINTER(ConvScanStepArgs), p]),
     'sq_causal_conv_workspace': (i64, [C.c_int] * 3),
     'sq_causal_conv_forward': (C.c_int, [C.POINTER(CausalConvArgs), p]),

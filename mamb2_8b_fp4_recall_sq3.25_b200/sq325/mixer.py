@@ -3,39 +3,70 @@
 
 Taken one after the other they keep for the backward pass the convolution's input and its output.  `conv_scan` keeps the
 input alone and computes the output again; with keep='int8' it keeps the input in 8 bits, 1.03 bytes a channel and token
-in place of four.  The output is then that of the given input, and the gradients are those at the kept values.
-`conv_scan_step` has the convolution's output in fp32 on its way to the state.
+in place of four.  The output is then that of the given input, and the gradients are those at the kept values.  Between
+the two the convolution's output is scaled fp16 (11 bits of a tile's largest value, also where the input is bf16), in
+`conv_scan_step` fp32.
 """
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
 from . import _lib
-from .activations import TYPES, PackedActivations, empty_packed
-from .conv import _ptr, checked_keep, checked_lengths, checked_weight, conv_backward, conv_forward, inner_packed
-from .selective import _HALF, N, checked_heads, checked_state, scan_backward, scan_forward
+from .activations import TYPES, PackedActivations, pack_activations
+from .conv import _ptr, checked_keep, checked_lengths, checked_weight, conv_args, inner_packed
+from .selective import _HALF, N, checked_heads, checked_state
 
 __all__ = ['conv_scan', 'conv_scan_step']
 
 
-def _split(z, heads, groups):
-    """x, B and C of the convolution's channels, as views."""
-    batch, length, width = z.shape
-    inner = width - 2 * groups * N
-    return (z[:, :, :inner].view(batch, length, heads, inner // heads), z[:, :, inner:inner + groups * N].view(batch, length, groups, N),
-            z[:, :, inner + groups * N:].view(batch, length, groups, N))
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(batch, length, heads, dim, groups, backward):
+    return int(_lib.load().sq_conv_scan_workspace(batch, length, heads, dim, groups, backward))
+
+
+def _args(shape, dtype, xbc, packed, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups, backward):
+    """The arguments of convolution and scan that forward and backward share, and the workspace."""
+    batch, length, width = shape
+    dim = (width - 2 * groups * N) // heads
+    conv = conv_args(shape, dtype, xbc, packed, weight, bias, conv_state, lengths, 1)
+    scan = _lib.SelectiveArgs(batch, length, heads, dim, groups, TYPES[dtype])
+    scan.dt, scan.dt_batch_stride, scan.dt_token_stride, scan.A = dt.data_ptr(), dt.stride(0), dt.stride(1), A.data_ptr()
+    if D is not None:
+        scan.D, scan.d_type = D.data_ptr(), TYPES[D.dtype]
+    if dt_bias is not None:
+        scan.dt_bias, scan.bias_type = dt_bias.data_ptr(), TYPES[dt_bias.dtype]
+    scan.state_in, scan.lengths = _ptr(state), _ptr(lengths)
+    nbytes = _workspace_bytes(batch, length, heads, dim, groups, backward)
+    work = torch.empty(nbytes, dtype=torch.uint8, device=dt.device)
+    scan.workspace, scan.workspace_bytes = work.data_ptr(), nbytes
+    return conv, scan, work
+
+
+def _forward(xbc, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups, want_state):
+    """(y, last inputs or None, state or None) of checked tensors."""
+    batch, length, width = xbc.shape
+    dim = (width - 2 * groups * N) // heads
+    device = xbc.device
+    conv, scan, work = _args(xbc.shape, xbc.dtype, xbc, None, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups, 0)
+    y = torch.empty(batch, length, heads, dim, dtype=xbc.dtype, device=device)
+    conv_last = torch.empty(batch, weight.shape[1] - 1, width, dtype=xbc.dtype, device=device) if want_state else None
+    last = torch.empty(batch, heads, dim, N, dtype=torch.float32, device=device) if want_state else None
+    conv.state_out, scan.state_out = _ptr(conv_last), _ptr(last)
+    scan.y, scan.y_batch_stride, scan.y_token_stride = y.data_ptr(), length * heads * dim, heads * dim
+    _lib.launch('sq_conv_scan_forward', device, C.byref(conv), C.byref(scan))
+    del work                                                 # alive until the launch
+    return y, conv_last, last
 
 
 class _ConvScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, xbc, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups, want_state, keep):
-        packed = empty_packed(xbc.shape, xbc.dtype, xbc.device) if keep else None
-        z, conv_last = conv_forward(xbc.shape, xbc.dtype, xbc, packed, weight, bias, conv_state, lengths, 1, want_state)
-        x, B, C_ = _split(z, heads, groups)
-        y, last = scan_forward(x, dt, A, B, C_, D, dt_bias, state, lengths, want_state)
-        ctx.save_for_backward(dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, *(packed[:2] if keep else (xbc,)))
+        y, conv_last, last = _forward(xbc, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups, want_state)
+        kept = pack_activations(xbc)[:2] if keep else (xbc,)
+        ctx.save_for_backward(dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, *kept)
         ctx.shape, ctx.dtype, ctx.heads, ctx.groups = xbc.shape, xbc.dtype, heads, groups
         ctx.set_materialize_grads(False)
         return (y, conv_last, last) if want_state else y
@@ -53,16 +84,24 @@ class _ConvScan(torch.autograd.Function):
             packed = PackedActivations(kept[0].contiguous(), kept[1].contiguous(), ctx.dtype)
         else:
             xbc = inner_packed(kept[0], 1)
-        conv = (ctx.shape, ctx.dtype, xbc, packed, weight, bias, conv_state, lengths, 1)
-        x, B, C_ = _split(conv_forward(*conv)[0], ctx.heads, ctx.groups)
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else inner_packed(dy, 2)
-        need = ctx.needs_input_grad
-        dz = torch.empty(ctx.shape, dtype=ctx.dtype, device=x.device)
-        ddt, dA, dD, ddt_bias, dstate = scan_backward(x, dt, A, B, C_, D, dt_bias, state, lengths, dy,
-                                                      None if dlast is None else dlast.contiguous(), *_split(dz, ctx.heads, ctx.groups),
-                                                      (need[2], need[5], need[6], need[8]))
-        dxbc, dweight, dbias, dconv_state = conv_backward(*conv, dz, None if dconv_last is None else dconv_last.contiguous(),
-                                                          need[3], need[4], need[7])
+        batch, length, width = ctx.shape
+        device, heads, need = dt.device, ctx.heads, ctx.needs_input_grad
+        if dy is None:
+            dy = torch.zeros(batch, length, heads, (width - 2 * ctx.groups * N) // heads, dtype=ctx.dtype, device=device)
+        else:
+            dy = inner_packed(dy, 2)
+        dconv_last, dlast = (None if t is None else t.contiguous() for t in (dconv_last, dlast))
+        conv, scan, work = _args(ctx.shape, ctx.dtype, xbc, packed, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads,
+                                 ctx.groups, 1)
+        dxbc = torch.empty(ctx.shape, dtype=ctx.dtype, device=device)
+        ddt = torch.empty(dt.shape, dtype=dt.dtype, device=device)
+        dA, dweight, dbias, dD, ddt_bias, dconv_state, dstate = (
+            torch.empty_like(t) if need[i] else None for i, t in ((2, A), (3, weight), (4, bias), (5, D), (6, dt_bias), (7, conv_state), (8, state)))
+        conv.dx, conv.dweight, conv.dbias, conv.dstate_in, conv.dstate_out = dxbc.data_ptr(), _ptr(dweight), _ptr(dbias), _ptr(dconv_state), _ptr(dconv_last)
+        scan.dy, scan.dy_batch_stride, scan.dy_token_stride, scan.dstate_out = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
+        scan.ddt, scan.dA, scan.dD, scan.ddt_bias, scan.dstate_in = ddt.data_ptr(), _ptr(dA), _ptr(dD), _ptr(ddt_bias), _ptr(dstate)
+        _lib.launch('sq_conv_scan_backward', device, C.byref(conv), C.byref(scan))
+        del work                                             # alive until the launch
         return dxbc, ddt, dA, dweight, dbias, dD, ddt_bias, dconv_state, dstate, None, None, None, None, None
 
 
@@ -111,9 +150,7 @@ def conv_scan(xbc, dt, A, conv_weight, conv_bias=None, D=None, dt_bias=None, *, 
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (xbc, dt, A, weight, bias, D, dt_bias, conv_state, state)):
         return _ConvScan.apply(xbc, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups,
                                bool(return_final_state), keep)
-    z, conv_last = conv_forward(xbc.shape, xbc.dtype, xbc, None, weight, bias, conv_state, lengths, 1, return_final_state)
-    x, B, C_ = _split(z, heads, groups)
-    y, last = scan_forward(x, dt, A, B, C_, D, dt_bias, state, lengths, return_final_state)
+    y, conv_last, last = _forward(xbc, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups, bool(return_final_state))
     return (y, conv_last, last) if return_final_state else y
 
 
