@@ -519,41 +519,53 @@ __device__ __forceinline__ void four_channels(const ConvParams& P, int b, int t,
 }
 
 // One CTA: a chunk's tile of x (64 channels of a head) or of B or C (128 of a group).  A thread has four channels of
-// TOKENS neighbouring tokens in registers; the tile's largest value gives its scale.
-template <typename T, typename WT, bool CODES, int TOKENS>
+// TOKENS neighbouring tokens in registers, all loads before the first use; the tile's largest value gives its scale.
+// VEC: four taps, and four channels are one aligned load.
+template <typename T, typename WT, bool CODES, int TOKENS, bool VEC>
 __device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk, int c0, int cols, int rows, uint16_t* out, float* back,
                                           uint32_t* tops) {
+  using In = Inputs<T, CODES, true, 4>;
   constexpr int kWideTile = TOKENS == 8 ? 16 : 32;                     // threads side by side: of 64 or 128 channels
-  const int at = threadIdx.x % kWideTile, c = c0 + at * 4, n = max(0, min(4, cols - at * 4)), r0 = threadIdx.x / kWideTile * TOKENS;
-  const bool vec = n == 4 && c % 4 == 0 && P.channels % 4 == 0 &&
-                   (CODES ? ((uintptr_t)P.codes & 3) == 0 : (((uintptr_t)P.x & 7) == 0 && ((P.x_sb | P.x_st) & 3) == 0));
-  float z[TOKENS][4];
-  float x[3][4];
-  const Taps<WT, 4> W(P.weight, P.bias, P.taps, n > 0 ? c : 0, n);
-  const int t0 = chunk * kScanChunk + r0;
-  uint32_t top = 0;
+  const int at = threadIdx.x % kWideTile, n = max(0, min(4, cols - at * 4)), c = n > 0 ? c0 + at * 4 : 0, r0 = threadIdx.x / kWideTile * TOKENS;
+  const int t0 = chunk * kScanChunk + r0, end = n > 0 ? chunk * kScanChunk + rows : 0;
+  float z[TOKENS][4], x[3][4];
+  typename In::Raw raw[VEC ? TOKENS + 3 : 1];
+  float scale[VEC ? TOKENS + 3 : 1];
+  const In in(P, b, c, 4);
+  if constexpr (VEC) {
 #pragma unroll
-  for (int k = 0; k < 3; ++k) four_channels<T, CODES>(P, b, n > 0 && r0 < rows ? t0 - 3 + k : -kTaps, n > 0 ? c : 0, n, vec, x[k]);
+    for (int j = 0; j < TOKENS + 3; ++j) raw[j] = in.load(t0 - 3 + j, t0 - 3 + j >= 0 && t0 - 3 + j < end, scale[j]);
+  }
+  const int taps = VEC ? kTaps : P.taps;
+  const Taps<WT, 4> W(P.weight, P.bias, taps, c, n);
+  if (VEC && t0 > 0) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) In::get(raw[k], scale[k], x[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) four_channels<T, CODES>(P, b, t0 < end ? t0 - 3 + k : -kTaps, c, n, false, x[k]);
+  }
+  float top = 0.f;
 #pragma unroll
   for (int j = 0; j < TOKENS; ++j) {
-    const bool in = n > 0 && r0 + j < rows;
     float f[4];
-    four_channels<T, CODES>(P, b, in ? t0 + j : -kTaps, n > 0 ? c : 0, n, vec, f);
+    if constexpr (VEC) In::get(raw[j + 3], scale[j + 3], f);
+    else four_channels<T, CODES>(P, b, t0 + j < end ? t0 + j : -kTaps, c, n, false, f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float v = conv_at<WT, 4>(W, P.taps, i, x[0][i], x[1][i], x[2][i], f[i]);
-      z[j][i] = in && i < n ? v * sigmoid<T>(v) : 0.f;
-      top = max(top, __float_as_uint(z[j][i]) & 0x7fffffffu);
+      const float v = conv_at<WT, 4>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
+      z[j][i] = t0 + j < end && (VEC || i < n) ? v * sigmoid<T>(v) : 0.f;
+      top = fmaxf(top, fabsf(z[j][i]));
       x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
     }
   }
-  top = __reduce_max_sync(0xffffffffu, top);
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
+  uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = bits;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 8; ++k) top = max(top, tops[k]);
-  int e = (int)(top >> 23) - 140;                                      // to [2^13, 2^14)
-  e = top ? max(-60, min(60, e)) : 0;
+  for (int k = 0; k < 8; ++k) bits = max(bits, tops[k]);
+  int e = (int)(bits >> 23) - 140;                                     // to [2^13, 2^14)
+  e = bits ? max(-60, min(60, e)) : 0;
   const float there = __uint_as_float((uint32_t)(127 - e) << 23);
   if (threadIdx.x == 0) *back = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
@@ -564,23 +576,27 @@ __device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk,
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
   }
 }
-template <typename T, typename WT, bool CODES>
-__global__ void __launch_bounds__(256) conv_tiles_kernel(const ConvParams P, const ConvTiles A) {
+template <typename T, typename WT, bool CODES, bool VEC, bool GROUPS>
+__global__ void __launch_bounds__(256, GROUPS ? 2 : 4) conv_tiles_kernel(const ConvParams P, const ConvTiles A) {
   __shared__ uint32_t tops[8];
   const int chunk = blockIdx.x, b = blockIdx.z, u = blockIdx.y;
   const int rows = min(kScanChunk, tokens_of(P, b) - chunk * kScanChunk);
   if (rows <= 0) return;                                               // not read
   const long long bc = (long long)b * A.chunks + chunk;
-  if (u < A.units) {
+  if constexpr (!GROUPS) {
     const int ptiles = A.units / A.heads, h = u / ptiles, p0 = (u % ptiles) * kScanTile, cols = min(kScanTile, A.dim - p0);
-    conv_tile<T, WT, CODES, 8>(P, b, chunk, h * A.dim + p0, cols, rows, A.x + (bc * A.units + u) * (kScanChunk * kScanTile),
-                               A.xback + bc * A.units + u, tops);
+    conv_tile<T, WT, CODES, 8, VEC>(P, b, chunk, h * A.dim + p0, cols, rows, A.x + (bc * A.units + u) * (kScanChunk * kScanTile),
+                                    A.xback + bc * A.units + u, tops);
   } else {
-    const int i = u - A.units, g = i >> 1;
+    const int g = u >> 1;
     const long long at = bc * A.groups + g;
-    conv_tile<T, WT, CODES, 16>(P, b, chunk, A.heads * A.dim + (i & 1 ? A.groups * 128 : 0) + g * 128, 128, rows,
-                                (i & 1 ? A.c : A.b) + at * (kScanChunk * 128), (i & 1 ? A.cback : A.bback) + at, tops);
+    conv_tile<T, WT, CODES, 16, VEC>(P, b, chunk, A.heads * A.dim + (u & 1 ? A.groups * 128 : 0) + g * 128, 128, rows,
+                                     (u & 1 ? A.c : A.b) + at * (kScanChunk * 128), (u & 1 ? A.cback : A.bback) + at, tops);
   }
+}
+template <typename T, typename WT, bool CODES, bool VEC> void conv_tiles(const ConvParams& P, const ConvTiles& A, cudaStream_t st) {
+  conv_tiles_kernel<T, WT, CODES, VEC, true><<<dim3(A.chunks, 2 * A.groups, P.batch), 256, 0, st>>>(P, A);
+  conv_tiles_kernel<T, WT, CODES, VEC, false><<<dim3(A.chunks, A.units, P.batch), 256, 0, st>>>(P, A);
 }
 // The last inputs of a sequence.
 template <typename T, bool CODES>
@@ -739,13 +755,14 @@ template <typename F> int by_type(int type, int weight_type, F f) {
 }  // namespace
 
 int launch_conv_tiles(const ConvParams& P, const ConvTiles& A, cudaStream_t st) {
-  const dim3 grid(A.chunks, A.units + 2 * A.groups, P.batch);
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
     if constexpr (sizeof(T) == 2) {
-      if (P.codes) conv_tiles_kernel<T, WT, true><<<grid, 256, 0, st>>>(P, A);
-      else conv_tiles_kernel<T, WT, false><<<grid, 256, 0, st>>>(P, A);
+      // every head's channels begin at a multiple of four, and so do the rows
+      const bool vec = P.taps == kTaps && A.dim % 4 == 0 && (P.codes ? P.channels % 4 == 0 && ((uintptr_t)P.codes & 3) == 0 : whole(P.x, P.type, 4, P.x_sb, P.x_st));
+      if (P.codes) vec ? conv_tiles<T, WT, true, true>(P, A, st) : conv_tiles<T, WT, true, false>(P, A, st);
+      else vec ? conv_tiles<T, WT, false, true>(P, A, st) : conv_tiles<T, WT, false, false>(P, A, st);
       return launch_status();
     }
     return (int)kEInval;
