@@ -205,7 +205,7 @@ struct Space {
   float2 *hs, *gs;                    // [B][nc][units]: scale of the state, scale of the chunk's weighted tokens
   float2* parts;                      // [B][units][lp]: gradient of A s, gradient of s through the tokens
   float2* unit_sums;                  // [B][nc][units]: gradients of D and of A by chunk
-  float* bias_sums;                   // [B][nc][H]: gradient of the bias by chunk
+  float* bias_sums;                   // [B][nc][H][4]: gradient of the bias by 32 tokens
   float *pb, *pc;                     // [splits][B][nc * Q][G][128]: dB and dC by split
   int splits;
   long long bytes;
@@ -260,7 +260,7 @@ Space space_of(const SelectiveParams& P, bool backward, bool tiled) {
     w.gs = reinterpret_cast<float2*>(take(bcu * 8));
     w.parts = reinterpret_cast<float2*>(take((long long)P.batch * w.units * w.lp * 8));
     w.unit_sums = reinterpret_cast<float2*>(take(bcu * 8));
-    w.bias_sums = reinterpret_cast<float*>(take(bc * P.heads * 4));
+    w.bias_sums = reinterpret_cast<float*>(take(bc * P.heads * 16));
     if (w.splits > 1) {
       const long long part = bc * Q * P.groups * kN * 4 * w.splits;
       w.pb = reinterpret_cast<float*>(take(part));
@@ -358,6 +358,7 @@ template <int COLS> __device__ __forceinline__ void tensor_end(uint32_t tmem) {
 __device__ __forceinline__ double decay_rate(float A) {
   return fabsf(A) < 1e-20f ? -1e-20 : (double)A * 1.4426950408889634;
 }
+__device__ __forceinline__ float decay_rate_f32(float A) { return fabsf(A) < 1e-20f ? -1e-20f : A * kLog2e; }
 // One CTA: a chunk of eight heads (a warp a head, four tokens a lane), or a chunk's tile of B or C.
 constexpr int kPrepHeads = 8;
 template <typename T>
@@ -481,7 +482,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
 constexpr uint32_t kPassX = 2 * kTile128, kPassW = kPassX + kTile64, kPassBytes = kPassW + 2 * kTile64, kPassSmem = kPassBytes + 64;
 
 template <typename T, bool REV, bool LO, bool TILED>
-__global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const SelectiveParams P, const Space W) {
+__device__ __forceinline__ void state_pass(const SelectiveParams& P, const Space& W, float* state_out) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kPassBytes);           // tensor cores, tile 0, tile 1, tokens (TILED)
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
   const int len = tokens_of(P, b), nc = (len + Q - 1) / Q;
   const int n = threadIdx.x & 127, half = threadIdx.x >> 7, quad = threadIdx.x >> 5 & 3;
   const float* first = REV ? P.dstate_out : P.state_in;
-  float* last = REV ? P.dstate_in : P.state_out;
+  float* last = REV ? P.dstate_in : state_out;
   uint16_t* planes = REV ? W.g : W.h;
   float2* scales = REV ? W.gs : W.hs;
   const T* tok = reinterpret_cast<const T*>(REV ? P.dy : P.x) + (long long)b * (REV ? P.dy_sb : P.x_sb) + (long long)h * P.dim + p0;
@@ -641,6 +642,16 @@ __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const Selective
       if (p + 1 < cols) last[state_at + (long long)(p + 1) * kN] = S[i].y;
     }
   tensor_end<128>(tmem);
+}
+template <typename T, bool TILED>
+__global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const SelectiveParams P, const Space W) {
+  state_pass<T, false, false, TILED>(P, W, P.state_out);
+}
+// A backward's: the states again, with remainders, and their gradients, whose walks do not need one another.
+template <typename T, bool TILED>
+__global__ void __launch_bounds__(kThreads, 2) state_passes_kernel(const SelectiveParams P, const Space W) {
+  if (blockIdx.z == 0) state_pass<T, false, true, TILED>(P, W, nullptr);
+  else state_pass<T, true, true, TILED>(P, W, nullptr);
 }
 
 // ---------------------------------------------------------------- outputs by chunk and group
@@ -835,24 +846,24 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
 //      by row and by column.
 //   3. the pairs' part of x's gradient; prefix and suffix sums over the tokens give the gradient of A s.
 // After the last unit the group's sum gives the pairs' part of dB and dC in two products.
-constexpr uint32_t kGRecBytes = 6 * Q * 4;               // of a token's record, all but the last number
+constexpr uint32_t kGRecBytes = kRecord * Q * 4;
 constexpr uint32_t kGB = 0, kGC = kTile128, kGX = 2 * kTile128, kGY = kGX + kTile64, kGHigh = kGY + 2 * kTile64,
                    kGLow = kGHigh + 2 * kTile64, kGM = kGLow + 2 * kTile64, kGRec = kGM + kTile128, kGRow = kGRec + 2 * kGRecBytes,
                    kGCol = kGRow + 13 * Q * 4, kGRed = kGCol + 4 * Q * 4, kGBar = kGRed + 64 * 4, kGradSmem = kGBar + 48;
 constexpr int kGradThreads = 512;                  // four threads a token: sixteen warps hide each other's waits
 
-// Sums over a warp's lanes of e[column], for column = lane.
-__device__ __forceinline__ float column_sums(float (&e)[32], int lane) {
+// Sums over a warp's lanes of e[column], for column = lane / 2.
+__device__ __forceinline__ float column_sums(float (&e)[16], int lane) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const bool up = lane & o;
+  for (int o = 8; o; o >>= 1) {
+    const bool up = lane & (2 * o);
 #pragma unroll
     for (int i = 0; i < o; ++i) {
       const float send = up ? e[i] : e[i + o], keep = up ? e[i + o] : e[i];
-      e[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+      e[i] = keep + __shfl_xor_sync(0xffffffffu, send, 2 * o);
     }
   }
-  return e[0];
+  return e[0] + __shfl_xor_sync(0xffffffffu, e[0], 1);
 }
 
 template <typename T, bool TILED>
@@ -871,27 +882,30 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   const int u0 = g * gunits + split * per, u1 = min(u0 + per, (g + 1) * gunits);
   const int len = tokens_of(P, b), rows = min(Q, len - c * Q), out_rows = min(Q, P.length - c * Q);
   const int row = threadIdx.x & 127, part = threadIdx.x >> 7, warp = threadIdx.x >> 5, quad = warp & 3, lane = threadIdx.x & 31;
-  const long long bc = (long long)b * W.nc + c, dx_st = P.dx_st, grp_st = P.dg_st, tile_at = bc * P.groups + g;
-  T* dx = reinterpret_cast<T*>(P.dx) + b * P.dx_sb + (long long)c * Q * dx_st;
-  const long long grp_at = b * P.dg_sb + (long long)c * Q * grp_st + g * kN;
-  T *dB = reinterpret_cast<T*>(P.dB) + grp_at, *dC = reinterpret_cast<T*>(P.dC) + grp_at;
+  const long long bc = (long long)b * W.nc + c, tile_at = bc * P.groups + g;
+  // Pointers are made where they are used: registers are what this kernel is short of.
+  auto dx_at = [&](int h, int p0) { return reinterpret_cast<T*>(P.dx) + b * P.dx_sb + (long long)c * Q * P.dx_st + (long long)h * P.dim + p0; };
+  auto group_at = [&](void* p) { return reinterpret_cast<T*>(p) + b * P.dg_sb + (long long)c * Q * P.dg_st + g * kN; };
   launch_dependents();
   if (rows <= 0) {                                       // behind the sequence's end
     for (int u = u0; u < u1; ++u) {
       const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
       for (int i = threadIdx.x; i < out_rows * cols; i += kGradThreads)
-        dx[(long long)(i / cols) * dx_st + (long long)h * P.dim + p0 + i % cols] = from_f32<T>(0.f);
+        dx_at(h, p0)[(long long)(i / cols) * P.dx_st + i % cols] = from_f32<T>(0.f);
       if (threadIdx.x == 0) W.unit_sums[bc * W.units + u] = make_float2(0.f, 0.f);
+      if (W.ptiles == 1) {
+        if (threadIdx.x < 4) W.bias_sums[(bc * P.heads + h) * 4 + threadIdx.x] = 0.f;
+        T* ddt = reinterpret_cast<T*>(P.ddt) + ((long long)b * P.length + (long long)c * Q) * P.heads + h;
+        for (int i = threadIdx.x; i < out_rows; i += kGradThreads) ddt[(long long)i * P.heads] = from_f32<T>(0.f);
+      }
     }
     if (W.splits == 1)
       for (int i = threadIdx.x; i < out_rows * kN; i += kGradThreads)
-        dB[(long long)(i / kN) * grp_st + i % kN] = dC[(long long)(i / kN) * grp_st + i % kN] = from_f32<T>(0.f);
+        group_at(P.dB)[(long long)(i / kN) * P.dg_st + i % kN] = group_at(P.dC)[(long long)(i / kN) * P.dg_st + i % kN] = from_f32<T>(0.f);
     wait_for_launch();
     return;
   }
   const bool has_h = c > 0 || P.state_in, has_g = (c + 1) * Q < len || P.dstate_out;
-  const T* xc = reinterpret_cast<const T*>(P.x) + (long long)b * P.x_sb + (long long)c * Q * P.x_st;
-  const T* yc = reinterpret_cast<const T*>(P.dy) + (long long)b * P.dy_sb + (long long)c * Q * P.dy_st;
   const uint32_t tmem = tensor_begin<512>(bars, 4, reinterpret_cast<uint32_t*>(smem + kGBar + 32));
   const uint32_t lanes = tmem + ((uint32_t)quad << 21), work = tmem + 128, sum_c = tmem + 256, sum_b = tmem + 384;
   wait_for_launch();
@@ -920,13 +934,13 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   auto load_x = [&](int u) {
     if constexpr (TILED) return;
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
-    const T* p = xc + (long long)h * P.dim + p0;
+    const T* p = reinterpret_cast<const T*>(P.x) + b * P.x_sb + (long long)c * Q * P.x_st + (long long)h * P.dim + p0;
     load_tile<T, kGradThreads>(base + kGX, p, P.x_st, rows, cols, vector_ok(p, P.x_st, 0, cols));
   };
   auto load_y = [&](int u) {
     if constexpr (TILED) return;
     const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
-    const T* p = yc + (long long)h * P.dim + p0;
+    const T* p = reinterpret_cast<const T*>(P.dy) + b * P.dy_sb + (long long)c * Q * P.dy_st + (long long)h * P.dim + p0;
     load_tile<T, kGradThreads>(base + kGY + ((u - u0) & 1) * kTile64, p, P.dy_st, rows, cols, vector_ok(p, P.dy_st, 0, cols));
   };
   if (threadIdx.x == 0) {
@@ -1084,74 +1098,77 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     const float sb = s * both_back * xy, sxy = s * xy;       // of a pair, and of a pair without C . B
     const int cb = part;
     if (cb >= quad) {
-      uint32_t r[32], d[32];
-      tmem_ld32_nowait(lanes + cb * 32, r);
-      tmem_ld32(lanes + 128 + cb * 32, d);
-      settle(r);
-      float e[32];
       float2 rs2 = make_float2(0.f, 0.f), time2 = make_float2(0.f, 0.f);
-      if (cb > quad) {
-        // a block of later tokens: the decay to its beginning and from there on are both at most 1
-        const float th = rec[Q + cb * 32 - 1] - lh, tl = rec[2 * Q + cb * 32 - 1] - ll, to_block = ex2(th + tl), ds_in = sxy * to_block, pairs_in = sb * to_block;
-        const float mine = kScaled ? to_block * sc.x : to_block;
-        const float4 *since = reinterpret_cast<const float4*>(rec + 4 * Q) + cb * 8, *in_block = reinterpret_cast<const float4*>(rec + 5 * Q) + cb * 8;
+      const bool later = cb > quad;
+      // a block of later tokens: the decay to its beginning and from there on are both at most 1
+      const float th = later ? rec[Q + cb * 32 - 1] - lh : 0.f, tl = later ? rec[2 * Q + cb * 32 - 1] - ll : 0.f, to_block = ex2(th + tl);
+      const float ds_in = sxy * to_block, pairs_in = sb * to_block, mine = kScaled ? to_block * sc.x : to_block;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          Eight f;
+      for (int part16 = 0; part16 < 2; ++part16) {       // sixteen columns in registers at a time
+        uint32_t r[16], d[16];
+        tmem_ld16_nowait(lanes + cb * 32 + part16 * 16, r);
+        tmem_ld16(lanes + 128 + cb * 32 + part16 * 16, d);
+        settle(r);
+        float e[16];
+        if (later) {
+          const float4 *since = reinterpret_cast<const float4*>(rec + 4 * Q) + cb * 8 + part16 * 4;
+          const float4 *in_block = reinterpret_cast<const float4*>(rec + 5 * Q) + cb * 8 + part16 * 4;
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float4 w4 = since[j * 2 + i], l4 = in_block[j * 2 + i];
+          for (int j = 0; j < 2; ++j) {
+            Eight f;
 #pragma unroll
-            for (int o = 0; o < 2; ++o) {
-              const int q = j * 8 + i * 4 + o * 2;
-              const float2 w = o ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y), l = o ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+            for (int i = 0; i < 2; ++i) {
+              const float4 w4 = since[j * 2 + i], l4 = in_block[j * 2 + i];
+#pragma unroll
+              for (int o = 0; o < 2; ++o) {
+                const int q = j * 8 + i * 4 + o * 2, at = part16 * 16 + q;
+                const float2 w = o ? make_float2(w4.z, w4.w) : make_float2(w4.x, w4.y), l = o ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y);
+                const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
+                ds[at >> 1] = fma2(mul2(dm, w), pair(ds_in), ds[at >> 1]);
+                f.v[i * 2 + o] = mul2(m, pair(mine));
+                const float2 both = mul2(mul2(m, dm), pair(pairs_in));
+                rs2 = add2(rs2, both);
+                time2 = fma2(both, l, time2);
+                e[q] = both.x;
+                e[q + 1] = both.y;
+              }
+            }
+            sts16(base + kGM + piece2(row, cb * 4 + part16 * 2 + j), pack8<X>(f));
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            Eight f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int q = j * 8 + i * 2, at = part16 * 16 + q, t = cb * 32 + at;
+              const float2 hv = *reinterpret_cast<const float2*>(rec + Q + t), lv = *reinterpret_cast<const float2*>(rec + 2 * Q + t);
+              float2 gap = add2(sub2(hv, pair(lh)), sub2(lv, pair(ll)));
+              if (t < row) gap.x = 0.f;
+              if (t + 1 < row) gap.y = 0.f;
+              float2 w = make_float2(ex2(gap.x), ex2(gap.y));
+              if (t < row) w.x = 0.f;                    // pairs under the diagonal weigh nothing
+              if (t + 1 < row) w.y = 0.f;
               const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
-              ds[q >> 1] = fma2(mul2(dm, w), pair(ds_in), ds[q >> 1]);
-              f.v[i * 2 + o] = mul2(m, pair(mine));
-              const float2 both = mul2(mul2(m, dm), pair(pairs_in));
+              ds[at >> 1] = fma2(pair(sxy), mul2(dm, w), ds[at >> 1]);
+              f.v[i] = kScaled ? mul2(m, pair(sc.x)) : m;
+              float2 both = mul2(m, dm);
+              if (t == row) { diag = dm.x; rself[row] = both.x * (both_back * xy); both.x = 0.f; }
+              if (t + 1 == row) { diag = dm.y; rself[row] = both.y * (both_back * xy); both.y = 0.f; }
+              both = mul2(both, pair(sb));               // no decay between a token and itself: kept out of the sums
               rs2 = add2(rs2, both);
-              time2 = fma2(both, l, time2);
+              time2 = fma2(both, gap, time2);
               e[q] = both.x;
               e[q + 1] = both.y;
             }
+            sts16(base + kGM + piece2(row, cb * 4 + part16 * 2 + j), pack8<X>(f));
           }
-          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<X>(f));
         }
-        r_sum = rs2.x + rs2.y;                           // by s: the row's own factor
-        pair_time = (time2.x + time2.y) + r_sum * (th + tl);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          Eight f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int q = j * 8 + i * 2, t = cb * 32 + q;
-            const float2 hv = *reinterpret_cast<const float2*>(rec + Q + t), lv = *reinterpret_cast<const float2*>(rec + 2 * Q + t);
-            float2 gap = add2(sub2(hv, pair(lh)), sub2(lv, pair(ll)));
-            if (t < row) gap.x = 0.f;
-            if (t + 1 < row) gap.y = 0.f;
-            float2 w = make_float2(ex2(gap.x), ex2(gap.y));
-            if (t < row) w.x = 0.f;                      // pairs under the diagonal weigh nothing
-            if (t + 1 < row) w.y = 0.f;
-            const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
-            ds[q >> 1] = fma2(pair(sxy), mul2(dm, w), ds[q >> 1]);
-            f.v[i] = kScaled ? mul2(m, pair(sc.x)) : m;
-            float2 both = mul2(mul2(m, dm), pair(sb));
-            if (t == row) { diag = dm.x; both.x = 0.f; } // no decay between a token and itself: kept out of the sums
-            if (t + 1 == row) { diag = dm.y; both.y = 0.f; }
-            if (t == row) rself[row] = m.x * dm.x * (both_back * xy);
-            if (t + 1 == row) rself[row] = m.y * dm.y * (both_back * xy);
-            rs2 = add2(rs2, both);
-            time2 = fma2(both, gap, time2);
-            e[q] = both.x;
-            e[q + 1] = both.y;
-          }
-          sts16(base + kGM + piece2(row, cb * 4 + j), pack8<X>(f));
-        }
-        r_sum = rs2.x + rs2.y;
-        pair_time = time2.x + time2.y;
+        const float column = column_sums(e, lane);
+        if (!(lane & 1)) qpairs[quad * Q + cb * 32 + part16 * 16 + (lane >> 1)] = column;
       }
-      qpairs[quad * Q + cb * 32 + lane] = column_sums(e, lane);
+      r_sum = rs2.x + rs2.y;                             // by s: the row's own factor
+      pair_time = (time2.x + time2.y) + r_sum * (th + tl);
     } else {
       for (int j = 0; j < 4; ++j) sts16(base + kGM + piece2(row, cb * 4 + j), make_uint4(0, 0, 0, 0));
       qpairs[quad * Q + cb * 32 + lane] = 0.f;
@@ -1169,47 +1186,46 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       mma<kK, kMn>(work, base + kGM, ytile, idesc<X>(TP, false, true), 8, false);
       umma_commit(done.bar);
     }
-    if (warp == 15) {                                    // four tokens a lane
-      float a[4], r[4], sa = 0.f, sum = 0.f, bs[4], time = 0.f;
-      float through = 0.f, dd = 0.f, da = 0.f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) { through += red[i]; dd += red[16 + i]; da += red[32 + i]; }
-      through *= ex2(eh + el) * (hs.x * gs.x);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int t = 4 * lane + i;
-        const auto four = [&](const float* v) { return (v[t] + v[Q + t]) + (v[2 * Q + t] + v[3 * Q + t]); };
-        const float st = rec[t], rp = four(rpairs), rs = four(rstate), qs = four(qstate);
-        r[i] = (st > 0.f ? rp / st : 0.f) + rs + rself[t];   // rp is by s, as the columns' sums are
-        a[i] = four(qpairs) + qs - rp;
-        bs[i] = st * rs;
-        time += qs * (rec[Q + t] + rec[2 * Q + t]) + bs[i] * ((eh - rec[Q + t]) + (el - rec[2 * Q + t]));
-        sa += a[i];
-        sum += bs[i];
-      }
-      float after = sa, before = sum;                    // sums over the lanes from mine on, and up to mine
+    if (warp >= 12) {                                    // four warps, a token a lane
+      const int t = quad * 32 + lane;
+      const float rate = P.A[h];
+      const auto four = [&](const float* v) { return (v[t] + v[Q + t]) + (v[2 * Q + t] + v[3 * Q + t]); };
+      const float st = rec[t], rp = four(rpairs), rs = four(rstate), qs = four(qstate), lt = rec[Q + t], lt2 = rec[2 * Q + t];
+      const float r = (st > 0.f ? __fdividef(rp, st) : 0.f) + rs + rself[t];   // rp is by s, as the columns' sums are
+      const float a = four(qpairs) + qs - rp, bs = st * rs;
+      float after = a, before = bs;                      // sums from this token on, and up to it
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const float va = __shfl_down_sync(0xffffffffu, after, o), vb = __shfl_up_sync(0xffffffffu, before, o);
         if (lane + o < 32) after += va;
         if (lane >= o) before += vb;
       }
-      before -= sum;
-      after -= sa;
-      float from[4];                                     // sum of a over t' >= t
+      const float time = warp_sum(qs * (lt + lt2) + bs * ((eh - lt) + (el - lt2)));
+      if (lane == 0) { red[48 + quad] = after; red[56 + quad] = time; }
+      if (lane == 31) red[52 + quad] = before;
+      const float through = warp_sum(lane < 16 ? red[lane] : 0.f) * ex2(eh + el) * (hs.x * gs.x);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      before -= bs;
 #pragma unroll
-      for (int i = 3; i >= 0; --i) { after += a[i]; from[i] = after; }
-      float2* out = W.parts + ((long long)b * W.units + u) * W.lp + (long long)c * Q + 4 * lane;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        out[i] = make_float2(from[i] + before + through, r[i]);
-        before += bs[i];
+      for (int k = 0; k < 4; ++k) {
+        if (k > quad) after += red[48 + k];
+        if (k < quad) before += red[52 + k];
       }
-      time = warp_sum(time);
-      // A's gradient: each contribution by the time that A works on it, which l tells; no differences of large sums
-      if (lane == 0) {
-        da = (da + time) + through * (eh + el);
-        W.unit_sums[bc * W.units + u] = make_float2(dd, (float)((double)da / decay_rate(P.A[h])));
+      const float all = after + before + through;        // gradient of A s
+      if (W.ptiles == 1) {
+        const float v = t < rows ? (rate * all + r) * rec[6 * Q + t] : 0.f;
+        if (t < out_rows) reinterpret_cast<T*>(P.ddt)[((long long)b * P.length + (long long)c * Q + t) * P.heads + h] = from_f32<T>(v);
+        const float sum_bias = warp_sum(v);
+        if (lane == 0) W.bias_sums[(bc * P.heads + h) * 4 + quad] = sum_bias;
+      } else {
+        W.parts[((long long)b * W.units + u) * W.lp + (long long)c * Q + t] = make_float2(all, r);
+      }
+      if (warp == 15) {
+        // A's gradient: each contribution by the time that A works on it, which l tells; no differences of large sums
+        const float dd = warp_sum(lane < 16 ? red[16 + lane] : 0.f);
+        float da = warp_sum(lane < 16 ? red[32 + lane] : 0.f);
+        da += ((red[56] + red[57]) + (red[58] + red[59])) + through * (eh + el);
+        if (lane == 0) W.unit_sums[bc * W.units + u] = make_float2(dd, __fdividef(da, decay_rate_f32(rate)));
       }
     }
     const float dskip = number(P.D, P.d_type, h) * yb, mixed = sc.y * both_back * yb;
@@ -1230,8 +1246,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       }
     }
     __syncthreads();
-    T* out = dx + (long long)h * P.dim + p0;
-    store_tile<T, kGradThreads>(out, dx_st, base + kGM, out_rows, cols, vector_ok(out, dx_st, 0, cols));
+    T* out = dx_at(h, p0);
+    store_tile<T, kGradThreads>(out, P.dx_st, base + kGM, out_rows, cols, vector_ok(out, P.dx_st, 0, cols));
   }
   __syncthreads();
 
@@ -1293,15 +1309,17 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   if (W.splits == 1) {
     __syncthreads();
     for (int hf = 0; hf < 2; ++hf) {
-      store_tile<T, kGradThreads>(dB + hf * 64, grp_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB + hf * 64, grp_st, 0, 64));
-      store_tile<T, kGradThreads>(dC + hf * 64, grp_st, base + kGHigh + hf * kTile64, out_rows, 64, vector_ok(dC + hf * 64, grp_st, 0, 64));
+      T *dB = group_at(P.dB) + hf * 64, *dC = group_at(P.dC) + hf * 64;
+      store_tile<T, kGradThreads>(dB, P.dg_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB, P.dg_st, 0, 64));
+      store_tile<T, kGradThreads>(dC, P.dg_st, base + kGHigh + hf * kTile64, out_rows, 64, vector_ok(dC, P.dg_st, 0, 64));
     }
   }
   tensor_end<512>(tmem);
 }
 
 // ---------------------------------------------------------------- sums behind the gradients
-// One CTA: a chunk of eight heads, a warp a head, four tokens a lane.  The gradient of dt, and the chunk's sum for the bias.
+// For heads of more than one unit (grad_kernel does the others itself): one CTA a chunk of eight heads, a warp a head, four
+// tokens a lane.  The gradient of dt, and the chunk's sum for the bias.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectiveParams P, const Space W) {
   __shared__ float grad[kPrepHeads][Q + 4];
@@ -1331,7 +1349,7 @@ __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectivePara
         if (4 * lane + i >= rows) out[i] = 0.f;
     }
     const float db = warp_sum((out[0] + out[1]) + (out[2] + out[3]));
-    if (lane == 0) W.bias_sums[((long long)b * W.nc + c) * P.heads + h] = db;
+    if (lane < 4) W.bias_sums[(((long long)b * W.nc + c) * P.heads + h) * 4 + lane] = lane ? 0.f : db;
     *reinterpret_cast<float4*>(&grad[warp][4 * lane]) = make_float4(out[0], out[1], out[2], out[3]);
   }
   __syncthreads();
@@ -1341,37 +1359,37 @@ __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectivePara
     if (h0 + hl < P.heads) ddt[(long long)t * P.heads + hl] = from_f32<T>(grad[hl][t]);
 }
 
-// One warp a head: gradients of A, the bias and D.
-__global__ void __launch_bounds__(128) finish_heads_kernel(const SelectiveParams P, const Space W) {
-  const int h = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+// The first `head_blocks` CTAs: gradients of A, the bias and D, a warp a head.  The others, where CTAs shared a group's
+// units: dB and dC from the splits' sums, four columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) finish_kernel(const SelectiveParams P, const Space W, int head_blocks) {
   launch_dependents();
   wait_for_launch();
-  if (h >= P.heads) return;
-  float da = 0.f, db = 0.f, dd = 0.f;
-  for (int i = lane; i < P.batch * W.nc; i += 32) {
-    db += W.bias_sums[(long long)i * P.heads + h];
-    for (int p = 0; p < W.ptiles; ++p) {
-      const float2 v = W.unit_sums[(long long)i * W.units + h * W.ptiles + p];
-      dd += v.x;
-      da += v.y;
+  if ((int)blockIdx.x < head_blocks) {
+    const int h = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (h >= P.heads) return;
+    float da = 0.f, db = 0.f, dd = 0.f;
+    for (int i = lane; i < P.batch * W.nc; i += 32) {
+      const float4 v4 = *reinterpret_cast<const float4*>(W.bias_sums + ((long long)i * P.heads + h) * 4);
+      db += (v4.x + v4.y) + (v4.z + v4.w);
+      for (int p = 0; p < W.ptiles; ++p) {
+        const float2 v = W.unit_sums[(long long)i * W.units + h * W.ptiles + p];
+        dd += v.x;
+        da += v.y;
+      }
     }
+    da = warp_sum(da);
+    db = warp_sum(db);
+    dd = warp_sum(dd);
+    if (lane == 0) {
+      if (P.dA) P.dA[h] = da;
+      if (P.dbias) put_number(P.dbias, P.bias_type, h, db);
+      if (P.dD) put_number(P.dD, P.d_type, h, dd);
+    }
+    return;
   }
-  da = warp_sum(da);
-  db = warp_sum(db);
-  dd = warp_sum(dd);
-  if (lane == 0) {
-    if (P.dA) P.dA[h] = da;
-    if (P.dbias) put_number(P.dbias, P.bias_type, h, db);
-    if (P.dD) put_number(P.dD, P.d_type, h, dd);
-  }
-}
-
-// dB and dC from the splits' sums, four columns a thread.
-template <typename T>
-__global__ void __launch_bounds__(256) finish_groups_kernel(const SelectiveParams P, const Space W) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x, width = (long long)P.groups * kN;
+  const long long i = (long long)(blockIdx.x - head_blocks) * kThreads + threadIdx.x, width = (long long)P.groups * kN;
   const long long all = (long long)P.batch * P.length * width;
-  wait_for_launch();
   if (i * 4 >= all) return;
   const long long token = i * 4 / width, b = token / P.length, t = token % P.length;
   const bool in = t < tokens_of(P, (int)b);
@@ -1496,11 +1514,6 @@ template <typename... A> int behind(void (*kernel)(A...), dim3 grid, int threads
   return launch_status();
 }
 
-template <typename T, bool REV, bool LO, bool TILED> int pass(const SelectiveParams& P, const Space& W, cudaStream_t st) {
-  if (int s = allow<state_pass_kernel<T, REV, LO, TILED>>(kPassSmem)) return s;
-  return behind(state_pass_kernel<T, REV, LO, TILED>, dim3(W.units, P.batch), kThreads, kPassSmem, st, P, W);
-}
-
 template <typename T> int prepare(const SelectiveParams& P, const Space& W, bool backward, cudaStream_t st) {
   const int head_blocks = (P.heads + kPrepHeads - 1) / kPrepHeads, tiles = !P.tiled ? 2 * P.groups : backward ? W.units : 0;
   prepare_kernel<T><<<dim3(W.nc, head_blocks + tiles, P.batch), kThreads, 0, st>>>(P, W, head_blocks);
@@ -1510,9 +1523,10 @@ template <typename T> int prepare(const SelectiveParams& P, const Space& W, bool
 template <typename T, bool TILED> int forward(const SelectiveParams& P, cudaStream_t st) {
   const Space W = space_of(P, false, TILED);
   if (int s = allow<out_kernel<T, TILED>>(kOutSmem)) return s;
+  if (int s = allow<state_pass_kernel<T, TILED>>(kPassSmem)) return s;
   if (int s = prepare<T>(P, W, false, st)) return s;
   if (W.nc > 1 || P.state_in || P.state_out)
-    if (int s = pass<T, false, false, TILED>(P, W, st)) return s;
+    if (int s = behind(state_pass_kernel<T, TILED>, dim3(W.units, P.batch), kThreads, kPassSmem, st, P, W)) return s;
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
   return behind(out_kernel<T, TILED>, dim3(W.nc, P.groups * W.splits, P.batch), kThreads, kOutSmem, st, P, W, per);
 }
@@ -1520,23 +1534,18 @@ template <typename T, bool TILED> int forward(const SelectiveParams& P, cudaStre
 template <typename T, bool TILED> int backward(const SelectiveParams& P, cudaStream_t st) {
   const Space W = space_of(P, true, TILED);
   if (int s = allow<grad_kernel<T, TILED>>(kGradSmem)) return s;
+  if (int s = allow<state_passes_kernel<T, TILED>>(kPassSmem)) return s;
   if (int s = prepare<T>(P, W, true, st)) return s;
-  if (W.nc > 1 || P.state_in || P.dstate_out || P.dstate_in) {
-    SelectiveParams F = P;
-    F.state_out = nullptr;
-    if (int s = pass<T, false, true, TILED>(F, W, st)) return s;
-    if (int s = pass<T, true, true, TILED>(P, W, st)) return s;
-  }
+  if (W.nc > 1 || P.state_in || P.dstate_out || P.dstate_in)
+    if (int s = behind(state_passes_kernel<T, TILED>, dim3(W.units, P.batch, 2), kThreads, kPassSmem, st, P, W)) return s;
   const int gunits = W.units / P.groups, per = (gunits + W.splits - 1) / W.splits;
   if (int s = behind(grad_kernel<T, TILED>, dim3(W.nc, P.groups * W.splits, P.batch), kGradThreads, kGradSmem, st, P, W, per)) return s;
-  if (int s = behind(finish_dt_kernel<T>, dim3(W.nc, (P.heads + kPrepHeads - 1) / kPrepHeads, P.batch), kThreads, 0, st, P, W)) return s;
-  if (P.dA || P.dD || P.dbias)
-    if (int s = behind(finish_heads_kernel, dim3((P.heads + 3) / 4), 128, 0, st, P, W)) return s;
-  if (W.splits > 1) {
-    const long long all = (long long)P.batch * P.length * P.groups * (kN / 4);
-    return behind(finish_groups_kernel<T>, dim3((unsigned)((all + 255) / 256)), 256, 0, st, P, W);
-  }
-  return kOk;
+  if (W.ptiles > 1)
+    if (int s = behind(finish_dt_kernel<T>, dim3(W.nc, (P.heads + kPrepHeads - 1) / kPrepHeads, P.batch), kThreads, 0, st, P, W)) return s;
+  const int head_blocks = P.dA || P.dD || P.dbias ? (P.heads + kThreads / 32 - 1) / (kThreads / 32) : 0;
+  const long long all = W.splits > 1 ? (long long)P.batch * P.length * P.groups * (kN / 4) : 0;
+  const long long blocks = head_blocks + (all + kThreads - 1) / kThreads;
+  return blocks ? behind(finish_kernel<T>, dim3((unsigned)blocks), kThreads, 0, st, P, W, head_blocks) : (int)kOk;
 }
 
 }  // namespace
