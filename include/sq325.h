@@ -415,9 +415,9 @@ int sq_distill_loss_grad(const sq_distill_args* args, void* stream);
  * x, y [batch,length,heads,dim], dt [batch,length,heads], B, C [batch,length,groups,128] of `type` SQ_F16 or SQ_BF16;
  * A fp32 [heads], <= 0; D, dt_bias [heads] of d_type / bias_type, or NULL (no term); state fp32 [batch,heads,dim,128]:
  * state_in (NULL: zero) before the first token, state_out (may be NULL) after the last.  dim <= 1024, heads a multiple
- * of groups; batch, and heads times dim / 64 rounded up, at most 65535; length <= 2^24.  The state and its sums are fp32; y, a 16-bit tensor, is made
- * from pairs' weights and states that are rounded to 16 bits (fp16: scaled) in the products.  A NaN or infinity in a
- * token reaches every token of its chunk of 128, and later ones.
+ * of groups; batch at most 65535, heads times dim / 64 rounded up at most 30000; length <= 2^24.  The state and its sums
+ * are fp32; y, a 16-bit tensor, is made from pairs' weights and states that are rounded to 16 bits (fp16: scaled) in the
+ * products.  A NaN or infinity in a token reaches every token of its chunk of 128, and later ones.
  * sq_selective_backward: gradients for the gradient dy of y and dstate_out of state_out (NULL: zero), with the forward's
  * inputs: dx, ddt (contiguous), dB, dC in `type`, and where not NULL dA fp32, dD, ddt_bias in their types and
  * dstate_in.  Sums have a fixed order.  workspace: sq_selective_workspace(..., backward) bytes. */
@@ -466,8 +466,8 @@ int sq_selective_step(const sq_selective_step_args* args, void* stream);
  *   z[t,c] = bias[c] + sum_k weight[c,k] x[t - (taps-1) + k, c],   y = z sigmoid(z) where silu, else z
  * weight [channels,taps], taps 2..4, bias [channels] or NULL, both of weight_type, which is `type` or SQ_F32.  state_in /
  * state_out [batch,taps-1,channels] in `type` hold the inputs before the first token (NULL: zero) and the last ones.
- * sq_causal_conv_forward with x and codes keeps the input in 8 bits (see below); with x NULL and codes it reads the kept
- * values in x's place.  sq_causal_conv_backward computes z again from x, or from the codes where x is NULL, and writes
+ * sq_causal_conv_forward with codes keeps the input in 8 bits besides (see below).  sq_causal_conv_backward computes z
+ * again from x, or from the codes where x is NULL, and writes
  * dx (contiguous, in `type`) and, where not NULL, dweight, dbias in weight_type and dstate_in; dstate_out may be NULL.
  * workspace: sq_causal_conv_workspace(...) bytes (backward). */
 typedef struct sq_causal_conv_args {
@@ -519,8 +519,8 @@ typedef struct sq_conv_scan_step_args {
 int sq_conv_scan_step(const sq_conv_scan_step_args* args, void* stream);
 
 /* Activations in 8 bits: in a row of x [rows,width] each 128 neighbouring values (the last block may have fewer) share
- * scale = max|x| (1 / 127), an fp32 product, and are kept as codes rint(x / scale) in [-127, 127]; scales [rows, ceil(width/128)].  A block
- * with a NaN or an infinity comes back as NaN.  sq_unpack_activations writes code * scale, rounded to `type`. */
+ * scale = max|x| (1 / 127), an fp32 product, and are kept as codes rint(x / scale) in [-127, 127]; scales [rows,
+ * ceil(width/128)].  A block with a NaN or an infinity comes back as NaN.  sq_unpack_activations writes code * scale, rounded to `type`. */
 int sq_pack_activations(const void* x, int64_t row_stride, int64_t rows, int width, int type, int8_t* codes, float* scales, void* stream);
 int sq_unpack_activations(const int8_t* codes, const float* scales, int64_t rows, int width, int type, void* out, void* stream);
 

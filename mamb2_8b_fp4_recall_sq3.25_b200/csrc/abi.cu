@@ -970,7 +970,7 @@ int selective_params(const sq_selective_args* a, const char* who, bool backward,
   if (a->batch < 1 || a->length < 1 || a->heads < 1 || a->dim < 1 || a->groups < 1) return bad("positive geometry required");
   if (a->heads % a->groups) return bad("heads must be divisible by B/C groups");
   if (a->dim > kScanMaxDim || a->length > 1 << 24 || a->batch > kMaxGrid) return bad("batch, length or dim is too large");
-  if ((int64_t)a->heads * ((a->dim + kScanTile - 1) / kScanTile) > kMaxGrid) return bad("heads is too large");
+  if ((int64_t)a->heads * ((a->dim + kScanTile - 1) / kScanTile) > kScanMaxUnits) return bad("heads is too large");
   if (!a->dt || !a->A || !a->workspace || (!tiled && (!a->x || !a->B || !a->C))) return bad("null pointer argument");
   if (!aligned(a->x, 2) || !aligned(a->dt, 2) || !aligned(a->B, 2) || !aligned(a->C, 2) || !aligned(a->A, 4) ||
       !aligned(a->state_in, 4) || !aligned(a->lengths, 4) || !aligned(a->workspace, 256))
@@ -1100,7 +1100,7 @@ int sq_causal_conv_forward(const sq_causal_conv_args* a, void* stream) {
   ConvParams P;
   if (int s = conv_params(a, "causal_conv_forward", P)) return s;
   const size_t n = a->type == SQ_F32 ? 4 : 2;
-  if (!a->y) return fail(SQ_EINVAL, "causal_conv_forward: null y");
+  if (!a->x || !a->y) return fail(SQ_EINVAL, "causal_conv_forward: null x or y");
   if (!aligned(a->y, n) || !aligned(a->state_out, n)) return fail(SQ_EINVAL, "causal_conv_forward: misaligned output");
   if (a->state_out && a->state_out == a->state_in) return fail(SQ_EINVAL, "causal_conv_forward: state_out must not be state_in");
   P.y = a->y; P.y_sb = a->y_batch_stride; P.y_st = a->y_token_stride; P.state_out = a->state_out;

@@ -4,9 +4,9 @@
 //   z[t,c] = bias[c] + sum_k w[c,k] x[t - (taps-1) + k, c],   y = z sigmoid(z) or z
 //
 // Tokens before the first are the carried state's, or zero.  Everything is fp32 inside and rounded once.  All of it is
-// bound by memory: a thread owns 16 bytes of channels and a strip of tokens, with the last taps' inputs in registers, so
-// that each input is read once but for the strips' edges.  The backward pass computes z again from the input (or from
-// its 8-bit codes); sums for weights and bias are kept a strip and added in order by a second kernel.
+// bound by memory: a thread owns four channels and a strip of tokens, with the last taps' inputs in registers, so that
+// each input is read once but for the strips' edges.  The backward pass computes z again from the input (or from its
+// 8-bit codes); sums for weights and bias are kept a strip and added in order by a second kernel, the same in every run.
 //
 // 8 bits: 128 neighbouring channels of a token share the scale max|x| (1 / 127), an fp32 product; a code is the fp32 quotient
 // x / scale rounded to even, at most 127.
@@ -14,6 +14,7 @@
 #include "selective.cuh"
 #include "device_util.cuh"
 #include "logits_util.cuh"
+#include "pairs.cuh"
 
 namespace sq {
 namespace {
@@ -55,14 +56,23 @@ template <typename T, int V> __device__ __forceinline__ void load_values(const T
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = to_f32(u.v[i]);
 }
-// Two neighbours are converted by one instruction.
-__device__ __forceinline__ void to_pair(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
-__device__ __forceinline__ void to_pair(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
-__device__ __forceinline__ void to_pair(float* p, float a, float b) { p[0] = a; p[1] = b; }
-template <typename T, int V> __device__ __forceinline__ void store_values(T* p, bool vec, int n, const float (&f)[V]) {
+// Neighbours 2i and 2i + 1.
+template <typename T, int V> __device__ __forceinline__ float2 two(const Values<T, V>& u, int i) {
+  if constexpr (sizeof(T) == 4) return make_float2(u.v[2 * i], u.v[2 * i + 1]);
+  else return unpack2<T>(reinterpret_cast<const uint32_t*>(&u)[i]);
+}
+template <typename T, int V> __device__ __forceinline__ void load_pairs(const T* p, bool vec, int n, float2 (&f)[V / 2]) {
+  const Values<T, V> u = raw_values<T, V>(p, vec, n);
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) f[i] = two<T, V>(u, i);
+}
+template <typename T, int V> __device__ __forceinline__ void store_pairs(T* p, bool vec, int n, const float2* f) {
   Values<T, V> u;
 #pragma unroll
-  for (int i = 0; i < V; i += 2) to_pair(&u.v[i], f[i], f[i + 1]);
+  for (int i = 0; i < V / 2; ++i) {
+    if constexpr (sizeof(T) == 4) { u.v[2 * i] = f[i].x; u.v[2 * i + 1] = f[i].y; }
+    else reinterpret_cast<uint32_t*>(&u)[i] = pack2<T>(f[i].x, f[i].y);
+  }
   if (vec) {
     *reinterpret_cast<decltype(u.q)*>(p) = u.q;
   } else {
@@ -85,11 +95,14 @@ template <int V> __device__ __forceinline__ void store_codes(int8_t* p, bool vec
   }
 }
 // A code as the low byte of 2^23 + 128 + code: no conversion, which has a sixteenth of the adds' rate.
-template <int V> __device__ __forceinline__ void decode(const Values<int8_t, V>& u, float scale, float (&f)[V]) {
+template <int V> __device__ __forceinline__ void decode(const Values<int8_t, V>& u, float scale, float2 (&f)[V / 2]) {
   const uint32_t* w = reinterpret_cast<const uint32_t*>(&u);
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    f[i] = (__uint_as_float(__byte_perm(w[i >> 2] ^ 0x80808080u, 0x4b000000u, 0x7540 + (i & 3))) - 8388736.0f) * scale;
+  for (int i = 0; i < V / 2; ++i) {
+    const uint32_t four = w[i >> 1] ^ 0x80808080u;
+    const float2 v = words2(__byte_perm(four, 0x4b000000u, 0x7540 + 2 * (i & 1)), __byte_perm(four, 0x4b000000u, 0x7541 + 2 * (i & 1)));
+    f[i] = mul2(add2(v, pair(-8388736.0f)), pair(scale));
+  }
 }
 // The largest magnitude of some values, as its fp32 bits; a NaN is larger than any number.
 template <int V> __device__ __forceinline__ uint32_t top_bits(const Values<float, V>& u) {
@@ -107,7 +120,7 @@ template <typename T, int V> __device__ __forceinline__ uint32_t top_bits(const 
 }
 // Scale and codes of the 128 values of which this thread has V; the others are its neighbours'.  A NaN or an infinity
 // makes the block's scale one, and its values NaN.
-template <typename T, int V> __device__ __forceinline__ float encode(const Values<T, V>& x, const float (&f)[V], Values<int8_t, V>& u) {
+template <typename T, int V> __device__ __forceinline__ float encode(const Values<T, V>& x, const float2 (&f)[V / 2], Values<int8_t, V>& u) {
   uint32_t m = top_bits(x);
 #pragma unroll
   for (int o = kPackBlock / V / 2; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -117,16 +130,17 @@ template <typename T, int V> __device__ __forceinline__ float encode(const Value
   if (top >= 1e-20f && top <= 3.0e38f) {
     // Quotients by the reciprocal: product, remainder, and the remainder's share give the quotient's rounding where
     // nothing underflows (Markstein).
-    const float inverse = __frcp_rn(scale);
+    const float2 inverse = pair(__frcp_rn(scale)), minus = pair(-scale);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float t = f[i] * inverse;
-      q[i] = __float_as_uint(fmaf(fmaf(-t, scale, f[i]), inverse, t) + kWhole);
+    for (int i = 0; i < V / 2; ++i) {
+      const float2 t = mul2(f[i], inverse), v = add2(fma2(fma2(t, minus, f[i]), inverse, t), pair(kWhole));
+      q[2 * i] = __float_as_uint(v.x);
+      q[2 * i + 1] = __float_as_uint(v.y);
     }
   } else {                                          // tiny ones by division; none of zeros, infinities and NaN
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      q[i] = scale > 0.f && scale <= 3.0e38f ? (uint32_t)__float2int_rn(fmaxf(-127.f, fminf(127.f, __fdiv_rn(f[i], scale)))) : 0;
+      q[i] = scale > 0.f && scale <= 3.0e38f ? (uint32_t)__float2int_rn(fmaxf(-127.f, fminf(127.f, __fdiv_rn(i & 1 ? f[i / 2].y : f[i / 2].x, scale)))) : 0;
   }
   uint32_t* w = reinterpret_cast<uint32_t*>(&u);
 #pragma unroll
@@ -140,40 +154,47 @@ __device__ __forceinline__ float reciprocal(float x) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-template <typename T> __device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (sizeof(T) == 4) return 1.0f / (1.0f + expf(-z));
-  else return reciprocal(1.0f + ex2(z * -kLog2e));  // a few ulp of fp32, far below a 16-bit result's half step
+template <typename T> __device__ __forceinline__ float2 sigmoid(float2 z) {
+  if constexpr (sizeof(T) == 4) {
+    return make_float2(1.0f / (1.0f + expf(-z.x)), 1.0f / (1.0f + expf(-z.y)));
+  } else {                                          // a few ulp of fp32, far below a 16-bit result's half step
+    float2 e = mul2(z, pair(-kLog2e));
+    e = add2(make_float2(ex2(e.x), ex2(e.y)), pair(1.0f));
+    return make_float2(reciprocal(e.x), reciprocal(e.y));
+  }
 }
 
 // A thread's V channels: weights and bias.
 template <typename WT, int V>
 struct Taps {
-  float w[kTaps][V], b[V];
+  float2 w[kTaps][V / 2], b[V / 2];
   __device__ Taps(const void* weights, const void* biases, int taps, int c, int n) {
     const WT* weight = reinterpret_cast<const WT*>(weights) + (long long)c * taps;
     if (taps == kTaps && n == V && ((uintptr_t)weight & (4 * sizeof(WT) - 1)) == 0) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float f[kTaps];
-        load_values<WT, kTaps>(weight + i * kTaps, true, kTaps, f);
+      for (int i = 0; i < V; i += 2) {
+        float f[2][kTaps];
+        load_values<WT, kTaps>(weight + i * kTaps, true, kTaps, f[0]);
+        load_values<WT, kTaps>(weight + (i + 1) * kTaps, true, kTaps, f[1]);
 #pragma unroll
-        for (int k = 0; k < kTaps; ++k) w[k][i] = f[k];
+        for (int k = 0; k < kTaps; ++k) w[k][i / 2] = make_float2(f[0][k], f[1][k]);
       }
     } else {
+      auto at = [&](int i, int j) { return i < n && j >= 0 ? to_f32(weight[i * taps + j]) : 0.f; };
 #pragma unroll
-      for (int i = 0; i < V; ++i)
+      for (int i = 0; i < V; i += 2)
 #pragma unroll
         for (int k = 0; k < kTaps; ++k) {
           const int j = k - (kTaps - taps);
-          w[k][i] = i < n && j >= 0 ? to_f32(weight[i * taps + j]) : 0.f;
+          w[k][i / 2] = make_float2(at(i, j), at(i + 1, j));
         }
     }
     const WT* bias = reinterpret_cast<const WT*>(biases) + c;
     if (biases) {
-      load_values<WT, V>(bias, n == V && ((uintptr_t)bias & (V * sizeof(WT) - 1)) == 0, n, b);
+      load_pairs<WT, V>(bias, n == V && ((uintptr_t)bias & (V * sizeof(WT) - 1)) == 0, n, b);
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) b[i] = 0.f;
+      for (int i = 0; i < V / 2; ++i) b[i] = pair(0.f);
     }
   }
 };
@@ -248,47 +269,49 @@ template <typename T, bool CODES, bool VEC, int V> struct Inputs {
       }
     }
   }
-  static __device__ __forceinline__ void get(const Raw& u, float scale, float (&f)[V]) {
+  static __device__ __forceinline__ void get(const Raw& u, float scale, float2 (&f)[V / 2]) {
     if constexpr (CODES) {
       decode<V>(u, scale, f);
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = to_f32(u.v[i]);
+      for (int i = 0; i < V / 2; ++i) f[i] = two<T, V>(u, i);
     }
   }
   // The input at any token, the state's before the first.
-  __device__ void at(const ConvParams& P, int b, int t, int c, float (&f)[V]) const {
+  __device__ void at(const ConvParams& P, int b, int t, int c, float2 (&f)[V / 2]) const {
     if (t >= 0) {
       float scale = 0.f;
       const Raw u = load(t, true, scale);
       get(u, scale, f);
     } else if (P.state_in && t >= 1 - P.taps) {
       const long long at = ((long long)b * (P.taps - 1) + t + P.taps - 1) * P.channels + c;
-      load_values<T, V>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
+      load_pairs<T, V>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
     } else {
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = 0.f;
+      for (int i = 0; i < V / 2; ++i) f[i] = pair(0.f);
     }
   }
 };
 
-// z of a token whose last four inputs are x[0..3], oldest first.  Taps that are not there are passed over, not
-// multiplied by zero: their inputs may be infinite.
+// z of a token's channels 2i and 2i + 1, whose last four inputs are x0..x3, oldest first.  Taps that are not there are
+// passed over, not multiplied by zero: their inputs may be infinite.
 template <typename WT, int V>
-__device__ __forceinline__ float conv_at(const Taps<WT, V>& W, const int taps, int i, float x0, float x1, float x2, float x3) {
-  float z = W.b[i];
-  if (taps > 3) z += W.w[0][i] * x0;
-  if (taps > 2) z += W.w[1][i] * x1;
-  return (z + W.w[2][i] * x2) + W.w[3][i] * x3;
+__device__ __forceinline__ float2 conv_at(const Taps<WT, V>& W, const int taps, int i, float2 x0, float2 x1, float2 x2, float2 x3) {
+  float2 z = W.b[i];
+  if (taps > 3) z = fma2(W.w[0][i], x0, z);
+  if (taps > 2) z = fma2(W.w[1][i], x1, z);
+  return fma2(W.w[3][i], x3, fma2(W.w[2][i], x2, z));
 }
 
-// MODE: 0 reads the input, 1 keeps it in 8 bits besides, 2 reads what was kept.  FAST: four taps, silu and whole aligned
-// pieces, as mixers have them; without them a third of the instructions would be the questions.
-template <typename T, typename WT, int MODE, bool FAST>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || MODE == 1 ? 5 : MODE == 2 ? 6 : 8) conv_kernel(const ConvParams P, int strip) {
+// KEEP: the input is kept in 8 bits besides.  FAST: four taps, silu and whole aligned pieces, as mixers have them; without
+// them a third of the instructions would be the questions.  Bound by memory, and by the latency of its loads: with the
+// next four tokens' loads under way while four are worked on, 4 x 2,048 tokens of 10,240 channels in bf16 take 43 us
+// (7.8 TB/s of input and output, part of it from L2).
+template <typename T, typename WT, bool KEEP, bool FAST>
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || KEEP ? 5 : 8) conv_kernel(const ConvParams P, int strip) {
   constexpr int V = kWide, U = 4;                                      // U: tokens whose loads are in flight together
-  constexpr bool KEEP = MODE == 1, CODES = MODE == 2, VEC = FAST;
-  using In = Inputs<T, CODES, VEC, V>;
+  constexpr bool VEC = FAST;
+  using In = Inputs<T, false, VEC, V>;
   const int taps = FAST ? kTaps : P.taps;
   const bool silu = FAST || P.silu;
   const int c = (blockIdx.y * kThreads + threadIdx.x) * V, b = blockIdx.z;
@@ -302,13 +325,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || MODE == 1 ? 5 : MO
   float* scales = KEEP ? P.scales + ((long long)b * P.length + t0) * blocks + c / kPackBlock : nullptr;
   if (n > 0 && blockIdx.x == 0 && P.state_out) {                       // the last inputs
     for (int j = 0; j < taps - 1; ++j) {
-      float f[V];
+      float2 f[V / 2];
       in.at(P, b, len - (taps - 1) + j, c, f);
-      store_values<T, V>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (taps - 1) + j) * P.channels + c, false, n, f);
+      store_pairs<T, V>(reinterpret_cast<T*>(P.state_out) + ((long long)b * (taps - 1) + j) * P.channels + c, false, n, f);
     }
   }
   if (t0 < end) {
-    float x[kTaps - 1][V], scale[U];
+    float2 x[kTaps - 1][V / 2];
+    float scale[U];
     typename In::Raw now[U];
     in.template load_batch<U>(t0, end, n > 0, now, scale);
     const Taps<WT, V> W(P.weight, P.bias, taps, n > 0 ? c : 0, n);
@@ -316,15 +340,15 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || MODE == 1 ? 5 : MO
     for (int k = 0; k < kTaps - 1; ++k)
       if (n > 0) in.at(P, b, t0 - (kTaps - 1) + k, c, x[k]);
     auto token = [&](const typename In::Raw& raw, float s, bool there) {
-      float out[V], f[V];
+      float2 out[V / 2], f[V / 2];
       In::get(raw, s, f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float z = conv_at<WT, V>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
-        out[i] = silu ? z * sigmoid<T>(z) : z;
+      for (int i = 0; i < V / 2; ++i) {
+        const float2 z = conv_at<WT, V>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
+        out[i] = silu ? mul2(z, sigmoid<T>(z)) : z;
         x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
       }
-      if (there) store_values<T, V>(y, VEC, n, out);
+      if (there) store_pairs<T, V>(y, VEC, n, out);
       y += P.y_st;
       if constexpr (KEEP) {
         Values<int8_t, V> q;
@@ -356,10 +380,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || MODE == 1 ? 5 : MO
     }
   }
   if (n <= 0) return;
-  const float zero[V] = {};
+  const float2 zero[V / 2] = {};
   y = reinterpret_cast<T*>(P.y) + b * P.y_sb + c;
   for (int t = max(t0, len); t < t1; ++t) {
-    store_values<T, V>(y + t * P.y_st, VEC, n, zero);
+    store_pairs<T, V>(y + t * P.y_st, VEC, n, zero);
     if constexpr (KEEP) {
       const long long row = (long long)b * P.length + t;
       store_codes<V>(P.codes + row * P.channels + c, VEC, n, Values<int8_t, V>{});
@@ -384,10 +408,11 @@ __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams
   const In in(P, b, c, n);
   const T* dy = reinterpret_cast<const T*>(P.dy) + b * P.dy_sb + c;
   T* dx = reinterpret_cast<T*>(P.dx) + (long long)b * P.length * P.channels + c;
-  float dw[kTaps][V] = {}, db[V] = {};
+  float2 dw[kTaps][V / 2] = {}, db[V / 2] = {};
   if (t0 < len || t0 == 0) {
     const int stop = t1 + kTaps - 1, end = min(stop, len), own = min(t1, len), lowest = t0 == 0 ? -back : t0;
-    float x[kTaps - 1][V], dz[kTaps - 1][V] = {}, scale[U];
+    float2 x[kTaps - 1][V / 2], dz[kTaps - 1][V / 2] = {};
+    float scale[U];
     typename In::Raw now[U];
     Values<T, V> up[U];
     auto load_up = [&](int t, Values<T, V>(&u)[U]) {
@@ -414,50 +439,50 @@ __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams
       constexpr bool INNER = decltype(inner)::value;
       const int to = at - (kTaps - 1);
       const bool mine = INNER || at < own;
-      float f[V], out[V];
+      float2 f[V / 2], out[V / 2];
       In::get(raw, s_in, f);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float d = to_f32(raw_up.v[i]);
+      for (int i = 0; i < V / 2; ++i) {
+        float2 d = two<T, V>(raw_up, i);
         if (silu) {
-          const float z = conv_at<WT, V>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
-          const float s = sigmoid<T>(z);
-          d *= fmaf(s, z * (1.0f - s), s);
+          const float2 z = conv_at<WT, V>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
+          const float2 s = sigmoid<T>(z);
+          d = mul2(d, fma2(s, mul2(z, fma2(s, pair(-1.0f), pair(1.0f))), s));
         }
-        if (!INNER && at >= end) d = 0.f;                              // z of what is not there may be anything
+        if (!INNER && at >= end) d = pair(0.f);                        // z of what is not there may be anything
         if (mine) {
-          db[i] += d;
-          if (taps > 3) dw[0][i] += d * x[0][i];
-          if (taps > 2) dw[1][i] += d * x[1][i];
-          dw[2][i] += d * x[2][i];
-          dw[3][i] += d * f[i];
+          db[i] = add2(db[i], d);
+          if (taps > 3) dw[0][i] = fma2(d, x[0][i], dw[0][i]);
+          if (taps > 2) dw[1][i] = fma2(d, x[1][i], dw[1][i]);
+          dw[2][i] = fma2(d, x[2][i], dw[2][i]);
+          dw[3][i] = fma2(d, f[i], dw[3][i]);
         }
         x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
         // dz[0..2] and d are those of `to` .. `to` + 3
-        float g = W.w[3][i] * dz[0][i] + W.w[2][i] * dz[1][i];
-        if (taps > 2) g += W.w[1][i] * dz[2][i];
-        if (taps > 3) g += W.w[0][i] * d;
+        float2 g = fma2(W.w[2][i], dz[1][i], mul2(W.w[3][i], dz[0][i]));
+        if (taps > 2) g = fma2(W.w[1][i], dz[2][i], g);
+        if (taps > 3) g = fma2(W.w[0][i], d, g);
         dz[0][i] = dz[1][i]; dz[1][i] = dz[2][i]; dz[2][i] = d;
         out[i] = g;
       }
       T* here = put;
       put += P.channels;
       if (INNER) {
-        store_values<T, V>(here, VEC, n, out);
+        store_pairs<T, V>(here, VEC, n, out);
         return;
       }
       if (to >= t1 || to < lowest) return;
       if (P.dstate_out && to >= len - back && to < len) {
-        float late[V];
+        float2 late[V / 2];
         const long long at_state = ((long long)b * back + to - (len - back)) * P.channels + c;
-        load_values<T, V>(reinterpret_cast<const T*>(P.dstate_out) + at_state, false, n, late);
+        load_pairs<T, V>(reinterpret_cast<const T*>(P.dstate_out) + at_state, false, n, late);
 #pragma unroll
-        for (int i = 0; i < V; ++i) out[i] += late[i];
+        for (int i = 0; i < V / 2; ++i) out[i] = add2(out[i], late[i]);
       }
       if (to >= 0) {
-        if (to < len) store_values<T, V>(here, VEC, n, out);
+        if (to < len) store_pairs<T, V>(here, VEC, n, out);
       } else if (P.dstate_in) {
-        store_values<T, V>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
+        store_pairs<T, V>(reinterpret_cast<T*>(P.dstate_in) + ((long long)b * back + to + back) * P.channels + c, false, n, out);
       }
     };
     const int calm = P.dstate_out ? min(own, len - back) : own;        // below it no gradient of the last inputs comes in
@@ -482,39 +507,37 @@ __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams
       }
     }
   }
-  const float zero[V] = {};
-  for (int t = max(t0, len); t < t1; ++t) store_values<T, V>(dx + (long long)t * P.channels, VEC, n, zero);
+  const float2 zero[V / 2] = {};
+  for (int t = max(t0, len); t < t1; ++t) store_pairs<T, V>(dx + (long long)t * P.channels, VEC, n, zero);
   if (P.dweight || P.dbias) {
     float* part = P.workspace + ((long long)b * gridDim.x + blockIdx.x) * (kTaps + 1) * P.channels + c;
 #pragma unroll
-    for (int k = 0; k <= kTaps; ++k) store_values<float, V>(part + (long long)k * P.channels, VEC, n, k < kTaps ? dw[k] : db);
+    for (int k = 0; k <= kTaps; ++k) store_pairs<float, V>(part + (long long)k * P.channels, VEC, n, k < kTaps ? dw[k] : db);
   }
 }
 
 // ---------------------------------------------------------------- tiles for a scan
 // Four channels c .. c + 3 of a token, `n` of them there; codes may lie on both sides of a block's border.
 template <typename T, bool CODES>
-__device__ __forceinline__ void four_channels(const ConvParams& P, int b, int t, int c, int n, bool vec, float (&f)[4]) {
+__device__ __forceinline__ void four_channels(const ConvParams& P, int b, int t, int c, int n, float2 (&f)[2]) {
   if (t < 0) {
     if (P.state_in && t >= 1 - P.taps) {
       const long long at = ((long long)b * (P.taps - 1) + t + P.taps - 1) * P.channels + c;
-      load_values<T, 4>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
+      load_pairs<T, 4>(reinterpret_cast<const T*>(P.state_in) + at, false, n, f);
     } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = 0.f;
+      f[0] = f[1] = pair(0.f);
     }
   } else if constexpr (CODES) {
     const long long row = (long long)b * P.length + t;
     const int8_t* q = P.codes + row * P.channels + c;
     const float* s = P.scales + row * ((P.channels + kPackBlock - 1) / kPackBlock);
-    if (vec) {
-      decode<4>(raw_values<int8_t, 4>(q, true, 4), s[c / kPackBlock], f);
-    } else {
+    float v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[i] = i < n ? (float)q[i] * s[(c + i) / kPackBlock] : 0.f;
-    }
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? (float)q[i] * s[(c + i) / kPackBlock] : 0.f;
+    f[0] = make_float2(v[0], v[1]);
+    f[1] = make_float2(v[2], v[3]);
   } else {
-    load_values<T, 4>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + t * P.x_st + c, vec, n, f);
+    load_pairs<T, 4>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + t * P.x_st + c, false, n, f);
   }
 }
 
@@ -528,7 +551,7 @@ __device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk,
   constexpr int kWideTile = TOKENS == 8 ? 16 : 32;                     // threads side by side: of 64 or 128 channels
   const int at = threadIdx.x % kWideTile, n = max(0, min(4, cols - at * 4)), c = n > 0 ? c0 + at * 4 : 0, r0 = threadIdx.x / kWideTile * TOKENS;
   const int t0 = chunk * kScanChunk + r0, end = n > 0 ? chunk * kScanChunk + rows : 0;
-  float z[TOKENS][4], x[3][4];
+  float2 z[TOKENS][2], x[3][2];
   typename In::Raw raw[VEC ? TOKENS + 3 : 1];
   float scale[VEC ? TOKENS + 3 : 1];
   const In in(P, b, c, 4);
@@ -543,22 +566,33 @@ __device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk,
     for (int k = 0; k < 3; ++k) In::get(raw[k], scale[k], x[k]);
   } else {
 #pragma unroll
-    for (int k = 0; k < 3; ++k) four_channels<T, CODES>(P, b, t0 < end ? t0 - 3 + k : -kTaps, c, n, false, x[k]);
+    for (int k = 0; k < 3; ++k) four_channels<T, CODES>(P, b, t0 < end ? t0 - 3 + k : -kTaps, c, n, x[k]);
   }
-  float top = 0.f;
 #pragma unroll
   for (int j = 0; j < TOKENS; ++j) {
-    float f[4];
+    float2 f[2];
     if constexpr (VEC) In::get(raw[j + 3], scale[j + 3], f);
-    else four_channels<T, CODES>(P, b, t0 + j < end ? t0 + j : -kTaps, c, n, false, f);
+    else four_channels<T, CODES>(P, b, t0 + j < end ? t0 + j : -kTaps, c, n, f);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float v = conv_at<WT, 4>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
-      z[j][i] = t0 + j < end && (VEC || i < n) ? v * sigmoid<T>(v) : 0.f;
-      top = fmaxf(top, fabsf(z[j][i]));
+    for (int i = 0; i < 2; ++i) {
+      const float2 v = conv_at<WT, 4>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
+      z[j][i] = mul2(v, sigmoid<T>(v));
       x[0][i] = x[1][i]; x[1][i] = x[2][i]; x[2][i] = f[i];
     }
   }
+  if (t0 + TOKENS > end || n < 4) {
+#pragma unroll
+    for (int j = 0; j < TOKENS; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (t0 + j >= end || 2 * i >= n) z[j][i].x = 0.f;
+        if (t0 + j >= end || 2 * i + 1 >= n) z[j][i].y = 0.f;
+      }
+  }
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < TOKENS; ++j)
+    top = fmaxf(top, fmaxf(fmaxf(fabsf(z[j][0].x), fabsf(z[j][0].y)), fmaxf(fabsf(z[j][1].x), fabsf(z[j][1].y))));
   uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = bits;
   __syncthreads();
@@ -568,12 +602,12 @@ __device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk,
   e = bits ? max(-60, min(60, e)) : 0;
   const float there = __uint_as_float((uint32_t)(127 - e) << 23);
   if (threadIdx.x == 0) *back = __uint_as_float((uint32_t)(127 + e) << 23);
+  const int piece = at / 2;
+  char* p = reinterpret_cast<char*>(out) + (piece >> 3) * 16384 + r0 * 128 + (at & 1) * 8;
 #pragma unroll
-  for (int j = 0; j < TOKENS; ++j) {
-    const int row = r0 + j, piece = at / 2;
-    const __half2 lo = __floats2half2_rn(z[j][0] * there, z[j][1] * there), hi = __floats2half2_rn(z[j][2] * there, z[j][3] * there);
-    char* p = reinterpret_cast<char*>(out) + (piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4) + (at & 1) * 8;
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+  for (int j = 0; j < TOKENS; ++j) {                                   // r0 is a multiple of eight
+    const float2 lo = mul2(z[j][0], pair(there)), hi = mul2(z[j][1], pair(there));
+    *reinterpret_cast<uint2*>(p + j * 128 + (((piece & 7) ^ (j & 7)) << 4)) = make_uint2(pack2<__half>(lo.x, lo.y), pack2<__half>(hi.x, hi.y));
   }
 }
 template <typename T, typename WT, bool CODES, bool VEC, bool GROUPS>
@@ -605,9 +639,9 @@ __global__ void __launch_bounds__(kThreads) conv_last_kernel(const ConvParams P)
   if (n <= 0) return;
   const int len = tokens_of(P, b);
   for (int j = 0; j < back; ++j) {
-    float f[4];
-    four_channels<T, CODES>(P, b, len - back + j, c, n, false, f);
-    store_values<T, 4>(reinterpret_cast<T*>(P.state_out) + ((long long)b * back + j) * P.channels + c, false, n, f);
+    float2 f[2];
+    four_channels<T, CODES>(P, b, len - back + j, c, n, f);
+    store_pairs<T, 4>(reinterpret_cast<T*>(P.state_out) + ((long long)b * back + j) * P.channels + c, false, n, f);
   }
 }
 
@@ -633,7 +667,7 @@ __global__ void __launch_bounds__(256) conv_weights_kernel(const ConvParams P, i
   }
 }
 
-// One token: a thread owns 16 bytes of channels, shifts their state and puts the token at its end.
+// One token: a thread owns four channels, shifts their state and puts the token at its end.
 template <typename T, typename WT, typename YT>
 __global__ void __launch_bounds__(kThreads) conv_step_kernel(const ConvStepParams P, int vec) {
   constexpr int V = kWide;
@@ -643,30 +677,26 @@ __global__ void __launch_bounds__(kThreads) conv_step_kernel(const ConvStepParam
   if (n <= 0) return;
   const bool v = vec && n == V;
   T* state = reinterpret_cast<T*>(P.state) + (long long)b * (P.taps - 1) * P.channels + c;
-  float x[kTaps][V] = {};
-  load_values<T, V>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + c, v, n, x[3]);
+  float2 x[kTaps][V / 2] = {};
+  load_pairs<T, V>(reinterpret_cast<const T*>(P.x) + b * P.x_sb + c, v, n, x[3]);
 #pragma unroll
   for (int k = 0; k < kTaps - 1; ++k) {
     const int j = k - (kTaps - P.taps);
-    if (j >= 0) load_values<T, V>(state + (long long)j * P.channels, v, n, x[k]);
+    if (j >= 0) load_pairs<T, V>(state + (long long)j * P.channels, v, n, x[k]);
   }
   const Taps<WT, V> W(P.weight, P.bias, P.taps, c, n);
-  float out[V];
+  float2 out[V / 2];
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], x[3][i]);
-    out[i] = P.silu ? z * sigmoid<T>(z) : z;
+  for (int i = 0; i < V / 2; ++i) {
+    const float2 z = conv_at<WT, V>(W, P.taps, i, x[0][i], x[1][i], x[2][i], x[3][i]);
+    out[i] = P.silu ? mul2(z, sigmoid<T>(z)) : z;
   }
   YT* y = reinterpret_cast<YT*>(P.y) + (long long)b * P.channels + c;
-  if constexpr (sizeof(YT) == sizeof(T)) {
-    store_values<T, V>(y, v, n, out);
-  } else {
-    store_values<float, V>(y, v, n, out);
-  }
+  store_pairs<YT, V>(y, v, n, out);
 #pragma unroll
   for (int k = 0; k < kTaps - 1; ++k) {
     const int j = k - (kTaps - P.taps);
-    if (j >= 0) store_values<T, V>(state + (long long)j * P.channels, v, n, x[k + 1]);
+    if (j >= 0) store_pairs<T, V>(state + (long long)j * P.channels, v, n, x[k + 1]);
   }
 }
 
@@ -685,9 +715,9 @@ __global__ void __launch_bounds__(kThreads, 10) pack_kernel(const PackParams P) 
                                       : no_values<T, V>();
 #pragma unroll
     for (int j = 0; j < kRows; ++j) {
-      float f[V];
+      float2 f[V / 2];
 #pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = to_f32(x[j].v[i]);
+      for (int i = 0; i < V / 2; ++i) f[i] = two<T, V>(x[j], i);
       Values<int8_t, V> q;
       const float scale = encode<T, V>(x[j], f, q);
       if (n > 0 && r0 + j < P.rows) {
@@ -717,16 +747,11 @@ __global__ void __launch_bounds__(kThreads, 10) unpack_kernel(const PackParams P
 #pragma unroll
     for (int j = 0; j < kRows; ++j)
       if (r0 + j < P.rows) {
-        float f[kCodes];
+        float2 f[kCodes / 2];
         decode<kCodes>(q[j], scale[j], f);
         T* out = reinterpret_cast<T*>(P.y) + (r0 + j) * P.width + c;
 #pragma unroll
-        for (int i = 0; i < kCodes; i += V) {
-          float part[V];
-#pragma unroll
-          for (int e = 0; e < V; ++e) part[e] = f[i + e];
-          store_values<T, V>(out + i, VEC, n - i, part);
-        }
+        for (int i = 0; i < kCodes; i += V) store_pairs<T, V>(out + i, VEC, n - i, f + i / 2);
       }
   }
 }
@@ -786,15 +811,13 @@ long long conv_workspace(int batch, int length, int channels) {
 int launch_conv_forward(const ConvParams& P, cudaStream_t st) {
   const int strip = strip_of(P.batch, P.length, P.channels, 16, 64), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
-  const bool fast = P.taps == kTaps && P.silu && (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) &&
+  const bool fast = P.taps == kTaps && P.silu && whole(P.x, P.type, kWide, P.x_sb, P.x_st) &&
                    whole(P.y, P.type, kWide, P.y_sb, P.y_st) && P.channels % kWide == 0 && ((uintptr_t)P.codes & (kWide - 1)) == 0;
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
-    const int mode = !P.codes ? 0 : P.x ? 1 : 2;
-    if (mode == 0) fast ? conv_kernel<T, WT, 0, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 0, false><<<grid, kThreads, 0, st>>>(P, strip);
-    else if (mode == 1) fast ? conv_kernel<T, WT, 1, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 1, false><<<grid, kThreads, 0, st>>>(P, strip);
-    else fast ? conv_kernel<T, WT, 2, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, 2, false><<<grid, kThreads, 0, st>>>(P, strip);
+    if (P.codes) fast ? conv_kernel<T, WT, true, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, true, false><<<grid, kThreads, 0, st>>>(P, strip);
+    else fast ? conv_kernel<T, WT, false, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_kernel<T, WT, false, false><<<grid, kThreads, 0, st>>>(P, strip);
     return launch_status();
   });
 }

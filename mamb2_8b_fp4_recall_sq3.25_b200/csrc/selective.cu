@@ -24,6 +24,7 @@
 #include <type_traits>
 #include "device_util.cuh"
 #include "logits_util.cuh"
+#include "pairs.cuh"
 #include "tc_util.cuh"
 
 namespace sq {
@@ -125,19 +126,6 @@ template <int N> __device__ __forceinline__ void settle(uint32_t (&r)[N]) {
     asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 h = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  } else {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v) {
-  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-  else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-}
 // Eight numbers are worked on as four pairs: the adders and multipliers take two fp32 numbers an instruction.
 struct Eight { float2 v[4]; };
 template <typename T> __device__ __forceinline__ Eight unpack8(uint4 u) {
@@ -146,12 +134,6 @@ template <typename T> __device__ __forceinline__ Eight unpack8(uint4 u) {
 template <typename T> __device__ __forceinline__ uint4 pack8(const Eight& f) {
   return make_uint4(pack2<T>(f.v[0].x, f.v[0].y), pack2<T>(f.v[1].x, f.v[1].y), pack2<T>(f.v[2].x, f.v[2].y), pack2<T>(f.v[3].x, f.v[3].y));
 }
-__device__ __forceinline__ float2 pair(float v) { return make_float2(v, v); }
-__device__ __forceinline__ float2 words2(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
-__device__ __forceinline__ float2 sub2(float2 a, float2 b) { return __ffma2_rn(b, pair(-1.f), a); }
 __device__ __forceinline__ Eight mul8(const Eight& a, float f) {
   return {{mul2(a.v[0], pair(f)), mul2(a.v[1], pair(f)), mul2(a.v[2], pair(f)), mul2(a.v[3], pair(f))}};
 }

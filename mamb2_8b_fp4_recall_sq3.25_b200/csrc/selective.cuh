@@ -8,6 +8,7 @@ namespace sq {
 constexpr int kScanChunk = 128;       // tokens of a chunk
 constexpr int kScanTile = 64;         // rows of a head's state that one CTA works on
 constexpr int kScanMaxDim = 1024;
+constexpr int kScanMaxUnits = 30000;                // heads * tiles of 64 rows: a grid holds two B/C tiles a group and eighths of the heads besides
 enum { SQ_TYPE_F16 = 0, SQ_TYPE_BF16 = 1, SQ_TYPE_F32 = 2 };
 
 struct SelectiveParams {

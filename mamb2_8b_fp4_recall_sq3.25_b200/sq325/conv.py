@@ -76,7 +76,7 @@ def conv_args(shape, dtype, x, packed, weight, bias, state, lengths, silu):
 
 
 def conv_forward(shape, dtype, x, packed, weight, bias, state, lengths, silu, want_state=False):
-    """(y, last inputs or None) on checked arguments: of x, or of the kept values where x is None."""
+    """(y, last inputs or None) on checked arguments; x is kept in 8 bits in `packed`, where that is given."""
     device = weight.device
     y = torch.empty(shape, dtype=dtype, device=device)
     last = torch.empty(shape[0], weight.shape[1] - 1, shape[2], dtype=dtype, device=device) if want_state else None

@@ -136,3 +136,20 @@ def test_tensors_on_the_host_are_refused():
                  lambda: sq325.conv_scan_step(x.half()[0], x, x, x, heads=1, groups=1, conv_state=x, state=x)):
         with pytest.raises(ValueError, match='CUDA'):
             call()
+
+
+def test_a_grid_has_room_for_every_tile():
+    lib = _lib()
+    for name in ('sq_selective_forward', 'sq_selective_backward'):
+        a = _scan(lib, name.endswith('backward'))
+        a.heads = a.groups = 30001                       # a grid's second dimension would hold two tiles a group and more
+        assert getattr(lib.load(), name)(C.byref(a), None) == lib.SQ_EINVAL
+        assert b'heads is too large' in lib.load().sq_last_error()
+
+
+def test_a_convolution_keeps_what_it_is_given():
+    lib = _lib()
+    a = _conv(lib)
+    a.x, a.codes, a.scales = 0, 4096, 4096
+    assert lib.load().sq_causal_conv_forward(C.byref(a), None) == lib.SQ_EINVAL
+    assert b'null x' in lib.load().sq_last_error()
