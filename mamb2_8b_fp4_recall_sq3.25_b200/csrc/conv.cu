@@ -541,23 +541,56 @@ __device__ __forceinline__ void four_channels(const ConvParams& P, int b, int t,
   }
 }
 
-// One CTA: a chunk's tile of x (64 channels of a head) or of B or C (128 of a group).  A thread has four channels of
-// TOKENS neighbouring tokens in registers, all loads before the first use; the tile's largest value gives its scale.
-// VEC: four taps, and four channels are one aligned load.
-template <typename T, typename WT, bool CODES, int TOKENS, bool VEC>
-__device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk, int c0, int cols, int rows, uint16_t* out, float* back,
-                                          uint32_t* tops) {
+// One CTA: a chunk's tile of B or C (128 channels of a group), or two of x (64 channels of a head each).  A thread has four
+// channels of eight neighbouring tokens in registers, all loads before the first use; a tile's largest value gives its
+// scale.  VEC: four taps, and four channels are one aligned load.
+constexpr int kTileThreads = 512;
+template <typename T, typename WT, bool CODES, bool VEC>
+__global__ void __launch_bounds__(kTileThreads, 2) conv_tiles_kernel(const ConvParams P, const ConvTiles A) {
+  constexpr int TOKENS = 8;
   using In = Inputs<T, CODES, true, 4>;
-  constexpr int kWideTile = TOKENS == 8 ? 16 : 32;                     // threads side by side: of 64 or 128 channels
-  const int at = threadIdx.x % kWideTile, n = max(0, min(4, cols - at * 4)), c = n > 0 ? c0 + at * 4 : 0, r0 = threadIdx.x / kWideTile * TOKENS;
+  __shared__ uint32_t tops[kTileThreads / 32];
+  const int chunk = blockIdx.x, b = blockIdx.z;
+  const int rows = min(kScanChunk, tokens_of(P, b) - chunk * kScanChunk);
+  if (rows <= 0) return;                                               // not read
+  const long long bc = (long long)b * A.chunks + chunk;
+  const bool group = (int)blockIdx.y < 2 * A.groups;
+  const int half = threadIdx.x >> 8;
+  int at, r0, c0, cols;
+  uint16_t* out = nullptr;
+  float* back = nullptr;
+  if (group) {
+    const int g = blockIdx.y >> 1, second = blockIdx.y & 1;
+    at = threadIdx.x & 31;
+    r0 = threadIdx.x / 32 * TOKENS;
+    c0 = A.heads * A.dim + (second ? A.groups * 128 : 0) + g * 128;
+    cols = 128;
+    out = (second ? A.c : A.b) + (bc * A.groups + g) * (kScanChunk * 128);
+    back = (second ? A.cback : A.bback) + bc * A.groups + g;
+  } else {
+    const int ptiles = A.units / A.heads, u = 2 * (blockIdx.y - 2 * A.groups) + half, p0 = (u % ptiles) * kScanTile;
+    at = threadIdx.x & 15;
+    r0 = (threadIdx.x & 255) / 16 * TOKENS;
+    c0 = u / ptiles * A.dim + p0;
+    cols = u < A.units ? min(kScanTile, A.dim - p0) : 0;
+    if (u < A.units) {
+      out = A.x + (bc * A.units + u) * (kScanChunk * kScanTile);
+      back = A.xback + bc * A.units + u;
+    }
+  }
+  const int n = max(0, min(4, cols - at * 4)), c = n > 0 ? c0 + at * 4 : 0;
   const int t0 = chunk * kScanChunk + r0, end = n > 0 ? chunk * kScanChunk + rows : 0;
   float2 z[TOKENS][2], x[3][2];
   typename In::Raw raw[VEC ? TOKENS + 3 : 1];
   float scale[VEC ? TOKENS + 3 : 1];
   const In in(P, b, c, 4);
   if constexpr (VEC) {
+    if (t0 > 0) {
+      in.template load_batch<TOKENS + 3>(t0 - 3, end, n > 0, raw, scale);
+    } else {
 #pragma unroll
-    for (int j = 0; j < TOKENS + 3; ++j) raw[j] = in.load(t0 - 3 + j, t0 - 3 + j >= 0 && t0 - 3 + j < end, scale[j]);
+      for (int j = 0; j < TOKENS + 3; ++j) raw[j] = in.load(j - 3, j >= 3 && j - 3 < end, scale[j]);
+    }
   }
   const int taps = VEC ? kTaps : P.taps;
   const Taps<WT, 4> W(P.weight, P.bias, taps, c, n);
@@ -597,11 +630,12 @@ __device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk,
   if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = bits;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 8; ++k) bits = max(bits, tops[k]);
+  for (int k = 0; k < 8; ++k) bits = max(bits, group ? max(tops[k], tops[8 + k]) : tops[half * 8 + k]);
+  if (!out) return;
   int e = (int)(bits >> 23) - 140;                                     // to [2^13, 2^14)
   e = bits ? max(-60, min(60, e)) : 0;
   const float there = __uint_as_float((uint32_t)(127 - e) << 23);
-  if (threadIdx.x == 0) *back = __uint_as_float((uint32_t)(127 + e) << 23);
+  if (r0 + at == 0) *back = __uint_as_float((uint32_t)(127 + e) << 23);
   const int piece = at / 2;
   char* p = reinterpret_cast<char*>(out) + (piece >> 3) * 16384 + r0 * 128 + (at & 1) * 8;
 #pragma unroll
@@ -610,27 +644,8 @@ __device__ __forceinline__ void conv_tile(const ConvParams& P, int b, int chunk,
     *reinterpret_cast<uint2*>(p + j * 128 + (((piece & 7) ^ (j & 7)) << 4)) = make_uint2(pack2<__half>(lo.x, lo.y), pack2<__half>(hi.x, hi.y));
   }
 }
-template <typename T, typename WT, bool CODES, bool VEC, bool GROUPS>
-__global__ void __launch_bounds__(256, GROUPS ? 2 : 4) conv_tiles_kernel(const ConvParams P, const ConvTiles A) {
-  __shared__ uint32_t tops[8];
-  const int chunk = blockIdx.x, b = blockIdx.z, u = blockIdx.y;
-  const int rows = min(kScanChunk, tokens_of(P, b) - chunk * kScanChunk);
-  if (rows <= 0) return;                                               // not read
-  const long long bc = (long long)b * A.chunks + chunk;
-  if constexpr (!GROUPS) {
-    const int ptiles = A.units / A.heads, h = u / ptiles, p0 = (u % ptiles) * kScanTile, cols = min(kScanTile, A.dim - p0);
-    conv_tile<T, WT, CODES, 8, VEC>(P, b, chunk, h * A.dim + p0, cols, rows, A.x + (bc * A.units + u) * (kScanChunk * kScanTile),
-                                    A.xback + bc * A.units + u, tops);
-  } else {
-    const int g = u >> 1;
-    const long long at = bc * A.groups + g;
-    conv_tile<T, WT, CODES, 16, VEC>(P, b, chunk, A.heads * A.dim + (u & 1 ? A.groups * 128 : 0) + g * 128, 128, rows,
-                                     (u & 1 ? A.c : A.b) + at * (kScanChunk * 128), (u & 1 ? A.cback : A.bback) + at, tops);
-  }
-}
 template <typename T, typename WT, bool CODES, bool VEC> void conv_tiles(const ConvParams& P, const ConvTiles& A, cudaStream_t st) {
-  conv_tiles_kernel<T, WT, CODES, VEC, true><<<dim3(A.chunks, 2 * A.groups, P.batch), 256, 0, st>>>(P, A);
-  conv_tiles_kernel<T, WT, CODES, VEC, false><<<dim3(A.chunks, A.units, P.batch), 256, 0, st>>>(P, A);
+  conv_tiles_kernel<T, WT, CODES, VEC><<<dim3(A.chunks, 2 * A.groups + (A.units + 1) / 2, P.batch), kTileThreads, 0, st>>>(P, A);
 }
 // The last inputs of a sequence.
 template <typename T, bool CODES>
