@@ -404,7 +404,7 @@ int sq_distill_loss_grad(const sq_distill_args* args, void* stream);
 /* ---------------------------------------------------------------- unquantised mixer states
  * The mixer's recurrence and short convolution in unquantised states, with their gradients, and activations in 8 bits
  * (no reference counterpart: the reference's scans carry quantised states, its training scan freezes A, D and dt_bias,
- * its convolution is mamba_ssm's).  All are asynchronous on `stream`, allocate nothing and keep nothing between calls
+ * its convolution comes from outside it).  All are asynchronous on `stream`, allocate nothing and keep nothing between calls
  * but the device's error word (sq_device_check).  Element (b,t,...) of a tensor lies at data + b * batch_stride +
  * t * token_stride, its last axes contiguous; tensors need their type's alignment only, workspaces 256 bytes.
  * lengths (int32 [batch], NULL: every sequence has `length` tokens) are held within [0, length]; tokens behind a

@@ -341,7 +341,9 @@ __device__ __forceinline__ double decay_rate(float A) {
   return fabsf(A) < 1e-20f ? -1e-20 : (double)A * 1.4426950408889634;
 }
 __device__ __forceinline__ float decay_rate_f32(float A) { return fabsf(A) < 1e-20f ? -1e-20f : A * kLog2e; }
-// One CTA: a chunk of eight heads (a warp a head, four tokens a lane), or a chunk's tile of B or C.
+// One CTA: a chunk of eight heads (a warp a head, four tokens a lane), or a chunk's tile of B or C (behind a convolution, of
+// dy).  Eight heads: their steps of a token are 16 neighbouring bytes.  2 x 2,048 tokens of 128 heads: 11 us, most of it a
+// launch's latency and the sums' chain in double; with the tiles of dy 28 us.
 constexpr int kPrepHeads = 8;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams P, const Space W, int head_blocks) {
@@ -460,7 +462,10 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
 // ---------------------------------------------------------------- states by chunk
 // One CTA walks the chunks of one unit (64 rows of a head's state), forwards or backwards.  The state is fp32 in
 // registers: thread (n, half) holds state[n][32 half .. +32].  A chunk's addition is B^T (w x), with w x as value and
-// remainder.  Written before each chunk: the state that enters it, value and (LO) remainder.
+// remainder.  Written before each chunk: the state that enters it, value and (LO) remainder.  Bound by the chain from chunk
+// to chunk (tokens, their largest value, the product, the new state: 2.9 us), not by bytes or products: 64 rows a CTA
+// let two walk side by side on an SM, 256 of them at once.  2 x 2,048 tokens of 128 heads: 48 us; both ways of a
+// backward pass, 512 walks on 296 places, 101 us.
 constexpr uint32_t kPassX = 2 * kTile128, kPassW = kPassX + kTile64, kPassBytes = kPassW + 2 * kTile64, kPassSmem = kPassBytes + 64;
 
 template <typename T, bool REV, bool LO, bool TILED>
@@ -639,7 +644,10 @@ __global__ void __launch_bounds__(kThreads, 2) state_passes_kernel(const Selecti
 // ---------------------------------------------------------------- outputs by chunk and group
 // One CTA: a chunk and some units of a group.  C B^T once (128 columns of TMEM), then a unit at a time: the pairs'
 // weights go to shared memory as the operand M, C H_in and M x to 64 columns each.  What a unit needs of the next is
-// on its way as soon as its products are done.
+// on its way as soon as its products are done.  Bound by a unit's chain (loads, weights, product, output: 5 us, three
+// CTA barriers) with two CTAs an SM, half of the issue slots in use: shared memory and TMEM have no room for a third.
+// 2 x 2,048 tokens of 128 heads: 74 us.  Exponentials a block in place of a pair on the diagonal, and L2 prefetches of
+// the next unit, change nothing.
 constexpr uint32_t kOutM = kTile128, kOutX = 2 * kTile128, kOutH = kOutX + kTile64, kOutRec = kOutH + kTile64, kRecBytes = 4 * Q * 4,
                    kOutTop = kOutRec + 2 * kRecBytes, kOutBar = kOutTop + 2 * Q * 4, kOutSmem = kOutBar + 32;
 
@@ -828,6 +836,10 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
 //      by row and by column.
 //   3. the pairs' part of x's gradient; prefix and suffix sums over the tokens give the gradient of A s.
 // After the last unit the group's sum gives the pairs' part of dB and dC in two products.
+// Bound by a unit's chain of three products and the barriers between them (four; they are the first stall), with one CTA an
+// SM: its shared memory and its 512 columns are full.  35% of the issue slots, 18% of memory.  2 x 2,048 tokens of 128
+// heads: 325 us (32 chunks x 8 groups, 16 units each).  Value and remainder side by side in
+// one product of 128 columns, as in state_pass_kernel, cost the overlap of a unit with the one before (345 us).
 constexpr uint32_t kGRecBytes = kRecord * Q * 4;
 constexpr uint32_t kGB = 0, kGC = kTile128, kGX = 2 * kTile128, kGY = kGX + kTile64, kGHigh = kGY + 2 * kTile64,
                    kGLow = kGHigh + 2 * kTile64, kGM = kGLow + 2 * kTile64, kGRec = kGM + kTile128, kGRow = kGRec + 2 * kGRecBytes,
@@ -1342,7 +1354,7 @@ __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectivePara
 }
 
 // The first `head_blocks` CTAs: gradients of A, the bias and D, a warp a head.  The others, where CTAs shared a group's
-// units: dB and dC from the splits' sums, four columns a thread.
+// units: dB and dC from the splits' sums, four columns a thread.  4 us.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const SelectiveParams P, const Space W, int head_blocks) {
   launch_dependents();
@@ -1410,7 +1422,8 @@ template <typename T> __device__ __forceinline__ float4 four(const T* p, bool ve
 }
 
 // A warp takes eight rows of a head's state, four at a time: eight lanes a row, four 16-byte loads a lane.  The state
-// does not wait for the kernel before, which may still be writing x, B and C.
+// does not wait for the kernel before, which may still be writing x, B and C.  Bound by memory: a state is read and written
+// once.  64 rows of 128 heads x 64 x 128: 537 MB in 80 us, 6.7 TB/s.
 template <typename T, typename X>
 __global__ void __launch_bounds__(128) step_kernel(const SelectiveStepParams P) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y, b = blockIdx.z, g = h / (P.heads / P.groups);
