@@ -392,15 +392,29 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || KEEP ? 5 : 8) conv
   }
 }
 
+// Copies to shared memory that a thread makes for itself: it alone waits for them and reads them.  `take`: else zeros.
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" :: "r"(dst), "l"(src), "r"(take ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ uint2 read_own(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
 // A strip's gradients: dz_t = dy_t y'(z_t), dx_t = sum_k w_k dz_{t + taps-1 - k}, and the strip's sums of dz_t x_{t - (taps-1) + k}
-// and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.  128 registers a thread (sums, taps and
-// two batches of loads) leave 16 warps an SM, which bounds it: half of the issue slots, 36% of memory.  4 x 2,048 tokens of
-// 10,240 channels in bf16: 119 us, 4.2 TB/s.  Two channels a thread have twice the warps and are slower (100 us
-// in place of 72 for ragged lengths): loads of four bytes keep less in flight.
+// and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.  Bound by registers (sums, taps and what
+// is under way) and with them by the loads in flight.  RING: those of 16-bit tensors go to shared memory, twelve tokens of
+// a thread, which leaves 96 registers and five CTAs an SM; 4 x 2,048 tokens of 10,240 channels in bf16 take 105 us, 4.8 TB/s.
+// In registers (odd forms, fp32, codes) eight tokens and four CTAs: 119 us, 117 from codes; codes in the ring, by
+// copies of four bytes, take 167.  Two channels a thread have twice the warps, but in loads of four bytes, and are slower by
+// a third.
+constexpr int kStages = 3, kRingCtas = 5;
 template <typename T, typename WT, bool CODES, bool FAST>
-__global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams P, int strip) {
+__global__ void __launch_bounds__(kThreads, FAST && !CODES && sizeof(T) == 2 ? kRingCtas : 4) conv_grad_kernel(const ConvParams P, int strip) {
   constexpr int V = kWide, U = 4;
-  constexpr bool VEC = FAST;
+  constexpr bool VEC = FAST, RING = FAST && !CODES && sizeof(T) == 2;
+  __shared__ __align__(16) uint2 ring[RING ? kStages * U * 2 * kThreads : 1];
   using In = Inputs<T, CODES, VEC, V>;
   const int taps = FAST ? kTaps : P.taps;
   const bool silu = FAST || P.silu;
@@ -415,9 +429,9 @@ __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams
   if (t0 < len || t0 == 0) {
     const int stop = t1 + kTaps - 1, end = min(stop, len), own = min(t1, len), lowest = t0 == 0 ? -back : t0;
     float2 x[kTaps - 1][V / 2], dz[kTaps - 1][V / 2] = {};
-    float scale[U];
-    typename In::Raw now[U];
-    Values<T, V> up[U];
+    float scale[RING ? 1 : U];
+    typename In::Raw now[RING ? 1 : U];
+    Values<T, V> up[RING ? 1 : U];
     auto load_up = [&](int t, Values<T, V>(&u)[U]) {
       const T* p = dy + t * P.dy_st;
       if (t + U <= end) {
@@ -431,8 +445,30 @@ __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams
         }
       }
     };
-    in.template load_batch<U>(t0, end, true, now, scale);
-    load_up(t0, up);
+    // RING: the next stages of U tokens each, x and dy by turns
+    const uint32_t slots = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 8;
+    uint32_t put_at = 0, get_at = 0;
+    const T *x_next = in.x + t0 * in.step, *dy_next = dy + t0 * P.dy_st;
+    auto stage = [&](int t) {
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const uint32_t a = slots + put_at + j * (2 * kThreads * 8);
+        const bool there = t + j < end;
+        copy_async(a, there ? x_next : in.x, there);
+        copy_async(a + kThreads * 8, there ? dy_next : dy, there);
+        x_next += in.step;
+        dy_next += P.dy_st;
+      }
+      put_at = (put_at + U * 2 * kThreads * 8) % (kStages * U * 2 * kThreads * 8);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (RING) {
+#pragma unroll
+      for (int k = 0; k < kStages - 1; ++k) stage(t0 + k * U);
+    } else {
+      in.template load_batch<U>(t0, end, true, now, scale);
+      load_up(t0, up);
+    }
     const Taps<WT, V> W(P.weight, P.bias, taps, c, n);
 #pragma unroll
     for (int k = 0; k < kTaps - 1; ++k) in.at(P, b, t0 - (kTaps - 1) + k, c, x[k]);
@@ -489,26 +525,46 @@ __global__ void __launch_bounds__(kThreads, 4) conv_grad_kernel(const ConvParams
       }
     };
     const int calm = P.dstate_out ? min(own, len - back) : own;        // below it no gradient of the last inputs comes in
-    for (int t = t0; t < stop; t += U) {
-      typename In::Raw next[U];
-      Values<T, V> up_next[U];
-      float later[U];
-      in.template load_batch<U>(t + U, end, true, next, later);
-      load_up(t + U, up_next);
-      if (t >= t0 + U && t + U <= calm) {
-#pragma unroll
-        for (int j = 0; j < U; ++j) token(now[j], scale[j], up[j], t + j, std::true_type{});
-      } else {
-#pragma unroll
-        for (int j = 0; j < U; ++j) token(now[j], scale[j], up[j], t + j, std::false_type{});
-      }
+    auto tokens = [&](int t, auto inner) {
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        now[j] = next[j];
-        scale[j] = later[j];
-        up[j] = up_next[j];
+        if constexpr (RING) {
+          const uint32_t a = slots + get_at + j * (2 * kThreads * 8);
+          typename In::Raw raw;
+          Values<T, V> raw_up;
+          raw.q = read_own(a);
+          raw_up.q = read_own(a + kThreads * 8);
+          token(raw, 0.f, raw_up, t + j, inner);
+        } else {
+          token(now[j], scale[j], up[j], t + j, inner);
+        }
+      }
+    };
+    for (int t = t0; t < stop; t += U) {
+      typename In::Raw next[RING ? 1 : U];
+      Values<T, V> up_next[RING ? 1 : U];
+      float later[RING ? 1 : U];
+      if constexpr (RING) {
+        stage(t + (kStages - 1) * U);                                  // its place was read a turn ago
+        asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
+      } else {
+        in.template load_batch<U>(t + U, end, true, next, later);
+        load_up(t + U, up_next);
+      }
+      if (t >= t0 + U && t + U <= calm) tokens(t, std::true_type{});
+      else tokens(t, std::false_type{});
+      if constexpr (RING) {
+        get_at = (get_at + U * 2 * kThreads * 8) % (kStages * U * 2 * kThreads * 8);
+      } else {
+#pragma unroll
+        for (int j = 0; j < U; ++j) {
+          now[j] = next[j];
+          scale[j] = later[j];
+          up[j] = up_next[j];
+        }
       }
     }
+    if constexpr (RING) asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
   const float2 zero[V / 2] = {};
   for (int t = max(t0, len); t < t1; ++t) store_pairs<T, V>(dx + (long long)t * P.channels, VEC, n, zero);
