@@ -406,12 +406,12 @@ __device__ __forceinline__ uint2 read_own(uint32_t a) {
 // and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.  Bound by registers (sums, taps and what
 // is under way) and with them by the loads in flight.  RING: those of 16-bit tensors go to shared memory, twelve tokens of
 // a thread, which leaves 96 registers and five CTAs an SM; 4 x 2,048 tokens of 10,240 channels in bf16 take 105 us, 4.8 TB/s.
-// In registers (odd forms, fp32, codes) eight tokens and four CTAs: 119 us, 117 from codes; codes in the ring, by
-// copies of four bytes, take 167.  Two channels a thread have twice the warps, but in loads of four bytes, and are slower by
+// In registers (odd forms, codes) eight tokens and four CTAs: 119 us, 117 from codes; codes in the ring, by
+// copies of four bytes, take 167.  fp32 has three CTAs (188 us; four spill, 215).  Two channels a thread have twice the warps, but in loads of four bytes, and are slower by
 // a third.
 constexpr int kStages = 3, kRingCtas = 5;
 template <typename T, typename WT, bool CODES, bool FAST>
-__global__ void __launch_bounds__(kThreads, FAST && !CODES && sizeof(T) == 2 ? kRingCtas : 4) conv_grad_kernel(const ConvParams P, int strip) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : FAST && !CODES ? kRingCtas : 4) conv_grad_kernel(const ConvParams P, int strip) {
   constexpr int V = kWide, U = 4;
   constexpr bool VEC = FAST, RING = FAST && !CODES && sizeof(T) == 2;
   __shared__ __align__(16) uint2 ring[RING ? kStages * U * 2 * kThreads : 1];
