@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
 // One CTA walks the chunks of one unit (64 rows of a head's state), forwards or backwards.  The state is fp32 in
 // registers: thread (n, half) holds state[n][32 half .. +32].  A chunk's addition is B^T (w x), with w x as value and
 // remainder.  Written before each chunk: the state that enters it, value and (LO) remainder.  Bound by the chain from chunk
-// to chunk (tokens, their largest value, the product, the new state: 2.9 us), not by bytes or products: 64 rows a CTA
+// to chunk (tokens, their largest value, the product, the new state: 2.6 to 3 us), not by bytes or products: 64 rows a CTA
 // let two walk side by side on an SM, 256 of them at once.  2 x 2,048 tokens of 128 heads: 48 us; both ways of a
 // backward pass, 512 walks on 296 places, 101 us.
 constexpr uint32_t kPassX = 2 * kTile128, kPassW = kPassX + kTile64, kPassBytes = kPassW + 2 * kTile64, kPassSmem = kPassBytes + 64;
