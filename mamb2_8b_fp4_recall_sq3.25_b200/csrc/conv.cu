@@ -365,9 +365,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || KEEP ? 5 : 8) conv
       typename In::Raw next[U];
       float later[U];
       in.template load_batch<U>(t + U, end, n > 0, next, later);
-      if (n > 0 && t + U <= end) {
+      if (t + U <= end) {                                              // the same for the whole CTA: codes take shuffles
 #pragma unroll
-        for (int j = 0; j < U; ++j) token(now[j], scale[j], true);
+        for (int j = 0; j < U; ++j) token(now[j], scale[j], n > 0);
       } else {
 #pragma unroll
         for (int j = 0; j < U; ++j) token(now[j], scale[j], n > 0 && t + j < end);
