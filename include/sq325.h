@@ -417,7 +417,9 @@ int sq_distill_loss_grad(const sq_distill_args* args, void* stream);
  * state_in (NULL: zero) before the first token, state_out (may be NULL) after the last.  dim <= 1024, heads a multiple
  * of groups; batch at most 65535, heads times dim / 64 rounded up at most 30000; length <= 2^24.  The state and its sums
  * are fp32; y, a 16-bit tensor, is made from pairs' weights and states that are rounded to 16 bits (fp16: scaled) in the
- * products.  A NaN or infinity in a token reaches every token of its chunk of 128, and later ones.
+ * products.  What depends on a NaN or an infinity is not finite; the rest of its chunk of 128 tokens, and of later ones (earlier
+ * ones, for gradients), is as without it or NaN, and behind B or C that holds for all heads of the group.  A dt of minus
+ * infinity passes its token over.
  * sq_selective_backward: gradients for the gradient dy of y and dstate_out of state_out (NULL: zero), with the forward's
  * inputs: dx, ddt (contiguous), dB, dC in `type`, and where not NULL dA fp32, dD, ddt_bias in their types and
  * dstate_in.  Sums have a fixed order.  workspace: sq_selective_workspace(..., backward) bytes. */

@@ -695,7 +695,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) conv_tiles_kernel(const ConvP
   int e = (int)(bits >> 23) - 140;                                     // to [2^13, 2^14)
   e = bits ? max(-60, min(60, e)) : 0;
   const float there = __uint_as_float((uint32_t)(127 - e) << 23);
-  if (r0 + at == 0) *back = __uint_as_float((uint32_t)(127 + e) << 23);
+  // an infinity leaves a tile's other numbers no scale: all that is made of them is NaN
+  if (r0 + at == 0) *back = __uint_as_float(bits >= 0x7f800000u ? 0x7fffffffu : (uint32_t)(127 + e) << 23);
   const int piece = at / 2;
   char* p = reinterpret_cast<char*>(out) + (piece >> 3) * 16384 + r0 * 128 + (at & 1) * 8;
 #pragma unroll

@@ -152,8 +152,10 @@ template <typename T> struct Two;
 template <> struct Two<__half> { using type = __half2; };
 template <> struct Two<__nv_bfloat16> { using type = __nv_bfloat162; };
 
-// The power of two that brings `bits` (a maximum's, sign cleared) to [2^13, 2^14) and its inverse: {there, back}.
+// The power of two that brings `bits` (a maximum's, sign cleared) to [2^13, 2^14) and its inverse: {there, back}.  NaN where the
+// maximum is an infinity or NaN, which leaves the other numbers no scale: what is made of them is then NaN, and not zero.
 __device__ __forceinline__ float2 scale_of(uint32_t bits, int most = 60) {
+  if (bits >= 0x7f800000u) return make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));
   int e = (int)(bits >> 23) - 140;
   e = bits ? max(-most, min(most, e)) : 0;              // products of two scales stay numbers
   return make_float2(__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23));

@@ -7,7 +7,8 @@ Per head, with s_t = softplus(dt_t + dt_bias),
 H is fp32 [dim, 128]; B and C are shared by the heads of a group.  Where `codec.scan` and `state_codec.scan` carry
 quantised states, this one carries them whole, and where `state_training.scan_training` freezes A, D and dt_bias, it has
 gradients for everything, the states among them.  Nothing but the inputs is kept for the backward pass.  A is negative
-(the largest decay is 1); a NaN or an infinity in a token reaches every token of its chunk of 128, and later ones.
+(the largest decay is 1).  What depends on a NaN or an infinity is not finite, and other values of its chunk of 128 tokens and
+of later ones may be NaN with it, in its head, or behind B and C in its group; a dt of minus infinity passes its token over.
 """
 from __future__ import annotations
 
