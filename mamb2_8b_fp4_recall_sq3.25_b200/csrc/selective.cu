@@ -154,11 +154,12 @@ template <> struct Two<__nv_bfloat16> { using type = __nv_bfloat162; };
 
 // The power of two that brings `bits` (a maximum's, sign cleared) to [2^13, 2^14) and its inverse: {there, back}.  NaN where the
 // maximum is an infinity or NaN, which leaves the other numbers no scale: what is made of them is then NaN, and not zero.
+// Zeros come back by 0, so that they weigh nothing where scales are compared.
 __device__ __forceinline__ float2 scale_of(uint32_t bits, int most = 60) {
   if (bits >= 0x7f800000u) return make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));
   int e = (int)(bits >> 23) - 140;
   e = bits ? max(-most, min(most, e)) : 0;              // products of two scales stay numbers
-  return make_float2(__uint_as_float((uint32_t)(127 - e) << 23), __uint_as_float((uint32_t)(127 + e) << 23));
+  return make_float2(__uint_as_float((uint32_t)(127 - e) << 23), bits ? __uint_as_float((uint32_t)(127 + e) << 23) : 0.f);
 }
 
 __device__ __forceinline__ float number(const void* p, int type, int i) {
@@ -188,7 +189,7 @@ struct Space {
   uint16_t *xt, *yt;                  // [B][nc][units][128][64]: x and dy in the same form, behind a convolution
   float *xback, *yback;               // [B][nc][units]
   uint16_t *h, *g;                    // [B][nc][units][2][8][128][8]: states entering a chunk, gradients of those leaving it
-  float2 *hs, *gs;                    // [B][nc][units]: scale of the state, scale of the chunk's weighted tokens
+  float2 *hs, *gs;                    // [B][nc][units]: scale of the state, scale of the chunk's weighted tokens; 0 of zeros
   float2* parts;                      // [B][units][lp]: gradient of A s, gradient of s through the tokens
   float2* unit_sums;                  // [B][nc][units]: gradients of D and of A by chunk
   float* bias_sums;                   // [B][nc][H][4]: gradient of the bias by 32 tokens
@@ -957,7 +958,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   load_x(u0);
   load_y(u0);
   cp_commit();
-  // units' sums for C and B share a scale: that of the largest product of a state's and its tokens' scales
+  // units' sums for C and B share a scale: that of the largest product of a state's and its tokens' scales.  A head whose
+  // state or tokens are zero has none: it would take the bits of heads with small gradients.
   float cscale = 0.f, bscale = 0.f;
   if (has_h || has_g)
     for (int u = u0; u < u1; ++u) {
@@ -965,6 +967,8 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       cscale = fmaxf(cscale, hs.x * gs.y);
       bscale = fmaxf(bscale, gs.x * hs.y);
     }
+  if (cscale == 0.f) cscale = 1.f;
+  if (bscale == 0.f) bscale = 1.f;
   const float bback = W.bback[tile_at], cback = W.cback[tile_at], both_back = bback * cback;
   if (threadIdx.x == 0) {
     tiles.wait(ok, P.err);
@@ -1021,7 +1025,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     float2 hs = make_float2(1.f, 1.f), gs = make_float2(1.f, 1.f);
     if (has_h || has_g) { hs = W.hs[bc * W.units + u]; gs = W.gs[bc * W.units + u]; }
     const float from_in = ex2(lh + ll), to_end = ex2((eh - lh) + (el - ll));
-    const float wy = has_h ? from_in * (hs.x / cscale) * yb : 0.f, wx = has_g ? s * to_end * (gs.x / bscale) * xb : 0.f;
+    const float wy = has_h && gs.y != 0.f ? from_in * (hs.x / cscale) * yb : 0.f, wx = has_g && hs.y != 0.f ? s * to_end * (gs.x / bscale) * xb : 0.f;
     float2 gh2 = make_float2(0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
