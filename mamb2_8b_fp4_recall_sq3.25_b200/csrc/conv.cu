@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) conv_tiles_kernel(const ConvP
   for (int k = 0; k < 8; ++k) bits = max(bits, group ? max(tops[k], tops[8 + k]) : tops[half * 8 + k]);
   if (!out) return;
   int e = (int)(bits >> 23) - 140;                                     // to [2^13, 2^14)
-  e = bits ? max(-60, min(60, e)) : 0;
+  e = bits ? max(-110, e) : 0;
   const float there = __uint_as_float((uint32_t)(127 - e) << 23);
   // an infinity leaves a tile's other numbers no scale: all that is made of them is NaN
   if (r0 + at == 0) *back = __uint_as_float(bits >= 0x7f800000u ? 0x7fffffffu : (uint32_t)(127 + e) << 23);

@@ -18,7 +18,9 @@
 //   * the pairs' weights exp(l_t - l_s) s_s (C_t . B_s) beside x and dy, in their type;
 //   * the states in y, and the operands of dB and dC beside the states and of the pairs' part, in fp16.
 // Their results are 16-bit tensors, whose own rounding is as large.  fp16 operands are scaled by powers of two per row,
-// tile, chunk or CTA.  A bf16 number of B or C below 2^-28 of its tile's largest loses bits that no sum can hold.
+// tile, chunk or CTA, whatever the range of bf16; tokens and states of up to 2^118 have sums that are fp32 numbers.  A bf16 number of B or
+// C below 2^-28 of its tile's largest loses bits that no sum can hold; so do a head's products for dB and dC below 2^-28 of the
+// largest among the heads of its CTA.
 // Sums of A s are doubles, kept as two floats: neighbours' differences keep 24 bits wherever in the chunk they lie.
 #include "selective.cuh"
 #include <type_traits>
@@ -151,14 +153,18 @@ __device__ __forceinline__ __nv_bfloat162 fold(__nv_bfloat162 m, uint32_t v) { r
 template <typename T> struct Two;
 template <> struct Two<__half> { using type = __half2; };
 template <> struct Two<__nv_bfloat16> { using type = __nv_bfloat162; };
+// Pairs' weights in bf16, a product of two scaled rows (2^35 at most) each: the sums that they make with tokens of up to 2^118 are fp32
+// numbers.
+constexpr float kWeightThere = 0x1p-32f, kWeightBack = 0x1p32f;
 
 // The power of two that brings `bits` (a maximum's, sign cleared) to [2^13, 2^14) and its inverse: {there, back}.  NaN where the
 // maximum is an infinity or NaN, which leaves the other numbers no scale: what is made of them is then NaN, and not zero.
 // Zeros come back by 0, so that they weigh nothing where scales are compared.
-__device__ __forceinline__ float2 scale_of(uint32_t bits, int most = 60) {
+// Maxima below 2^-97 are brought less far, so that a scale is a normal number.
+__device__ __forceinline__ float2 scale_of(uint32_t bits) {
   if (bits >= 0x7f800000u) return make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));
   int e = (int)(bits >> 23) - 140;
-  e = bits ? max(-most, min(most, e)) : 0;              // products of two scales stay numbers
+  e = bits ? max(-110, e) : 0;
   return make_float2(__uint_as_float((uint32_t)(127 - e) << 23), bits ? __uint_as_float((uint32_t)(127 + e) << 23) : 0.f);
 }
 
@@ -396,7 +402,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const SelectiveParams
     m = 0;
 #pragma unroll
     for (int k = 0; k < kThreads / 32; ++k) m = max(m, tops[k]);
-    const float2 sc = scale_of(__float_as_uint(to_f32(from_bits<T>(m))), narrow ? 60 : 110);
+    const float2 sc = scale_of(__float_as_uint(to_f32(from_bits<T>(m))));
     const long long bc = (long long)b * W.nc + c, at = narrow ? bc * W.units + u : bc * P.groups + g;
     char* out = reinterpret_cast<char*>(narrow ? W.yt + at * (Q * TP) : (i & 1 ? W.ct : W.bt) + at * (Q * kN));
 #pragma unroll
@@ -761,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     uint4 x[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] = lds16(base + kOutX + piece(row, half * 4 + j));
-    float2 sc = make_float2(1.f, 1.f);
+    float2 sc = make_float2(kWeightThere, kWeightBack);
     if (kScaled) sc = scale_of(__float_as_uint(top * W.smax[((long long)b * P.heads + h) * W.nc + c]) & 0x7fffffffu);
     for (int cb = half; cb <= quad; cb += 2) {
       uint32_t r[32];
@@ -792,7 +798,7 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
                          lv = *reinterpret_cast<const float2*>(rec + 2 * Q + col);
             const float2 gap = add2(sub2(pair(lh), hv), sub2(pair(ll), lv));
             float2 v = mul2(mul2(make_float2(ex2(gap.x), ex2(gap.y)), sv), words2(r[k * 8 + e], r[k * 8 + e + 1]));
-            if (kScaled) v = mul2(v, pair(sc.x));
+            v = mul2(v, pair(sc.x));
             f.v[e >> 1] = make_float2(col <= row ? v.x : 0.f, col + 1 <= row ? v.y : 0.f);
           }
           sts16(base + kOutM + piece2(row, cb * 4 + k), pack8<X>(f));
@@ -967,7 +973,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       cscale = fmaxf(cscale, hs.x * gs.y);
       bscale = fmaxf(bscale, gs.x * hs.y);
     }
-  if (cscale == 0.f) cscale = 1.f;
+  if (cscale == 0.f) cscale = 1.f;                       // zeros, or products that no number here can hold
   if (bscale == 0.f) bscale = 1.f;
   const float bback = W.bback[tile_at], cback = W.cback[tile_at], both_back = bback * cback;
   if (threadIdx.x == 0) {
@@ -980,7 +986,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   }
   done.wait(ok, P.err);
   tc_fence_after();
-  float2 sc = make_float2(1.f, 1.f);
+  float2 sc = make_float2(kWeightThere, kWeightBack);
   if (kScaled) {                                         // by the largest |B_s . C_t| of my row's pairs
     uint32_t m = 0;
     if (part >= quad) {
@@ -1066,14 +1072,15 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       }
       if (has_h) {
         tmem_ld16(lanes + 192 + part * 16, r);
+        const float f = from_in * hs.x * cback;
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const Eight y = unpack8<X>(lds16(ytile + piece(row, part * 2 + j)));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum = fma2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), y.v[e], sum);
+          for (int e = 0; e < 4; ++e) sum = fma2(mul2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), pair(f)), y.v[e], sum);
         }
-        q_part = (sum.x + sum.y) * (from_in * hs.x * cback * yb);
+        q_part = (sum.x + sum.y) * yb;
       }
       tc_fence_before();
     }
@@ -1103,14 +1110,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       cp_commit();
     }
     float r_sum = 0.f, diag = 0.f, pair_time = 0.f;
-    const float sb = s * both_back * xy, sxy = s * xy;       // of a pair, and of a pair without C . B
+    const float one_back = sc.y * both_back * xy, sb = s * one_back, sxy = s * xy;   // of a pair's weight, and of a pair without C . B
     const int cb = part;
     if (cb >= quad) {
       float2 rs2 = make_float2(0.f, 0.f), time2 = make_float2(0.f, 0.f);
       const bool later = cb > quad;
       // a block of later tokens: the decay to its beginning and from there on are both at most 1
       const float th = later ? rec[Q + cb * 32 - 1] - lh : 0.f, tl = later ? rec[2 * Q + cb * 32 - 1] - ll : 0.f, to_block = ex2(th + tl);
-      const float ds_in = sxy * to_block, pairs_in = sb * to_block, mine = kScaled ? to_block * sc.x : to_block;
+      const float ds_in = sxy * to_block, mine = to_block * sc.x;
 #pragma unroll
       for (int part16 = 0; part16 < 2; ++part16) {       // sixteen columns in registers at a time
         uint32_t r[16], d[16];
@@ -1134,7 +1141,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
                 const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
                 ds[at >> 1] = fma2(mul2(dm, w), pair(ds_in), ds[at >> 1]);
                 f.v[i * 2 + o] = mul2(m, pair(mine));
-                const float2 both = mul2(mul2(m, dm), pair(pairs_in));
+                const float2 both = mul2(mul2(f.v[i * 2 + o], dm), pair(sb));
                 rs2 = add2(rs2, both);
                 time2 = fma2(both, l, time2);
                 e[q] = both.x;
@@ -1159,10 +1166,10 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
               if (t + 1 < row) w.y = 0.f;
               const float2 dm = words2(d[q], d[q + 1]), m = mul2(words2(r[q], r[q + 1]), w);
               ds[at >> 1] = fma2(pair(sxy), mul2(dm, w), ds[at >> 1]);
-              f.v[i] = kScaled ? mul2(m, pair(sc.x)) : m;
-              float2 both = mul2(m, dm);
-              if (t == row) { diag = dm.x; rself[row] = both.x * (both_back * xy); both.x = 0.f; }
-              if (t + 1 == row) { diag = dm.y; rself[row] = both.y * (both_back * xy); both.y = 0.f; }
+              f.v[i] = mul2(m, pair(sc.x));
+              float2 both = mul2(f.v[i], dm);
+              if (t == row) { diag = dm.x; rself[row] = both.x * one_back; both.x = 0.f; }
+              if (t + 1 == row) { diag = dm.y; rself[row] = both.y * one_back; both.y = 0.f; }
               both = mul2(both, pair(sb));               // no decay between a token and itself: kept out of the sums
               rs2 = add2(rs2, both);
               time2 = fma2(both, gap, time2);
