@@ -419,8 +419,8 @@ int sq_distill_loss_grad(const sq_distill_args* args, void* stream);
  * are fp32; y, a 16-bit tensor, is made from pairs' weights and states that are rounded to 16 bits (fp16: scaled) in the
  * products.  What depends on a NaN or an infinity is not finite; the rest of its chunk of 128 tokens, and of later ones (earlier
  * ones, for gradients), is as without it or NaN, and behind B or C that holds for all heads of the group.  A dt of minus
- * infinity passes its token over.  Tensors may be of any size that bf16 has, as long as tokens and states times 2^10 and all results
- * are fp32 numbers; the operands' scales go by their largest values, a number below 2^-28 of which loses bits.
+ * infinity passes its token over.  Tensors may be of any size that bf16 has, tokens up to 2^118, while all results are fp32
+ * numbers; the operands' scales go by their largest values, and a number below 2^-28 of those loses bits.
  * sq_selective_backward: gradients for the gradient dy of y and dstate_out of state_out (NULL: zero), with the forward's
  * inputs: dx, ddt (contiguous), dB, dC in `type`, and where not NULL dA fp32, dD, ddt_bias in their types and
  * dstate_in.  Sums have a fixed order.  workspace: sq_selective_workspace(..., backward) bytes. */

@@ -66,6 +66,13 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def written(*tensors):
+    """Tells autograd that a kernel wrote tensors in place: a gradient that saved one of them raises."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 def conv_args(shape, dtype, x, packed, weight, bias, state, lengths, silu):
     """The arguments that forward and backward share."""
     batch, length, channels = shape
@@ -174,4 +181,5 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu'):
     y = torch.empty(batch, channels, dtype=x.dtype, device=x.device)
     _lib.launch('sq_causal_conv_step', x.device, x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _ptr(bias),
                 y.data_ptr(), batch, channels, weight.shape[1], silu, TYPES[x.dtype], TYPES[weight.dtype])
+    written(state)
     return y

@@ -16,7 +16,7 @@ import torch
 
 from . import _lib
 from .activations import TYPES, PackedActivations, pack_activations
-from .conv import _ptr, checked_keep, checked_lengths, checked_weight, conv_args, inner_packed
+from .conv import _ptr, checked_keep, checked_lengths, checked_weight, conv_args, inner_packed, written
 from .selective import _HALF, N, checked_heads, checked_state
 
 __all__ = ['conv_scan', 'conv_scan_step']
@@ -176,4 +176,5 @@ def conv_scan_step(xbc, dt, A, conv_weight, conv_bias=None, D=None, dt_bias=None
                               _ptr(D), 0 if D is None else TYPES[D.dtype], _ptr(dt_bias), 0 if dt_bias is None else TYPES[dt_bias.dtype],
                               conv_state.data_ptr(), state.data_ptr(), y.data_ptr(), work.data_ptr(), batch * width * 4)
     _lib.launch('sq_conv_scan_step', device, C.byref(a))
+    written(conv_state, state)
     return y

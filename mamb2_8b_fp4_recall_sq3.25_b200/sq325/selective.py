@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from .activations import TYPES
-from .conv import _ptr, checked_lengths, inner_packed
+from .conv import _ptr, checked_lengths, inner_packed, written
 
 __all__ = ['selective_scan', 'selective_step']
 
@@ -180,4 +180,5 @@ def selective_step(x, dt, A, B, C_, state, D=None, dt_bias=None):
                                _ptr(D), 0 if D is None else TYPES[D.dtype], _ptr(dt_bias), 0 if dt_bias is None else TYPES[dt_bias.dtype],
                                state.data_ptr(), y.data_ptr())
     _lib.launch('sq_selective_step', device, C.byref(a))
+    written(state)
     return y
