@@ -264,5 +264,15 @@ def launch(name, device, *args):
     return call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def refuse_tangents(what, *tensors):
+    """There are no forward-mode derivatives here: a tensor's tangent is refused, where a kernel would drop it."""
+    from torch.autograd import forward_ad
+    if forward_ad._current_level < 0:                        # outside every dual_level
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f'{what} has no forward-mode derivative')
+
+
 def ptr(t):
     return C.c_void_p(t.data_ptr()) if t is not None else C.c_void_p(0)

@@ -158,6 +158,7 @@ def causal_conv(x, weight, bias=None, initial_state=None, lengths=None, activati
                 or initial_state.dtype != x.dtype or initial_state.device != x.device:
             raise ValueError(f"initial_state must be [{batch}, {weight.shape[1] - 1}, {channels}] in x's dtype, on its device")
         initial_state = initial_state.contiguous()
+    _lib.refuse_tangents('causal_conv', x, weight, bias, initial_state)
     x = inner_packed(x, 1)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, initial_state)):
         return _CausalConv.apply(x, weight, bias, initial_state, lengths, silu, bool(return_final_state), keep)
@@ -177,6 +178,7 @@ def causal_conv_step(x, state, weight, bias=None, activation='silu'):
     if not isinstance(state, torch.Tensor) or state.shape != (batch, weight.shape[1] - 1, channels) or state.dtype != x.dtype \
             or state.device != x.device or not state.is_contiguous():
         raise ValueError(f"state must be contiguous [{batch}, {weight.shape[1] - 1}, {channels}] in x's dtype, on its device")
+    _lib.refuse_tangents('causal_conv_step', x, weight, bias, state)
     x = inner_packed(x, 1)
     y = torch.empty(batch, channels, dtype=x.dtype, device=x.device)
     _lib.launch('sq_causal_conv_step', x.device, x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), _ptr(bias),

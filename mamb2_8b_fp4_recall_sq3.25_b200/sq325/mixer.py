@@ -146,6 +146,7 @@ def conv_scan(xbc, dt, A, conv_weight, conv_bias=None, D=None, dt_bias=None, *, 
     conv_state = _checked_conv_state(conv_state, batch, weight, xbc)
     state = checked_state(initial_state, (batch, heads, dim, N), device)
     lengths = checked_lengths(lengths, batch, device)
+    _lib.refuse_tangents('conv_scan', xbc, dt, A, weight, bias, D, dt_bias, conv_state, state)
     xbc, dt = inner_packed(xbc, 1), inner_packed(dt, 1)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (xbc, dt, A, weight, bias, D, dt_bias, conv_state, state)):
         return _ConvScan.apply(xbc, dt, A, weight, bias, D, dt_bias, conv_state, state, lengths, heads, groups,
@@ -168,6 +169,7 @@ def conv_scan_step(xbc, dt, A, conv_weight, conv_bias=None, D=None, dt_bias=None
                               ('state', state, checked_state(state, (batch, heads, dim, N), device, 'state'))):
         if given is None or held is not given:
             raise ValueError(f'{name} must be given, and contiguous: it is updated in place')
+    _lib.refuse_tangents('conv_scan_step', xbc, dt, A, weight, bias, D, dt_bias, conv_state, state)
     xbc, dt = inner_packed(xbc, 1), inner_packed(dt, 1)
     y = torch.empty(batch, heads, dim, dtype=xbc.dtype, device=device)
     work = torch.empty(batch, width, dtype=torch.float32, device=device)

@@ -149,6 +149,7 @@ def selective_scan(x, dt, A, B, C_, D=None, dt_bias=None, initial_state=None, le
     A, D, dt_bias = checked_heads(A, D, dt_bias, heads, device)
     state = checked_state(initial_state, (batch, heads, dim, N), device)
     lengths = checked_lengths(lengths, batch, device)
+    _lib.refuse_tangents('selective_scan', x, dt, A, B, C_, D, dt_bias, state)
     x, dt, B, C_ = packed_like_forward(x, dt, B, C_)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, dt, A, B, C_, D, dt_bias, state)):
         return _SelectiveScan.apply(x, dt, A, B, C_, D, dt_bias, state, lengths, bool(return_final_state))
@@ -173,6 +174,7 @@ def selective_step(x, dt, A, B, C_, state, D=None, dt_bias=None):
     A, D, dt_bias = checked_heads(A, D, dt_bias, heads, device)
     if checked_state(state, (batch, heads, dim, N), device, 'state') is not state:
         raise ValueError('state must be contiguous: it is updated in place')
+    _lib.refuse_tangents('selective_step', x, dt, A, B, C_, D, dt_bias, state)
     x, dt, B, C_ = inner_packed(x, 2), inner_packed(dt, 1), inner_packed(B, 2), inner_packed(C_, 2)
     y = torch.empty(batch, heads, dim, dtype=x.dtype, device=device)
     a = _lib.SelectiveStepArgs(batch, heads, dim, groups[1], TYPES[x.dtype], x.data_ptr(), x.stride(0), dt.data_ptr(), dt.stride(0),
