@@ -102,6 +102,7 @@ def distillation_loss(logits, values, indices, temperature=1.0):
     """Per-row distillation loss, fp32 [...], of the student's logits [..., vocab] against the
     teacher's record (values [..., k], int32 indices [..., k], k <= 1024).  Differentiable in the
     logits; the record receives no gradient."""
+    _lib.refuse_tangents('distillation_loss', *(t for t in (logits, values) if isinstance(t, torch.Tensor)))
     if torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad:
         return _DistillationLoss.apply(logits, values, indices, temperature)
     x, values, indices, lead = _checked(logits, values, indices, temperature)
@@ -120,6 +121,7 @@ def distillation_loss_grad(logits, values, indices, temperature=1.0, weight=None
                 or weight.get_device() != x.get_device():
             raise ValueError(f'weight must be a float32 tensor of shape {tuple(lead)} on {x.device}')
         weight = _row_weights(weight)
+    _lib.refuse_tangents('distillation_loss_grad', logits, values, weight)
     loss = row_numbers(x, lead)
     grad = torch.empty(*logits.shape, dtype=x.dtype, device=x.device)
     _lib.launch('sq_distill_loss_grad', x.device,
