@@ -56,9 +56,10 @@ def unpack_activations(packed, dtype=None):
     dtype = was if dtype is None else dtype
     if dtype not in TYPES:
         raise ValueError('dtype must be FP16, BF16 or FP32')
-    if codes.dtype != torch.int8 or scales.dtype != torch.float32 or not codes.is_cuda or scales.device != codes.device \
-            or not codes.shape or scales.shape != (*codes.shape[:-1], -(-codes.shape[-1] // BLOCK)):
-        raise ValueError('Codes must be CUDA int8 [..., width], scales fp32 [..., ceil(width / 128)] on the same device')
+    if not isinstance(codes, torch.Tensor) or not isinstance(scales, torch.Tensor) or codes.dtype != torch.int8 \
+            or scales.dtype != torch.float32 or not codes.is_cuda or scales.device != codes.device or not codes.shape \
+            or codes.shape[-1] < 1 or scales.shape != (*codes.shape[:-1], -(-codes.shape[-1] // BLOCK)):
+        raise ValueError('Codes must be CUDA int8 [..., width] with a positive width, scales fp32 [..., ceil(width / 128)] on the same device')
     codes, scales = codes.contiguous(), scales.contiguous()
     out = torch.empty(codes.shape, dtype=dtype, device=codes.device)
     rows = codes.numel() // codes.shape[-1]
