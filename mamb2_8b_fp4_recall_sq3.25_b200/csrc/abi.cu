@@ -89,7 +89,19 @@ int device_error_word(int** out) {
     } relaxed;
     // [0]: the sticky error word; [1]: per-call flags of sq_fp4_validate
     if (cudaMalloc(&p, 2 * sizeof(int)) != cudaSuccess) return cuda_fail("cudaMalloc (error word)");
-    if (cudaMemset(p, 0, 2 * sizeof(int)) != cudaSuccess) { cudaFree(p); return cuda_fail("cudaMemset (error word)"); }
+    // on a stream of its own: the legacy one would depend on a blocking stream that is captured
+    cudaStream_t own = nullptr;
+    cudaError_t e = cudaStreamCreateWithFlags(&own, cudaStreamNonBlocking);
+    if (e == cudaSuccess) {
+      e = cudaMemsetAsync(p, 0, 2 * sizeof(int), own);
+      if (e == cudaSuccess) e = cudaStreamSynchronize(own);
+      cudaStreamDestroy(own);
+    }
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      cudaFree(p);
+      return fail(SQ_ECUDA, std::string("error word: ") + cudaGetErrorString(e));
+    }
     g_dev_err[dev] = p;
   }
   *out = g_dev_err[dev];
