@@ -499,7 +499,8 @@ int sq_causal_conv_step(const void* x, int64_t x_batch_stride, void* state, cons
  * `type`.  conv's y, and scan's
  * x, B, C, dx, dB and dC are not used; both have the same lengths.  The forward reads conv's x, or the codes where x is
  * NULL, and so does the backward, whose results are conv's dx, dweight, dbias, dstate_in and scan's ddt, dA, dD, ddt_bias,
- * dstate_in.  scan's workspace: sq_conv_scan_workspace(...) bytes. */
+ * dstate_in.  scan's workspace: sq_conv_scan_workspace(...) bytes.  Twice the groups and half of heads times dim / 64 rounded up
+ * are at most 65535 together. */
 int64_t sq_conv_scan_workspace(int batch, int length, int heads, int dim, int groups, int backward);
 int sq_conv_scan_forward(const sq_causal_conv_args* conv, const sq_selective_args* scan, void* stream);
 int sq_conv_scan_backward(const sq_causal_conv_args* conv, const sq_selective_args* scan, void* stream);

@@ -1166,6 +1166,8 @@ int conv_scan_params(const sq_causal_conv_args* c, const sq_selective_args* a, c
   if (!c->silu) return bad("the convolution before a scan ends in silu");
   if (c->lengths != a->lengths) return bad("the convolution's lengths are not the scan's");
   if (c->x) C.codes = nullptr;
+  // tiles of B and C, and pairs of tiles of x: a grid's second dimension
+  if (2 * (int64_t)a->groups + ((int64_t)a->heads * ((a->dim + kScanTile - 1) / kScanTile) + 1) / 2 > kMaxGrid) return bad("heads or groups is too large");
   return selective_params(a, who, backward, P, true, conv_scan_extra(a->batch, a->length, a->heads, a->dim, a->groups, backward));
 }
 }  // namespace
