@@ -875,9 +875,12 @@ int launch_conv_last(const ConvParams& P, cudaStream_t st) {
   const dim3 grid((P.channels + 4 * kThreads - 1) / (4 * kThreads), P.batch);
   return by_type(P.type, P.weight_type, [&](auto t, auto) {
     using T = decltype(t);
-    if (P.codes) conv_last_kernel<T, true><<<grid, kThreads, 0, st>>>(P);
-    else conv_last_kernel<T, false><<<grid, kThreads, 0, st>>>(P);
-    return launch_status();
+    if constexpr (sizeof(T) == 2) {                 // before a scan, which takes no fp32
+      if (P.codes) conv_last_kernel<T, true><<<grid, kThreads, 0, st>>>(P);
+      else conv_last_kernel<T, false><<<grid, kThreads, 0, st>>>(P);
+      return launch_status();
+    }
+    return (int)kEInval;
   });
 }
 
