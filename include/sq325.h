@@ -495,9 +495,8 @@ int sq_causal_conv_step(const void* x, int64_t x_batch_stride, void* state, cons
                         int batch, int channels, int taps, int silu, int type, int weight_type, void* stream);
 
 /* Convolution (silu) and scan as one: conv's output [batch, length, heads*dim + 2*groups*128] is x, B and C side by side, and
- * goes to the scan in scaled fp16 (11 bits of a tile's largest value, whatever `type`), not in `type`; its gradient comes back in
- * `type`.  conv's y, and scan's
- * x, B, C, dx, dB and dC are not used; both have the same lengths.  The forward reads conv's x, or the codes where x is
+ * goes to the scan in scaled fp16 (11 bits, down to 2^-28 of a tile's largest value, whatever `type`), not in `type`; its gradient
+ * comes back in fp32, by the workspace.  conv's y, and scan's x, B, C, dx, dB and dC are not used; both have the same lengths.  The forward reads conv's x, or the codes where x is
  * NULL, and so does the backward, whose results are conv's dx, dweight, dbias, dstate_in and scan's ddt, dA, dD, ddt_bias,
  * dstate_in.  scan's workspace: sq_conv_scan_workspace(...) bytes.  Twice the groups and half of heads times dim / 64 rounded up
  * are at most 65535 together. */

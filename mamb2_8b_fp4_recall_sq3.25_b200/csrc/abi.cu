@@ -1150,11 +1150,11 @@ int sq_causal_conv_step(const void* x, int64_t x_batch_stride, void* state, cons
 
 namespace {
 int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
-// Bytes of a conv_scan's workspace behind the scan's: the gradient of the convolution's output, and its own workspace.
+// Bytes of a conv_scan's workspace behind the scan's: the gradient of the convolution's output in fp32, and its own workspace.
 int64_t conv_scan_extra(int batch, int length, int heads, int dim, int groups, bool backward) {
   if (!backward) return 0;
   const int64_t width = (int64_t)heads * dim + 256ll * groups;
-  return round256((int64_t)batch * length * width * 2) + conv_workspace(batch, length, (int)width);
+  return round256((int64_t)batch * length * width * 4) + conv_workspace(batch, length, (int)width);
 }
 int conv_scan_params(const sq_causal_conv_args* c, const sq_selective_args* a, const char* who, bool backward, ConvParams& C, SelectiveParams& P) {
   if (!a) return fail(SQ_EINVAL, std::string(who) + ": null argument");
@@ -1205,17 +1205,17 @@ int sq_conv_scan_backward(const sq_causal_conv_args* c, const sq_selective_args*
       !aligned(c->dstate_in, 2) || !aligned(c->dweight, w) || !aligned(c->dbias, w))
     return bad("misaligned gradient");
   const int64_t inner = (int64_t)a->heads * a->dim, width = inner + 256ll * a->groups;
-  uint16_t* dz = reinterpret_cast<uint16_t*>(reinterpret_cast<char*>(a->workspace) +
-                                             selective_workspace(a->batch, a->length, a->heads, a->dim, a->groups, true, true));
+  float* dz = reinterpret_cast<float*>(reinterpret_cast<char*>(a->workspace) +
+                                       selective_workspace(a->batch, a->length, a->heads, a->dim, a->groups, true, true));
   P.dy = a->dy; P.dy_sb = a->dy_batch_stride; P.dy_st = a->dy_token_stride; P.dstate_out = a->dstate_out;
   P.dx = dz; P.dB = dz + inner; P.dC = dz + inner + 128ll * a->groups;
   P.dx_sb = P.dg_sb = a->length * width; P.dx_st = P.dg_st = width; P.ddt = a->ddt;
   P.dA = a->dA; P.dD = a->D ? a->dD : nullptr; P.dbias = a->dt_bias ? a->ddt_bias : nullptr; P.dstate_in = a->dstate_in;
   if (int s = check(launch_conv_tiles(C, selective_tiles(P, true), (cudaStream_t)stream), "conv_scan_backward")) return s;
   if (int s = check(launch_selective_backward(P, (cudaStream_t)stream), "conv_scan_backward")) return s;
-  C.dy = dz; C.dy_sb = a->length * width; C.dy_st = width; C.dstate_out = c->dstate_out;
+  C.dy = dz; C.dy_sb = a->length * width; C.dy_st = width; C.dy_f32 = 1; C.dstate_out = c->dstate_out;
   C.dx = c->dx; C.dstate_in = c->dstate_in; C.dweight = c->dweight; C.dbias = c->dbias;
-  C.workspace = reinterpret_cast<float*>(reinterpret_cast<char*>(dz) + round256((int64_t)a->batch * a->length * width * 2));
+  C.workspace = reinterpret_cast<float*>(reinterpret_cast<char*>(dz) + round256((int64_t)a->batch * a->length * width * 4));
   return check(launch_conv_backward(C, (cudaStream_t)stream), "conv_scan_backward");
 }
 

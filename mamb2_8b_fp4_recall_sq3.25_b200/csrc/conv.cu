@@ -393,13 +393,14 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || KEEP ? 5 : 8) conv
 }
 
 // Copies to shared memory that a thread makes for itself: it alone waits for them and reads them.  `take`: else zeros.
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool take) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" :: "r"(dst), "l"(src), "r"(take ? 8 : 0) : "memory");
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" :: "r"(dst), "l"(src), "n"(BYTES), "r"(take ? BYTES : 0) : "memory");
 }
-__device__ __forceinline__ uint2 read_own(uint32_t a) {
-  uint2 v;
+__device__ __forceinline__ void read_own(uint32_t a, uint2& v) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
+}
+__device__ __forceinline__ void read_own(uint32_t a, uint4& v) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
 }
 
 // A strip's gradients: dz_t = dy_t y'(z_t), dx_t = sum_k w_k dz_{t + taps-1 - k}, and the strip's sums of dz_t x_{t - (taps-1) + k}
@@ -410,11 +411,13 @@ __device__ __forceinline__ uint2 read_own(uint32_t a) {
 // copies of four bytes, take 167.  fp32 has three CTAs (188 us; four spill, 215).  Two channels a thread have twice the warps, but in loads of four bytes, and are slower by
 // a third.
 constexpr int kStages = 3, kRingCtas = 5;
-template <typename T, typename WT, bool CODES, bool FAST>
+template <typename T, typename WT, typename DY, bool CODES, bool FAST>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : FAST && !CODES ? kRingCtas : 4) conv_grad_kernel(const ConvParams P, int strip) {
   constexpr int V = kWide, U = 4;
-  constexpr bool VEC = FAST, RING = FAST && !CODES && sizeof(T) == 2;
-  __shared__ __align__(16) uint2 ring[RING ? kStages * U * 2 * kThreads : 1];
+  // what goes through the ring: x of 16 bits, and with it dy; an fp32 dy also beside codes
+  constexpr bool VEC = FAST, RING_X = FAST && !CODES && sizeof(T) == 2, RING = RING_X || (FAST && sizeof(DY) > sizeof(T));
+  constexpr uint32_t kXBytes = RING_X ? kThreads * 8 : 0, kToken = kXBytes + kThreads * V * (uint32_t)sizeof(DY), kRing = RING ? kStages * U * kToken : 16;
+  __shared__ __align__(16) unsigned char ring[kRing];
   using In = Inputs<T, CODES, VEC, V>;
   const int taps = FAST ? kTaps : P.taps;
   const bool silu = FAST || P.silu;
@@ -423,58 +426,62 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : FAST && !CODES 
   if (n <= 0) return;
   const int len = tokens_of(P, b), t0 = blockIdx.x * strip, t1 = min(P.length, t0 + strip), back = taps - 1;
   const In in(P, b, c, n);
-  const T* dy = reinterpret_cast<const T*>(P.dy) + b * P.dy_sb + c;
+  const DY* dy = reinterpret_cast<const DY*>(P.dy) + b * P.dy_sb + c;
   T* dx = reinterpret_cast<T*>(P.dx) + (long long)b * P.length * P.channels + c;
   float2 dw[kTaps][V / 2] = {}, db[V / 2] = {};
   if (t0 < len || t0 == 0) {
     const int stop = t1 + kTaps - 1, end = min(stop, len), own = min(t1, len), lowest = t0 == 0 ? -back : t0;
     float2 x[kTaps - 1][V / 2], dz[kTaps - 1][V / 2] = {};
-    float scale[RING ? 1 : U];
-    typename In::Raw now[RING ? 1 : U];
-    Values<T, V> up[RING ? 1 : U];
-    auto load_up = [&](int t, Values<T, V>(&u)[U]) {
-      const T* p = dy + t * P.dy_st;
+    float scale[RING_X ? 1 : U];
+    typename In::Raw now[RING_X ? 1 : U];
+    Values<DY, V> up[RING ? 1 : U];
+    auto load_up = [&](int t, Values<DY, V>(&u)[U]) {
+      const DY* p = dy + t * P.dy_st;
       if (t + U <= end) {
 #pragma unroll
-        for (int j = 0; j < U; ++j, p += P.dy_st) u[j] = raw_values<T, V>(p, VEC, n);
+        for (int j = 0; j < U; ++j, p += P.dy_st) u[j] = raw_values<DY, V>(p, VEC, n);
       } else {
 #pragma unroll
         for (int j = 0; j < U; ++j, p += P.dy_st) {
-          if (t + j < end) u[j] = raw_values<T, V>(p, VEC, n);
-          else u[j] = no_values<T, V>();
+          if (t + j < end) u[j] = raw_values<DY, V>(p, VEC, n);
+          else u[j] = no_values<DY, V>();
         }
       }
     };
-    // RING: the next stages of U tokens each, x and dy by turns
-    const uint32_t slots = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 8;
+    // RING: the next stages of U tokens each, a token's x before its dy
+    const uint32_t slots = (uint32_t)__cvta_generic_to_shared(ring), x_slot = slots + threadIdx.x * 8,
+                   dy_slot = slots + kXBytes + threadIdx.x * (V * (uint32_t)sizeof(DY));
     uint32_t put_at = 0, get_at = 0;
-    const T *x_next = in.x + t0 * in.step, *dy_next = dy + t0 * P.dy_st;
+    const T* x_next = in.x + t0 * in.step;
+    const DY* dy_next = dy + t0 * P.dy_st;
     auto stage = [&](int t) {
 #pragma unroll
       for (int j = 0; j < U; ++j) {
-        const uint32_t a = slots + put_at + j * (2 * kThreads * 8);
+        const uint32_t at = put_at + j * kToken;
         const bool there = t + j < end;
-        copy_async(a, there ? x_next : in.x, there);
-        copy_async(a + kThreads * 8, there ? dy_next : dy, there);
-        x_next += in.step;
+        if constexpr (RING_X) {
+          copy_async<8>(x_slot + at, there ? x_next : in.x, there);
+          x_next += in.step;
+        }
+        copy_async<V * (int)sizeof(DY)>(dy_slot + at, there ? dy_next : dy, there);
         dy_next += P.dy_st;
       }
-      put_at = (put_at + U * 2 * kThreads * 8) % (kStages * U * 2 * kThreads * 8);
+      put_at = (put_at + U * kToken) % (kStages * U * kToken);
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     if constexpr (RING) {
 #pragma unroll
       for (int k = 0; k < kStages - 1; ++k) stage(t0 + k * U);
     } else {
-      in.template load_batch<U>(t0, end, true, now, scale);
       load_up(t0, up);
     }
+    if constexpr (!RING_X) in.template load_batch<U>(t0, end, true, now, scale);
     const Taps<WT, V> W(P.weight, P.bias, taps, c, n);
 #pragma unroll
     for (int k = 0; k < kTaps - 1; ++k) in.at(P, b, t0 - (kTaps - 1) + k, c, x[k]);
     T* put = dx + (long long)(t0 - (kTaps - 1)) * P.channels;          // of the token whose input's gradient is whole next
     // inner: the token and the one whose gradient becomes whole are both this strip's
-    auto token = [&](const typename In::Raw& raw, float s_in, const Values<T, V>& raw_up, int at, auto inner) {
+    auto token = [&](const typename In::Raw& raw, float s_in, const Values<DY, V>& raw_up, int at, auto inner) {
       constexpr bool INNER = decltype(inner)::value;
       const int to = at - (kTaps - 1);
       const bool mine = INNER || at < own;
@@ -482,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : FAST && !CODES 
       In::get(raw, s_in, f);
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) {
-        float2 d = two<T, V>(raw_up, i);
+        float2 d = two<DY, V>(raw_up, i);
         if (silu) {
           const float2 z = conv_at<WT, V>(W, taps, i, x[0][i], x[1][i], x[2][i], f[i]);
           const float2 s = sigmoid<T>(z);
@@ -529,39 +536,39 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 ? 3 : FAST && !CODES 
 #pragma unroll
       for (int j = 0; j < U; ++j) {
         if constexpr (RING) {
-          const uint32_t a = slots + get_at + j * (2 * kThreads * 8);
-          typename In::Raw raw;
-          Values<T, V> raw_up;
-          raw.q = read_own(a);
-          raw_up.q = read_own(a + kThreads * 8);
-          token(raw, 0.f, raw_up, t + j, inner);
+          const uint32_t at = get_at + j * kToken;
+          Values<DY, V> raw_up;
+          read_own(dy_slot + at, raw_up.q);
+          if constexpr (RING_X) {
+            typename In::Raw raw;
+            read_own(x_slot + at, raw.q);
+            token(raw, 0.f, raw_up, t + j, inner);
+          } else {
+            token(now[j], scale[j], raw_up, t + j, inner);
+          }
         } else {
           token(now[j], scale[j], up[j], t + j, inner);
         }
       }
     };
     for (int t = t0; t < stop; t += U) {
-      typename In::Raw next[RING ? 1 : U];
-      Values<T, V> up_next[RING ? 1 : U];
-      float later[RING ? 1 : U];
-      if constexpr (RING) {
-        stage(t + (kStages - 1) * U);                                  // its place was read a turn ago
-        asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
-      } else {
-        in.template load_batch<U>(t + U, end, true, next, later);
-        load_up(t + U, up_next);
-      }
+      typename In::Raw next[RING_X ? 1 : U];
+      Values<DY, V> up_next[RING ? 1 : U];
+      float later[RING_X ? 1 : U];
+      if constexpr (RING) stage(t + (kStages - 1) * U);                // its place was read a turn ago
+      if constexpr (!RING_X) in.template load_batch<U>(t + U, end, true, next, later);
+      if constexpr (RING) asm volatile("cp.async.wait_group %0;" :: "n"(kStages - 1) : "memory");
+      else load_up(t + U, up_next);
       if (t >= t0 + U && t + U <= calm) tokens(t, std::true_type{});
       else tokens(t, std::false_type{});
-      if constexpr (RING) {
-        get_at = (get_at + U * 2 * kThreads * 8) % (kStages * U * 2 * kThreads * 8);
-      } else {
+      if constexpr (RING) get_at = (get_at + U * kToken) % (kStages * U * kToken);
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
+      for (int j = 0; j < U; ++j) {
+        if constexpr (!RING_X) {
           now[j] = next[j];
           scale[j] = later[j];
-          up[j] = up_next[j];
         }
+        if constexpr (!RING) up[j] = up_next[j];
       }
     }
     if constexpr (RING) asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -907,12 +914,17 @@ int launch_conv_backward(const ConvParams& P, cudaStream_t st) {
   const int strip = strip_of(P.batch, P.length, P.channels, kLeast, kMost), per = kThreads * kWide;
   const dim3 grid((P.length + strip - 1) / strip, (P.channels + per - 1) / per, P.batch);
   const bool fast = P.taps == kTaps && P.silu && (!P.x || whole(P.x, P.type, kWide, P.x_sb, P.x_st)) &&
-                   whole(P.dy, P.type, kWide, P.dy_sb, P.dy_st) && whole(P.dx, P.type, kWide, P.channels) && whole(P.workspace, 2, kWide, 0) && ((uintptr_t)P.codes & (kWide - 1)) == 0;
+                   whole(P.dy, P.dy_f32 ? 2 : P.type, kWide, P.dy_sb, P.dy_st) && whole(P.dx, P.type, kWide, P.channels) && whole(P.workspace, 2, kWide, 0) && ((uintptr_t)P.codes & (kWide - 1)) == 0;
   return by_type(P.type, P.weight_type, [&](auto t, auto w) {
     using T = decltype(t);
     using WT = decltype(w);
-    if (P.codes) fast ? conv_grad_kernel<T, WT, true, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, true, false><<<grid, kThreads, 0, st>>>(P, strip);
-    else fast ? conv_grad_kernel<T, WT, false, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, false, false><<<grid, kThreads, 0, st>>>(P, strip);
+    const auto launch = [&](auto d) {
+      using DY = decltype(d);
+      if (P.codes) fast ? conv_grad_kernel<T, WT, DY, true, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, DY, true, false><<<grid, kThreads, 0, st>>>(P, strip);
+      else fast ? conv_grad_kernel<T, WT, DY, false, true><<<grid, kThreads, 0, st>>>(P, strip) : conv_grad_kernel<T, WT, DY, false, false><<<grid, kThreads, 0, st>>>(P, strip);
+    };
+    if (P.dy_f32) launch(float{});
+    else launch(T{});
     if (int s = launch_status()) return s;
     if (P.dweight || P.dbias) {
       conv_weights_kernel<WT><<<dim3((P.channels + 31) / 32, kTaps + 1), 256, 0, st>>>(P, (int)grid.x * P.batch);

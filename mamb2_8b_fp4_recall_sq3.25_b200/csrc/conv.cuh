@@ -17,7 +17,8 @@ struct ConvParams {
   void* y; long long y_sb, y_st;
   void* state_out;                                  // [B,taps-1,C], may be null
   // backward
-  const void* dy; long long dy_sb, dy_st;
+  const void* dy; long long dy_sb, dy_st;           // in `type`, or fp32 where dy_f32 (a 16-bit type's)
+  int dy_f32;
   const void* dstate_out;                           // [B,taps-1,C], may be null
   void* dx;                                         // contiguous
   void* dstate_in;                                  // may be null

@@ -306,6 +306,26 @@ __device__ __forceinline__ void store_tile(T* dst, long long stride, uint32_t sr
     }
   }
 }
+// The same of a tile [128][64] of fp32: rows of 256 bytes, 16-byte piece j of row r at r * 256 + ((j ^ (r & 7)) << 4).
+__device__ __forceinline__ uint32_t piece_f32(int row, int j) { return (uint32_t)(row * 256 + ((j ^ (row & 7)) << 4)); }
+template <int THREADS>
+__device__ __forceinline__ void store_tile(float* dst, long long stride, uint32_t src, int rows, int cols, bool) {
+  const bool vec = ((uintptr_t)dst & 15) == 0 && ((stride | cols) & 3) == 0;
+  for (int i = threadIdx.x; i < Q * 16; i += THREADS) {
+    const int r = i >> 4, j = i & 15;
+    if (r >= rows || j * 4 >= cols) continue;
+    const uint4 v = lds16(src + piece_f32(r, j));
+    float* p = dst + (long long)r * stride + j * 4;
+    if (vec) {
+      *reinterpret_cast<uint4*>(p) = v;
+    } else {
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j * 4 + e < cols) p[e] = __uint_as_float(u[e]);
+    }
+  }
+}
 __device__ __forceinline__ bool vector_ok(const void* p, long long s0, long long s1, int cols) {
   return ((uintptr_t)p & 15) == 0 && ((s0 | s1 | cols) & 7) == 0;
 }
@@ -880,6 +900,7 @@ __device__ __forceinline__ float column_sums(float (&e)[16], int lane) {
 template <typename T, bool TILED>
 __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectiveParams P, const Space W, int per) {
   using X = typename std::conditional<TILED, __half, T>::type;
+  using G = typename std::conditional<TILED, float, T>::type;    // of dx, dB and dC
   constexpr bool kScaled = std::is_same<X, __half>::value;
   extern __shared__ __align__(1024) unsigned char smem[];
   const uint32_t base = smem_u32(smem);
@@ -895,14 +916,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
   const int row = threadIdx.x & 127, part = threadIdx.x >> 7, warp = threadIdx.x >> 5, quad = warp & 3, lane = threadIdx.x & 31;
   const long long bc = (long long)b * W.nc + c, tile_at = bc * P.groups + g;
   // Pointers are made where they are used: registers are what this kernel is short of.
-  auto dx_at = [&](int h, int p0) { return reinterpret_cast<T*>(P.dx) + b * P.dx_sb + (long long)c * Q * P.dx_st + (long long)h * P.dim + p0; };
-  auto group_at = [&](void* p) { return reinterpret_cast<T*>(p) + b * P.dg_sb + (long long)c * Q * P.dg_st + g * kN; };
+  auto dx_at = [&](int h, int p0) { return reinterpret_cast<G*>(P.dx) + b * P.dx_sb + (long long)c * Q * P.dx_st + (long long)h * P.dim + p0; };
+  auto group_at = [&](void* p) { return reinterpret_cast<G*>(p) + b * P.dg_sb + (long long)c * Q * P.dg_st + g * kN; };
   launch_dependents();
   if (rows <= 0) {                                       // behind the sequence's end
     for (int u = u0; u < u1; ++u) {
       const int h = u / W.ptiles, p0 = (u % W.ptiles) * TP, cols = min(TP, P.dim - p0);
       for (int i = threadIdx.x; i < out_rows * cols; i += kGradThreads)
-        dx_at(h, p0)[(long long)(i / cols) * P.dx_st + i % cols] = from_f32<T>(0.f);
+        dx_at(h, p0)[(long long)(i / cols) * P.dx_st + i % cols] = from_f32<G>(0.f);
       if (threadIdx.x == 0) W.unit_sums[bc * W.units + u] = make_float2(0.f, 0.f);
       if (W.ptiles == 1) {
         if (threadIdx.x < 4) W.bias_sums[(bc * P.heads + h) * 4 + threadIdx.x] = 0.f;
@@ -912,7 +933,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
     }
     if (W.splits == 1)
       for (int i = threadIdx.x; i < out_rows * kN; i += kGradThreads)
-        group_at(P.dB)[(long long)(i / kN) * P.dg_st + i % kN] = group_at(P.dC)[(long long)(i / kN) * P.dg_st + i % kN] = from_f32<T>(0.f);
+        group_at(P.dB)[(long long)(i / kN) * P.dg_st + i % kN] = group_at(P.dC)[(long long)(i / kN) * P.dg_st + i % kN] = from_f32<G>(0.f);
     wait_for_launch();
     return;
   }
@@ -1257,12 +1278,21 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           f.v[e] = fma2(fma2(words2(r[j * 8 + 2 * e], r[j * 8 + 2 * e + 1]), pair(mixed), dxi[j * 4 + e]), pair(s), f.v[e]);
-        sts16(base + kGM + at, row < rows ? pack8<T>(f) : make_uint4(0, 0, 0, 0));
+        if (row >= rows) f = {};
+        if constexpr (TILED) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sts16(base + kGM + piece_f32(row, part * 4 + j * 2 + e), make_uint4(__float_as_uint(f.v[2 * e].x), __float_as_uint(f.v[2 * e].y),
+                                                                                __float_as_uint(f.v[2 * e + 1].x), __float_as_uint(f.v[2 * e + 1].y)));
+        } else {
+          sts16(base + kGM + at, pack8<T>(f));
+        }
       }
     }
     __syncthreads();
-    T* out = dx_at(h, p0);
-    store_tile<T, kGradThreads>(out, P.dx_st, base + kGM, out_rows, cols, vector_ok(out, P.dx_st, 0, cols));
+    G* out = dx_at(h, p0);
+    if constexpr (TILED) store_tile<kGradThreads>(out, P.dx_st, base + kGM, out_rows, cols, true);
+    else store_tile<T, kGradThreads>(out, P.dx_st, base + kGM, out_rows, cols, vector_ok(out, P.dx_st, 0, cols));
   }
   __syncthreads();
 
@@ -1311,7 +1341,19 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
           if (has) f.v[e] = fma2(words2(d[j * 8 + 2 * e], d[j * 8 + 2 * e + 1]), pair(back), f.v[e]);
           if (row >= rows) f.v[e] = make_float2(0.f, 0.f);
         }
-        if (W.splits > 1) {
+        if (TILED && W.splits == 1) {
+          // whole lines a thread, once a CTA: through shared memory they would need twice its room
+          if (row < out_rows) {
+            float* p = reinterpret_cast<float*>(group_at(which ? P.dC : P.dB)) + (long long)row * P.dg_st + part * 32 + j * 8;
+            if (((uintptr_t)p & 15) == 0) {
+              *reinterpret_cast<float4*>(p) = make_float4(f.v[0].x, f.v[0].y, f.v[1].x, f.v[1].y);
+              *reinterpret_cast<float4*>(p + 4) = make_float4(f.v[2].x, f.v[2].y, f.v[3].x, f.v[3].y);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) { p[2 * e] = f.v[e].x; p[2 * e + 1] = f.v[e].y; }
+            }
+          }
+        } else if (W.splits > 1) {
           float* p = sums + ((((long long)split * P.batch + b) * W.lp + (long long)c * Q + row) * P.groups + g) * kN + part * 32 + j * 8;
           *reinterpret_cast<float4*>(p) = make_float4(f.v[0].x, f.v[0].y, f.v[1].x, f.v[1].y);
           *reinterpret_cast<float4*>(p + 4) = make_float4(f.v[2].x, f.v[2].y, f.v[3].x, f.v[3].y);
@@ -1321,12 +1363,14 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       }
     }
   }
-  if (W.splits == 1) {
-    __syncthreads();
-    for (int hf = 0; hf < 2; ++hf) {
-      T *dB = group_at(P.dB) + hf * 64, *dC = group_at(P.dC) + hf * 64;
-      store_tile<T, kGradThreads>(dB, P.dg_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB, P.dg_st, 0, 64));
-      store_tile<T, kGradThreads>(dC, P.dg_st, base + kGHigh + hf * kTile64, out_rows, 64, vector_ok(dC, P.dg_st, 0, 64));
+  if constexpr (!TILED) {
+    if (W.splits == 1) {
+      __syncthreads();
+      for (int hf = 0; hf < 2; ++hf) {
+        T *dB = group_at(P.dB) + hf * 64, *dC = group_at(P.dC) + hf * 64;
+        store_tile<T, kGradThreads>(dB, P.dg_st, base + kGM + hf * kTile64, out_rows, 64, vector_ok(dB, P.dg_st, 0, 64));
+        store_tile<T, kGradThreads>(dC, P.dg_st, base + kGHigh + hf * kTile64, out_rows, 64, vector_ok(dC, P.dg_st, 0, 64));
+      }
     }
   }
   tensor_end<512>(tmem);
@@ -1376,7 +1420,7 @@ __global__ void __launch_bounds__(kThreads) finish_dt_kernel(const SelectivePara
 
 // The first `head_blocks` CTAs: gradients of A, the bias and D, a warp a head.  The others, where CTAs shared a group's
 // units: dB and dC from the splits' sums, four columns a thread.  4 us.
-template <typename T>
+template <typename G>
 __global__ void __launch_bounds__(kThreads) finish_kernel(const SelectiveParams P, const Space W, int head_blocks) {
   launch_dependents();
   wait_for_launch();
@@ -1418,13 +1462,21 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const SelectiveParams 
         const float4 a = *reinterpret_cast<const float4*>(p + s * step + at);
         v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
       }
-    T* out = reinterpret_cast<T*>(which ? P.dC : P.dB) + b * P.dg_sb + t * P.dg_st + i * 4 % width;
-    const uint32_t lo = pack2<T>(v.x, v.y), hi = pack2<T>(v.z, v.w);
-    if (((uintptr_t)out & 7) == 0) {
-      *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
+    G* out = reinterpret_cast<G*>(which ? P.dC : P.dB) + b * P.dg_sb + t * P.dg_st + i * 4 % width;
+    if constexpr (std::is_same<G, float>::value) {
+      if (((uintptr_t)out & 15) == 0) {
+        *reinterpret_cast<float4*>(out) = v;
+      } else {
+        out[0] = v.x; out[1] = v.y; out[2] = v.z; out[3] = v.w;
+      }
     } else {
-      uint16_t* o = reinterpret_cast<uint16_t*>(out);
-      o[0] = (uint16_t)lo; o[1] = (uint16_t)(lo >> 16); o[2] = (uint16_t)hi; o[3] = (uint16_t)(hi >> 16);
+      const uint32_t lo = pack2<G>(v.x, v.y), hi = pack2<G>(v.z, v.w);
+      if (((uintptr_t)out & 7) == 0) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
+      } else {
+        uint16_t* o = reinterpret_cast<uint16_t*>(out);
+        o[0] = (uint16_t)lo; o[1] = (uint16_t)(lo >> 16); o[2] = (uint16_t)hi; o[3] = (uint16_t)(hi >> 16);
+      }
     }
   }
 }
@@ -1561,7 +1613,7 @@ template <typename T, bool TILED> int backward(const SelectiveParams& P, cudaStr
   const int head_blocks = P.dA || P.dD || P.dbias ? (P.heads + kThreads / 32 - 1) / (kThreads / 32) : 0;
   const long long all = W.splits > 1 ? (long long)P.batch * P.length * P.groups * (kN / 4) : 0;
   const long long blocks = head_blocks + (all + kThreads - 1) / kThreads;
-  return blocks ? behind(finish_kernel<T>, dim3((unsigned)blocks), kThreads, 0, st, P, W, head_blocks) : (int)kOk;
+  return blocks ? behind(finish_kernel<typename std::conditional<TILED, float, T>::type>, dim3((unsigned)blocks), kThreads, 0, st, P, W, head_blocks) : (int)kOk;
 }
 
 }  // namespace

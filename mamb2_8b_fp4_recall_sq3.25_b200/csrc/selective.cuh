@@ -27,7 +27,7 @@ struct SelectiveParams {
   // backward
   const void* dy; long long dy_sb, dy_st;
   const float* dstate_out;                                  // may be null
-  void* dx; long long dx_sb, dx_st;                         // gradients in `type`, of x, dt (contiguous), B and C
+  void* dx; long long dx_sb, dx_st;                         // gradients in `type`, of x, dt (contiguous), B and C; tiled: of x, B and C in fp32
   void* ddt;
   void *dB, *dC; long long dg_sb, dg_st;
   float* dA; void* dD; void* dbias;                         // each may be null

@@ -4,8 +4,8 @@
 Taken one after the other they keep for the backward pass the convolution's input and its output.  `conv_scan` keeps the
 input alone and computes the output again; with keep='int8' it keeps the input in 8 bits, 1.03 bytes a channel and token
 in place of four.  The output is then that of the given input, and the gradients are those at the kept values.  Between
-the two the convolution's output is scaled fp16 (11 bits of a tile's largest value, also where the input is bf16), in
-`conv_scan_step` fp32.
+the two the convolution's output is scaled fp16 (11 bits, down to 2^-28 of a tile's largest value, also where the input is
+bf16), its gradient fp32; in `conv_scan_step` the output is fp32.
 """
 from __future__ import annotations
 
