@@ -306,7 +306,7 @@ __device__ __forceinline__ float2 conv_at(const Taps<WT, V>& W, const int taps, 
 // KEEP: the input is kept in 8 bits besides.  FAST: four taps, silu and whole aligned pieces, as mixers have them; without
 // them a third of the instructions would be the questions.  Bound by the latency of loads: the next four tokens' are under
 // way while four are worked on, 32 KB an SM.  4 x 2,048 tokens of 10,240 channels in bf16: 68 us, 4.9 TB/s of input and
-// output (fp32 120 us, 5.6 TB/s); keeping the input in 8 bits besides 114 us, 3.7 TB/s, for the rows' maxima.
+// output (fp32 120 us, 5.6 TB/s); keeping the input in 8 bits besides 105 us, 4.0 TB/s, for the rows' maxima.
 template <typename T, typename WT, bool KEEP, bool FAST>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || KEEP ? 5 : 8) conv_kernel(const ConvParams P, int strip) {
   constexpr int V = kWide, U = 4;                                      // U: tokens whose loads are in flight together
@@ -406,9 +406,9 @@ __device__ __forceinline__ void read_own(uint32_t a, uint4& v) {
 // A strip's gradients: dz_t = dy_t y'(z_t), dx_t = sum_k w_k dz_{t + taps-1 - k}, and the strip's sums of dz_t x_{t - (taps-1) + k}
 // and dz_t.  The walk goes three tokens past the strip, whose dz its last inputs need.  Bound by registers (sums, taps and what
 // is under way) and with them by the loads in flight.  RING: those of 16-bit tensors go to shared memory, twelve tokens of
-// a thread, which leaves 96 registers and five CTAs an SM; 4 x 2,048 tokens of 10,240 channels in bf16 take 105 us, 4.8 TB/s.
-// In registers (odd forms, codes) eight tokens and four CTAs: 119 us, 117 from codes; codes in the ring, by
-// copies of four bytes, take 167.  fp32 has three CTAs (188 us; four spill, 215).  Two channels a thread have twice the warps, but in loads of four bytes, and are slower by
+// a thread, which leaves 96 registers and five CTAs an SM; 4 x 2,048 tokens of 10,240 channels in bf16 take 105 us, 4.8 TB/s, and
+// conv_weights_kernel 6 us more.  In registers (odd forms, codes) eight tokens and four CTAs: 119 us, from codes too; codes in the ring, by
+// copies of four bytes, take 167.  An fp32 dy, a scan's, goes through the ring also beside codes: 2 x 2,048 tokens 69 us, with a bf16 dy 64.  fp32 has three CTAs (188 us; four spill, 215).  Two channels a thread have twice the warps, but in loads of four bytes, and are slower by
 // a third.
 constexpr int kStages = 3, kRingCtas = 5;
 template <typename T, typename WT, typename DY, bool CODES, bool FAST>

@@ -3,7 +3,8 @@
 
 Taken one after the other they keep for the backward pass the convolution's input and its output.  `conv_scan` keeps the
 input alone and computes the output again; with keep='int8' it keeps the input in 8 bits, 1.03 bytes a channel and token
-in place of four.  The output is then that of the given input, and the gradients are those at the kept values.  Between
+in place of four.  The output is then that of the given input, and the gradients are those at the kept values.  A call's
+workspace, which it gives back, is larger than what is kept (2 x 2,048 tokens at 128 heads: 233 MB forward, 619 MB backward).  Between
 the two the convolution's output is scaled fp16 (11 bits, down to 2^-28 of a tile's largest value, also where the input is
 bf16), its gradient fp32; in `conv_scan_step` the output is fp32.
 """
