@@ -359,7 +359,13 @@ __device__ __forceinline__ uint32_t tensor_begin(uint64_t* bars, int count, uint
   tc_fence_after();
   return *slot;
 }
-template <int COLS> __device__ __forceinline__ void tensor_end(uint32_t tmem) {
+// A CTA whose wait expired (`ok` false) gives what it has in flight, bulk copies and products, two milliseconds before its shared
+// memory and TMEM are another's: a thousand times what they take.
+template <int COLS> __device__ __forceinline__ void tensor_end(uint32_t tmem, bool ok) {
+  if (!ok) {
+    const uint64_t since = gtime();
+    for (int i = 0; i < 4000 && gtime() - since < 2000000; ++i) __nanosleep(1000);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -665,7 +671,7 @@ __device__ __forceinline__ void state_pass(const SelectiveParams& P, const Space
       if (p < cols) last[state_at + (long long)p * kN] = S[i].x;
       if (p + 1 < cols) last[state_at + (long long)(p + 1) * kN] = S[i].y;
     }
-  tensor_end<128>(tmem);
+  tensor_end<128>(tmem, ok);
 }
 template <typename T, bool TILED>
 __global__ void __launch_bounds__(kThreads, 2) state_pass_kernel(const SelectiveParams P, const Space W) {
@@ -859,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 2) out_kernel(const SelectiveParams 
     T* out = y + (long long)h * P.dim + p0;
     store_tile<T>(out, P.y_st, base + kOutM, out_rows, cols, vector_ok(out, P.y_st, 0, cols));
   }
-  tensor_end<256>(tmem);
+  tensor_end<256>(tmem, ok);
 }
 
 // ---------------------------------------------------------------- gradients by chunk and group
@@ -1373,7 +1379,7 @@ __global__ void __launch_bounds__(kGradThreads, 1) grad_kernel(const SelectivePa
       }
     }
   }
-  tensor_end<512>(tmem);
+  tensor_end<512>(tmem, ok);
 }
 
 // ---------------------------------------------------------------- sums behind the gradients
